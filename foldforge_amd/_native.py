@@ -74,6 +74,28 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int32,
         [c_void_p] * 7 + [c_size_t, c_int64, c_int32, c_int32, c_void_p],
     ),
+    "ffk_quantize_activation": (
+        c_int32,
+        [c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_void_p],
+    ),
+    "ffk_restore_activation": (
+        c_int32,
+        [c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_void_p],
+    ),
+    "ffk_layer_norm_checkpoint": (
+        c_int32,
+        [c_void_p] * 6 + [c_int64, c_int32, c_float, c_int32, c_void_p],
+    ),
+    "ffk_layer_norm_backward_workspace": (c_size_t, [c_int64, c_int32]),
+    "ffk_layer_norm_backward": (
+        c_int32,
+        [c_void_p] * 8 + [c_size_t, c_int64, c_int32, c_float, c_int32, c_int32, c_void_p],
+    ),
+    "ffk_transition_backward_workspace": (c_size_t, [c_int64, c_int32, c_int32]),
+    "ffk_transition_backward": (
+        c_int32,
+        [c_void_p] * 15 + [c_size_t, c_int64, c_int32, c_int32, c_int32, c_float, c_int32, c_void_p],
+    ),
     "ffk_msa_pair_weighted_averaging_workspace": (
         c_size_t,
         [c_int64, c_int64, c_int64, c_int32, c_int32, c_int32, c_int32],

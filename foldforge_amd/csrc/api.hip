@@ -275,6 +275,22 @@ TransitionWs transition_ws(void* ws, int64_t rows, int d, int factor) {
   return w;
 }
 
+TransitionGradArgs transition_grad_ws(void* ws, size_t* bytes, const TransitionGradPlan& p, int d, int hidden) {
+  Carver cv{static_cast<char*>(ws)};
+  TransitionGradArgs a{};
+  const size_t w = (size_t)hidden * d;
+  a.ab = cv.take<bf16>(2 * w);
+  a.st = cv.take<bf16>(w);
+  a.abt = cv.take<bf16>(2 * w);
+  a.n = cv.take<bf16>((size_t)p.chunk * d);
+  a.E = cv.take<bf16>((size_t)p.chunk * 3 * hidden);
+  a.dn = cv.take<float>((size_t)p.dn_splits * p.chunk * d);
+  a.norm_part = cv.take<float>((size_t)p.norm_blocks * 2 * d);
+  a.dw_part = cv.take<float>((size_t)p.dw_splits * 3 * w);
+  *bytes = cv.used;
+  return a;
+}
+
 int64_t pad32(int64_t n) { return (n + 31) / 32 * 32; }
 
 int64_t pad64(int64_t n) { return (n + 63) / 64 * 64; }
@@ -351,6 +367,20 @@ ApbWs apb_ws(void* ws, int64_t batch, int64_t n, int cs, int heads) {
 }
 
 // Argument checks shared by the transition entry points (not the workspace).
+// Widths of the transition's backward pass.
+bool transition_grad_shape(int d, int factor) {
+  return d > 0 && d % 64 == 0 && d <= kLnGemmMaxK && factor > 0 && factor <= 64;
+}
+
+int32_t activation_check(const char* what, const void* x, const void* codes, const void* scales, int64_t rows,
+                         int cols, int dtype) {
+  if (rows < 0 || cols <= 0) return fail(FFK_ERR_INVALID, "%s: bad shape rows=%lld cols=%d", what, (long long)rows, cols);
+  if (dtype != FFK_DTYPE_BF16 && dtype != FFK_DTYPE_F32)
+    return fail(FFK_ERR_INVALID, "%s: dtype %d is neither bf16 nor fp32", what, dtype);
+  if (rows > 0 && (!x || !codes || !scales)) return fail(FFK_ERR_INVALID, "%s: null tensor", what);
+  return FFK_OK;
+}
+
 int32_t transition_check(const void* x, const float* ln_w, const float* ln_b, const float* wa,
                          const float* wb, const float* wsq, const void* out, int64_t rows, int d,
                          int factor) {
@@ -494,6 +524,78 @@ int32_t ffk_layer_norm(const void* x, const float* weight, const float* bias, vo
   if (rows == 0) return ok();
   launch_layer_norm(x, weight, bias, y, rows, cols, eps, dtype, static_cast<hipStream_t>(stream));
   return check_launch("layer_norm");
+}
+
+int32_t ffk_quantize_activation(const void* x, void* codes, void* scales, int64_t rows, int32_t cols,
+                                int32_t dtype, void* stream) {
+  if (int32_t s = check_device()) return s;
+  if (int32_t s = activation_check("quantize_activation", x, codes, scales, rows, cols, dtype)) return s;
+  if (rows == 0) return ok();
+  launch_quantize(x, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), rows, cols, dtype,
+                  static_cast<hipStream_t>(stream));
+  return check_launch("quantize_activation");
+}
+
+int32_t ffk_restore_activation(const void* codes, const void* scales, void* x, int64_t rows, int32_t cols,
+                               int32_t dtype, void* stream) {
+  if (int32_t s = check_device()) return s;
+  if (int32_t s = activation_check("restore_activation", x, codes, scales, rows, cols, dtype)) return s;
+  if (rows == 0) return ok();
+  launch_restore(static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), x, rows, cols, dtype,
+                 static_cast<hipStream_t>(stream));
+  return check_launch("restore_activation");
+}
+
+int32_t ffk_layer_norm_checkpoint(const void* x, const float* weight, const float* bias, void* y, void* codes,
+                                  void* scales, int64_t rows, int32_t cols, float eps, int32_t dtype, void* stream) {
+  if (int32_t s = check_device()) return s;
+  if (int32_t s = activation_check("layer_norm_checkpoint", x, codes, scales, rows, cols, dtype)) return s;
+  if (rows == 0) return ok();
+  if (!y || y == x) return fail(FFK_ERR_INVALID, "layer_norm_checkpoint: y must be a tensor of its own");
+  launch_layer_norm_keep(x, weight, bias, y, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), rows, cols,
+                         eps, dtype, static_cast<hipStream_t>(stream));
+  return check_launch("layer_norm_checkpoint");
+}
+
+size_t ffk_layer_norm_backward_workspace(int64_t rows, int32_t cols) {
+  if (rows < 0 || cols <= 0) return 0;
+  return up256(layer_norm_grad_floats(rows, cols) * sizeof(float));
+}
+
+int32_t ffk_layer_norm_backward(const void* dy, const void* x, const void* scales, const float* weight, void* dx,
+                                void* dweight, void* dbias, void* workspace, size_t workspace_bytes, int64_t rows,
+                                int32_t cols, float eps, int32_t dtype, int32_t grad_dtype, void* stream) {
+  if (int32_t s = check_device()) return s;
+  if (rows < 0 || cols <= 0)
+    return fail(FFK_ERR_INVALID, "layer_norm_backward: bad shape rows=%lld cols=%d", (long long)rows, cols);
+  if (rows > 0 && (!dy || !x || !dx)) return fail(FFK_ERR_INVALID, "layer_norm_backward: null tensor");
+  if (dtype != FFK_DTYPE_BF16 && dtype != FFK_DTYPE_F32)
+    return fail(FFK_ERR_INVALID, "layer_norm_backward: dtype %d is neither bf16 nor fp32", dtype);
+  if (grad_dtype != FFK_DTYPE_BF16 && grad_dtype != FFK_DTYPE_F32)
+    return fail(FFK_ERR_INVALID, "layer_norm_backward: gradient dtype %d is neither bf16 nor fp32", grad_dtype);
+  const size_t need = ffk_layer_norm_backward_workspace(rows, cols);
+  if (!workspace || workspace_bytes < need || !aligned16(workspace))
+    return fail(FFK_ERR_WORKSPACE, "layer_norm_backward: workspace %zu bytes < %zu", workspace_bytes, need);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  LayerNormGradArgs a{};
+  a.x = x;
+  a.scales = static_cast<const uint8_t*>(scales);
+  a.dy = dy;
+  a.w = weight;
+  a.dx = dx;
+  a.dw = dweight;
+  a.db = dbias;
+  a.part = static_cast<float*>(workspace);
+  a.rows = rows;
+  a.cols = cols;
+  a.dtype = dtype;
+  a.grad_dtype = grad_dtype;
+  a.eps = eps;
+  if (rows > 0)
+    launch_layer_norm_grad(a, st);
+  else if (dweight || dbias)  // sums over no rows
+    launch_sum_partials(a.part, 0, 2 * cols, cols, dweight, dbias, grad_dtype, st);
+  return check_launch("layer_norm_backward");
 }
 
 size_t ffk_triangle_multiplication_workspace(int64_t batch, int64_t n, int32_t d_pair,
@@ -1019,6 +1121,62 @@ int32_t ffk_transition_noalloc(const void* x, const float* ln_w, const float* ln
   if (int32_t s = noalloc_scratch(&base)) return s;
   return transition_run(transition_ws(base, rows, d, factor), x, ln_w, ln_b, w_expand_a, w_expand_b,
                         w_squeeze, out, rows, d, factor, residual, eps, static_cast<hipStream_t>(stream));
+}
+
+size_t ffk_transition_backward_workspace(int64_t rows, int32_t d, int32_t factor) {
+  if (rows < 0 || !transition_grad_shape(d, factor)) return 0;
+  size_t bytes = 0;
+  transition_grad_ws(nullptr, &bytes, transition_grad_plan(rows, d, factor * d), d, factor * d);
+  return bytes;
+}
+
+int32_t ffk_transition_backward(const void* dy, const void* x, const void* scales, const float* ln_w,
+                                const float* ln_b, const float* w_expand_a, const float* w_expand_b,
+                                const float* w_squeeze, void* dx, void* dln_w, void* dln_b, void* dw_expand_a,
+                                void* dw_expand_b, void* dw_squeeze, void* workspace, size_t workspace_bytes,
+                                int64_t rows, int32_t d, int32_t factor, int32_t residual, float eps,
+                                int32_t grad_dtype, void* stream) {
+  if (int32_t s = check_device()) return s;
+  if (!transition_grad_shape(d, factor))
+    return fail(FFK_ERR_INVALID, "transition_backward: d=%d factor=%d (d a multiple of 64 up to %d, factor up to 64)", d,
+                factor, kLnGemmMaxK);
+  if (rows < 0 || rows > (int64_t)1 << 40) return fail(FFK_ERR_INVALID, "transition_backward: rows=%lld", (long long)rows);
+  if (rows > 0 && (!dy || !x || !dx)) return fail(FFK_ERR_INVALID, "transition_backward: null tensor");
+  if (!ln_w || !ln_b || !w_expand_a || !w_expand_b || !w_squeeze || !dln_w || !dln_b || !dw_expand_a ||
+      !dw_expand_b || !dw_squeeze)
+    return fail(FFK_ERR_INVALID, "transition_backward: null parameter or gradient");
+  if (grad_dtype != FFK_DTYPE_BF16 && grad_dtype != FFK_DTYPE_F32)
+    return fail(FFK_ERR_INVALID, "transition_backward: gradient dtype %d is neither bf16 nor fp32", grad_dtype);
+  if (!aligned16(dy) || !aligned16(x) || !aligned16(dx))
+    return fail(FFK_ERR_INVALID, "transition_backward: dy, x and dx must be 16-byte aligned");
+  const int hidden = factor * d;
+  const TransitionGradPlan plan = transition_grad_plan(rows, d, hidden);
+  size_t need = 0;
+  TransitionGradArgs a = transition_grad_ws(workspace, &need, plan, d, hidden);
+  if (!workspace || workspace_bytes < need || !aligned16(workspace))
+    return fail(FFK_ERR_WORKSPACE, "transition_backward: workspace %zu bytes < %zu", workspace_bytes, need);
+  a.x = x;
+  a.scales = static_cast<const uint8_t*>(scales);
+  a.dy = static_cast<const bf16*>(dy);
+  a.ln_w = ln_w;
+  a.ln_b = ln_b;
+  a.wa = w_expand_a;
+  a.wb = w_expand_b;
+  a.ws = w_squeeze;
+  a.dx = static_cast<bf16*>(dx);
+  a.dln_w = dln_w;
+  a.dln_b = dln_b;
+  a.dwa = dw_expand_a;
+  a.dwb = dw_expand_b;
+  a.dws = dw_squeeze;
+  a.rows = rows;
+  a.d = d;
+  a.hidden = hidden;
+  a.residual = residual;
+  a.grad_dtype = grad_dtype;
+  a.eps = eps;
+  launch_transition_grad(a, plan, static_cast<hipStream_t>(stream));
+  return check_launch("transition_backward");
 }
 
 int32_t ffk_layer_norm_linear(const void* x, const float* ln_w, const float* ln_b,

@@ -115,6 +115,13 @@ PyMethodDef methods[] = {
     FFK_CALL(ffk_outer_product_mean),
     FFK_CALL(ffk_outer_product_mean_grouped_workspace),
     FFK_CALL(ffk_outer_product_mean_grouped),
+    FFK_CALL(ffk_quantize_activation),
+    FFK_CALL(ffk_restore_activation),
+    FFK_CALL(ffk_layer_norm_checkpoint),
+    FFK_CALL(ffk_layer_norm_backward_workspace),
+    FFK_CALL(ffk_layer_norm_backward),
+    FFK_CALL(ffk_transition_backward_workspace),
+    FFK_CALL(ffk_transition_backward),
     {nullptr, nullptr, 0, nullptr},
 };
 

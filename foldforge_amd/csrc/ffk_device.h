@@ -266,6 +266,20 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
+// Sum over aligned groups of L lanes, L = 8, 16, 32 or 64 (every lane of the group gets the total).
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
+  v = sum4(v);
+  v += dpp_f<kDppHalfMirror>(v);
+  if constexpr (L >= 16) v += dpp_f<kDppMirror>(v);
+  if constexpr (L >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if constexpr (L >= 64) v = pair_sum(v);
+  return v;
+}
+
 // Row stride (elements) of a 128-channel bf16 tile in LDS: 16 bytes of padding per row.
 constexpr int kRow = 136;
 

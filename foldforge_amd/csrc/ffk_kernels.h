@@ -382,4 +382,57 @@ int resident_blocks(const void* kernel, int threads, size_t dynamic_lds) noexcep
 void launch_layer_norm(const void* x, const float* w, const float* b, void* y, int64_t rows,
                        int cols, float eps, int dtype, hipStream_t stream);
 
+// 8-bit activations (ffk_activation.h): codes [rows][cols], scales [rows][ceil(cols / 32)].
+void launch_quantize(const void* x, uint8_t* codes, uint8_t* scales, int64_t rows, int cols, int dtype,
+                     hipStream_t stream);
+void launch_restore(const uint8_t* codes, const uint8_t* scales, void* x, int64_t rows, int cols, int dtype,
+                    hipStream_t stream);
+
+// LayerNorm and the 8-bit activation of its input (y may not alias x).
+void launch_layer_norm_keep(const void* x, const float* w, const float* b, void* y, uint8_t* codes, uint8_t* scales,
+                            int64_t rows, int cols, float eps, int dtype, hipStream_t stream);
+
+// Backward pass of LayerNorm.
+struct LayerNormGradArgs {
+  const void* x;          // the kept input, or (scales non-null) its codes
+  const uint8_t* scales;
+  const void* dy;
+  const float* w;         // may be null (1)
+  void* dx;               // dtype, as x and dy
+  void *dw, *db;          // grad_dtype; either may be null
+  float* part;            // layer_norm_grad_floats(rows, cols) floats
+  int64_t rows;
+  int cols, dtype, grad_dtype;
+  float eps;
+};
+size_t layer_norm_grad_floats(int64_t rows, int cols);
+void launch_layer_norm_grad(const LayerNormGradArgs& a, hipStream_t stream);
+
+// out[c] = sum over k < count of part[k][c] in a fixed order: the first split columns to out0, the rest to out1.
+void launch_sum_partials(const float* part, int count, int width, int split, void* out0, void* out1, int dtype,
+                         hipStream_t stream);
+
+// Backward pass of the SwiGLU transition (rows > 0; d a multiple of 64 up to 768, hidden of 64).
+struct TransitionGradPlan {
+  int64_t chunk;                         // rows at once, a multiple of 64
+  int dn_splits, dw_splits, norm_blocks;
+};
+TransitionGradPlan transition_grad_plan(int64_t rows, int d, int hidden);
+struct TransitionGradArgs {
+  const void* x;          // the kept input bf16, or (scales non-null) its codes
+  const uint8_t* scales;
+  const bf16* dy;
+  const float *ln_w, *ln_b, *wa, *wb, *ws;
+  bf16* dx;
+  void *dln_w, *dln_b, *dwa, *dwb, *dws;  // grad_dtype
+  int64_t rows;
+  int d, hidden, residual, grad_dtype;
+  float eps;
+  // workspace
+  bf16 *ab, *st, *abt;    // [2 hidden][d], [hidden][d], [d][2 hidden]
+  bf16 *n, *E;            // [chunk][d], [chunk][3 hidden]
+  float *dn, *norm_part, *dw_part;  // [dn_splits][chunk][d], [norm_blocks][2][d], [dw_splits][3 hidden][d]
+};
+void launch_transition_grad(const TransitionGradArgs& a, const TransitionGradPlan& p, hipStream_t stream);
+
 }  // namespace ffk

@@ -31,20 +31,6 @@ struct LnPiece {
   typedef T vec __attribute__((__vector_size__(16)));
 };
 
-// Sum over aligned groups of L lanes (every lane of the group gets the total).
-template <int L>
-__device__ __forceinline__ float lanes_sum(float v) {
-  v = sum4(v);
-  v += dpp_f<kDppHalfMirror>(v);
-  if constexpr (L >= 16) v += dpp_f<kDppMirror>(v);
-  if constexpr (L >= 32) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-  }
-  if constexpr (L >= 64) v = pair_sum(v);
-  return v;
-}
-
 // Rows of exactly L * P pieces; x and y 16-byte aligned. grid min(ceil(rows / (R 256 / L)),
 // 32 per CU); block 256.
 template <typename T, int L, int P>

@@ -14,6 +14,9 @@ module classes decide what to refuse (``unsupported``) before a call ever gets h
 
 from __future__ import annotations
 
+from dataclasses import dataclass
+from typing import NamedTuple
+
 import torch
 
 from foldforge_amd import _native
@@ -218,6 +221,155 @@ def swiglu_ffn(x: Tensor, w_a: Tensor, w_b: Tensor, w_out: Tensor, residual: Ten
     return out
 
 
+#: channels of a row that share a scale in an :class:`Activation8`
+ACTIVATION_BLOCK = 32
+
+
+@dataclass(frozen=True)
+class Activation8:
+    """A bf16 or fp32 row tensor kept in 8 bits for a backward pass (``include/foldforge_amd.h``,
+    ``ffk_quantize_activation``): e4m3 ``codes`` of the tensor's shape and, for each block of 32
+    channels of a row, the byte ``s + 127`` of the power of two that its codes are multiples of,
+    ``scales [..., ceil(c / 32)]``. ``dtype``: the tensor's. 33 / 32 bytes a value; a value is off
+    by at most 2^-4 of itself, or half a step of 2^(s-9) where it is below 2^(s-6); NaN and
+    infinities become NaN."""
+
+    codes: Tensor
+    scales: Tensor
+    dtype: torch.dtype
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.codes.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def restore(self) -> Tensor:
+        """The tensor that the codes stand for (:func:`restore_activation`)."""
+        return restore_activation(self)
+
+
+def _call(device: torch.device, name: str, *args) -> None:
+    """``ffk_<name>(*args, stream)`` on ``device`` and its current stream."""
+    fn = getattr(_native.calls(), "ffk_" + name)
+    if device.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            status = fn(*args, _stream(device))
+    else:
+        status = fn(*args, _stream(device))
+    _native.check(status, name)
+
+
+def _dtype_code(dtype: torch.dtype) -> int:
+    return 0 if dtype == torch.bfloat16 else 1
+
+
+def _rows_tensor(x: Tensor, name: str) -> int:
+    """The rows of a contiguous bf16 / fp32 device tensor with a last axis."""
+    if not (isinstance(x, Tensor) and _on_device(x) and x.is_contiguous()):
+        _refuse(f"{name} must be a contiguous device tensor")
+    if x.dtype not in (torch.bfloat16, torch.float32):
+        _refuse(f"{name} must be bf16 or fp32 (got {x.dtype})")
+    if x.dim() == 0 or x.shape[-1] == 0:
+        _refuse(f"{name} needs a last axis of channels (got {tuple(x.shape)})")
+    return x.numel() // x.shape[-1]
+
+
+def _new_activation(x: Tensor) -> Activation8:
+    blocks = -(-x.shape[-1] // ACTIVATION_BLOCK)
+    return Activation8(torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device),
+                       torch.empty((*x.shape[:-1], blocks), dtype=torch.uint8, device=x.device), x.dtype)
+
+
+def _check_activation(a: Activation8, name: str) -> None:
+    """An :class:`Activation8` as :func:`quantize_activation` makes it (the C-ABI receives no sizes)."""
+    c, s = a.codes, a.scales
+    if not (_on_device(c) and c.is_contiguous() and c.dtype == torch.float8_e4m3fn and c.dim() > 0 and c.shape[-1] > 0):
+        _refuse(f"{name}: codes must be a contiguous float8_e4m3fn device tensor")
+    want = (*c.shape[:-1], -(-c.shape[-1] // ACTIVATION_BLOCK))
+    if not (s.device == c.device and s.is_contiguous() and s.dtype == torch.uint8 and tuple(s.shape) == want):
+        _refuse(f"{name}: scales must be contiguous uint8 {want} beside the codes (got {tuple(s.shape)} {s.dtype})")
+    if a.dtype not in (torch.bfloat16, torch.float32):
+        _refuse(f"{name}: dtype must be bf16 or fp32 (got {a.dtype})")
+
+
+def quantize_activation(x: Tensor) -> Activation8:
+    """``x [..., c]`` (bf16 or fp32) in 8 bits."""
+    rows = _rows_tensor(x, "x")
+    a = _new_activation(x)
+    if rows:
+        _call(x.device, "quantize_activation", x, a.codes, a.scales, rows, x.shape[-1], _dtype_code(x.dtype))
+    return a
+
+
+def restore_activation(a: Activation8, *, out: Tensor | None = None) -> Tensor:
+    """The values that ``a`` stands for, in its ``dtype``."""
+    _check_activation(a, "activation")
+    out = _output(out, tuple(a.shape), a.dtype, a.device)
+    if out.numel():
+        _call(a.device, "restore_activation", a.codes, a.scales, out, out.numel() // out.shape[-1], out.shape[-1],
+              _dtype_code(a.dtype))
+    return out
+
+
+def _affine(t: Tensor | None, device: torch.device, name: str, cols: int) -> Tensor | None:
+    return None if t is None else _param(t, device, name, (cols,))
+
+
+def layer_norm_checkpoint(x: Tensor, weight: Tensor | None, bias: Tensor | None,
+                          eps: float = 1e-5) -> tuple[Tensor, Activation8]:
+    """:func:`layer_norm` of ``x`` and the 8-bit activation of ``x`` that its backward pass takes, in one pass
+    (rows of at most 1024 channels; two for wider ones)."""
+    rows, cols = _rows_tensor(x, "x"), x.shape[-1]
+    weight, bias = _affine(weight, x.device, "weight", cols), _affine(bias, x.device, "bias", cols)
+    y, a = torch.empty_like(x), _new_activation(x)
+    if rows:
+        _call(x.device, "layer_norm_checkpoint", x, weight, bias, y, a.codes, a.scales, rows, cols, float(eps),
+              _dtype_code(x.dtype))
+    return y, a
+
+
+def _kept(x: Tensor | Activation8, dy: Tensor) -> tuple[Tensor, Tensor | None]:
+    """The pointers of a kept input (tensor or codes, and scales), checked against the gradient."""
+    if isinstance(x, Activation8):
+        _check_activation(x, "x")
+        kept = x.codes, x.scales
+    else:
+        _rows_tensor(x, "x")
+        kept = x, None
+    if x.dtype != dy.dtype or tuple(x.shape) != tuple(dy.shape) or x.device != dy.device:
+        _refuse(f"dy {tuple(dy.shape)} {dy.dtype} on {dy.device} is not like x {tuple(x.shape)} {x.dtype} on {x.device}")
+    return kept
+
+
+def _grad_dtype(dtype: torch.dtype) -> int:
+    if dtype not in (torch.bfloat16, torch.float32):
+        _refuse(f"grad_dtype must be bf16 or fp32 (got {dtype})")
+    return _dtype_code(dtype)
+
+
+def layer_norm_backward(dy: Tensor, x: Tensor | Activation8, weight: Tensor | None = None, eps: float = 1e-5, *,
+                        with_bias: bool = True, grad_dtype: torch.dtype = torch.float32,
+                        ) -> tuple[Tensor, Tensor | None, Tensor | None]:
+    """``(dx, dweight, dbias)`` of :func:`layer_norm` from the output's gradient ``dy`` and the kept input
+    ``x``: the tensor itself or its 8-bit activation (the gradient at the restored values). ``dx`` in
+    ``dy.dtype``; the affine's gradients, sums over the rows in fp32 and a fixed order, in ``grad_dtype``
+    (``dweight`` None without ``weight``, ``dbias`` None without ``with_bias``)."""
+    rows, cols, dev = _rows_tensor(dy, "dy"), dy.shape[-1], dy.device
+    kept, scales = _kept(x, dy)
+    weight = _affine(weight, dev, "weight", cols)
+    code = _grad_dtype(grad_dtype)
+    dx = torch.empty_like(dy)
+    dweight = None if weight is None else torch.empty(cols, dtype=grad_dtype, device=dev)
+    dbias = torch.empty(cols, dtype=grad_dtype, device=dev) if with_bias else None
+    ws = _workspace(_native.calls().ffk_layer_norm_backward_workspace(rows, cols), dev)
+    _call(dev, "layer_norm_backward", dy, kept, scales, weight, dx, dweight, dbias, ws, ws.numel(), rows, cols,
+          float(eps), _dtype_code(dy.dtype), code)
+    return dx, dweight, dbias
+
+
 def triangle_multiplicative_update(
     z: Tensor,
     mask: Tensor,
@@ -375,6 +527,70 @@ def transition(
     )
     _native.check(status, "transition")
     return out
+
+
+def transition_backward_supported(d: int, factor: int) -> bool:
+    """Widths of the transition's backward kernels."""
+    return 0 < d <= 768 and d % 64 == 0 and 0 < factor <= 64
+
+
+class TransitionGradients(NamedTuple):
+    """Gradients of a transition's input and parameters (named as :func:`transition` takes them)."""
+
+    x: Tensor
+    ln_weight: Tensor
+    ln_bias: Tensor
+    expand_a: Tensor
+    expand_b: Tensor
+    squeeze: Tensor
+
+
+def transition_checkpoint(x: Tensor, *, residual: bool = True, eps: float = 1e-5,
+                          **params: Tensor) -> tuple[Tensor, Activation8]:
+    """:func:`transition` of ``x`` and the 8-bit activation of ``x`` that its backward pass takes."""
+    out = transition(x, residual=residual, eps=eps, **params)
+    return out, quantize_activation(x)
+
+
+def transition_backward(
+    dy: Tensor,
+    x: Tensor | Activation8,
+    *,
+    ln_weight: Tensor,
+    ln_bias: Tensor,
+    expand_a: Tensor,
+    expand_b: Tensor,
+    squeeze: Tensor,
+    residual: bool = True,
+    eps: float = 1e-5,
+    grad_dtype: torch.dtype = torch.float32,
+) -> TransitionGradients:
+    """Gradients of :func:`transition` from the output's gradient ``dy [..., d]`` bf16 and the kept input
+    ``x``: the bf16 tensor itself or its 8-bit activation (the gradient at the restored values). The hidden
+    rows are computed again; products on bf16 operands, fp32 sums in a fixed order. The parameters'
+    gradients in ``grad_dtype``. d a multiple of 64 up to 768."""
+    rows, d, dev = _rows_tensor(dy, "dy"), dy.shape[-1], dy.device
+    if dy.dtype != torch.bfloat16:
+        _refuse(f"dy must be bf16 (got {dy.dtype})")
+    kept, scales = _kept(x, dy)
+    factor = expand_a.shape[0] // d
+    if not transition_backward_supported(d, factor):
+        _refuse(f"width {d} x {factor} (the backward kernels take a multiple of 64 up to 768, factor up to 64)")
+    shapes = {"ln_weight": (d,), "ln_bias": (d,), "expand_a": (factor * d, d), "expand_b": (factor * d, d),
+              "squeeze": (d, factor * d)}
+    given = {"ln_weight": ln_weight, "ln_bias": ln_bias, "expand_a": expand_a, "expand_b": expand_b,
+             "squeeze": squeeze}
+    ps = _params(dy, tuple((nm, given[nm], shape) for nm, shape in shapes.items()))
+    code = _grad_dtype(grad_dtype)
+    for t, name in ((dy, "dy"), (kept, "x")):
+        if t.data_ptr() % 16:
+            _refuse(f"{name} must be 16-byte aligned")
+    grads = TransitionGradients(torch.empty_like(dy), *(torch.empty(shape, dtype=grad_dtype, device=dev)
+                                                        for shape in shapes.values()))
+    ws = _workspace(_native.calls().ffk_transition_backward_workspace(rows, d, factor), dev)
+    _call(dev, "transition_backward", dy, kept, scales, *ps, *grads, ws, ws.numel(), rows, d, factor, int(residual),
+          float(eps), code)
+    return grads
 
 
 #: the engine's name for the transition kernel (``docs/guides/ENGINE-2.4.2.md:19``)

@@ -93,6 +93,42 @@ int32_t ffk_swiglu_ffn(const void* x, const float* w_a, const float* w_b, const 
                        int64_t rows, int32_t d, int32_t hidden, void* stream);
 
 /*
+ * 8-bit activations: what a forward pass keeps of its input for the backward pass. For each block of
+ * 32 consecutive channels of a row (the last of a row may be shorter), with a the largest finite |x| of
+ * the block and s the least whole number >= -126 with a <= 448 * 2^s:
+ *   scales = s + 127,  codes = e4m3(x / 2^s) (OCP, nearest, ties to even),  restored = codes * 2^s
+ * NaN and infinities become NaN. x [rows, cols] bf16 or fp32 (dtype), codes [rows, cols] bytes,
+ * scales [rows, ceil(cols / 32)] bytes. Any width; rows of whole blocks on 16-byte aligned x and 8-byte
+ * aligned codes take the wide path. No counterpart in the reference.
+ */
+int32_t ffk_quantize_activation(const void* x, void* codes, void* scales, int64_t rows, int32_t cols,
+                                int32_t dtype, void* stream);
+int32_t ffk_restore_activation(const void* codes, const void* scales, void* x, int64_t rows, int32_t cols,
+                               int32_t dtype, void* stream);
+
+/*
+ * ffk_layer_norm that keeps its input as an 8-bit activation in the same pass (y may not alias x).
+ */
+int32_t ffk_layer_norm_checkpoint(const void* x, const float* weight, const float* bias, void* y,
+                                  void* codes, void* scales, int64_t rows, int32_t cols, float eps,
+                                  int32_t dtype, void* stream);
+
+/*
+ * Backward pass of ffk_layer_norm at the kept input. With xh = (x - mean) rstd and g = dy * weight:
+ *   dx = rstd (g - mean(g) - xh mean(g xh)),  dweight = sum over rows of dy xh,  dbias = sum over rows of dy
+ * x: the input itself (scales NULL; dtype, as dy and dx) or the codes of its 8-bit activation with their
+ * scales; statistics, sums and products in fp32, the statistics taken from the kept input again. weight
+ * may be NULL (1); dweight / dbias [cols] in grad_dtype, either may be NULL. dx aliases nothing. The row
+ * sums are added in a fixed order. Workspace: ffk_layer_norm_backward_workspace bytes.
+ * Reference: the gradient of torch.nn.LayerNorm that its training path takes (train/step.py:320-338).
+ */
+size_t ffk_layer_norm_backward_workspace(int64_t rows, int32_t cols);
+int32_t ffk_layer_norm_backward(const void* dy, const void* x, const void* scales, const float* weight,
+                                void* dx, void* dweight, void* dbias, void* workspace,
+                                size_t workspace_bytes, int64_t rows, int32_t cols, float eps,
+                                int32_t dtype, int32_t grad_dtype, void* stream);
+
+/*
  * Triangle multiplicative update, outgoing (outgoing = 1) or incoming (0), including
  * the LayerNorm + gated projections prologue and the centre norm + output projection +
  * output gate epilogue. d_pair = d_hidden = 128 runs the fused kernels; other widths (d_pair
@@ -231,6 +267,26 @@ int32_t ffk_transition_noalloc(const void* x, const float* ln_w, const float* ln
                                const float* w_expand_a, const float* w_expand_b,
                                const float* w_squeeze, void* out, int64_t rows, int32_t d,
                                int32_t factor, int32_t residual, float eps, void* stream);
+
+/*
+ * Backward pass of ffk_transition at the kept input: with n = LN(x), a = n w_a^T, b = n w_b^T,
+ * u = silu(a) b and s the logistic function,
+ *   du = dy w_squeeze, da = du b s(a) (1 + a (1 - s(a))), db = du silu(a)
+ *   dw_a = da^T n, dw_b = db^T n, dw_squeeze = dy^T u, dn = da w_a + db w_b
+ *   dx = (residual ? dy : 0) + (LayerNorm's backward of dn), dln_w, dln_b its affine's
+ * x: the bf16 input (scales NULL) or the codes of its 8-bit activation with their scales; dy, dx
+ * [rows, d] bf16; parameters as in ffk_transition; their gradients in grad_dtype (FFK_DTYPE_*), shaped
+ * like the parameters. The hidden rows are computed again from x: nothing else is kept. Products on bf16
+ * operands with fp32 sums in a fixed order. d a multiple of 64 up to 768, factor * d of 64. dx aliases
+ * nothing. Reference: the training path's gradient of the transition (train/step.py:320-338).
+ */
+size_t ffk_transition_backward_workspace(int64_t rows, int32_t d, int32_t factor);
+int32_t ffk_transition_backward(const void* dy, const void* x, const void* scales, const float* ln_w,
+                                const float* ln_b, const float* w_expand_a, const float* w_expand_b,
+                                const float* w_squeeze, void* dx, void* dln_w, void* dln_b,
+                                void* dw_expand_a, void* dw_expand_b, void* dw_squeeze, void* workspace,
+                                size_t workspace_bytes, int64_t rows, int32_t d, int32_t factor,
+                                int32_t residual, float eps, int32_t grad_dtype, void* stream);
 
 /*
  * Single-track attention with pair bias, residual included:
