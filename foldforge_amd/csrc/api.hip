@@ -279,14 +279,20 @@ TransitionGradArgs transition_grad_ws(void* ws, size_t* bytes, const TransitionG
   Carver cv{static_cast<char*>(ws)};
   TransitionGradArgs a{};
   const size_t w = (size_t)hidden * d;
-  a.ab = cv.take<bf16>(2 * w);
+  a.peaks = cv.take<float>(p.peaks);
+  a.scale = cv.take<float>(2);
+  a.offset = cv.take<float>(2 * (size_t)hidden);
+  a.aw = cv.take<f16>(2 * w);
   a.st = cv.take<bf16>(w);
   a.abt = cv.take<bf16>(2 * w);
-  a.n = cv.take<bf16>((size_t)p.chunk * d);
+  a.xh = cv.take<f16>((size_t)p.chunk * d);
+  a.xhb = cv.take<bf16>((size_t)p.chunk * d);
+  a.rstd = cv.take<float>((size_t)p.chunk);
   a.E = cv.take<bf16>((size_t)p.chunk * 3 * hidden);
-  a.dn = cv.take<float>((size_t)p.dn_splits * p.chunk * d);
-  a.norm_part = cv.take<float>((size_t)p.norm_blocks * 2 * d);
+  a.dxh = cv.take<float>((size_t)p.dxh_splits * p.chunk * d);
   a.dw_part = cv.take<float>((size_t)p.dw_splits * 3 * w);
+  a.sums = cv.take<float>((size_t)p.dw_splits * 2 * hidden);
+  a.norm_part = cv.take<float>((size_t)hidden / 16 * 2 * d);
   *bytes = cv.used;
   return a;
 }

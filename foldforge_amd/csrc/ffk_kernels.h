@@ -414,8 +414,8 @@ void launch_sum_partials(const float* part, int count, int width, int split, voi
 
 // Backward pass of the SwiGLU transition (rows > 0; d a multiple of 64 up to 768, hidden of 64).
 struct TransitionGradPlan {
-  int64_t chunk;                         // rows at once, a multiple of 64
-  int dn_splits, dw_splits, norm_blocks;
+  int64_t chunk;  // rows at once, a multiple of 64
+  int dxh_splits, dw_splits, peaks;
 };
 TransitionGradPlan transition_grad_plan(int64_t rows, int d, int hidden);
 struct TransitionGradArgs {
@@ -428,10 +428,15 @@ struct TransitionGradArgs {
   int64_t rows;
   int d, hidden, residual, grad_dtype;
   float eps;
-  // workspace
-  bf16 *ab, *st, *abt;    // [2 hidden][d], [hidden][d], [d][2 hidden]
-  bf16 *n, *E;            // [chunk][d], [chunk][3 hidden]
-  float *dn, *norm_part, *dw_part;  // [dn_splits][chunk][d], [norm_blocks][2][d], [dw_splits][3 hidden][d]
+  // workspace: the weights in the products' orders and their scales,
+  float *peaks, *scale, *offset;        // [peaks], [2], [2 hidden]
+  f16* aw;                              // [2 hidden][d]
+  bf16 *st, *abt;                       // [hidden][d], [d][2 hidden]
+  // a chunk's normalised rows, hidden gradients and the products' parts
+  f16* xh;                              // [chunk][d]
+  bf16 *xhb, *E;                        // [chunk][d], [chunk][3 hidden]
+  float *rstd, *dxh;                    // [chunk], [dxh_splits][chunk][d]
+  float *dw_part, *sums, *norm_part;    // [dw_splits][3 hidden][d], [dw_splits][2 hidden], [hidden / 16][2][d]
 };
 void launch_transition_grad(const TransitionGradArgs& a, const TransitionGradPlan& p, hipStream_t stream);
 

@@ -1,18 +1,22 @@
 // Backward pass of the SwiGLU transition on gfx950.
 //
-//   n = LN(x), a = n A^T, b = n B^T, u = silu(a) b, y = x + u S^T          (A, B [H][d], S [d][H])
-//   du = dy S,  da = du b s(a) (1 + a (1 - s(a))),  db = du silu(a)        (s: the logistic function)
+//   n = LN(x) = xh w + v, a = n A^T, b = n B^T, u = silu(a) b, y = x + u S^T     (A, B [H][d], S [d][H])
+//   du = dy S,  da = du b s(a) (1 + a (1 - s(a))),  db = du silu(a)              (s: the logistic function)
 //   dA = da^T n,  dB = db^T n,  dS = dy^T u,  dn = da A + db B,  dx = dy + LN'(dn)
 // at the kept x (the input or its 8-bit activation): the hidden rows are computed again, nothing but x is
-// kept between the passes. 16 M d H flops for M rows, on bf16 operands with fp32 sums.
+// kept between the passes. 16 M d H flops for M rows, fp32 sums.
 //
-// The form for every width (d and H multiples of 64), in chunks of rows:
-//   norm_rows        n in bf16
-//   hidden_grad      a, b and du tile by tile, their elementwise part in registers -> E = [da | db | u]
-//   gemm64<false>    dn = [da | db] [A; B], split over the hidden channels where the rows are few
-//   norm_grad_rows   dx, and the sums of the affine's gradients
-//   gemm64<true>     E^T [n or dy], split over the rows: dA, dB and dS^T
-// and at the end the partial sums are added in a fixed order.
+// The norm's affine is taken out of the rows' way: with Aw = A diag(w) and Bw = B diag(w),
+//   a = xh Aw^T + A v,   dxh = da Aw + db Bw,   dx = dy + rstd (dxh - mean(dxh) - xh mean(dxh xh))
+//   dA = (da^T xh) diag(w) + (sum da) v^T,   dw = sum over h of A (da^T xh) + B (db^T xh),
+//   dv = A^T (sum da) + B^T (sum db)
+// so dw and dv come out of the weights' gradients, and the products see xh alone, whose values are at most
+// sqrt(d): a and b are products of fp16 operands (Aw and Bw times a power of two that puts their largest
+// entry at 2^14 .. 2^15, so that entries down to 2^-29 of it keep fp16's 11 bits), which leaves their errors at an
+// eighth of bf16's. The gradients' operands are bf16, whose range they need: three bf16 roundings lie between
+// dy and a gradient, and one of the result (relative error 3.3e-3 rather than the 4.6e-3 of bf16 throughout).
+// The powers of two 2^ka, 2^kb ride along: a' = 2^ka a, b' = 2^kb b, so silu' = 2^ka silu, da' = 2^kb da,
+// db' = 2^ka db, u' = 2^(ka+kb) u; the transposed weights carry their inverses, the join takes the rest out.
 #include <algorithm>
 
 #include "ffk_activation.h"
@@ -23,6 +27,13 @@ namespace ffk {
 
 namespace {
 
+typedef f16 f16x8 __attribute__((__vector_size__(8 * sizeof(f16))));
+
+__device__ __forceinline__ f32x16 mfma32h(f16x8 a, f16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f16x8 ld8h(const f16* p) { return *reinterpret_cast<const f16x8*>(p); }
+
 // A tile of 64-channel bf16 rows in LDS (128 bytes a row, 8 pieces of 16): piece p of row r lies at piece
 // p ^ swz64(r). Sixteen lanes that read one piece of sixteen consecutive rows (an operand fetch) fall on all
 // 64 banks, and eight rows' 64-byte halves (a transposing fetch) on each bank twice, the least for 512 bytes.
@@ -31,8 +42,9 @@ __device__ __forceinline__ int off64(int r, int p) { return r * 64 + 8 * (p ^ sw
 
 // This wave's share of a 64 x 64 tile (rows row0 .. row0 + 63 of src, clamped to `last`, channels c0 .. c0 + 63)
 // into LDS at byte address dst: 8 rows an instruction. 4 waves.
-__device__ __forceinline__ void tile_dma(const bf16* src, int64_t ld, int64_t row0, int64_t last, int c0, uint32_t dst,
+__device__ __forceinline__ void tile_dma(const void* src_, int64_t ld, int64_t row0, int64_t last, int c0, uint32_t dst,
                                          int wave, int lane) {
+  const bf16* src = static_cast<const bf16*>(src_);  // (or fp16: 2 bytes a value)
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int r0 = 8 * (2 * wave + u), r = r0 + (lane >> 3);
@@ -64,76 +76,160 @@ __device__ __forceinline__ bf16x8 ld_turned(const bf16* tile, int c0, int k0, in
   return o.v;
 }
 
-// fp32 parameters -> bf16, each in the orders the products read: ab [2 H][d] (A, then B), st [H][d] (S^T),
-// abt [d][2 H]. A 32 x 32 tile a workgroup: grid (H / 32, d / 32, 3); block 256.
+// What a call's kernels share: the scales' exponents as factors.
+//   scale[0] = 2^-ka, scale[1] = 2^-kb
+// The largest |A w| and |B w| of each workgroup's share of the entries. grid (kPeakBlocks, 2); block 256.
+constexpr int kPeakBlocks = 32;
+__global__ __launch_bounds__(256) void weight_peaks(const float* __restrict__ wa, const float* __restrict__ wb,
+                                                    const float* __restrict__ w, float* __restrict__ peaks, int d,
+                                                    int H) {
+  __shared__ float red[4];
+  const float* src = blockIdx.y ? wb : wa;
+  float top = 0.f;
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < (int64_t)H * d; i += (int64_t)kPeakBlocks * 1024) {
+    const f32x4_a4 v = *reinterpret_cast<const f32x4_a4*>(src + i);
+    const int c = (int)(i % d);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = fmaxf(top, finite_abs(v[e] * w[c + e]));
+  }
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    peaks[blockIdx.y * kPeakBlocks + blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+// k with peak 2^k in [2^14, 2^15) (within what fp32 powers allow; 0 for a matrix of zeros).
+__device__ __forceinline__ int peak_power(float peak) {
+  if (peak == 0.f) return 0;
+  const int k = 14 + 127 - (int)(__float_as_uint(peak) >> 23);
+  return k < -110 ? -110 : k > 110 ? 110 : k;
+}
+__device__ __forceinline__ float two_to(int k) { return __uint_as_float((uint32_t)(127 + k) << 23); }
+
+// fp32 parameters in the orders the products read: aw [2 H][d] fp16 (Aw 2^ka, then Bw 2^kb), st [H][d] bf16 (S^T),
+// abt [d][2 H] bf16 (Aw^T 2^-kb, Bw^T 2^-ka; within each 16 hidden channels in accumulator order 0-3, 8-11, 4-7,
+// 12-15 where turned, else in order), offset [2][H] fp32 (A v 2^ka, B v 2^kb), scale. 32 hidden channels a
+// workgroup: grid (H / 32, 3); block 256.
 __global__ __launch_bounds__(256) void pack_grad_weights(const float* __restrict__ wa, const float* __restrict__ wb,
-                                                         const float* __restrict__ ws, bf16* __restrict__ ab,
-                                                         bf16* __restrict__ st, bf16* __restrict__ abt, int d, int H) {
-  __shared__ bf16 tile[32][33];
-  const int h0 = blockIdx.x * 32, c0 = blockIdx.y * 32, which = blockIdx.z;
+                                                         const float* __restrict__ ws, const float* __restrict__ w,
+                                                         const float* __restrict__ v, const float* __restrict__ peaks,
+                                                         f16* __restrict__ aw, bf16* __restrict__ st,
+                                                         bf16* __restrict__ abt, float* __restrict__ offset,
+                                                         float* __restrict__ scale, int d, int H, int turned) {
+  __shared__ float tile[32][33];
+  const int h0 = blockIdx.x * 32, which = blockIdx.y;
   const int col = threadIdx.x & 31, row = threadIdx.x >> 5;
-  if (which < 2) {
-    const float* src = which ? wb : wa;
-    for (int r = row; r < 32; r += 8) {
-      const bf16 v = (bf16)src[(int64_t)(h0 + r) * d + c0 + col];
-      ab[(int64_t)(which * H + h0 + r) * d + c0 + col] = v;
-      tile[r][col] = v;
+  if (which == 2) {
+    for (int c0 = 0; c0 < d; c0 += 32) {
+      __syncthreads();
+      for (int r = row; r < 32; r += 8) tile[r][col] = ws[(int64_t)(c0 + r) * H + h0 + col];
+      __syncthreads();
+      for (int r = row; r < 32; r += 8) st[(int64_t)(h0 + r) * d + c0 + col] = (bf16)tile[col][r];
+    }
+    return;
+  }
+  float peak[2] = {0.f, 0.f};
+  for (int i = 0; i < kPeakBlocks; ++i) {
+    peak[0] = fmaxf(peak[0], peaks[i]);
+    peak[1] = fmaxf(peak[1], peaks[kPeakBlocks + i]);
+  }
+  const int ka = peak_power(peak[0]), kb = peak_power(peak[1]);
+  if (blockIdx.x == 0 && which == 0 && threadIdx.x == 0) {
+    scale[0] = two_to(-ka);
+    scale[1] = two_to(-kb);
+  }
+  const float up = two_to(which ? kb : ka), down = two_to(which ? -ka : -kb);
+  const float* src = which ? wb : wa;
+  float dot[4] = {0.f, 0.f, 0.f, 0.f};
+  // hidden channel of place `col` of the turned order
+  const int hid = turned ? (col & ~12) | ((col & 4) << 1) | ((col & 8) >> 1) : col;
+  for (int c0 = 0; c0 < d; c0 += 32) {
+    const float wc = w[c0 + col], vc = v[c0 + col];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = row + 8 * i;
+      const float t = src[(int64_t)(h0 + r) * d + c0 + col];
+      dot[i] += t * vc;
+      tile[r][col] = t * wc;
+      aw[(int64_t)(which * H + h0 + r) * d + c0 + col] = (f16)(t * wc * up);
     }
     __syncthreads();
-    for (int r = row; r < 32; r += 8) abt[(int64_t)(c0 + r) * 2 * H + which * H + h0 + col] = tile[col][r];
-  } else {
-    for (int r = row; r < 32; r += 8) tile[r][col] = (bf16)ws[(int64_t)(c0 + r) * H + h0 + col];
-    __syncthreads();
-    for (int r = row; r < 32; r += 8) st[(int64_t)(h0 + r) * d + c0 + col] = tile[col][r];
+    for (int r = row; r < 32; r += 8)
+      abt[(int64_t)(c0 + r) * 2 * H + which * H + h0 + col] = (bf16)(tile[hid][r] * down);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float t = lanes_sum<32>(dot[i]);
+    if (col == 0) offset[which * H + h0 + row + 8 * i] = t * up;
   }
 }
 
-// n = LN(x) in bf16, one wave a row, K = d / 64 channels a lane. grid-strided; block 256.
+// xh in fp16 and bf16 and rstd of the kept rows: 8 lanes a row, K = d / 64 pieces of 8 channels each.
+// grid-strided; block 256 (32 rows).
 template <bool CODES, int K>
-__global__ __launch_bounds__(256) void norm_rows(const void* x, const uint8_t* scales, const float* __restrict__ w,
-                                                 const float* __restrict__ b, bf16* __restrict__ n, int64_t rows,
+__global__ __launch_bounds__(256) void norm_rows(const void* x, const uint8_t* scales, f16* __restrict__ xh,
+                                                 bf16* __restrict__ xhb, float* __restrict__ rstd_out, int64_t rows,
                                                  float eps) {
   constexpr int d = 64 * K, blocks = d / kActBlock;
-  const int lane = threadIdx.x & 63;
-  for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += (int64_t)gridDim.x * 4) {
-    float v[K];
+  const int sub = threadIdx.x & 7;
+  for (int64_t row = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3); row - (threadIdx.x >> 3) < rows;
+       row += (int64_t)gridDim.x * 32) {
+    const bool real = row < rows;
+    float v[8 * K];
     float s = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      KeptPiece<bf16, CODES, 1> p;
-      p.load(x, scales, row, lane + 64 * k, d, blocks);
-      p.values(&v[k]);
-      s += v[k];
+      KeptPiece<bf16, CODES, 8> p;
+      p.load(x, scales, real ? row : rows - 1, 8 * sub + 64 * k, d, blocks);
+      p.values(v + 8 * k);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += v[8 * k + e];
     }
-    const float mean = lanes_sum<64>(s) * (1.f / d);
+    const float mean = lanes_sum<8>(s) * (1.f / d);
     float q = 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      v[k] -= mean;
-      q += v[k] * v[k];
+    for (int i = 0; i < 8 * K; ++i) {
+      v[i] -= mean;
+      q += v[i] * v[i];
     }
-    const float rstd = __builtin_amdgcn_rsqf(lanes_sum<64>(q) * (1.f / d) + eps);
+    const float rstd = __builtin_amdgcn_rsqf(lanes_sum<8>(q) * (1.f / d) + eps);
+    if (!real) continue;
+    if (sub == 0) rstd_out[row] = rstd;
 #pragma unroll
-    for (int k = 0; k < K; ++k) n[row * d + lane + 64 * k] = (bf16)(v[k] * rstd * w[lane + 64 * k] + b[lane + 64 * k]);
+    for (int k = 0; k < K; ++k) {
+      f16x8 h;
+      bf16x8 b;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        h[e] = (f16)(v[8 * k + e] * rstd);
+        b[e] = (bf16)(v[8 * k + e] * rstd);
+      }
+      *reinterpret_cast<f16x8*>(xh + row * d + 8 * sub + 64 * k) = h;
+      *reinterpret_cast<bf16x8*>(xhb + row * d + 8 * sub + 64 * k) = b;
+    }
   }
 }
 
-// da, db and u of an element from a, b and du.
+// da', db' and u' of an element from a', b' and du; slow = -log2(e) 2^-ka, ia = 2^-ka.
 struct SwigluGrad {
   float da, db, u;
 };
-__device__ __forceinline__ SwigluGrad swiglu_grad(float a, float b, float du) {
-  const float s = sigmoidf_(a), sa = a * s;
-  return {du * b * (s + sa * (1.f - s)), du * sa, sa * b};
+__device__ __forceinline__ SwigluGrad swiglu_grad(float a, float b, float du, float slow, float ia) {
+  const float s = __builtin_amdgcn_rcpf(1.f + fast_exp2(a * slow)), sa = a * s;
+  const float slope = s * fmaf(a * (1.f - s), ia, 1.f);
+  return {du * b * slope, du * sa, sa * b};
 }
 
-// E [rows][3 H] = [da | db | u]. A workgroup: 64 rows x 64 hidden channels, a wave 32 x 32 of each of a, b and du
+// E [rows][3 H] = [da' | db' | u']. A workgroup: 64 rows x 64 hidden channels, a wave 32 x 32 of each of a, b and du
 // (D = weight rows x token rows: a lane holds a token and 16 channels). k in steps of 64, double-buffered by
 // LDS DMA. grid (ceil(rows / 64), H / 64); block 256.
-__global__ __launch_bounds__(256) void hidden_grad(const bf16* __restrict__ n, const bf16* __restrict__ dy,
-                                                   const bf16* __restrict__ ab, const bf16* __restrict__ st,
+__global__ __launch_bounds__(256) void hidden_grad(const f16* __restrict__ xh, const bf16* __restrict__ dy,
+                                                   const f16* __restrict__ aw, const bf16* __restrict__ st,
+                                                   const float* __restrict__ offset, const float* __restrict__ scale,
                                                    bf16* __restrict__ E, int64_t rows, int d, int H) {
-  __shared__ bf16 buf[2][5][64 * 64];  // n, dy, A, B, S^T
+  __shared__ __attribute__((aligned(16))) bf16 buf[2][5][64 * 64];  // xh, dy, Aw, Bw, S^T
   const int lane = threadIdx.x & 63, g = lane >> 5, li = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row0 = (int64_t)blockIdx.x * 64;
@@ -141,13 +237,20 @@ __global__ __launch_bounds__(256) void hidden_grad(const bf16* __restrict__ n, c
   const uint32_t lds = lds_addr(buf);
   auto fetch = [&](int c0, int which) __attribute__((always_inline)) {
     const uint32_t at = lds + which * 5 * 8192;
-    tile_dma(n, d, row0, rows - 1, c0, at, wave, lane);
+    tile_dma(xh, d, row0, rows - 1, c0, at, wave, lane);
     tile_dma(dy, d, row0, rows - 1, c0, at + 8192, wave, lane);
-    tile_dma(ab, d, h0, 2 * H - 1, c0, at + 2 * 8192, wave, lane);
-    tile_dma(ab, d, H + h0, 2 * H - 1, c0, at + 3 * 8192, wave, lane);
+    tile_dma(aw, d, h0, 2 * H - 1, c0, at + 2 * 8192, wave, lane);
+    tile_dma(aw, d, H + h0, 2 * H - 1, c0, at + 3 * 8192, wave, lane);
     tile_dma(st, d, h0, H - 1, c0, at + 4 * 8192, wave, lane);
   };
-  f32x16 a = zero16(), b = zero16(), du = zero16();
+  f32x16 a, b, du = zero16();
+  const int hw = h0 + 32 * (wave >> 1);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    a[r] = offset[hw + acc_row(r, g)];
+    b[r] = offset[H + hw + acc_row(r, g)];
+  }
+  const float ia = scale[0], slow = -kLog2e * ia;
   const int rt = 32 * (wave & 1) + li, rh = 32 * (wave >> 1) + li;
   fetch(0, 0);
   int which = 0;
@@ -161,10 +264,13 @@ __global__ __launch_bounds__(256) void hidden_grad(const bf16* __restrict__ n, c
     __syncthreads();
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
-      const bf16x8 nt = ld8(&buf[which][0][off64(rt, 2 * kk + g)]);
+      const auto half = [&](int k, int r) __attribute__((always_inline)) {
+        return ld8h(reinterpret_cast<const f16*>(&buf[which][k][off64(r, 2 * kk + g)]));
+      };
+      const f16x8 nt = half(0, rt);
       const bf16x8 dt = ld8(&buf[which][1][off64(rt, 2 * kk + g)]);
-      a = mfma32(ld8(&buf[which][2][off64(rh, 2 * kk + g)]), nt, a);
-      b = mfma32(ld8(&buf[which][3][off64(rh, 2 * kk + g)]), nt, b);
+      a = mfma32h(half(2, rh), nt, a);
+      b = mfma32h(half(3, rh), nt, b);
       du = mfma32(ld8(&buf[which][4][off64(rh, 2 * kk + g)]), dt, du);
     }
     __syncthreads();
@@ -172,7 +278,7 @@ __global__ __launch_bounds__(256) void hidden_grad(const bf16* __restrict__ n, c
   f32x16 u;
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    const SwigluGrad e = swiglu_grad(a[r], b[r], du[r]);
+    const SwigluGrad e = swiglu_grad(a[r], b[r], du[r], slow, ia);
     a[r] = e.da;
     b[r] = e.db;
     u[r] = e.u;
@@ -202,11 +308,12 @@ __global__ __launch_bounds__(256) void hidden_grad(const bf16* __restrict__ n, c
 //   TURN false: C[m][n] = sum over k of A[m][k] B[n][k]    (m clamped to m_rows, n in range)
 //   TURN true:  C[m][n] = sum over k of A[k][m] B[k][n]    (k rows past k_rows count as zero)
 // Split s of the k axis: k from s * k_share, to C + s * split_stride; add: C is added to. B2 takes the place
-// of B from m tile m_two on. grid (m tiles, n tiles, splits); block 256.
+// of B from m tile m_two on. TURN: sums[s][m] = sum over k of A[k][m] for the m tiles before m_two (by a product
+// with ones, in the workgroups of the first n tile). grid (m tiles, n tiles, splits); block 256.
 struct Gemm64Args {
   const bf16 *A, *B, *B2;
-  float* C;
-  int64_t lda, ldb, m_rows, k_rows, k_share, split_stride;
+  float *C, *sums;
+  int64_t lda, ldb, m_rows, k_rows, k_share, split_stride, sums_stride;
   int ldc, m_two, add;
 };
 template <bool TURN>
@@ -233,7 +340,12 @@ __global__ __launch_bounds__(256) void gemm64(const Gemm64Args p) {
       tile_dma(B + k, p.ldb, n0, n0 + 63, 0, at + 8192, wave, lane);
     }
   };
-  f32x16 acc[2][2];
+  const bool summed = TURN && blockIdx.y == 0 && (int)blockIdx.x < p.m_two;
+  f32x16 acc[2][2], total[2];
+  total[0] = total[1] = zero16();
+  bf16x8 ones;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ones[e] = (bf16)1.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] = zero16();
 #pragma unroll
@@ -279,6 +391,10 @@ __global__ __launch_bounds__(256) void gemm64(const Gemm64Args p) {
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] = mfma32(fa[i >> 1], fb[i & 1], acc[i >> 1][i & 1]);
+    if (TURN && summed) {
+      total[0] = mfma32(fa[0], ones, total[0]);
+      total[1] = mfma32(fa[1], ones, total[1]);
+    }
   }
   __syncthreads();
   // the waves' sums: [wave][tile][register][lane] fp32 in the buffers' place (64 KB)
@@ -301,137 +417,152 @@ __global__ __launch_bounds__(256) void gemm64(const Gemm64Args p) {
       *to = p.add ? *to + v : v;
     }
   }
+  if (TURN && summed) {
+    __syncthreads();
+    // (every column of a total is the same: lane 0 of each half)
+    if (li == 0) {
+#pragma unroll
+      for (int r = 0; r < 32; ++r) red[wave * 64 + 32 * (r >> 4) + acc_row(r & 15, g)] = total[r >> 4][r & 15];
+    }
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      float* to = p.sums + blockIdx.z * p.sums_stride + m0 + threadIdx.x;
+      const float v = (red[threadIdx.x] + red[64 + threadIdx.x]) + (red[128 + threadIdx.x] + red[192 + threadIdx.x]);
+      *to = p.add ? *to + v : v;
+    }
+  }
 }
 static_assert(4 * 2 * 64 * 64 * sizeof(bf16) >= 4 * 4 * 16 * 64 * sizeof(float), "the waves' sums fit the buffers");
 
-// dx = (residual ? dy : 0) + LN'(dn) of the rows, dn the sum of `splits` fp32 parts, and this workgroup's sums
-// of dn xh and dn (part [gridDim.x][2][d], added to where add). One wave a row, K = d / 64; block 256.
-template <bool CODES, int K>
-__global__ __launch_bounds__(256) void norm_grad_rows(const void* x, const uint8_t* scales, const bf16* __restrict__ dy,
-                                                      const float* __restrict__ dn, int splits, int64_t split_stride,
-                                                      const float* __restrict__ w, bf16* __restrict__ dx,
-                                                      float* __restrict__ part, int64_t rows, int residual, int add,
-                                                      float eps) {
-  constexpr int d = 64 * K, blocks = d / kActBlock;
-  __shared__ float red[2][4][d];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  float sw[K], sb[K], wv[K];
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    sw[k] = sb[k] = 0.f;
-    wv[k] = w[lane + 64 * k];
-  }
-  for (int64_t row = (int64_t)blockIdx.x * 4 + wave; row < rows; row += (int64_t)gridDim.x * 4) {
-    float v[K], t[K];
-    float s = 0.f, sg = 0.f;
+// dx = (residual ? dy : 0) + rstd (g - mean(g) - xh mean(g xh)), g the sum of `splits` fp32 parts [rows][d]: 8 lanes
+// a row, K = d / 64 pieces of 8 channels each. grid-strided; block 256 (32 rows).
+template <int K>
+__global__ __launch_bounds__(256) void norm_grad_rows(const f16* __restrict__ xh, const float* __restrict__ rstd_in,
+                                                      const bf16* __restrict__ dy, const float* __restrict__ dxh,
+                                                      int splits, int64_t split_stride, bf16* __restrict__ dx,
+                                                      int64_t rows, int residual) {
+  constexpr int d = 64 * K;
+  const int sub = threadIdx.x & 7;
+  for (int64_t row = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3); row - (threadIdx.x >> 3) < rows;
+       row += (int64_t)gridDim.x * 32) {
+    const bool real = row < rows;
+    const int64_t at = (real ? row : rows - 1) * d + 8 * sub;
+    float t[8 * K], h[8 * K];
+    float sg = 0.f, sx = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = lane + 64 * k;
-      KeptPiece<bf16, CODES, 1> p;
-      p.load(x, scales, row, c, d, blocks);
-      p.values(&v[k]);
-      t[k] = 0.f;
-      for (int i = 0; i < splits; ++i) t[k] += dn[i * split_stride + row * d + c];
-      s += v[k];
-      sg += t[k] * wv[k];
+      const f16x8 hv = ld8h(xh + at + 64 * k);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        h[8 * k + e] = (float)hv[e];
+        t[8 * k + e] = 0.f;
+      }
+      for (int i = 0; i < splits; ++i) {
+        const float* q = dxh + i * split_stride + at + 64 * k;
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(q), hi = *reinterpret_cast<const f32x4*>(q + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          t[8 * k + e] += lo[e];
+          t[8 * k + 4 + e] += hi[e];
+        }
+      }
+#pragma unroll
+      for (int e = 8 * k; e < 8 * k + 8; ++e) {
+        sg += t[e];
+        sx += t[e] * h[e];
+      }
     }
-    const float mean = lanes_sum<64>(s) * (1.f / d), c1 = lanes_sum<64>(sg) * (1.f / d);
-    float q = 0.f, sx = 0.f;
+    const float c1 = lanes_sum<8>(sg) * (1.f / d), c2 = lanes_sum<8>(sx) * (1.f / d);
+    if (!real) continue;
+    const float rstd = rstd_in[row];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      v[k] -= mean;
-      q += v[k] * v[k];
-      sx += (t[k] * wv[k] - c1) * v[k];
-    }
-    const float rstd = __builtin_amdgcn_rsqf(lanes_sum<64>(q) * (1.f / d) + eps);
-    const float c2 = lanes_sum<64>(sx) * (1.f / d) * rstd * rstd;
+      const bf16x8 y = ld8(dy + at + 64 * k);
+      bf16x8 o;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int64_t at = row * d + lane + 64 * k;
-      sw[k] += t[k] * (v[k] * rstd);
-      sb[k] += t[k];
-      dx[at] = (bf16)((residual ? (float)dy[at] : 0.f) + rstd * (t[k] * wv[k] - c1 - v[k] * c2));
+      for (int e = 0; e < 8; ++e)
+        o[e] = (bf16)((residual ? (float)y[e] : 0.f) + rstd * (t[8 * k + e] - c1 - h[8 * k + e] * c2));
+      *reinterpret_cast<bf16x8*>(dx + at + 64 * k) = o;
     }
-  }
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    red[0][wave][lane + 64 * k] = sw[k];
-    red[1][wave][lane + 64 * k] = sb[k];
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < 2 * d; i += 256) {
-    const float* r = &red[0][0][0] + (i / d) * 4 * d + i % d;
-    float* to = part + (int64_t)blockIdx.x * 2 * d + i;
-    const float v = (r[0] + r[d]) + (r[2 * d] + r[3 * d]);
-    *to = add ? *to + v : v;
   }
 }
 
-// The weights' gradients from `count` parts [3 H][d] (dA, dB, dS^T): dA and dB in order, dS turned. A 32 x 32
-// tile a workgroup: grid (d / 32, 3 H / 32); block 256.
-__global__ __launch_bounds__(256) void join_weight_grads(const float* __restrict__ part, int count, int d, int H,
-                                                         void* da, void* db, void* ds, int dtype) {
-  __shared__ float tile[32][33];
+// The weights' gradients from `count` parts G [3 H][d] (da'^T xh, db'^T xh, u'^T dy) and sums [2 H] (of da', db'), and
+// the rows' shares of the affine's: part [2 H / 32][2][d]. A 32 x 32 tile a workgroup: grid (d / 32, 3 H / 32);
+// block 1024.
+__global__ __launch_bounds__(1024) void join_weight_grads(const float* __restrict__ G, const float* __restrict__ sums,
+                                                          int count, const float* __restrict__ wa,
+                                                          const float* __restrict__ wb, const float* __restrict__ w,
+                                                          const float* __restrict__ v, const float* __restrict__ scale,
+                                                          float* __restrict__ part, int d, int H, void* da, void* db,
+                                                          void* ds, int dtype) {
+  __shared__ float tile[32][33], tile2[32][33];
   const int c0 = blockIdx.x * 32, h0 = blockIdx.y * 32;
   const int col = threadIdx.x & 31, row = threadIdx.x >> 5;
   const int64_t size = (int64_t)3 * H * d;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = row + 8 * i;
-    const float* p = part + (int64_t)(h0 + r) * d + c0 + col;
-    float v = 0.f;
-    for (int k = 0; k < count; ++k) v += p[k * size];
-    if (h0 < 2 * H) {
-      void* to = h0 < H ? da : db;
-      const int64_t at = (int64_t)(h0 + r - (h0 < H ? 0 : H)) * d + c0 + col;
-      if (dtype == 0)
-        static_cast<bf16*>(to)[at] = (bf16)v;
-      else
-        static_cast<float*>(to)[at] = v;
-    } else {
-      tile[r][col] = v;
-    }
-  }
-  if (h0 < 2 * H) return;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = row + 8 * i;
-    const int64_t at = (int64_t)(c0 + r) * H + h0 - 2 * H + col;
+  const auto put = [&](void* to, int64_t at, float t) __attribute__((always_inline)) {
     if (dtype == 0)
-      static_cast<bf16*>(ds)[at] = (bf16)tile[col][r];
+      static_cast<bf16*>(to)[at] = (bf16)t;
     else
-      static_cast<float*>(ds)[at] = tile[col][r];
+      static_cast<float*>(to)[at] = t;
+  };
+  const float* p = G + (int64_t)(h0 + row) * d + c0 + col;
+  float t = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < count; ++k) t += p[k * size];
+  if (h0 >= 2 * H) {
+    tile[row][col] = count ? t * (scale[0] * scale[1]) : 0.f;
+    __syncthreads();
+    put(ds, (int64_t)(c0 + row) * H + h0 - 2 * H + col, tile[col][row]);
+    return;
+  }
+  // (32 hidden channels' sums: every thread of a row adds the same ones)
+  float total = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < count; ++k) total += sums[(int64_t)k * 2 * H + h0 + row];
+  const bool first = h0 < H;
+  const float back = count ? scale[first ? 1 : 0] : 0.f;
+  t *= back;
+  total *= back;
+  const int64_t at = (int64_t)(h0 + row - (first ? 0 : H)) * d + c0 + col;
+  put(first ? da : db, at, t * w[c0 + col] + total * v[c0 + col]);
+  const float own = (first ? wa : wb)[at];
+  tile[row][col] = own * t;
+  tile2[row][col] = own * total;
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const float(*from)[33] = threadIdx.x < 32 ? tile : tile2;
+    float r = 0.f;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) r += from[k][col];
+    part[((int64_t)blockIdx.y * 2 + (threadIdx.x >> 5)) * d + c0 + col] = r;
   }
 }
 
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
 template <bool CODES>
-void run_norm_rows(const void* x, const uint8_t* scales, const float* w, const float* b, bf16* n, int64_t rows, int d,
-                   float eps, hipStream_t st) {
-  const dim3 grid((unsigned)std::min<int64_t>((rows + 3) / 4, (int64_t)cu_count() * 8));
-  switch (d / 64) {
-#define FFK_K(K_) case K_: norm_rows<CODES, K_><<<grid, 256, 0, st>>>(x, scales, w, b, n, rows, eps); break;
+void run_norm_rows(const TransitionGradArgs& a, const void* x, const uint8_t* scales, int64_t rows, hipStream_t st) {
+  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(rows, 32), (int64_t)cu_count() * 16));
+  switch (a.d / 64) {
+#define FFK_K(K_) case K_: norm_rows<CODES, K_><<<grid, 256, 0, st>>>(x, scales, a.xh, a.xhb, a.rstd, rows, a.eps); break;
     FFK_K(1) FFK_K(2) FFK_K(3) FFK_K(4) FFK_K(5) FFK_K(6) FFK_K(7) FFK_K(8) FFK_K(9) FFK_K(10) FFK_K(11) FFK_K(12)
 #undef FFK_K
   }
 }
 
-template <bool CODES>
-void run_norm_grad_rows(const void* x, const uint8_t* scales, const bf16* dy, const float* dn, int splits,
-                        int64_t split_stride, const float* w, bf16* dx, float* part, int blocks, int64_t rows, int d,
-                        int residual, int add, float eps, hipStream_t st) {
-  switch (d / 64) {
+void run_norm_grad_rows(const TransitionGradArgs& a, const bf16* dy, int splits, int64_t split_stride, bf16* dx,
+                        int64_t rows, hipStream_t st) {
+  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(rows, 32), (int64_t)cu_count() * 16));
+  switch (a.d / 64) {
 #define FFK_K(K_)                                                                                                 \
   case K_:                                                                                                        \
-    norm_grad_rows<CODES, K_><<<blocks, 256, 0, st>>>(x, scales, dy, dn, splits, split_stride, w, dx, part, rows, \
-                                                      residual, add, eps);                                        \
+    norm_grad_rows<K_><<<grid, 256, 0, st>>>(a.xh, a.rstd, dy, a.dxh, splits, split_stride, dx, rows, a.residual); \
     break;
     FFK_K(1) FFK_K(2) FFK_K(3) FFK_K(4) FFK_K(5) FFK_K(6) FFK_K(7) FFK_K(8) FFK_K(9) FFK_K(10) FFK_K(11) FFK_K(12)
 #undef FFK_K
   }
 }
-
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 }  // namespace
 
@@ -442,27 +573,31 @@ TransitionGradPlan transition_grad_plan(int64_t rows, int d, int H) {
   p.chunk = std::min<int64_t>(ceil_div(rows, 64) * 64, fit);
   const int64_t cus = cu_count();
   // both products want a workgroup a CU at least, and four steps of 64 in each
-  p.dn_splits = (int)std::max<int64_t>(1, std::min<int64_t>(cus / std::max<int64_t>(1, p.chunk / 64 * (d / 64)), 2 * H / 256));
+  p.dxh_splits = (int)std::max<int64_t>(1, std::min<int64_t>(cus / std::max<int64_t>(1, p.chunk / 64 * (d / 64)), 2 * H / 256));
   p.dw_splits = (int)std::max<int64_t>(1, std::min<int64_t>(2 * cus / std::max<int64_t>(1, 3 * H / 64 * (d / 64)), p.chunk / 256));
-  p.norm_blocks = (int)std::min<int64_t>(ceil_div(std::min(rows, p.chunk), 4), cus * 4);
+  p.peaks = 2 * kPeakBlocks;
   return p;
 }
 
 void launch_transition_grad(const TransitionGradArgs& a, const TransitionGradPlan& p, hipStream_t st) {
   const int d = a.d, H = a.hidden;
-  pack_grad_weights<<<dim3(H / 32, d / 32, 3), 256, 0, st>>>(a.wa, a.wb, a.ws, a.ab, a.st, a.abt, d, H);
+  if (a.rows > 0) {
+    weight_peaks<<<dim3(kPeakBlocks, 2), 256, 0, st>>>(a.wa, a.wb, a.ln_w, a.peaks, d, H);
+    pack_grad_weights<<<dim3(H / 32, 3), 256, 0, st>>>(a.wa, a.wb, a.ws, a.ln_w, a.ln_b, a.peaks, a.aw, a.st, a.abt,
+                                                       a.offset, a.scale, d, H, 0);
+  }
   const char* x = static_cast<const char*>(a.x);
   for (int64_t r0 = 0; r0 < a.rows; r0 += p.chunk) {
     const int64_t rows = std::min(p.chunk, a.rows - r0);
     const void* xc = x + r0 * d * (a.scales ? 1 : 2);
-    const uint8_t* sc = a.scales ? a.scales + r0 * (d / kActBlock) : nullptr;
     const bf16* dy = a.dy + r0 * d;
     const int add = r0 > 0;
-    if (sc)
-      run_norm_rows<true>(xc, sc, a.ln_w, a.ln_b, a.n, rows, d, a.eps, st);
+    if (a.scales)
+      run_norm_rows<true>(a, xc, a.scales + r0 * (d / kActBlock), rows, st);
     else
-      run_norm_rows<false>(xc, sc, a.ln_w, a.ln_b, a.n, rows, d, a.eps, st);
-    hidden_grad<<<dim3((unsigned)ceil_div(rows, 64), H / 64), 256, 0, st>>>(a.n, dy, a.ab, a.st, a.E, rows, d, H);
+      run_norm_rows<false>(a, xc, nullptr, rows, st);
+    hidden_grad<<<dim3((unsigned)ceil_div(rows, 64), H / 64), 256, 0, st>>>(a.xh, dy, a.aw, a.st, a.offset, a.scale, a.E,
+                                                                            rows, d, H);
     Gemm64Args g{};
     g.A = a.E;
     g.lda = 3 * H;
@@ -470,23 +605,18 @@ void launch_transition_grad(const TransitionGradArgs& a, const TransitionGradPla
     g.B = g.B2 = a.abt;
     g.ldb = 2 * H;
     g.k_rows = 2 * H;
-    g.k_share = ceil_div(ceil_div(2 * H, p.dn_splits), 64) * 64;
-    g.C = a.dn;
+    g.k_share = ceil_div(ceil_div(2 * H, p.dxh_splits), 64) * 64;
+    g.C = a.dxh;
     g.ldc = d;
     g.split_stride = p.chunk * d;
     g.m_two = 0x7fffffff;
-    gemm64<false><<<dim3((unsigned)ceil_div(rows, 64), d / 64, p.dn_splits), 256, 0, st>>>(g);
-    if (sc)
-      run_norm_grad_rows<true>(xc, sc, dy, a.dn, p.dn_splits, g.split_stride, a.ln_w, a.dx + r0 * d, a.norm_part,
-                               p.norm_blocks, rows, d, a.residual, add, a.eps, st);
-    else
-      run_norm_grad_rows<false>(xc, sc, dy, a.dn, p.dn_splits, g.split_stride, a.ln_w, a.dx + r0 * d, a.norm_part,
-                                p.norm_blocks, rows, d, a.residual, add, a.eps, st);
+    gemm64<false><<<dim3((unsigned)ceil_div(rows, 64), d / 64, p.dxh_splits), 256, 0, st>>>(g);
+    run_norm_grad_rows(a, dy, p.dxh_splits, g.split_stride, a.dx + r0 * d, rows, st);
     Gemm64Args t{};
     t.A = a.E;
     t.lda = 3 * H;
     t.m_rows = 3 * H;
-    t.B = a.n;
+    t.B = a.xhb;
     t.B2 = dy;
     t.m_two = 2 * H / 64;
     t.ldb = d;
@@ -495,13 +625,16 @@ void launch_transition_grad(const TransitionGradArgs& a, const TransitionGradPla
     t.C = a.dw_part;
     t.ldc = d;
     t.split_stride = (int64_t)3 * H * d;
+    t.sums = a.sums;
+    t.sums_stride = 2 * H;
     t.add = add;
     gemm64<true><<<dim3(3 * H / 64, d / 64, p.dw_splits), 256, 0, st>>>(t);
   }
   // (no rows: sums over nothing)
-  launch_sum_partials(a.norm_part, a.rows > 0 ? p.norm_blocks : 0, 2 * d, d, a.dln_w, a.dln_b, a.grad_dtype, st);
-  join_weight_grads<<<dim3(d / 32, 3 * H / 32), 256, 0, st>>>(a.dw_part, a.rows > 0 ? p.dw_splits : 0, d, H, a.dwa, a.dwb, a.dws,
-                                                              a.grad_dtype);
+  join_weight_grads<<<dim3(d / 32, 3 * H / 32), 1024, 0, st>>>(a.dw_part, a.sums, a.rows > 0 ? p.dw_splits : 0, a.wa,
+                                                               a.wb, a.ln_w, a.ln_b, a.scale, a.norm_part, d, H, a.dwa,
+                                                               a.dwb, a.dws, a.grad_dtype);
+  launch_sum_partials(a.norm_part, a.rows > 0 ? 2 * H / 32 : 0, 2 * d, d, a.dln_w, a.dln_b, a.grad_dtype, st);
 }
 
 }  // namespace ffk

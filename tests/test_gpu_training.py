@@ -3,12 +3,12 @@
 Tolerances. An 8-bit activation is compared exactly. LayerNorm's gradients are fp32 computations: each of
 the operations between the inputs and an output is off by at most 2^-24 of its result, and
 ``_norm_bounds`` multiplies the magnitudes of those results by the count of the operations; a bf16 output
-adds half a step, 2^-8 of the value. The transition's products take bf16 operands: a rounded operand is off
-by r = 2^-8 / sqrt(3) of itself in root mean square at most, up to 8 roundings lie on the way to a gradient (n,
-the two uses of the weights, dy S's weight, a's and b's gradients, the output), they add in quadrature, and
-the logistic function's slope carries those of a on at no more than their size: r sqrt(8) = 6.4e-3 of the
-result's norm, held to 1e-2 as every op of the stack. A single value is held to 6 of its own standard
-deviations, which ``_deviations`` follows through the formulas.
+adds half a step, 2^-8 of the value. The transition's products take rounded operands: one rounded to bf16 is off by
+r = 2^-8 / sqrt(3) of itself in root mean square at most, to fp16 by r / 8. On the way to a gradient lie the
+rounding of S under dy, of a hidden gradient or u, of xh or a weight beside it, and of the result, in bf16, and
+an eighth of two more in a and b; they add in quadrature: r sqrt(4 + 2 / 64) = 4.6e-3 of the result's norm at most
+(2 r for an ordinary r of 1.7e-3: 3.3e-3), held to 1e-2 as every op of the stack. A single value is held to 6 of
+its own standard deviations, which ``_deviations`` follows through the formulas.
 """
 
 from __future__ import annotations
@@ -247,21 +247,24 @@ def _transition_case(rows, d, factor, seed):
 
 
 def _deviations(dy, x, p, eps):
-    """The standard deviation of each gradient's values under the roundings of the operands, r of each at most.
-    (A value of a product's sum over channels: the terms' deviations in quadrature, since every term has
-    roundings of its own. A sum over rows: the magnitudes added, since a weight's rounding is the same in every
-    row. A function of a and b: its derivatives' magnitudes times theirs.)"""
+    """The standard deviation of each gradient's values under the roundings of the operands (bf16: r of each at
+    most; fp16, under a and b: r / 8). (A value of a product's sum over channels: the terms' deviations in
+    quadrature, since every term has roundings of its own. A sum over rows: the magnitudes added, since a weight's
+    rounding is the same in every row, and one of xh the same for every hidden channel. A function of a and b: its
+    derivatives' magnitudes times theirs. The rows' operand is xh, and the norm's affine comes after it: where
+    xh w and the offset cancel in n, the error is that of xh w.)"""
     r = 2.0**-8 / 3**0.5
     dy, x = dy.double(), x.double()
-    w, wa, wb, wo = (p[k].double() for k in ("ln_weight", "expand_a", "expand_b", "squeeze"))
+    w, v, wa, wb, wo = (p[k].double() for k in ("ln_weight", "ln_bias", "expand_a", "expand_b", "squeeze"))
     xh, rstd = oracle.normalised(x, eps)
-    n = xh * w + p["ln_bias"].double()
+    scaled = xh * w
+    n = scaled + v
 
     def quad(u, v):  # sqrt(sum over k of (u v)^2)
         return ((u * u) @ (v * v)).sqrt()
 
     a, b, du = n @ wa.T, n @ wb.T, dy @ wo
-    sa, sb, sdu = 2**0.5 * r * quad(n, wa.T), 2**0.5 * r * quad(n, wb.T), r * quad(dy, wo)
+    sa, sb, sdu = 2**0.5 * r / 8 * quad(scaled, wa.T), 2**0.5 * r / 8 * quad(scaled, wb.T), r * quad(dy, wo)
     s = torch.sigmoid(a)
     silu, slope = a * s, s * (1 + a * (1 - s))
     bend = s * (1 - s) * (2 + a * (1 - 2 * s))  # slope's derivative
@@ -269,12 +272,13 @@ def _deviations(dy, x, p, eps):
     su = (b * slope).abs() * sa + silu.abs() * sb + r * u.abs()
     sdb = silu.abs() * sdu + (du * slope).abs() * sa + r * db.abs()
     sda = (b * slope).abs() * sdu + (du * slope).abs() * sb + (du * b * bend).abs() * sa + r * da.abs()
+    dn = da @ wa + db @ wb
     sdn = (quad(sda, wa) ** 2 + quad(sdb, wb) ** 2 + r * r * (quad(da, wa) ** 2 + quad(db, wb) ** 2)).sqrt()
     g = sdn * w.abs()
     dx = rstd * (g + g.mean(-1, keepdim=True) + xh.abs() * (g * xh.abs()).mean(-1, keepdim=True))
-    return dict(x=dx, ln_weight=(sdn * xh.abs()).sum(0), ln_bias=sdn.sum(0),
-                expand_a=sda.T @ n.abs() + r * da.abs().T @ n.abs(), expand_b=sdb.T @ n.abs() + r * db.abs().T @ n.abs(),
-                squeeze=dy.abs().T @ su)
+    return dict(x=dx, ln_weight=(sdn * xh.abs() + r * (dn * xh).abs()).sum(0), ln_bias=sdn.sum(0),
+                expand_a=sda.T @ n.abs() + r * da.abs().T @ scaled.abs(),
+                expand_b=sdb.T @ n.abs() + r * db.abs().T @ scaled.abs(), squeeze=dy.abs().T @ su)
 
 
 def _near(got, want, deviation, name, dtype, norm):
@@ -330,7 +334,7 @@ def test_transition_backward_no_rows():
 
 def test_transition_backward_large_gates():
     """Gates far to both sides: the logistic function at 0 and 1, no NaN. Values of a of about 60 are off by
-    60 * 2^(1/2) * 2^-8 / 3^(1/2) = 0.19 where the slope goes from 0 to 1 within a few units, so the norms' bound,
+    60 * 2^(1/2) * 2^-8 / 3^(1/2) / 8 = 0.024 where the slope goes from 0 to 1 within a few units, so the norms' bound,
     which is for gates of order one, says nothing here; each value's own deviations (bend times that of a) do."""
     x, dy, params = _transition_case(96, 128, 4, 1)
     params["expand_a"] *= 60
