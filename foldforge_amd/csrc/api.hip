@@ -288,7 +288,10 @@ TransitionGradArgs transition_grad_ws(void* ws, size_t* bytes, const TransitionG
   a.xh = cv.take<f16>((size_t)p.chunk * d);
   a.xhb = cv.take<bf16>((size_t)p.chunk * d);
   a.rstd = cv.take<float>((size_t)p.chunk);
-  a.E = cv.take<bf16>((size_t)p.chunk * 3 * hidden);
+  if (p.fused)
+    a.split = cv.take<bf16>((size_t)16 * hidden);
+  else
+    a.E = cv.take<bf16>((size_t)p.chunk * 3 * hidden);
   a.dxh = cv.take<float>((size_t)p.dxh_splits * p.chunk * d);
   a.dw_part = cv.take<float>((size_t)p.dw_splits * 3 * w);
   a.sums = cv.take<float>((size_t)p.dw_splits * 2 * hidden);

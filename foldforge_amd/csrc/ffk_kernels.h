@@ -416,6 +416,7 @@ void launch_sum_partials(const float* part, int count, int width, int split, voi
 struct TransitionGradPlan {
   int64_t chunk;  // rows at once, a multiple of 64
   int dxh_splits, dw_splits, peaks;
+  int fused;      // the hidden rows stay in registers (no E, no dxh)
 };
 TransitionGradPlan transition_grad_plan(int64_t rows, int d, int hidden);
 struct TransitionGradArgs {
@@ -432,6 +433,7 @@ struct TransitionGradArgs {
   float *peaks, *scale, *offset;        // [peaks], [2], [2 hidden]
   f16* aw;                              // [2 hidden][d]
   bf16 *st, *abt;                       // [hidden][d], [d][2 hidden]
+  bf16* split;                          // [2][hidden][8] (fused)
   // a chunk's normalised rows, hidden gradients and the products' parts
   f16* xh;                              // [chunk][d]
   bf16 *xhb, *E;                        // [chunk][d], [chunk][3 hidden]

@@ -434,6 +434,360 @@ __global__ __launch_bounds__(256) void gemm64(const Gemm64Args p) {
 }
 static_assert(4 * 2 * 64 * 64 * sizeof(bf16) >= 4 * 4 * 16 * 64 * sizeof(float), "the waves' sums fit the buffers");
 
+// ---------------------------------------------------------------------------------------------------------
+// The fused form (d = 64 or 128): two kernels, the hidden rows stay in registers.
+
+// A row of D values of 2 bytes in LDS, D / 8 pieces of 16 bytes: piece p of row r lies at piece p ^ swz(r), the low
+// bits of r in reverse order. Sixteen lanes reading one piece of sixteen rows, and eight rows' 64-byte parts (a
+// transposing fetch), spread over the banks evenly.
+template <int D>
+__device__ __forceinline__ int swz(int r) {
+  if constexpr (D == 64) return swz64(r);
+  return (r & 1) << 3 | (r & 2) << 1 | (r & 4) >> 1 | (r & 8) >> 3;
+}
+template <int D>
+__device__ __forceinline__ int off_row(int r, int p) { return r * D + 8 * (p ^ swz<D>(r)); }
+
+// 1 KB (512 / D rows) of a row-major array into LDS at dst, swizzled; r0: the KB's first row in the LDS tile, a
+// multiple of 512 / D (rows row0 + .. of src, clamped to last).
+template <int D>
+__device__ __forceinline__ void rows_kb(const void* src, int64_t row0, int r0, int64_t last, uint32_t dst, int lane) {
+  constexpr int P = D / 8;  // pieces of a row
+  const int r = r0 + lane / P;
+  const int64_t row = row0 + r < last ? row0 + r : last;
+  dma16_at(static_cast<const bf16*>(src) + row * D + 8 * ((lane % P) ^ swz<D>(r)), dst + 1024u * (r0 * D / 512));
+}
+
+// MFMA operand of a tile of D-channel rows that are k, as ld_turned.
+template <int D>
+__device__ __forceinline__ bf16x8 ld_turned_row(const bf16* tile, int c0, int k0, int lane) {
+  const int j = lane & 15, q = lane >> 4;
+  const int r = k0 + 4 * (q >> 1) + (j >> 2), c = c0 + 16 * (q & 1) + 4 * (j & 3);
+  union {
+    s16x4 s[2];
+    bf16x8 v;
+  } o;
+  o.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(&tile[off_row<D>(r, c >> 3) + (c & 7)]));
+  o.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(&tile[off_row<D>(r + 8, c >> 3) + (c & 7)]));
+  return o.v;
+}
+
+// The weights' gradients G = [da'^T xh; db'^T xh; u'^T dy] and the sums of da', db'.
+//
+// A wave owns 32 hidden channels: its operands of Aw, Bw and S^T (D k of 32 channels each) and its sums (3 x 32 x D
+// fp32) stay in registers while the rows stream by; a workgroup's four waves share the rows in LDS. Per 32 rows:
+// a', b', du as D = rows x hidden (a lane holds a hidden channel at 16 rows), their elementwise part in place, and the
+// rounded results are directly the operand [hidden x rows] of the gradients' products, whose other operand (channels
+// x rows) comes out of the same rows by transposing LDS reads, in the same order of k. No hidden value leaves the
+// registers, nothing is turned through LDS. D = 128: 288 registers of operands and sums, one wave per SIMD.
+// grid (ceil(H / 128), splits): split s takes the stages s, s + splits, .. of 64 rows. block 256.
+constexpr int kStageRows = 64;
+template <int D>
+constexpr int kWeightBuffers = D == 128 ? 3 : 2;
+template <int D>
+__global__ __launch_bounds__(256, D == 128 ? 1 : 2) void transition_grad_weights(
+    const f16* __restrict__ xh, const bf16* __restrict__ xhb, const bf16* __restrict__ dy, const f16* __restrict__ aw,
+    const bf16* __restrict__ st, const float* __restrict__ offset, const float* __restrict__ scale,
+    float* __restrict__ G, float* __restrict__ sums, int64_t rows, int H, int add) {
+  constexpr int NB = kWeightBuffers<D>, KK = D / 16, CT = D / 32;
+  constexpr int kTile = kStageRows * D;              // elements of a tile
+  constexpr int kLoads = 3 * (kTile / 512) / 4;      // transfers of a wave a stage
+  __shared__ __attribute__((aligned(16))) bf16 buf[NB][3][kTile];  // xh fp16, xh bf16, dy
+  const int lane = threadIdx.x & 63, g = lane >> 5, li = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h0 = blockIdx.x * 128 + 32 * wave;
+  const bool own = h0 < H;  // H a multiple of 64: the last workgroup's upper waves may own nothing
+  const int hr = own ? h0 + li : li;
+  const uint32_t lds = lds_addr(buf);
+  const int64_t stages = (rows + kStageRows - 1) / kStageRows;
+  auto fetch = [&](int64_t stage, int b) __attribute__((always_inline)) {
+    const int64_t row0 = stage * kStageRows;
+#pragma unroll
+    for (int t = 0; t < 3; ++t) {
+      const void* src = t == 0 ? (const void*)xh : t == 1 ? (const void*)xhb : (const void*)dy;
+#pragma unroll
+      for (int u = 0; u < kLoads / 3; ++u)
+        rows_kb<D>(src, row0, (kLoads / 3 * wave + u) * (512 / D), rows - 1,
+                   lds + (uint32_t)((b * 3 + t) * kTile * sizeof(bf16)), lane);
+    }
+  };
+  f16x8 wa[KK], wb[KK];
+  bf16x8 ws[KK];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) {
+    wa[kk] = ld8h(aw + (int64_t)hr * D + 16 * kk + 8 * g);
+    wb[kk] = ld8h(aw + (int64_t)(H + hr) * D + 16 * kk + 8 * g);
+    ws[kk] = ld8(st + (int64_t)hr * D + 16 * kk + 8 * g);
+  }
+  const float oa = offset[hr], ob = offset[H + hr], ia = scale[0], slow = -kLog2e * ia;
+  // the parameters have landed: without this the compiler waits for them again in every stage
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) asm volatile("" ::"v"(wa[kk]), "v"(wb[kk]), "v"(ws[kk]));
+  asm volatile("" ::"v"(oa), "v"(ob), "v"(slow));
+  f32x16 ga[CT], gb[CT], gs[CT];
+#pragma unroll
+  for (int c = 0; c < CT; ++c) ga[c] = gb[c] = gs[c] = zero16();
+  float ta = 0.f, tb = 0.f;
+#pragma unroll
+  for (int b = 0; b < NB - 1; ++b) {
+    const int64_t stage = blockIdx.y + (int64_t)b * gridDim.y;
+    fetch(stage < stages ? stage : stages - 1, b);
+  }
+  int b = 0;
+#pragma unroll 1
+  for (int64_t stage = blockIdx.y; stage < stages; stage += gridDim.y) {
+    wait_vm_lds<(NB - 2) * kLoads>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    {  // (past the end: the last rows again, which nothing reads)
+      const int64_t ahead = stage + (int64_t)(NB - 1) * gridDim.y;
+      fetch(ahead < stages ? ahead : stages - 1, b == 0 ? NB - 1 : b - 1);
+    }
+    const f16* th = reinterpret_cast<const f16*>(buf[b][0]);
+    const bf16* tb16 = buf[b][1];
+    bf16* td = buf[b][2];
+    const int64_t left = rows - stage * kStageRows;
+    if (left < kStageRows) {  // rows past the end: dy = 0 makes their gradients 0
+      for (int i = threadIdx.x; i < kTile / 8; i += 256)
+        if (i / (D / 8) >= left) {
+          bf16x8 z;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) z[e] = (bf16)0.f;
+          *reinterpret_cast<bf16x8*>(td + 8 * i) = z;
+        }
+      __syncthreads();
+    }
+#pragma unroll 1
+    for (int r0 = 0; r0 < kStageRows; r0 += 32) {
+      f32x16 a, bb, du = zero16();
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        a[r] = oa;
+        bb[r] = ob;
+      }
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        const f16x8 x = ld8h(&th[off_row<D>(r0 + li, 2 * kk + g)]);
+        const bf16x8 y = ld8(&td[off_row<D>(r0 + li, 2 * kk + g)]);
+        a = mfma32h(x, wa[kk], a);
+        bb = mfma32h(x, wb[kk], bb);
+        du = mfma32(y, ws[kk], du);
+      }
+      bf16x8 fa[2], fb[2], fu[2];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const SwigluGrad e = swiglu_grad(a[r], bb[r], du[r], slow, ia);
+        ta += e.da;
+        tb += e.db;
+        fa[r >> 3][r & 7] = (bf16)e.da;
+        fb[r >> 3][r & 7] = (bf16)e.db;
+        fu[r >> 3][r & 7] = (bf16)e.u;
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          const bf16x8 x = ld_turned_row<D>(tb16, 32 * c, r0 + 16 * s, lane);
+          const bf16x8 y = ld_turned_row<D>(td, 32 * c, r0 + 16 * s, lane);
+          ga[c] = mfma32(fa[s], x, ga[c]);
+          gb[c] = mfma32(fb[s], x, gb[c]);
+          gs[c] = mfma32(fu[s], y, gs[c]);
+        }
+    }
+    b = b + 1 == NB ? 0 : b + 1;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the transfers past the end
+  if (!own) return;
+  float* to = G + (int64_t)blockIdx.y * 3 * H * D + (int64_t)h0 * D;
+#pragma unroll
+  for (int c = 0; c < CT; ++c)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int at = acc_row(r, g) * D + 32 * c + li;
+#pragma unroll
+      for (int m = 0; m < 3; ++m) {
+        float* q = to + (int64_t)m * H * D + at;
+        const float v = m == 0 ? ga[c][r] : m == 1 ? gb[c][r] : gs[c][r];
+        *q = add ? *q + v : v;
+      }
+    }
+  ta = pair_sum(ta);
+  tb = pair_sum(tb);
+  if (g == 0) {
+    float* q = sums + (int64_t)blockIdx.y * 2 * H + h0 + li;
+    q[0] = add ? q[0] + ta : ta;
+    q[H] = add ? q[H] + tb : tb;
+  }
+}
+
+// dx. A wave owns 32 rows: its operands xh and dy and the sums dxh^T (D x 32 fp32) stay in registers while the weights
+// stream by in chunks of 32 hidden channels, double-buffered by LDS DMA and shared by the workgroup's D / 16
+// waves. Per chunk: a', b', du as D = hidden x rows (a lane holds a row at 16 hidden channels), and da', db'
+// rounded are directly the operand [hidden x rows] of dxh^T = Aw^T da' + Bw^T db' (abt packed in that order of k).
+// The offset comes in by one more product step: three bf16 parts of it (24 bits) times ones. At the end the sums over
+// channels of the norm's backward pass are a lane's own registers and its partner's (lane ^ 32).
+// grid: persistent; block 64 NW, NW = D / 16.
+template <int D>
+struct GradChunk {
+  f16 wa[32 * D], wb[32 * D];   // rows h0 .. h0 + 31 (swizzled)
+  bf16 ws[32 * D];
+  bf16 at[D * 32], bt[D * 32];  // channel rows, the chunk's 32 hidden channels (pieces swizzled)
+};
+// piece p (of 4) of row r of a 32-wide tile
+__device__ __forceinline__ int off_narrow(int r, int p) { return r * 32 + 8 * (p ^ ((r >> 2) & 3)); }
+
+template <int D>
+__global__ __launch_bounds__(4 * D, 2) void transition_grad_rows(
+    const f16* __restrict__ xh, const bf16* __restrict__ dy, const float* __restrict__ rstd_in,
+    const f16* __restrict__ aw, const bf16* __restrict__ st, const bf16* __restrict__ abt,
+    const bf16* __restrict__ split, const float* __restrict__ scale, bf16* __restrict__ dx, int64_t rows, int H,
+    int residual) {
+  constexpr int NW = D / 16, KK = D / 16, CT = D / 32, P = D / 8;
+  __shared__ __attribute__((aligned(16))) GradChunk<D> W[2];
+  extern __shared__ __attribute__((aligned(16))) bf16 off_lds[];  // [2][H][8]: the offsets' parts
+  const int lane = threadIdx.x & 63, g = lane >> 5, li = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t lds = lds_addr(W);
+  const int chunks = H / 32;
+  const float ia = scale[0], slow = -kLog2e * ia;
+  for (int i = threadIdx.x; i < 2 * H; i += 64 * NW)
+    *reinterpret_cast<bf16x8*>(off_lds + 8 * i) = ld8(split + 8 * (int64_t)i);
+  // a wave's transfers of a chunk: one KB of each of its five arrays
+  auto fetch = [&](int c, int b) __attribute__((always_inline)) {
+    const uint32_t at = lds + b * sizeof(GradChunk<D>);
+    const int h0 = 32 * c, r0 = wave * (512 / D);
+    rows_kb<D>(aw, h0, r0, 2 * H - 1, at, lane);
+    rows_kb<D>(aw, H + h0, r0, 2 * H - 1, at + 64 * D, lane);
+    rows_kb<D>(st, h0, r0, H - 1, at + 128 * D, lane);
+    const int cr = 16 * wave + (lane >> 2), piece = (lane & 3) ^ ((cr >> 2) & 3);
+    const bf16* from = abt + (int64_t)cr * 2 * H + h0 + 8 * piece;
+    dma16_at(from, at + 192 * D + 1024 * wave);
+    dma16_at(from + H, at + 256 * D + 1024 * wave);
+  };
+  bf16x8 ones;  // the offsets' operand: 1 at the first three k
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ones[e] = (bf16)(g == 0 && e < 3 ? 1.f : 0.f);
+  const int64_t tiles = (rows + 32 * NW - 1) / (32 * NW);
+  fetch(0, 0);
+  int b = 0;
+#pragma unroll 1
+  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const int64_t row = tile * 32 * NW + 32 * wave + li;
+    const int64_t rc = row < rows ? row : rows - 1;  // rows past the end: the last one again, never stored
+    f16x8 xb[KK];
+    bf16x8 yb[KK];
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      xb[kk] = ld8h(xh + rc * D + 16 * kk + 8 * g);
+      yb[kk] = ld8(dy + rc * D + 16 * kk + 8 * g);
+    }
+    const float rstd = rstd_in[rc];
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) asm volatile("" ::"v"(xb[kk]), "v"(yb[kk]));
+    asm volatile("" ::"v"(rstd));
+    f32x16 acc[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) acc[c] = zero16();
+#pragma unroll 1
+    for (int c = 0; c < chunks; ++c, b ^= 1) {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();  // the chunk is whole; the other buffer has been read
+      asm volatile("" ::: "memory");
+      fetch(c + 1 == chunks ? 0 : c + 1, b ^ 1);  // (wraps into the next tile)
+      const GradChunk<D>* w = &W[b];
+      f32x16 a = zero16(), bb = zero16(), du = zero16();
+      a = mfma32(ld8(off_lds + 8 * (32 * c + li)), ones, a);
+      bb = mfma32(ld8(off_lds + 8 * (H + 32 * c + li)), ones, bb);
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        a = mfma32h(ld8h(&w->wa[off_row<D>(li, 2 * kk + g)]), xb[kk], a);
+        bb = mfma32h(ld8h(&w->wb[off_row<D>(li, 2 * kk + g)]), xb[kk], bb);
+        du = mfma32(ld8(&w->ws[off_row<D>(li, 2 * kk + g)]), yb[kk], du);
+      }
+      bf16x8 fa[2], fb[2];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const SwigluGrad e = swiglu_grad(a[r], bb[r], du[r], slow, ia);
+        fa[r >> 3][r & 7] = (bf16)e.da;
+        fb[r >> 3][r & 7] = (bf16)e.db;
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          acc[ct] = mfma32(ld8(&w->at[off_narrow(32 * ct + li, 2 * s + g)]), fa[s], acc[ct]);
+          acc[ct] = mfma32(ld8(&w->bt[off_narrow(32 * ct + li, 2 * s + g)]), fb[s], acc[ct]);
+        }
+    }
+    // dxh^T: acc[ct] register 4 v + e holds channel 32 ct + 8 v + 4 g + e. xh and dy in the same places: a lane holds
+    // 8 channels 16 kk + 8 g .. of them; its halves and its partner's are exchanged.
+    float sg = 0.f, sx = 0.f;
+    float xv[KK][8];  // channels 16 kk + 4 g + 0..3, 16 kk + 8 + 4 g + 0..3
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      union {
+        f16x8 h;
+        uint32_t u[4];
+      } q;
+      q.h = xb[kk];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const auto sw = __builtin_amdgcn_permlane32_swap(q.u[t], q.u[2 + t], false, false);
+        q.u[t] = sw[0];
+        q.u[2 + t] = sw[1];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        xv[kk][e] = (float)q.h[e];
+        const float t = acc[kk >> 1][8 * (kk & 1) + e];
+        sg += t;
+        sx += t * xv[kk][e];
+      }
+    }
+    const float c1 = pair_sum(sg) * (1.f / D), c2 = pair_sum(sx) * (1.f / D);
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      union {
+        bf16x8 v;
+        uint32_t u[4];
+      } q;
+      q.v = yb[kk];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const auto sw = __builtin_amdgcn_permlane32_swap(q.u[t], q.u[2 + t], false, false);
+        q.u[t] = sw[0];
+        q.u[2 + t] = sw[1];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        q.v[e] = (bf16)((residual ? (float)q.v[e] : 0.f) + rstd * (acc[kk >> 1][8 * (kk & 1) + e] - c1 - xv[kk][e] * c2));
+      // back to whole pieces (the exchange is its own inverse)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const auto sw = __builtin_amdgcn_permlane32_swap(q.u[t], q.u[2 + t], false, false);
+        q.u[t] = sw[0];
+        q.u[2 + t] = sw[1];
+      }
+      if (row < rows) *reinterpret_cast<bf16x8*>(dx + row * D + 16 * kk + 8 * g) = q.v;
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the transfers past the last chunk
+}
+
+// The offsets in three bf16 parts each: split [2][H][8] = {hi, mid, lo, 0, ..}. block 256.
+__global__ __launch_bounds__(256) void split_offsets(const float* __restrict__ offset, bf16* __restrict__ split, int n) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  bf16x8 o;
+  float t = offset[i];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    o[e] = (bf16)(e < 3 ? t : 0.f);
+    t -= (float)o[e];
+  }
+  *reinterpret_cast<bf16x8*>(split + 8 * (int64_t)i) = o;
+}
+
 // dx = (residual ? dy : 0) + rstd (g - mean(g) - xh mean(g xh)), g the sum of `splits` fp32 parts [rows][d]: 8 lanes
 // a row, K = d / 64 pieces of 8 channels each. grid-strided; block 256 (32 rows).
 template <int K>
@@ -564,18 +918,45 @@ void run_norm_grad_rows(const TransitionGradArgs& a, const bf16* dy, int splits,
   }
 }
 
+// Widths the fused kernels take: their offsets and two weight chunks within the 160 KB of LDS.
+bool fused_shape(int d, int H) { return (d == 64 || d == 128) && H <= 2048; }
+
+template <int D>
+size_t grad_rows_lds(int H) { return (size_t)2 * H * 8 * sizeof(bf16); }
+
+template <int D>
+void launch_fused(const TransitionGradArgs& a, const TransitionGradPlan& p, const bf16* dy, bf16* dx, int64_t rows,
+                  int add, hipStream_t st) {
+  constexpr int NW = D / 16;
+  const int H = a.hidden;
+  const auto rows_kernel = transition_grad_rows<D>;
+  const int held = resident_blocks(reinterpret_cast<const void*>(rows_kernel), 64 * NW, grad_rows_lds<D>(H));
+  const int64_t tiles = ceil_div(rows, 32 * NW);
+  rows_kernel<<<dim3((unsigned)std::min<int64_t>(tiles, (int64_t)cu_count() * held)), 64 * NW, grad_rows_lds<D>(H), st>>>(
+      a.xh, dy, a.rstd, a.aw, a.st, a.abt, a.split, a.scale, dx, rows, H, a.residual);
+  transition_grad_weights<D><<<dim3((unsigned)ceil_div(H, 128), (unsigned)p.dw_splits), 256, 0, st>>>(
+      a.xh, a.xhb, dy, a.aw, a.st, a.offset, a.scale, a.dw_part, a.sums, rows, H, add);
+}
+
 }  // namespace
 
 TransitionGradPlan transition_grad_plan(int64_t rows, int d, int H) {
   TransitionGradPlan p{};
+  const int64_t cus = cu_count();
+  p.peaks = 2 * kPeakBlocks;
+  p.fused = fused_shape(d, H) && rows >= 4096;
+  if (p.fused) {
+    p.chunk = std::min<int64_t>(ceil_div(rows, 64) * 64, 1 << 18);
+    const int64_t groups = ceil_div(H, 128);
+    p.dw_splits = (int)std::max<int64_t>(1, std::min<int64_t>((d == 64 ? 2 : 1) * cus / groups, p.chunk / kStageRows));
+    return p;
+  }
   // E of a chunk within 96 MB, so that it is still in the 256 MB last-level cache when the products read it
   const int64_t fit = std::max<int64_t>((int64_t)(96 << 20) / (6 * H) / 64 * 64, 64);
   p.chunk = std::min<int64_t>(ceil_div(rows, 64) * 64, fit);
-  const int64_t cus = cu_count();
   // both products want a workgroup a CU at least, and four steps of 64 in each
   p.dxh_splits = (int)std::max<int64_t>(1, std::min<int64_t>(cus / std::max<int64_t>(1, p.chunk / 64 * (d / 64)), 2 * H / 256));
   p.dw_splits = (int)std::max<int64_t>(1, std::min<int64_t>(2 * cus / std::max<int64_t>(1, 3 * H / 64 * (d / 64)), p.chunk / 256));
-  p.peaks = 2 * kPeakBlocks;
   return p;
 }
 
@@ -584,7 +965,8 @@ void launch_transition_grad(const TransitionGradArgs& a, const TransitionGradPla
   if (a.rows > 0) {
     weight_peaks<<<dim3(kPeakBlocks, 2), 256, 0, st>>>(a.wa, a.wb, a.ln_w, a.peaks, d, H);
     pack_grad_weights<<<dim3(H / 32, 3), 256, 0, st>>>(a.wa, a.wb, a.ws, a.ln_w, a.ln_b, a.peaks, a.aw, a.st, a.abt,
-                                                       a.offset, a.scale, d, H, 0);
+                                                       a.offset, a.scale, d, H, p.fused);
+    if (p.fused) split_offsets<<<dim3((unsigned)ceil_div(2 * H, 256)), 256, 0, st>>>(a.offset, a.split, 2 * H);
   }
   const char* x = static_cast<const char*>(a.x);
   for (int64_t r0 = 0; r0 < a.rows; r0 += p.chunk) {
@@ -596,6 +978,13 @@ void launch_transition_grad(const TransitionGradArgs& a, const TransitionGradPla
       run_norm_rows<true>(a, xc, a.scales + r0 * (d / kActBlock), rows, st);
     else
       run_norm_rows<false>(a, xc, nullptr, rows, st);
+    if (p.fused) {
+      if (d == 64)
+        launch_fused<64>(a, p, dy, a.dx + r0 * d, rows, add, st);
+      else
+        launch_fused<128>(a, p, dy, a.dx + r0 * d, rows, add, st);
+      continue;
+    }
     hidden_grad<<<dim3((unsigned)ceil_div(rows, 64), H / 64), 256, 0, st>>>(a.xh, dy, a.aw, a.st, a.offset, a.scale, a.E,
                                                                             rows, d, H);
     Gemm64Args g{};
