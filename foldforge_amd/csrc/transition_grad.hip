@@ -458,44 +458,54 @@ __device__ __forceinline__ void rows_kb(const void* src, int64_t row0, int r0, i
   dma16_at(static_cast<const bf16*>(src) + row * D + 8 * ((lane % P) ^ swz<D>(r)), dst + 1024u * (r0 * D / 512));
 }
 
-// MFMA operand of a tile of D-channel rows that are k, as ld_turned.
+// Operand of a 16 x 16 product over 32 k from a tile of D-channel rows that are k: channels c0 .. c0 + 15, rows
+// k0 .. k0 + 31. Lanes of quarter q hold rows k0 + 4 q + 0..3 and k0 + 16 + 4 q + 0..3 of one channel.
 template <int D>
-__device__ __forceinline__ bf16x8 ld_turned_row(const bf16* tile, int c0, int k0, int lane) {
+__device__ __forceinline__ bf16x8 ld_turned16(const bf16* tile, int c0, int k0, int lane) {
   const int j = lane & 15, q = lane >> 4;
-  const int r = k0 + 4 * (q >> 1) + (j >> 2), c = c0 + 16 * (q & 1) + 4 * (j & 3);
+  const int r = k0 + 4 * q + (j >> 2), c = c0 + 4 * (j & 3);
   union {
     s16x4 s[2];
     bf16x8 v;
   } o;
   o.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(&tile[off_row<D>(r, c >> 3) + (c & 7)]));
-  o.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(&tile[off_row<D>(r + 8, c >> 3) + (c & 7)]));
+  o.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(&tile[off_row<D>(r + 16, c >> 3) + (c & 7)]));
   return o.v;
+}
+// One wave's 16 x 16 tile over 32 k: a lane holds row / column lane % 16 of its operands at 8 k, and rows 4 (lane / 16)
+// + 0..3 of column lane % 16 of the result.
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16h(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
 // The weights' gradients G = [da'^T xh; db'^T xh; u'^T dy] and the sums of da', db'.
 //
-// A wave owns 32 hidden channels: its operands of Aw, Bw and S^T (D k of 32 channels each) and its sums (3 x 32 x D
-// fp32) stay in registers while the rows stream by; a workgroup's four waves share the rows in LDS. Per 32 rows:
-// a', b', du as D = rows x hidden (a lane holds a hidden channel at 16 rows), their elementwise part in place, and the
+// A wave owns 16 hidden channels: its operands of Aw, Bw and S^T (D k of 16 channels each) and its sums (3 x 16 x D
+// fp32) stay in registers while the rows stream by; a workgroup's eight waves share the rows in LDS. Per 32 rows:
+// a', b', du as D = rows x hidden (a lane holds a hidden channel at 8 rows), their elementwise part in place, and the
 // rounded results are directly the operand [hidden x rows] of the gradients' products, whose other operand (channels
 // x rows) comes out of the same rows by transposing LDS reads, in the same order of k. No hidden value leaves the
-// registers, nothing is turned through LDS. D = 128: 288 registers of operands and sums, one wave per SIMD.
-// grid (ceil(H / 128), splits): split s takes the stages s, s + splits, .. of 64 rows. block 256.
+// registers, nothing is turned through LDS. (32 hidden channels a wave, one wave per SIMD, read half as much LDS, but
+// products and elementwise part then waited for each other: 430 us at 262144 rows x 128 x 512.)
+// grid (ceil(H / 128), splits): split s takes the stages s, s + splits, .. of 64 rows. block 512.
 constexpr int kStageRows = 64;
 template <int D>
 constexpr int kWeightBuffers = D == 128 ? 3 : 2;
 template <int D>
-__global__ __launch_bounds__(256, D == 128 ? 1 : 2) void transition_grad_weights(
+__global__ __launch_bounds__(512, D == 128 ? 2 : 3) void transition_grad_weights(
     const f16* __restrict__ xh, const bf16* __restrict__ xhb, const bf16* __restrict__ dy, const f16* __restrict__ aw,
     const bf16* __restrict__ st, const float* __restrict__ offset, const float* __restrict__ scale,
     float* __restrict__ G, float* __restrict__ sums, int64_t rows, int H, int add) {
-  constexpr int NB = kWeightBuffers<D>, KK = D / 16, CT = D / 32;
+  constexpr int NB = kWeightBuffers<D>, NW = 8, KK = D / 32, CT = D / 16;
   constexpr int kTile = kStageRows * D;              // elements of a tile
-  constexpr int kLoads = 3 * (kTile / 512) / 4;      // transfers of a wave a stage
+  constexpr int kLoads = 3 * (kTile / 512) / NW;     // transfers of a wave a stage
   __shared__ __attribute__((aligned(16))) bf16 buf[NB][3][kTile];  // xh fp16, xh bf16, dy
-  const int lane = threadIdx.x & 63, g = lane >> 5, li = lane & 31;
+  const int lane = threadIdx.x & 63, q = lane >> 4, li = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int h0 = blockIdx.x * 128 + 32 * wave;
+  const int h0 = blockIdx.x * 128 + 16 * wave;
   const bool own = h0 < H;  // H a multiple of 64: the last workgroup's upper waves may own nothing
   const int hr = own ? h0 + li : li;
   const uint32_t lds = lds_addr(buf);
@@ -515,18 +525,19 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void transition_grad_weights
   bf16x8 ws[KK];
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) {
-    wa[kk] = ld8h(aw + (int64_t)hr * D + 16 * kk + 8 * g);
-    wb[kk] = ld8h(aw + (int64_t)(H + hr) * D + 16 * kk + 8 * g);
-    ws[kk] = ld8(st + (int64_t)hr * D + 16 * kk + 8 * g);
+    wa[kk] = ld8h(aw + (int64_t)hr * D + 32 * kk + 8 * q);
+    wb[kk] = ld8h(aw + (int64_t)(H + hr) * D + 32 * kk + 8 * q);
+    ws[kk] = ld8(st + (int64_t)hr * D + 32 * kk + 8 * q);
   }
   const float oa = offset[hr], ob = offset[H + hr], ia = scale[0], slow = -kLog2e * ia;
   // the parameters have landed: without this the compiler waits for them again in every stage
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) asm volatile("" ::"v"(wa[kk]), "v"(wb[kk]), "v"(ws[kk]));
   asm volatile("" ::"v"(oa), "v"(ob), "v"(slow));
-  f32x16 ga[CT], gb[CT], gs[CT];
+  const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
+  f32x4 ga[CT], gb[CT], gs[CT];
 #pragma unroll
-  for (int c = 0; c < CT; ++c) ga[c] = gb[c] = gs[c] = zero16();
+  for (int c = 0; c < CT; ++c) ga[c] = gb[c] = gs[c] = zero4;
   float ta = 0.f, tb = 0.f;
 #pragma unroll
   for (int b = 0; b < NB - 1; ++b) {
@@ -544,11 +555,11 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void transition_grad_weights
       fetch(ahead < stages ? ahead : stages - 1, b == 0 ? NB - 1 : b - 1);
     }
     const f16* th = reinterpret_cast<const f16*>(buf[b][0]);
-    const bf16* tb16 = buf[b][1];
+    const bf16* tx = buf[b][1];
     bf16* td = buf[b][2];
     const int64_t left = rows - stage * kStageRows;
     if (left < kStageRows) {  // rows past the end: dy = 0 makes their gradients 0
-      for (int i = threadIdx.x; i < kTile / 8; i += 256)
+      for (int i = threadIdx.x; i < kTile / 8; i += 64 * NW)
         if (i / (D / 8) >= left) {
           bf16x8 z;
 #pragma unroll
@@ -559,40 +570,41 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void transition_grad_weights
     }
 #pragma unroll 1
     for (int r0 = 0; r0 < kStageRows; r0 += 32) {
-      f32x16 a, bb, du = zero16();
+      f32x4 a[2], bb[2], du[2];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        a[r] = oa;
-        bb[r] = ob;
+      for (int t = 0; t < 2; ++t) {
+        a[t] = f32x4{oa, oa, oa, oa};
+        bb[t] = f32x4{ob, ob, ob, ob};
+        du[t] = zero4;
       }
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        const f16x8 x = ld8h(&th[off_row<D>(r0 + li, 2 * kk + g)]);
-        const bf16x8 y = ld8(&td[off_row<D>(r0 + li, 2 * kk + g)]);
-        a = mfma32h(x, wa[kk], a);
-        bb = mfma32h(x, wb[kk], bb);
-        du = mfma32(y, ws[kk], du);
-      }
-      bf16x8 fa[2], fb[2], fu[2];
+      for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const SwigluGrad e = swiglu_grad(a[r], bb[r], du[r], slow, ia);
+        for (int t = 0; t < 2; ++t) {
+          const f16x8 x = ld8h(&th[off_row<D>(r0 + 16 * t + li, 4 * kk + q)]);
+          const bf16x8 y = ld8(&td[off_row<D>(r0 + 16 * t + li, 4 * kk + q)]);
+          a[t] = mfma16h(x, wa[kk], a[t]);
+          bb[t] = mfma16h(x, wb[kk], bb[t]);
+          du[t] = mfma16(y, ws[kk], du[t]);
+        }
+      bf16x8 fa, fb, fu;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const SwigluGrad e = swiglu_grad(a[r >> 2][r & 3], bb[r >> 2][r & 3], du[r >> 2][r & 3], slow, ia);
         ta += e.da;
         tb += e.db;
-        fa[r >> 3][r & 7] = (bf16)e.da;
-        fb[r >> 3][r & 7] = (bf16)e.db;
-        fu[r >> 3][r & 7] = (bf16)e.u;
+        fa[r] = (bf16)e.da;
+        fb[r] = (bf16)e.db;
+        fu[r] = (bf16)e.u;
       }
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
-          const bf16x8 x = ld_turned_row<D>(tb16, 32 * c, r0 + 16 * s, lane);
-          const bf16x8 y = ld_turned_row<D>(td, 32 * c, r0 + 16 * s, lane);
-          ga[c] = mfma32(fa[s], x, ga[c]);
-          gb[c] = mfma32(fb[s], x, gb[c]);
-          gs[c] = mfma32(fu[s], y, gs[c]);
-        }
+      for (int c = 0; c < CT; ++c) {
+        const bf16x8 x = ld_turned16<D>(tx, 16 * c, r0, lane);
+        const bf16x8 y = ld_turned16<D>(td, 16 * c, r0, lane);
+        ga[c] = mfma16(fa, x, ga[c]);
+        gb[c] = mfma16(fb, x, gb[c]);
+        gs[c] = mfma16(fu, y, gs[c]);
+      }
     }
     b = b + 1 == NB ? 0 : b + 1;
   }
@@ -602,21 +614,24 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void transition_grad_weights
 #pragma unroll
   for (int c = 0; c < CT; ++c)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int at = acc_row(r, g) * D + 32 * c + li;
+    for (int r = 0; r < 4; ++r) {
+      const int at = (4 * q + r) * D + 16 * c + li;
 #pragma unroll
       for (int m = 0; m < 3; ++m) {
-        float* q = to + (int64_t)m * H * D + at;
+        float* p = to + (int64_t)m * H * D + at;
         const float v = m == 0 ? ga[c][r] : m == 1 ? gb[c][r] : gs[c][r];
-        *q = add ? *q + v : v;
+        *p = add ? *p + v : v;
       }
     }
+  // a lane's sums are over its quarter's rows
+  ta += __shfl_xor(ta, 16, 64);
+  tb += __shfl_xor(tb, 16, 64);
   ta = pair_sum(ta);
   tb = pair_sum(tb);
-  if (g == 0) {
-    float* q = sums + (int64_t)blockIdx.y * 2 * H + h0 + li;
-    q[0] = add ? q[0] + ta : ta;
-    q[H] = add ? q[H] + tb : tb;
+  if (q == 0) {
+    float* p = sums + (int64_t)blockIdx.y * 2 * H + h0 + li;
+    p[0] = add ? p[0] + ta : ta;
+    p[H] = add ? p[H] + tb : tb;
   }
 }
 
@@ -934,7 +949,7 @@ void launch_fused(const TransitionGradArgs& a, const TransitionGradPlan& p, cons
   const int64_t tiles = ceil_div(rows, 32 * NW);
   rows_kernel<<<dim3((unsigned)std::min<int64_t>(tiles, (int64_t)cu_count() * held)), 64 * NW, grad_rows_lds<D>(H), st>>>(
       a.xh, dy, a.rstd, a.aw, a.st, a.abt, a.split, a.scale, dx, rows, H, a.residual);
-  transition_grad_weights<D><<<dim3((unsigned)ceil_div(H, 128), (unsigned)p.dw_splits), 256, 0, st>>>(
+  transition_grad_weights<D><<<dim3((unsigned)ceil_div(H, 128), (unsigned)p.dw_splits), 512, 0, st>>>(
       a.xh, a.xhb, dy, a.aw, a.st, a.offset, a.scale, a.dw_part, a.sums, rows, H, add);
 }
 
