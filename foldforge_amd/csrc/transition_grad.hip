@@ -36,8 +36,11 @@ __device__ __forceinline__ f16x8 ld8h(const f16* p) { return *reinterpret_cast<c
 
 // A tile of 64-channel bf16 rows in LDS (128 bytes a row, 8 pieces of 16): piece p of row r lies at piece
 // p ^ swz64(r). Sixteen lanes that read one piece of sixteen consecutive rows (an operand fetch) fall on all
-// 64 banks, and eight rows' 64-byte halves (a transposing fetch) on each bank twice, the least for 512 bytes.
-__device__ __forceinline__ int swz64(int r) { return ((r >> 1) & 1) << 2 | ((r >> 2) & 1) << 1 | ((r >> 3) & 1); }
+// 64 banks. A transposing fetch is served in two halves, the wave's quarters 0 and 2, then 1 and 3 (seen in the conflict
+// counter): 4 rows' 32 bytes a quarter, rows 0-3 and 8-11 (or 4-7) together, which bit 2 ^ bit 3 keeps apart.
+__device__ __forceinline__ int swz64(int r) {
+  return ((r >> 1) & 1) << 2 | (((r >> 2) ^ (r >> 3)) & 1) << 1 | ((r >> 2) & 1);
+}
 __device__ __forceinline__ int off64(int r, int p) { return r * 64 + 8 * (p ^ swz64(r)); }
 
 // This wave's share of a 64 x 64 tile (rows row0 .. row0 + 63 of src, clamped to `last`, channels c0 .. c0 + 63)
@@ -218,7 +221,7 @@ struct SwigluGrad {
 };
 __device__ __forceinline__ SwigluGrad swiglu_grad(float a, float b, float du, float slow, float ia) {
   const float s = __builtin_amdgcn_rcpf(1.f + fast_exp2(a * slow)), sa = a * s;
-  const float slope = s * fmaf(a * (1.f - s), ia, 1.f);
+  const float slope = fmaf(fmaf(-sa, s, sa), ia, s);  // s + silu(a) (1 - s)
   return {du * b * slope, du * sa, sa * b};
 }
 
@@ -437,13 +440,11 @@ static_assert(4 * 2 * 64 * 64 * sizeof(bf16) >= 4 * 4 * 16 * 64 * sizeof(float),
 // ---------------------------------------------------------------------------------------------------------
 // The fused form (d = 64 or 128): two kernels, the hidden rows stay in registers.
 
-// A row of D values of 2 bytes in LDS, D / 8 pieces of 16 bytes: piece p of row r lies at piece p ^ swz(r), the low
-// bits of r in reverse order. Sixteen lanes reading one piece of sixteen rows, and eight rows' 64-byte parts (a
-// transposing fetch), spread over the banks evenly.
+// A row of D values of 2 bytes in LDS, D / 8 pieces of 16 bytes: piece p of row r lies at piece p ^ swz(r), as above.
 template <int D>
 __device__ __forceinline__ int swz(int r) {
   if constexpr (D == 64) return swz64(r);
-  return (r & 1) << 3 | (r & 2) << 1 | (r & 4) >> 1 | (r & 8) >> 3;
+  return (r & 1) << 3 | (r & 2) << 1 | (((r >> 2) ^ (r >> 3)) & 1) << 1 | ((r >> 2) & 1);
 }
 template <int D>
 __device__ __forceinline__ int off_row(int r, int p) { return r * D + 8 * (p ^ swz<D>(r)); }
@@ -458,6 +459,13 @@ __device__ __forceinline__ void rows_kb(const void* src, int64_t row0, int r0, i
   dma16_at(static_cast<const bf16*>(src) + row * D + 8 * ((lane % P) ^ swz<D>(r)), dst + 1024u * (r0 * D / 512));
 }
 
+// 1 KB (512 / D rows) of a row-major array of D-value rows goes to LDS in one transfer, swizzled: lane L copies piece
+// (L % P) ^ swz of row r0 + L / P (P = D / 8; r0 a multiple of 512 / D). The lane's offset from row r0, in bytes:
+template <int D>
+__device__ __forceinline__ uint32_t kb_offset(int r0, int lane) {
+  constexpr int P = D / 8;
+  return 2 * D * (lane / P) + 16 * ((lane % P) ^ swz<D>(r0 + lane / P));
+}
 // Operand of a 16 x 16 product over 32 k from a tile of D-channel rows that are k: channels c0 .. c0 + 15, rows
 // k0 .. k0 + 31. Lanes of quarter q hold rows k0 + 4 q + 0..3 and k0 + 16 + 4 q + 0..3 of one channel.
 template <int D>
@@ -538,7 +546,10 @@ __global__ __launch_bounds__(512, D == 128 ? 2 : 3) void transition_grad_weights
   f32x4 ga[CT], gb[CT], gs[CT];
 #pragma unroll
   for (int c = 0; c < CT; ++c) ga[c] = gb[c] = gs[c] = zero4;
-  float ta = 0.f, tb = 0.f;
+  f32x4 ta = zero4, tb = zero4;  // sums of da', db': products with ones (every column the same)
+  bf16x8 ones;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ones[e] = (bf16)1.f;
 #pragma unroll
   for (int b = 0; b < NB - 1; ++b) {
     const int64_t stage = blockIdx.y + (int64_t)b * gridDim.y;
@@ -591,12 +602,12 @@ __global__ __launch_bounds__(512, D == 128 ? 2 : 3) void transition_grad_weights
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
         const SwigluGrad e = swiglu_grad(a[r >> 2][r & 3], bb[r >> 2][r & 3], du[r >> 2][r & 3], slow, ia);
-        ta += e.da;
-        tb += e.db;
         fa[r] = (bf16)e.da;
         fb[r] = (bf16)e.db;
         fu[r] = (bf16)e.u;
       }
+      ta = mfma16(fa, ones, ta);
+      tb = mfma16(fb, ones, tb);
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
         const bf16x8 x = ld_turned16<D>(tx, 16 * c, r0, lane);
@@ -623,15 +634,13 @@ __global__ __launch_bounds__(512, D == 128 ? 2 : 3) void transition_grad_weights
         *p = add ? *p + v : v;
       }
     }
-  // a lane's sums are over its quarter's rows
-  ta += __shfl_xor(ta, 16, 64);
-  tb += __shfl_xor(tb, 16, 64);
-  ta = pair_sum(ta);
-  tb = pair_sum(tb);
-  if (q == 0) {
-    float* p = sums + (int64_t)blockIdx.y * 2 * H + h0 + li;
-    p[0] = add ? p[0] + ta : ta;
-    p[H] = add ? p[H] + tb : tb;
+  if (li == 0) {
+    float* p = sums + (int64_t)blockIdx.y * 2 * H + h0 + 4 * q;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      p[r] = add ? p[r] + ta[r] : ta[r];
+      p[H + r] = add ? p[H + r] + tb[r] : tb[r];
+    }
   }
 }
 
@@ -667,23 +676,24 @@ __global__ __launch_bounds__(4 * D, 2) void transition_grad_rows(
   const float ia = scale[0], slow = -kLog2e * ia;
   for (int i = threadIdx.x; i < 2 * H; i += 64 * NW)
     *reinterpret_cast<bf16x8*>(off_lds + 8 * i) = ld8(split + 8 * (int64_t)i);
-  // a wave's transfers of a chunk: one KB of each of its five arrays
-  auto fetch = [&](int c, int b) __attribute__((always_inline)) {
-    const uint32_t at = lds + b * sizeof(GradChunk<D>);
-    const int h0 = 32 * c, r0 = wave * (512 / D);
-    rows_kb<D>(aw, h0, r0, 2 * H - 1, at, lane);
-    rows_kb<D>(aw, H + h0, r0, 2 * H - 1, at + 64 * D, lane);
-    rows_kb<D>(st, h0, r0, H - 1, at + 128 * D, lane);
-    const int cr = 16 * wave + (lane >> 2), piece = (lane & 3) ^ ((cr >> 2) & 3);
-    const bf16* from = abt + (int64_t)cr * 2 * H + h0 + 8 * piece;
-    dma16_at(from, at + 192 * D + 1024 * wave);
-    dma16_at(from + H, at + 256 * D + 1024 * wave);
+  // a wave's transfers of a chunk, one KB of each of its five arrays (u = 0 .. 4)
+  const int r0 = wave * (512 / D), cr = lane >> 2;
+  const uint32_t w_off = kb_offset<D>(r0, lane);
+  const uint32_t t_off = 4 * H * cr + 16 * ((lane & 3) ^ ((cr >> 2) & 3));  // 16 channel rows of 2 H values
+  auto fetch = [&](int c, int b, int u) __attribute__((always_inline)) {
+    const uint32_t at = lds + b * sizeof(GradChunk<D>) + u * 64 * D + 1024 * wave;
+    const int64_t row = 32 * c + r0;
+    if (u == 0) dma16(aw + row * D, w_off, at);
+    if (u == 1) dma16(aw + (H + row) * D, w_off, at);
+    if (u == 2) dma16(st + row * D, w_off, at);
+    if (u >= 3) dma16(abt + (int64_t)16 * wave * 2 * H + (u == 4 ? H : 0) + 32 * c, t_off, at);
   };
   bf16x8 ones;  // the offsets' operand: 1 at the first three k
 #pragma unroll
   for (int e = 0; e < 8; ++e) ones[e] = (bf16)(g == 0 && e < 3 ? 1.f : 0.f);
   const int64_t tiles = (rows + 32 * NW - 1) / (32 * NW);
-  fetch(0, 0);
+#pragma unroll
+  for (int u = 0; u < 5; ++u) fetch(0, 0, u);
   int b = 0;
 #pragma unroll 1
   for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
@@ -703,21 +713,34 @@ __global__ __launch_bounds__(4 * D, 2) void transition_grad_rows(
     f32x16 acc[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) acc[c] = zero16();
+    uint32_t touched[2] = {0, 0};
 #pragma unroll 1
     for (int c = 0; c < chunks; ++c, b ^= 1) {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();  // the chunk is whole; the other buffer has been read
       asm volatile("" ::: "memory");
-      fetch(c + 1 == chunks ? 0 : c + 1, b ^ 1);  // (wraps into the next tile)
+      // the next chunk's transfers are spread over this one (all at once, the waves waited for the queue they fill)
+      const int ahead = c + 1 == chunks ? 0 : c + 1;  // (wraps into the next tile)
       const GradChunk<D>* w = &W[b];
       f32x16 a = zero16(), bb = zero16(), du = zero16();
       a = mfma32(ld8(off_lds + 8 * (32 * c + li)), ones, a);
       bb = mfma32(ld8(off_lds + 8 * (H + 32 * c + li)), ones, bb);
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
+        if (kk % (KK / 4) == 0) fetch(ahead, b ^ 1, kk / (KK / 4));
         a = mfma32h(ld8h(&w->wa[off_row<D>(li, 2 * kk + g)]), xb[kk], a);
         bb = mfma32h(ld8h(&w->wb[off_row<D>(li, 2 * kk + g)]), xb[kk], bb);
         du = mfma32(ld8(&w->ws[off_row<D>(li, 2 * kk + g)]), yb[kk], du);
+      }
+      fetch(ahead, b ^ 1, 4);
+      if (c == chunks / 2) {
+        // a value of each line of the next tile's rows: they come into the cache under this tile's products (all tiles
+        // start at once, and waiting for their rows took 40 of 230 us)
+        constexpr int L = D / 64;  // 128-byte lines of a row
+        const int64_t r = (tile + gridDim.x) * 32 * NW + 32 * wave + lane / L % 32;
+        const int64_t at = (r < rows ? r : rows - 1) * D + 64 * (lane % L);
+        touched[0] = *reinterpret_cast<const uint32_t*>(xh + at);
+        touched[1] = *reinterpret_cast<const uint32_t*>(dy + at);
       }
       bf16x8 fa[2], fb[2];
 #pragma unroll
@@ -734,6 +757,7 @@ __global__ __launch_bounds__(4 * D, 2) void transition_grad_rows(
           acc[ct] = mfma32(ld8(&w->bt[off_narrow(32 * ct + li, 2 * s + g)]), fb[s], acc[ct]);
         }
     }
+    asm volatile("" ::"v"(touched[0]), "v"(touched[1]));
     // dxh^T: acc[ct] register 4 v + e holds channel 32 ct + 8 v + 4 g + e. xh and dy in the same places: a lane holds
     // 8 channels 16 kk + 8 g .. of them; its halves and its partner's are exchanged.
     float sg = 0.f, sx = 0.f;
