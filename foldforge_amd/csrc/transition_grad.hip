@@ -449,16 +449,6 @@ __device__ __forceinline__ int swz(int r) {
 template <int D>
 __device__ __forceinline__ int off_row(int r, int p) { return r * D + 8 * (p ^ swz<D>(r)); }
 
-// 1 KB (512 / D rows) of a row-major array into LDS at dst, swizzled; r0: the KB's first row in the LDS tile, a
-// multiple of 512 / D (rows row0 + .. of src, clamped to last).
-template <int D>
-__device__ __forceinline__ void rows_kb(const void* src, int64_t row0, int r0, int64_t last, uint32_t dst, int lane) {
-  constexpr int P = D / 8;  // pieces of a row
-  const int r = r0 + lane / P;
-  const int64_t row = row0 + r < last ? row0 + r : last;
-  dma16_at(static_cast<const bf16*>(src) + row * D + 8 * ((lane % P) ^ swz<D>(r)), dst + 1024u * (r0 * D / 512));
-}
-
 // 1 KB (512 / D rows) of a row-major array of D-value rows goes to LDS in one transfer, swizzled: lane L copies piece
 // (L % P) ^ swz of row r0 + L / P (P = D / 8; r0 a multiple of 512 / D). The lane's offset from row r0, in bytes:
 template <int D>
@@ -466,18 +456,31 @@ __device__ __forceinline__ uint32_t kb_offset(int r0, int lane) {
   constexpr int P = D / 8;
   return 2 * D * (lane / P) + 16 * ((lane % P) ^ swz<D>(r0 + lane / P));
 }
-// Operand of a 16 x 16 product over 32 k from a tile of D-channel rows that are k: channels c0 .. c0 + 15, rows
-// k0 .. k0 + 31. Lanes of quarter q hold rows k0 + 4 q + 0..3 and k0 + 16 + 4 q + 0..3 of one channel.
+// Nothing is scheduled across: left alone the compiler fetches each operand right before its product and waits out the
+// LDS latency every time, so the products' loops fetch a step or two ahead in the order they are written.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
+
+// LDS reads by byte address. A piece's number enters an address by XOR (of bits below the row's), so that a lane needs one
+// address for a tile: piece p + 2^i, with bit i of p clear, is at the address of p with that bit turned over.
+template <typename V>
+__device__ __forceinline__ V lds_at(uint32_t a) {
+  return *(const __attribute__((address_space(3))) V*)(a);
+}
+// Operand of a 16 x 16 product over 32 k from a tile of D-channel rows that are k: lanes of quarter q hold rows 4 q + 0..3
+// and 16 + 4 q + 0..3 of one channel. a: turned_at(...) of the tile, its channels 16 c .. by ^ (c << 5).
 template <int D>
-__device__ __forceinline__ bf16x8 ld_turned16(const bf16* tile, int c0, int k0, int lane) {
-  const int j = lane & 15, q = lane >> 4;
-  const int r = k0 + 4 * q + (j >> 2), c = c0 + 4 * (j & 3);
+__device__ __forceinline__ uint32_t turned_at(int lane) {
+  const int j = lane & 15, r = 4 * (lane >> 4) + (j >> 2);
+  return 2 * off_row<D>(r, (j & 3) >> 1) + 8 * (j & 1);
+}
+template <int D>
+__device__ __forceinline__ bf16x8 ld_turned16(uint32_t a) {
   union {
     s16x4 s[2];
     bf16x8 v;
   } o;
-  o.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(&tile[off_row<D>(r, c >> 3) + (c & 7)]));
-  o.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(&tile[off_row<D>(r + 16, c >> 3) + (c & 7)]));
+  o.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a));
+  o.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + 32 * D));
   return o.v;
 }
 // One wave's 16 x 16 tile over 32 k: a lane holds row / column lane % 16 of its operands at 8 k, and rows 4 (lane / 16)
@@ -518,16 +521,19 @@ __global__ __launch_bounds__(512, D == 128 ? 2 : 3) void transition_grad_weights
   const int hr = own ? h0 + li : li;
   const uint32_t lds = lds_addr(buf);
   const int64_t stages = (rows + kStageRows - 1) / kStageRows;
-  auto fetch = [&](int64_t stage, int b) __attribute__((always_inline)) {
-    const int64_t row0 = stage * kStageRows;
-#pragma unroll
-    for (int t = 0; t < 3; ++t) {
-      const void* src = t == 0 ? (const void*)xh : t == 1 ? (const void*)xhb : (const void*)dy;
-#pragma unroll
-      for (int u = 0; u < kLoads / 3; ++u)
-        rows_kb<D>(src, row0, (kLoads / 3 * wave + u) * (512 / D), rows - 1,
-                   lds + (uint32_t)((b * 3 + t) * kTile * sizeof(bf16)), lane);
-    }
+  const uint32_t rows_at = 2 * off_row<D>(li, q), turned = turned_at<D>(lane);  // a lane's places in a tile
+  // transfer u = 0 .. kLoads - 1 of a wave; rows past the end: the last one again
+  constexpr int kKb = kLoads / 3;  // its KBs of each array
+  const uint32_t lane_row = 2 * D * (lane / (D / 8)), lane_piece = kb_offset<D>(0, lane) - lane_row;
+  auto fetch = [&](int64_t stage, int b, int u) __attribute__((always_inline)) {
+    const int t = u / kKb, kb = kKb * wave + u % kKb, r0 = kb * (512 / D);
+    const int64_t row = stage * kStageRows + r0, from = row < rows ? row : rows - 1;
+    const uint32_t most = rows - 1 - from < 512 / D ? 2 * D * (uint32_t)(rows - 1 - from) : 1024u;
+    const void* src = t == 0 ? (const void*)xh : t == 1 ? (const void*)xhb : (const void*)dy;
+    // (the swizzle of row r0 + i is that of i, turned over by that of r0: their bits are apart)
+    dma16(static_cast<const bf16*>(src) + from * D,
+          (lane_row < most ? lane_row : most) + (lane_piece ^ (16 * swz<D>(r0))),
+          lds + (uint32_t)((b * 3 + t) * kTile * sizeof(bf16)) + 1024 * kb);
   };
   f16x8 wa[KK], wb[KK];
   bf16x8 ws[KK];
@@ -542,7 +548,7 @@ __global__ __launch_bounds__(512, D == 128 ? 2 : 3) void transition_grad_weights
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) asm volatile("" ::"v"(wa[kk]), "v"(wb[kk]), "v"(ws[kk]));
   asm volatile("" ::"v"(oa), "v"(ob), "v"(slow));
-  const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
+  const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f}, oa4 = {oa, oa, oa, oa}, ob4 = {ob, ob, ob, ob};
   f32x4 ga[CT], gb[CT], gs[CT];
 #pragma unroll
   for (int c = 0; c < CT; ++c) ga[c] = gb[c] = gs[c] = zero4;
@@ -553,7 +559,8 @@ __global__ __launch_bounds__(512, D == 128 ? 2 : 3) void transition_grad_weights
 #pragma unroll
   for (int b = 0; b < NB - 1; ++b) {
     const int64_t stage = blockIdx.y + (int64_t)b * gridDim.y;
-    fetch(stage < stages ? stage : stages - 1, b);
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) fetch(stage < stages ? stage : stages - 1, b, u);
   }
   int b = 0;
 #pragma unroll 1
@@ -561,12 +568,10 @@ __global__ __launch_bounds__(512, D == 128 ? 2 : 3) void transition_grad_weights
     wait_vm_lds<(NB - 2) * kLoads>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    {  // (past the end: the last rows again, which nothing reads)
-      const int64_t ahead = stage + (int64_t)(NB - 1) * gridDim.y;
-      fetch(ahead < stages ? ahead : stages - 1, b == 0 ? NB - 1 : b - 1);
-    }
-    const f16* th = reinterpret_cast<const f16*>(buf[b][0]);
-    const bf16* tx = buf[b][1];
+    // the next stage's transfers are spread over this one (past the end: the last rows again, which nothing reads)
+    int64_t ahead = stage + (int64_t)(NB - 1) * gridDim.y;
+    ahead = ahead < stages ? ahead : stages - 1;
+    const int into = b == 0 ? NB - 1 : b - 1;
     bf16* td = buf[b][2];
     const int64_t left = rows - stage * kStageRows;
     if (left < kStageRows) {  // rows past the end: dy = 0 makes their gradients 0
@@ -580,24 +585,47 @@ __global__ __launch_bounds__(512, D == 128 ? 2 : 3) void transition_grad_weights
       __syncthreads();
     }
 #pragma unroll 1
-    for (int r0 = 0; r0 < kStageRows; r0 += 32) {
+    for (int half = 0; half < 2; ++half) {
+      const uint32_t tile = lds + (uint32_t)((b * 3 * kTile + half * 32 * D) * sizeof(bf16));
+      const uint32_t rows_a = tile + rows_at, turned_a = tile + turned;
+      constexpr uint32_t kArray = kTile * sizeof(bf16);
       f32x4 a[2], bb[2], du[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        a[t] = f32x4{oa, oa, oa, oa};
-        bb[t] = f32x4{ob, ob, ob, ob};
-        du[t] = zero4;
-      }
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk)
+      f16x8 lx[2][2];
+      bf16x8 ly[2][2];
+      auto take = [&](int kk) __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const f16x8 x = ld8h(&th[off_row<D>(r0 + 16 * t + li, 4 * kk + q)]);
-          const bf16x8 y = ld8(&td[off_row<D>(r0 + 16 * t + li, 4 * kk + q)]);
-          a[t] = mfma16h(x, wa[kk], a[t]);
-          bb[t] = mfma16h(x, wb[kk], bb[t]);
-          du[t] = mfma16(y, ws[kk], du[t]);
+          lx[kk & 1][t] = lds_at<f16x8>((rows_a ^ (kk << 6)) + 32 * D * t);
+          ly[kk & 1][t] = lds_at<bf16x8>((rows_a ^ (kk << 6)) + 32 * D * t + 2 * kArray);
         }
+        in_order();
+      };
+      bf16x8 tx8[2], ty8[2];
+      auto take2 = [&](int c) __attribute__((always_inline)) {
+        tx8[c & 1] = ld_turned16<D>((turned_a ^ (c << 5)) + kArray);
+        ty8[c & 1] = ld_turned16<D>((turned_a ^ (c << 5)) + 2 * kArray);
+        in_order();
+      };
+      take(0);
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        if (kk + 1 < KK) take(kk + 1);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          a[t] = mfma16h(lx[kk & 1][t], wa[kk], kk ? a[t] : oa4);
+          bb[t] = mfma16h(lx[kk & 1][t], wb[kk], kk ? bb[t] : ob4);
+          du[t] = mfma16(ly[kk & 1][t], ws[kk], kk ? du[t] : zero4);
+        }
+        in_order();
+      }
+      if (half == 0) {
+#pragma unroll
+        for (int u = 0; u < kLoads / 2; ++u) fetch(ahead, into, u);
+      } else {
+#pragma unroll
+        for (int u = kLoads / 2; u < kLoads; ++u) fetch(ahead, into, u);
+      }
+      take2(0);
       bf16x8 fa, fb, fu;
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
@@ -606,15 +634,17 @@ __global__ __launch_bounds__(512, D == 128 ? 2 : 3) void transition_grad_weights
         fb[r] = (bf16)e.db;
         fu[r] = (bf16)e.u;
       }
+      in_order();
+      take2(1);
       ta = mfma16(fa, ones, ta);
       tb = mfma16(fb, ones, tb);
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
-        const bf16x8 x = ld_turned16<D>(tx, 16 * c, r0, lane);
-        const bf16x8 y = ld_turned16<D>(td, 16 * c, r0, lane);
-        ga[c] = mfma16(fa, x, ga[c]);
-        gb[c] = mfma16(fb, x, gb[c]);
-        gs[c] = mfma16(fu, y, gs[c]);
+        ga[c] = mfma16(fa, tx8[c & 1], ga[c]);
+        gb[c] = mfma16(fb, tx8[c & 1], gb[c]);
+        gs[c] = mfma16(fu, ty8[c & 1], gs[c]);
+        in_order();
+        if (c + 2 < CT) take2(c + 2);
       }
     }
     b = b + 1 == NB ? 0 : b + 1;
