@@ -513,7 +513,7 @@ __global__ __launch_bounds__(512, D == 128 ? 2 : 3) void transition_grad_weights
   constexpr int NB = kWeightBuffers<D>, NW = 8, KK = D / 32, CT = D / 16;
   constexpr int kTile = kStageRows * D;              // elements of a tile
   constexpr int kLoads = 3 * (kTile / 512) / NW;     // transfers of a wave a stage
-  __shared__ __attribute__((aligned(16))) bf16 buf[NB][3][kTile];  // xh fp16, xh bf16, dy
+  __shared__ __attribute__((aligned(256))) bf16 buf[NB][3][kTile];  // xh fp16, xh bf16, dy
   const int lane = threadIdx.x & 63, q = lane >> 4, li = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h0 = blockIdx.x * 128 + 16 * wave;
@@ -697,12 +697,13 @@ __global__ __launch_bounds__(4 * D, 2) void transition_grad_rows(
     const bf16* __restrict__ split, const float* __restrict__ scale, bf16* __restrict__ dx, int64_t rows, int H,
     int residual) {
   constexpr int NW = D / 16, KK = D / 16, CT = D / 32, P = D / 8;
-  __shared__ __attribute__((aligned(16))) GradChunk<D> W[2];
+  __shared__ __attribute__((aligned(256))) GradChunk<D> W[2];
   extern __shared__ __attribute__((aligned(16))) bf16 off_lds[];  // [2][H][8]: the offsets' parts
   const int lane = threadIdx.x & 63, g = lane >> 5, li = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t lds = lds_addr(W);
   const int chunks = H / 32;
+  const uint32_t rows_at = 2 * off_row<D>(li, g), narrow_at = 2 * off_narrow(li, g);  // a lane's places in a chunk
   const float ia = scale[0], slow = -kLog2e * ia;
   for (int i = threadIdx.x; i < 2 * H; i += 64 * NW)
     *reinterpret_cast<bf16x8*>(off_lds + 8 * i) = ld8(split + 8 * (int64_t)i);
@@ -751,16 +752,39 @@ __global__ __launch_bounds__(4 * D, 2) void transition_grad_rows(
       asm volatile("" ::: "memory");
       // the next chunk's transfers are spread over this one (all at once, the waves waited for the queue they fill)
       const int ahead = c + 1 == chunks ? 0 : c + 1;  // (wraps into the next tile)
-      const GradChunk<D>* w = &W[b];
+      const uint32_t at = lds + b * sizeof(GradChunk<D>);
+      const uint32_t rows_a = at + rows_at, narrow_a = at + 192 * D + narrow_at;
       f32x16 a = zero16(), bb = zero16(), du = zero16();
       a = mfma32(ld8(off_lds + 8 * (32 * c + li)), ones, a);
       bb = mfma32(ld8(off_lds + 8 * (H + 32 * c + li)), ones, bb);
+      f16x8 la[2], lb[2];
+      bf16x8 ls[2], lt[2][2];
+      auto take = [&](int kk) __attribute__((always_inline)) {
+        const uint32_t p = rows_a ^ (kk << 5);
+        la[kk & 1] = lds_at<f16x8>(p);
+        lb[kk & 1] = lds_at<f16x8>(p + 64 * D);
+        ls[kk & 1] = lds_at<bf16x8>(p + 128 * D);
+        in_order();
+      };
+      // i = 0 .. 2 CT - 1: half s of the hidden channels, Aw^T or Bw^T, two channel tiles
+      auto take2 = [&](int i) __attribute__((always_inline)) {
+        const uint32_t p = (narrow_a ^ (32 * (i / CT))) + 64 * D * (i / (CT / 2) % 2) + 2048 * (2 * i % CT);
+        lt[i & 1][0] = lds_at<bf16x8>(p);
+        lt[i & 1][1] = lds_at<bf16x8>(p + 2048);
+        in_order();
+      };
+      take(0);
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
         if (kk % (KK / 4) == 0) fetch(ahead, b ^ 1, kk / (KK / 4));
-        a = mfma32h(ld8h(&w->wa[off_row<D>(li, 2 * kk + g)]), xb[kk], a);
-        bb = mfma32h(ld8h(&w->wb[off_row<D>(li, 2 * kk + g)]), xb[kk], bb);
-        du = mfma32(ld8(&w->ws[off_row<D>(li, 2 * kk + g)]), yb[kk], du);
+        if (kk + 1 < KK)
+          take(kk + 1);
+        else
+          take2(0);
+        a = mfma32h(la[kk & 1], xb[kk], a);
+        bb = mfma32h(lb[kk & 1], xb[kk], bb);
+        du = mfma32(ls[kk & 1], yb[kk], du);
+        in_order();
       }
       fetch(ahead, b ^ 1, 4);
       if (c == chunks / 2) {
@@ -773,19 +797,28 @@ __global__ __launch_bounds__(4 * D, 2) void transition_grad_rows(
         touched[1] = *reinterpret_cast<const uint32_t*>(dy + at);
       }
       bf16x8 fa[2], fb[2];
+      auto elements = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const SwigluGrad e = swiglu_grad(a[r], bb[r], du[r], slow, ia);
-        fa[r >> 3][r & 7] = (bf16)e.da;
-        fb[r >> 3][r & 7] = (bf16)e.db;
-      }
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          acc[ct] = mfma32(ld8(&w->at[off_narrow(32 * ct + li, 2 * s + g)]), fa[s], acc[ct]);
-          acc[ct] = mfma32(ld8(&w->bt[off_narrow(32 * ct + li, 2 * s + g)]), fb[s], acc[ct]);
+        for (int r = 0; r < 8; ++r) {
+          const SwigluGrad e = swiglu_grad(a[8 * s + r], bb[8 * s + r], du[8 * s + r], slow, ia);
+          fa[s][r] = (bf16)e.da;
+          fb[s][r] = (bf16)e.db;
         }
+      };
+      auto second = [&](int i) __attribute__((always_inline)) {
+        const int s = i / CT, m = i / (CT / 2) % 2, ct = 2 * i % CT;
+        acc[ct] = mfma32(lt[i & 1][0], m ? fb[s] : fa[s], acc[ct]);
+        acc[ct + 1] = mfma32(lt[i & 1][1], m ? fb[s] : fa[s], acc[ct + 1]);
+      };
+      elements(0);
+      elements(1);
+      in_order();
+#pragma unroll
+      for (int i = 0; i < 2 * CT; ++i) {
+        if (i + 1 < 2 * CT) take2(i + 1);
+        second(i);
+        in_order();
+      }
     }
     asm volatile("" ::"v"(touched[0]), "v"(touched[1]));
     // dxh^T: acc[ct] register 4 v + e holds channel 32 ct + 8 v + 4 g + e. xh and dy in the same places: a lane holds
