@@ -279,9 +279,10 @@ TransitionGradArgs transition_grad_ws(void* ws, size_t* bytes, const TransitionG
   Carver cv{static_cast<char*>(ws)};
   TransitionGradArgs a{};
   const size_t w = (size_t)hidden * d;
-  a.peaks = cv.take<float>(p.peaks);
+  a.peaks = cv.take<float>((size_t)hidden / 2);
   a.scale = cv.take<float>(2);
   a.offset = cv.take<float>(2 * (size_t)hidden);
+  a.shift = cv.take<float>(2 * (size_t)hidden);
   a.aw = cv.take<f16>(2 * w);
   a.st = cv.take<bf16>(w);
   a.abt = cv.take<bf16>(2 * w);

@@ -415,7 +415,7 @@ void launch_sum_partials(const float* part, int count, int width, int split, voi
 // Backward pass of the SwiGLU transition (rows > 0; d a multiple of 64 up to 768, hidden of 64).
 struct TransitionGradPlan {
   int64_t chunk;  // rows at once, a multiple of 64
-  int dxh_splits, dw_splits, peaks;
+  int dxh_splits, dw_splits;
   int fused;      // the hidden rows stay in registers (no E, no dxh)
 };
 TransitionGradPlan transition_grad_plan(int64_t rows, int d, int hidden);
@@ -430,7 +430,7 @@ struct TransitionGradArgs {
   int d, hidden, residual, grad_dtype;
   float eps;
   // workspace: the weights in the products' orders and their scales,
-  float *peaks, *scale, *offset;        // [peaks], [2], [2 hidden]
+  float *peaks, *scale, *offset, *shift;  // [hidden / 2], [2], [2 hidden], [2 hidden]
   f16* aw;                              // [2 hidden][d]
   bf16 *st, *abt;                       // [hidden][d], [d][2 hidden]
   bf16* split;                          // [2][hidden][8] (fused)

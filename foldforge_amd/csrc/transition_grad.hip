@@ -79,29 +79,6 @@ __device__ __forceinline__ bf16x8 ld_turned(const bf16* tile, int c0, int k0, in
   return o.v;
 }
 
-// What a call's kernels share: the scales' exponents as factors.
-//   scale[0] = 2^-ka, scale[1] = 2^-kb
-// The largest |A w| and |B w| of each workgroup's share of the entries. grid (kPeakBlocks, 2); block 256.
-constexpr int kPeakBlocks = 32;
-__global__ __launch_bounds__(256) void weight_peaks(const float* __restrict__ wa, const float* __restrict__ wb,
-                                                    const float* __restrict__ w, float* __restrict__ peaks, int d,
-                                                    int H) {
-  __shared__ float red[4];
-  const float* src = blockIdx.y ? wb : wa;
-  float top = 0.f;
-  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < (int64_t)H * d; i += (int64_t)kPeakBlocks * 1024) {
-    const f32x4_a4 v = *reinterpret_cast<const f32x4_a4*>(src + i);
-    const int c = (int)(i % d);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) top = fmaxf(top, finite_abs(v[e] * w[c + e]));
-  }
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
-  __syncthreads();
-  if (threadIdx.x == 0)
-    peaks[blockIdx.y * kPeakBlocks + blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-}
 // k with peak 2^k in [2^14, 2^15) (within what fp32 powers allow; 0 for a matrix of zeros).
 __device__ __forceinline__ int peak_power(float peak) {
   if (peak == 0.f) return 0;
@@ -110,75 +87,118 @@ __device__ __forceinline__ int peak_power(float peak) {
 }
 __device__ __forceinline__ float two_to(int k) { return __uint_as_float((uint32_t)(127 + k) << 23); }
 
-// fp32 parameters in the orders the products read: aw [2 H][d] fp16 (Aw 2^ka, then Bw 2^kb), st [H][d] bf16 (S^T),
-// abt [d][2 H] bf16 (Aw^T 2^-kb, Bw^T 2^-ka; within each 16 hidden channels in accumulator order 0-3, 8-11, 4-7,
-// 12-15 where turned, else in order), offset [2][H] fp32 (A v 2^ka, B v 2^kb), scale. 32 hidden channels a
-// workgroup: grid (H / 32, 3); block 256.
-__global__ __launch_bounds__(256) void pack_grad_weights(const float* __restrict__ wa, const float* __restrict__ wb,
-                                                         const float* __restrict__ ws, const float* __restrict__ w,
-                                                         const float* __restrict__ v, const float* __restrict__ peaks,
-                                                         f16* __restrict__ aw, bf16* __restrict__ st,
-                                                         bf16* __restrict__ abt, float* __restrict__ offset,
-                                                         float* __restrict__ scale, int d, int H, int turned) {
-  __shared__ float tile[32][33];
-  const int h0 = blockIdx.x * 32, which = blockIdx.y;
-  const int col = threadIdx.x & 31, row = threadIdx.x >> 5;
-  if (which == 2) {
-    for (int c0 = 0; c0 < d; c0 += 32) {
-      __syncthreads();
-      for (int r = row; r < 32; r += 8) tile[r][col] = ws[(int64_t)(c0 + r) * H + h0 + col];
-      __syncthreads();
-      for (int r = row; r < 32; r += 8) st[(int64_t)(h0 + r) * d + c0 + col] = (bf16)tile[col][r];
-    }
-    return;
+// Of each row h of A and B: offset [2][H] = the row's product with v, and of each four rows (a workgroup's) the largest
+// |A w| in peaks [2][H / 4]. One wave a row; block 256, 2 H / 4 of them.
+__device__ __forceinline__ void weight_rows(int block, const float* __restrict__ wa, const float* __restrict__ wb,
+                                            const float* __restrict__ w, const float* __restrict__ v,
+                                            float* __restrict__ offset, float* __restrict__ peaks, int d, int H) {
+  __shared__ float red[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = block * 4 + wave;
+  const float* row = (h < H ? wa : wb) + (int64_t)(h < H ? h : h - H) * d;
+  float top = 0.f, dot = 0.f;
+#pragma unroll 4
+  for (int c = lane; c < d; c += 64) {
+    const float t = row[c];
+    top = fmaxf(top, finite_abs(t * w[c]));
+    dot += t * v[c];
   }
-  float peak[2] = {0.f, 0.f};
-  for (int i = 0; i < kPeakBlocks; ++i) {
-    peak[0] = fmaxf(peak[0], peaks[i]);
-    peak[1] = fmaxf(peak[1], peaks[kPeakBlocks + i]);
-  }
-  const int ka = peak_power(peak[0]), kb = peak_power(peak[1]);
-  if (blockIdx.x == 0 && which == 0 && threadIdx.x == 0) {
-    scale[0] = two_to(-ka);
-    scale[1] = two_to(-kb);
-  }
-  const float up = two_to(which ? kb : ka), down = two_to(which ? -ka : -kb);
-  const float* src = which ? wb : wa;
-  float dot[4] = {0.f, 0.f, 0.f, 0.f};
-  // hidden channel of place `col` of the turned order
-  const int hid = turned ? (col & ~12) | ((col & 4) << 1) | ((col & 8) >> 1) : col;
-  for (int c0 = 0; c0 < d; c0 += 32) {
-    const float wc = w[c0 + col], vc = v[c0 + col];
-    __syncthreads();
+  dot = lanes_sum<64>(dot);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = row + 8 * i;
-      const float t = src[(int64_t)(h0 + r) * d + c0 + col];
-      dot[i] += t * vc;
-      tile[r][col] = t * wc;
-      aw[(int64_t)(which * H + h0 + r) * d + c0 + col] = (f16)(t * wc * up);
-    }
-    __syncthreads();
-    for (int r = row; r < 32; r += 8)
-      abt[(int64_t)(c0 + r) * 2 * H + which * H + h0 + col] = (bf16)(tile[hid][r] * down);
+  for (int m = 32; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+  if (lane == 0) {
+    offset[h] = dot;
+    red[wave] = top;
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float t = lanes_sum<32>(dot[i]);
-    if (col == 0) offset[which * H + h0 + row + 8 * i] = t * up;
-  }
+  __syncthreads();
+  if (threadIdx.x == 0) peaks[block] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
 
-// xh in fp16 and bf16 and rstd of the kept rows: 8 lanes a row, K = d / 64 pieces of 8 channels each.
-// grid-strided; block 256 (32 rows).
+// fp32 parameters in the orders the products read: aw [2 H][d] fp16 (Aw 2^ka, then Bw 2^kb), st [H][d] bf16 (S^T),
+// abt [d][2 H] bf16 (Aw^T 2^-kb, Bw^T 2^-ka; within each 16 hidden channels in accumulator order 0-3, 8-11, 4-7,
+// 12-15 where turned, else in order); scale = {2^-ka, 2^-kb}; the offsets times 2^ka, 2^kb, as fp32 in shift [2][H] and
+// (turned) in three bf16 parts, split [2][H][8] = {hi, mid, lo, 0, ..}. A 32 x 32 tile of one matrix a workgroup: grid
+// (H / 32, d / 32, 3); block 256.
+__global__ __launch_bounds__(256) void pack_grad_weights(const float* __restrict__ wa, const float* __restrict__ wb,
+                                                         const float* __restrict__ ws, const float* __restrict__ w,
+                                                         const float* __restrict__ peaks,
+                                                         const float* __restrict__ offset, f16* __restrict__ aw,
+                                                         bf16* __restrict__ st, bf16* __restrict__ abt,
+                                                         float* __restrict__ shift, bf16* __restrict__ split,
+                                                         float* __restrict__ scale, int d, int H, int turned) {
+  __shared__ float tile[32][33], red[2][4];
+  const int h0 = blockIdx.x * 32, c0 = blockIdx.y * 32, which = blockIdx.z;
+  const int col = threadIdx.x & 31, row = threadIdx.x >> 5;
+  if (which == 2) {
+    for (int r = row; r < 32; r += 8) tile[r][col] = ws[(int64_t)(c0 + r) * H + h0 + col];
+    __syncthreads();
+    for (int r = row; r < 32; r += 8) st[(int64_t)(h0 + r) * d + c0 + col] = (bf16)tile[col][r];
+    return;
+  }
+  float t[4];
+  const float* src = which ? wb : wa;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) t[i] = src[(int64_t)(h0 + row + 8 * i) * d + c0 + col];
+  const float wc = w[c0 + col];
+  float peak[2] = {0.f, 0.f};
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    for (int i = threadIdx.x; i < H / 4; i += 256) peak[m] = fmaxf(peak[m], peaks[m * (H / 4) + i]);
+#pragma unroll
+    for (int x = 32; x >= 1; x >>= 1) peak[m] = fmaxf(peak[m], __shfl_xor(peak[m], x, 64));
+    if ((threadIdx.x & 63) == 0) red[m][threadIdx.x >> 6] = peak[m];
+  }
+  __syncthreads();
+  int k[2];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+    k[m] = peak_power(fmaxf(fmaxf(red[m][0], red[m][1]), fmaxf(red[m][2], red[m][3])));
+  const float up = two_to(which ? k[1] : k[0]), down = two_to(which ? -k[0] : -k[1]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = row + 8 * i;
+    tile[r][col] = t[i] * wc;
+    aw[(int64_t)(which * H + h0 + r) * d + c0 + col] = (f16)(t[i] * wc * up);
+  }
+  if (c0 == 0 && threadIdx.x < 32) {
+    const int h = which * H + h0 + threadIdx.x;
+    float o = offset[h] * up;
+    shift[h] = o;
+    if (turned) {
+      bf16x8 parts;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        parts[e] = (bf16)(e < 3 ? o : 0.f);
+        o -= (float)parts[e];
+      }
+      *reinterpret_cast<bf16x8*>(split + 8 * (int64_t)h) = parts;
+    }
+  }
+  if (blockIdx.x + blockIdx.y + which == 0 && threadIdx.x < 2) scale[threadIdx.x] = two_to(-k[threadIdx.x]);
+  __syncthreads();
+  // hidden channel of place `col` of the turned order
+  const int hid = turned ? (col & ~12) | ((col & 4) << 1) | ((col & 8) >> 1) : col;
+  for (int r = row; r < 32; r += 8)
+    abt[(int64_t)(c0 + r) * 2 * H + which * H + h0 + col] = (bf16)(tile[hid][r] * down);
+}
+
+// What a call makes of its inputs first, in one launch: the rows of the weights (the first `weight_blocks` workgroups:
+// weight_rows), and xh in fp16 and bf16 and rstd of the kept rows: 8 lanes a row, K = d / 64 pieces of 8 channels each,
+// the other workgroups grid-strided over rows. block 256 (32 rows).
 template <bool CODES, int K>
 __global__ __launch_bounds__(256) void norm_rows(const void* x, const uint8_t* scales, f16* __restrict__ xh,
                                                  bf16* __restrict__ xhb, float* __restrict__ rstd_out, int64_t rows,
-                                                 float eps) {
+                                                 float eps, int weight_blocks, const float* __restrict__ wa,
+                                                 const float* __restrict__ wb, const float* __restrict__ w,
+                                                 const float* __restrict__ v, float* __restrict__ offset,
+                                                 float* __restrict__ peaks, int H) {
   constexpr int d = 64 * K, blocks = d / kActBlock;
+  if ((int)blockIdx.x < weight_blocks) {
+    weight_rows(blockIdx.x, wa, wb, w, v, offset, peaks, d, H);
+    return;
+  }
   const int sub = threadIdx.x & 7;
-  for (int64_t row = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3); row - (threadIdx.x >> 3) < rows;
-       row += (int64_t)gridDim.x * 32) {
+  for (int64_t row = (int64_t)(blockIdx.x - weight_blocks) * 32 + (threadIdx.x >> 3); row - (threadIdx.x >> 3) < rows;
+       row += (int64_t)(gridDim.x - weight_blocks) * 32) {
     const bool real = row < rows;
     float v[8 * K];
     float s = 0.f;
@@ -876,44 +896,30 @@ __global__ __launch_bounds__(4 * D, 2) void transition_grad_rows(
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the transfers past the last chunk
 }
 
-// The offsets in three bf16 parts each: split [2][H][8] = {hi, mid, lo, 0, ..}. block 256.
-__global__ __launch_bounds__(256) void split_offsets(const float* __restrict__ offset, bf16* __restrict__ split, int n) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  bf16x8 o;
-  float t = offset[i];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    o[e] = (bf16)(e < 3 ? t : 0.f);
-    t -= (float)o[e];
-  }
-  *reinterpret_cast<bf16x8*>(split + 8 * (int64_t)i) = o;
-}
-
 // dx = (residual ? dy : 0) + rstd (g - mean(g) - xh mean(g xh)), g the sum of `splits` fp32 parts [rows][d]: 8 lanes
-// a row, K = d / 64 pieces of 8 channels each. grid-strided; block 256 (32 rows).
+// a row, K = d / 64 pieces of 8 channels each. grid-strided; block 64 (8 rows: few rows still make many workgroups).
 template <int K>
-__global__ __launch_bounds__(256) void norm_grad_rows(const f16* __restrict__ xh, const float* __restrict__ rstd_in,
-                                                      const bf16* __restrict__ dy, const float* __restrict__ dxh,
-                                                      int splits, int64_t split_stride, bf16* __restrict__ dx,
-                                                      int64_t rows, int residual) {
+__global__ __launch_bounds__(64) void norm_grad_rows(const f16* __restrict__ xh, const float* __restrict__ rstd_in,
+                                                     const bf16* __restrict__ dy, const float* __restrict__ dxh,
+                                                     int splits, int64_t split_stride, bf16* __restrict__ dx,
+                                                     int64_t rows, int residual) {
   constexpr int d = 64 * K;
-  const int sub = threadIdx.x & 7;
-  for (int64_t row = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3); row - (threadIdx.x >> 3) < rows;
-       row += (int64_t)gridDim.x * 32) {
+  const int sub = threadIdx.x & 7, lead = threadIdx.x >> 3;
+  for (int64_t row = (int64_t)blockIdx.x * 8 + lead; row - lead < rows; row += (int64_t)gridDim.x * 8) {
     const bool real = row < rows;
     const int64_t at = (real ? row : rows - 1) * d + 8 * sub;
-    float t[8 * K], h[8 * K];
+    float t[8 * K];
+    f16x8 h[K];
     float sg = 0.f, sx = 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const f16x8 hv = ld8h(xh + at + 64 * k);
+    for (int k = 0; k < K; ++k) h[k] = ld8h(xh + at + 64 * k);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        h[8 * k + e] = (float)hv[e];
-        t[8 * k + e] = 0.f;
-      }
-      for (int i = 0; i < splits; ++i) {
+    for (int i = 0; i < 8 * K; ++i) t[i] = 0.f;
+    // (a part's pieces are all on their way together; the parts' order is fixed)
+#pragma unroll 2
+    for (int i = 0; i < splits; ++i) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
         const float* q = dxh + i * split_stride + at + 64 * k;
         const f32x4 lo = *reinterpret_cast<const f32x4*>(q), hi = *reinterpret_cast<const f32x4*>(q + 4);
 #pragma unroll
@@ -922,11 +928,11 @@ __global__ __launch_bounds__(256) void norm_grad_rows(const f16* __restrict__ xh
           t[8 * k + 4 + e] += hi[e];
         }
       }
+    }
 #pragma unroll
-      for (int e = 8 * k; e < 8 * k + 8; ++e) {
-        sg += t[e];
-        sx += t[e] * h[e];
-      }
+    for (int i = 0; i < 8 * K; ++i) {
+      sg += t[i];
+      sx += t[i] * (float)h[i / 8][i % 8];
     }
     const float c1 = lanes_sum<8>(sg) * (1.f / d), c2 = lanes_sum<8>(sx) * (1.f / d);
     if (!real) continue;
@@ -937,7 +943,7 @@ __global__ __launch_bounds__(256) void norm_grad_rows(const f16* __restrict__ xh
       bf16x8 o;
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        o[e] = (bf16)((residual ? (float)y[e] : 0.f) + rstd * (t[8 * k + e] - c1 - h[8 * k + e] * c2));
+        o[e] = (bf16)((residual ? (float)y[e] : 0.f) + rstd * (t[8 * k + e] - c1 - (float)h[k][e] * c2));
       *reinterpret_cast<bf16x8*>(dx + at + 64 * k) = o;
     }
   }
@@ -997,11 +1003,18 @@ __global__ __launch_bounds__(1024) void join_weight_grads(const float* __restric
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// weights: with the weights' rows (a call's first chunk).
 template <bool CODES>
-void run_norm_rows(const TransitionGradArgs& a, const void* x, const uint8_t* scales, int64_t rows, hipStream_t st) {
-  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(rows, 32), (int64_t)cu_count() * 16));
+void run_norm_rows(const TransitionGradArgs& a, const void* x, const uint8_t* scales, int64_t rows, bool weights,
+                   hipStream_t st) {
+  const int extra = weights ? 2 * a.hidden / 4 : 0;
+  const dim3 grid((unsigned)(extra + std::min<int64_t>(ceil_div(rows, 32), (int64_t)cu_count() * 16)));
   switch (a.d / 64) {
-#define FFK_K(K_) case K_: norm_rows<CODES, K_><<<grid, 256, 0, st>>>(x, scales, a.xh, a.xhb, a.rstd, rows, a.eps); break;
+#define FFK_K(K_)                                                                                                   \
+  case K_:                                                                                                          \
+    norm_rows<CODES, K_><<<grid, 256, 0, st>>>(x, scales, a.xh, a.xhb, a.rstd, rows, a.eps, extra, a.wa, a.wb, a.ln_w, \
+                                               a.ln_b, a.offset, a.peaks, a.hidden);                                \
+    break;
     FFK_K(1) FFK_K(2) FFK_K(3) FFK_K(4) FFK_K(5) FFK_K(6) FFK_K(7) FFK_K(8) FFK_K(9) FFK_K(10) FFK_K(11) FFK_K(12)
 #undef FFK_K
   }
@@ -1009,11 +1022,11 @@ void run_norm_rows(const TransitionGradArgs& a, const void* x, const uint8_t* sc
 
 void run_norm_grad_rows(const TransitionGradArgs& a, const bf16* dy, int splits, int64_t split_stride, bf16* dx,
                         int64_t rows, hipStream_t st) {
-  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(rows, 32), (int64_t)cu_count() * 16));
+  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(rows, 8), (int64_t)cu_count() * 32));
   switch (a.d / 64) {
 #define FFK_K(K_)                                                                                                 \
   case K_:                                                                                                        \
-    norm_grad_rows<K_><<<grid, 256, 0, st>>>(a.xh, a.rstd, dy, a.dxh, splits, split_stride, dx, rows, a.residual); \
+    norm_grad_rows<K_><<<grid, 64, 0, st>>>(a.xh, a.rstd, dy, a.dxh, splits, split_stride, dx, rows, a.residual); \
     break;
     FFK_K(1) FFK_K(2) FFK_K(3) FFK_K(4) FFK_K(5) FFK_K(6) FFK_K(7) FFK_K(8) FFK_K(9) FFK_K(10) FFK_K(11) FFK_K(12)
 #undef FFK_K
@@ -1037,7 +1050,7 @@ void launch_fused(const TransitionGradArgs& a, const TransitionGradPlan& p, cons
   rows_kernel<<<dim3((unsigned)std::min<int64_t>(tiles, (int64_t)cu_count() * held)), 64 * NW, grad_rows_lds<D>(H), st>>>(
       a.xh, dy, a.rstd, a.aw, a.st, a.abt, a.split, a.scale, dx, rows, H, a.residual);
   transition_grad_weights<D><<<dim3((unsigned)ceil_div(H, 128), (unsigned)p.dw_splits), 512, 0, st>>>(
-      a.xh, a.xhb, dy, a.aw, a.st, a.offset, a.scale, a.dw_part, a.sums, rows, H, add);
+      a.xh, a.xhb, dy, a.aw, a.st, a.shift, a.scale, a.dw_part, a.sums, rows, H, add);
 }
 
 }  // namespace
@@ -1045,7 +1058,6 @@ void launch_fused(const TransitionGradArgs& a, const TransitionGradPlan& p, cons
 TransitionGradPlan transition_grad_plan(int64_t rows, int d, int H) {
   TransitionGradPlan p{};
   const int64_t cus = cu_count();
-  p.peaks = 2 * kPeakBlocks;
   p.fused = fused_shape(d, H) && rows >= 4096;
   if (p.fused) {
     p.chunk = std::min<int64_t>(ceil_div(rows, 64) * 64, 1 << 18);
@@ -1064,12 +1076,6 @@ TransitionGradPlan transition_grad_plan(int64_t rows, int d, int H) {
 
 void launch_transition_grad(const TransitionGradArgs& a, const TransitionGradPlan& p, hipStream_t st) {
   const int d = a.d, H = a.hidden;
-  if (a.rows > 0) {
-    weight_peaks<<<dim3(kPeakBlocks, 2), 256, 0, st>>>(a.wa, a.wb, a.ln_w, a.peaks, d, H);
-    pack_grad_weights<<<dim3(H / 32, 3), 256, 0, st>>>(a.wa, a.wb, a.ws, a.ln_w, a.ln_b, a.peaks, a.aw, a.st, a.abt,
-                                                       a.offset, a.scale, d, H, p.fused);
-    if (p.fused) split_offsets<<<dim3((unsigned)ceil_div(2 * H, 256)), 256, 0, st>>>(a.offset, a.split, 2 * H);
-  }
   const char* x = static_cast<const char*>(a.x);
   for (int64_t r0 = 0; r0 < a.rows; r0 += p.chunk) {
     const int64_t rows = std::min(p.chunk, a.rows - r0);
@@ -1077,9 +1083,12 @@ void launch_transition_grad(const TransitionGradArgs& a, const TransitionGradPla
     const bf16* dy = a.dy + r0 * d;
     const int add = r0 > 0;
     if (a.scales)
-      run_norm_rows<true>(a, xc, a.scales + r0 * (d / kActBlock), rows, st);
+      run_norm_rows<true>(a, xc, a.scales + r0 * (d / kActBlock), rows, r0 == 0, st);
     else
-      run_norm_rows<false>(a, xc, nullptr, rows, st);
+      run_norm_rows<false>(a, xc, nullptr, rows, r0 == 0, st);
+    if (r0 == 0)
+      pack_grad_weights<<<dim3(H / 32, d / 32, 3), 256, 0, st>>>(a.wa, a.wb, a.ws, a.ln_w, a.peaks, a.offset, a.aw, a.st,
+                                                                 a.abt, a.shift, a.split, a.scale, d, H, p.fused);
     if (p.fused) {
       if (d == 64)
         launch_fused<64>(a, p, dy, a.dx + r0 * d, rows, add, st);
@@ -1087,7 +1096,7 @@ void launch_transition_grad(const TransitionGradArgs& a, const TransitionGradPla
         launch_fused<128>(a, p, dy, a.dx + r0 * d, rows, add, st);
       continue;
     }
-    hidden_grad<<<dim3((unsigned)ceil_div(rows, 64), H / 64), 256, 0, st>>>(a.xh, dy, a.aw, a.st, a.offset, a.scale, a.E,
+    hidden_grad<<<dim3((unsigned)ceil_div(rows, 64), H / 64), 256, 0, st>>>(a.xh, dy, a.aw, a.st, a.shift, a.scale, a.E,
                                                                             rows, d, H);
     Gemm64Args g{};
     g.A = a.E;
