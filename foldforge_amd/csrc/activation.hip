@@ -61,67 +61,67 @@ __global__ __launch_bounds__(256) void restore_pieces(const uint8_t* __restrict_
   }
 }
 
-// Any width and alignment: a half wave a block. grid-strided over blocks (row, block of the row), walked by
-// adding the stride's two digits; block 256 (8 blocks at once).
-struct BlockAt {
-  int64_t row;
-  int blk;
-};
-__device__ __forceinline__ BlockAt block_at(int64_t i, int blocks) {
-  return {i / blocks, (int)(i % blocks)};
-}
-__device__ __forceinline__ BlockAt block_add(BlockAt t, const BlockAt& step, int blocks) {
-  t.blk += step.blk;
-  const int carry = t.blk >= blocks ? 1 : 0;
-  t.blk -= carry * blocks;
-  t.row += step.row + carry;
-  return t;
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void quantize_blocks(const T* __restrict__ x, uint8_t* __restrict__ codes,
-                                                       uint8_t* __restrict__ scales, int64_t rows, int cols) {
-  const int blocks = (cols + kActBlock - 1) / kActBlock, sub = threadIdx.x & 31, lead = threadIdx.x >> 5;
-  const BlockAt step = block_at((int64_t)gridDim.x * 8, blocks);
-  BlockAt at[kActUnroll];
-  at[0] = block_at((int64_t)blockIdx.x * 8 * kActUnroll + lead, blocks);
-  const BlockAt eight = block_at(8, blocks);
+// Any width up to 64 K and any alignment: a wave a row, K values a lane (channels lane + 64 k: a block is half a wave).
+// grid-strided; block 256.
+template <typename T, int K>
+__global__ __launch_bounds__(256) void quantize_rows(const T* __restrict__ x, uint8_t* __restrict__ codes,
+                                                     uint8_t* __restrict__ scales, int64_t rows, int cols) {
+  const int blocks = (cols + kActBlock - 1) / kActBlock, lane = threadIdx.x & 63;
+  for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += (int64_t)gridDim.x * 4) {
+    float v[K];
 #pragma unroll
-  for (int u = 1; u < kActUnroll; ++u) at[u] = block_add(at[u - 1], eight, blocks);
-  // at[0] of the wave's first half is its least block: the loop ends for the whole wave when that is past
-  // the last row (the halves differ by one block, so both are asked)
-  while (__ballot(at[0].row < rows) != 0) {
-    float v[kActUnroll];
+    for (int k = 0; k < K; ++k) v[k] = lane + 64 * k < cols ? (float)x[row * cols + lane + 64 * k] : 0.f;
 #pragma unroll
-    for (int u = 0; u < kActUnroll; ++u) {
-      const int c = at[u].blk * kActBlock + sub;
-      v[u] = at[u].row < rows && c < cols ? (float)x[at[u].row * cols + c] : 0.f;
+    for (int k = 0; k < K; ++k) {
+      const int c = lane + 64 * k;
+      act_store<1>(&v[k], c < cols, c % kActBlock == 0, codes + row * cols + c, scales + row * blocks + c / kActBlock);
     }
+  }
+}
+template <typename T, int K>
+__global__ __launch_bounds__(256) void restore_rows(const uint8_t* __restrict__ codes,
+                                                    const uint8_t* __restrict__ scales, T* __restrict__ x, int64_t rows,
+                                                    int cols) {
+  const int blocks = (cols + kActBlock - 1) / kActBlock, lane = threadIdx.x & 63;
+  for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += (int64_t)gridDim.x * 4) {
+    KeptPiece<T, true, 1> v[K];
 #pragma unroll
-    for (int u = 0; u < kActUnroll; ++u) {
-      const int c = at[u].blk * kActBlock + sub;
-      act_store<1>(&v[u], at[u].row < rows && c < cols, sub == 0, codes + at[u].row * cols + c,
-                   scales + at[u].row * blocks + at[u].blk);
+    for (int k = 0; k < K; ++k)
+      if (lane + 64 * k < cols) v[k].load(codes, scales, row, lane + 64 * k, cols, blocks);
 #pragma unroll
-      for (int k = 0; k < kActUnroll; ++k) at[u] = block_add(at[u], step, blocks);
+    for (int k = 0; k < K; ++k) {
+      float f;
+      v[k].values(&f);
+      if (lane + 64 * k < cols) x[row * cols + lane + 64 * k] = (T)f;
     }
   }
 }
 
+// Wider rows: a wave takes 64 channels at a time.
 template <typename T>
-__global__ __launch_bounds__(256) void restore_blocks(const uint8_t* __restrict__ codes,
-                                                      const uint8_t* __restrict__ scales, T* __restrict__ x,
-                                                      int64_t rows, int cols) {
-  const int blocks = (cols + kActBlock - 1) / kActBlock, sub = threadIdx.x & 31, lead = threadIdx.x >> 5;
-  const BlockAt step = block_at((int64_t)gridDim.x * 8, blocks);
-  for (BlockAt at = block_at((int64_t)blockIdx.x * 8 + lead, blocks); at.row < rows; at = block_add(at, step, blocks)) {
-    const int c = at.blk * kActBlock + sub;
-    if (c < cols) {
+__global__ __launch_bounds__(256) void quantize_wide(const T* __restrict__ x, uint8_t* __restrict__ codes,
+                                                     uint8_t* __restrict__ scales, int64_t rows, int cols) {
+  const int blocks = (cols + kActBlock - 1) / kActBlock, lane = threadIdx.x & 63;
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    for (int c0 = 64 * (threadIdx.x >> 6); c0 < cols; c0 += 256) {  // (uniform in a wave)
+      const int c = c0 + lane;
+      const float v = c < cols ? (float)x[row * cols + c] : 0.f;
+      act_store<1>(&v, c < cols, c % kActBlock == 0, codes + row * cols + c, scales + row * blocks + c / kActBlock);
+    }
+  }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void restore_wide(const uint8_t* __restrict__ codes,
+                                                    const uint8_t* __restrict__ scales, T* __restrict__ x, int64_t rows,
+                                                    int cols) {
+  const int blocks = (cols + kActBlock - 1) / kActBlock;
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    for (int c = threadIdx.x; c < cols; c += 256) {
       KeptPiece<T, true, 1> k;
       float v;
-      k.load(codes, scales, at.row, c, cols, blocks);
+      k.load(codes, scales, row, c, cols, blocks);
       k.values(&v);
-      x[at.row * cols + c] = (T)v;
+      x[row * cols + c] = (T)v;
     }
   }
 }
@@ -139,9 +139,13 @@ void quantize_typed(const T* x, uint8_t* codes, uint8_t* scales, int64_t rows, i
     quantize_pieces<T, VE><<<grid, 256, 0, st>>>(x, codes, scales, pieces);
     return;
   }
-  const int64_t all = rows * ((cols + kActBlock - 1) / kActBlock), per = 8 * kActUnroll;
-  const dim3 grid((unsigned)std::min<int64_t>((all + per - 1) / per, (int64_t)cu_count() * 32));
-  quantize_blocks<T><<<grid, 256, 0, st>>>(x, codes, scales, rows, cols);
+  const dim3 grid((unsigned)std::min<int64_t>((rows + 3) / 4, (int64_t)cu_count() * 32));
+  if (cols <= 64) quantize_rows<T, 1><<<grid, 256, 0, st>>>(x, codes, scales, rows, cols);
+  else if (cols <= 128) quantize_rows<T, 2><<<grid, 256, 0, st>>>(x, codes, scales, rows, cols);
+  else if (cols <= 256) quantize_rows<T, 4><<<grid, 256, 0, st>>>(x, codes, scales, rows, cols);
+  else if (cols <= 512) quantize_rows<T, 8><<<grid, 256, 0, st>>>(x, codes, scales, rows, cols);
+  else if (cols <= 1024) quantize_rows<T, 16><<<grid, 256, 0, st>>>(x, codes, scales, rows, cols);
+  else quantize_wide<T><<<dim3((unsigned)std::min<int64_t>(rows, (int64_t)cu_count() * 8)), 256, 0, st>>>(x, codes, scales, rows, cols);
 }
 
 template <typename T>
@@ -153,9 +157,13 @@ void restore_typed(const uint8_t* codes, const uint8_t* scales, T* x, int64_t ro
     restore_pieces<T, VE><<<grid, 256, 0, st>>>(codes, scales, x, pieces);
     return;
   }
-  const int64_t all = rows * ((cols + kActBlock - 1) / kActBlock);
-  const dim3 grid((unsigned)std::min<int64_t>((all + 7) / 8, (int64_t)cu_count() * 32));
-  restore_blocks<T><<<grid, 256, 0, st>>>(codes, scales, x, rows, cols);
+  const dim3 grid((unsigned)std::min<int64_t>((rows + 3) / 4, (int64_t)cu_count() * 32));
+  if (cols <= 64) restore_rows<T, 1><<<grid, 256, 0, st>>>(codes, scales, x, rows, cols);
+  else if (cols <= 128) restore_rows<T, 2><<<grid, 256, 0, st>>>(codes, scales, x, rows, cols);
+  else if (cols <= 256) restore_rows<T, 4><<<grid, 256, 0, st>>>(codes, scales, x, rows, cols);
+  else if (cols <= 512) restore_rows<T, 8><<<grid, 256, 0, st>>>(codes, scales, x, rows, cols);
+  else if (cols <= 1024) restore_rows<T, 16><<<grid, 256, 0, st>>>(codes, scales, x, rows, cols);
+  else restore_wide<T><<<dim3((unsigned)std::min<int64_t>(rows, (int64_t)cu_count() * 8)), 256, 0, st>>>(codes, scales, x, rows, cols);
 }
 
 }  // namespace

@@ -296,7 +296,7 @@ TransitionGradArgs transition_grad_ws(void* ws, size_t* bytes, const TransitionG
   a.dxh = cv.take<float>((size_t)p.dxh_splits * p.chunk * d);
   a.dw_part = cv.take<float>((size_t)p.dw_splits * 3 * w);
   a.sums = cv.take<float>((size_t)p.dw_splits * 2 * hidden);
-  a.norm_part = cv.take<float>((size_t)hidden / 16 * 2 * d);
+  a.norm_part = cv.take<float>((size_t)hidden / 4 * 2 * d);
   *bytes = cv.used;
   return a;
 }

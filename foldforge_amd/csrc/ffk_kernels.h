@@ -438,7 +438,7 @@ struct TransitionGradArgs {
   f16* xh;                              // [chunk][d]
   bf16 *xhb, *E;                        // [chunk][d], [chunk][3 hidden]
   float *rstd, *dxh;                    // [chunk], [dxh_splits][chunk][d]
-  float *dw_part, *sums, *norm_part;    // [dw_splits][3 hidden][d], [dw_splits][2 hidden], [hidden / 16][2][d]
+  float *dw_part, *sums, *norm_part;    // [dw_splits][3 hidden][d], [dw_splits][2 hidden], [hidden / 4][2][d]
 };
 void launch_transition_grad(const TransitionGradArgs& a, const TransitionGradPlan& p, hipStream_t stream);
 

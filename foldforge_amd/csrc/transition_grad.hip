@@ -896,72 +896,57 @@ __global__ __launch_bounds__(4 * D, 2) void transition_grad_rows(
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the transfers past the last chunk
 }
 
-// dx = (residual ? dy : 0) + rstd (g - mean(g) - xh mean(g xh)), g the sum of `splits` fp32 parts [rows][d]: 8 lanes
-// a row, K = d / 64 pieces of 8 channels each. grid-strided; block 64 (8 rows: few rows still make many workgroups).
+// dx = (residual ? dy : 0) + rstd (g - mean(g) - xh mean(g xh)), g the sum of `splits` fp32 parts [rows][d]: a wave a row,
+// K = d / 64 channels a lane. grid-strided; block 64 (few rows still make many workgroups).
 template <int K>
 __global__ __launch_bounds__(64) void norm_grad_rows(const f16* __restrict__ xh, const float* __restrict__ rstd_in,
                                                      const bf16* __restrict__ dy, const float* __restrict__ dxh,
                                                      int splits, int64_t split_stride, bf16* __restrict__ dx,
                                                      int64_t rows, int residual) {
   constexpr int d = 64 * K;
-  const int sub = threadIdx.x & 7, lead = threadIdx.x >> 3;
-  for (int64_t row = (int64_t)blockIdx.x * 8 + lead; row - lead < rows; row += (int64_t)gridDim.x * 8) {
-    const bool real = row < rows;
-    const int64_t at = (real ? row : rows - 1) * d + 8 * sub;
-    float t[8 * K];
-    f16x8 h[K];
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const int64_t at = row * d + threadIdx.x;
+    float t[K], h[K], y[K];
     float sg = 0.f, sx = 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k) h[k] = ld8h(xh + at + 64 * k);
-#pragma unroll
-    for (int i = 0; i < 8 * K; ++i) t[i] = 0.f;
-    // (a part's pieces are all on their way together; the parts' order is fixed)
-#pragma unroll 2
+    for (int k = 0; k < K; ++k) {
+      h[k] = (float)xh[at + 64 * k];
+      y[k] = residual ? (float)dy[at + 64 * k] : 0.f;
+      t[k] = 0.f;
+    }
+    const float rstd = rstd_in[row];
+    // (some parts' values are on their way together; the parts' order is fixed)
+#pragma unroll 4
     for (int i = 0; i < splits; ++i) {
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const float* q = dxh + i * split_stride + at + 64 * k;
-        const f32x4 lo = *reinterpret_cast<const f32x4*>(q), hi = *reinterpret_cast<const f32x4*>(q + 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          t[8 * k + e] += lo[e];
-          t[8 * k + 4 + e] += hi[e];
-        }
-      }
+      for (int k = 0; k < K; ++k) t[k] += dxh[i * split_stride + at + 64 * k];
     }
-#pragma unroll
-    for (int i = 0; i < 8 * K; ++i) {
-      sg += t[i];
-      sx += t[i] * (float)h[i / 8][i % 8];
-    }
-    const float c1 = lanes_sum<8>(sg) * (1.f / d), c2 = lanes_sum<8>(sx) * (1.f / d);
-    if (!real) continue;
-    const float rstd = rstd_in[row];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const bf16x8 y = ld8(dy + at + 64 * k);
-      bf16x8 o;
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        o[e] = (bf16)((residual ? (float)y[e] : 0.f) + rstd * (t[8 * k + e] - c1 - (float)h[k][e] * c2));
-      *reinterpret_cast<bf16x8*>(dx + at + 64 * k) = o;
+      sg += t[k];
+      sx += t[k] * h[k];
     }
+    const float c1 = lanes_sum<64>(sg) * (1.f / d), c2 = lanes_sum<64>(sx) * (1.f / d);
+#pragma unroll
+    for (int k = 0; k < K; ++k) dx[at + 64 * k] = (bf16)(y[k] + rstd * (t[k] - c1 - h[k] * c2));
   }
 }
 
 // The weights' gradients from `count` parts G [3 H][d] (da'^T xh, db'^T xh, u'^T dy) and sums [2 H] (of da', db'), and
-// the rows' shares of the affine's: part [2 H / 32][2][d]. A 32 x 32 tile a workgroup: grid (d / 32, 3 H / 32);
-// block 1024.
-__global__ __launch_bounds__(1024) void join_weight_grads(const float* __restrict__ G, const float* __restrict__ sums,
+// eight hidden channels' shares of the affine's: part [2 H / 8][2][d]. A workgroup: 32 channels x 8 hidden channels, in Q
+// shares of the parts (0, Q, 2 Q, ..; joined in LDS in that order). grid (d / 32, 3 H / 8); block 256 Q.
+template <int Q>
+__global__ __launch_bounds__(256 * Q) void join_weight_grads(const float* __restrict__ G, const float* __restrict__ sums,
                                                           int count, const float* __restrict__ wa,
                                                           const float* __restrict__ wb, const float* __restrict__ w,
                                                           const float* __restrict__ v, const float* __restrict__ scale,
                                                           float* __restrict__ part, int d, int H, void* da, void* db,
                                                           void* ds, int dtype) {
-  __shared__ float tile[32][33], tile2[32][33];
-  const int c0 = blockIdx.x * 32, h0 = blockIdx.y * 32;
-  const int col = threadIdx.x & 31, row = threadIdx.x >> 5;
+  __shared__ float share[2][Q][8][33], tile[2][8][33];
+  const int c0 = blockIdx.x * 32, h0 = blockIdx.y * 8;
+  const int col = threadIdx.x & 31, row = (threadIdx.x >> 5) & 7, quarter = threadIdx.x >> 8;
   const int64_t size = (int64_t)3 * H * d;
+  const bool summed = h0 < 2 * H;
   const auto put = [&](void* to, int64_t at, float t) __attribute__((always_inline)) {
     if (dtype == 0)
       static_cast<bf16*>(to)[at] = (bf16)t;
@@ -969,19 +954,28 @@ __global__ __launch_bounds__(1024) void join_weight_grads(const float* __restric
       static_cast<float*>(to)[at] = t;
   };
   const float* p = G + (int64_t)(h0 + row) * d + c0 + col;
-  float t = 0.f;
+  float t = 0.f, total = 0.f;
 #pragma unroll 8
-  for (int k = 0; k < count; ++k) t += p[k * size];
-  if (h0 >= 2 * H) {
-    tile[row][col] = count ? t * (scale[0] * scale[1]) : 0.f;
-    __syncthreads();
-    put(ds, (int64_t)(c0 + row) * H + h0 - 2 * H + col, tile[col][row]);
+  for (int k = quarter; k < count; k += Q) t += p[k * size];
+  if (summed && col < 4) {  // (the sums' parts: a share over four lanes)
+#pragma unroll 4
+    for (int k = quarter + Q * col; k < count; k += 4 * Q) total += sums[(int64_t)k * 2 * H + h0 + row];
+  }
+  share[0][quarter][row][col] = t;
+  share[1][quarter][row][col] = total;
+  __syncthreads();
+  if (quarter) return;
+  t = 0.f;
+#pragma unroll
+  for (int i = 0; i < Q; ++i) t += share[0][i][row][col];
+  if (!summed) {
+    // 8 hidden channels of a row of dS: 16 or 32 bytes
+    put(ds, (int64_t)(c0 + col) * H + h0 - 2 * H + row, count ? t * (scale[0] * scale[1]) : 0.f);
     return;
   }
-  // (32 hidden channels' sums: every thread of a row adds the same ones)
-  float total = 0.f;
-#pragma unroll 8
-  for (int k = 0; k < count; ++k) total += sums[(int64_t)k * 2 * H + h0 + row];
+  total = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4 * Q; ++i) total += share[1][i >> 2][row][i & 3];
   const bool first = h0 < H;
   const float back = count ? scale[first ? 1 : 0] : 0.f;
   t *= back;
@@ -989,15 +983,15 @@ __global__ __launch_bounds__(1024) void join_weight_grads(const float* __restric
   const int64_t at = (int64_t)(h0 + row - (first ? 0 : H)) * d + c0 + col;
   put(first ? da : db, at, t * w[c0 + col] + total * v[c0 + col]);
   const float own = (first ? wa : wb)[at];
-  tile[row][col] = own * t;
-  tile2[row][col] = own * total;
+  tile[0][row][col] = own * t;
+  tile[1][row][col] = own * total;
   __syncthreads();
   if (threadIdx.x < 64) {
-    const float(*from)[33] = threadIdx.x < 32 ? tile : tile2;
+    const int which = threadIdx.x >> 5;
     float r = 0.f;
 #pragma unroll
-    for (int k = 0; k < 32; ++k) r += from[k][col];
-    part[((int64_t)blockIdx.y * 2 + (threadIdx.x >> 5)) * d + c0 + col] = r;
+    for (int k = 0; k < 8; ++k) r += tile[which][k][col];
+    part[((int64_t)blockIdx.y * 2 + which) * d + c0 + col] = r;
   }
 }
 
@@ -1022,7 +1016,7 @@ void run_norm_rows(const TransitionGradArgs& a, const void* x, const uint8_t* sc
 
 void run_norm_grad_rows(const TransitionGradArgs& a, const bf16* dy, int splits, int64_t split_stride, bf16* dx,
                         int64_t rows, hipStream_t st) {
-  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(rows, 8), (int64_t)cu_count() * 32));
+  const dim3 grid((unsigned)std::min<int64_t>(rows, (int64_t)cu_count() * 64));
   switch (a.d / 64) {
 #define FFK_K(K_)                                                                                                 \
   case K_:                                                                                                        \
@@ -1131,10 +1125,16 @@ void launch_transition_grad(const TransitionGradArgs& a, const TransitionGradPla
     gemm64<true><<<dim3(3 * H / 64, d / 64, p.dw_splits), 256, 0, st>>>(t);
   }
   // (no rows: sums over nothing)
-  join_weight_grads<<<dim3(d / 32, 3 * H / 32), 1024, 0, st>>>(a.dw_part, a.sums, a.rows > 0 ? p.dw_splits : 0, a.wa,
-                                                               a.wb, a.ln_w, a.ln_b, a.scale, a.norm_part, d, H, a.dwa,
-                                                               a.dwb, a.dws, a.grad_dtype);
-  launch_sum_partials(a.norm_part, a.rows > 0 ? 2 * H / 32 : 0, 2 * d, d, a.dln_w, a.dln_b, a.grad_dtype, st);
+  const int parts = a.rows > 0 ? p.dw_splits : 0;
+  const auto join = [&](auto kernel, int q) {
+    kernel<<<dim3(d / 32, 3 * H / 8), 256 * q, 0, st>>>(a.dw_part, a.sums, parts, a.wa, a.wb, a.ln_w, a.ln_b, a.scale,
+                                                       a.norm_part, d, H, a.dwa, a.dwb, a.dws, a.grad_dtype);
+  };
+  if (parts >= 16)
+    join(join_weight_grads<4>, 4);
+  else
+    join(join_weight_grads<1>, 1);
+  launch_sum_partials(a.norm_part, a.rows > 0 ? 2 * H / 8 : 0, 2 * d, d, a.dln_w, a.dln_b, a.grad_dtype, st);
 }
 
 }  // namespace ffk
