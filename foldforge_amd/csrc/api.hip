@@ -584,7 +584,7 @@ int32_t ffk_layer_norm_backward(const void* dy, const void* x, const void* scale
   if (grad_dtype != FFK_DTYPE_BF16 && grad_dtype != FFK_DTYPE_F32)
     return fail(FFK_ERR_INVALID, "layer_norm_backward: gradient dtype %d is neither bf16 nor fp32", grad_dtype);
   const size_t need = ffk_layer_norm_backward_workspace(rows, cols);
-  if (!workspace || workspace_bytes < need || !aligned16(workspace))
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(FFK_ERR_WORKSPACE, "layer_norm_backward: workspace %zu bytes < %zu", workspace_bytes, need);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   LayerNormGradArgs a{};

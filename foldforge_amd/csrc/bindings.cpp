@@ -3,6 +3,7 @@
 // microsecond of host time where ctypes with 25 to 30 arguments takes eight. Checks stay in
 // kernels.py; the one that runs over every parameter of every call (device, dtype, layout,
 // shape) is params_ok below.
+#include <ATen/ops/empty.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -91,9 +92,48 @@ PyObject* params_ok(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// empties(tensor, ((shape, kind), ...)): new tensors on the tensor's device, kind 0 bf16, 1 fp32, 2 uint8, 3 e4m3 (a
+// call's outputs and workspace in one step: four torch.empty cost 5 us of the caller's time).
+PyObject* empties(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  static constexpr at::ScalarType kKinds[] = {at::kBFloat16, at::kFloat, at::kByte, at::kFloat8_e4m3fn};
+  if (n != 2 || !THPVariable_Check(args[0]) || !PyTuple_Check(args[1]))
+    return PyErr_Format(PyExc_TypeError, "empties(tensor, tuple of (shape, kind))");
+  const at::TensorOptions options = at::TensorOptions().device(THPVariable_Unpack(args[0]).device());
+  const Py_ssize_t count = PyTuple_GET_SIZE(args[1]);
+  PyObject* out = PyTuple_New(count);
+  if (out == nullptr) return nullptr;
+  for (Py_ssize_t i = 0; i < count; ++i) {
+    PyObject* spec = PyTuple_GET_ITEM(args[1], i);
+    PyObject* shape = PyTuple_Check(spec) && PyTuple_GET_SIZE(spec) == 2 ? PyTuple_GET_ITEM(spec, 0) : nullptr;
+    const long kind = shape ? PyLong_AsLong(PyTuple_GET_ITEM(spec, 1)) : -1;
+    if (shape == nullptr || !PyTuple_Check(shape) || kind < 0 || kind > 3) {
+      Py_DECREF(out);
+      return PyErr_Occurred() ? nullptr : PyErr_Format(PyExc_TypeError, "empties: (shape, kind), kind 0 to 3");
+    }
+    c10::SmallVector<int64_t, 6> sizes;
+    for (Py_ssize_t k = 0; k < PyTuple_GET_SIZE(shape); ++k) {
+      sizes.push_back(PyLong_AsLongLong(PyTuple_GET_ITEM(shape, k)));
+      if (sizes.back() < 0) {
+        Py_DECREF(out);
+        return PyErr_Occurred() ? nullptr : PyErr_Format(PyExc_ValueError, "empties: negative size");
+      }
+    }
+    try {
+      PyTuple_SET_ITEM(out, i, THPVariable_Wrap(at::empty(sizes, options.dtype(kKinds[kind]))));
+    } catch (...) {
+      Py_DECREF(out);
+      throw;
+    }
+  }
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
 #define FFK_CALL(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&Call<&name>::run)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     {"params_ok", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&params_ok)), METH_FASTCALL, nullptr},
+    {"empties", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&empties)), METH_FASTCALL, nullptr},
     FFK_CALL(ffk_layer_norm),
     FFK_CALL(ffk_layer_norm_linear),
     FFK_CALL(ffk_swiglu_ffn_workspace),

@@ -484,10 +484,12 @@ RowForm grad_form(const LayerNormGradArgs& a) {
 }  // namespace
 
 // The workspace holds the partial sums of whichever form the call takes: single values make the most
-// workgroups of few rows each (a step of 4 rows), and the wide rows' statistics come behind the sums.
+// workgroups of few rows each (a step of 4 rows: up to 4 rows are one workgroup, which needs none), and the wide
+// rows' statistics come behind the sums.
 size_t layer_norm_grad_floats(int64_t rows, int cols) {
-  const int64_t parts = cols > 1024 ? 64 : std::min<int64_t>((rows + 3) / 4, (int64_t)cu_count() * kGradBlocksPerCu);
-  return (size_t)parts * 2 * cols + (cols > 1024 ? 2 * (size_t)rows : 0);
+  if (cols > 1024) return (size_t)64 * 2 * cols + 2 * (size_t)rows;
+  const int64_t parts = std::min<int64_t>((rows + 3) / 4, (int64_t)cu_count() * kGradBlocksPerCu);
+  return parts <= 1 ? 0 : (size_t)parts * 2 * cols;
 }
 
 void launch_sum_partials(const float* part, int count, int width, int split, void* out0, void* out1, int dtype,

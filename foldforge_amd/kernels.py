@@ -268,7 +268,7 @@ def _dtype_code(dtype: torch.dtype) -> int:
 
 def _rows_tensor(x: Tensor, name: str) -> int:
     """The rows of a contiguous bf16 / fp32 device tensor with a last axis."""
-    if not (isinstance(x, Tensor) and _on_device(x) and x.is_contiguous()):
+    if not (isinstance(x, Tensor) and (x.is_cuda or _on_device(x)) and x.is_contiguous()):
         _refuse(f"{name} must be a contiguous device tensor")
     if x.dtype not in (torch.bfloat16, torch.float32):
         _refuse(f"{name} must be bf16 or fp32 (got {x.dtype})")
@@ -277,10 +277,13 @@ def _rows_tensor(x: Tensor, name: str) -> int:
     return x.numel() // x.shape[-1]
 
 
-def _new_activation(x: Tensor) -> Activation8:
-    blocks = -(-x.shape[-1] // ACTIVATION_BLOCK)
-    return Activation8(torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device),
-                       torch.empty((*x.shape[:-1], blocks), dtype=torch.uint8, device=x.device), x.dtype)
+#: kinds of :func:`_native.calls`'s ``empties``
+_BF16, _F32, _U8, _E4M3 = 0, 1, 2, 3
+
+
+def _activation_spec(x: Tensor) -> tuple:
+    shape = tuple(x.shape)
+    return (shape, _E4M3), ((*shape[:-1], -(-shape[-1] // ACTIVATION_BLOCK)), _U8)
 
 
 def _check_activation(a: Activation8, name: str) -> None:
@@ -298,7 +301,7 @@ def _check_activation(a: Activation8, name: str) -> None:
 def quantize_activation(x: Tensor) -> Activation8:
     """``x [..., c]`` (bf16 or fp32) in 8 bits."""
     rows = _rows_tensor(x, "x")
-    a = _new_activation(x)
+    a = Activation8(*_native.calls().empties(x, _activation_spec(x)), x.dtype)
     if rows:
         _call(x.device, "quantize_activation", x, a.codes, a.scales, rows, x.shape[-1], _dtype_code(x.dtype))
     return a
@@ -324,7 +327,8 @@ def layer_norm_checkpoint(x: Tensor, weight: Tensor | None, bias: Tensor | None,
     (rows of at most 1024 channels; two for wider ones)."""
     rows, cols = _rows_tensor(x, "x"), x.shape[-1]
     weight, bias = _affine(weight, x.device, "weight", cols), _affine(bias, x.device, "bias", cols)
-    y, a = torch.empty_like(x), _new_activation(x)
+    y, codes, scales = _native.calls().empties(x, ((tuple(x.shape), _dtype_code(x.dtype)), *_activation_spec(x)))
+    a = Activation8(codes, scales, x.dtype)
     if rows:
         _call(x.device, "layer_norm_checkpoint", x, weight, bias, y, a.codes, a.scales, rows, cols, float(eps),
               _dtype_code(x.dtype))
@@ -361,10 +365,12 @@ def layer_norm_backward(dy: Tensor, x: Tensor | Activation8, weight: Tensor | No
     kept, scales = _kept(x, dy)
     weight = _affine(weight, dev, "weight", cols)
     code = _grad_dtype(grad_dtype)
-    dx = torch.empty_like(dy)
-    dweight = None if weight is None else torch.empty(cols, dtype=grad_dtype, device=dev)
-    dbias = torch.empty(cols, dtype=grad_dtype, device=dev) if with_bias else None
-    ws = _workspace(_native.calls().ffk_layer_norm_backward_workspace(rows, cols), dev)
+    lib = _native.calls()
+    dx, ws, *sums = lib.empties(dy, (
+        (tuple(dy.shape), _dtype_code(dy.dtype)), ((lib.ffk_layer_norm_backward_workspace(rows, cols),), _U8),
+        *(((cols,), code),) * ((weight is not None) + with_bias)))
+    dweight = None if weight is None else sums[0]
+    dbias = sums[-1] if with_bias else None
     _call(dev, "layer_norm_backward", dy, kept, scales, weight, dx, dweight, dbias, ws, ws.numel(), rows, cols,
           float(eps), _dtype_code(dy.dtype), code)
     return dx, dweight, dbias
@@ -585,9 +591,10 @@ def transition_backward(
     for t, name in ((dy, "dy"), (kept, "x")):
         if t.data_ptr() % 16:
             _refuse(f"{name} must be 16-byte aligned")
-    grads = TransitionGradients(torch.empty_like(dy), *(torch.empty(shape, dtype=grad_dtype, device=dev)
-                                                        for shape in shapes.values()))
-    ws = _workspace(_native.calls().ffk_transition_backward_workspace(rows, d, factor), dev)
+    lib = _native.calls()
+    ws, *grads = lib.empties(dy, (((lib.ffk_transition_backward_workspace(rows, d, factor),), _U8),
+                                  (tuple(dy.shape), _BF16), *((shape, code) for shape in shapes.values())))
+    grads = TransitionGradients(*grads)
     _call(dev, "transition_backward", dy, kept, scales, *ps, *grads, ws, ws.numel(), rows, d, factor, int(residual),
           float(eps), code)
     return grads

@@ -30,7 +30,7 @@ from typing import Any
 import torch
 from torch import nn
 
-from foldforge_amd import dispatch, kernels, torch_ops
+from foldforge_amd import dispatch, kernels, torch_ops, training
 
 Tensor = torch.Tensor
 
@@ -201,6 +201,10 @@ class LayerNorm(EngineOp, nn.LayerNorm):
     """The engine LayerNorm: fp32 affine under any cast, output in the input dtype
     (``src/foldforge/modules/engine/modules.py:230-238``)."""
 
+    #: what a differentiated ``hip`` call keeps of its input (:func:`foldforge_amd.training.install`; None: the
+    #: ``hip`` backend does not differentiate)
+    keep: str | None = None
+
     def __init__(self, normalized_shape, eps: float = 1e-5, bias: bool = True,
                  elementwise_affine: bool = True, backend: str = "pytorch") -> None:
         nn.LayerNorm.__init__(self, normalized_shape, eps=eps,
@@ -230,6 +234,8 @@ class LayerNorm(EngineOp, nn.LayerNorm):
         return torch_ops.layer_norm(self, x)
 
     def _forward_hip(self, x: Tensor) -> Tensor:
+        if training.wanted(self, x):
+            return training.layer_norm(x, self.weight, self.bias, self.eps, keep=self.keep)
         return kernels.layer_norm(x.contiguous(), self.weight, self.bias, self.eps)
 
 
@@ -435,6 +441,9 @@ class Transition(EngineOp, MasterWeights, nn.Module):
     """SwiGLU transition, residual included (``legacy/reference/transition.py:28-59``;
     parameters ``legacy/released.py:211-224``)."""
 
+    #: what a differentiated ``hip`` call keeps of its input (as :class:`LayerNorm`)
+    keep: str | None = None
+
     def __init__(self, d_hidden: int, n: int = 4, backend: str = "pytorch") -> None:
         nn.Module.__init__(self)
         self.d, self.n = d_hidden, n
@@ -453,6 +462,8 @@ class Transition(EngineOp, MasterWeights, nn.Module):
         if not kernels.transition_supported(self.d, self.n):
             return (f"width {self.d} x {self.n} (the kernels take 128 x 4, or d and "
                     "n * d multiples of 64)")
+        if training.wanted(self, x) and not kernels.transition_backward_supported(self.d, self.n):
+            return f"width {self.d} x {self.n} (the backward kernels take a multiple of 64 up to 768, factor up to 64)"
         return None
 
     def _forward_pytorch(self, x: Tensor, *, residual: bool = True) -> Tensor:
@@ -463,6 +474,9 @@ class Transition(EngineOp, MasterWeights, nn.Module):
     def _forward_hip(self, x: Tensor, *, residual: bool = True) -> Tensor:
         if self.dead:
             return x if residual else torch.zeros_like(x)
+        if training.wanted(self, x):
+            return training.transition(x, residual=residual, eps=self.ln_in.eps, keep=self.keep,
+                                       **_read(self, _TRANSITION))
         return kernels.transition(
             x.contiguous(), residual=residual, eps=self.ln_in.eps, **_read(self, _TRANSITION))
 
@@ -682,7 +696,8 @@ def attention_then_transition(att: "TriangleAttention", tr: "Transition", z: Ten
     (``kernels.triangle_attention_transition``: the same results, the attention output never
     written). Each op is routed (refusal policy, ledger) exactly as its own call would be."""
     b_att = att._route((z, mask), {})
-    if b_att == "hip" and fuse and _fused_attention_transition(att, tr):
+    # (a transition that is to be differentiated runs by itself: it keeps its input)
+    if b_att == "hip" and fuse and _fused_attention_transition(att, tr) and not training.wanted(tr, z):
         # the transition's refusal reasons (device, dtype, width) read the same on z as on the
         # attention's output, which has z's shape, dtype and device
         b_tr = tr._route((z,), {})

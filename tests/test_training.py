@@ -1,0 +1,169 @@
+"""The training operators on the host: what :mod:`foldforge_amd.kernels` and :mod:`foldforge_amd.training` refuse, the
+sizes the library asks for, and what ``install`` makes of a model. Nothing here reaches a device."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from foldforge_amd import _native, build, factories, kernels, modules, training
+from foldforge_amd.trunk import randomise
+
+BF16 = torch.bfloat16
+
+
+@pytest.fixture
+def cpu_checks(monkeypatch):
+    monkeypatch.setattr(kernels, "DEVICE_TYPE", "cpu")
+
+    def refuse_native():
+        raise AssertionError("an argument check let a bad call reach the library")
+
+    monkeypatch.setattr(kernels._native, "lib", refuse_native)
+    monkeypatch.setattr(kernels._native, "calls", refuse_native)
+
+
+def _activation(rows=4, cols=40, dtype=BF16, **change):
+    parts = dict(codes=torch.zeros(rows, cols, dtype=torch.float8_e4m3fn),
+                 scales=torch.zeros(rows, -(-cols // 32), dtype=torch.uint8), dtype=dtype)
+    return kernels.Activation8(**{**parts, **change})
+
+
+@pytest.mark.parametrize("x,match", [
+    (torch.zeros(4, 8, dtype=torch.float16), "bf16 or fp32"),
+    (torch.zeros(4, 8).t(), "contiguous"),
+    (torch.tensor(1.0), "last axis"),
+    (torch.zeros(4, 0), "last axis"),
+    (None, "contiguous device tensor"),
+])
+def test_quantize_refuses(cpu_checks, x, match):
+    with pytest.raises(ValueError, match=match):
+        kernels.quantize_activation(x)
+    with pytest.raises(ValueError, match=match):
+        kernels.layer_norm_checkpoint(x, None, None)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(codes=torch.zeros(4, 40, dtype=torch.uint8)), "codes"),
+    (dict(scales=torch.zeros(4, 1, dtype=torch.uint8)), "scales"),
+    (dict(scales=torch.zeros(4, 2)), "scales"),
+    (dict(scales=torch.zeros(2, 4, dtype=torch.uint8).t()), "scales"),
+    (dict(dtype=torch.float16), "dtype"),
+])
+def test_a_bad_activation_is_refused(cpu_checks, change, match):
+    a = _activation(**change)
+    with pytest.raises(ValueError, match=match):
+        kernels.restore_activation(a)
+    with pytest.raises(ValueError, match=match):
+        kernels.layer_norm_backward(torch.zeros(4, 40, dtype=BF16), a)
+
+
+def test_restore_refuses_a_bad_out(cpu_checks):
+    for out, match in ((torch.zeros(4, 41, dtype=BF16), "shape"), (torch.zeros(4, 40), "must be"),
+                       (torch.zeros(40, 4, dtype=BF16).t(), "contiguous")):
+        with pytest.raises(ValueError, match=match):
+            kernels.restore_activation(_activation(), out=out)
+
+
+def test_layer_norm_backward_refuses(cpu_checks):
+    dy = torch.zeros(4, 40, dtype=BF16)
+    for x in (torch.zeros(4, 41, dtype=BF16), torch.zeros(4, 40), torch.zeros(5, 40, dtype=BF16),
+              _activation(cols=41), _activation(dtype=torch.float32)):
+        with pytest.raises(ValueError, match="not like x"):
+            kernels.layer_norm_backward(dy, x)
+    with pytest.raises(ValueError, match="weight"):
+        kernels.layer_norm_backward(dy, dy, torch.ones(41))
+    with pytest.raises(ValueError, match="fp32"):
+        kernels.layer_norm_backward(dy, dy, torch.ones(40, dtype=BF16))
+    with pytest.raises(ValueError, match="grad_dtype"):
+        kernels.layer_norm_backward(dy, dy, torch.ones(40), grad_dtype=torch.float16)
+
+
+def _params(d=64, h=128, **change):
+    return {**dict(ln_weight=torch.ones(d), ln_bias=torch.zeros(d), expand_a=torch.zeros(h, d),
+                   expand_b=torch.zeros(h, d), squeeze=torch.zeros(d, h)), **change}
+
+
+def test_transition_backward_refuses(cpu_checks):
+    x = torch.zeros(4, 64, dtype=BF16)
+    for change, match in ((dict(squeeze=torch.zeros(128, 64)), "squeeze"), (dict(ln_weight=torch.ones(65)), "ln_weight"),
+                          (dict(expand_b=torch.zeros(64, 64)), "expand_b"), (dict(ln_bias=None), "ln_bias"),
+                          (dict(expand_a=torch.zeros(128, 64, dtype=BF16)), "expand_a"),
+                          (dict(expand_a=torch.zeros(32, 64)), "width")):
+        with pytest.raises(ValueError, match=match):
+            kernels.transition_backward(x, x, **_params(**change))
+    for d in (32, 96, 832):
+        t = torch.zeros(4, d, dtype=BF16)
+        with pytest.raises(ValueError, match="width"):
+            kernels.transition_backward(t, t, **_params(d, 4 * d))
+    with pytest.raises(ValueError, match="bf16"):
+        kernels.transition_backward(x.float(), x.float(), **_params())
+    with pytest.raises(ValueError, match="not like x"):
+        kernels.transition_backward(x, torch.zeros(5, 64, dtype=BF16), **_params())
+    with pytest.raises(ValueError, match="grad_dtype"):
+        kernels.transition_backward(x, x, **_params(), grad_dtype=torch.float64)
+    odd = torch.zeros(1 + 4 * 64, dtype=BF16)[1:].view(4, 64)
+    with pytest.raises(ValueError, match="aligned"):
+        kernels.transition_backward(x, odd, **_params())
+
+
+def test_functions_refuse_a_bad_keep_and_a_capturing_stream(monkeypatch):
+    x = torch.zeros(4, 64, dtype=BF16)
+    with pytest.raises(ValueError, match="keep"):
+        training.layer_norm(x, None, None, keep="4bit")
+    with pytest.raises(ValueError, match="keep"):
+        training.install(factories.layer_norm(64), "4bit")
+    with pytest.raises(ValueError, match="width"):
+        training.transition(torch.zeros(4, 96, dtype=BF16), **_params(96, 192))
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    for call in (lambda: training.layer_norm(x, None, None), lambda: training.transition(x, **_params())):
+        with pytest.raises(RuntimeError, match="capture"):
+            call()
+
+
+def test_workspaces():
+    if not build.LIBRARY.exists():
+        build.build()
+    lib = _native.lib()
+    assert lib.ffk_layer_norm_backward_workspace(-1, 64) == lib.ffk_layer_norm_backward_workspace(4, 0) == 0
+    assert lib.ffk_layer_norm_backward_workspace(4, 64) == 0  # one workgroup
+    # a workgroup's sums of two gradients for every 4 rows, up to 4 workgroups a CU (256 without a device)
+    assert lib.ffk_layer_norm_backward_workspace(400, 96) == 100 * 2 * 96 * 4
+    assert lib.ffk_layer_norm_backward_workspace(1 << 30, 96) == 1024 * 2 * 96 * 4
+    assert lib.ffk_layer_norm_backward_workspace(1000, 1500) >= (64 * 2 * 1500 + 2000) * 4
+    for bad in ((-1, 64, 4), (10, 32, 4), (10, 832, 4), (10, 64, 0), (10, 64, 65)):
+        assert lib.ffk_transition_backward_workspace(*bad) == 0
+    # rows are taken in chunks: the workspace stops growing
+    assert lib.ffk_transition_backward_workspace(1 << 30, 128, 4) == lib.ffk_transition_backward_workspace(1 << 26, 128, 4)
+    assert lib.ffk_transition_backward_workspace(1 << 30, 256, 4) == lib.ffk_transition_backward_workspace(1 << 26, 256, 4)
+
+
+def test_install_and_take_back():
+    block = randomise(factories.pairformer_block(d_pair=64, triangle_model="af3", d_single=128), 0)
+    block.set_backend("hip")
+    block.requires_grad_(False)
+    report = training.install(block, "8bit")
+    assert {"transition_pair", "single_transition"} <= set(report["hip"])
+    assert {"tri_multi_outgoing", "tri_atten_ending", "single_attention"} <= set(report["pytorch"])
+    assert all(p.requires_grad for p in block.parameters())
+    assert block.transition_pair.keep == "8bit" and block.transition_pair.backend == "hip"
+    assert block.tri_atten_starting.backend == "pytorch"
+    x = torch.zeros(1, 4, 4, 64, dtype=BF16)
+    assert training.wanted(block.transition_pair, x)
+    with torch.no_grad():
+        assert not training.wanted(block.transition_pair, x)
+    training.install(block, None)
+    assert block.transition_pair.keep is None and not training.wanted(block.transition_pair, x)
+
+
+def test_a_width_without_backward_kernels_is_refused_when_it_is_to_be_differentiated(monkeypatch):
+    m = modules.Transition(832, 1)
+    m.set_backend("hip")
+    monkeypatch.setattr(modules, "hip_reason", lambda *t: None)
+    x = torch.zeros(2, 832, dtype=BF16)
+    assert m.unsupported(x) is None
+    m.keep = "8bit"
+    assert "backward" in m.unsupported(x)
+    with torch.no_grad():
+        assert m.unsupported(x) is None
