@@ -416,6 +416,8 @@ void launch_sum_partials(const float* part, int count, int width, int split, voi
 struct TransitionGradPlan {
   int64_t chunk;  // rows at once, a multiple of 64
   int dxh_splits, dw_splits;
+  int dxh_wide, dw_wide;  // the products in 128 x 128 tiles
+  int stream;             // the hidden gradients from rows that stream by
   int fused;      // the hidden rows stay in registers (no E, no dxh)
 };
 TransitionGradPlan transition_grad_plan(int64_t rows, int d, int hidden);

@@ -457,6 +457,107 @@ __global__ __launch_bounds__(256) void gemm64(const Gemm64Args p) {
 }
 static_assert(4 * 2 * 64 * 64 * sizeof(bf16) >= 4 * 4 * 16 * 64 * sizeof(float), "the waves' sums fit the buffers");
 
+// The same products in 128 x 128 tiles, a wave 64 x 64 of it over all k, where the matrix is made of such tiles and they
+// are enough for every CU: sixteen products a wave between two barriers, and half the reads from memory.
+// grid (m tiles, n tiles, splits); block 256.
+template <bool TURN>
+__global__ __launch_bounds__(256, 2) void gemm128(const Gemm64Args p) {
+  __shared__ __attribute__((aligned(16))) bf16 buf[2][4][64 * 64];  // A's two tiles, B's two
+  const int lane = threadIdx.x & 63, g = lane >> 5, li = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
+  const int64_t m0 = (int64_t)blockIdx.x * 128;
+  const int n0 = blockIdx.y * 128;
+  const int64_t kb = (int64_t)blockIdx.z * p.k_share;
+  const int64_t ke = kb + p.k_share < p.k_rows ? kb + p.k_share : p.k_rows;
+  const bf16* B = (int)blockIdx.x * 2 >= p.m_two ? p.B2 : p.B;
+  const int steps = ke > kb ? (int)((ke - kb + 63) / 64) : 0;
+  const uint32_t lds = lds_addr(buf);
+  auto fetch = [&](int step) __attribute__((always_inline)) {
+    const uint32_t at = lds + (step & 1) * 4 * 8192;
+    const int64_t k = kb + 64 * (int64_t)step;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (TURN) {
+        tile_dma(p.A, p.lda, k, p.k_rows - 1, (int)m0 + 64 * i, at + 8192 * i, wave, lane);
+        tile_dma(B, p.ldb, k, p.k_rows - 1, n0 + 64 * i, at + 8192 * (2 + i), wave, lane);
+      } else {
+        tile_dma(p.A + k, p.lda, m0 + 64 * i, p.m_rows - 1, 0, at + 8192 * i, wave, lane);
+        tile_dma(B + k, p.ldb, n0 + 64 * i, n0 + 127, 0, at + 8192 * (2 + i), wave, lane);
+      }
+    }
+  };
+  const bool summed = TURN && blockIdx.y == 0 && wn == 0 && (int)blockIdx.x * 2 < p.m_two;
+  f32x16 acc[2][2], total[2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] = zero16();
+  total[0] = total[1] = zero16();
+  bf16x8 ones;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ones[e] = (bf16)1.f;
+  if (steps > 0) fetch(0);
+  for (int s = 0; s < steps; ++s) {
+    wait_vm_lds<0>();
+    __syncthreads();  // the step has landed; the other buffer has been read
+    if (s + 1 < steps) fetch(s + 1);
+    bf16(*t)[64 * 64] = buf[s & 1];
+    if (TURN) {
+      const int64_t left = ke - (kb + 64 * (int64_t)s);  // rows of this step that count
+      if (left < 64) {
+        for (int i = threadIdx.x; i < 4 * 64 * 8; i += 256) {
+          const int r = (i >> 3) & 63;
+          if (r >= left) {
+            bf16x8 z;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[e] = (bf16)0.f;
+            *reinterpret_cast<bf16x8*>(t[i >> 9] + r * 64 + 8 * (i & 7)) = z;
+          }
+        }
+        __syncthreads();
+      }
+    }
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      bf16x8 fa[2], fb[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (TURN) {
+          fa[i] = ld_turned(t[wm], 32 * i, 16 * kk, lane);
+          fb[i] = ld_turned(t[2 + wn], 32 * i, 16 * kk, lane);
+        } else {
+          fa[i] = ld8(&t[wm][off64(32 * i + li, 2 * kk + g)]);
+          fb[i] = ld8(&t[2 + wn][off64(32 * i + li, 2 * kk + g)]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] = mfma32(fa[i >> 1], fb[i & 1], acc[i >> 1][i & 1]);
+      if (TURN && summed) {
+        total[0] = mfma32(fa[0], ones, total[0]);
+        total[1] = mfma32(fa[1], ones, total[1]);
+      }
+    }
+  }
+  float* C = p.C + blockIdx.z * p.split_stride;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int64_t m = m0 + 64 * wm + 32 * i + acc_row(r, g);
+      if (m < p.m_rows) {
+        float* to = C + m * p.ldc + n0 + 64 * wn + li;
+        to[0] = p.add ? to[0] + acc[i][0][r] : acc[i][0][r];
+        to[32] = p.add ? to[32] + acc[i][1][r] : acc[i][1][r];
+      }
+    }
+  if (summed && li == 0) {  // (every column of a total is the same)
+    float* to = p.sums + blockIdx.z * p.sums_stride + m0 + 64 * wm;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) {
+      float* q = to + 32 * (r >> 4) + acc_row(r & 15, g);
+      *q = p.add ? *q + total[r >> 4][r & 15] : total[r >> 4][r & 15];
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------------------------------------
 // The fused form (d = 64 or 128): two kernels, the hidden rows stay in registers.
 
@@ -692,6 +793,115 @@ __global__ __launch_bounds__(512, D == 128 ? 2 : 3) void transition_grad_weights
       p[H + r] = add ? p[H + r] + tb[r] : tb[r];
     }
   }
+}
+
+// E as hidden_grad makes it, for 256 channels and many rows (20000 rows x 512: 74 -> 49 us): as above a wave keeps its operands of Aw, Bw and S^T of 16 hidden
+// channels in registers (12 D / 32 of them) and the rows stream by through LDS, D = hidden x rows (a lane holds a row at
+// 4 hidden channels). grid (ceil(H / 128), splits); block 512.
+template <int D>
+__global__ __launch_bounds__(512, 2) void hidden_stream(const f16* __restrict__ xh, const bf16* __restrict__ dy,
+                                                        const f16* __restrict__ aw, const bf16* __restrict__ st,
+                                                        const float* __restrict__ shift, const float* __restrict__ scale,
+                                                        bf16* __restrict__ E, int64_t rows, int H) {
+  constexpr int KK = D / 32, NB = 4, U = D / 128;  // U: a wave's KBs of its 4 rows of an array
+  constexpr uint32_t kTile = 32 * D * sizeof(bf16);
+  __shared__ __attribute__((aligned(256))) bf16 buf[NB][2][32 * D];  // xh fp16, dy
+  const int lane = threadIdx.x & 63, q = lane >> 4, li = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h0 = blockIdx.x * 128 + 16 * wave;
+  const bool own = h0 < H;
+  const int hr = own ? h0 + li : li;
+  const uint32_t lds = lds_addr(buf), rows_at = 2 * off_row<D>(li, q);
+  const int64_t blocks = (rows + 31) / 32;
+  // piece u of the wave's 4 rows: its row's and its own place, in bytes (rows past the end: the last one again)
+  uint32_t lane_row[U], lane_piece[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = 64 * u + lane, r = i / (D / 8);
+    lane_row[u] = 2 * D * r;
+    lane_piece[u] = 16 * ((i % (D / 8)) ^ swz<D>(4 * wave + r));
+  }
+  auto fetch = [&](int64_t block, int b) __attribute__((always_inline)) {
+    const int64_t row = (block < blocks ? block : blocks - 1) * 32 + 4 * wave, from = row < rows ? row : rows - 1;
+    const uint32_t most = rows - 1 - from < 4 ? 2 * D * (uint32_t)(rows - 1 - from) : 8u * D;
+    const uint32_t at = lds + 2 * kTile * b + 8 * D * wave;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t off = (lane_row[u] < most ? lane_row[u] : most) + lane_piece[u];
+      dma16(xh + from * D, off, at + 1024 * u);
+      dma16(dy + from * D, off, at + kTile + 1024 * u);
+    }
+  };
+  f16x8 wa[KK], wb[KK];
+  bf16x8 ws[KK];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) {
+    wa[kk] = ld8h(aw + (int64_t)hr * D + 32 * kk + 8 * q);
+    wb[kk] = ld8h(aw + (int64_t)(H + hr) * D + 32 * kk + 8 * q);
+    ws[kk] = ld8(st + (int64_t)hr * D + 32 * kk + 8 * q);
+  }
+  const int hq = own ? h0 + 4 * q : 4 * q;
+  const f32x4 oa = *reinterpret_cast<const f32x4*>(shift + hq), ob = *reinterpret_cast<const f32x4*>(shift + H + hq);
+  const float ia = scale[0], slow = -kLog2e * ia;
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) asm volatile("" ::"v"(wa[kk]), "v"(wb[kk]), "v"(ws[kk]));
+  asm volatile("" ::"v"(oa), "v"(ob), "v"(slow));
+  const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int b = 0; b < NB - 1; ++b) fetch(blockIdx.y + (int64_t)b * gridDim.y, b);
+  int b = 0;
+#pragma unroll 1
+  for (int64_t block = blockIdx.y; block < blocks; block += gridDim.y) {
+    // (this block has landed: NB - 2 later ones of 2 U transfers, and the stores behind them, stay on their way)
+    wait_vm_lds<(NB - 2) * 2 * U>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    const uint32_t tile = lds + 2 * kTile * b + rows_at;
+    f32x4 a[2], bb[2], du[2];
+    f16x8 lx[2][2];
+    bf16x8 ly[2][2];
+    auto take = [&](int kk) __attribute__((always_inline)) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const uint32_t p = (tile ^ ((kk & 3) << 6)) + 256 * (kk >> 2) + 32 * D * t;
+        lx[kk & 1][t] = lds_at<f16x8>(p);
+        ly[kk & 1][t] = lds_at<bf16x8>(p + kTile);
+      }
+      in_order();
+    };
+    take(0);
+    fetch(block + (int64_t)(NB - 1) * gridDim.y, b == 0 ? NB - 1 : b - 1);
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      if (kk + 1 < KK) take(kk + 1);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        a[t] = mfma16h(wa[kk], lx[kk & 1][t], kk ? a[t] : oa);
+        bb[t] = mfma16h(wb[kk], lx[kk & 1][t], kk ? bb[t] : ob);
+        du[t] = mfma16(ws[kk], ly[kk & 1][t], kk ? du[t] : zero4);
+      }
+      in_order();
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      bf16x4 o[3];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const SwigluGrad e = swiglu_grad(a[t][r], bb[t][r], du[t][r], slow, ia);
+        o[0][r] = (bf16)e.da;
+        o[1][r] = (bf16)e.db;
+        o[2][r] = (bf16)e.u;
+      }
+      const int64_t row = block * 32 + 16 * t + li;
+      if (own && row < rows) {
+        bf16* to = E + row * 3 * H + h0 + 4 * q;
+#pragma unroll
+        for (int m = 0; m < 3; ++m) *reinterpret_cast<bf16x4*>(to + m * H) = o[m];
+      }
+    }
+    b = b + 1 == NB ? 0 : b + 1;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the transfers past the end
 }
 
 // dx. A wave owns 32 rows: its operands xh and dy and the sums dxh^T (D x 32 fp32) stay in registers while the weights
@@ -1052,19 +1262,28 @@ void launch_fused(const TransitionGradArgs& a, const TransitionGradPlan& p, cons
 TransitionGradPlan transition_grad_plan(int64_t rows, int d, int H) {
   TransitionGradPlan p{};
   const int64_t cus = cu_count();
-  p.fused = fused_shape(d, H) && rows >= 4096;
+  // Rows from which the fused kernels win (a workgroup walks all chunks of weights however few its rows). Separate kernels
+  // against fused ones, us: 128 x 512 channels, 8192 rows 58 / 76, 16384 rows 83 / 82; 128 x 256, 16384 rows 62 / 63; 64 x 256,
+  // 4096 rows 35 / 36, 8192 rows 44 / 41; 64 x 128, 4096 rows 31 / 28.
+  p.fused = fused_shape(d, H) && rows >= (d == 64 ? 4096 : 16384);
   if (p.fused) {
     p.chunk = std::min<int64_t>(ceil_div(rows, 64) * 64, 1 << 18);
     const int64_t groups = ceil_div(H, 128);
     p.dw_splits = (int)std::max<int64_t>(1, std::min<int64_t>((d == 64 ? 2 : 1) * cus / groups, p.chunk / kStageRows));
     return p;
   }
-  // E of a chunk within 96 MB, so that it is still in the 256 MB last-level cache when the products read it
-  const int64_t fit = std::max<int64_t>((int64_t)(96 << 20) / (6 * H) / 64 * 64, 64);
+  // E of a chunk within 192 MB, so that much of it is still in the 256 MB last-level cache when the products read it, in
+  // few chunks (40000 x 256 x 2: 222 us in one, 344 in two of 96 MB)
+  const int64_t fit = std::max<int64_t>((int64_t)(192 << 20) / (6 * H) / 64 * 64, 64);
   p.chunk = std::min<int64_t>(ceil_div(rows, 64) * 64, fit);
-  // both products want a workgroup a CU at least, and four steps of 64 in each
-  p.dxh_splits = (int)std::max<int64_t>(1, std::min<int64_t>(cus / std::max<int64_t>(1, p.chunk / 64 * (d / 64)), 2 * H / 256));
-  p.dw_splits = (int)std::max<int64_t>(1, std::min<int64_t>(2 * cus / std::max<int64_t>(1, 3 * H / 64 * (d / 64)), p.chunk / 256));
+  // both products want a workgroup a CU at least, and four steps of 64 in each; 128 x 128 tiles where they make so many
+  p.dxh_wide = d % 128 == 0 && ceil_div(p.chunk, 128) * (d / 128) >= cus;
+  const int64_t dxh_tiles = p.dxh_wide ? ceil_div(p.chunk, 128) * (d / 128) : p.chunk / 64 * (d / 64);
+  p.dxh_splits = (int)std::max<int64_t>(1, std::min<int64_t>(cus / std::max<int64_t>(1, dxh_tiles), 2 * H / 256));
+  p.dw_wide = d % 128 == 0 && H % 128 == 0 && p.chunk >= 4096;
+  p.stream = d == 256 && p.chunk >= 4096;
+  const int64_t dw_tiles = p.dw_wide ? 3 * H / 128 * (d / 128) : 3 * H / 64 * (d / 64);
+  p.dw_splits = (int)std::max<int64_t>(1, std::min<int64_t>(2 * cus / std::max<int64_t>(1, dw_tiles), p.chunk / 256));
   return p;
 }
 
@@ -1090,8 +1309,14 @@ void launch_transition_grad(const TransitionGradArgs& a, const TransitionGradPla
         launch_fused<128>(a, p, dy, a.dx + r0 * d, rows, add, st);
       continue;
     }
-    hidden_grad<<<dim3((unsigned)ceil_div(rows, 64), H / 64), 256, 0, st>>>(a.xh, dy, a.aw, a.st, a.shift, a.scale, a.E,
+    if (p.stream) {
+      const int64_t groups = ceil_div(H, 128);
+      const dim3 grid((unsigned)groups, (unsigned)std::max<int64_t>(1, std::min(cu_count() / groups, ceil_div(rows, 32))));
+      hidden_stream<256><<<grid, 512, 0, st>>>(a.xh, dy, a.aw, a.st, a.shift, a.scale, a.E, rows, H);
+    } else {
+      hidden_grad<<<dim3((unsigned)ceil_div(rows, 64), H / 64), 256, 0, st>>>(a.xh, dy, a.aw, a.st, a.shift, a.scale, a.E,
                                                                             rows, d, H);
+    }
     Gemm64Args g{};
     g.A = a.E;
     g.lda = 3 * H;
@@ -1104,7 +1329,10 @@ void launch_transition_grad(const TransitionGradArgs& a, const TransitionGradPla
     g.ldc = d;
     g.split_stride = p.chunk * d;
     g.m_two = 0x7fffffff;
-    gemm64<false><<<dim3((unsigned)ceil_div(rows, 64), d / 64, p.dxh_splits), 256, 0, st>>>(g);
+    if (p.dxh_wide)
+      gemm128<false><<<dim3((unsigned)ceil_div(rows, 128), d / 128, p.dxh_splits), 256, 0, st>>>(g);
+    else
+      gemm64<false><<<dim3((unsigned)ceil_div(rows, 64), d / 64, p.dxh_splits), 256, 0, st>>>(g);
     run_norm_grad_rows(a, dy, p.dxh_splits, g.split_stride, a.dx + r0 * d, rows, st);
     Gemm64Args t{};
     t.A = a.E;
@@ -1122,7 +1350,10 @@ void launch_transition_grad(const TransitionGradArgs& a, const TransitionGradPla
     t.sums = a.sums;
     t.sums_stride = 2 * H;
     t.add = add;
-    gemm64<true><<<dim3(3 * H / 64, d / 64, p.dw_splits), 256, 0, st>>>(t);
+    if (p.dw_wide)
+      gemm128<true><<<dim3(3 * H / 128, d / 128, p.dw_splits), 256, 0, st>>>(t);
+    else
+      gemm64<true><<<dim3(3 * H / 64, d / 64, p.dw_splits), 256, 0, st>>>(t);
   }
   // (no rows: sums over nothing)
   const int parts = a.rows > 0 ? p.dw_splits : 0;
@@ -1130,7 +1361,7 @@ void launch_transition_grad(const TransitionGradArgs& a, const TransitionGradPla
     kernel<<<dim3(d / 32, 3 * H / 8), 256 * q, 0, st>>>(a.dw_part, a.sums, parts, a.wa, a.wb, a.ln_w, a.ln_b, a.scale,
                                                        a.norm_part, d, H, a.dwa, a.dwb, a.dws, a.grad_dtype);
   };
-  if (parts >= 16)
+  if (parts >= 32)  // (21 parts of 1536 x 256: 13.7 us in four shares, 9 in one)
     join(join_weight_grads<4>, 4);
   else
     join(join_weight_grads<1>, 1);

@@ -314,7 +314,15 @@ def test_transition_backward(rows, d, factor, keep, residual):
     _check_transition(x, dy, params, kept, residual=residual)
 
 
-@pytest.mark.parametrize("rows,d,factor", [(5000, 128, 4), (20001, 64, 4), (9999, 64, 2), (23000, 256, 4), (45000, 128, 4)])
+@pytest.mark.parametrize("rows,d,factor", [
+    (5000, 128, 4), (20001, 64, 4), (9999, 64, 2), (23000, 256, 4), (45000, 128, 4),
+    # the fused kernels from where they begin, one row past a tile, hidden widths that fill no workgroup
+    (4096, 64, 4), (4097, 64, 1), (4223, 64, 3), (16384, 128, 4), (16385, 128, 1), (16641, 128, 3), (17000, 128, 16),
+    (16400, 128, 17), (4500, 64, 33),
+    # two chunks of rows, the second a short one
+    (262144 + 33, 128, 4), (262144 + 65, 64, 2), (33001, 256, 4), (66001, 256, 2),
+    # 128 x 128 and 64 x 64 tiles
+    (4095, 256, 2), (4097, 256, 1), (5001, 384, 4), (6000, 192, 3), (4100, 320, 2), (9000, 512, 1), (4200, 768, 2)])
 def test_transition_backward_many_rows(rows, d, factor):
     x, dy, params = _transition_case(rows, d, factor, rows)
     first = _check_transition(x, dy, params, x.to(DEV), residual=True, grad_dtype=BF16)
@@ -322,6 +330,25 @@ def test_transition_backward_many_rows(rows, d, factor):
     again = kernels.transition_backward(dy.to(DEV), x.to(DEV), **dev, grad_dtype=BF16)
     assert all(torch.equal(a, b) for a, b in zip(first, again))  # the same bits on every run
     _check_transition(x, dy, params, kernels.quantize_activation(x.to(DEV)), residual=False)
+
+
+def test_transition_backward_past_32_bits():
+    """More than 2^31 values: the last rows' gradients are those of the rows alone."""
+    rows, d = (1 << 24) + 77, 128
+    g = torch.Generator(device=DEV).manual_seed(2)
+    x = torch.empty(rows, d, dtype=BF16, device=DEV).normal_(generator=g)
+    dy = torch.empty(rows, d, dtype=BF16, device=DEV).normal_(generator=g)
+    params = {k: v.to(DEV) for k, v in _transition_case(1, d, 1, 5)[2].items()}
+    got = kernels.transition_backward(dy, x, **params)
+    tail = slice(rows - 400, rows)
+    want = oracle.transition_backward(dy[tail], x[tail], **params)
+    _near(got.x[tail], want["x"], _deviations(dy[tail], x[tail], params, 1e-5)["x"], "x", BF16, True)
+    # the sums over all rows are those of two halves
+    half = [kernels.transition_backward(dy[s], x[s], **params) for s in (slice(0, 1 << 23), slice(1 << 23, rows))]
+    for name in ("ln_weight", "ln_bias", "expand_a", "expand_b", "squeeze"):
+        a, b, c = (getattr(t, name) for t in (got, *half))
+        # (fp32 sums of the same products in another order: 2^-24 of their magnitudes for each of some 2^10 additions)
+        assert float((a - b - c).norm()) <= 2.0**-14 * float(b.norm() + c.norm()) + 1e-30, name
 
 
 def test_transition_backward_no_rows():
