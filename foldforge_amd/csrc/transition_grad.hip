@@ -337,7 +337,7 @@ struct Gemm64Args {
   const bf16 *A, *B, *B2;
   float *C, *sums;
   int64_t lda, ldb, m_rows, k_rows, k_share, split_stride, sums_stride;
-  int ldc, m_two, add;
+  int ldc, m_two, add, m_tiles, n_tiles;
 };
 template <bool TURN>
 __global__ __launch_bounds__(256) void gemm64(const Gemm64Args p) {
@@ -459,17 +459,22 @@ static_assert(4 * 2 * 64 * 64 * sizeof(bf16) >= 4 * 4 * 16 * 64 * sizeof(float),
 
 // The same products in 128 x 128 tiles, a wave 64 x 64 of it over all k, where the matrix is made of such tiles and they
 // are enough for every CU: sixteen products a wave between two barriers, and half the reads from memory.
-// grid (m tiles, n tiles, splits); block 256.
+// grid m tiles x n tiles x splits; block 256.
 template <bool TURN>
 __global__ __launch_bounds__(256, 2) void gemm128(const Gemm64Args p) {
   __shared__ __attribute__((aligned(16))) bf16 buf[2][4][64 * 64];  // A's two tiles, B's two
   const int lane = threadIdx.x & 63, g = lane >> 5, li = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
-  const int64_t m0 = (int64_t)blockIdx.x * 128;
-  const int n0 = blockIdx.y * 128;
-  const int64_t kb = (int64_t)blockIdx.z * p.k_share;
+  // neighbours on an XCD share its L2: TURN, the tiles of one share of k (A by the n tiles, B by all m tiles); else the n
+  // tiles of an m tile (A), then the next m tile (B)
+  const uint32_t id = xcd_remap(blockIdx.x, gridDim.x);
+  const int mt = p.m_tiles, nt = p.n_tiles;
+  const int bx = TURN ? id % mt : id / nt % mt, by = TURN ? id / mt % nt : id % nt, bz = id / (mt * nt);
+  const int64_t m0 = (int64_t)bx * 128;
+  const int n0 = by * 128;
+  const int64_t kb = (int64_t)bz * p.k_share;
   const int64_t ke = kb + p.k_share < p.k_rows ? kb + p.k_share : p.k_rows;
-  const bf16* B = (int)blockIdx.x * 2 >= p.m_two ? p.B2 : p.B;
+  const bf16* B = bx * 2 >= p.m_two ? p.B2 : p.B;
   const int steps = ke > kb ? (int)((ke - kb + 63) / 64) : 0;
   const uint32_t lds = lds_addr(buf);
   auto fetch = [&](int step) __attribute__((always_inline)) {
@@ -486,7 +491,7 @@ __global__ __launch_bounds__(256, 2) void gemm128(const Gemm64Args p) {
       }
     }
   };
-  const bool summed = TURN && blockIdx.y == 0 && wn == 0 && (int)blockIdx.x * 2 < p.m_two;
+  const bool summed = TURN && by == 0 && wn == 0 && bx * 2 < p.m_two;
   f32x16 acc[2][2], total[2];
 #pragma unroll
   for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] = zero16();
@@ -536,7 +541,7 @@ __global__ __launch_bounds__(256, 2) void gemm128(const Gemm64Args p) {
       }
     }
   }
-  float* C = p.C + blockIdx.z * p.split_stride;
+  float* C = p.C + bz * p.split_stride;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -549,7 +554,7 @@ __global__ __launch_bounds__(256, 2) void gemm128(const Gemm64Args p) {
       }
     }
   if (summed && li == 0) {  // (every column of a total is the same)
-    float* to = p.sums + blockIdx.z * p.sums_stride + m0 + 64 * wm;
+    float* to = p.sums + bz * p.sums_stride + m0 + 64 * wm;
 #pragma unroll
     for (int r = 0; r < 32; ++r) {
       float* q = to + 32 * (r >> 4) + acc_row(r & 15, g);
@@ -613,6 +618,16 @@ __device__ __forceinline__ f32x4 mfma16h(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
+// A workgroup's group of hidden channels and share of the rows, in a grid of (groups, splits): the groups of one share, which
+// read the same rows, are neighbours on one XCD and share its L2.
+struct RowsAt {
+  int group, split, splits;
+};
+__device__ __forceinline__ RowsAt rows_at_of() {
+  const uint32_t id = xcd_remap(blockIdx.x + gridDim.x * blockIdx.y, gridDim.x * gridDim.y);
+  return {(int)(id % gridDim.x), (int)(id / gridDim.x), (int)gridDim.y};
+}
+
 // The weights' gradients G = [da'^T xh; db'^T xh; u'^T dy] and the sums of da', db'.
 //
 // A wave owns 16 hidden channels: its operands of Aw, Bw and S^T (D k of 16 channels each) and its sums (3 x 16 x D
@@ -635,9 +650,10 @@ __global__ __launch_bounds__(512, D == 128 ? 2 : 3) void transition_grad_weights
   constexpr int kTile = kStageRows * D;              // elements of a tile
   constexpr int kLoads = 3 * (kTile / 512) / NW;     // transfers of a wave a stage
   __shared__ __attribute__((aligned(256))) bf16 buf[NB][3][kTile];  // xh fp16, xh bf16, dy
+  const RowsAt at_ = rows_at_of();
   const int lane = threadIdx.x & 63, q = lane >> 4, li = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int h0 = blockIdx.x * 128 + 16 * wave;
+  const int h0 = at_.group * 128 + 16 * wave;
   const bool own = h0 < H;  // H a multiple of 64: the last workgroup's upper waves may own nothing
   const int hr = own ? h0 + li : li;
   const uint32_t lds = lds_addr(buf);
@@ -679,18 +695,18 @@ __global__ __launch_bounds__(512, D == 128 ? 2 : 3) void transition_grad_weights
   for (int e = 0; e < 8; ++e) ones[e] = (bf16)1.f;
 #pragma unroll
   for (int b = 0; b < NB - 1; ++b) {
-    const int64_t stage = blockIdx.y + (int64_t)b * gridDim.y;
+    const int64_t stage = at_.split + (int64_t)b * at_.splits;
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) fetch(stage < stages ? stage : stages - 1, b, u);
   }
   int b = 0;
 #pragma unroll 1
-  for (int64_t stage = blockIdx.y; stage < stages; stage += gridDim.y) {
+  for (int64_t stage = at_.split; stage < stages; stage += at_.splits) {
     wait_vm_lds<(NB - 2) * kLoads>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     // the next stage's transfers are spread over this one (past the end: the last rows again, which nothing reads)
-    int64_t ahead = stage + (int64_t)(NB - 1) * gridDim.y;
+    int64_t ahead = stage + (int64_t)(NB - 1) * at_.splits;
     ahead = ahead < stages ? ahead : stages - 1;
     const int into = b == 0 ? NB - 1 : b - 1;
     bf16* td = buf[b][2];
@@ -772,7 +788,7 @@ __global__ __launch_bounds__(512, D == 128 ? 2 : 3) void transition_grad_weights
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the transfers past the end
   if (!own) return;
-  float* to = G + (int64_t)blockIdx.y * 3 * H * D + (int64_t)h0 * D;
+  float* to = G + (int64_t)at_.split * 3 * H * D + (int64_t)h0 * D;
 #pragma unroll
   for (int c = 0; c < CT; ++c)
 #pragma unroll
@@ -786,7 +802,7 @@ __global__ __launch_bounds__(512, D == 128 ? 2 : 3) void transition_grad_weights
       }
     }
   if (li == 0) {
-    float* p = sums + (int64_t)blockIdx.y * 2 * H + h0 + 4 * q;
+    float* p = sums + (int64_t)at_.split * 2 * H + h0 + 4 * q;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       p[r] = add ? p[r] + ta[r] : ta[r];
@@ -806,9 +822,10 @@ __global__ __launch_bounds__(512, 2) void hidden_stream(const f16* __restrict__ 
   constexpr int KK = D / 32, NB = 4, U = D / 128;  // U: a wave's KBs of its 4 rows of an array
   constexpr uint32_t kTile = 32 * D * sizeof(bf16);
   __shared__ __attribute__((aligned(256))) bf16 buf[NB][2][32 * D];  // xh fp16, dy
+  const RowsAt at_ = rows_at_of();
   const int lane = threadIdx.x & 63, q = lane >> 4, li = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int h0 = blockIdx.x * 128 + 16 * wave;
+  const int h0 = at_.group * 128 + 16 * wave;
   const bool own = h0 < H;
   const int hr = own ? h0 + li : li;
   const uint32_t lds = lds_addr(buf), rows_at = 2 * off_row<D>(li, q);
@@ -848,10 +865,10 @@ __global__ __launch_bounds__(512, 2) void hidden_stream(const f16* __restrict__ 
   asm volatile("" ::"v"(oa), "v"(ob), "v"(slow));
   const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int b = 0; b < NB - 1; ++b) fetch(blockIdx.y + (int64_t)b * gridDim.y, b);
+  for (int b = 0; b < NB - 1; ++b) fetch(at_.split + (int64_t)b * at_.splits, b);
   int b = 0;
 #pragma unroll 1
-  for (int64_t block = blockIdx.y; block < blocks; block += gridDim.y) {
+  for (int64_t block = at_.split; block < blocks; block += at_.splits) {
     // (this block has landed: NB - 2 later ones of 2 U transfers, and the stores behind them, stay on their way)
     wait_vm_lds<(NB - 2) * 2 * U>();
     __builtin_amdgcn_s_barrier();
@@ -870,7 +887,7 @@ __global__ __launch_bounds__(512, 2) void hidden_stream(const f16* __restrict__ 
       in_order();
     };
     take(0);
-    fetch(block + (int64_t)(NB - 1) * gridDim.y, b == 0 ? NB - 1 : b - 1);
+    fetch(block + (int64_t)(NB - 1) * at_.splits, b == 0 ? NB - 1 : b - 1);
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
       if (kk + 1 < KK) take(kk + 1);
@@ -1329,8 +1346,10 @@ void launch_transition_grad(const TransitionGradArgs& a, const TransitionGradPla
     g.ldc = d;
     g.split_stride = p.chunk * d;
     g.m_two = 0x7fffffff;
+    g.m_tiles = (int)ceil_div(rows, 128);
+    g.n_tiles = d / 128;
     if (p.dxh_wide)
-      gemm128<false><<<dim3((unsigned)ceil_div(rows, 128), d / 128, p.dxh_splits), 256, 0, st>>>(g);
+      gemm128<false><<<dim3((unsigned)(g.m_tiles * g.n_tiles * p.dxh_splits)), 256, 0, st>>>(g);
     else
       gemm64<false><<<dim3((unsigned)ceil_div(rows, 64), d / 64, p.dxh_splits), 256, 0, st>>>(g);
     run_norm_grad_rows(a, dy, p.dxh_splits, g.split_stride, a.dx + r0 * d, rows, st);
@@ -1350,8 +1369,10 @@ void launch_transition_grad(const TransitionGradArgs& a, const TransitionGradPla
     t.sums = a.sums;
     t.sums_stride = 2 * H;
     t.add = add;
+    t.m_tiles = 3 * H / 128;
+    t.n_tiles = d / 128;
     if (p.dw_wide)
-      gemm128<true><<<dim3(3 * H / 128, d / 128, p.dw_splits), 256, 0, st>>>(t);
+      gemm128<true><<<dim3((unsigned)(t.m_tiles * t.n_tiles * p.dw_splits)), 256, 0, st>>>(t);
     else
       gemm64<true><<<dim3(3 * H / 64, d / 64, p.dw_splits), 256, 0, st>>>(t);
   }
