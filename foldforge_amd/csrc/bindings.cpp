@@ -92,6 +92,24 @@ PyObject* params_ok(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// activation_ok(codes, scales): whether they are an 8-bit activation: contiguous e4m3 codes [.., c], c > 0, and contiguous
+// uint8 scales [.., ceil(c / 32)] on one device.
+PyObject* activation_ok(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 2) return PyErr_Format(PyExc_TypeError, "activation_ok(codes, scales)");
+  if (!THPVariable_Check(args[0]) || !THPVariable_Check(args[1])) Py_RETURN_FALSE;
+  const at::Tensor &c = THPVariable_Unpack(args[0]), &s = THPVariable_Unpack(args[1]);
+  const int64_t dims = c.dim();
+  if (c.scalar_type() != at::kFloat8_e4m3fn || s.scalar_type() != at::kByte || c.device() != s.device() || dims == 0 ||
+      s.dim() != dims || !c.is_contiguous() || !s.is_contiguous() || c.size(dims - 1) <= 0 ||
+      s.size(dims - 1) != (c.size(dims - 1) + 31) / 32)
+    Py_RETURN_FALSE;
+  for (int64_t d = 0; d + 1 < dims; ++d)
+    if (c.size(d) != s.size(d)) Py_RETURN_FALSE;
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 // empties(tensor, ((shape, kind), ...)): new tensors on the tensor's device, kind 0 bf16, 1 fp32, 2 uint8, 3 e4m3 (a
 // call's outputs and workspace in one step: four torch.empty cost 5 us of the caller's time).
 PyObject* empties(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -133,6 +151,7 @@ PyObject* empties(PyObject*, PyObject* const* args, Py_ssize_t n) {
 #define FFK_CALL(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&Call<&name>::run)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     {"params_ok", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&params_ok)), METH_FASTCALL, nullptr},
+    {"activation_ok", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&activation_ok)), METH_FASTCALL, nullptr},
     {"empties", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&empties)), METH_FASTCALL, nullptr},
     FFK_CALL(ffk_layer_norm),
     FFK_CALL(ffk_layer_norm_linear),

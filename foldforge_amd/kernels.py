@@ -225,7 +225,7 @@ def swiglu_ffn(x: Tensor, w_a: Tensor, w_b: Tensor, w_out: Tensor, residual: Ten
 ACTIVATION_BLOCK = 32
 
 
-@dataclass(frozen=True)
+@dataclass(eq=False, slots=True)
 class Activation8:
     """A bf16 or fp32 row tensor kept in 8 bits for a backward pass (``include/foldforge_amd.h``,
     ``ffk_quantize_activation``): e4m3 ``codes`` of the tensor's shape and, for each block of 32
@@ -253,13 +253,14 @@ class Activation8:
 
 def _call(device: torch.device, name: str, *args) -> None:
     """``ffk_<name>(*args, stream)`` on ``device`` and its current stream."""
-    fn = getattr(_native.calls(), "ffk_" + name)
+    fn = getattr(_native.calls(), f"ffk_{name}")
     if device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             status = fn(*args, _stream(device))
     else:
         status = fn(*args, _stream(device))
-    _native.check(status, name)
+    if status:
+        _native.check(status, name)
 
 
 def _dtype_code(dtype: torch.dtype) -> int:
@@ -289,6 +290,8 @@ def _activation_spec(x: Tensor) -> tuple:
 def _check_activation(a: Activation8, name: str) -> None:
     """An :class:`Activation8` as :func:`quantize_activation` makes it (the C-ABI receives no sizes)."""
     c, s = a.codes, a.scales
+    if c.is_cuda and a.dtype in (torch.bfloat16, torch.float32) and _native.calls().activation_ok(c, s):
+        return
     if not (_on_device(c) and c.is_contiguous() and c.dtype == torch.float8_e4m3fn and c.dim() > 0 and c.shape[-1] > 0):
         _refuse(f"{name}: codes must be a contiguous float8_e4m3fn device tensor")
     want = (*c.shape[:-1], -(-c.shape[-1] // ACTIVATION_BLOCK))
@@ -317,8 +320,10 @@ def restore_activation(a: Activation8, *, out: Tensor | None = None) -> Tensor:
     return out
 
 
-def _affine(t: Tensor | None, device: torch.device, name: str, cols: int) -> Tensor | None:
-    return None if t is None else _param(t, device, name, (cols,))
+def _affine(t: Tensor | None, like: Tensor, name: str, cols: int) -> Tensor | None:
+    if t is None or (like.is_cuda and _native.calls().params_ok(like, (t,), ((cols,),))):
+        return t
+    return _param(t, like.device, name, (cols,))
 
 
 def layer_norm_checkpoint(x: Tensor, weight: Tensor | None, bias: Tensor | None,
@@ -326,7 +331,7 @@ def layer_norm_checkpoint(x: Tensor, weight: Tensor | None, bias: Tensor | None,
     """:func:`layer_norm` of ``x`` and the 8-bit activation of ``x`` that its backward pass takes, in one pass
     (rows of at most 1024 channels; two for wider ones)."""
     rows, cols = _rows_tensor(x, "x"), x.shape[-1]
-    weight, bias = _affine(weight, x.device, "weight", cols), _affine(bias, x.device, "bias", cols)
+    weight, bias = _affine(weight, x, "weight", cols), _affine(bias, x, "bias", cols)
     y, codes, scales = _native.calls().empties(x, ((tuple(x.shape), _dtype_code(x.dtype)), *_activation_spec(x)))
     a = Activation8(codes, scales, x.dtype)
     if rows:
@@ -343,7 +348,7 @@ def _kept(x: Tensor | Activation8, dy: Tensor) -> tuple[Tensor, Tensor | None]:
     else:
         _rows_tensor(x, "x")
         kept = x, None
-    if x.dtype != dy.dtype or tuple(x.shape) != tuple(dy.shape) or x.device != dy.device:
+    if x.dtype != dy.dtype or x.shape != dy.shape or x.device != dy.device:
         _refuse(f"dy {tuple(dy.shape)} {dy.dtype} on {dy.device} is not like x {tuple(x.shape)} {x.dtype} on {x.device}")
     return kept
 
@@ -363,7 +368,7 @@ def layer_norm_backward(dy: Tensor, x: Tensor | Activation8, weight: Tensor | No
     (``dweight`` None without ``weight``, ``dbias`` None without ``with_bias``)."""
     rows, cols, dev = _rows_tensor(dy, "dy"), dy.shape[-1], dy.device
     kept, scales = _kept(x, dy)
-    weight = _affine(weight, dev, "weight", cols)
+    weight = _affine(weight, dy, "weight", cols)
     code = _grad_dtype(grad_dtype)
     lib = _native.calls()
     dx, ws, *sums = lib.empties(dy, (
