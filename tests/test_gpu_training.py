@@ -368,6 +368,30 @@ def test_transition_backward_large_gates():
     _check_transition(x, dy, params, x.to(DEV), residual=True, norm=False)
 
 
+@pytest.mark.parametrize("rows,d", [(3, 64), (300, 128), (20000, 128)])
+def test_transition_backward_with_zero_weights_of_the_norm(rows, d):
+    """Channels whose LayerNorm weight is 0 (or all of them): their gradient is still the sum over the rows."""
+    x, dy, params = _transition_case(rows, d, 4, 11)
+    params["ln_weight"][::3] = 0
+    _check_transition(x, dy, params, x.to(DEV), residual=False)
+    params["ln_weight"].zero_()
+    _check_transition(x, dy, params, x.to(DEV), residual=True)
+
+
+def test_transition_backward_scales():
+    """Weights and gradients far from 1 (fp16 holds neither as they are): the results scale with them exactly."""
+    x, dy, params = _transition_case(130, 128, 4, 12)
+    want = kernels.transition_backward(dy.to(DEV), x.to(DEV), **{k: v.to(DEV) for k, v in params.items()}, residual=False)
+    # expand_b and dy times powers of two: u and db scale, so every gradient does
+    for kb, ky in ((-40, 0), (30, -60), (0, 40)):
+        p = {**params, "expand_b": params["expand_b"] * 2.0**kb}
+        got = kernels.transition_backward((dy.float() * 2.0**ky).to(BF16).to(DEV), x.to(DEV),
+                                          **{k: v.to(DEV) for k, v in p.items()}, residual=False)
+        for name, e in (("x", kb + ky), ("ln_weight", kb + ky), ("ln_bias", kb + ky), ("expand_a", kb + ky),
+                        ("expand_b", ky), ("squeeze", kb + ky)):
+            assert torch.equal(getattr(got, name).float(), getattr(want, name).float() * 2.0**e), (name, kb, ky)
+
+
 def test_transition_checkpoint_is_the_forward():
     x, _, params = _transition_case(333, 128, 4, 2)
     dev = {k: v.to(DEV) for k, v in params.items()}
