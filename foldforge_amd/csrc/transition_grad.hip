@@ -79,16 +79,17 @@ __device__ __forceinline__ bf16x8 ld_turned(const bf16* tile, int c0, int k0, in
   return o.v;
 }
 
-// k with peak 2^k in [2^14, 2^15) (within what fp32 powers allow; 0 for a matrix of zeros).
+// k with peak 2^k in [2^14, 2^15); 0 for a peak of 0, at most 110 (2^-k and peak 2^k stay normal numbers).
 __device__ __forceinline__ int peak_power(float peak) {
   if (peak == 0.f) return 0;
   const int k = 14 + 127 - (int)(__float_as_uint(peak) >> 23);
-  return k < -110 ? -110 : k > 110 ? 110 : k;
+  return k > 110 ? 110 : k;
 }
 __device__ __forceinline__ float two_to(int k) { return __uint_as_float((uint32_t)(127 + k) << 23); }
 
 // Of each row h of A and B: offset [2][H] = the row's product with v, and of each four rows (a workgroup's) the largest
-// |A w| in peaks [2][H / 4]. One wave a row; block 256, 2 H / 4 of them.
+// |A w| or |offset| in peaks [2][H / 4]: a', b' <= 2^15 (1 + d) whatever w, v and the weights are, so no product of theirs
+// leaves fp32. One wave a row; block 256, 2 H / 4 of them.
 __device__ __forceinline__ void weight_rows(int block, const float* __restrict__ wa, const float* __restrict__ wb,
                                             const float* __restrict__ w, const float* __restrict__ v,
                                             float* __restrict__ offset, float* __restrict__ peaks, int d, int H) {
@@ -107,7 +108,7 @@ __device__ __forceinline__ void weight_rows(int block, const float* __restrict__
   for (int m = 32; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
   if (lane == 0) {
     offset[h] = dot;
-    red[wave] = top;
+    red[wave] = fmaxf(top, finite_abs(dot));
   }
   __syncthreads();
   if (threadIdx.x == 0) peaks[block] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
@@ -1197,7 +1198,9 @@ __global__ __launch_bounds__(256 * Q) void join_weight_grads(const float* __rest
   for (int i = 0; i < Q; ++i) t += share[0][i][row][col];
   if (!summed) {
     // 8 hidden channels of a row of dS: 16 or 32 bytes
-    put(ds, (int64_t)(c0 + col) * H + h0 - 2 * H + row, count ? t * (scale[0] * scale[1]) : 0.f);
+    // (2^-ka 2^-kb may leave fp32 where the gradient does not)
+    const int power = count ? __builtin_amdgcn_frexp_expf(scale[0]) + __builtin_amdgcn_frexp_expf(scale[1]) - 2 : 0;
+    put(ds, (int64_t)(c0 + col) * H + h0 - 2 * H + row, __builtin_ldexpf(t, power));
     return;
   }
   total = 0.f;

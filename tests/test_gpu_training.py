@@ -392,6 +392,30 @@ def test_transition_backward_scales():
             assert torch.equal(getattr(got, name).float(), getattr(want, name).float() * 2.0**e), (name, kb, ky)
 
 
+@pytest.mark.parametrize("rows", [130, 16400])
+def test_transition_backward_scales_of_the_affine(rows):
+    """The norm's weight or bias or a weight matrix powers of two away from the rest. A weight or a matrix scaled by
+    powers whose product is 1 leaves the hidden values, so every gradient scales exactly; a weight far below its bias
+    still gives the formula's gradients."""
+    x, dy, params = _transition_case(rows, 128, 4, 12)
+    x, dy = x.to(DEV), dy.to(DEV)
+    dev = {k: v.to(DEV) for k, v in params.items()}
+    want = kernels.transition_backward(dy, x, **dev, residual=False)
+    for k in (-90, -40, 60):  # weight and bias by 2^k, the matrices by 2^-k
+        p = {**dev, **{n: dev[n] * 2.0**k for n in ("ln_weight", "ln_bias")},
+             **{n: dev[n] * 2.0**-k for n in ("expand_a", "expand_b")}}
+        got = kernels.transition_backward(dy, x, **p, residual=False)
+        for name, e in (("x", 0), ("ln_weight", -k), ("ln_bias", -k), ("expand_a", k), ("expand_b", k), ("squeeze", 0)):
+            assert torch.equal(getattr(got, name).float(), getattr(want, name).float() * 2.0**e), (name, k)
+    for k in (-100, -30):
+        p = {**params, "ln_weight": params["ln_weight"] * 2.0**k}
+        _check_transition(x.cpu(), dy.cpu(), p, x, residual=False)
+    # both matrices tiny: u and dS (2^-160) end below fp32, the other gradients scale
+    p = {**dev, **{n: dev[n] * 2.0**-80 for n in ("expand_a", "expand_b")}}
+    got = kernels.transition_backward(dy, x, **p, residual=False)
+    assert all(torch.isfinite(t.float()).all() for t in got) and not got.squeeze.any()
+
+
 def test_transition_checkpoint_is_the_forward():
     x, _, params = _transition_case(333, 128, 4, 2)
     dev = {k: v.to(DEV) for k, v in params.items()}
