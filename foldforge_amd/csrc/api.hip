@@ -1157,8 +1157,8 @@ int32_t ffk_transition_backward(const void* dy, const void* x, const void* scale
     return fail(FFK_ERR_INVALID, "transition_backward: null parameter or gradient");
   if (grad_dtype != FFK_DTYPE_BF16 && grad_dtype != FFK_DTYPE_F32)
     return fail(FFK_ERR_INVALID, "transition_backward: gradient dtype %d is neither bf16 nor fp32", grad_dtype);
-  if (!aligned16(dy) || !aligned16(x) || !aligned16(dx))
-    return fail(FFK_ERR_INVALID, "transition_backward: dy, x and dx must be 16-byte aligned");
+  if (!aligned16(dy) || !aligned16(x) || !aligned16(dx) || !aligned16(dw_squeeze))
+    return fail(FFK_ERR_INVALID, "transition_backward: dy, x, dx and dw_squeeze must be 16-byte aligned");
   const int hidden = factor * d;
   const TransitionGradPlan plan = transition_grad_plan(rows, d, hidden);
   size_t need = 0;

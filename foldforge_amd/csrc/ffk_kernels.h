@@ -418,7 +418,8 @@ struct TransitionGradPlan {
   int dxh_splits, dw_splits;
   int dxh_wide, dw_wide;  // the products in 128 x 128 tiles
   int stream;             // the hidden gradients from rows that stream by
-  int fused;      // the hidden rows stay in registers (no E, no dxh)
+  int fused;              // the hidden rows stay in registers (no E, no dxh)
+  int few;                // one chunk whose weights' gradients need no join
 };
 TransitionGradPlan transition_grad_plan(int64_t rows, int d, int hidden);
 struct TransitionGradArgs {

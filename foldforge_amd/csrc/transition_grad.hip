@@ -340,17 +340,31 @@ struct Gemm64Args {
   int64_t lda, ldb, m_rows, k_rows, k_share, split_stride, sums_stride;
   int ldc, m_two, add, m_tiles, n_tiles;
 };
-template <bool TURN>
-__global__ __launch_bounds__(256) void gemm64(const Gemm64Args p) {
+struct Gemm64Lds {
+  bf16 buf[4][2][64 * 64];
+  float total[4][64], affine[2][2][64];  // (of a call whose products are the gradients)
+};
+// What the weights' gradients take where one workgroup has all of a tile's sum: see store_weight_grads.
+struct WeightGradArgs {
+  const float *wa, *wb, *w, *v, *scale;
+  float* part;
+  void *da, *db, *ds;
+  int d, H, dtype;
+};
+__device__ __forceinline__ void store_weight_grads(const WeightGradArgs& q, float (&t)[16], Gemm64Lds& lds, int m0, int n0);
+
+template <bool TURN, bool GRADS>
+__device__ __forceinline__ void gemm64_tile(const Gemm64Args& p, const WeightGradArgs& q, Gemm64Lds& sh, int bx, int by,
+                                            int bz) {
   constexpr int NB = 4;
-  __shared__ __attribute__((aligned(16))) bf16 buf[NB][2][64 * 64];
+  auto& buf = sh.buf;
   const int lane = threadIdx.x & 63, g = lane >> 5, li = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t m0 = (int64_t)blockIdx.x * 64;
-  const int n0 = blockIdx.y * 64;
-  const int64_t kb = (int64_t)blockIdx.z * p.k_share;
+  const int64_t m0 = (int64_t)bx * 64;
+  const int n0 = by * 64;
+  const int64_t kb = (int64_t)bz * p.k_share;
   const int64_t ke = kb + p.k_share < p.k_rows ? kb + p.k_share : p.k_rows;
-  const bf16* B = (int)blockIdx.x >= p.m_two ? p.B2 : p.B;
+  const bf16* B = bx >= p.m_two ? p.B2 : p.B;
   const int steps = ke > kb ? (int)((ke - kb + 63) / 64) : 0;
   const uint32_t lds = lds_addr(buf);
   auto fetch = [&](int step) __attribute__((always_inline)) {
@@ -364,7 +378,7 @@ __global__ __launch_bounds__(256) void gemm64(const Gemm64Args p) {
       tile_dma(B + k, p.ldb, n0, n0 + 63, 0, at + 8192, wave, lane);
     }
   };
-  const bool summed = TURN && blockIdx.y == 0 && (int)blockIdx.x < p.m_two;
+  const bool summed = TURN && (GRADS || by == 0) && bx < p.m_two;
   f32x16 acc[2][2], total[2];
   total[0] = total[1] = zero16();
   bf16x8 ones;
@@ -427,36 +441,120 @@ __global__ __launch_bounds__(256) void gemm64(const Gemm64Args p) {
   for (int t = 0; t < 4; ++t)
 #pragma unroll
     for (int r = 0; r < 16; ++r) red[((wave * 4 + t) * 16 + r) * 64 + lane] = acc[t >> 1][t & 1][r];
+  if (TURN && summed && li == 0) {  // (every column of a total is the same)
+#pragma unroll
+    for (int r = 0; r < 32; ++r) sh.total[wave][32 * (r >> 4) + acc_row(r & 15, g)] = total[r >> 4][r & 15];
+  }
   __syncthreads();
-  // wave t stores tile t
-  float* C = p.C + blockIdx.z * p.split_stride;
+  // wave t has tile t
+  float v[16];
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    float v = 0.f;
+    v[r] = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) v += red[((w * 4 + wave) * 16 + r) * 64 + lane];
+    for (int w = 0; w < 4; ++w) v[r] += red[((w * 4 + wave) * 16 + r) * 64 + lane];
+  }
+  if constexpr (GRADS) {
+    store_weight_grads(q, v, sh, (int)m0, n0);
+    return;
+  }
+  float* C = p.C + bz * p.split_stride;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
     const int64_t m = m0 + 32 * (wave >> 1) + acc_row(r, g);
     if (m < p.m_rows) {
       float* to = C + m * p.ldc + n0 + 32 * (wave & 1) + li;
-      *to = p.add ? *to + v : v;
+      *to = p.add ? *to + v[r] : v[r];
     }
   }
-  if (TURN && summed) {
-    __syncthreads();
-    // (every column of a total is the same: lane 0 of each half)
-    if (li == 0) {
-#pragma unroll
-      for (int r = 0; r < 32; ++r) red[wave * 64 + 32 * (r >> 4) + acc_row(r & 15, g)] = total[r >> 4][r & 15];
-    }
-    __syncthreads();
-    if (threadIdx.x < 64) {
-      float* to = p.sums + blockIdx.z * p.sums_stride + m0 + threadIdx.x;
-      const float v = (red[threadIdx.x] + red[64 + threadIdx.x]) + (red[128 + threadIdx.x] + red[192 + threadIdx.x]);
-      *to = p.add ? *to + v : v;
-    }
+  if (TURN && summed && threadIdx.x < 64) {
+    const int i = threadIdx.x;
+    float* to = p.sums + bz * p.sums_stride + m0 + i;
+    const float t = (sh.total[0][i] + sh.total[1][i]) + (sh.total[2][i] + sh.total[3][i]);
+    *to = p.add ? *to + t : t;
   }
 }
 static_assert(4 * 2 * 64 * 64 * sizeof(bf16) >= 4 * 4 * 16 * 64 * sizeof(float), "the waves' sums fit the buffers");
+
+template <bool TURN>
+__global__ __launch_bounds__(256) void gemm64(const Gemm64Args p) {
+  __shared__ __attribute__((aligned(16))) Gemm64Lds sh;
+  gemm64_tile<TURN, false>(p, {}, sh, blockIdx.x, blockIdx.y, blockIdx.z);
+}
+
+// gradient `at` of an output in bf16 (dtype 0) or fp32
+__device__ __forceinline__ void put_grad(void* to, int64_t at, float t, int dtype) {
+  if (dtype == 0)
+    static_cast<bf16*>(to)[at] = (bf16)t;
+  else
+    static_cast<float*>(to)[at] = t;
+}
+// 2^-ka 2^-kb t (the product of the two may leave fp32 where the gradient does not)
+__device__ __forceinline__ float unscale_both(float t, const float* scale) {
+  return __builtin_ldexpf(t, __builtin_amdgcn_frexp_expf(scale[0]) + __builtin_amdgcn_frexp_expf(scale[1]) - 2);
+}
+
+// As join_weight_grads, from a 64 x 64 tile of G in registers (a wave 32 x 32 of it): part [2 H / 64][2][d].
+__device__ __forceinline__ void store_weight_grads(const WeightGradArgs& q, float (&t)[16], Gemm64Lds& sh, int m0, int n0) {
+  const int lane = threadIdx.x & 63, g = lane >> 5, li = lane & 31, wave = threadIdx.x >> 6;
+  const int mw = 32 * (wave >> 1), c = 32 * (wave & 1) + li;
+  if (m0 >= 2 * q.H) {  // dS [d][H]: 4 hidden channels of a row together
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t at = (int64_t)(n0 + c) * q.H + m0 - 2 * q.H + mw + acc_row(4 * k, g);
+      float o[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = unscale_both(t[4 * k + e], q.scale);
+      if (q.dtype == 0) {
+        const bf16x4 b = {(bf16)o[0], (bf16)o[1], (bf16)o[2], (bf16)o[3]};
+        *reinterpret_cast<bf16x4*>(static_cast<bf16*>(q.ds) + at) = b;
+      } else {
+        *reinterpret_cast<f32x4*>(static_cast<float*>(q.ds) + at) = f32x4{o[0], o[1], o[2], o[3]};
+      }
+    }
+    return;
+  }
+  const bool first = m0 < q.H;
+  const float back = q.scale[first ? 1 : 0], w = q.w[n0 + c], v = q.v[n0 + c];
+  float aw = 0.f, av = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int i = mw + acc_row(r, g);
+    const float total = ((sh.total[0][i] + sh.total[1][i]) + (sh.total[2][i] + sh.total[3][i])) * back;
+    const int64_t at = (int64_t)(m0 + i - (first ? 0 : q.H)) * q.d + n0 + c;
+    t[r] *= back;
+    const float own = (first ? q.wa : q.wb)[at];
+    put_grad(first ? q.da : q.db, at, t[r] * w + total * v, q.dtype);
+    aw += own * t[r];
+    av += own * total;
+  }
+  aw += __shfl_xor(aw, 32, 64);
+  av += __shfl_xor(av, 32, 64);
+  if (g == 0) {
+    sh.affine[wave >> 1][0][c] = aw;
+    sh.affine[wave >> 1][1][c] = av;
+  }
+  __syncthreads();
+  if (threadIdx.x < 128) {
+    const int which = threadIdx.x >> 6, i = threadIdx.x & 63;
+    q.part[((int64_t)(m0 / 64) * 2 + which) * q.d + n0 + i] = sh.affine[0][which][i] + sh.affine[1][which][i];
+  }
+}
+
+// Few rows: both products of E in one launch, the weights' gradients finished where they are summed. The first
+// `tiles` workgroups are those of t (m_tiles = 3 H / 64 by n_tiles = d / 64), the others those of g (m_tiles by n_tiles
+// by the splits of k). block 256.
+__global__ __launch_bounds__(256) void grad_products(const Gemm64Args t, const WeightGradArgs q, const Gemm64Args g,
+                                                     int tiles) {
+  __shared__ __attribute__((aligned(16))) Gemm64Lds sh;
+  const int i = blockIdx.x;
+  if (i < tiles) {
+    gemm64_tile<true, true>(t, q, sh, i % t.m_tiles, i / t.m_tiles, 0);
+  } else {
+    const int j = i - tiles, mn = g.m_tiles * g.n_tiles;
+    gemm64_tile<false, false>(g, {}, sh, j % g.m_tiles, j % mn / g.m_tiles, j / mn);
+  }
+}
 
 // The same products in 128 x 128 tiles, a wave 64 x 64 of it over all k, where the matrix is made of such tiles and they
 // are enough for every CU: sixteen products a wave between two barriers, and half the reads from memory.
@@ -1124,16 +1222,16 @@ __global__ __launch_bounds__(4 * D, 2) void transition_grad_rows(
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the transfers past the last chunk
 }
 
-// dx = (residual ? dy : 0) + rstd (g - mean(g) - xh mean(g xh)), g the sum of `splits` fp32 parts [rows][d]: a wave a row,
-// K = d / 64 channels a lane. grid-strided; block 64 (few rows still make many workgroups).
+// dx = (residual ? dy : 0) + rstd (g - mean(g) - xh mean(g xh)), g the sum of `splits` fp32 parts [rows][d]: a wave a row
+// (from row `first` in steps), K = d / 64 channels a lane.
 template <int K>
-__global__ __launch_bounds__(64) void norm_grad_rows(const f16* __restrict__ xh, const float* __restrict__ rstd_in,
-                                                     const bf16* __restrict__ dy, const float* __restrict__ dxh,
-                                                     int splits, int64_t split_stride, bf16* __restrict__ dx,
-                                                     int64_t rows, int residual) {
+__device__ __forceinline__ void norm_grad(int64_t first, int64_t step, const f16* __restrict__ xh,
+                                          const float* __restrict__ rstd_in, const bf16* __restrict__ dy,
+                                          const float* __restrict__ dxh, int splits, int64_t split_stride,
+                                          bf16* __restrict__ dx, int64_t rows, int residual) {
   constexpr int d = 64 * K;
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const int64_t at = row * d + threadIdx.x;
+  for (int64_t row = first; row < rows; row += step) {
+    const int64_t at = row * d + (threadIdx.x & 63);
     float t[K], h[K], y[K];
     float sg = 0.f, sx = 0.f;
 #pragma unroll
@@ -1159,6 +1257,43 @@ __global__ __launch_bounds__(64) void norm_grad_rows(const f16* __restrict__ xh,
     for (int k = 0; k < K; ++k) dx[at + 64 * k] = (bf16)(y[k] + rstd * (t[k] - c1 - h[k] * c2));
   }
 }
+template <int K>
+__global__ __launch_bounds__(64) void norm_grad_rows(const f16* __restrict__ xh, const float* __restrict__ rstd,
+                                                     const bf16* __restrict__ dy, const float* __restrict__ dxh,
+                                                     int splits, int64_t split_stride, bf16* __restrict__ dx,
+                                                     int64_t rows, int residual) {
+  norm_grad<K>(blockIdx.x, gridDim.x, xh, rstd, dy, dxh, splits, split_stride, dx, rows, residual);
+}
+// Few rows: dx, and the affine's gradients from grad_products' parts [count][2 d], in one launch: the first d / 8
+// workgroups sum 16 columns each (a thread every 16th part in order, then the 16 sums in order), the others take 4 rows.
+// block 256.
+template <int K>
+__global__ __launch_bounds__(256) void finish_rows(const f16* __restrict__ xh, const float* __restrict__ rstd,
+                                                   const bf16* __restrict__ dy, const float* __restrict__ dxh, int splits,
+                                                   int64_t split_stride, bf16* __restrict__ dx, int64_t rows, int residual,
+                                                   const float* __restrict__ part, int count, void* dln_w, void* dln_b,
+                                                   int dtype) {
+  constexpr int d = 64 * K, sums = d / 8;
+  __shared__ float red[16][17];
+  const int block = blockIdx.x;
+  if (block >= sums) {
+    norm_grad<K>(4 * (int64_t)(block - sums) + (threadIdx.x >> 6), 4 * (int64_t)(gridDim.x - sums), xh, rstd, dy, dxh,
+                 splits, split_stride, dx, rows, residual);
+    return;
+  }
+  const int col = threadIdx.x & 15, row = threadIdx.x >> 4, c = 16 * block + col;
+  float s = 0.f;
+#pragma unroll 8
+  for (int k = row; k < count; k += 16) s += part[(int64_t)k * 2 * d + c];
+  red[row][col] = s;
+  __syncthreads();
+  if (threadIdx.x < 16) {
+    s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s += red[k][col];
+    put_grad(c < d ? dln_w : dln_b, c < d ? c : c - d, s, dtype);
+  }
+}
 
 // The weights' gradients from `count` parts G [3 H][d] (da'^T xh, db'^T xh, u'^T dy) and sums [2 H] (of da', db'), and
 // eight hidden channels' shares of the affine's: part [2 H / 8][2][d]. A workgroup: 32 channels x 8 hidden channels, in Q
@@ -1175,12 +1310,6 @@ __global__ __launch_bounds__(256 * Q) void join_weight_grads(const float* __rest
   const int col = threadIdx.x & 31, row = (threadIdx.x >> 5) & 7, quarter = threadIdx.x >> 8;
   const int64_t size = (int64_t)3 * H * d;
   const bool summed = h0 < 2 * H;
-  const auto put = [&](void* to, int64_t at, float t) __attribute__((always_inline)) {
-    if (dtype == 0)
-      static_cast<bf16*>(to)[at] = (bf16)t;
-    else
-      static_cast<float*>(to)[at] = t;
-  };
   const float* p = G + (int64_t)(h0 + row) * d + c0 + col;
   float t = 0.f, total = 0.f;
 #pragma unroll 8
@@ -1198,9 +1327,7 @@ __global__ __launch_bounds__(256 * Q) void join_weight_grads(const float* __rest
   for (int i = 0; i < Q; ++i) t += share[0][i][row][col];
   if (!summed) {
     // 8 hidden channels of a row of dS: 16 or 32 bytes
-    // (2^-ka 2^-kb may leave fp32 where the gradient does not)
-    const int power = count ? __builtin_amdgcn_frexp_expf(scale[0]) + __builtin_amdgcn_frexp_expf(scale[1]) - 2 : 0;
-    put(ds, (int64_t)(c0 + col) * H + h0 - 2 * H + row, __builtin_ldexpf(t, power));
+    put_grad(ds, (int64_t)(c0 + col) * H + h0 - 2 * H + row, count ? unscale_both(t, scale) : 0.f, dtype);
     return;
   }
   total = 0.f;
@@ -1211,7 +1338,7 @@ __global__ __launch_bounds__(256 * Q) void join_weight_grads(const float* __rest
   t *= back;
   total *= back;
   const int64_t at = (int64_t)(h0 + row - (first ? 0 : H)) * d + c0 + col;
-  put(first ? da : db, at, t * w[c0 + col] + total * v[c0 + col]);
+  put_grad(first ? da : db, at, t * w[c0 + col] + total * v[c0 + col], dtype);
   const float own = (first ? wa : wb)[at];
   tile[0][row][col] = own * t;
   tile[1][row][col] = own * total;
@@ -1251,6 +1378,19 @@ void run_norm_grad_rows(const TransitionGradArgs& a, const bf16* dy, int splits,
 #define FFK_K(K_)                                                                                                 \
   case K_:                                                                                                        \
     norm_grad_rows<K_><<<grid, 64, 0, st>>>(a.xh, a.rstd, dy, a.dxh, splits, split_stride, dx, rows, a.residual); \
+    break;
+    FFK_K(1) FFK_K(2) FFK_K(3) FFK_K(4) FFK_K(5) FFK_K(6) FFK_K(7) FFK_K(8) FFK_K(9) FFK_K(10) FFK_K(11) FFK_K(12)
+#undef FFK_K
+  }
+}
+
+void run_finish_rows(const TransitionGradArgs& a, int splits, int64_t split_stride, int64_t rows, hipStream_t st) {
+  const dim3 grid((unsigned)(a.d / 8 + std::min<int64_t>(ceil_div(rows, 4), (int64_t)cu_count() * 16)));
+  switch (a.d / 64) {
+#define FFK_K(K_)                                                                                                     \
+  case K_:                                                                                                            \
+    finish_rows<K_><<<grid, 256, 0, st>>>(a.xh, a.rstd, a.dy, a.dxh, splits, split_stride, a.dx, rows, a.residual,    \
+                                          a.norm_part, 2 * a.hidden / 64, a.dln_w, a.dln_b, a.grad_dtype);            \
     break;
     FFK_K(1) FFK_K(2) FFK_K(3) FFK_K(4) FFK_K(5) FFK_K(6) FFK_K(7) FFK_K(8) FFK_K(9) FFK_K(10) FFK_K(11) FFK_K(12)
 #undef FFK_K
@@ -1304,6 +1444,8 @@ TransitionGradPlan transition_grad_plan(int64_t rows, int d, int H) {
   p.stream = d == 256 && p.chunk >= 4096;
   const int64_t dw_tiles = p.dw_wide ? 3 * H / 128 * (d / 128) : 3 * H / 64 * (d / 64);
   p.dw_splits = (int)std::max<int64_t>(1, std::min<int64_t>(2 * cus / std::max<int64_t>(1, dw_tiles), p.chunk / 256));
+  // both products and the gradients' ends in two launches instead of five
+  p.few = rows > 0 && rows <= p.chunk && p.dw_splits == 1 && !p.dw_wide && !p.dxh_wide && !p.stream;
   return p;
 }
 
@@ -1351,11 +1493,6 @@ void launch_transition_grad(const TransitionGradArgs& a, const TransitionGradPla
     g.m_two = 0x7fffffff;
     g.m_tiles = (int)ceil_div(rows, 128);
     g.n_tiles = d / 128;
-    if (p.dxh_wide)
-      gemm128<false><<<dim3((unsigned)(g.m_tiles * g.n_tiles * p.dxh_splits)), 256, 0, st>>>(g);
-    else
-      gemm64<false><<<dim3((unsigned)ceil_div(rows, 64), d / 64, p.dxh_splits), 256, 0, st>>>(g);
-    run_norm_grad_rows(a, dy, p.dxh_splits, g.split_stride, a.dx + r0 * d, rows, st);
     Gemm64Args t{};
     t.A = a.E;
     t.lda = 3 * H;
@@ -1374,6 +1511,22 @@ void launch_transition_grad(const TransitionGradArgs& a, const TransitionGradPla
     t.add = add;
     t.m_tiles = 3 * H / 128;
     t.n_tiles = d / 128;
+    if (p.few) {
+      g.m_tiles = (int)ceil_div(rows, 64);
+      g.n_tiles = d / 64;
+      t.m_tiles = 3 * H / 64;
+      t.n_tiles = d / 64;
+      const WeightGradArgs q{a.wa, a.wb, a.ln_w, a.ln_b, a.scale, a.norm_part, a.dwa, a.dwb, a.dws, d, H, a.grad_dtype};
+      const int tiles = t.m_tiles * t.n_tiles;
+      grad_products<<<dim3((unsigned)(tiles + g.m_tiles * g.n_tiles * p.dxh_splits)), 256, 0, st>>>(t, q, g, tiles);
+      run_finish_rows(a, p.dxh_splits, g.split_stride, rows, st);
+      return;
+    }
+    if (p.dxh_wide)
+      gemm128<false><<<dim3((unsigned)(g.m_tiles * g.n_tiles * p.dxh_splits)), 256, 0, st>>>(g);
+    else
+      gemm64<false><<<dim3((unsigned)ceil_div(rows, 64), d / 64, p.dxh_splits), 256, 0, st>>>(g);
+    run_norm_grad_rows(a, dy, p.dxh_splits, g.split_stride, a.dx + r0 * d, rows, st);
     if (p.dw_wide)
       gemm128<true><<<dim3((unsigned)(t.m_tiles * t.n_tiles * p.dw_splits)), 256, 0, st>>>(t);
     else
