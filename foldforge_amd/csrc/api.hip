@@ -280,7 +280,7 @@ TransitionGradArgs transition_grad_ws(void* ws, size_t* bytes, const TransitionG
   TransitionGradArgs a{};
   const size_t w = (size_t)hidden * d;
   a.peaks = cv.take<float>((size_t)hidden / 2);
-  a.scale = cv.take<float>(2);
+  a.scale = cv.take<float>(2 * (size_t)hidden);
   a.offset = cv.take<float>(2 * (size_t)hidden);
   a.shift = cv.take<float>(2 * (size_t)hidden);
   a.aw = cv.take<f16>(2 * w);
