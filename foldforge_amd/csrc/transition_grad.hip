@@ -12,9 +12,10 @@
 //   dv = A^T (sum da) + B^T (sum db)
 // so dw and dv come out of the weights' gradients, and the products see xh alone, whose values are at most
 // sqrt(d): a and b are products of fp16 operands (Aw and Bw times a power of two that puts their largest
-// entry at 2^14 .. 2^15, so that entries down to 2^-29 of it keep fp16's 11 bits), which leaves their errors at an
-// eighth of bf16's. The gradients' operands are bf16, whose range they need: three bf16 roundings lie between
-// dy and a gradient, and one of the result (relative error 3.3e-3 rather than the 4.6e-3 of bf16 throughout).
+// entry, of the matrix or of a hidden channel's row, at 2^14 .. 2^15, so that entries down to 2^-29 of it keep
+// fp16's 11 bits), which leaves their errors at an eighth of bf16's. The gradients' operands are bf16, whose
+// range they need: three bf16 roundings lie between dy and a gradient, and one of the result (relative error
+// 3.3e-3 rather than the 4.6e-3 of bf16 throughout).
 // The powers of two 2^ka, 2^kb ride along: a' = 2^ka a, b' = 2^kb b, so silu' = 2^ka silu, da' = 2^kb da,
 // db' = 2^ka db, u' = 2^(ka+kb) u; the transposed weights carry their inverses, the join takes the rest out.
 #include <algorithm>
@@ -257,7 +258,7 @@ __global__ __launch_bounds__(256) void pack_grad_weights(const WeightArgs q, bf1
 
 // What a call makes of its inputs first, in one launch: the weights (the first `weight_blocks` workgroups: weight_rows or
 // pack_rows), and xh in fp16 and bf16 and rstd of the kept rows: 8 lanes a row, K = d / 64 pieces of 8 channels each,
-// the other workgroups grid-strided over rows. block 256 (32 rows).
+// the other workgroups grid-strided over rows. block 256 (32 rows). 262144 8-bit rows of 128: 31 us, 5.4 TB/s.
 template <bool CODES, int K, bool FUSED>
 __global__ __launch_bounds__(256) void norm_rows(const void* x, const uint8_t* scales, f16* __restrict__ xh,
                                                  bf16* __restrict__ xhb, float* __restrict__ rstd_out, int64_t rows,
@@ -322,7 +323,8 @@ __device__ __forceinline__ SwigluGrad swiglu_grad(float a, float b, float du, fl
 
 // E [rows][3 H] = [da' | db' | u']. A workgroup: 64 rows x 64 hidden channels, a wave 32 x 32 of each of a, b and du
 // (D = weight rows x token rows: a lane holds a token and 16 channels). k in steps of 64, double-buffered by
-// LDS DMA. grid (ceil(rows / 64), H / 64); block 256.
+// LDS DMA. grid (ceil(rows / 64), H / 64); block 256. 100 rows x 384 x 1536: 9 us, a chain of six steps' latencies in 48
+// workgroups (a third buffer: the same; 32 x 32 a wave straight from memory: 8, but 18 against 12 at 500 rows).
 __global__ __launch_bounds__(256) void hidden_grad(const f16* __restrict__ xh, const bf16* __restrict__ dy,
                                                    const f16* __restrict__ aw, const bf16* __restrict__ st,
                                                    const float* __restrict__ offset, const float* __restrict__ scale,
@@ -407,7 +409,8 @@ __global__ __launch_bounds__(256) void hidden_grad(const f16* __restrict__ xh, c
 //   TURN true:  C[m][n] = sum over k of A[k][m] B[k][n]    (k rows past k_rows count as zero)
 // Split s of the k axis: k from s * k_share, to C + s * split_stride; add: C is added to. B2 takes the place
 // of B from m tile m_two on. TURN: sums[s][m] = sum over k of A[k][m] for the m tiles before m_two (by a product
-// with ones, in the workgroups of the first n tile). grid (m tiles, n tiles, splits); block 256.
+// with ones, in the workgroups of the first n tile). grid (m tiles, n tiles, splits); block 256. 2000 rows x 128 x 512: 9 us
+// (TURN) and 6.5: latency, three steps in flight.
 struct Gemm64Args {
   const bf16 *A, *B, *B2;
   float *C, *sums;
@@ -620,7 +623,7 @@ __device__ __forceinline__ void store_weight_grads(const WeightGradArgs& q, floa
 
 // Few rows: both products of E in one launch, the weights' gradients finished where they are summed. The first
 // `tiles` workgroups are those of t (m_tiles = 3 H / 64 by n_tiles = d / 64), the others those of g (m_tiles by n_tiles
-// by the splits of k). block 256.
+// by the splits of k). block 256. 100 rows x 384 x 1536: 11 us, where the two products and the join took 6, 7 and 9.
 __global__ __launch_bounds__(256) void grad_products(const Gemm64Args t, const WeightGradArgs q, const Gemm64Args g,
                                                      int tiles) {
   __shared__ __attribute__((aligned(16))) Gemm64Lds sh;
@@ -635,7 +638,9 @@ __global__ __launch_bounds__(256) void grad_products(const Gemm64Args t, const W
 
 // The same products in 128 x 128 tiles, a wave 64 x 64 of it over all k, where the matrix is made of such tiles and they
 // are enough for every CU: sixteen products a wave between two barriers, and half the reads from memory.
-// grid m tiles x n tiles x splits; block 256.
+// grid m tiles x n tiles x splits; block 256. 40000 rows x 256 x 512: 57 us (TURN; 75 before neighbours shared an XCD) and 40,
+// 0.55 and 0.52 PFLOP/s at 2.6 and 3.1 TB/s (E of 123 MB from the last-level cache, the fp32 result): the waits at the two
+// buffers' barriers, 30 to 50% of the waves' time (eight waves that split k: 81).
 template <bool TURN>
 __global__ __launch_bounds__(256, 2) void gemm128(const Gemm64Args p) {
   __shared__ __attribute__((aligned(16))) bf16 buf[2][4][64 * 64];  // A's two tiles, B's two
@@ -812,7 +817,8 @@ __device__ __forceinline__ RowsAt rows_at_of() {
 // rounded results are directly the operand [hidden x rows] of the gradients' products, whose other operand (channels
 // x rows) comes out of the same rows by transposing LDS reads, in the same order of k. No hidden value leaves the
 // registers, nothing is turned through LDS. (32 hidden channels a wave, one wave per SIMD, read half as much LDS, but
-// products and elementwise part then waited for each other: 430 us at 262144 rows x 128 x 512.)
+// products and elementwise part then waited for each other: 430 us at 262144 rows x 128 x 512, here 248: 0.83 PFLOP/s, the
+// matrix cores busy in 52% of the cycles, no LDS conflicts. A SIMD's two waves hide half of each other's elementwise part.)
 // grid (ceil(H / 128), splits): split s takes the stages s, s + splits, .. of 64 rows. block 512.
 constexpr int kStageRows = 64;
 template <int D>
@@ -987,9 +993,11 @@ __global__ __launch_bounds__(512, D == 128 ? 2 : 3) void transition_grad_weights
   }
 }
 
-// E as hidden_grad makes it, for 256 channels and many rows (20000 rows x 512: 74 -> 49 us): as above a wave keeps its operands of Aw, Bw and S^T of 16 hidden
-// channels in registers (12 D / 32 of them) and the rows stream by through LDS, D = hidden x rows (a lane holds a row at
-// 4 hidden channels). grid (ceil(H / 128), splits); block 512.
+// E as hidden_grad makes it, for 256 channels and many rows (40000 rows x 512: 58 us, 0.54 PFLOP/s, 123 MB of E at 2.1 TB/s:
+// the matrix cores are busy 27% of the cycles, the elementwise part and the stores take turns with them; 20000 rows:
+// hidden_grad 74, here 49): as above a wave keeps its operands of Aw, Bw and S^T of 16 hidden channels in
+// registers (12 D / 32 of them) and the rows stream by through LDS, D = hidden x rows (a lane holds a row at 4 hidden
+// channels). grid (ceil(H / 128), splits); block 512.
 template <int D>
 __global__ __launch_bounds__(512, 2) void hidden_stream(const f16* __restrict__ xh, const bf16* __restrict__ dy,
                                                         const f16* __restrict__ aw, const bf16* __restrict__ st,
@@ -1102,7 +1110,9 @@ __global__ __launch_bounds__(512, 2) void hidden_stream(const f16* __restrict__ 
 // waves. Per chunk: a', b', du as D = hidden x rows (a lane holds a row at 16 hidden channels), and da', db'
 // rounded are directly the operand [hidden x rows] of dxh^T = Aw^T da' + Bw^T db' (abt packed in that order of k).
 // The offset comes in by one more product step: three bf16 parts of it (24 bits) times ones. At the end the sums over
-// channels of the norm's backward pass are a lane's own registers and its partner's (lane ^ 32).
+// channels of the norm's backward pass are a lane's own registers and its partner's (lane ^ 32). 262144 rows x 128 x 512:
+// 210 us, 0.82 PFLOP/s, the matrix cores busy in 52% of the cycles; without the elementwise part it would take 180, without
+// the transfers too 150: the products, fed by one LDS read each, and the two waves of a SIMD that share it.
 // grid: persistent; block 64 NW, NW = D / 16.
 template <int D>
 struct GradChunk {
@@ -1300,7 +1310,7 @@ __global__ __launch_bounds__(4 * D, 2) void transition_grad_rows(
 }
 
 // dx = (residual ? dy : 0) + rstd (g - mean(g) - xh mean(g xh)), g the sum of `splits` fp32 parts [rows][d]: a wave a row
-// (from row `first` in steps), K = d / 64 channels a lane.
+// (from row `first` in steps), K = d / 64 channels a lane. 40000 rows of 256: 18 us, 5.6 TB/s.
 template <int K>
 __device__ __forceinline__ void norm_grad(int64_t first, int64_t step, const f16* __restrict__ xh,
                                           const float* __restrict__ rstd_in, const bf16* __restrict__ dy,
@@ -1343,7 +1353,7 @@ __global__ __launch_bounds__(64) void norm_grad_rows(const f16* __restrict__ xh,
 }
 // Few rows: dx, and the affine's gradients from grad_products' parts [count][2 d], in one launch: the first d / 8
 // workgroups sum 16 columns each (a thread every 16th part in order, then the 16 sums in order), the others take 4 rows.
-// block 256.
+// block 256. 100 rows of 384, 48 parts: 5 us, where two launches took 5 and 4.
 template <int K>
 __global__ __launch_bounds__(256) void finish_rows(const f16* __restrict__ xh, const float* __restrict__ rstd,
                                                    const bf16* __restrict__ dy, const float* __restrict__ dxh, int splits,
@@ -1374,7 +1384,8 @@ __global__ __launch_bounds__(256) void finish_rows(const f16* __restrict__ xh, c
 
 // The weights' gradients from `count` parts G [3 H][d] (da'^T xh, db'^T xh, u'^T dy) and sums [2 H] (of da', db'), and
 // eight hidden channels' shares of the affine's: part [2 H / 8][2][d]. A workgroup: 32 channels x 8 hidden channels, in Q
-// shares of the parts (0, Q, 2 Q, ..; joined in LDS in that order). grid (d / 32, 3 H / 8); block 256 Q.
+// shares of the parts (0, Q, 2 Q, ..; joined in LDS in that order). grid (d / 32, 3 H / 8); block 256 Q. 64 parts of
+// 1536 x 128: 12 us, 50 MB at 4.3 TB/s.
 template <int Q>
 __global__ __launch_bounds__(256 * Q) void join_weight_grads(const float* __restrict__ G, const float* __restrict__ sums,
                                                           int count, const float* __restrict__ wa,
@@ -1502,8 +1513,8 @@ TransitionGradPlan transition_grad_plan(int64_t rows, int d, int H) {
   TransitionGradPlan p{};
   const int64_t cus = cu_count();
   // Rows from which the fused kernels win (a workgroup walks all chunks of weights however few its rows). Separate kernels
-  // against fused ones, us: 128 x 512 channels, 8192 rows 58 / 76, 16384 rows 83 / 82; 128 x 256, 16384 rows 62 / 63; 64 x 256,
-  // 4096 rows 35 / 36, 8192 rows 44 / 41; 64 x 128, 4096 rows 31 / 28.
+  // against fused ones, us: 128 x 512 channels, 8192 rows 55 / 75, 16384 rows 78 / 81, 24576 rows 101 / 88; 128 x 256, 16384
+  // rows 57 / 61, 24576 rows 74 / 66; 64 x 256, 4096 rows 33 / 36, 16384 rows 50 / 48; 64 x 128, 4096 rows 32 / 29.
   p.fused = fused_shape(d, H) && rows >= (d == 64 ? 4096 : 16384);
   if (p.fused) {
     p.chunk = std::min<int64_t>(ceil_div(rows, 64) * 64, 1 << 18);
