@@ -640,7 +640,7 @@ __global__ __launch_bounds__(256) void grad_products(const Gemm64Args t, const W
 // are enough for every CU: sixteen products a wave between two barriers, and half the reads from memory.
 // grid m tiles x n tiles x splits; block 256. 40000 rows x 256 x 512: 57 us (TURN; 75 before neighbours shared an XCD) and 40,
 // 0.55 and 0.52 PFLOP/s at 2.6 and 3.1 TB/s (E of 123 MB from the last-level cache, the fp32 result): the waits at the two
-// buffers' barriers, 30 to 50% of the waves' time (eight waves that split k: 81).
+// buffers' barriers, 38 and 52% of the waves' time (eight waves that split k: 81).
 template <bool TURN>
 __global__ __launch_bounds__(256, 2) void gemm128(const Gemm64Args p) {
   __shared__ __attribute__((aligned(16))) bf16 buf[2][4][64 * 64];  // A's two tiles, B's two

@@ -22,6 +22,9 @@ Modules
                product's ``output_w``), restated independently of ``pairstack``;
                it pins the released-to-engine conversion.
 
+``training``   fp64 8-bit activations and backward passes of LayerNorm and the
+               transition, written out from the formulas.
+
 Pinning status (what each function is checked against, in ``tests/test_oracle.py``
 and ``tests/test_released.py``):
 
@@ -49,6 +52,9 @@ and ``tests/test_released.py``):
                             schedule equals the sum of the ops' updates.
 * ``released``              the converted engine modules on the ``pytorch``
                             backend match it (2e-5 per op, 1e-4 per block).
+* ``training``              autograd in fp64, differences, torch's own e4m3, and
+                            half a step's bound of the codes
+                            (``tests/test_training_oracle.py``).
 
 Conventions the reference leaves open (engine ``pytorch`` backend outputs at
 padded positions are not pinned by any reference test, which compare valid
