@@ -279,9 +279,7 @@ TransitionGradArgs transition_grad_ws(void* ws, size_t* bytes, const TransitionG
   Carver cv{static_cast<char*>(ws)};
   TransitionGradArgs a{};
   const size_t w = (size_t)hidden * d;
-  a.peaks = cv.take<float>((size_t)hidden / 2);
   a.scale = cv.take<float>(2 * (size_t)hidden);
-  a.offset = cv.take<float>(2 * (size_t)hidden);
   a.shift = cv.take<float>(2 * (size_t)hidden);
   a.aw = cv.take<f16>(2 * w);
   a.st = cv.take<bf16>(w);
@@ -294,8 +292,10 @@ TransitionGradArgs transition_grad_ws(void* ws, size_t* bytes, const TransitionG
   else
     a.E = cv.take<bf16>((size_t)p.chunk * 3 * hidden);
   a.dxh = cv.take<float>((size_t)p.dxh_splits * p.chunk * d);
-  a.dw_part = cv.take<float>((size_t)p.dw_splits * 3 * w);
-  a.sums = cv.take<float>((size_t)p.dw_splits * 2 * hidden);
+  if (!p.few) {
+    a.dw_part = cv.take<float>((size_t)p.dw_splits * 3 * w);
+    a.sums = cv.take<float>((size_t)p.dw_splits * 2 * hidden);
+  }
   a.norm_part = cv.take<float>((size_t)hidden / 4 * 2 * d);
   *bytes = cv.used;
   return a;

@@ -433,7 +433,7 @@ struct TransitionGradArgs {
   int d, hidden, residual, grad_dtype;
   float eps;
   // workspace: the weights in the products' orders and their scales,
-  float *peaks, *scale, *offset, *shift;  // [hidden / 2], [2 hidden], [2 hidden], [2 hidden]
+  float *scale, *shift;                 // [2 hidden] each
   f16* aw;                              // [2 hidden][d]
   bf16 *st, *abt;                       // [hidden][d], [d][2 hidden]
   bf16* split;                          // [2][hidden][8] (fused)

@@ -12,7 +12,7 @@
 //   dv = A^T (sum da) + B^T (sum db)
 // so dw and dv come out of the weights' gradients, and the products see xh alone, whose values are at most
 // sqrt(d): a and b are products of fp16 operands (Aw and Bw times a power of two that puts their largest
-// entry, of the matrix or of a hidden channel's row, at 2^14 .. 2^15, so that entries down to 2^-29 of it keep
+// entry, of a hidden channel's row or of 32 of them, at 2^14 .. 2^15, so that entries down to 2^-29 of it keep
 // fp16's 11 bits), which leaves their errors at an eighth of bf16's. The gradients' operands are bf16, whose
 // range they need: three bf16 roundings lie between dy and a gradient, and one of the result (relative error
 // 3.3e-3 rather than the 4.6e-3 of bf16 throughout).
@@ -91,37 +91,15 @@ __device__ __forceinline__ float two_to(int k) { return __uint_as_float((uint32_
 // What a call makes of its parameters.
 struct WeightArgs {
   const float *wa, *wb, *ws, *w, *v;  // A, B [H][d], S [d][H]; the norm's weight and bias
-  float *offset, *peaks;              // (weight_rows)
   f16* aw;
-  bf16 *st, *abt;
+  bf16 *st, *abt, *split;
   float *shift, *scale;
   int d, H;
 };
 
-// Of each row h of A and B: offset [2][H] = the row's product with v, and of each four rows (a workgroup's) the largest
-// |A w| or |offset| in peaks [2][H / 4]: a', b' <= 2^15 (1 + d) whatever w, v and the weights are, so no product of theirs
-// leaves fp32. One wave a row; block 256, 2 H / 4 of them.
-__device__ __forceinline__ void weight_rows(int block, const WeightArgs& q) {
-  __shared__ float red[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = block * 4 + wave, d = q.d, H = q.H;
-  const float* row = (h < H ? q.wa : q.wb) + (int64_t)(h < H ? h : h - H) * d;
-  float top = 0.f, dot = 0.f;
-#pragma unroll 4
-  for (int c = lane; c < d; c += 64) {
-    const float t = row[c];
-    top = fmaxf(top, finite_abs(t * q.w[c]));
-    dot += t * q.v[c];
-  }
-  dot = lanes_sum<64>(dot);
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
-  if (lane == 0) {
-    q.offset[h] = dot;
-    red[wave] = fmaxf(top, finite_abs(dot));
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) q.peaks[block] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-}
+// hidden channels of a packing workgroup
+template <bool FUSED>
+constexpr int kPackGroup = FUSED ? 32 : 8;
 
 // A 32 x 32 tile of S^T [H][d] in bf16. block 256.
 __device__ __forceinline__ void turn_squeeze(const WeightArgs& q, int h0, int c0, float (&tile)[32][33]) {
@@ -131,28 +109,33 @@ __device__ __forceinline__ void turn_squeeze(const WeightArgs& q, int h0, int c0
   for (int r = row; r < 32; r += 8) q.st[(int64_t)(h0 + r) * q.d + c0 + col] = (bf16)tile[col][r];
 }
 
-// The parameters in the orders the separate kernels read, each hidden channel with powers ka, kb of its own, so that
-// one pass over them does it all: aw [2 H][d] fp16 (Aw 2^ka, then Bw 2^kb), shift [2][H] (the offsets so scaled), scale
-// [2][H] = {2^-ka, 2^-kb}, abt [d][2 H] bf16 (Aw^T 2^-kb, Bw^T 2^-ka), st [H][d] bf16 (S^T). H / 8 workgroups of 8
-// hidden channels, a wave 2 of them in registers, then H / 32 x d / 32 of a tile of S^T. block 256. (In one launch with the
-// rows 8.0 us at 384 x 4, in a launch after it 4.1 + 7.1; with abt in pieces of 4 hidden channels 11.)
-template <int K>
+// The parameters in the orders the products read, each hidden channel (FUSED: each 32 of them, the rows kernel's chunk)
+// with powers ka, kb of its own, so that one pass over them does it all: aw [2 H][d] fp16 (Aw 2^ka, then Bw 2^kb), shift
+// [2][H] (the offsets A v, B v so scaled), scale [2][H] = {2^-ka, 2^-kb}, abt [d][2 H] bf16 (Aw^T 2^-kb, Bw^T 2^-ka), st
+// [H][d] bf16 (S^T). FUSED: abt within each 16 hidden channels in accumulator order 0-3, 8-11, 4-7, 12-15, and split
+// [2][H][8] bf16 = {the scaled offset in three parts, 2^-ka, 0, ..}. The peaks count the offsets, so a', b' <= 2^15 (1 + d)
+// whatever w, v and the weights are, and no product of theirs leaves fp32. H / G workgroups of G hidden channels, a
+// quarter of them in a wave's registers, then H / 32 x d / 32 of a tile of S^T. block 256. (In one launch with the rows 8.0 us
+// at 384 x 4, in a launch after it 4.1 + 7.1; with abt in pieces of 4 hidden channels 11.)
+template <int K, bool FUSED>
 __device__ __forceinline__ void pack_rows(int block, const WeightArgs& q) {
-  constexpr int d = 64 * K;
-  __shared__ __attribute__((aligned(16))) bf16 turned[2][d][8];
+  constexpr int d = 64 * K, N = FUSED ? 8 : 2, G = kPackGroup<FUSED>;
+  static_assert(G == 4 * N, "a quarter a wave");
+  __shared__ __attribute__((aligned(16))) bf16 turned[2][d][FUSED ? G + 8 : G];
   const int H = q.H;
-  if (block >= H / 8) {
-    const int t = block - H / 8;
+  if (block >= H / G) {
+    const int t = block - H / G;
     __shared__ float tile[32][33];
     turn_squeeze(q, t % (H / 32) * 32, t / (H / 32) * 32, tile);
     return;
   }
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h0 = 8 * block + 2 * wave;
-  float t[2][2][K], up[2][2], down[2][2], w[K], v[K];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h0 = G * block + N * wave;
+  float t[2][N][K], dot[2][N], w[K], v[K];
+  int power[2][N];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+    for (int r = 0; r < N; ++r)
 #pragma unroll
       for (int k = 0; k < K; ++k) t[m][r][k] = (m ? q.wb : q.wa)[(int64_t)(h0 + r) * d + lane + 64 * k];
 #pragma unroll
@@ -160,104 +143,81 @@ __device__ __forceinline__ void pack_rows(int block, const WeightArgs& q) {
     w[k] = q.w[lane + 64 * k];
     v[k] = q.v[lane + 64 * k];
   }
+  float peak[2] = {0.f, 0.f};
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      float top = 0.f, dot = 0.f;
+    for (int r = 0; r < N; ++r) {
+      float top = 0.f, sum = 0.f;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        dot += t[m][r][k] * v[k];
+        sum += t[m][r][k] * v[k];
         t[m][r][k] *= w[k];
         top = fmaxf(top, finite_abs(t[m][r][k]));
       }
-      dot = lanes_sum<64>(dot);
+      dot[m][r] = lanes_sum<64>(sum);
+      top = fmaxf(top, finite_abs(dot[m][r]));
+      if constexpr (FUSED) {
+        peak[m] = fmaxf(peak[m], top);
+      } else {
 #pragma unroll
-      for (int x = 32; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
-      const int power = peak_power(fmaxf(top, finite_abs(dot)));
-      up[m][r] = two_to(power);
-      down[m][r] = two_to(-power);
-      if (lane == 0) {
-        q.shift[m * H + h0 + r] = dot * up[m][r];
-        q.scale[m * H + h0 + r] = down[m][r];
+        for (int x = 32; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
+        power[m][r] = peak_power(top);
       }
     }
+  if constexpr (FUSED) {
+    __shared__ float red[2][4];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+#pragma unroll
+      for (int x = 32; x >= 1; x >>= 1) peak[m] = fmaxf(peak[m], __shfl_xor(peak[m], x, 64));
+      if (lane == 0) red[m][wave] = peak[m];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int r = 0; r < N; ++r)
+        power[m][r] = peak_power(fmaxf(fmaxf(red[m][0], red[m][1]), fmaxf(red[m][2], red[m][3])));
+  }
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+    for (int r = 0; r < N; ++r) {
+      const int h = m * H + h0 + r, place = N * wave + r;
+      const float up = two_to(power[m][r]), down = two_to(-power[1 - m][r]);
+      if (lane == 0) {
+        float o = dot[m][r] * up;
+        q.shift[h] = o;
+        q.scale[h] = two_to(-power[m][r]);
+        if constexpr (FUSED) {
+          bf16x8 parts;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            parts[e] = (bf16)(e < 3 ? o : 0.f);
+            o -= (float)parts[e];
+          }
+          if (m == 0) parts[3] = (bf16)two_to(-power[m][r]);
+          *reinterpret_cast<bf16x8*>(q.split + 8 * (int64_t)h) = parts;
+        }
+      }
+      const int at = FUSED ? (place & ~12) | ((place & 4) << 1) | ((place & 8) >> 1) : place;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        q.aw[(int64_t)(m * H + h0 + r) * d + lane + 64 * k] = (f16)(t[m][r][k] * up[m][r]);
-        turned[m][lane + 64 * k][2 * wave + r] = (bf16)(t[m][r][k] * down[1 - m][r]);
+        q.aw[(int64_t)h * d + lane + 64 * k] = (f16)(t[m][r][k] * up);
+        turned[m][lane + 64 * k][at] = (bf16)(t[m][r][k] * down);
       }
-  __syncthreads();
-  for (int i = threadIdx.x; i < 2 * d; i += 256) {
-    const int m = i >= d, c = m ? i - d : i;
-    *reinterpret_cast<bf16x8*>(q.abt + (int64_t)c * 2 * H + m * H + 8 * block) =
-        *reinterpret_cast<const bf16x8*>(&turned[m][c][0]);
-  }
-}
-
-// The same for the fused kernels, with one ka and kb of all hidden channels (the rows kernel holds 16 channels of a row in
-// a lane: a scale each would be an operand more): abt within each 16 hidden channels in accumulator order 0-3, 8-11, 4-7,
-// 12-15, and the scaled offsets as fp32 in shift and in three bf16 parts, split [2][H][8] = {hi, mid, lo, 0, ..}. A 32 x 32
-// tile of one matrix a workgroup: grid (H / 32, d / 32, 3); block 256.
-__global__ __launch_bounds__(256) void pack_grad_weights(const WeightArgs q, bf16* __restrict__ split) {
-  __shared__ float tile[32][33], red[2][4];
-  const int h0 = blockIdx.x * 32, c0 = blockIdx.y * 32, which = blockIdx.z, d = q.d, H = q.H;
-  const int col = threadIdx.x & 31, row = threadIdx.x >> 5;
-  if (which == 2) {
-    turn_squeeze(q, h0, c0, tile);
-    return;
-  }
-  float t[4];
-  const float* src = which ? q.wb : q.wa;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) t[i] = src[(int64_t)(h0 + row + 8 * i) * d + c0 + col];
-  const float wc = q.w[c0 + col];
-  float peak[2] = {0.f, 0.f};
-#pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    for (int i = threadIdx.x; i < H / 4; i += 256) peak[m] = fmaxf(peak[m], q.peaks[m * (H / 4) + i]);
-#pragma unroll
-    for (int x = 32; x >= 1; x >>= 1) peak[m] = fmaxf(peak[m], __shfl_xor(peak[m], x, 64));
-    if ((threadIdx.x & 63) == 0) red[m][threadIdx.x >> 6] = peak[m];
-  }
-  __syncthreads();
-  int k[2];
-#pragma unroll
-  for (int m = 0; m < 2; ++m)
-    k[m] = peak_power(fmaxf(fmaxf(red[m][0], red[m][1]), fmaxf(red[m][2], red[m][3])));
-  const float up = two_to(which ? k[1] : k[0]), down = two_to(which ? -k[0] : -k[1]);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = row + 8 * i;
-    tile[r][col] = t[i] * wc;
-    q.aw[(int64_t)(which * H + h0 + r) * d + c0 + col] = (f16)(t[i] * wc * up);
-  }
-  if (c0 == 0 && threadIdx.x < 32) {
-    const int h = which * H + h0 + threadIdx.x;
-    float o = q.offset[h] * up;
-    q.shift[h] = o;
-    q.scale[h] = two_to(which ? -k[1] : -k[0]);
-    bf16x8 parts;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      parts[e] = (bf16)(e < 3 ? o : 0.f);
-      o -= (float)parts[e];
     }
-    *reinterpret_cast<bf16x8*>(split + 8 * (int64_t)h) = parts;
-  }
   __syncthreads();
-  // hidden channel of place `col` of the accumulator order
-  const int hid = (col & ~12) | ((col & 4) << 1) | ((col & 8) >> 1);
-  for (int r = row; r < 32; r += 8)
-    q.abt[(int64_t)(c0 + r) * 2 * H + which * H + h0 + col] = (bf16)(tile[hid][r] * down);
+  for (int i = threadIdx.x; i < 2 * d * (G / 8); i += 256) {
+    const int piece = i % (G / 8), c = i / (G / 8) % d, m = i / (G / 8) / d;
+    *reinterpret_cast<bf16x8*>(q.abt + (int64_t)c * 2 * H + m * H + G * block + 8 * piece) =
+        *reinterpret_cast<const bf16x8*>(&turned[m][c][8 * piece]);
+  }
 }
 
-// What a call makes of its inputs first, in one launch: the weights (the first `weight_blocks` workgroups: weight_rows or
-// pack_rows), and xh in fp16 and bf16 and rstd of the kept rows: 8 lanes a row, K = d / 64 pieces of 8 channels each,
+// What a call makes of its inputs first, in one launch: the weights (the first `weight_blocks` workgroups: pack_rows),
+// and xh in fp16 and bf16 and rstd of the kept rows: 8 lanes a row, K = d / 64 pieces of 8 channels each,
 // the other workgroups grid-strided over rows. block 256 (32 rows). 262144 8-bit rows of 128: 31 us, 5.4 TB/s.
 template <bool CODES, int K, bool FUSED>
 __global__ __launch_bounds__(256) void norm_rows(const void* x, const uint8_t* scales, f16* __restrict__ xh,
@@ -265,10 +225,7 @@ __global__ __launch_bounds__(256) void norm_rows(const void* x, const uint8_t* s
                                                  float eps, int weight_blocks, const WeightArgs q) {
   constexpr int d = 64 * K, blocks = d / kActBlock;
   if ((int)blockIdx.x < weight_blocks) {
-    if constexpr (FUSED)
-      weight_rows(blockIdx.x, q);
-    else
-      pack_rows<K>(blockIdx.x, q);
+    pack_rows<K, FUSED>(blockIdx.x, q);
     return;
   }
   const int sub = threadIdx.x & 7;
@@ -862,11 +819,11 @@ __global__ __launch_bounds__(512, D == 128 ? 2 : 3) void transition_grad_weights
     wb[kk] = ld8h(aw + (int64_t)(H + hr) * D + 32 * kk + 8 * q);
     ws[kk] = ld8(st + (int64_t)hr * D + 32 * kk + 8 * q);
   }
-  const float oa = offset[hr], ob = offset[H + hr], ia = scale[0], slow = -kLog2e * ia;
+  const float oa = offset[hr], ob = offset[H + hr], ia = scale[hr], slow = -kLog2e * ia;
   // the parameters have landed: without this the compiler waits for them again in every stage
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) asm volatile("" ::"v"(wa[kk]), "v"(wb[kk]), "v"(ws[kk]));
-  asm volatile("" ::"v"(oa), "v"(ob), "v"(slow));
+  asm volatile("" ::"v"(oa), "v"(ob), "v"(ia));
   const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f}, oa4 = {oa, oa, oa, oa}, ob4 = {ob, ob, ob, ob};
   f32x4 ga[CT], gb[CT], gs[CT];
 #pragma unroll
@@ -1127,17 +1084,15 @@ template <int D>
 __global__ __launch_bounds__(4 * D, 2) void transition_grad_rows(
     const f16* __restrict__ xh, const bf16* __restrict__ dy, const float* __restrict__ rstd_in,
     const f16* __restrict__ aw, const bf16* __restrict__ st, const bf16* __restrict__ abt,
-    const bf16* __restrict__ split, const float* __restrict__ scale, bf16* __restrict__ dx, int64_t rows, int H,
-    int residual) {
+    const bf16* __restrict__ split, bf16* __restrict__ dx, int64_t rows, int H, int residual) {
   constexpr int NW = D / 16, KK = D / 16, CT = D / 32, P = D / 8;
   __shared__ __attribute__((aligned(256))) GradChunk<D> W[2];
-  extern __shared__ __attribute__((aligned(16))) bf16 off_lds[];  // [2][H][8]: the offsets' parts
+  extern __shared__ __attribute__((aligned(16))) bf16 off_lds[];  // [2][H][8]: the offsets' parts and 2^-ka
   const int lane = threadIdx.x & 63, g = lane >> 5, li = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t lds = lds_addr(W);
   const int chunks = H / 32;
   const uint32_t rows_at = 2 * off_row<D>(li, g), narrow_at = 2 * off_narrow(li, g);  // a lane's places in a chunk
-  const float ia = scale[0], slow = -kLog2e * ia;
   for (int i = threadIdx.x; i < 2 * H; i += 64 * NW)
     *reinterpret_cast<bf16x8*>(off_lds + 8 * i) = ld8(split + 8 * (int64_t)i);
   // a wave's transfers of a chunk, one KB of each of its five arrays (u = 0 .. 4)
@@ -1190,6 +1145,7 @@ __global__ __launch_bounds__(4 * D, 2) void transition_grad_rows(
       f32x16 a = zero16(), bb = zero16(), du = zero16();
       a = mfma32(ld8(off_lds + 8 * (32 * c + li)), ones, a);
       bb = mfma32(ld8(off_lds + 8 * (H + 32 * c + li)), ones, bb);
+      const float ia = (float)off_lds[8 * 32 * c + 3], slow = -kLog2e * ia;
       f16x8 la[2], lb[2];
       bf16x8 ls[2], lt[2][2];
       auto take = [&](int kk) __attribute__((always_inline)) {
@@ -1448,7 +1404,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 template <bool CODES>
 void run_norm_rows(const TransitionGradArgs& a, const void* x, const uint8_t* scales, int64_t rows, bool weights,
                    bool fused, const WeightArgs& q, hipStream_t st) {
-  const int extra = !weights ? 0 : fused ? 2 * q.H / 4 : q.H / 8 + q.H / 32 * (q.d / 32);
+  const int extra = !weights ? 0 : q.H / (fused ? kPackGroup<true> : kPackGroup<false>) + q.H / 32 * (q.d / 32);
   const dim3 grid((unsigned)(extra + std::min<int64_t>(ceil_div(rows, 32), (int64_t)cu_count() * 16)));
   const auto run = [&](auto kernel) { kernel<<<grid, 256, 0, st>>>(x, scales, a.xh, a.xhb, a.rstd, rows, a.eps, extra, q); };
   if (fused) return a.d == 64 ? run(norm_rows<CODES, 1, true>) : run(norm_rows<CODES, 2, true>);
@@ -1502,7 +1458,7 @@ void launch_fused(const TransitionGradArgs& a, const TransitionGradPlan& p, cons
   const int held = resident_blocks(reinterpret_cast<const void*>(rows_kernel), 64 * NW, grad_rows_lds<D>(H));
   const int64_t tiles = ceil_div(rows, 32 * NW);
   rows_kernel<<<dim3((unsigned)std::min<int64_t>(tiles, (int64_t)cu_count() * held)), 64 * NW, grad_rows_lds<D>(H), st>>>(
-      a.xh, dy, a.rstd, a.aw, a.st, a.abt, a.split, a.scale, dx, rows, H, a.residual);
+      a.xh, dy, a.rstd, a.aw, a.st, a.abt, a.split, dx, rows, H, a.residual);
   transition_grad_weights<D><<<dim3((unsigned)ceil_div(H, 128), (unsigned)p.dw_splits), 512, 0, st>>>(
       a.xh, a.xhb, dy, a.aw, a.st, a.shift, a.scale, a.dw_part, a.sums, rows, H, add);
 }
@@ -1513,8 +1469,8 @@ TransitionGradPlan transition_grad_plan(int64_t rows, int d, int H) {
   TransitionGradPlan p{};
   const int64_t cus = cu_count();
   // Rows from which the fused kernels win (a workgroup walks all chunks of weights however few its rows). Separate kernels
-  // against fused ones, us: 128 x 512 channels, 8192 rows 55 / 75, 16384 rows 78 / 81, 24576 rows 101 / 88; 128 x 256, 16384
-  // rows 57 / 61, 24576 rows 74 / 66; 64 x 256, 4096 rows 33 / 36, 16384 rows 50 / 48; 64 x 128, 4096 rows 32 / 29.
+  // against fused ones, us: 128 x 512 channels, 8192 rows 55 / 75, 16384 rows 79 / 81, 24576 rows 101 / 89; 128 x 256, 16384
+  // rows 57 / 62, 24576 rows 74 / 67; 64 x 256, 4096 rows 33 / 35, 8192 rows 40 / 37; 64 x 128, 4096 rows 32 / 28.
   p.fused = fused_shape(d, H) && rows >= (d == 64 ? 4096 : 16384);
   if (p.fused) {
     p.chunk = std::min<int64_t>(ceil_div(rows, 64) * 64, 1 << 18);
@@ -1547,13 +1503,12 @@ void launch_transition_grad(const TransitionGradArgs& a, const TransitionGradPla
     const void* xc = x + r0 * d * (a.scales ? 1 : 2);
     const bf16* dy = a.dy + r0 * d;
     const int add = r0 > 0;
-    const WeightArgs w{a.wa, a.wb, a.ws, a.ln_w, a.ln_b, a.offset, a.peaks, a.aw, a.st, a.abt, a.shift, a.scale, d, H};
+    const WeightArgs w{a.wa, a.wb, a.ws, a.ln_w, a.ln_b, a.aw, a.st, a.abt, a.split, a.shift, a.scale, d, H};
     if (a.scales)
       run_norm_rows<true>(a, xc, a.scales + r0 * (d / kActBlock), rows, r0 == 0, p.fused, w, st);
     else
       run_norm_rows<false>(a, xc, nullptr, rows, r0 == 0, p.fused, w, st);
     if (p.fused) {
-      if (r0 == 0) pack_grad_weights<<<dim3(H / 32, d / 32, 3), 256, 0, st>>>(w, a.split);
       if (d == 64)
         launch_fused<64>(a, p, dy, a.dx + r0 * d, rows, add, st);
       else

@@ -578,7 +578,7 @@ def transition_backward(
 ) -> TransitionGradients:
     """Gradients of :func:`transition` from the output's gradient ``dy [..., d]`` bf16 and the kept input
     ``x``: the bf16 tensor itself or its 8-bit activation (the gradient at the restored values). The hidden
-    rows are computed again; products on bf16 operands, fp32 sums in a fixed order. The parameters'
+    rows are computed again; products on fp16 and bf16 operands, fp32 sums in a fixed order. The parameters'
     gradients in ``grad_dtype``. d a multiple of 64 up to 768."""
     rows, d, dev = _rows_tensor(dy, "dy"), dy.shape[-1], dy.device
     if dy.dtype != torch.bfloat16:

@@ -276,9 +276,9 @@ int32_t ffk_transition_noalloc(const void* x, const float* ln_w, const float* ln
  *   dx = (residual ? dy : 0) + (LayerNorm's backward of dn), dln_w, dln_b its affine's
  * x: the bf16 input (scales NULL) or the codes of its 8-bit activation with their scales; dy, dx
  * [rows, d] bf16; parameters as in ffk_transition; their gradients in grad_dtype (FFK_DTYPE_*), shaped
- * like the parameters. The hidden rows are computed again from x: nothing else is kept. Products on bf16
- * operands with fp32 sums in a fixed order. d a multiple of 64 up to 768, factor * d of 64. dx aliases
- * nothing. Reference: the training path's gradient of the transition (train/step.py:320-338).
+ * like the parameters. The hidden rows are computed again from x: nothing else is kept. Products on fp16
+ * (a, b) and bf16 operands with fp32 sums in a fixed order. d a multiple of 64 up to 768, factor up to 64;
+ * x, dy, dx and dw_squeeze 16-byte aligned. dx aliases nothing. Reference: the training path's gradient of the transition (train/step.py:320-338).
  */
 size_t ffk_transition_backward_workspace(int64_t rows, int32_t d, int32_t factor);
 int32_t ffk_transition_backward(const void* dy, const void* x, const void* scales, const float* ln_w,

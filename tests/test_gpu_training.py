@@ -440,6 +440,26 @@ def test_on_another_stream():
     assert all(torch.equal(a, b) for a, b in zip((*want, *norm), (*got, *got_norm)))
 
 
+@pytest.mark.parametrize("rows,d,factor", [(100, 384, 4), (1, 64, 2), (2000, 128, 4), (4200, 64, 4), (16500, 128, 4),
+                                           (4500, 256, 2)])
+def test_every_form_captured(rows, d, factor):
+    """Each form's call in a graph, replayed on new inputs and parameters."""
+    x, dy, params = _transition_case(rows, d, factor, rows)
+    x, dy, dev = x.to(DEV), dy.to(DEV), {k: v.to(DEV) for k, v in params.items()}
+    kernels.transition_backward(dy, x, **dev)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = kernels.transition_backward(dy, x, **dev)
+    for turn in range(3):
+        x.copy_(torch.randn_like(x))
+        dev["expand_a"].mul_(0.75)
+        want = kernels.transition_backward(dy, x, **dev)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), turn
+
+
 def test_two_graphs_replayed():
     """Two captured steps, replayed in turn with eager work between them, on new inputs each time."""
     cases = []
