@@ -779,13 +779,11 @@ __device__ __forceinline__ RowsAt rows_at_of() {
 // grid (ceil(H / 128), splits): split s takes the stages s, s + splits, .. of 64 rows. block 512.
 constexpr int kStageRows = 64;
 template <int D>
-constexpr int kWeightBuffers = D == 128 ? 3 : 2;
-template <int D>
-__global__ __launch_bounds__(512, D == 128 ? 2 : 3) void transition_grad_weights(
+__global__ __launch_bounds__(512, 2) void transition_grad_weights(
     const f16* __restrict__ xh, const bf16* __restrict__ xhb, const bf16* __restrict__ dy, const f16* __restrict__ aw,
     const bf16* __restrict__ st, const float* __restrict__ offset, const float* __restrict__ scale,
     float* __restrict__ G, float* __restrict__ sums, int64_t rows, int H, int add) {
-  constexpr int NB = kWeightBuffers<D>, NW = 8, KK = D / 32, CT = D / 16;
+  constexpr int NB = 3, NW = 8, KK = D / 32, CT = D / 16;
   constexpr int kTile = kStageRows * D;              // elements of a tile
   constexpr int kLoads = 3 * (kTile / 512) / NW;     // transfers of a wave a stage
   __shared__ __attribute__((aligned(256))) bf16 buf[NB][3][kTile];  // xh fp16, xh bf16, dy
@@ -1470,12 +1468,14 @@ TransitionGradPlan transition_grad_plan(int64_t rows, int d, int H) {
   const int64_t cus = cu_count();
   // Rows from which the fused kernels win (a workgroup walks all chunks of weights however few its rows). Separate kernels
   // against fused ones, us: 128 x 512 channels, 8192 rows 55 / 75, 16384 rows 79 / 81, 24576 rows 101 / 89; 128 x 256, 16384
-  // rows 57 / 62, 24576 rows 74 / 67; 64 x 256, 4096 rows 33 / 35, 8192 rows 40 / 37; 64 x 128, 4096 rows 32 / 28.
+  // rows 57 / 62, 24576 rows 74 / 67; 64 x 256, 4096 rows 33 / 34, 8192 rows 40 / 37; 64 x 128, 4096 rows 32 / 28.
   p.fused = fused_shape(d, H) && rows >= (d == 64 ? 4096 : 16384);
   if (p.fused) {
     p.chunk = std::min<int64_t>(ceil_div(rows, 64) * 64, 1 << 18);
     const int64_t groups = ceil_div(H, 128);
-    p.dw_splits = (int)std::max<int64_t>(1, std::min<int64_t>((d == 64 ? 2 : 1) * cus / groups, p.chunk / kStageRows));
+    // a workgroup a CU (its registers let no second one run beside it: 49152 rows x 64 x 256 in twice as many parts 60.5 us,
+    // so 52.6), two stages each at least (4096 rows: one 35.5, two 33.6)
+    p.dw_splits = (int)std::max<int64_t>(1, std::min<int64_t>(cus / groups, p.chunk / (2 * kStageRows)));
     return p;
   }
   // E of a chunk within 192 MB, so that much of it is still in the 256 MB last-level cache when the products read it, in
