@@ -8,8 +8,8 @@
 // 33 / 32 bytes a value), dy and dx once each.
 //
 // A row is held by L lanes, P pieces each, as in the forward kernel: 16-byte pieces where the width is
-// one of the stacks' (64 to 768 channels) and the tensors are aligned, single values (L = 64) for any other
-// width up to 1024. A workgroup walks over rows and fetches the next ones while it works on the current
+// one of the stacks' (64 to 768 channels, and 1536 in bf16) and the tensors are aligned, single values (L = 64) for
+// any other width up to 1024. A workgroup walks over rows and fetches the next ones while it works on the current
 // ones; every lane keeps the sums of dw and db of its channels in registers over all its rows, the
 // workgroup joins them in LDS at the end and writes one row of partial sums, and a second kernel adds those
 // in a fixed order (the same result on every run). One workgroup writes the gradients itself. Wider rows
@@ -485,13 +485,16 @@ RowForm grad_form(const LayerNormGradArgs& a) {
 
 }  // namespace
 
-// The workspace holds the partial sums of whichever form the call takes: single values make the most
-// workgroups of few rows each (a step of 4 rows: up to 4 rows are one workgroup, which needs none), and the wide
-// rows' statistics come behind the sums.
+// The workspace holds the partial sums of whichever form the call takes (types and alignment are not known here): rows in
+// registers make at most a workgroup for every 4 rows (form_rows), one alone needs none, and the wide rows' statistics come
+// behind their sums. Beyond 1024 channels a width may still be one of the 16-byte pieces' (bf16 rows of 1536).
 size_t layer_norm_grad_floats(int64_t rows, int cols) {
-  if (cols > 1024) return (size_t)64 * 2 * cols + 2 * (size_t)rows;
   const int64_t parts = std::min<int64_t>((rows + 3) / 4, (int64_t)cu_count() * kGradBlocksPerCu);
-  return parts <= 1 ? 0 : (size_t)parts * 2 * cols;
+  const size_t held = parts <= 1 ? 0 : (size_t)parts * 2 * cols;
+  if (cols <= 1024) return held;
+  const size_t wide = (size_t)64 * 2 * cols + 2 * (size_t)rows;
+  const bool pieces = row_form(cols, 8, true) != kFormWide || row_form(cols, 4, true) != kFormWide;
+  return pieces ? std::max(held, wide) : wide;
 }
 
 void launch_sum_partials(const float* part, int count, int width, int split, void* out0, void* out1, int dtype,

@@ -158,6 +158,23 @@ def test_layer_norm_backward_many_rows(rows, cols, dtype):
     _check_norm(x, dy, w, kernels.quantize_activation(x.to(DEV)))
 
 
+@pytest.mark.parametrize("rows,dtype,off", [(3, BF16, 0), (257, BF16, 0), (300, BF16, 0), (5003, BF16, 0), (300, BF16, 1),
+                                           (300, F32, 0)])
+def test_layer_norm_backward_1536_channels(rows, dtype, off):
+    """The widest rows that lie in registers (bf16, aligned): each of up to 1024 workgroups has a part of the affine's
+    sums. Off alignment and in fp32 the same width takes the wide form."""
+    cols = 1536
+    g = torch.Generator().manual_seed(rows)
+    x, dy = _stream_rows(g, rows, cols, dtype), torch.randn(rows, cols, generator=g).to(dtype)
+    w = 1 + 0.1 * torch.randn(cols, generator=g)
+    moved = torch.empty(off + x.numel(), dtype=dtype, device=DEV)[off:].view(rows, cols)
+    moved.copy_(x)
+    first = _check_norm(x, dy, w, moved)
+    again = kernels.layer_norm_backward(dy.to(DEV), moved, w.to(DEV))
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    _check_norm(x, dy, w, kernels.layer_norm_checkpoint(x.to(DEV), w.to(DEV), None)[1], grad_dtype=BF16)
+
+
 def test_layer_norm_backward_forms():
     g = torch.Generator().manual_seed(3)
     x, dy = _stream_rows(g, 6 * 5, 128, BF16).view(2, 3, 5, 128), torch.randn(2, 3, 5, 128, generator=g).to(BF16)

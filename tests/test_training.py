@@ -139,6 +139,23 @@ def test_workspaces():
     assert lib.ffk_transition_backward_workspace(1 << 30, 256, 4) == lib.ffk_transition_backward_workspace(1 << 26, 256, 4)
 
 
+@pytest.mark.parametrize("cols", [1024, 1025, 1536, 1600, 2048])
+@pytest.mark.parametrize("rows", [1, 4, 256, 257, 300, 1000, 1 << 20])
+def test_layer_norm_backward_workspace_holds_every_form(rows, cols):
+    """Whichever form a call takes, by its type and its tensors' alignment: rows of up to 1024 channels, and bf16 rows
+    of 1536 in 16-byte pieces, lie in registers, up to 4 workgroups a CU (256 without a device) of 4 rows at least,
+    each with a row of sums of two gradients; others have 64 such rows and every row's mean and rstd."""
+    if not build.LIBRARY.exists():
+        build.build()
+    floats = 0
+    if cols <= 1024 or cols == 1536:
+        parts = min(-(-rows // 4), 1024)
+        floats = parts * 2 * cols if parts > 1 else 0
+    if cols > 1024:
+        floats = max(floats, 64 * 2 * cols + 2 * rows)
+    assert _native.lib().ffk_layer_norm_backward_workspace(rows, cols) >= 4 * floats
+
+
 def test_install_and_take_back():
     block = randomise(factories.pairformer_block(d_pair=64, triangle_model="af3", d_single=128), 0)
     block.set_backend("hip")
