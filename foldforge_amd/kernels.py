@@ -558,9 +558,10 @@ class TransitionGradients(NamedTuple):
 
 def transition_checkpoint(x: Tensor, *, residual: bool = True, eps: float = 1e-5,
                           **params: Tensor) -> tuple[Tensor, Activation8]:
-    """:func:`transition` of ``x`` and the 8-bit activation of ``x`` that its backward pass takes."""
-    out = transition(x, residual=residual, eps=eps, **params)
-    return out, quantize_activation(x)
+    """:func:`transition` of ``x`` and the 8-bit activation of ``x`` that its backward pass takes (taken first: ``out=``
+    may be ``x``)."""
+    a = quantize_activation(x)
+    return transition(x, residual=residual, eps=eps, **params), a
 
 
 def transition_backward(

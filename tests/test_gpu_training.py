@@ -441,6 +441,23 @@ def test_transition_checkpoint_is_the_forward():
     assert torch.equal(a.restore().cpu().double(), oracle.held(x)[0])
 
 
+@pytest.mark.parametrize("rows,d,factor", [(333, 128, 4), (70, 384, 4)])
+def test_transition_checkpoint_in_place(rows, d, factor):
+    """Written over its input (or into another tensor) it keeps the 8 bits of the input."""
+    x, dy, params = _transition_case(rows, d, factor, 3)
+    dev = {k: v.to(DEV) for k, v in params.items()}
+    y, a = kernels.transition_checkpoint(x.to(DEV), **dev)
+    other = torch.empty(rows, d, dtype=BF16, device=DEV)
+    for given, out in ((x.to(DEV), other), (x.to(DEV), None)):
+        out = given if out is None else out
+        got, kept = kernels.transition_checkpoint(given, out=out, **dev)
+        assert got is out and torch.equal(got, y)
+        assert torch.equal(kept.restore(), a.restore()) and torch.equal(kept.scales, a.scales)
+        for t, want in zip(kernels.transition_backward(dy.to(DEV), kept, **dev),
+                           kernels.transition_backward(dy.to(DEV), a, **dev)):
+            assert torch.equal(t, want)
+
+
 # ------------------------------------------------------------------------------------ streams and graphs
 def test_on_another_stream():
     x, dy, params = _transition_case(400, 128, 4, 6)

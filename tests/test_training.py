@@ -107,6 +107,17 @@ def test_transition_backward_refuses(cpu_checks):
         kernels.transition_backward(x, odd, **_params())
 
 
+def test_transition_checkpoint_keeps_the_input_of_an_in_place_call(monkeypatch):
+    """The transition may write over its input: the 8 bits are those of the input all the same."""
+    x = torch.arange(8.0)
+    monkeypatch.setattr(kernels, "transition", lambda x, *, out=None, **_: (out if out is not None else x.clone()).mul_(-1))
+    monkeypatch.setattr(kernels, "quantize_activation", lambda x: x.clone())
+    for out in (None, x):
+        y, kept = kernels.transition_checkpoint(x, **({} if out is None else {"out": out}))
+        assert torch.equal(kept, torch.arange(8.0)) and torch.equal(y, -torch.arange(8.0))
+        assert out is None or y is x
+
+
 def test_functions_refuse_a_bad_keep_and_a_capturing_stream(monkeypatch):
     x = torch.zeros(4, 64, dtype=BF16)
     with pytest.raises(ValueError, match="keep"):
