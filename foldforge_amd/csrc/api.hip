@@ -376,21 +376,28 @@ ApbWs apb_ws(void* ws, int64_t batch, int64_t n, int cs, int heads) {
   return w;
 }
 
-// Argument checks shared by the transition entry points (not the workspace).
 // Widths of the transition's backward pass.
 bool transition_grad_shape(int d, int factor) {
   return d > 0 && d % 64 == 0 && d <= kLnGemmMaxK && factor > 0 && factor <= 64;
 }
 
+// The kernels count a row's channels in 32 bits, and a workgroup's step past the last one.
+constexpr int kMostChannels = 0x7fffffff - 1023;
+// LayerNorm's backward pass sums 32 of the affine's 2 cols gradients in a workgroup of 1024, and a launch has less than
+// 2^32 threads.
+constexpr int kMostGradChannels = (1 << 26) - 16;
+
 int32_t activation_check(const char* what, const void* x, const void* codes, const void* scales, int64_t rows,
                          int cols, int dtype) {
-  if (rows < 0 || cols <= 0) return fail(FFK_ERR_INVALID, "%s: bad shape rows=%lld cols=%d", what, (long long)rows, cols);
+  if (rows < 0 || cols <= 0 || cols > kMostChannels)
+    return fail(FFK_ERR_INVALID, "%s: bad shape rows=%lld cols=%d", what, (long long)rows, cols);
   if (dtype != FFK_DTYPE_BF16 && dtype != FFK_DTYPE_F32)
     return fail(FFK_ERR_INVALID, "%s: dtype %d is neither bf16 nor fp32", what, dtype);
   if (rows > 0 && (!x || !codes || !scales)) return fail(FFK_ERR_INVALID, "%s: null tensor", what);
   return FFK_OK;
 }
 
+// Argument checks shared by the transition entry points (not the workspace).
 int32_t transition_check(const void* x, const float* ln_w, const float* ln_b, const float* wa,
                          const float* wb, const float* wsq, const void* out, int64_t rows, int d,
                          int factor) {
@@ -576,7 +583,7 @@ int32_t ffk_layer_norm_backward(const void* dy, const void* x, const void* scale
                                 void* dweight, void* dbias, void* workspace, size_t workspace_bytes, int64_t rows,
                                 int32_t cols, float eps, int32_t dtype, int32_t grad_dtype, void* stream) {
   if (int32_t s = check_device()) return s;
-  if (rows < 0 || cols <= 0)
+  if (rows < 0 || cols <= 0 || cols > kMostGradChannels)
     return fail(FFK_ERR_INVALID, "layer_norm_backward: bad shape rows=%lld cols=%d", (long long)rows, cols);
   if (rows > 0 && (!dy || !x || !dx)) return fail(FFK_ERR_INVALID, "layer_norm_backward: null tensor");
   if (dtype != FFK_DTYPE_BF16 && dtype != FFK_DTYPE_F32)

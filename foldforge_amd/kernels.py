@@ -223,6 +223,10 @@ def swiglu_ffn(x: Tensor, w_a: Tensor, w_b: Tensor, w_out: Tensor, residual: Ten
 
 #: channels of a row that share a scale in an :class:`Activation8`
 ACTIVATION_BLOCK = 32
+#: the widest row of the training calls (the kernels count channels in 32 bits, a workgroup's step past the last), and of
+#: LayerNorm's backward pass (its sums take 64 threads a channel, a launch has less than 2^32)
+MOST_CHANNELS = 2**31 - 1024
+MOST_GRAD_CHANNELS = 2**26 - 16
 
 
 @dataclass(eq=False, slots=True)
@@ -275,7 +279,13 @@ def _rows_tensor(x: Tensor, name: str) -> int:
         _refuse(f"{name} must be bf16 or fp32 (got {x.dtype})")
     if x.dim() == 0 or x.shape[-1] == 0:
         _refuse(f"{name} needs a last axis of channels (got {tuple(x.shape)})")
+    _check_channels(x.shape[-1], MOST_CHANNELS, name)
     return x.numel() // x.shape[-1]
+
+
+def _check_channels(cols: int, most: int, name: str) -> None:
+    if cols > most:
+        _refuse(f"{name} has {cols} channels (the kernels take up to {most})")
 
 
 #: kinds of :func:`_native.calls`'s ``empties``
@@ -290,6 +300,8 @@ def _activation_spec(x: Tensor) -> tuple:
 def _check_activation(a: Activation8, name: str) -> None:
     """An :class:`Activation8` as :func:`quantize_activation` makes it (the C-ABI receives no sizes)."""
     c, s = a.codes, a.scales
+    if c.dim():
+        _check_channels(c.shape[-1], MOST_CHANNELS, name)
     if c.is_cuda and a.dtype in (torch.bfloat16, torch.float32) and _native.calls().activation_ok(c, s):
         return
     if not (_on_device(c) and c.is_contiguous() and c.dtype == torch.float8_e4m3fn and c.dim() > 0 and c.shape[-1] > 0):
@@ -367,6 +379,7 @@ def layer_norm_backward(dy: Tensor, x: Tensor | Activation8, weight: Tensor | No
     ``dy.dtype``; the affine's gradients, sums over the rows in fp32 and a fixed order, in ``grad_dtype``
     (``dweight`` None without ``weight``, ``dbias`` None without ``with_bias``)."""
     rows, cols, dev = _rows_tensor(dy, "dy"), dy.shape[-1], dy.device
+    _check_channels(cols, MOST_GRAD_CHANNELS, "dy")
     kept, scales = _kept(x, dy)
     weight = _affine(weight, dy, "weight", cols)
     code = _grad_dtype(grad_dtype)

@@ -98,7 +98,7 @@ int32_t ffk_swiglu_ffn(const void* x, const float* w_a, const float* w_b, const 
  * the block and s the least whole number >= -126 with a <= 448 * 2^s:
  *   scales = s + 127,  codes = e4m3(x / 2^s) (OCP, nearest, ties to even),  restored = codes * 2^s
  * NaN and infinities become NaN. x [rows, cols] bf16 or fp32 (dtype), codes [rows, cols] bytes,
- * scales [rows, ceil(cols / 32)] bytes. Any width; rows of whole blocks on 16-byte aligned x and 8-byte
+ * scales [rows, ceil(cols / 32)] bytes. Any width up to 2^31 - 1024; rows of whole blocks on 16-byte aligned x and 8-byte
  * aligned codes take the wide path. No counterpart in the reference.
  */
 int32_t ffk_quantize_activation(const void* x, void* codes, void* scales, int64_t rows, int32_t cols,
@@ -119,7 +119,7 @@ int32_t ffk_layer_norm_checkpoint(const void* x, const float* weight, const floa
  * x: the input itself (scales NULL; dtype, as dy and dx) or the codes of its 8-bit activation with their
  * scales; statistics, sums and products in fp32, the statistics taken from the kept input again. weight
  * may be NULL (1); dweight / dbias [cols] in grad_dtype, either may be NULL. dx aliases nothing. The row
- * sums are added in a fixed order. Workspace: ffk_layer_norm_backward_workspace bytes.
+ * sums are added in a fixed order. cols up to 2^26 - 16. Workspace: ffk_layer_norm_backward_workspace bytes.
  * Reference: the gradient of torch.nn.LayerNorm that its training path takes (train/step.py:320-338).
  */
 size_t ffk_layer_norm_backward_workspace(int64_t rows, int32_t cols);

@@ -79,6 +79,23 @@ def test_layer_norm_backward_refuses(cpu_checks):
         kernels.layer_norm_backward(dy, dy, torch.ones(40), grad_dtype=torch.float16)
 
 
+@pytest.mark.parametrize("cols,narrower", [(2**31 - 1023, True), (2**31 - 1, True), (2**26 - 15, False), (2**30, False)])
+def test_more_channels_than_the_kernels_count(cpu_checks, monkeypatch, cols, narrower):
+    """A row's channels are counted in 32 bits, with a workgroup's step beyond them; the sums of the backward pass
+    take 64 threads a channel, and a launch has less than 2^32."""
+    monkeypatch.setattr(kernels, "DEVICE_TYPE", "meta")
+    x = torch.empty(1, cols, dtype=BF16, device="meta")
+    with pytest.raises(ValueError, match="channels"):
+        kernels.layer_norm_backward(x, x)
+    if narrower:
+        a = kernels.Activation8(x.to(torch.float8_e4m3fn), torch.empty(1, -(-cols // 32), dtype=torch.uint8, device="meta"),
+                                BF16)
+        for call in (lambda: kernels.quantize_activation(x), lambda: kernels.layer_norm_checkpoint(x, None, None),
+                     lambda: kernels.restore_activation(a)):
+            with pytest.raises(ValueError, match="channels"):
+                call()
+
+
 def _params(d=64, h=128, **change):
     return {**dict(ln_weight=torch.ones(d), ln_bias=torch.zeros(d), expand_a=torch.zeros(h, d),
                    expand_b=torch.zeros(h, d), squeeze=torch.zeros(d, h)), **change}
