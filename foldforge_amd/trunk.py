@@ -92,6 +92,8 @@ class PairformerTrunk(nn.Module):
         side = _side_stream(pair.device)
         # the single track starts from state the main stream produced
         side.wait_stream(main)
+        # (what the side stream's ops keep for a backward pass is read there as well)
+        single.record_stream(side)
         for _ in range(passes):
             for block in self.blocks:
                 pair_in = pair

@@ -10,12 +10,13 @@ them; two sides that differ by up to 5e-3 in one of eight ops' gradients stay wi
 from __future__ import annotations
 
 import copy
+import dataclasses
 
 import pytest
 import torch
 
 from foldforge_amd import dispatch, factories, kernels, modules, training
-from foldforge_amd.trunk import randomise
+from foldforge_amd.trunk import PairformerTrunk, randomise
 
 pytestmark = pytest.mark.gpu
 
@@ -154,3 +155,44 @@ def test_block_step(keep):
     assert all(p.isfinite().all() for p in block.parameters())
     with torch.no_grad():
         assert block(z, mask, s)[0].isfinite().all()
+
+
+@pytest.mark.parametrize("parallel", [False, True])
+@pytest.mark.parametrize("keep", ["input", "8bit"])
+def test_trunk_step(keep, parallel):
+    """Two blocks whose single tracks run on a second stream (the trunk's default): the gradients are those of the blocks
+    one after the other. The caller drops the inputs before the backward pass, and the memory that comes free in it is
+    written over on the first stream."""
+    g = torch.Generator().manual_seed(6)
+    n = 40
+    trunk = randomise(PairformerTrunk(2, d_single=128, n_head_single=4), 5, out_scale=0.3).to(DEV)
+    for block in trunk.blocks:
+        block.config = dataclasses.replace(block.config, parallel=parallel)
+    training.install(trunk, keep)
+    z, s = torch.randn(1, n, n, 128, generator=g).to(DEV, BF16), torch.randn(1, n, 128, generator=g).to(DEV, BF16)
+    mask = torch.ones(1, n, dtype=torch.bool, device=DEV)
+    mask[0, -3:] = False
+    weights = torch.randn(1, n, n, 128, generator=g).to(DEV), torch.randn(1, n, 128, generator=g).to(DEV)
+
+    def write_over(_):
+        torch.full((n, 128), float("nan"), device=DEV, dtype=BF16)
+
+    def step(overlap):
+        trunk.overlap_single = overlap
+        for p in trunk.parameters():
+            p.grad = None
+        pair, single = trunk(z.clone(), mask, s.clone())
+        loss = (pair.float() * weights[0]).mean() + (single.float() * weights[1]).mean()
+        del pair, single
+        hooks = [p.register_post_accumulate_grad_hook(write_over) for p in trunk.parameters()]
+        loss.backward()
+        for h in hooks:
+            h.remove()
+        return {k: p.grad for k, p in trunk.named_parameters()}
+
+    want = step(False)
+    for _ in range(3):
+        got = step(True)
+        for k, t in want.items():
+            if t is not None and float(t.norm()) > 0:
+                assert _rel(got[k], t) <= 2e-2, k

@@ -3,10 +3,12 @@ sizes the library asks for, and what ``install`` makes of a model. Nothing here 
 
 from __future__ import annotations
 
+import contextlib
+
 import pytest
 import torch
 
-from foldforge_amd import _native, build, factories, kernels, modules, training
+from foldforge_amd import _native, build, factories, kernels, modules, training, trunk
 from foldforge_amd.trunk import randomise
 
 BF16 = torch.bfloat16
@@ -212,3 +214,25 @@ def test_a_width_without_backward_kernels_is_refused_when_it_is_to_be_differenti
     assert "backward" in m.unsupported(x)
     with torch.no_grad():
         assert m.unsupported(x) is None
+
+
+def test_overlapped_trunk_records_what_its_second_stream_keeps(monkeypatch):
+    """A step keeps tensors of the main stream for the second one's backward pass: each is recorded there, so that its
+    memory is not handed out while that still reads it, whoever drops it first."""
+    class Stream:
+        wait_stream = wait_event = lambda self, other: None
+
+    class Event:
+        record = lambda self, stream: None  # noqa: E731
+
+    recorded, side = [], Stream()
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream())
+    monkeypatch.setattr(torch.cuda, "Event", Event)
+    monkeypatch.setattr(torch.cuda, "stream", lambda stream: contextlib.nullcontext())
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, stream: stream is side and recorded.append(t))
+    monkeypatch.setattr(trunk, "_side_stream", lambda device: side)
+    model = randomise(trunk.PairformerTrunk(1, d_pair=64, d_single=64, n_head_single=4), 0)
+    pair, single, mask = torch.randn(1, 3, 3, 64), torch.randn(1, 3, 64), torch.ones(1, 3, dtype=torch.bool)
+    out, _ = model._forward_overlapped(pair, mask, single, 1)
+    for t in (pair, out, single, mask):
+        assert any(r is t for r in recorded)
