@@ -1,8 +1,9 @@
 """Training with the hip kernels: LayerNorm and the SwiGLU transition under autograd.
 
 The hip kernels of the other ops are forward-only. :func:`install` makes a model of engine-op modules ready for a
-fine-tuning step: LayerNorm and Transition keep their inputs (as they are, or in 8 bits) and run their backward
-kernels, every other op takes its ``pytorch`` backend, whose equations autograd differentiates
+fine-tuning step: Transitions, and LayerNorms that are modules of their own, keep their inputs (as they are, or in 8
+bits) and run their backward kernels; every other op, the norms inside it included, takes its ``pytorch`` backend, whose
+equations autograd differentiates
 (the reference's fine-tuning runs its modules the same way, ``src/foldforge/train/step.py:320-338``).
 
 :func:`layer_norm` and :func:`transition` are the differentiable functions on their own, the autograd side of
@@ -17,6 +18,8 @@ calls the kernels' functions themselves (``transition_checkpoint``, ``transition
 """
 
 from __future__ import annotations
+
+from collections.abc import Iterator
 
 import torch
 from torch import nn
@@ -129,28 +132,43 @@ def wanted(module: nn.Module, *inputs: Tensor) -> bool:
             and (any(t.requires_grad for t in inputs) or any(p.requires_grad for p in module.parameters())))
 
 
-def install(model: nn.Module, keep: str | None = "8bit", *, requires_grad: bool = True) -> dict[str, list[str]]:
-    """Make ``model``'s engine ops trainable: every LayerNorm and Transition that lists ``hip`` keeps ``keep`` of its
-    input and runs forward and backward on the hip kernels, every other op goes to ``pytorch``. ``keep=None`` takes
-    the former back (backends stay). ``requires_grad``: switch the parameters' gradients on (models are placed
-    without). Returns the names of the modules by what they became: ``{"hip": [...], "pytorch": [...]}``."""
-    from foldforge_amd.modules import EngineOp, LayerNorm, Transition
+def _ops(model: nn.Module) -> Iterator[tuple[str, nn.Module]]:
+    """The engine ops of ``model``, without those inside another (an op reads its norms as parameters, it does not call
+    them)."""
+    from foldforge_amd.modules import EngineOp
 
+    inside: set[nn.Module] = set()
+    for name, module in model.named_modules():
+        if isinstance(module, EngineOp) and module not in inside:
+            inside.update(module.modules())
+            yield name, module
+
+
+def _has_backward(module: nn.Module) -> bool:
+    """Whether the kernels differentiate an op of its kind and width."""
+    from foldforge_amd.modules import LayerNorm, Transition
+
+    if isinstance(module, LayerNorm):
+        return len(module.normalized_shape) == 1
+    return isinstance(module, Transition) and kernels.transition_backward_supported(module.d, module.n)
+
+
+def install(model: nn.Module, keep: str | None = "8bit", *, requires_grad: bool = True) -> dict[str, list[str]]:
+    """Make ``model``'s engine ops trainable: every Transition, and every LayerNorm that is a module of its own (not a
+    part of another op), keeps ``keep`` of its input and runs forward and backward on the hip kernels; every other op,
+    and widths without backward kernels, go to ``pytorch``. ``keep=None`` takes the former back (backends stay).
+    ``requires_grad``: switch the parameters' gradients on (models are placed without). Returns the names of the ops by
+    what they became: ``{"hip": [...], "pytorch": [...]}``."""
     if keep is not None and keep not in KEEPS:
         raise ValueError(f"keep must be one of {KEEPS} or None (got {keep!r})")
     report: dict[str, list[str]] = {"hip": [], "pytorch": []}
-    for name, module in model.named_modules():
-        if not isinstance(module, EngineOp):
-            continue
-        if isinstance(module, (LayerNorm, Transition)):
+    for name, module in _ops(model):
+        served = _has_backward(module)
+        if served:
             module.keep = keep
-            if keep is not None:
-                module.set_backend("hip")
-            report[module.backend].append(name)
-        else:
-            if keep is not None:
-                module.set_backend("pytorch")
-            report[module.backend].append(name)
+        if keep is not None:
+            module.set_backend("hip" if served else "pytorch")
+        report[module.backend].append(name)
     if keep is not None and requires_grad:
         model.requires_grad_(True)
     return report

@@ -196,3 +196,24 @@ def test_trunk_step(keep, parallel):
         for k, t in want.items():
             if t is not None and float(t.norm()) > 0:
                 assert _rel(got[k], t) <= 2e-2, k
+
+
+@pytest.mark.parametrize("keep", ["input", "8bit"])
+def test_what_install_names_is_what_runs(keep):
+    """A step of a block and of a norm beside it: every module named under ``hip`` ran there once, forward and backward,
+    every other op on ``pytorch``."""
+    n = 12
+    block = factories.pairformer_block(d_pair=128, triangle_model="af3", d_single=384)
+    model = randomise(torch.nn.ModuleDict({"norm": factories.layer_norm(128), "block": block}), 7).to(DEV)
+    report = training.install(model, keep)
+    z = torch.randn(1, n, n, 128, device=DEV, dtype=BF16)
+    s = torch.randn(1, n, 384, device=DEV, dtype=BF16)
+    pair, single = model["block"](model["norm"](z), torch.ones(1, n, dtype=torch.bool, device=DEV), s)
+    (pair.float().square().mean() + single.float().square().mean()).backward()
+    assert report["hip"] == ["norm", "block.transition_pair", "block.single_transition"]
+    for backend, names in report.items():
+        for name in names:
+            module = model.get_submodule(name)
+            assert dispatch.ledger_of(module).served == {backend: 1}, name
+    for name in report["hip"]:
+        assert all(p.grad is not None for p in model.get_submodule(name).parameters()), name

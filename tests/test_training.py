@@ -204,6 +204,27 @@ def test_install_and_take_back():
     assert block.transition_pair.keep is None and not training.wanted(block.transition_pair, x)
 
 
+def test_install_names_the_modules_that_run_on_the_kernels():
+    """The norms inside an op are parameters of it: they are neither called nor named. Ops without backward kernels of
+    their kind or width take ``pytorch``."""
+    block = randomise(factories.pairformer_block(d_pair=64, triangle_model="af3", d_single=128), 0)
+    report = training.install(block, "8bit")
+    assert sorted(report["hip"]) == ["single_transition", "transition_pair"]
+    assert sorted(report["pytorch"]) == ["single_attention", "tri_atten_ending", "tri_atten_starting",
+                                         "tri_multi_incoming", "tri_multi_outgoing"]
+    assert all(m.keep is None and m.backend == "pytorch" for m in block.modules() if isinstance(m, modules.LayerNorm))
+    model = torch.nn.ModuleDict({
+        "norm": factories.layer_norm(100), "wide": modules.Transition(832, 1), "odd": modules.Transition(96, 2),
+        "grid": modules.LayerNorm((4, 8)), "inner": torch.nn.Sequential(modules.Transition(64, 4))})
+    report = training.install(model, "input")
+    assert sorted(report["hip"]) == ["inner.0", "norm"] and sorted(report["pytorch"]) == ["grid", "odd", "wide"]
+    for name, module in (("norm", model["norm"]), ("inner.0", model["inner"][0])):
+        assert (module.backend, module.keep) == ("hip", "input"), name
+    for name in ("grid", "odd", "wide"):
+        assert (model[name].backend, model[name].keep) == ("pytorch", None), name
+    assert training.install(factories.layer_norm(64))["hip"] == [""]
+
+
 def test_a_width_without_backward_kernels_is_refused_when_it_is_to_be_differentiated(monkeypatch):
     m = modules.Transition(832, 1)
     m.set_backend("hip")
