@@ -3,8 +3,8 @@
 The hip kernels of the other ops are forward-only. :func:`install` makes a model of engine-op modules ready for a
 fine-tuning step: Transitions, and LayerNorms that are modules of their own, keep their inputs (as they are, or in 8
 bits) and run their backward kernels; every other op, the norms inside it included, takes its ``pytorch`` backend, whose
-equations autograd differentiates
-(the reference's fine-tuning runs its modules the same way, ``src/foldforge/train/step.py:320-338``).
+equations autograd differentiates (the reference's fine-tuning runs its modules the same way,
+``src/foldforge/train/step.py:320-338``).
 
 :func:`layer_norm` and :func:`transition` are the differentiable functions on their own, the autograd side of
 :func:`foldforge_amd.kernels.layer_norm_backward` and :func:`foldforge_amd.kernels.transition_backward`. Nothing
@@ -153,12 +153,53 @@ def _has_backward(module: nn.Module) -> bool:
     return isinstance(module, Transition) and kernels.transition_backward_supported(module.d, module.n)
 
 
+#: a module's record of what :func:`install` changed
+_BEFORE = "_before_training"
+
+
+def _place(module: nn.Module, backend: str) -> None:
+    """Give an op its backend for training and keep the one it had (a caller's own choice since the last time counts
+    as such)."""
+    before, given = module.__dict__.get(_BEFORE, (None, None))
+    if module.backend != given:
+        before = module.backend
+    module.set_backend(backend)
+    module.__dict__[_BEFORE] = (before, backend)
+
+
+def _take_back(module: nn.Module) -> None:
+    before, given = module.__dict__.pop(_BEFORE, (None, None))
+    if before is not None and module.backend == given:
+        module.set_backend(before)
+
+
+#: a module's record of the parameters of its own whose gradients :func:`install` switched on
+_FROZEN = "_frozen_before_training"
+
+
+def _unfreeze(model: nn.Module) -> None:
+    for module in model.modules():
+        frozen = {n for n, p in module.named_parameters(recurse=False, remove_duplicate=False) if not p.requires_grad}
+        if frozen:
+            module.__dict__[_FROZEN] = module.__dict__.get(_FROZEN, set()) | frozen
+    model.requires_grad_(True)
+
+
+def _freeze_again(model: nn.Module) -> None:
+    for module in model.modules():
+        frozen = module.__dict__.pop(_FROZEN, ())
+        for name, p in module.named_parameters(recurse=False, remove_duplicate=False):
+            if name in frozen:
+                p.requires_grad_(False)
+
+
 def install(model: nn.Module, keep: str | None = "8bit", *, requires_grad: bool = True) -> dict[str, list[str]]:
     """Make ``model``'s engine ops trainable: every Transition, and every LayerNorm that is a module of its own (not a
     part of another op), keeps ``keep`` of its input and runs forward and backward on the hip kernels; every other op,
-    and widths without backward kernels, go to ``pytorch``. ``keep=None`` takes the former back (backends stay).
-    ``requires_grad``: switch the parameters' gradients on (models are placed without). Returns the names of the ops by
-    what they became: ``{"hip": [...], "pytorch": [...]}``."""
+    and widths without backward kernels, go to ``pytorch``. ``requires_grad``: switch the parameters' gradients on
+    (models are placed without). ``keep=None`` takes it all back: ops that still have the backend they were given here
+    get the one they had before, parameters whose gradients were switched on here lose them. Returns the names of the
+    ops by the backend they then have: ``{"hip": [...], "pytorch": [...]}``."""
     if keep is not None and keep not in KEEPS:
         raise ValueError(f"keep must be one of {KEEPS} or None (got {keep!r})")
     report: dict[str, list[str]] = {"hip": [], "pytorch": []}
@@ -166,9 +207,13 @@ def install(model: nn.Module, keep: str | None = "8bit", *, requires_grad: bool 
         served = _has_backward(module)
         if served:
             module.keep = keep
-        if keep is not None:
-            module.set_backend("hip" if served else "pytorch")
-        report[module.backend].append(name)
-    if keep is not None and requires_grad:
-        model.requires_grad_(True)
+        if keep is None:
+            _take_back(module)
+        else:
+            _place(module, "hip" if served else "pytorch")
+        report.setdefault(module.backend, []).append(name)
+    if keep is None:
+        _freeze_again(model)
+    elif requires_grad:
+        _unfreeze(model)
     return report

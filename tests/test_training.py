@@ -4,6 +4,7 @@ sizes the library asks for, and what ``install`` makes of a model. Nothing here 
 from __future__ import annotations
 
 import contextlib
+import copy
 
 import pytest
 import torch
@@ -223,6 +224,47 @@ def test_install_names_the_modules_that_run_on_the_kernels():
     for name in ("grid", "odd", "wide"):
         assert (model[name].backend, model[name].keep) == ("pytorch", None), name
     assert training.install(factories.layer_norm(64))["hip"] == [""]
+
+
+def test_taking_back_restores_backends_and_gradients():
+    block = randomise(factories.pairformer_block(d_pair=64, triangle_model="af3", d_single=128), 0)
+    block.set_backend("hip")
+    block.requires_grad_(False)
+    block.tri_multi_incoming.set_backend("pytorch")
+    block.single_attention.requires_grad_(True)
+    ops = {n: m for n, m in block.named_children()}
+    backends = {n: m.backend for n, m in ops.items()}
+    asked = {n: p.requires_grad for n, p in block.named_parameters()}
+    training.install(block, "8bit")
+    training.install(block, "input")  # (another kind: what there was before the first is still known)
+    block.single_transition.set_backend("pytorch")  # a later choice of the caller's stays
+    report = training.install(block, None)
+    backends["single_transition"] = "pytorch"
+    assert {n: m.backend for n, m in ops.items()} == backends
+    assert {n: p.requires_grad for n, p in block.named_parameters()} == asked
+    assert sorted(report["hip"] + report["pytorch"]) == sorted(ops) and set(report["hip"]) == {
+        n for n, b in backends.items() if b == "hip"}
+    block.requires_grad_(True)
+    block.set_backend("pytorch")
+    training.install(block, None)  # nothing to take back: nothing changes
+    assert all(p.requires_grad for p in block.parameters()) and all(m.backend == "pytorch" for m in ops.values())
+    training.install(block, "8bit", requires_grad=False)
+    training.install(block, None)
+    assert all(p.requires_grad for p in block.parameters())
+
+
+def test_taking_back_a_part_and_a_copy():
+    block = randomise(factories.pairformer_block(d_pair=64, triangle_model="af3", d_single=128), 0)
+    block.set_backend("hip")
+    block.requires_grad_(False)
+    training.install(block, "8bit")
+    other = copy.deepcopy(block)
+    training.install(block.single_attention, None)
+    assert block.single_attention.backend == "hip" and not any(p.requires_grad for p in block.single_attention.parameters())
+    assert block.tri_multi_outgoing.backend == "pytorch" and all(p.requires_grad for p in block.transition_pair.parameters())
+    for model in (block, other):
+        training.install(model, None)
+        assert all(m.backend == "hip" for m in model.children()) and not any(p.requires_grad for p in model.parameters())
 
 
 def test_a_width_without_backward_kernels_is_refused_when_it_is_to_be_differentiated(monkeypatch):
