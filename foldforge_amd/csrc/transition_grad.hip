@@ -11,11 +11,11 @@
 //   dA = (da^T xh) diag(w) + (sum da) v^T,   dw = sum over h of A (da^T xh) + B (db^T xh),
 //   dv = A^T (sum da) + B^T (sum db)
 // so dw and dv come out of the weights' gradients, and the products see xh alone, whose values are at most
-// sqrt(d): a and b are products of fp16 operands (Aw and Bw times a power of two that puts their largest
-// entry, of a hidden channel's row or of 32 of them, at 2^14 .. 2^15, so that entries down to 2^-29 of it keep
-// fp16's 11 bits), which leaves their errors at an eighth of bf16's. The gradients' operands are bf16, whose
-// range they need: three bf16 roundings lie between dy and a gradient, and one of the result (relative error
-// 3.3e-3 rather than the 4.6e-3 of bf16 throughout).
+// sqrt(d): a and b are products of fp16 operands (Aw and Bw times a power of two that puts the largest of their
+// entries and offsets A v, B v, of a hidden channel or (fused kernels) of 32 of them, at 2^14 .. 2^15: entries down to
+// 2^-28 of that peak keep fp16's 11 bits, smaller ones lose them, and below 2^-40 of it are 0), which leaves their errors
+// at an eighth of bf16's. The gradients' operands are bf16, whose range they need: three bf16 roundings lie between dy
+// and a gradient, and one of the result (relative error 3.3e-3 rather than the 4.6e-3 of bf16 throughout).
 // The powers of two 2^ka, 2^kb ride along: a' = 2^ka a, b' = 2^kb b, so silu' = 2^ka silu, da' = 2^kb da,
 // db' = 2^ka db, u' = 2^(ka+kb) u; the transposed weights carry their inverses, the join takes the rest out.
 #include <algorithm>
