@@ -433,6 +433,49 @@ def test_transition_backward_scales_of_the_affine(rows):
     assert all(torch.isfinite(t.float()).all() for t in got) and not got.squeeze.any()
 
 
+@pytest.mark.parametrize("rows,d,factor", [(130, 128, 4), (4100, 64, 4), (24600, 128, 2), (4500, 256, 1)])
+def test_transition_backward_hidden_channels_of_unlike_size(rows, d, factor):
+    """Hidden channels up to 2^20 apart, neighbours among them: the fused kernels scale 32 of them by one power of two
+    for fp16, whose range leaves the small ones their bits (their entries' last bit is 2^-25, 2^-17 of the entries of
+    the smallest channel, far below r / 8). Every channel's gradients are held to its own deviations."""
+    x, dy, params = _transition_case(rows, d, factor, 13)
+    g = torch.Generator().manual_seed(14)
+    for name in ("expand_a", "expand_b"):
+        params[name] *= torch.exp2(-torch.randint(0, 21, (factor * d, 1), generator=g).float())
+    _check_transition(x, dy, params, x.to(DEV), residual=False)
+
+
+@pytest.mark.parametrize("keep", ["input", "8bit"])
+@pytest.mark.parametrize("rows,d,factor", [
+    (33, 128, 4), (100, 384, 4),  # few rows
+    (2001, 128, 4), (6001, 192, 3),  # 64 x 64 tiles
+    (4101, 256, 2), (5001, 384, 2),  # streamed hidden gradients, 128 x 128 tiles
+    (4129, 64, 4), (24641, 128, 1)])  # the fused kernels
+def test_transition_backward_keeps_non_finite_rows_apart(rows, d, factor, keep):
+    """Rows share tiles, and the last one stands in for those behind the end: one that is not finite leaves the others'
+    dx as they are, bit for bit, and reaches every gradient of the parameters."""
+    x, dy, params = _transition_case(rows, d, factor, 15)
+    dev = {k: v.to(DEV) for k, v in params.items()}
+
+    def run(x, dy):
+        kept = x.to(DEV) if keep == "input" else kernels.quantize_activation(x.to(DEV))
+        return kernels.transition_backward(dy.to(DEV), kept, **dev)
+
+    clean = run(x, dy).x
+    bad_x, bad_dy = x.clone(), dy.clone()
+    bad_x[7, 5] = bad_x[-1, 0] = float("nan")
+    bad_dy[21, 3] = float("inf")
+    for got, bad in ((run(bad_x, dy), [7, rows - 1]), (run(x, bad_dy), [21])):
+        kept = torch.ones(rows, dtype=torch.bool, device=DEV)
+        kept[bad] = False
+        assert torch.equal(got.x[kept], clean[kept]) and not got.x[~kept].isfinite().any()
+        for name, t in list(got._asdict().items())[1:]:
+            if name == "squeeze" and bad == [21]:  # dS = dy^T u: the one channel's
+                assert t[torch.arange(d, device=DEV) != 3].isfinite().all()
+                t = t[3]
+            assert not t.isfinite().any(), name
+
+
 def test_transition_checkpoint_is_the_forward():
     x, _, params = _transition_case(333, 128, 4, 2)
     dev = {k: v.to(DEV) for k, v in params.items()}
