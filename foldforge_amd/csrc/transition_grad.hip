@@ -950,10 +950,11 @@ __global__ __launch_bounds__(512, 2) void transition_grad_weights(
 }
 
 // E as hidden_grad makes it, for 256 channels and many rows (40000 rows x 512: 58 us, 0.54 PFLOP/s, 123 MB of E at 2.1 TB/s:
-// the matrix cores are busy 27% of the cycles, the elementwise part and the stores take turns with them; 20000 rows:
-// hidden_grad 74, here 49): as above a wave keeps its operands of Aw, Bw and S^T of 16 hidden channels in
-// registers (12 D / 32 of them) and the rows stream by through LDS, D = hidden x rows (a lane holds a row at 4 hidden
-// channels). grid (ceil(H / 128), splits); block 512.
+// the matrix cores are busy 27% of the cycles, the elementwise part and the stores take turns with them, and the wait for a
+// block's rows, which counts the stores, leaves half a block of rows on its way; 20000 rows: hidden_grad 74, here 49): as
+// above a wave keeps its operands of Aw, Bw and S^T of 16 hidden channels in registers (12 D / 32 of them) and the rows
+// stream by through LDS, D = hidden x rows (a lane holds a row at 4 hidden channels). grid (ceil(H / 128), splits); block
+// 512.
 template <int D>
 __global__ __launch_bounds__(512, 2) void hidden_stream(const f16* __restrict__ xh, const bf16* __restrict__ dy,
                                                         const f16* __restrict__ aw, const bf16* __restrict__ st,
@@ -1009,7 +1010,9 @@ __global__ __launch_bounds__(512, 2) void hidden_stream(const f16* __restrict__ 
   int b = 0;
 #pragma unroll 1
   for (int64_t block = at_.split; block < blocks; block += at_.splits) {
-    // (this block has landed: NB - 2 later ones of 2 U transfers, and the stores behind them, stay on their way)
+    // This block has landed. The count takes the stores in too: from the second block on, what stays on its way in a wave
+    // that owns channels is the last block's 6 stores and 2 of the transfers issued in it (a wave that owns none, and the
+    // first block, leave two blocks of 2 U transfers).
     wait_vm_lds<(NB - 2) * 2 * U>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
