@@ -4,7 +4,8 @@
 // largest finite |x| of the block and s the least whole number >= -126 with a <= 448 2^s, value x is
 // kept as the e4m3 code of x / 2^s (nearest, halves to even; 448 is e4m3's largest number, so no code
 // overflows) and read back as code * 2^s. The scale is the byte s + 127, the exponent field of 2^s as
-// fp32, so both directions multiply by an exact power of two. NaN and infinities become NaN.
+// fp32, so both directions multiply by an exact power of two. NaN and infinities become NaN. Finite values
+// from 1.9375 * 2^127 on, at the end of the types' range, are nearest to 256 * 2^120 and read back as infinities.
 #pragma once
 
 #include "ffk_device.h"

@@ -235,8 +235,9 @@ class Activation8:
     ``ffk_quantize_activation``): e4m3 ``codes`` of the tensor's shape and, for each block of 32
     channels of a row, the byte ``s + 127`` of the power of two that its codes are multiples of,
     ``scales [..., ceil(c / 32)]``. ``dtype``: the tensor's. 33 / 32 bytes a value; a value is off
-    by at most 2^-4 of itself, or half a step of 2^(s-9) where it is below 2^(s-6); NaN and
-    infinities become NaN."""
+    by at most 2^-4 of itself, or half a step of 2^(s-9) where it is below 2^(s-6); values
+    from 1.9375 * 2^127 on, at the end of the types' range, round to 2^128 and come back infinite; NaN and infinities
+    become NaN."""
 
     codes: Tensor
     scales: Tensor

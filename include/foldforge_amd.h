@@ -97,8 +97,9 @@ int32_t ffk_swiglu_ffn(const void* x, const float* w_a, const float* w_b, const 
  * 32 consecutive channels of a row (the last of a row may be shorter), with a the largest finite |x| of
  * the block and s the least whole number >= -126 with a <= 448 * 2^s:
  *   scales = s + 127,  codes = e4m3(x / 2^s) (OCP, nearest, ties to even),  restored = codes * 2^s
- * NaN and infinities become NaN. x [rows, cols] bf16 or fp32 (dtype), codes [rows, cols] bytes,
- * scales [rows, ceil(cols / 32)] bytes. Any width up to 2^31 - 1024; rows of whole blocks on 16-byte aligned x and 8-byte
+ * NaN and infinities become NaN; finite values from 1.9375 * 2^127 on are restored as infinities (2^128).
+ * x [rows, cols] bf16 or fp32 (dtype), codes [rows, cols] bytes, scales [rows, ceil(cols / 32)] bytes. Any
+ * width up to 2^31 - 1024; rows of whole blocks on 16-byte aligned x and 8-byte
  * aligned codes take the wide path. No counterpart in the reference.
  */
 int32_t ffk_quantize_activation(const void* x, void* codes, void* scales, int64_t rows, int32_t cols,

@@ -27,6 +27,16 @@ def test_held_values_are_within_half_a_step(cols):
     assert (top <= 448 * torch.exp2(exps)).all() and (top > 224 * torch.exp2(exps)).all()
 
 
+def test_held_values_at_the_end_of_the_range():
+    """From 1.9375 * 2^127 on (half way from e4m3's 240 to 256, times 2^120) a value is nearest to 2^128, which neither
+    type has; below it the bound holds."""
+    last = torch.finfo(torch.float32).max
+    x = torch.tensor([[1.9375 * 2.0**127, last, torch.finfo(torch.bfloat16).max, (1.9375 - 2.0**-23) * 2.0**127]])
+    values, _ = oracle.held(x)
+    assert values.tolist() == [[2.0**128, 2.0**128, 2.0**128, 240 * 2.0**120]]
+    assert values.float().isinf().tolist() == [[True, True, True, False]]
+
+
 def _case(rows=7, d=10, h=14):
     g = torch.Generator().manual_seed(1)
     n = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)  # noqa: E731
