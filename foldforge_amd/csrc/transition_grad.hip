@@ -1470,10 +1470,12 @@ void launch_fused(const TransitionGradArgs& a, const TransitionGradPlan& p, cons
 TransitionGradPlan transition_grad_plan(int64_t rows, int d, int H) {
   TransitionGradPlan p{};
   const int64_t cus = cu_count();
-  // Rows from which the fused kernels win (a workgroup walks all chunks of weights however few its rows). Separate kernels
-  // against fused ones, us: 128 x 512 channels, 8192 rows 55 / 75, 16384 rows 79 / 81, 24576 rows 101 / 89; 128 x 256, 16384
-  // rows 57 / 62, 24576 rows 74 / 67; 64 x 256, 4096 rows 33 / 34, 8192 rows 40 / 37; 64 x 128, 4096 rows 32 / 28.
-  p.fused = fused_shape(d, H) && rows >= (d == 64 ? 4096 : 16384);
+  // Rows from which the fused kernels win (a workgroup walks all chunks of weights however few its rows; the separate ones
+  // step up where their 64-row tiles come to one a CU). Separate kernels against fused ones, us, on both sides of the rule:
+  // 128 x 128 channels 16384 rows 47 / 48, 16448 rows 53 / 49; 128 x 512 81 / 84 and 91 / 83; 128 x 1024 116 / 123 and (18432
+  // rows) 131 / 126; 64 x 256 4096 rows 32.6 / 33.0, 4160 rows 34.2 / 32.9; 64 x 512 6144 rows 46.4 / 46.0, 8192 rows 50.4 /
+  // 46.5, 4096 rows 39 / 45; 64 x 1024 8192 rows 62 / 65, 12288 rows 77 / 68; 64 x 64, 4096 rows 27 / 24, 2048 rows 25 / 23.
+  p.fused = fused_shape(d, H) && (d == 128 ? rows > 16384 : rows >= (H <= 256 ? 4096 : 8192));
   if (p.fused) {
     p.chunk = std::min<int64_t>(ceil_div(rows, 64) * 64, 1 << 18);
     const int64_t groups = ceil_div(H, 128);
@@ -1490,8 +1492,13 @@ TransitionGradPlan transition_grad_plan(int64_t rows, int d, int H) {
   p.dxh_wide = d % 128 == 0 && ceil_div(p.chunk, 128) * (d / 128) >= cus;
   const int64_t dxh_tiles = p.dxh_wide ? ceil_div(p.chunk, 128) * (d / 128) : p.chunk / 64 * (d / 64);
   p.dxh_splits = (int)std::max<int64_t>(1, std::min<int64_t>(cus / std::max<int64_t>(1, dxh_tiles), 2 * H / 256));
+  // (64 x 64 against 128 x 128 tiles, us a call: 256 x 1024 channels 4096 rows 71 / 72, 8192 rows 104 / 97; 768 x 1536 180 / 178
+  // and 319 / 292; 256 x 256, 3072 rows 42 / 45, 4096 rows 48 / 46. Where the small tiles need no join they hold out a
+  // little longer: 384 x 1536 4096 rows 106 / 111, 8192 rows 180 / 177; 512 x 1024 91 / 100 and 176 / 157)
   p.dw_wide = d % 128 == 0 && H % 128 == 0 && p.chunk >= 4096;
-  p.stream = d == 256 && p.chunk >= 4096;
+  // (hidden_grad against hidden_stream, us a call, below the rule and above: 256 x 256 channels 16384 rows 77.0 / 77.7, 20000
+  // rows 90 / 86; 256 x 512 8192 rows 71 / 72, 10240 rows 84.5 / 82.9; 256 x 1024 4096 rows 70 / 72, 6144 rows 86.3 / 85.9)
+  p.stream = d == 256 && p.chunk >= 4096 && p.chunk * H >= 5000000;
   const int64_t dw_tiles = p.dw_wide ? 3 * H / 128 * (d / 128) : 3 * H / 64 * (d / 64);
   p.dw_splits = (int)std::max<int64_t>(1, std::min<int64_t>(2 * cus / std::max<int64_t>(1, dw_tiles), p.chunk / 256));
   // both products and the gradients' ends in two launches instead of five (100 rows x 384 x 4: 47 -> 34 us)

@@ -349,6 +349,16 @@ def test_transition_backward_many_rows(rows, d, factor):
     _check_transition(x, dy, params, kernels.quantize_activation(x.to(DEV)), residual=False)
 
 
+@pytest.mark.parametrize("rows,d,factor", [
+    # both sides of the rule for the fused kernels
+    (16384, 128, 1), (16448, 128, 2), (8191, 64, 8), (8192, 64, 5), (8193, 64, 32), (4096, 64, 2),
+    # and of the one for rows that stream by
+    (9728, 256, 2), (9729, 256, 2), (4100, 256, 8), (19600, 256, 1)])
+def test_transition_backward_at_the_rules(rows, d, factor):
+    x, dy, params = _transition_case(rows, d, factor, rows + factor)
+    _check_transition(x, dy, params, x.to(DEV), residual=True)
+
+
 def test_transition_backward_past_32_bits():
     """More than 2^31 values: the last rows' gradients are those of the rows alone."""
     rows, d = (1 << 24) + 77, 128
@@ -449,7 +459,7 @@ def test_transition_backward_hidden_channels_of_unlike_size(rows, d, factor):
 @pytest.mark.parametrize("rows,d,factor", [
     (33, 128, 4), (100, 384, 4),  # few rows
     (2001, 128, 4), (6001, 192, 3),  # 64 x 64 tiles
-    (4101, 256, 2), (5001, 384, 2),  # streamed hidden gradients, 128 x 128 tiles
+    (9801, 256, 2), (5001, 384, 2),  # streamed hidden gradients, 128 x 128 tiles
     (4129, 64, 4), (24641, 128, 1)])  # the fused kernels
 def test_transition_backward_keeps_non_finite_rows_apart(rows, d, factor, keep):
     """Rows share tiles, and the last one stands in for those behind the end: one that is not finite leaves the others'
@@ -535,6 +545,10 @@ def test_every_form_captured(rows, d, factor):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), turn
+
+
+def test_streamed_form_captured():
+    test_every_form_captured(9800, 256, 2)
 
 
 def test_two_graphs_replayed():
