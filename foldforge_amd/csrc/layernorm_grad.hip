@@ -380,7 +380,7 @@ __global__ __launch_bounds__(256) void layer_norm_keep(const T* __restrict__ x, 
 }
 
 // How a call's rows are laid over lanes: 16-byte pieces where the width splits evenly and every tensor is
-// aligned, else single values; beyond 1024 channels no row fits a wave's registers.
+// aligned, else single values of up to 1024 channels; other rows lie in no wave's registers.
 enum RowForm { kFormWide, kForm8x1, kForm16x1, kForm32x1, kForm16x3, kForm64x1, kForm32x3, kForm64x3,
                kFormOne1, kFormOne2, kFormOne4, kFormOne8, kFormOne16 };
 

@@ -342,7 +342,7 @@ def _affine(t: Tensor | None, like: Tensor, name: str, cols: int) -> Tensor | No
 def layer_norm_checkpoint(x: Tensor, weight: Tensor | None, bias: Tensor | None,
                           eps: float = 1e-5) -> tuple[Tensor, Activation8]:
     """:func:`layer_norm` of ``x`` and the 8-bit activation of ``x`` that its backward pass takes, in one pass
-    (rows of at most 1024 channels; two for wider ones)."""
+    (rows of at most 1024 channels, and bf16 rows of 1536; two for others)."""
     rows, cols = _rows_tensor(x, "x"), x.shape[-1]
     weight, bias = _affine(weight, x, "weight", cols), _affine(bias, x, "bias", cols)
     y, codes, scales = _native.calls().empties(x, ((tuple(x.shape), _dtype_code(x.dtype)), *_activation_spec(x)))

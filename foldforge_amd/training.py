@@ -10,7 +10,8 @@ equations autograd differentiates (the reference's fine-tuning runs its modules 
 :func:`foldforge_amd.kernels.layer_norm_backward` and :func:`foldforge_amd.kernels.transition_backward`. Nothing
 but the input is kept between the passes (the backward kernels take the statistics and the hidden rows from it
 again); with ``keep="8bit"`` the gradient is taken at the values that the 8 bits stand for. The gradients of fp32
-parameters are fp32. They differentiate once.
+parameters are fp32; the transition's come from products on bf16 and fp16 operands, as its forward pass, and are off by some
+3e-3 of their norm (``pytorch``: fp32 throughout). They differentiate once.
 
 Autograd does not reach into graph capture here: a backward pass whose leaves were used by an eager graph on
 another stream ends the process when it is captured, so these functions refuse a capturing stream. A captured step
