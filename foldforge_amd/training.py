@@ -146,9 +146,11 @@ def _ops(model: nn.Module) -> Iterator[tuple[str, nn.Module]]:
 
 
 def _has_backward(module: nn.Module) -> bool:
-    """Whether the kernels differentiate an op of its kind and width."""
+    """Whether the kernels differentiate an op of its kind and width (and it lists them)."""
     from foldforge_amd.modules import LayerNorm, Transition
 
+    if "hip" not in module.backends:
+        return False
     if isinstance(module, LayerNorm):
         return len(module.normalized_shape) == 1
     return isinstance(module, Transition) and kernels.transition_backward_supported(module.d, module.n)

@@ -226,6 +226,15 @@ def test_install_names_the_modules_that_run_on_the_kernels():
     assert training.install(factories.layer_norm(64))["hip"] == [""]
 
 
+def test_install_leaves_an_op_that_lists_no_hip_on_pytorch():
+    class Plain(modules.Transition):
+        backends = ("pytorch",)
+
+    model = torch.nn.Sequential(Plain(64, 4), modules.Transition(64, 4))
+    assert training.install(model, "8bit") == {"hip": ["1"], "pytorch": ["0"]}
+    assert model[0].keep is None
+
+
 def test_taking_back_restores_backends_and_gradients():
     block = randomise(factories.pairformer_block(d_pair=64, triangle_model="af3", d_single=128), 0)
     block.set_backend("hip")
