@@ -1493,8 +1493,8 @@ TransitionGradPlan transition_grad_plan(int64_t rows, int d, int H) {
   const int64_t dxh_tiles = p.dxh_wide ? ceil_div(p.chunk, 128) * (d / 128) : p.chunk / 64 * (d / 64);
   p.dxh_splits = (int)std::max<int64_t>(1, std::min<int64_t>(cus / std::max<int64_t>(1, dxh_tiles), 2 * H / 256));
   // (64 x 64 against 128 x 128 tiles, us a call: 256 x 1024 channels 4096 rows 71 / 72, 8192 rows 104 / 97; 768 x 1536 180 / 178
-  // and 319 / 292; 256 x 256, 3072 rows 42 / 45, 4096 rows 48 / 46. Where the small tiles need no join they hold out a
-  // little longer: 384 x 1536 4096 rows 106 / 111, 8192 rows 180 / 177; 512 x 1024 91 / 100 and 176 / 157)
+  // and 319 / 292; 256 x 512, 2048 rows 42.5 / 44.6, 4096 rows 53.9 / 53.6. Where the small tiles need no join they hold out
+  // to some 7000 rows: 384 x 1536 4096 rows 106 / 111, 8192 rows 180 / 177; 512 x 1024 91 / 100 and 176 / 157)
   p.dw_wide = d % 128 == 0 && H % 128 == 0 && p.chunk >= 4096;
   // (hidden_grad against hidden_stream, us a call, below the rule and above: 256 x 256 channels 16384 rows 77.0 / 77.7, 20000
   // rows 90 / 86; 256 x 512 8192 rows 71 / 72, 10240 rows 84.5 / 82.9; 256 x 1024 4096 rows 70 / 72, 6144 rows 86.3 / 85.9)
