@@ -82,6 +82,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int32,
         [c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_void_p],
     ),
+    "ffk_dropout_add": (
+        c_int32,
+        [c_void_p] * 4 + [c_int64] * 5 + [c_int32, c_int32, c_void_p],
+    ),
     "ffk_layer_norm_checkpoint": (
         c_int32,
         [c_void_p] * 6 + [c_int64, c_int32, c_float, c_int32, c_void_p],

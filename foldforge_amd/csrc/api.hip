@@ -105,6 +105,9 @@ int resident_blocks(const void* kernel, int threads, size_t dynamic_lds) noexcep
 
 namespace {
 
+// (a byte count of it stays within 63 bits)
+constexpr int64_t kMostValues = int64_t(1) << 60;
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
@@ -572,6 +575,35 @@ int32_t ffk_layer_norm_checkpoint(const void* x, const float* weight, const floa
   launch_layer_norm_keep(x, weight, bias, y, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), rows, cols,
                          eps, dtype, static_cast<hipStream_t>(stream));
   return check_launch("layer_norm_checkpoint");
+}
+
+int32_t ffk_dropout_add(const void* x, const void* residual, void* out, const int64_t* state, int64_t seed,
+                        int64_t offset, int64_t outer, int64_t shared, int64_t inner, int32_t dropped, int32_t dtype,
+                        void* stream) {
+  if (int32_t s = check_device()) return s;
+  if (outer < 0 || shared < 0 || inner < 0 || dropped < 0 || dropped > 65536 || seed < 0 || offset < 0)
+    return fail(FFK_ERR_INVALID, "dropout_add: outer=%lld shared=%lld inner=%lld dropped=%d (of 65536); seed and offset are not negative", (long long)outer, (long long)shared, (long long)inner, dropped);
+  if (dtype != FFK_DTYPE_BF16 && dtype != FFK_DTYPE_F32)
+    return fail(FFK_ERR_INVALID, "dropout_add: dtype=%d (bf16 or fp32)", dtype);
+  if (outer == 0 || shared == 0 || inner == 0) return ok();
+  if (!x || !out) return fail(FFK_ERR_INVALID, "dropout_add: null argument");
+  if (outer > kMostValues / shared || outer * shared > kMostValues / inner)
+    return fail(FFK_ERR_INVALID, "dropout_add: more values than memory holds");
+  DropoutArgs a{};
+  a.x = x;
+  a.residual = residual;
+  a.y = out;
+  a.state = state;
+  a.seed = (uint64_t)seed;
+  a.offset = (uint64_t)offset;
+  a.outer = shared == 1 ? 1 : outer;
+  a.shared = shared;
+  a.inner = shared == 1 ? outer * inner : inner;
+  a.threshold = dropped;
+  a.scale = dropped < 65536 ? 65536.f / (float)(65536 - dropped) : 0.f;
+  a.dtype = dtype;
+  launch_dropout(a, static_cast<hipStream_t>(stream));
+  return check_launch("dropout_add");
 }
 
 size_t ffk_layer_norm_backward_workspace(int64_t rows, int32_t cols) {

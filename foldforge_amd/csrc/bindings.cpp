@@ -176,6 +176,7 @@ PyMethodDef methods[] = {
     FFK_CALL(ffk_outer_product_mean_grouped),
     FFK_CALL(ffk_quantize_activation),
     FFK_CALL(ffk_restore_activation),
+    FFK_CALL(ffk_dropout_add),
     FFK_CALL(ffk_layer_norm_checkpoint),
     FFK_CALL(ffk_layer_norm_backward_workspace),
     FFK_CALL(ffk_layer_norm_backward),

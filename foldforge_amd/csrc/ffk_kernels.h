@@ -412,6 +412,19 @@ void launch_layer_norm_grad(const LayerNormGradArgs& a, hipStream_t stream);
 void launch_sum_partials(const float* part, int count, int width, int split, void* out0, void* out1, int dtype,
                          hipStream_t stream);
 
+// Dropout of x [outer][shared][inner] under a mask [outer][inner] (dropout.hip); shared = 1: outer = 1.
+struct DropoutArgs {
+  const void *x, *residual;  // residual may be null (0)
+  void* y;
+  const int64_t* state;      // null, or {seed, what is added to the offset} on the device
+  uint64_t seed, offset;
+  int64_t outer, shared, inner;
+  int threshold;             // dropped of 65536
+  float scale;
+  int dtype;
+};
+void launch_dropout(const DropoutArgs& a, hipStream_t stream);
+
 // Backward pass of the SwiGLU transition (rows > 0; d a multiple of 64 up to 768, hidden of 64).
 struct TransitionGradPlan {
   int64_t chunk;  // rows at once, a multiple of 64

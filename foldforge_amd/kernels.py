@@ -14,6 +14,7 @@ module classes decide what to refuse (``unsupported``) before a call ever gets h
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from typing import NamedTuple
 
@@ -393,6 +394,72 @@ def layer_norm_backward(dy: Tensor, x: Tensor | Activation8, weight: Tensor | No
     _call(dev, "layer_norm_backward", dy, kept, scales, weight, dx, dweight, dbias, ws, ws.numel(), rows, cols,
           float(eps), _dtype_code(dy.dtype), code)
     return dx, dweight, dbias
+
+
+#: what a dropout's random numbers are out of (16 bits each)
+DROPOUT_LEVELS = 65536
+
+
+def _drawn(seed: int | Tensor, offset: int, device: torch.device) -> tuple[Tensor | None, int, int]:
+    """The C-ABI's (state, seed, offset)."""
+    if not 0 <= offset < 2**63:
+        _refuse(f"offset must be in [0, 2^63) (got {offset})")
+    if not isinstance(seed, Tensor):
+        if not 0 <= seed < 2**63:
+            _refuse(f"seed must be in [0, 2^63) (got {seed})")
+        return None, seed, offset
+    if not (seed.device == device and seed.dtype == torch.int64 and seed.shape == (2,) and seed.is_contiguous()):
+        _refuse(f"a seed on the device is a contiguous int64 (seed, offset) on {device} (got {tuple(seed.shape)} "
+                f"{seed.dtype} on {seed.device})")
+    return seed, 0, offset
+
+
+def dropped_of_levels(p: float) -> int:
+    """How many of the ``DROPOUT_LEVELS`` numbers a rate drops: the rate drawn is the nearest multiple of 2^-16."""
+    if not 0.0 <= p <= 1.0:
+        _refuse(f"p must be in [0, 1] (got {p})")
+    return round(DROPOUT_LEVELS * p)
+
+
+def mask_axes(shape: tuple[int, ...], shared: int | None) -> tuple[int, int, int]:
+    """``(outer, shared, inner)`` of a tensor whose mask has size 1 along the axis ``shared`` (None: the whole mask)."""
+    if shared is None:
+        return 1, 1, math.prod(shape)
+    if not -len(shape) <= shared < len(shape):
+        _refuse(f"shared={shared} is no axis of {tuple(shape)}")
+    at = shared % len(shape)
+    return math.prod(shape[:at]), shape[at], math.prod(shape[at + 1:])
+
+
+def dropout_add(update: Tensor, residual: Tensor | None = None, *, p: float, seed: int | Tensor, offset: int = 0,
+                shared: int | None = None, out: Tensor | None = None) -> Tensor:
+    """``residual + dropout(update)`` (without ``residual``: the dropout alone) of bf16 or fp32 tensors, ``out`` may be
+    either. ``shared``: the axis along which the mask is one (AF3's row-wise dropout of a pair tensor: 1, column-wise: 2;
+    None: every value its own). The mask is a function of the mask's shape, ``p`` (to the nearest 2^-16), ``seed`` and
+    ``offset``, drawn in the call and kept nowhere (``include/foldforge_amd.h``, ``ffk_dropout_add``, states it):
+    :func:`dropout_backward` with the same ones draws it again. Calls of one seed are told apart by their offsets.
+    ``seed`` on the device, int64 ``(seed, offset)`` read when the kernel runs, is for captured calls: a graph that counts
+    its offset up draws anew at each replay. A dropped value does not reach the result, whatever it is."""
+    _rows_tensor(update, "update")
+    if residual is not None and not (isinstance(residual, Tensor) and residual.shape == update.shape
+                                     and residual.dtype == update.dtype and residual.device == update.device
+                                     and residual.is_contiguous()):
+        _refuse(f"residual must be a contiguous {update.dtype} tensor {tuple(update.shape)} on {update.device}")
+    dropped = dropped_of_levels(p)
+    state, seed, offset = _drawn(seed, offset, update.device)
+    axes = mask_axes(update.shape, shared)
+    out = _output(out, tuple(update.shape), update.dtype, update.device)
+    if update.numel():
+        _call(update.device, "dropout_add", update, residual, out, state, seed, offset, *axes, dropped,
+              _dtype_code(update.dtype))
+    return out
+
+
+def dropout_backward(dy: Tensor, *, p: float, seed: int | Tensor, offset: int = 0, shared: int | None = None,
+                     out: Tensor | None = None) -> Tensor:
+    """The gradient of :func:`dropout_add`'s ``update`` from the output's (the residual's is ``dy`` itself): the same mask,
+    drawn again. ``out`` may be ``dy``."""
+    return dropout_add(dy, p=p, seed=seed, offset=offset, shared=shared, out=out)
 
 
 def triangle_multiplicative_update(

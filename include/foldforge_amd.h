@@ -108,6 +108,20 @@ int32_t ffk_restore_activation(const void* codes, const void* scales, void* x, i
                                int32_t dtype, void* stream);
 
 /*
+ * Dropout and the residual add: out = residual + (kept ? x * 65536 / (65536 - dropped) : 0), the mask drawn in the call and
+ * not stored (draw it again for the backward pass: the same call on the gradient, residual NULL). x, residual (NULL: none),
+ * out [outer, shared, inner] bf16 or fp32 (dtype); out may be x or the residual. The mask is [outer, inner], the same for all
+ * `shared` (1: every value its own). Value m of it is dropped where the 16-bit number m is below `dropped` (0 .. 65536: the
+ * rate times 65536, 65536 drops everything): numbers 8 b .. 8 b + 7 are the four 32-bit words, low halves first, of
+ * Philox4x32-10 at the counter (b, offset), 64 bits each, low words first, under the 64-bit key `seed`. state (NULL: none) is
+ * two int64 on the device, read when the kernel runs: the seed (in the place of `seed`) and what is added to `offset`, so that
+ * a captured call draws anew at each replay. No counterpart in the reference, whose op classes carry the rate (p_drop).
+ */
+int32_t ffk_dropout_add(const void* x, const void* residual, void* out, const int64_t* state, int64_t seed,
+                        int64_t offset, int64_t outer, int64_t shared, int64_t inner, int32_t dropped, int32_t dtype,
+                        void* stream);
+
+/*
  * ffk_layer_norm that keeps its input as an 8-bit activation in the same pass (y may not alias x).
  */
 int32_t ffk_layer_norm_checkpoint(const void* x, const float* weight, const float* bias, void* y,

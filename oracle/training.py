@@ -1,9 +1,12 @@
 """The training operators at 64 bits, from their definitions: the 8-bit activation, LayerNorm's backward
 pass and the SwiGLU transition's (the gradients of ``legacy/reference/transition.py:28-59`` of the
-reference and of the LayerNorm in front of it)."""
+reference and of the LayerNorm in front of it), dropout's mask and its sum with the residual."""
 
 from __future__ import annotations
 
+import math
+
+import numpy as np
 import torch
 
 Tensor = torch.Tensor
@@ -84,3 +87,37 @@ def transition_backward(dy: Tensor, x: Tensor, *, ln_weight: Tensor, ln_bias: Te
     dx, dw, dbias = layer_norm_backward(da @ wa + db @ wb, x, ln_weight, eps)
     return dict(x=((dy if residual else 0) + dx).reshape(shape), ln_weight=dw, ln_bias=dbias, expand_a=da.T @ n,
                 expand_b=db.T @ n, squeeze=dy.T @ (a * s * b))
+
+
+def philox(counter: np.ndarray, key: int) -> np.ndarray:
+    """Philox4x32-10 of counters ``[n, 4]`` (32-bit words in uint64) under a 64-bit key: the four words ``[n, 4]``."""
+    word, half = np.uint64(0xFFFFFFFF), np.uint64(32)
+    a, b, c, d = (counter[:, i].astype(np.uint64) for i in range(4))
+    k = [key & 0xFFFFFFFF, key >> 32]
+    for _ in range(10):
+        left, right = a * np.uint64(0xD2511F53), c * np.uint64(0xCD9E8D57)
+        a, b, c, d = ((right >> half) ^ b ^ np.uint64(k[0]), right & word,
+                      (left >> half) ^ d ^ np.uint64(k[1]), left & word)
+        k = [(k[0] + 0x9E3779B9) % 2**32, (k[1] + 0xBB67AE85) % 2**32]
+    return np.stack([a, b, c, d], 1)
+
+
+def dropout_mask(shape: tuple[int, ...], shared: int | None, p: float, seed: int, offset: int) -> Tensor:
+    """Which values of a tensor are kept, ``[...]`` with size 1 along ``shared``."""
+    shape = list(shape)
+    if shared is not None:
+        shape[shared] = 1
+    n = math.prod(shape)
+    blocks = np.arange(-(-n // 8), dtype=np.uint64)
+    counter = np.stack([blocks % 2**32, blocks // 2**32, np.full_like(blocks, offset % 2**32),
+                        np.full_like(blocks, offset // 2**32)], 1)
+    words = philox(counter, seed)
+    numbers = np.stack([words % 2**16, words // 2**16], 2).reshape(-1)[:n]
+    return torch.from_numpy((numbers >= round(65536 * p)).reshape(shape))
+
+
+def dropout_add(update: Tensor, residual: Tensor | None, shared: int | None, p: float, seed: int, offset: int) -> Tensor:
+    drop = round(65536 * p)
+    keep = dropout_mask(update.shape, shared, p, seed, offset)
+    y = torch.where(keep, update.double() * 65536 / max(65536 - drop, 1), 0.0)
+    return y if residual is None else residual.double() + y
