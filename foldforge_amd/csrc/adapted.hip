@@ -1,0 +1,893 @@
+// A projection with the low-rank adapters of many requests beside it, forward and backward:
+//   y_t  = W x_t + b + s_a B_a (A_a x_t)          W [d_out][d_in], A_a [rank][d_in], B_a [d_out][rank]
+//   dx_t = W^T dy_t + A_a^T v_t,  v_t = s_a B_a^T dy_t,  u_t = s_a A_a x_t
+//   dA_a = sum over its rows of v_t x_t^T,  dB_a = sum over its rows of dy_t u_t^T
+// a: the adapter of the request that row t belongs to (request r has the rows offsets[r] .. offsets[r + 1] - 1; rows of no
+// request, and requests whose adapter is none of them, have W and b alone). W is frozen: no gradient.
+//
+// The thin products (u, v: d x rank) go first, into rows of rank numbers; the wide product then takes them as rank more
+// channels of the same sum, so its rows are read and written once. Operands of the products are bf16, sums fp32. For the
+// adapters' gradients, which are sums over up to 10^5 rows in fp32, u and v are kept as two bf16 (high and low part: 16 bits)
+// and fp32 adapters enter as two as well: off by some 2^-17 of the terms. The forward pass keeps the high parts, whose
+// rounding is that of its output.
+// Rows of other adapters are left out by selection, not by factors of zero: infinities and NaN of one request (or of one
+// adapter's weights) reach no other's rows or gradients.
+#include <algorithm>
+
+#include "ffk_device.h"
+#include "ffk_kernels.h"
+
+namespace ffk {
+
+namespace {
+
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// which adapter a row has
+
+struct Requests {
+  const int32_t *offsets, *adapter;  // [count + 1], [count]
+  const float* scale;                // [adapters], or null (1)
+  int count, adapters;
+  int64_t rows;
+};
+
+// id[i], i < 64: the adapter of row row0 + i, -1 for none (and behind the last row). All threads of the workgroup (of NT);
+// start and before are its scratch. One pass over the offsets: how many begin at or before the first row, and which begin at
+// each of the others; then the latest request that begins at or before each row. Offsets out of order give some adapter or
+// none, never an access out of range.
+template <int NT>
+__device__ __forceinline__ void tile_ids(const Requests& q, int64_t row0, int* id, int* start, int* before) {
+  const int tid = threadIdx.x;
+  if (tid < 64) start[tid] = -1;
+  if (tid == 0) *before = 0;
+  __syncthreads();
+  for (int i = tid; i <= q.count; i += NT) {
+    const int64_t at = (int64_t)q.offsets[i] - row0;
+    if (at <= 0)
+      atomicMax(before, i + 1);  // (in order: the number of such offsets)
+    else if (at < 64)
+      atomicMax(&start[at], i);
+  }
+  __syncthreads();
+  if (tid < 64) {
+    int r = tid == 0 ? *before - 1 : start[tid];
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) {
+      const int o = __shfl_up(r, m, 64);
+      if (tid >= m && o > r) r = o;
+    }
+    int a = -1;
+    if (r >= 0 && r < q.count && row0 + tid < q.rows) a = q.adapter[r];
+    id[tid] = a >= 0 && a < q.adapters ? a : -1;
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ float scale_of(const Requests& q, int a) { return q.scale ? q.scale[a] : 1.f; }
+
+// ---------------------------------------------------------------------------------------------------------
+// operands in the products' orders
+
+// dst [batch][out_rows][out_cols] bf16 (and what its rounding left, in lo) from src [batch][rows][cols] (turn: transposed),
+// zeros outside.
+struct PackJob {
+  const void* src;
+  bf16 *hi, *lo;  // lo may be null
+  int64_t rows, cols, out_rows, out_cols, tiles;  // tiles: of 32 x 32, all batches
+  int f32, turn;
+};
+constexpr int kPackJobs = 6;
+struct PackArgs {
+  PackJob job[kPackJobs];
+  int jobs;
+};
+
+// The 32 x 32 tiles of the destinations, the jobs' one after the other. block 256.
+__global__ __launch_bounds__(256) void adapted_pack(const PackArgs p, int64_t tiles) {
+  __shared__ float t[32][33];
+  const int col = threadIdx.x & 31, row = threadIdx.x >> 5;
+  for (int64_t at = blockIdx.x; at < tiles; at += gridDim.x) {
+    int64_t tile = at;
+    int which = 0;
+    while (which + 1 < p.jobs && tile >= p.job[which].tiles) tile -= p.job[which++].tiles;
+    const PackJob& j = p.job[which];
+    const int64_t across = (j.out_cols + 31) / 32, down = (j.out_rows + 31) / 32;
+    const int64_t c0 = tile % across * 32, r0 = tile / across % down * 32, batch = tile / across / down;
+    const int64_t sr = j.turn ? c0 : r0, sc = j.turn ? r0 : c0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t r = sr + row + 8 * i, c = sc + col;
+      float v = 0.f;
+      if (r < j.rows && c < j.cols) {
+        const int64_t from = (batch * j.rows + r) * j.cols + c;
+        v = j.f32 ? static_cast<const float*>(j.src)[from] : (float)static_cast<const bf16*>(j.src)[from];
+      }
+      t[row + 8 * i][col] = v;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t r = r0 + row + 8 * i, c = c0 + col;
+      if (r >= j.out_rows || c >= j.out_cols) continue;
+      const float v = j.turn ? t[col][row + 8 * i] : t[row + 8 * i][col];
+      const int64_t to = (batch * j.out_rows + r) * j.out_cols + c;
+      const bf16 h = (bf16)v;
+      j.hi[to] = h;
+      if (j.lo) j.lo[to] = (bf16)(v - (float)h);
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// the thin products
+
+struct ThinJob {
+  const bf16 *x, *hi, *lo;  // x [rows][K], the adapters' matrices [adapters][mat_rows][K] (lo: their low parts, or null)
+  bf16* u;                  // [rows][ld]: s_a (matrix x) in RP channels, zeros from `rank` on; behind them the low parts
+  int K, mat_rows;          // K a multiple of 64
+};
+struct ThinArgs {
+  ThinJob job[2];
+  Requests q;
+  int32_t* ids;  // [rows], written by the first job's first workgroups
+  int rank, ld;
+};
+
+// 64 / KS rows a workgroup, of 4 waves: KS = 1, 16 rows a wave; KS = 4, all 16 rows, a quarter of K a wave (few rows: more
+// workgroups). Each adapter of the rows in turn, gridDim.y workgroups share them; a lane holds a token and 4 channels.
+// grid (ceil(rows / (64 / KS)), share, jobs); block 256. LO: the adapters have low parts. OUT2: u keeps its own.
+template <int RP, bool LO, bool OUT2, int KS>
+__global__ __launch_bounds__(256) void adapted_thin(const ThinArgs p) {
+  constexpr int N = RP / 16, TM = 64 / KS;
+  __shared__ int id[64], start[64], before;
+  __shared__ f32x4 red[KS == 1 ? 1 : 4][N][64];
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row0 = (int64_t)blockIdx.x * TM;
+  const ThinJob& j = p.job[blockIdx.z];
+  tile_ids<256>(p.q, row0, id, start, &before);
+  if (blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x < TM && row0 + threadIdx.x < p.q.rows)
+    p.ids[row0 + threadIdx.x] = id[threadIdx.x];
+  const int first = KS == 1 ? 16 * wave : 0;  // of the wave's rows
+  const int64_t row = row0 + first + i;
+  const int mine = id[first + i];
+  const bf16* x = j.x + (row < p.q.rows ? row : p.q.rows - 1) * j.K + 8 * g;
+  auto store = [&](int n, const f32x4& v) __attribute__((always_inline)) {
+    bf16x4 h, l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float t = 16 * n + 4 * g + e < p.rank ? v[e] : 0.f;
+      h[e] = (bf16)t;
+      l[e] = (bf16)(t - (float)h[e]);
+    }
+    bf16* to = j.u + row * p.ld + 16 * n + 4 * g;
+    *reinterpret_cast<bf16x4*>(to) = h;
+    if constexpr (OUT2) *reinterpret_cast<bf16x4*>(to + RP) = l;
+  };
+  const f32x4 none = {0.f, 0.f, 0.f, 0.f};
+  if (blockIdx.y == 0 && mine < 0 && row < p.q.rows && (KS == 1 || wave == 0)) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) store(n, none);
+  }
+  uint64_t todo = __ballot(mine >= 0) & 0xffffu;
+  for (int turn = 0; todo != 0; ++turn) {
+    const int a = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
+    const bool is = mine == a;
+    todo &= ~__ballot(is);
+    if (turn % gridDim.y != blockIdx.y) continue;
+    f32x4 acc[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) acc[n] = none;
+    const bf16* m[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int r = 16 * n + i < j.mat_rows ? 16 * n + i : j.mat_rows - 1;
+      m[n] = j.hi + ((int64_t)a * j.mat_rows + r) * j.K + 8 * g;
+    }
+    const int64_t low = LO ? j.lo - j.hi : 0;
+#pragma unroll 4
+    for (int k = KS == 1 ? 0 : 32 * wave; k < j.K; k += 32 * KS) {
+      const bf16x8 xf = ld8(x + k);
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        acc[n] = mfma16(ld8(m[n] + k), xf, acc[n]);
+        if constexpr (LO) acc[n] = mfma16(ld8(m[n] + k + low), xf, acc[n]);
+      }
+    }
+    const float s = scale_of(p.q, a);
+    if constexpr (KS == 1) {
+      if (is) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) store(n, acc[n] * s);
+      }
+    } else {
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < N; ++n) red[wave][n][lane] = acc[n];
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        if (n % 4 == wave && is) store(n, (red[0][n][lane] + red[1][n][lane] + (red[2][n][lane] + red[3][n][lane])) * s);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// the wide product
+
+struct ProductArgs {
+  const bf16 *x, *w;  // [rows][K], [N][K], K a multiple of 64
+  const bf16 *u, *b;  // [rows][ld], the adapters' [adapters][N][RP]
+  const int32_t* ids;
+  const float* bias;  // or null
+  bf16* out;          // [rows][N]
+  int64_t rows;
+  int K, N, RP, ld, n_tiles;
+};
+
+// out = x W^T + u B_a^T + bias in TM rows x TN channels a workgroup, a quarter of them a wave: weight rows x token rows, so a
+// lane holds a token. K in steps of 64 through STAGES buffers by LDS DMA. The adapters of a wave's 32 tokens one after the
+// other at the end, each added to the lanes that have it. grid: m tiles x n tiles, the n tiles of an m tile neighbours (they
+// share its rows in an XCD's L2); block 256.
+template <int TM, int TN, int STAGES>
+__global__ __launch_bounds__(256, 2) void adapted_product(const ProductArgs p) {
+  constexpr int XT = TM / 64, WT = TN / 64, PER = 2 * (XT + WT);  // 64 x 64 tiles a step, transfers of a wave
+  __shared__ __attribute__((aligned(16))) bf16 buf[STAGES][XT + WT][64 * 64];
+  const int lane = threadIdx.x & 63, g = lane >> 5, li = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
+  const uint32_t id = xcd_remap(blockIdx.x, gridDim.x);
+  const int64_t m0 = (int64_t)(id / p.n_tiles) * TM;
+  const int n0 = (int)(id % p.n_tiles) * TN;
+  const int steps = p.K / 64;
+  const uint32_t lds = lds_addr(buf);
+  auto fetch = [&](int step) __attribute__((always_inline)) {
+    const uint32_t at = lds + step % STAGES * (XT + WT) * 8192;
+#pragma unroll
+    for (int t = 0; t < XT; ++t) tile_dma(p.x + 64 * step, p.K, m0 + 64 * t, p.rows - 1, 0, at + 8192 * t, wave, lane);
+#pragma unroll
+    for (int t = 0; t < WT; ++t)
+      tile_dma(p.w + 64 * step, p.K, n0 + 64 * t, p.N - 1, 0, at + 8192 * (XT + t), wave, lane);
+  };
+  f32x16 acc[WT][XT];
+#pragma unroll
+  for (int c = 0; c < WT; ++c)
+#pragma unroll
+    for (int t = 0; t < XT; ++t) acc[c][t] = zero16();
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s)
+    if (s < steps) fetch(s);
+  for (int s = 0; s < steps; ++s) {
+    if (s + STAGES - 1 <= steps)
+      wait_vm_lds<(STAGES - 2) * PER>();
+    else
+      wait_vm_lds<0>();
+    __syncthreads();  // the step has landed; the buffer of the one before has been read
+    if (s + STAGES - 1 < steps) fetch(s + STAGES - 1);
+    const bf16(*t)[64 * 64] = buf[s % STAGES];
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      bf16x8 fw[WT], fx[XT];
+#pragma unroll
+      for (int c = 0; c < WT; ++c) {
+        const int r = wn * (TN / 2) + 32 * c + li;
+        fw[c] = ld8(&t[XT + (r >> 6)][off64(r & 63, 2 * kk + g)]);
+      }
+#pragma unroll
+      for (int c = 0; c < XT; ++c) {
+        const int r = wm * (TM / 2) + 32 * c + li;
+        fx[c] = ld8(&t[r >> 6][off64(r & 63, 2 * kk + g)]);
+      }
+#pragma unroll
+      for (int c = 0; c < WT; ++c)
+#pragma unroll
+        for (int x = 0; x < XT; ++x) acc[c][x] = mfma32(fw[c], fx[x], acc[c][x]);
+    }
+  }
+  const int nw = n0 + wn * (TN / 2);
+#pragma unroll
+  for (int x = 0; x < XT; ++x) {
+    const int64_t row = m0 + wm * (TM / 2) + 32 * x + li;
+    const bool real = row < p.rows;
+    const int mine = real ? p.ids[row] : -1;
+    const bf16* u = p.u + (real ? row : p.rows - 1) * p.ld + 8 * g;
+    uint64_t todo = __ballot(mine >= 0) & 0xffffffffu;
+    while (todo != 0) {
+      const int a = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
+      todo &= ~__ballot(mine == a);
+      f32x16 add[WT];
+      const bf16* b[WT];
+#pragma unroll
+      for (int c = 0; c < WT; ++c) {
+        add[c] = zero16();
+        const int n = nw + 32 * c + li;
+        b[c] = p.b + ((int64_t)a * p.N + (n < p.N ? n : p.N - 1)) * p.RP + 8 * g;
+      }
+      for (int j = 0; j < p.RP; j += 16) {
+        const bf16x8 uf = ld8(u + j);
+#pragma unroll
+        for (int c = 0; c < WT; ++c) add[c] = mfma32(ld8(b[c] + j), uf, add[c]);
+      }
+#pragma unroll
+      for (int c = 0; c < WT; ++c)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[c][x][r] += mine == a ? add[c][r] : 0.f;
+    }
+#pragma unroll
+    for (int c = 0; c < WT; ++c) {
+      float y[2][8];
+      acc_pieces(acc[c][x], y);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int n = nw + 32 * c + 8 * (2 * k + g);
+        if (!real || n >= p.N) continue;
+        if (p.bias) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[k][e] += n + e < p.N ? p.bias[n + e] : 0.f;
+        }
+        bf16* to = p.out + row * p.N + n;
+        if (p.N % 8 == 0) {
+          bf16x8 v;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = (bf16)y[k][e];
+          *reinterpret_cast<bf16x8*>(to) = v;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (n + e < p.N) to[e] = (bf16)y[k][e];
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// the adapters' gradients
+
+struct GradJob {
+  const bf16 *x, *v;       // [rows][ld_x] (ld_x a multiple of 64), [rows][2 RP]: high and low parts
+  void* to;                // element (chunk, a, channel j, column c) at chunk * chunk_stride + (a * rank) * cols + j * sj + c * sc
+  int64_t sj, sc;
+  int cols, ld_x, tiles;   // tiles = ld_x / 64
+};
+struct GradArgs {
+  GradJob job[2];
+  const int32_t* ids;
+  int64_t rows, chunk, chunk_stride[2];  // rows of a chunk: a multiple of 64, at most 64 * kMostGradTiles
+  int rank, to_bf16;
+};
+constexpr int kMostGradTiles = 256;
+
+// sum over a chunk's rows of adapter blockIdx.y of v x^T: RP channels x 64 columns a workgroup. Tiles of 64 rows that have a
+// row of the adapter's, in order, through three buffers by LDS DMA; the rows of others in them are zeroed there. A wave takes
+// 16 of a tile's rows (k of the product; both operands turned as they are read), the waves' sums meet at the end in a fixed
+// order. RP = 16: the high and low channels are the 32 rows of one product, else two products. grid (both jobs' tiles,
+// adapters, chunks); block 256.
+template <int RP>
+__global__ __launch_bounds__(256) void adapted_grad(const GradArgs p) {
+  constexpr int VT = RP <= 32 ? 1 : RP / 32, JB = RP <= 32 ? 1 : RP / 32, STAGES = 3, PER = 2 * (1 + VT);
+  __shared__ __attribute__((aligned(16))) bf16 buf[STAGES][1 + VT][64 * 64];
+  __shared__ uint64_t has[kMostGradTiles];  // which rows of a tile are the adapter's
+  __shared__ int list[kMostGradTiles], listed;
+  const int lane = threadIdx.x & 63, g = lane >> 5, li = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int which = (int)blockIdx.x >= p.job[0].tiles ? 1 : 0;
+  const GradJob& j = p.job[which];
+  const int c0 = 64 * ((int)blockIdx.x - (which ? p.job[0].tiles : 0)), a = blockIdx.y;
+  const int64_t begin = blockIdx.z * p.chunk, end = begin + p.chunk < p.rows ? begin + p.chunk : p.rows;
+  const int tiles = (int)((end - begin + 63) / 64);
+  for (int t = wave; t < tiles; t += 4) {
+    const int64_t row = begin + 64 * t + lane;
+    const uint64_t m = __ballot(row < end && p.ids[row] == a);
+    if (lane == 0) has[t] = m;
+  }
+  __syncthreads();
+  if (wave == 0) {
+    int n = 0;
+    for (int t0 = 0; t0 < tiles; t0 += 64) {
+      const bool some = t0 + lane < tiles && has[t0 + lane] != 0;
+      const uint64_t m = __ballot(some);
+      if (some) list[n + __popcll(m & ((1ull << lane) - 1))] = t0 + lane;
+      n += __popcll(m);
+    }
+    if (lane == 0) listed = n;
+  }
+  __syncthreads();
+  const int steps = listed;
+  const uint32_t lds = lds_addr(buf);
+  auto fetch = [&](int step) __attribute__((always_inline)) {
+    const uint32_t at = lds + step % STAGES * (1 + VT) * 8192;
+    const int64_t row0 = begin + 64 * list[step];
+    tile_dma(j.x, j.ld_x, row0, p.rows - 1, c0, at, wave, lane);
+    if constexpr (RP == 16) {  // rows of 32 channels in tiles of 64: the pieces twice
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int r0 = 8 * (2 * wave + u), r = r0 + (lane >> 3);
+        const int64_t row = row0 + r < p.rows ? row0 + r : p.rows - 1;
+        dma16_at(j.v + row * 32 + 8 * (((lane & 7) ^ swz64(r)) & 3), at + 8192 + 128 * r0);
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < VT; ++t) tile_dma(j.v, 2 * RP, row0, p.rows - 1, 64 * t, at + 8192 * (1 + t), wave, lane);
+    }
+  };
+  f32x16 acc[JB][2];
+#pragma unroll
+  for (int b = 0; b < JB; ++b) acc[b][0] = acc[b][1] = zero16();
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s)
+    if (s < steps) fetch(s);
+  for (int s = 0; s < steps; ++s) {
+    if (s + STAGES - 1 <= steps)
+      wait_vm_lds<(STAGES - 2) * PER>();
+    else
+      wait_vm_lds<0>();
+    __syncthreads();  // the tile has landed; the buffer of the one before has been read
+    if (s + STAGES - 1 < steps) fetch(s + STAGES - 1);
+    bf16(*t)[64 * 64] = buf[s % STAGES];
+    const uint64_t rows = has[list[s]];
+    if (~rows != 0) {
+      bf16x8 z;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z[e] = (bf16)0.f;
+      for (int i = threadIdx.x; i < (1 + VT) * 64 * 8; i += 256)
+        if (!(rows >> ((i >> 3) & 63) & 1u)) *reinterpret_cast<bf16x8*>(t[i >> 9] + 8 * (i & 511)) = z;
+      __syncthreads();
+    }
+    bf16x8 x[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) x[h] = ld_turned(t[0], 32 * h, 16 * wave, lane);
+#pragma unroll
+    for (int b = 0; b < (RP == 16 ? 1 : 2 * JB); ++b) {  // 32 channels each: the high parts, then the low ones
+      const bf16x8 v = ld_turned(t[1 + b / 2], 32 * (b & 1), 16 * wave, lane);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) acc[b % JB][h] = mfma32(v, x[h], acc[b % JB][h]);
+    }
+  }
+  float* sum = reinterpret_cast<float*>(buf);  // [wave][32][64]
+#pragma unroll
+  for (int b = 0; b < JB; ++b) {
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum[(wave * 32 + acc_row(r, g)) * 64 + 32 * h + li] = acc[b][h][r];
+    __syncthreads();
+    for (int i = threadIdx.x; i < (RP == 16 ? 16 : 32) * 64; i += 256) {
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) v += sum[w * 2048 + i];
+      if constexpr (RP == 16) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) v += sum[w * 2048 + 1024 + i];
+      }
+      const int row = 32 * b + (i >> 6), c = c0 + (i & 63);
+      if (row >= p.rank || c >= j.cols) continue;
+      const int64_t at =
+          blockIdx.z * p.chunk_stride[which] + (int64_t)a * p.rank * j.cols + row * j.sj + c * j.sc;
+      if (p.to_bf16)
+        static_cast<bf16*>(j.to)[at] = (bf16)v;
+      else
+        static_cast<float*>(j.to)[at] = v;
+    }
+  }
+}
+
+struct JoinJob {
+  const float* part;  // [chunks][adapters][rank][cols]
+  void* to;
+  int64_t sj, sc;     // as GradJob's
+  int64_t count;      // adapters * rank * cols
+  int cols;
+};
+struct JoinArgs {
+  JoinJob job[2];
+  int chunks, rank, to_bf16;
+};
+
+// The chunks' sums in order. grid: ceil of both jobs' counts / 256; block 256.
+__global__ __launch_bounds__(256) void adapted_join(const JoinArgs p) {
+  int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t head = (p.job[0].count + 255) / 256 * 256;
+  const int which = i >= head ? 1 : 0;
+  const JoinJob& j = p.job[which];
+  if (which) i -= head;
+  if (i >= j.count) return;
+  float v = 0.f;
+  for (int k = 0; k < p.chunks; ++k) v += j.part[k * j.count + i];
+  const int64_t c = i % j.cols, row = i / j.cols % p.rank, a = i / j.cols / p.rank;
+  const int64_t at = a * p.rank * j.cols + row * j.sj + c * j.sc;
+  if (p.to_bf16)
+    static_cast<bf16*>(j.to)[at] = (bf16)v;
+  else
+    static_cast<float*>(j.to)[at] = v;
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// few rows
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int64_t left, float (&v)[8]) {
+  typedef T vec __attribute__((__vector_size__(8 * sizeof(T)), aligned(sizeof(T))));
+  if (left >= 8) {
+    const vec t = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)t[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < left ? (float)p[e] : 0.f;
+  }
+}
+
+struct FewArgs {
+  const bf16* x;
+  const void *w, *down, *up;
+  const float* bias;
+  bf16* out;
+  Requests q;
+  float* u;      // [rows][rank]
+  int32_t* ids;  // [rows]
+  int K, N, rank;
+};
+
+// u of one row a workgroup in fp32, four channels a wave at a time, k across the lanes. grid rows; block 256.
+template <typename TA>
+__global__ __launch_bounds__(256) void adapted_few_thin(const FewArgs p) {
+  __shared__ int id[64], start[64], before;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row = blockIdx.x;
+  tile_ids<256>(p.q, row, id, start, &before);
+  const int a = id[0];
+  if (threadIdx.x == 0) p.ids[row] = a;
+  if (a < 0) return;
+  const TA* m = static_cast<const TA*>(p.down) + (int64_t)a * p.rank * p.K;
+  const float s = scale_of(p.q, a);
+  for (int j0 = 4 * wave; j0 < p.rank; j0 += 16) {
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int k = 8 * lane; k < p.K; k += 512) {
+      float x[8];
+      load8(p.x + row * p.K + k, p.K - k, x);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float v[8];
+        load8(m + (int64_t)(j0 + j < p.rank ? j0 + j : p.rank - 1) * p.K + k, p.K - k, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[j] += x[e] * v[e];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float v = lanes_sum<64>(sum[j]);
+      if (lane == 0 && j0 + j < p.rank) p.u[row * p.rank + j0 + j] = s * v;
+    }
+  }
+}
+
+// 16 channels x 16 RT rows a workgroup, a quarter of k a wave, operands straight from memory; the adapters as dot products of
+// rank terms, a thread for each output. grid (ceil(N / 16), ceil(rows / (16 RT))); block 256.
+template <typename TW, typename TA, int RT>
+__global__ __launch_bounds__(256) void adapted_few(const FewArgs p) {
+  __shared__ float red[4][RT][16][20];  // [wave][..][token][channel], rows of 20: 16-byte stores without conflicts
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
+  const int n0 = 16 * blockIdx.x;
+  const int64_t row0 = 16 * RT * (int64_t)blockIdx.y;
+  f32x4 acc[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const TW* w = static_cast<const TW*>(p.w) + (int64_t)(n0 + i < p.N ? n0 + i : p.N - 1) * p.K;
+  const bf16* x[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int64_t row = row0 + 16 * t + i;
+    x[t] = p.x + (row < p.q.rows ? row : p.q.rows - 1) * p.K;
+  }
+#pragma unroll 2
+  for (int k = 32 * wave + 8 * g; k - 8 * g < p.K; k += 128) {
+    float v[8];
+    load8(w + k, p.K - k, v);
+    bf16x8 wf;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) wf[e] = (bf16)v[e];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      load8(x[t] + k, p.K - k, v);
+      bf16x8 xf;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) xf[e] = (bf16)v[e];
+      acc[t] = mfma16(wf, xf, acc[t]);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < RT; ++t) *reinterpret_cast<f32x4*>(&red[wave][t][i][4 * g]) = acc[t];
+  __syncthreads();
+  const int token = threadIdx.x >> 4, c = threadIdx.x & 15, n = n0 + c;
+  if (n >= p.N) return;
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int64_t row = row0 + 16 * t + token;
+    if (row >= p.q.rows) return;
+    float y = (red[0][t][token][c] + red[1][t][token][c]) + (red[2][t][token][c] + red[3][t][token][c]);
+    if (p.bias) y += p.bias[n];
+    const int a = p.ids[row];
+    if (a >= 0) {
+      const TA* b = static_cast<const TA*>(p.up) + ((int64_t)a * p.N + n) * p.rank;
+      const float* u = p.u + row * p.rank;
+      float sum = 0.f;
+      for (int j = 0; j < p.rank; j += 8) {
+        float v[8], q[8];
+        load8(b + j, p.rank - j, v);
+        load8(u + j, p.rank - j, q);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += v[e] * q[e];
+      }
+      y += sum;
+    }
+    p.out[row * p.N + n] = (bf16)y;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// launches
+
+template <typename TW, typename TA>
+void launch_few(const FewArgs& f, hipStream_t st) {
+  const int64_t rows = f.q.rows;
+  adapted_few_thin<TA><<<dim3((unsigned)rows), 256, 0, st>>>(f);
+  const unsigned across = (unsigned)((f.N + 15) / 16);
+  if (rows <= 16)
+    adapted_few<TW, TA, 1><<<dim3(across), 256, 0, st>>>(f);
+  else if (rows <= 32)
+    adapted_few<TW, TA, 2><<<dim3(across), 256, 0, st>>>(f);
+  else
+    adapted_few<TW, TA, 4><<<dim3(across, (unsigned)((rows + 63) / 64)), 256, 0, st>>>(f);
+}
+
+int64_t tiles32(int64_t batch, int64_t rows, int64_t cols) { return batch * ((rows + 31) / 32) * ((cols + 31) / 32); }
+
+struct Packer {
+  PackArgs args{};
+  int64_t tiles = 0;
+  void add(const void* src, int f32, bf16* hi, bf16* lo, int64_t batch, int64_t rows, int64_t cols, int64_t out_rows,
+           int64_t out_cols, bool turn) {
+    PackJob j;
+    j.src = src;
+    j.hi = hi;
+    j.lo = lo;
+    j.rows = rows;
+    j.cols = cols;
+    j.out_rows = out_rows;
+    j.out_cols = out_cols;
+    j.tiles = tiles32(batch, out_rows, out_cols);
+    j.f32 = f32;
+    j.turn = turn;
+    args.job[args.jobs++] = j;
+    tiles += j.tiles;
+  }
+  void launch(hipStream_t st) const {
+    if (tiles > 0) adapted_pack<<<dim3((unsigned)std::min<int64_t>(tiles, 1 << 20)), 256, 0, st>>>(args, tiles);
+  }
+};
+
+template <bool LO, bool OUT2>
+void launch_thin(const ThinArgs& a, int rp, int jobs, hipStream_t st) {
+  const int64_t rows = a.q.rows;
+  // few rows: a quarter of k a wave, so that the chip is filled, and the adapters of 16 rows shared out where they may be many
+  const bool split = rows < 64 * 256;
+  const int share = split && a.q.count > (int)(rows / 16) ? 4 : 1;
+  const dim3 grid((unsigned)((rows + (split ? 15 : 63)) / (split ? 16 : 64)), share, jobs);
+#define FFK_THIN(RP)                                      \
+  if (rp == RP) {                                         \
+    if (split)                                            \
+      adapted_thin<RP, LO, OUT2, 4><<<grid, 256, 0, st>>>(a); \
+    else                                                  \
+      adapted_thin<RP, LO, OUT2, 1><<<grid, 256, 0, st>>>(a); \
+  }
+  FFK_THIN(16)
+  FFK_THIN(32)
+  FFK_THIN(64)
+  FFK_THIN(128)
+#undef FFK_THIN
+}
+
+void launch_product(ProductArgs a, hipStream_t st) {
+  const int64_t big = ((a.rows + 127) / 128) * ((a.N + 127) / 128);
+  if (big >= 256 && a.N > 64) {
+    a.n_tiles = (a.N + 127) / 128;
+    adapted_product<128, 128, 2><<<dim3((unsigned)big), 256, 0, st>>>(a);
+  } else {
+    a.n_tiles = (a.N + 63) / 64;
+    adapted_product<64, 64, 4><<<dim3((unsigned)((a.rows + 63) / 64 * a.n_tiles)), 256, 0, st>>>(a);
+  }
+}
+
+int64_t up64(int64_t n) { return (n + 63) / 64 * 64; }
+
+Requests requests_of(const AdaptedArgs& a) {
+  Requests q;
+  q.offsets = a.offsets;
+  q.adapter = a.adapter;
+  q.scale = a.scale;
+  q.count = a.requests;
+  q.adapters = a.adapters;
+  q.rows = a.rows;
+  return q;
+}
+
+}  // namespace
+
+AdaptedPlan adapted_plan(int64_t rows, int d_in, int d_out, int adapters, int rank, int w_f32, int a_f32, int backward) {
+  AdaptedPlan p{};
+  p.rp = rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128;
+  p.kp = up64(d_in);
+  p.np = up64(d_out);
+  p.few = !backward && rows <= 256;
+  if (backward) {
+    p.pack_x = d_in % 64 != 0;
+    p.pack_dy = d_out % 64 != 0;
+    p.pack_down = a_f32 || d_in % 64 != 0;
+    const int64_t tiles = (p.kp + p.np) / 64 * adapters;
+    // some four workgroups a CU, of chunks of 256 rows at least
+    int64_t chunks = std::max<int64_t>(1, std::min<int64_t>((1024 + tiles - 1) / tiles, (rows + 255) / 256));
+    p.chunk = std::min<int64_t>(up64((rows + chunks - 1) / chunks), 64 * kMostGradTiles);
+    p.chunks = (int)((rows + p.chunk - 1) / p.chunk);
+  } else {
+    p.pack_x = d_in % 64 != 0;
+    p.pack_w = w_f32 || d_in % 64 != 0;
+    p.pack_down = a_f32 || d_in % 64 != 0;
+    p.pack_up = a_f32 || rank != p.rp;
+  }
+  return p;
+}
+
+void launch_adapted(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t st) {
+  const Requests q = requests_of(a);
+  if (p.few) {
+    FewArgs f{};
+    f.x = a.x;
+    f.w = a.w;
+    f.down = a.down;
+    f.up = a.up;
+    f.bias = a.bias;
+    f.out = a.out;
+    f.q = q;
+    f.u = a.few_u;
+    f.ids = a.ids;
+    f.K = a.d_in;
+    f.N = a.d_out;
+    f.rank = a.rank;
+    if (a.w_f32)
+      a.a_f32 ? launch_few<float, float>(f, st) : launch_few<float, bf16>(f, st);
+    else
+      a.a_f32 ? launch_few<bf16, float>(f, st) : launch_few<bf16, bf16>(f, st);
+    return;
+  }
+  Packer pack;
+  if (p.pack_x) pack.add(a.x, 0, a.xp, nullptr, 1, a.rows, a.d_in, a.rows, p.kp, false);
+  if (p.pack_w) pack.add(a.w, a.w_f32, a.wp, nullptr, 1, a.d_out, a.d_in, a.d_out, p.kp, false);
+  if (p.pack_down) pack.add(a.down, a.a_f32, a.down_hi, nullptr, a.adapters, a.rank, a.d_in, a.rank, p.kp, false);
+  if (p.pack_up) pack.add(a.up, a.a_f32, a.upp, nullptr, a.adapters, a.d_out, a.rank, a.d_out, p.rp, false);
+  pack.launch(st);
+  ThinArgs t{};
+  t.job[0].x = p.pack_x ? a.xp : a.x;
+  t.job[0].hi = p.pack_down ? a.down_hi : static_cast<const bf16*>(a.down);
+  t.job[0].u = a.u;
+  t.job[0].K = p.kp;
+  t.job[0].mat_rows = a.rank;
+  t.q = q;
+  t.ids = a.ids;
+  t.rank = a.rank;
+  t.ld = p.rp;
+  launch_thin<false, false>(t, p.rp, 1, st);
+  ProductArgs g{};
+  g.x = t.job[0].x;
+  g.w = p.pack_w ? a.wp : static_cast<const bf16*>(a.w);
+  g.u = a.u;
+  g.b = p.pack_up ? a.upp : static_cast<const bf16*>(a.up);
+  g.ids = a.ids;
+  g.bias = a.bias;
+  g.out = a.out;
+  g.rows = a.rows;
+  g.K = p.kp;
+  g.N = a.d_out;
+  g.RP = p.rp;
+  g.ld = p.rp;
+  launch_product(g, st);
+}
+
+void launch_adapted_grad(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t st) {
+  Packer pack;
+  if (p.pack_x) pack.add(a.x, 0, a.xp, nullptr, 1, a.rows, a.d_in, a.rows, p.kp, false);
+  if (p.pack_dy) pack.add(a.dy, 0, a.dyp, nullptr, 1, a.rows, a.d_out, a.rows, p.np, false);
+  if (a.out) pack.add(a.w, a.w_f32, a.wp, nullptr, 1, a.d_out, a.d_in, a.d_in, p.np, true);
+  if (p.pack_down) pack.add(a.down, a.a_f32, a.down_hi, a.a_f32 ? a.down_lo : nullptr, a.adapters, a.rank, a.d_in, a.rank,
+                            p.kp, false);
+  pack.add(a.up, a.a_f32, a.up_hi, a.a_f32 ? a.up_lo : nullptr, a.adapters, a.d_out, a.rank, a.rank, p.np, true);
+  if (a.out) pack.add(a.down, a.a_f32, a.down_t, nullptr, a.adapters, a.rank, a.d_in, a.d_in, p.rp, true);
+  pack.launch(st);
+  ThinArgs t{};
+  t.job[0].x = p.pack_x ? a.xp : a.x;
+  t.job[0].hi = p.pack_down ? a.down_hi : static_cast<const bf16*>(a.down);
+  t.job[0].lo = a.a_f32 ? a.down_lo : nullptr;
+  t.job[0].u = a.u;
+  t.job[0].K = p.kp;
+  t.job[1].x = p.pack_dy ? a.dyp : a.dy;
+  t.job[1].hi = a.up_hi;
+  t.job[1].lo = a.a_f32 ? a.up_lo : nullptr;
+  t.job[1].u = a.v;
+  t.job[1].K = p.np;
+  t.job[0].mat_rows = t.job[1].mat_rows = a.rank;
+  t.q = requests_of(a);
+  t.ids = a.ids;
+  t.rank = a.rank;
+  t.ld = 2 * p.rp;
+  a.a_f32 ? launch_thin<true, true>(t, p.rp, 2, st) : launch_thin<false, true>(t, p.rp, 2, st);
+  if (a.out) {
+    ProductArgs g{};
+    g.x = t.job[1].x;
+    g.w = a.wp;
+    g.u = a.v;
+    g.b = a.down_t;
+    g.ids = a.ids;
+    g.out = a.out;
+    g.rows = a.rows;
+    g.K = p.np;
+    g.N = a.d_in;
+    g.RP = p.rp;
+    g.ld = 2 * p.rp;
+    launch_product(g, st);
+  }
+  const bool join = p.chunks > 1;
+  GradArgs d{};
+  d.job[0].x = t.job[0].x;
+  d.job[0].v = a.v;
+  d.job[0].cols = a.d_in;
+  d.job[0].ld_x = p.kp;
+  d.job[1].x = t.job[1].x;
+  d.job[1].v = a.u;
+  d.job[1].cols = a.d_out;
+  d.job[1].ld_x = p.np;
+  void* to[2] = {a.ddown, a.dup};
+  const int64_t sj[2] = {a.d_in, 1}, sc[2] = {1, a.rank};
+  JoinArgs e{};
+  int64_t counts = 0;
+  for (int i = 0; i < 2; ++i) {
+    GradJob& j = d.job[i];
+    const int64_t count = (int64_t)a.adapters * a.rank * j.cols;
+    j.tiles = j.ld_x / 64;
+    j.to = join ? (i ? a.part[1] : a.part[0]) : to[i];
+    j.sj = join ? j.cols : sj[i];
+    j.sc = join ? 1 : sc[i];
+    d.chunk_stride[i] = join ? count : 0;
+    e.job[i].part = a.part[i];
+    e.job[i].to = to[i];
+    e.job[i].sj = sj[i];
+    e.job[i].sc = sc[i];
+    e.job[i].count = count;
+    e.job[i].cols = j.cols;
+    counts += (count + 255) / 256;
+  }
+  d.ids = a.ids;
+  d.rows = a.rows;
+  d.chunk = p.chunk;
+  d.rank = a.rank;
+  d.to_bf16 = !join && a.grad_dtype == 0;
+  const dim3 grid((unsigned)(d.job[0].tiles + d.job[1].tiles), (unsigned)a.adapters, (unsigned)p.chunks);
+  switch (p.rp) {
+    case 16: adapted_grad<16><<<grid, 256, 0, st>>>(d); break;
+    case 32: adapted_grad<32><<<grid, 256, 0, st>>>(d); break;
+    case 64: adapted_grad<64><<<grid, 256, 0, st>>>(d); break;
+    default: adapted_grad<128><<<grid, 256, 0, st>>>(d);
+  }
+  if (join) {
+    e.chunks = p.chunks;
+    e.rank = a.rank;
+    e.to_bf16 = a.grad_dtype == 0;
+    adapted_join<<<dim3((unsigned)counts), 256, 0, st>>>(e);
+  }
+}
+
+}  // namespace ffk

@@ -9,6 +9,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <algorithm>
 #include <map>
 #include <mutex>
 #include <string>
@@ -604,6 +605,171 @@ int32_t ffk_dropout_add(const void* x, const void* residual, void* out, const in
   a.dtype = dtype;
   launch_dropout(a, static_cast<hipStream_t>(stream));
   return check_launch("dropout_add");
+}
+
+namespace {
+
+// The workspace of a projection with adapters, into `a`; its size.
+size_t adapted_ws(void* ws, const AdaptedPlan& p, AdaptedArgs& a, int backward) {
+  Carver cv{static_cast<char*>(ws)};
+  a.ids = cv.take<int32_t>(a.rows);
+  if (p.few) {
+    a.few_u = cv.take<float>((size_t)a.rows * a.rank);
+    return cv.used;
+  }
+  const size_t mats = (size_t)a.adapters * a.rank;
+  if (p.pack_x) a.xp = cv.take<bf16>((size_t)a.rows * p.kp);
+  if (p.pack_down) a.down_hi = cv.take<bf16>(mats * p.kp);
+  if (!backward) {
+    if (p.pack_w) a.wp = cv.take<bf16>((size_t)a.d_out * p.kp);
+    if (p.pack_up) a.upp = cv.take<bf16>((size_t)a.adapters * a.d_out * p.rp);
+    a.u = cv.take<bf16>((size_t)a.rows * p.rp);
+    return cv.used;
+  }
+  if (p.pack_dy) a.dyp = cv.take<bf16>((size_t)a.rows * p.np);
+  a.wp = cv.take<bf16>((size_t)a.d_in * p.np);
+  a.down_t = cv.take<bf16>((size_t)a.adapters * a.d_in * p.rp);
+  a.up_hi = cv.take<bf16>(mats * p.np);
+  if (a.a_f32) {
+    a.down_lo = cv.take<bf16>(mats * p.kp);
+    a.up_lo = cv.take<bf16>(mats * p.np);
+  }
+  a.u = cv.take<bf16>((size_t)a.rows * 2 * p.rp);
+  a.v = cv.take<bf16>((size_t)a.rows * 2 * p.rp);
+  if (p.chunks > 1) {
+    a.part[0] = cv.take<float>(p.chunks * mats * a.d_in);
+    a.part[1] = cv.take<float>(p.chunks * mats * a.d_out);
+  }
+  return cv.used;
+}
+
+constexpr int kMostAdapted = 1 << 16;  // widths and adapters
+constexpr int kMostRank = 128;
+
+// (sizes that are in range; dtypes as FFK_DTYPE_*)
+bool adapted_sizes(int64_t rows, int32_t d_in, int32_t d_out, int32_t adapters, int32_t rank, int32_t requests) {
+  return rows >= 0 && rows <= 0x7fffffffLL && d_in > 0 && d_in <= kMostAdapted && d_out > 0 && d_out <= kMostAdapted &&
+         adapters > 0 && adapters < kMostAdapted && rank > 0 && rank <= kMostRank && requests >= 0 &&
+         (int64_t)adapters * rank * std::max(d_in, d_out) <= 0x7fffffffLL &&
+         ((rows + 63) / 64) * ((std::max(d_in, d_out) + 63) / 64) < (1 << 24);
+}
+
+int32_t adapted_check(const char* what, const AdaptedArgs& a, int32_t weight_dtype, int32_t adapter_dtype) {
+  if (!adapted_sizes(a.rows, a.d_in, a.d_out, a.adapters, a.rank, a.requests))
+    return fail(FFK_ERR_INVALID, "%s: rows=%lld d_in=%d d_out=%d adapters=%d rank=%d requests=%d (widths up to 65536, rank up to 128, fewer than 65536 adapters)", what, (long long)a.rows, a.d_in, a.d_out, a.adapters, a.rank, a.requests);
+  for (int32_t t : {weight_dtype, adapter_dtype})
+    if (t != FFK_DTYPE_BF16 && t != FFK_DTYPE_F32) return fail(FFK_ERR_INVALID, "%s: dtype=%d (bf16 or fp32)", what, t);
+  if (a.rows == 0) return FFK_OK;
+  if (!a.x || !a.w || !a.down || !a.up || !a.offsets || (a.requests > 0 && !a.adapter))
+    return fail(FFK_ERR_INVALID, "%s: null argument", what);
+  for (const void* t : {static_cast<const void*>(a.x), a.w, a.down, a.up, static_cast<const void*>(a.out)})
+    if (!aligned16(t)) return fail(FFK_ERR_INVALID, "%s: x, the weights and the output must be 16-byte aligned", what);
+  return FFK_OK;
+}
+
+}  // namespace
+
+size_t ffk_adapted_linear_workspace(int64_t rows, int32_t d_in, int32_t d_out, int32_t adapters, int32_t rank,
+                                    int32_t weight_dtype, int32_t adapter_dtype) {
+  if (!adapted_sizes(rows, d_in, d_out, adapters, rank, 0) || rows == 0) return 0;
+  AdaptedArgs a{};
+  a.rows = rows;
+  a.d_in = d_in;
+  a.d_out = d_out;
+  a.adapters = adapters;
+  a.rank = rank;
+  a.a_f32 = adapter_dtype == FFK_DTYPE_F32;
+  return adapted_ws(nullptr, adapted_plan(rows, d_in, d_out, adapters, rank, weight_dtype == FFK_DTYPE_F32, a.a_f32, 0),
+                    a, 0);
+}
+
+int32_t ffk_adapted_linear(const void* x, const void* weight, const float* bias, const void* down, const void* up,
+                           const float* scale, const int32_t* offsets, const int32_t* adapter, void* out, void* workspace,
+                           size_t workspace_bytes, int64_t rows, int32_t d_in, int32_t d_out, int32_t adapters,
+                           int32_t rank, int32_t requests, int32_t weight_dtype, int32_t adapter_dtype, void* stream) {
+  if (int32_t s = check_device()) return s;
+  AdaptedArgs a{};
+  a.x = static_cast<const bf16*>(x);
+  a.w = weight;
+  a.bias = bias;
+  a.down = down;
+  a.up = up;
+  a.scale = scale;
+  a.offsets = offsets;
+  a.adapter = adapter;
+  a.out = static_cast<bf16*>(out);
+  a.rows = rows;
+  a.d_in = d_in;
+  a.d_out = d_out;
+  a.adapters = adapters;
+  a.rank = rank;
+  a.requests = requests;
+  a.w_f32 = weight_dtype == FFK_DTYPE_F32;
+  a.a_f32 = adapter_dtype == FFK_DTYPE_F32;
+  if (int32_t s = adapted_check("adapted_linear", a, weight_dtype, adapter_dtype)) return s;
+  if (rows == 0) return ok();
+  if (!out) return fail(FFK_ERR_INVALID, "adapted_linear: null argument");
+  const AdaptedPlan p = adapted_plan(rows, d_in, d_out, adapters, rank, a.w_f32, a.a_f32, 0);
+  const size_t need = adapted_ws(workspace, p, a, 0);
+  if (!workspace || workspace_bytes < need || !aligned16(workspace))
+    return fail(FFK_ERR_WORKSPACE, "adapted_linear: workspace %zu bytes < %zu", workspace_bytes, need);
+  launch_adapted(a, p, static_cast<hipStream_t>(stream));
+  return check_launch("adapted_linear");
+}
+
+size_t ffk_adapted_linear_backward_workspace(int64_t rows, int32_t d_in, int32_t d_out, int32_t adapters, int32_t rank,
+                                             int32_t weight_dtype, int32_t adapter_dtype) {
+  if (!adapted_sizes(rows, d_in, d_out, adapters, rank, 0) || rows == 0) return 0;
+  AdaptedArgs a{};
+  a.rows = rows;
+  a.d_in = d_in;
+  a.d_out = d_out;
+  a.adapters = adapters;
+  a.rank = rank;
+  a.a_f32 = adapter_dtype == FFK_DTYPE_F32;
+  return adapted_ws(nullptr, adapted_plan(rows, d_in, d_out, adapters, rank, weight_dtype == FFK_DTYPE_F32, a.a_f32, 1),
+                    a, 1);
+}
+
+int32_t ffk_adapted_linear_backward(const void* dy, const void* x, const void* weight, const void* down, const void* up,
+                                    const float* scale, const int32_t* offsets, const int32_t* adapter, void* dx,
+                                    void* ddown, void* dup, void* workspace, size_t workspace_bytes, int64_t rows,
+                                    int32_t d_in, int32_t d_out, int32_t adapters, int32_t rank, int32_t requests,
+                                    int32_t weight_dtype, int32_t adapter_dtype, int32_t grad_dtype, void* stream) {
+  if (int32_t s = check_device()) return s;
+  AdaptedArgs a{};
+  a.x = static_cast<const bf16*>(x);
+  a.dy = static_cast<const bf16*>(dy);
+  a.w = weight;
+  a.down = down;
+  a.up = up;
+  a.scale = scale;
+  a.offsets = offsets;
+  a.adapter = adapter;
+  a.out = static_cast<bf16*>(dx);
+  a.ddown = ddown;
+  a.dup = dup;
+  a.rows = rows;
+  a.d_in = d_in;
+  a.d_out = d_out;
+  a.adapters = adapters;
+  a.rank = rank;
+  a.requests = requests;
+  a.w_f32 = weight_dtype == FFK_DTYPE_F32;
+  a.a_f32 = adapter_dtype == FFK_DTYPE_F32;
+  a.grad_dtype = grad_dtype;
+  if (int32_t s = adapted_check("adapted_linear_backward", a, weight_dtype, adapter_dtype)) return s;
+  if (grad_dtype != FFK_DTYPE_BF16 && grad_dtype != FFK_DTYPE_F32)
+    return fail(FFK_ERR_INVALID, "adapted_linear_backward: grad_dtype=%d (bf16 or fp32)", grad_dtype);
+  if (rows == 0) return fail(FFK_ERR_INVALID, "adapted_linear_backward: no rows (the gradients are zeros)");
+  if (!dy || !ddown || !dup || !aligned16(dy))
+    return fail(FFK_ERR_INVALID, "adapted_linear_backward: null argument, or dy off 16-byte alignment");
+  const AdaptedPlan p = adapted_plan(rows, d_in, d_out, adapters, rank, a.w_f32, a.a_f32, 1);
+  const size_t need = adapted_ws(workspace, p, a, 1);
+  if (!workspace || workspace_bytes < need || !aligned16(workspace))
+    return fail(FFK_ERR_WORKSPACE, "adapted_linear_backward: workspace %zu bytes < %zu", workspace_bytes, need);
+  launch_adapted_grad(a, p, static_cast<hipStream_t>(stream));
+  return check_launch("adapted_linear_backward");
 }
 
 size_t ffk_layer_norm_backward_workspace(int64_t rows, int32_t cols) {

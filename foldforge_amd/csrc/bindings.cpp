@@ -177,6 +177,10 @@ PyMethodDef methods[] = {
     FFK_CALL(ffk_quantize_activation),
     FFK_CALL(ffk_restore_activation),
     FFK_CALL(ffk_dropout_add),
+    FFK_CALL(ffk_adapted_linear_workspace),
+    FFK_CALL(ffk_adapted_linear),
+    FFK_CALL(ffk_adapted_linear_backward_workspace),
+    FFK_CALL(ffk_adapted_linear_backward),
     FFK_CALL(ffk_layer_norm_checkpoint),
     FFK_CALL(ffk_layer_norm_backward_workspace),
     FFK_CALL(ffk_layer_norm_backward),

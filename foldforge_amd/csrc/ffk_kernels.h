@@ -425,6 +425,37 @@ struct DropoutArgs {
 };
 void launch_dropout(const DropoutArgs& a, hipStream_t stream);
 
+// A projection with low-rank adapters of many requests (adapted.hip; rows > 0).
+struct AdaptedPlan {
+  int rp;            // rank rounded up to 16, 32, 64 or 128
+  int64_t kp, np;    // d_in and d_out rounded up to 64
+  int few;           // few rows: operands straight from the call's tensors
+  int pack_x, pack_dy, pack_w, pack_down, pack_up;  // which the products read from copies (backward: w and up always)
+  int64_t chunk;     // backward: rows of a workgroup's sums
+  int chunks;
+};
+AdaptedPlan adapted_plan(int64_t rows, int d_in, int d_out, int adapters, int rank, int w_f32, int a_f32, int backward);
+struct AdaptedArgs {
+  const bf16 *x, *dy;
+  const void *w, *down, *up;
+  const float *bias, *scale;          // either may be null
+  const int32_t *offsets, *adapter;
+  bf16* out;                          // y, or dx (may be null)
+  void *ddown, *dup;                  // grad_dtype
+  int64_t rows;
+  int d_in, d_out, adapters, rank, requests, w_f32, a_f32, grad_dtype;
+  // workspace (adapted_ws)
+  int32_t* ids;                       // [rows]
+  bf16 *xp, *dyp, *wp;                // padded copies of x, dy; w bf16 (backward: turned)
+  bf16 *down_hi, *down_lo, *down_t;   // [adapters][rank][kp] twice, [adapters][d_in][rp]
+  bf16 *upp, *up_hi, *up_lo;          // [adapters][d_out][rp], [adapters][rank][np] twice
+  bf16 *u, *v;                        // [rows][rp], backward [rows][2 rp]
+  float* few_u;                       // [rows][rank]
+  float* part[2];                     // [chunks][adapters][rank][d_in], .. [d_out]
+};
+void launch_adapted(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t stream);
+void launch_adapted_grad(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t stream);
+
 // Backward pass of the SwiGLU transition (rows > 0; d a multiple of 64 up to 768, hidden of 64).
 struct TransitionGradPlan {
   int64_t chunk;  // rows at once, a multiple of 64

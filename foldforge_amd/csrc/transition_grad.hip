@@ -35,51 +35,6 @@ __device__ __forceinline__ f32x16 mfma32h(f16x8 a, f16x8 b, f32x16 c) {
 }
 __device__ __forceinline__ f16x8 ld8h(const f16* p) { return *reinterpret_cast<const f16x8*>(p); }
 
-// A tile of 64-channel bf16 rows in LDS (128 bytes a row, 8 pieces of 16): piece p of row r lies at piece
-// p ^ swz64(r). Sixteen lanes that read one piece of sixteen consecutive rows (an operand fetch) fall on all
-// 64 banks. A transposing fetch is served in two halves, the wave's quarters 0 and 2, then 1 and 3 (seen in the conflict
-// counter): 4 rows' 32 bytes a quarter, rows 0-3 and 8-11 (or 4-7) together, which bit 2 ^ bit 3 keeps apart.
-__device__ __forceinline__ int swz64(int r) {
-  return ((r >> 1) & 1) << 2 | (((r >> 2) ^ (r >> 3)) & 1) << 1 | ((r >> 2) & 1);
-}
-__device__ __forceinline__ int off64(int r, int p) { return r * 64 + 8 * (p ^ swz64(r)); }
-
-// This wave's share of a 64 x 64 tile (rows row0 .. row0 + 63 of src, clamped to `last`, channels c0 .. c0 + 63)
-// into LDS at byte address dst: 8 rows an instruction. 4 waves.
-__device__ __forceinline__ void tile_dma(const void* src_, int64_t ld, int64_t row0, int64_t last, int c0, uint32_t dst,
-                                         int wave, int lane) {
-  const bf16* src = static_cast<const bf16*>(src_);  // (or fp16: 2 bytes a value)
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int r0 = 8 * (2 * wave + u), r = r0 + (lane >> 3);
-    const int64_t row = row0 + r < last ? row0 + r : last;
-    dma16_at(src + row * ld + c0 + 8 * ((lane & 7) ^ swz64(r)), dst + 128 * r0);
-  }
-}
-
-typedef short s16x4 __attribute__((__vector_size__(8)));
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-
-// MFMA operand of a tile whose rows are k: 32 channels from c0 (a multiple of 32), k0 .. k0 + 15. One
-// transposing read gives a lane one channel at four k: sixteen lanes take 4 rows x 16 channels (the lane's
-// address: row j / 4, channels 4 (j % 4) ..), lane j of them gets channel j. Lanes of half g hold k0 + 4 g + 0..3
-// and k0 + 8 + 4 g + 0..3: every operand read this way pairs the same k.
-__device__ __forceinline__ bf16x8 ld_turned(const bf16* tile, int c0, int k0, int lane) {
-  const int j = lane & 15, q = lane >> 4;
-  const int r = k0 + 4 * (q >> 1) + (j >> 2), c = c0 + 16 * (q & 1) + 4 * (j & 3);
-  const bf16* p0 = &tile[off64(r, c >> 3) + (c & 7)];
-  const bf16* p1 = &tile[off64(r + 8, c >> 3) + (c & 7)];
-  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p0));
-  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p1));
-  union {
-    s16x4 s[2];
-    bf16x8 v;
-  } o;
-  o.s[0] = lo;
-  o.s[1] = hi;
-  return o.v;
-}
-
 // k with peak 2^k in [2^14, 2^15); 0 for a peak of 0, at most 110 (2^-k and peak 2^k stay normal numbers).
 __device__ __forceinline__ int peak_power(float peak) {
   if (peak == 0.f) return 0;

@@ -462,6 +462,132 @@ def dropout_backward(dy: Tensor, *, p: float, seed: int | Tensor, offset: int = 
     return dropout_add(dy, p=p, seed=seed, offset=offset, shared=shared, out=out)
 
 
+#: the widest projection with adapters, its highest rank, and the first count of adapters that is too many
+MOST_ADAPTED_WIDTH, MOST_RANK, TOO_MANY_ADAPTERS = 65536, 128, 65536
+
+
+def adapted_linear_supported(d_in: int, d_out: int, rank: int, adapters: int = 1) -> bool:
+    """Sizes of the projections with low-rank adapters."""
+    return (0 < d_in <= MOST_ADAPTED_WIDTH and 0 < d_out <= MOST_ADAPTED_WIDTH and 0 < rank <= MOST_RANK
+            and 0 < adapters < TOO_MANY_ADAPTERS and adapters * rank * max(d_in, d_out) < 2**31)
+
+
+def _matrix(t: Tensor, name: str, dims: int, device: torch.device) -> int:
+    """The dtype code of a contiguous, aligned bf16 / fp32 weight on ``device``."""
+    if not (isinstance(t, Tensor) and t.dim() == dims):
+        _refuse(f"{name} must be a tensor of {dims} axes")
+    if t.device != device:
+        _refuse(f"{name} is on {t.device}, expected {device}")
+    if t.dtype not in (torch.bfloat16, torch.float32):
+        _refuse(f"{name} must be bf16 or fp32 (got {t.dtype})")
+    if not t.is_contiguous() or t.data_ptr() % 16:
+        _refuse(f"{name} must be contiguous and 16-byte aligned")
+    return _dtype_code(t.dtype)
+
+
+class _Adapted(NamedTuple):
+    rows: int
+    d_in: int
+    d_out: int
+    adapters: int
+    rank: int
+    requests: int
+    weight_dtype: int
+    adapter_dtype: int
+
+
+def _adapted(x: Tensor, weight: Tensor, down: Tensor, up: Tensor, scale: Tensor | None, offsets: Tensor,
+             adapter: Tensor) -> _Adapted:
+    """The sizes of a projection with adapters, its tensors checked (the C-ABI receives pointers)."""
+    rows, dev = _rows_tensor(x, "x"), x.device
+    if x.dtype != torch.bfloat16:
+        _refuse(f"x must be bf16 (got {x.dtype})")
+    codes = _matrix(weight, "weight", 2, dev), _matrix(down, "down", 3, dev), _matrix(up, "up", 3, dev)
+    d_out, d_in = weight.shape
+    n, rank = down.shape[:2]
+    if x.shape[-1] != d_in or down.shape[2] != d_in or tuple(up.shape) != (n, d_out, rank):
+        _refuse(f"x [.., d_in], weight [d_out, d_in], down [adapters, rank, d_in], up [adapters, d_out, rank] (got "
+                f"{tuple(x.shape)}, {tuple(weight.shape)}, {tuple(down.shape)}, {tuple(up.shape)})")
+    if codes[1] != codes[2]:
+        _refuse(f"down and up must be of one type (got {down.dtype} and {up.dtype})")
+    if not adapted_linear_supported(d_in, d_out, rank, n):
+        _refuse(f"d_in={d_in} d_out={d_out} rank={rank} adapters={n} (widths up to {MOST_ADAPTED_WIDTH}, rank up to "
+                f"{MOST_RANK}, fewer than {TOO_MANY_ADAPTERS} adapters)")
+    if scale is not None:
+        _affine(scale, x, "scale", n)
+        if not scale.is_contiguous():
+            _refuse("scale must be contiguous")
+    for t, name in ((offsets, "offsets"), (adapter, "adapter")):
+        if not (isinstance(t, Tensor) and t.dim() == 1 and t.dtype == torch.int32 and t.device == dev
+                and t.is_contiguous()):
+            _refuse(f"{name} must be a contiguous int32 tensor of one axis on {dev}")
+    if offsets.numel() != adapter.numel() + 1:
+        _refuse(f"offsets has {offsets.numel()} entries for {adapter.numel()} requests (one more than they)")
+    if rows >= 2**31:
+        _refuse(f"x has {rows} rows (fewer than 2^31)")
+    return _Adapted(rows, d_in, d_out, n, rank, adapter.numel(), codes[0], codes[1])
+
+
+def adapted_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, down: Tensor, up: Tensor,
+                   scale: Tensor | None = None, offsets: Tensor, adapter: Tensor, out: Tensor | None = None) -> Tensor:
+    """``x W^T + b + s_a (x A_a^T) B_a^T`` over the last axis of ``x [..., d_in]`` bf16: a projection and, beside it, the
+    low-rank adapter ``a`` of the request that a row belongs to. ``weight [d_out, d_in]`` bf16 or fp32, ``bias [d_out]``
+    fp32; ``down [adapters, rank, d_in]`` (A) and ``up [adapters, d_out, rank]`` (B) bf16 or fp32; ``scale [adapters]`` fp32
+    (None: 1). Request ``r`` has the rows ``offsets[r]`` to ``offsets[r + 1]`` of ``x`` (its leading axes flattened) and the
+    adapter ``adapter[r]`` (int32, on the device): one row each in a batch of single tokens, ``[0, N^2, 2 N^2, ...]`` for
+    pair tensors of several targets. Rows of no request, and requests whose adapter is none of them (-1), have the
+    projection alone. Output bf16 ``[..., d_out]``. Any widths; rank up to 128."""
+    q = _adapted(x, weight, down, up, scale, offsets, adapter)
+    if x.data_ptr() % 16:
+        _refuse("x must be 16-byte aligned")
+    bias = _affine(bias, x, "bias", q.d_out)
+    out = _output(out, (*x.shape[:-1], q.d_out), torch.bfloat16, x.device)
+    if out.data_ptr() % 16:
+        _refuse("out must be 16-byte aligned")
+    if q.rows:
+        ws = _workspace(_native.calls().ffk_adapted_linear_workspace(
+            q.rows, q.d_in, q.d_out, q.adapters, q.rank, q.weight_dtype, q.adapter_dtype), x.device)
+        _call(x.device, "adapted_linear", x, weight, bias, down, up, scale, offsets, adapter, out, ws, ws.numel(), *q)
+    return out
+
+
+class AdaptedGradients(NamedTuple):
+    """Gradients of :func:`adapted_linear`'s input and adapters (``x`` None where it was not asked for)."""
+
+    x: Tensor | None
+    down: Tensor
+    up: Tensor
+
+
+def adapted_linear_backward(dy: Tensor, x: Tensor, weight: Tensor, *, down: Tensor, up: Tensor,
+                            scale: Tensor | None = None, offsets: Tensor, adapter: Tensor, with_x: bool = True,
+                            grad_dtype: torch.dtype = torch.float32) -> AdaptedGradients:
+    """Gradients of :func:`adapted_linear` from the output's gradient ``dy [..., d_out]`` bf16 and its input: ``x`` in bf16
+    (``with_x=False``: not computed), ``down`` and ``up`` in ``grad_dtype``, sums over all rows of an adapter in fp32 and a
+    fixed order (zeros for an adapter without rows). The projection itself is frozen: ``weight`` and the bias have no
+    gradient here."""
+    q = _adapted(x, weight, down, up, scale, offsets, adapter)
+    if not (isinstance(dy, Tensor) and dy.dtype == torch.bfloat16 and dy.device == x.device and dy.is_contiguous()
+            and tuple(dy.shape) == (*x.shape[:-1], q.d_out)):
+        _refuse(f"dy must be a contiguous bf16 tensor {(*x.shape[:-1], q.d_out)} on {x.device}")
+    for t, name in ((dy, "dy"), (x, "x")):
+        if t.data_ptr() % 16:
+            _refuse(f"{name} must be 16-byte aligned")
+    code = _grad_dtype(grad_dtype)
+    if not q.rows:
+        return AdaptedGradients(torch.empty_like(x) if with_x else None, torch.zeros_like(down, dtype=grad_dtype),
+                                torch.zeros_like(up, dtype=grad_dtype))
+    lib = _native.calls()
+    size = lib.ffk_adapted_linear_backward_workspace(q.rows, q.d_in, q.d_out, q.adapters, q.rank, q.weight_dtype,
+                                                     q.adapter_dtype)
+    ws, ddown, dup, *dx = lib.empties(x, (((size,), _U8), (tuple(down.shape), code), (tuple(up.shape), code),
+                                          *(((tuple(x.shape), _BF16),) if with_x else ())))
+    dx = dx[0] if with_x else None
+    _call(x.device, "adapted_linear_backward", dy, x, weight, down, up, scale, offsets, adapter, dx, ddown, dup, ws,
+          ws.numel(), *q, code)
+    return AdaptedGradients(dx, ddown, dup)
+
+
 def triangle_multiplicative_update(
     z: Tensor,
     mask: Tensor,

@@ -122,6 +122,36 @@ int32_t ffk_dropout_add(const void* x, const void* residual, void* out, const in
                         void* stream);
 
 /*
+ * A projection with the low-rank adapters of many requests beside it:
+ *   out_t = W x_t + bias + s_a B_a (A_a x_t),   a = adapter[r] of the request r that row t belongs to.
+ * x [rows, d_in] bf16, out [rows, d_out] bf16; weight W [d_out, d_in] in weight_dtype, bias [d_out] fp32 or NULL; down A
+ * [adapters, rank, d_in] and up B [adapters, d_out, rank] in adapter_dtype (bf16 or fp32 each); scale s [adapters] fp32 or
+ * NULL (1). Request r has the rows offsets[r] .. offsets[r + 1] - 1 (offsets [requests + 1], not decreasing; none where they
+ * are the same); rows of no request, and requests whose adapter is not in [0, adapters), get W x + bias. Two requests may
+ * share an adapter. x, out, the weights: 16-byte aligned; rank up to 128, widths up to 65536. Products of bf16
+ * operands (fp32 ones are rounded), fp32 sums; the rows A x in fp32 up to 256 rows, in bf16 above.
+ */
+size_t ffk_adapted_linear_workspace(int64_t rows, int32_t d_in, int32_t d_out, int32_t adapters, int32_t rank,
+                                    int32_t weight_dtype, int32_t adapter_dtype);
+int32_t ffk_adapted_linear(const void* x, const void* weight, const float* bias, const void* down, const void* up,
+                           const float* scale, const int32_t* offsets, const int32_t* adapter, void* out, void* workspace,
+                           size_t workspace_bytes, int64_t rows, int32_t d_in, int32_t d_out, int32_t adapters,
+                           int32_t rank, int32_t requests, int32_t weight_dtype, int32_t adapter_dtype, void* stream);
+
+/*
+ * The gradients of ffk_adapted_linear at the output's gradient dy [rows, d_out] bf16, rows > 0: dx [rows, d_in] bf16 (NULL:
+ * not wanted; may not be dy or x), ddown and dup like down and up in grad_dtype, each the sum over all rows of its adapter in
+ * fp32 and a fixed order (zeros for an adapter without rows). W and bias are frozen: no gradient.
+ */
+size_t ffk_adapted_linear_backward_workspace(int64_t rows, int32_t d_in, int32_t d_out, int32_t adapters, int32_t rank,
+                                             int32_t weight_dtype, int32_t adapter_dtype);
+int32_t ffk_adapted_linear_backward(const void* dy, const void* x, const void* weight, const void* down, const void* up,
+                                    const float* scale, const int32_t* offsets, const int32_t* adapter, void* dx,
+                                    void* ddown, void* dup, void* workspace, size_t workspace_bytes, int64_t rows,
+                                    int32_t d_in, int32_t d_out, int32_t adapters, int32_t rank, int32_t requests,
+                                    int32_t weight_dtype, int32_t adapter_dtype, int32_t grad_dtype, void* stream);
+
+/*
  * ffk_layer_norm that keeps its input as an 8-bit activation in the same pass (y may not alias x).
  */
 int32_t ffk_layer_norm_checkpoint(const void* x, const float* weight, const float* bias, void* y,

@@ -121,3 +121,41 @@ def dropout_add(update: Tensor, residual: Tensor | None, shared: int | None, p: 
     keep = dropout_mask(update.shape, shared, p, seed, offset)
     y = torch.where(keep, update.double() * 65536 / max(65536 - drop, 1), 0.0)
     return y if residual is None else residual.double() + y
+
+
+def adapter_of_rows(rows: int, offsets: Tensor, adapter: Tensor, adapters: int) -> Tensor:
+    """Each row's adapter, -1 for none."""
+    of = torch.full((rows,), -1, dtype=torch.long)
+    ends = offsets.tolist()
+    for lo, hi, a in zip(ends, ends[1:], adapter.tolist()):
+        if 0 <= a < adapters:
+            of[lo:hi] = a
+    return of
+
+
+def adapted_linear(x: Tensor, weight: Tensor, bias: Tensor | None, down: Tensor, up: Tensor, scale: Tensor | None,
+                   of: Tensor) -> Tensor:
+    """``[rows, d_out]`` of ``x [rows, d_in]`` whose rows have the adapters ``of``."""
+    x, y = x.double(), x.double() @ weight.double().T
+    if bias is not None:
+        y = y + bias.double()
+    for a in set(of.tolist()) - {-1}:
+        s = 1.0 if scale is None else scale[a].double()
+        y[of == a] += s * (x[of == a] @ down[a].double().T) @ up[a].double().T
+    return y
+
+
+def adapted_linear_backward(dy: Tensor, x: Tensor, weight: Tensor, down: Tensor, up: Tensor, scale: Tensor | None,
+                            of: Tensor) -> tuple[Tensor, Tensor, Tensor]:
+    """``(dx, d_down, d_up)``."""
+    dy, x = dy.double(), x.double()
+    dx = dy @ weight.double()
+    ddown, dup = torch.zeros_like(down, dtype=torch.float64), torch.zeros_like(up, dtype=torch.float64)
+    for a in set(of.tolist()) - {-1}:
+        at = of == a
+        s = 1.0 if scale is None else scale[a].double()
+        v = s * dy[at] @ up[a].double()
+        dx[at] += v @ down[a].double()
+        ddown[a] = v.T @ x[at]
+        dup[a] = s * dy[at].T @ (x[at] @ down[a].double().T)
+    return dx, ddown, dup
