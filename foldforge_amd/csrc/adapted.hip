@@ -6,13 +6,14 @@
 // request, and requests whose adapter is none of them, have W and b alone). W is frozen: no gradient.
 //
 // The thin products (u, v: d x rank) go first, into rows of rank numbers; the wide product then takes them as rank more
-// channels of the same sum, so its rows are read and written once. Operands of the products are bf16, sums fp32. For the
-// adapters' gradients, which are sums over up to 10^5 rows in fp32, u and v are kept as two bf16 (high and low part: 16 bits)
-// and fp32 adapters enter as two as well: off by some 2^-17 of the terms. The forward pass keeps the high parts, whose
-// rounding is that of its output.
+// channels of the same sum, so its rows are read and written once. Operands of the products are bf16, sums fp32. The
+// adapters' gradients are fp32: u and v are kept as three bf16 that add up to the fp32 value, and fp32 adapters enter as
+// three (the products of a bf16 pair are exact in fp32, three of them cost little beside the rows' way from memory). The
+// outputs, bf16 themselves, take the rounded u and v and rounded weights.
 // Rows of other adapters are left out by selection, not by factors of zero: infinities and NaN of one request (or of one
 // adapter's weights) reach no other's rows or gradients.
 #include <algorithm>
+#include <type_traits>
 
 #include "ffk_device.h"
 #include "ffk_kernels.h"
@@ -72,11 +73,11 @@ __device__ __forceinline__ float scale_of(const Requests& q, int a) { return q.s
 // ---------------------------------------------------------------------------------------------------------
 // operands in the products' orders
 
-// dst [batch][out_rows][out_cols] bf16 (and what its rounding left, in lo) from src [batch][rows][cols] (turn: transposed),
-// zeros outside.
+// dst [batch][out_rows][out_cols] bf16 from src [batch][rows][cols] (turn: transposed), zeros outside; with mid and lo in
+// three parts that add up to the fp32 value.
 struct PackJob {
   const void* src;
-  bf16 *hi, *lo;  // lo may be null
+  bf16 *hi, *mid, *lo;  // mid and lo may be null
   int64_t rows, cols, out_rows, out_cols, tiles;  // tiles: of 32 x 32, all batches
   int f32, turn;
 };
@@ -117,7 +118,12 @@ __global__ __launch_bounds__(256) void adapted_pack(const PackArgs p, int64_t ti
       const int64_t to = (batch * j.out_rows + r) * j.out_cols + c;
       const bf16 h = (bf16)v;
       j.hi[to] = h;
-      if (j.lo) j.lo[to] = (bf16)(v - (float)h);
+      if (j.mid) {
+        const float left = v - (float)h;
+        const bf16 m = (bf16)left;
+        j.mid[to] = m;
+        j.lo[to] = (bf16)(left - (float)m);
+      }
     }
     __syncthreads();
   }
@@ -126,24 +132,28 @@ __global__ __launch_bounds__(256) void adapted_pack(const PackArgs p, int64_t ti
 // ---------------------------------------------------------------------------------------------------------
 // the thin products
 
+// Channels of a row of u or v that keeps its parts: RP each of the high, middle and low ones (RP = 16: and of zeros), then none.
+constexpr int parts_ld(int rp) { return rp == 16 ? 64 : rp == 32 ? 128 : 3 * rp; }
+
 struct ThinJob {
-  const bf16 *x, *hi, *lo;  // x [rows][K], the adapters' matrices [adapters][mat_rows][K] (lo: their low parts, or null)
-  bf16* u;                  // [rows][ld]: s_a (matrix x) in RP channels, zeros from `rank` on; behind them the low parts
-  int K, mat_rows;          // K a multiple of 64
+  const bf16 *x, *mat[3];  // x [rows][K], the adapters' matrices [adapters][mat_rows][K] (PARTS = 3: in three parts)
+  bf16* u;                 // [rows][ld]: s_a (matrix x) in RP channels, zeros from `rank` on
+  int K, mat_rows;         // K a multiple of 64
 };
 struct ThinArgs {
   ThinJob job[2];
   Requests q;
   int32_t* ids;  // [rows], written by the first job's first workgroups
-  int rank, ld;
+  int rank;
 };
 
 // 64 / KS rows a workgroup, of 4 waves: KS = 1, 16 rows a wave; KS = 4, all 16 rows, a quarter of K a wave (few rows: more
 // workgroups). Each adapter of the rows in turn, gridDim.y workgroups share them; a lane holds a token and 4 channels.
-// grid (ceil(rows / (64 / KS)), share, jobs); block 256. LO: the adapters have low parts. OUT2: u keeps its own.
-template <int RP, bool LO, bool OUT2, int KS>
+// grid (ceil(rows / (64 / KS)), share, jobs); block 256. KEEP: u in three parts (rows of parts_ld), else rounded (of RP).
+template <int RP, int PARTS, bool KEEP, int KS>
 __global__ __launch_bounds__(256) void adapted_thin(const ThinArgs p) {
-  constexpr int N = RP / 16, TM = 64 / KS;
+  constexpr int N = RP / 16, TM = 64 / KS, U = N * PARTS <= 3 ? 4 : N * PARTS <= 6 ? 2 : 1;  // steps of k in flight
+  constexpr int ld = KEEP ? parts_ld(RP) : RP;
   __shared__ int id[64], start[64], before;
   __shared__ f32x4 red[KS == 1 ? 1 : 4][N][64];
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
@@ -158,16 +168,26 @@ __global__ __launch_bounds__(256) void adapted_thin(const ThinArgs p) {
   const int mine = id[first + i];
   const bf16* x = j.x + (row < p.q.rows ? row : p.q.rows - 1) * j.K + 8 * g;
   auto store = [&](int n, const f32x4& v) __attribute__((always_inline)) {
-    bf16x4 h, l;
+    bf16x4 part[3];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float t = 16 * n + 4 * g + e < p.rank ? v[e] : 0.f;
-      h[e] = (bf16)t;
-      l[e] = (bf16)(t - (float)h[e]);
+      float t = 16 * n + 4 * g + e < p.rank ? v[e] : 0.f;
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        part[k][e] = (bf16)t;
+        t -= (float)part[k][e];
+      }
     }
-    bf16* to = j.u + row * p.ld + 16 * n + 4 * g;
-    *reinterpret_cast<bf16x4*>(to) = h;
-    if constexpr (OUT2) *reinterpret_cast<bf16x4*>(to + RP) = l;
+    bf16* to = j.u + row * ld + 16 * n + 4 * g;
+    *reinterpret_cast<bf16x4*>(to) = part[0];
+    if constexpr (KEEP) {
+      *reinterpret_cast<bf16x4*>(to + RP) = part[1];
+      *reinterpret_cast<bf16x4*>(to + 2 * RP) = part[2];
+      if constexpr (RP == 16) {
+        const bf16x4 z = {(bf16)0.f, (bf16)0.f, (bf16)0.f, (bf16)0.f};
+        *reinterpret_cast<bf16x4*>(to + 3 * RP) = z;
+      }
+    }
   };
   const f32x4 none = {0.f, 0.f, 0.f, 0.f};
   if (blockIdx.y == 0 && mine < 0 && row < p.q.rows && (KS == 1 || wave == 0)) {
@@ -183,22 +203,35 @@ __global__ __launch_bounds__(256) void adapted_thin(const ThinArgs p) {
     f32x4 acc[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) acc[n] = none;
-    const bf16* m[N];
+    const bf16* m[PARTS][N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int r = 16 * n + i < j.mat_rows ? 16 * n + i : j.mat_rows - 1;
-      m[n] = j.hi + ((int64_t)a * j.mat_rows + r) * j.K + 8 * g;
-    }
-    const int64_t low = LO ? j.lo - j.hi : 0;
-#pragma unroll 4
-    for (int k = KS == 1 ? 0 : 32 * wave; k < j.K; k += 32 * KS) {
-      const bf16x8 xf = ld8(x + k);
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
-        acc[n] = mfma16(ld8(m[n] + k), xf, acc[n]);
-        if constexpr (LO) acc[n] = mfma16(ld8(m[n] + k + low), xf, acc[n]);
-      }
+      for (int k = 0; k < PARTS; ++k) m[k][n] = j.mat[k] + ((int64_t)a * j.mat_rows + r) * j.K + 8 * g;
     }
+    const auto steps = [&](int k, auto count) __attribute__((always_inline)) {
+      constexpr int C = decltype(count)::value;
+      bf16x8 xf[C], mf[C][PARTS][N];
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        xf[c] = ld8(x + k + 32 * KS * c);
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q)
+#pragma unroll
+          for (int n = 0; n < N; ++n) mf[c][q][n] = ld8(m[q][n] + k + 32 * KS * c);
+      }
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q)
+#pragma unroll
+          for (int n = 0; n < N; ++n) acc[n] = mfma16(mf[c][q][n], xf[c], acc[n]);
+    };
+    int k = KS == 1 ? 0 : 32 * wave;
+    for (; k + 32 * KS * (U - 1) < j.K; k += 32 * KS * U) steps(k, std::integral_constant<int, U>());
+    if constexpr (U > 1)
+      for (; k < j.K; k += 32 * KS) steps(k, std::integral_constant<int, 1>());
     const float s = scale_of(p.q, a);
     if constexpr (KS == 1) {
       if (is) {
@@ -349,7 +382,7 @@ __global__ __launch_bounds__(256, 2) void adapted_product(const ProductArgs p) {
 // the adapters' gradients
 
 struct GradJob {
-  const bf16 *x, *v;       // [rows][ld_x] (ld_x a multiple of 64), [rows][2 RP]: high and low parts
+  const bf16 *x, *v;       // [rows][ld_x] (ld_x a multiple of 64), [rows][parts_ld]
   void* to;                // element (chunk, a, channel j, column c) at chunk * chunk_stride + (a * rank) * cols + j * sj + c * sc
   int64_t sj, sc;
   int cols, ld_x, tiles;   // tiles = ld_x / 64
@@ -365,11 +398,12 @@ constexpr int kMostGradTiles = 256;
 // sum over a chunk's rows of adapter blockIdx.y of v x^T: RP channels x 64 columns a workgroup. Tiles of 64 rows that have a
 // row of the adapter's, in order, through three buffers by LDS DMA; the rows of others in them are zeroed there. A wave takes
 // 16 of a tile's rows (k of the product; both operands turned as they are read), the waves' sums meet at the end in a fixed
-// order. RP = 16: the high and low channels are the 32 rows of one product, else two products. grid (both jobs' tiles,
-// adapters, chunks); block 256.
+// order. The parts are products of their own into one sum (RP = 16: high and middle ones the 32 rows of one, low ones and
+// zeros of another). grid (both jobs' tiles, adapters, chunks); block 256.
 template <int RP>
 __global__ __launch_bounds__(256) void adapted_grad(const GradArgs p) {
-  constexpr int VT = RP <= 32 ? 1 : RP / 32, JB = RP <= 32 ? 1 : RP / 32, STAGES = 3, PER = 2 * (1 + VT);
+  constexpr int ld = parts_ld(RP), VT = ld / 64, JB = RP <= 32 ? 1 : RP / 32, BLOCKS = RP == 16 ? 2 : 3 * RP / 32;
+  constexpr int STAGES = RP == 128 ? 2 : 3, PER = 2 * (1 + VT);
   __shared__ __attribute__((aligned(16))) bf16 buf[STAGES][1 + VT][64 * 64];
   __shared__ uint64_t has[kMostGradTiles];  // which rows of a tile are the adapter's
   __shared__ int list[kMostGradTiles], listed;
@@ -403,17 +437,8 @@ __global__ __launch_bounds__(256) void adapted_grad(const GradArgs p) {
     const uint32_t at = lds + step % STAGES * (1 + VT) * 8192;
     const int64_t row0 = begin + 64 * list[step];
     tile_dma(j.x, j.ld_x, row0, p.rows - 1, c0, at, wave, lane);
-    if constexpr (RP == 16) {  // rows of 32 channels in tiles of 64: the pieces twice
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int r0 = 8 * (2 * wave + u), r = r0 + (lane >> 3);
-        const int64_t row = row0 + r < p.rows ? row0 + r : p.rows - 1;
-        dma16_at(j.v + row * 32 + 8 * (((lane & 7) ^ swz64(r)) & 3), at + 8192 + 128 * r0);
-      }
-    } else {
-#pragma unroll
-      for (int t = 0; t < VT; ++t) tile_dma(j.v, 2 * RP, row0, p.rows - 1, 64 * t, at + 8192 * (1 + t), wave, lane);
-    }
+    for (int t = 0; t < VT; ++t) tile_dma(j.v, ld, row0, p.rows - 1, 64 * t, at + 8192 * (1 + t), wave, lane);
   };
   f32x16 acc[JB][2];
 #pragma unroll
@@ -442,7 +467,7 @@ __global__ __launch_bounds__(256) void adapted_grad(const GradArgs p) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) x[h] = ld_turned(t[0], 32 * h, 16 * wave, lane);
 #pragma unroll
-    for (int b = 0; b < (RP == 16 ? 1 : 2 * JB); ++b) {  // 32 channels each: the high parts, then the low ones
+    for (int b = 0; b < BLOCKS; ++b) {  // 32 channels each: the high parts, the middle, the low ones
       const bf16x8 v = ld_turned(t[1 + b / 2], 32 * (b & 1), 16 * wave, lane);
 #pragma unroll
       for (int h = 0; h < 2; ++h) acc[b % JB][h] = mfma32(v, x[h], acc[b % JB][h]);
@@ -510,18 +535,32 @@ __global__ __launch_bounds__(256) void adapted_join(const JoinArgs p) {
 // ---------------------------------------------------------------------------------------------------------
 // few rows
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int64_t left, float (&v)[8]) {
+// Eight values at p[k ..], those from n on read as zeros. EVEN: n a multiple of 8 (the values lie in one 16- or 32-byte
+// piece or none do): no branch, so that loads can run ahead of each other.
+template <typename T, bool EVEN>
+struct Raw8 {
   typedef T vec __attribute__((__vector_size__(8 * sizeof(T)), aligned(sizeof(T))));
-  if (left >= 8) {
-    const vec t = *reinterpret_cast<const vec*>(p);
+  vec v;
+  bool in;
+  __device__ __forceinline__ void load(const T* p, int k, int n) {
+    in = k < n;
+    if constexpr (EVEN) {
+      v = *reinterpret_cast<const vec*>(p + (in ? k : 0));
+    } else if (k + 8 <= n) {
+      v = *reinterpret_cast<const vec*>(p + k);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (float)t[e];
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e < left ? (float)p[e] : 0.f;
+      for (int e = 0; e < 8; ++e) v[e] = k + e < n ? p[k + e] : (T)0.f;
+    }
   }
-}
+  __device__ __forceinline__ float operator[](int e) const { return in ? (float)v[e] : 0.f; }
+  __device__ __forceinline__ bf16x8 operand() const {
+    bf16x8 o;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = in ? (bf16)(float)v[e] : (bf16)0.f;
+    return o;
+  }
+};
 
 struct FewArgs {
   const bf16* x;
@@ -534,47 +573,59 @@ struct FewArgs {
   int K, N, rank;
 };
 
-// u of one row a workgroup in fp32, four channels a wave at a time, k across the lanes. grid rows; block 256.
-template <typename TA>
-__global__ __launch_bounds__(256) void adapted_few_thin(const FewArgs p) {
+// u of one row a workgroup in fp32, two channels a wave at a time, k across the lanes. grid rows; block 512.
+template <typename TA, bool EVEN>
+__global__ __launch_bounds__(512) void adapted_few_thin(const FewArgs p) {
   __shared__ int id[64], start[64], before;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t row = blockIdx.x;
-  tile_ids<256>(p.q, row, id, start, &before);
+  tile_ids<512>(p.q, row, id, start, &before);
   const int a = id[0];
   if (threadIdx.x == 0) p.ids[row] = a;
   if (a < 0) return;
   const TA* m = static_cast<const TA*>(p.down) + (int64_t)a * p.rank * p.K;
   const float s = scale_of(p.q, a);
-  for (int j0 = 4 * wave; j0 < p.rank; j0 += 16) {
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 8 * lane; k < p.K; k += 512) {
-      float x[8];
-      load8(p.x + row * p.K + k, p.K - k, x);
+  for (int j0 = 2 * wave; j0 < p.rank; j0 += 16) {
+    const TA* mj[2] = {m + (int64_t)j0 * p.K, m + (int64_t)(j0 + 1 < p.rank ? j0 + 1 : j0) * p.K};
+    float sum[2] = {0.f, 0.f};
+    for (int k = 8 * lane; k < p.K; k += 1024) {
+      Raw8<bf16, EVEN> x[2];
+      Raw8<TA, EVEN> v[2][2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float v[8];
-        load8(m + (int64_t)(j0 + j < p.rank ? j0 + j : p.rank - 1) * p.K + k, p.K - k, v);
+      for (int c = 0; c < 2; ++c) {
+        x[c].load(p.x + row * p.K, k + 512 * c, p.K);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum[j] += x[e] * v[e];
+        for (int j = 0; j < 2; ++j) v[c][j].load(mj[j], k + 512 * c, p.K);
       }
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum[j] += x[c][e] * v[c][j][e];
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 2; ++j) {
       const float v = lanes_sum<64>(sum[j]);
       if (lane == 0 && j0 + j < p.rank) p.u[row * p.rank + j0 + j] = s * v;
     }
   }
 }
 
-// 16 channels x 16 RT rows a workgroup, a quarter of k a wave, operands straight from memory; the adapters as dot products of
-// rank terms, a thread for each output. grid (ceil(N / 16), ceil(rows / (16 RT))); block 256.
-template <typename TW, typename TA, int RT>
-__global__ __launch_bounds__(256) void adapted_few(const FewArgs p) {
-  __shared__ float red[4][RT][16][20];  // [wave][..][token][channel], rows of 20: 16-byte stores without conflicts
-  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
+// 16 channels x 16 RT rows a workgroup, an eighth of k a wave, operands straight from memory; the adapters as dot products of
+// rank terms, a thread for each output. grid (ceil(N / 16), ceil(rows / (16 RT))); block 512.
+template <typename TW, typename TA, int RT, bool EVEN>
+__global__ __launch_bounds__(512) void adapted_few(const FewArgs p) {
+  __shared__ float red[8][RT][16][20];  // [wave][..][token][channel], rows of 20: 16-byte stores without conflicts
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n0 = 16 * blockIdx.x;
   const int64_t row0 = 16 * RT * (int64_t)blockIdx.y;
+  // the output of this thread
+  const int part = threadIdx.x >> 8, token = (threadIdx.x >> 4) & 15, c = threadIdx.x & 15, n = n0 + c;
+  const int64_t row = row0 + 16 * part + token;
+  const bool mine = part < RT && row < p.q.rows && n < p.N;
+  const int a = mine ? p.ids[row] : -1;
   f32x4 acc[RT];
 #pragma unroll
   for (int t = 0; t < RT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -582,68 +633,63 @@ __global__ __launch_bounds__(256) void adapted_few(const FewArgs p) {
   const bf16* x[RT];
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
-    const int64_t row = row0 + 16 * t + i;
-    x[t] = p.x + (row < p.q.rows ? row : p.q.rows - 1) * p.K;
+    const int64_t r = row0 + 16 * t + i;
+    x[t] = p.x + (r < p.q.rows ? r : p.q.rows - 1) * p.K;
   }
-#pragma unroll 2
-  for (int k = 32 * wave + 8 * g; k - 8 * g < p.K; k += 128) {
-    float v[8];
-    load8(w + k, p.K - k, v);
-    bf16x8 wf;
+  constexpr int U = 3;
+  for (int k = 32 * wave; k < p.K; k += 256 * U) {
+    Raw8<TW, EVEN> wf[U];
+    Raw8<bf16, EVEN> xf[U][RT];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) wf[e] = (bf16)v[e];
+    for (int u = 0; u < U; ++u) {
+      wf[u].load(w, k + 256 * u + 8 * g, p.K);
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      load8(x[t] + k, p.K - k, v);
-      bf16x8 xf;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) xf[e] = (bf16)v[e];
-      acc[t] = mfma16(wf, xf, acc[t]);
+      for (int t = 0; t < RT; ++t) xf[u][t].load(x[t], k + 256 * u + 8 * g, p.K);
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int t = 0; t < RT; ++t) acc[t] = mfma16(wf[u].operand(), xf[u][t].operand(), acc[t]);
   }
 #pragma unroll
   for (int t = 0; t < RT; ++t) *reinterpret_cast<f32x4*>(&red[wave][t][i][4 * g]) = acc[t];
-  __syncthreads();
-  const int token = threadIdx.x >> 4, c = threadIdx.x & 15, n = n0 + c;
-  if (n >= p.N) return;
+  float sum = mine && p.bias ? p.bias[n] : 0.f;
+  if (a >= 0) {
+    const TA* b = static_cast<const TA*>(p.up) + ((int64_t)a * p.N + n) * p.rank;
+    const float* u = p.u + row * p.rank;
+    for (int j = 0; j < p.rank; j += 8) {
+      Raw8<TA, false> v;
+      Raw8<float, false> q;
+      v.load(b, j, p.rank);
+      q.load(u, j, p.rank);
 #pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    const int64_t row = row0 + 16 * t + token;
-    if (row >= p.q.rows) return;
-    float y = (red[0][t][token][c] + red[1][t][token][c]) + (red[2][t][token][c] + red[3][t][token][c]);
-    if (p.bias) y += p.bias[n];
-    const int a = p.ids[row];
-    if (a >= 0) {
-      const TA* b = static_cast<const TA*>(p.up) + ((int64_t)a * p.N + n) * p.rank;
-      const float* u = p.u + row * p.rank;
-      float sum = 0.f;
-      for (int j = 0; j < p.rank; j += 8) {
-        float v[8], q[8];
-        load8(b + j, p.rank - j, v);
-        load8(u + j, p.rank - j, q);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum += v[e] * q[e];
-      }
-      y += sum;
+      for (int e = 0; e < 8; ++e) sum += v[e] * q[e];
     }
-    p.out[row * p.N + n] = (bf16)y;
   }
+  __syncthreads();
+  if (!mine) return;
+  float y = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) y += red[k][part][token][c];
+  p.out[row * p.N + n] = (bf16)(y + sum);
 }
 
 // ---------------------------------------------------------------------------------------------------------
 // launches
 
-template <typename TW, typename TA>
+template <typename TW, typename TA, bool EVEN>
 void launch_few(const FewArgs& f, hipStream_t st) {
   const int64_t rows = f.q.rows;
-  adapted_few_thin<TA><<<dim3((unsigned)rows), 256, 0, st>>>(f);
+  adapted_few_thin<TA, EVEN><<<dim3((unsigned)rows), 512, 0, st>>>(f);
   const unsigned across = (unsigned)((f.N + 15) / 16);
   if (rows <= 16)
-    adapted_few<TW, TA, 1><<<dim3(across), 256, 0, st>>>(f);
-  else if (rows <= 32)
-    adapted_few<TW, TA, 2><<<dim3(across), 256, 0, st>>>(f);
+    adapted_few<TW, TA, 1, EVEN><<<dim3(across), 512, 0, st>>>(f);
   else
-    adapted_few<TW, TA, 4><<<dim3(across, (unsigned)((rows + 63) / 64)), 256, 0, st>>>(f);
+    adapted_few<TW, TA, 2, EVEN><<<dim3(across, (unsigned)((rows + 31) / 32)), 512, 0, st>>>(f);
+}
+template <typename TW, typename TA>
+void launch_few(const FewArgs& f, hipStream_t st) {
+  f.K % 8 == 0 ? launch_few<TW, TA, true>(f, st) : launch_few<TW, TA, false>(f, st);
 }
 
 int64_t tiles32(int64_t batch, int64_t rows, int64_t cols) { return batch * ((rows + 31) / 32) * ((cols + 31) / 32); }
@@ -651,11 +697,12 @@ int64_t tiles32(int64_t batch, int64_t rows, int64_t cols) { return batch * ((ro
 struct Packer {
   PackArgs args{};
   int64_t tiles = 0;
-  void add(const void* src, int f32, bf16* hi, bf16* lo, int64_t batch, int64_t rows, int64_t cols, int64_t out_rows,
+  void add(const void* src, int f32, bf16* hi, bf16* mid, bf16* lo, int64_t batch, int64_t rows, int64_t cols, int64_t out_rows,
            int64_t out_cols, bool turn) {
     PackJob j;
     j.src = src;
     j.hi = hi;
+    j.mid = mid;
     j.lo = lo;
     j.rows = rows;
     j.cols = cols;
@@ -672,7 +719,7 @@ struct Packer {
   }
 };
 
-template <bool LO, bool OUT2>
+template <int PARTS, bool KEEP>
 void launch_thin(const ThinArgs& a, int rp, int jobs, hipStream_t st) {
   const int64_t rows = a.q.rows;
   // few rows: a quarter of k a wave, so that the chip is filled, and the adapters of 16 rows shared out where they may be many
@@ -682,9 +729,9 @@ void launch_thin(const ThinArgs& a, int rp, int jobs, hipStream_t st) {
 #define FFK_THIN(RP)                                      \
   if (rp == RP) {                                         \
     if (split)                                            \
-      adapted_thin<RP, LO, OUT2, 4><<<grid, 256, 0, st>>>(a); \
+      adapted_thin<RP, PARTS, KEEP, 4><<<grid, 256, 0, st>>>(a); \
     else                                                  \
-      adapted_thin<RP, LO, OUT2, 1><<<grid, 256, 0, st>>>(a); \
+      adapted_thin<RP, PARTS, KEEP, 1><<<grid, 256, 0, st>>>(a); \
   }
   FFK_THIN(16)
   FFK_THIN(32)
@@ -722,6 +769,7 @@ Requests requests_of(const AdaptedArgs& a) {
 AdaptedPlan adapted_plan(int64_t rows, int d_in, int d_out, int adapters, int rank, int w_f32, int a_f32, int backward) {
   AdaptedPlan p{};
   p.rp = rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128;
+  p.ld = backward ? parts_ld(p.rp) : p.rp;
   p.kp = up64(d_in);
   p.np = up64(d_out);
   p.few = !backward && rows <= 256;
@@ -766,22 +814,21 @@ void launch_adapted(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t st) 
     return;
   }
   Packer pack;
-  if (p.pack_x) pack.add(a.x, 0, a.xp, nullptr, 1, a.rows, a.d_in, a.rows, p.kp, false);
-  if (p.pack_w) pack.add(a.w, a.w_f32, a.wp, nullptr, 1, a.d_out, a.d_in, a.d_out, p.kp, false);
-  if (p.pack_down) pack.add(a.down, a.a_f32, a.down_hi, nullptr, a.adapters, a.rank, a.d_in, a.rank, p.kp, false);
-  if (p.pack_up) pack.add(a.up, a.a_f32, a.upp, nullptr, a.adapters, a.d_out, a.rank, a.d_out, p.rp, false);
+  if (p.pack_x) pack.add(a.x, 0, a.xp, nullptr, nullptr, 1, a.rows, a.d_in, a.rows, p.kp, false);
+  if (p.pack_w) pack.add(a.w, a.w_f32, a.wp, nullptr, nullptr, 1, a.d_out, a.d_in, a.d_out, p.kp, false);
+  if (p.pack_down) pack.add(a.down, a.a_f32, a.down_hi, nullptr, nullptr, a.adapters, a.rank, a.d_in, a.rank, p.kp, false);
+  if (p.pack_up) pack.add(a.up, a.a_f32, a.upp, nullptr, nullptr, a.adapters, a.d_out, a.rank, a.d_out, p.rp, false);
   pack.launch(st);
   ThinArgs t{};
   t.job[0].x = p.pack_x ? a.xp : a.x;
-  t.job[0].hi = p.pack_down ? a.down_hi : static_cast<const bf16*>(a.down);
+  t.job[0].mat[0] = p.pack_down ? a.down_hi : static_cast<const bf16*>(a.down);
   t.job[0].u = a.u;
   t.job[0].K = p.kp;
   t.job[0].mat_rows = a.rank;
   t.q = q;
   t.ids = a.ids;
   t.rank = a.rank;
-  t.ld = p.rp;
-  launch_thin<false, false>(t, p.rp, 1, st);
+  launch_thin<1, false>(t, p.rp, 1, st);
   ProductArgs g{};
   g.x = t.job[0].x;
   g.w = p.pack_w ? a.wp : static_cast<const bf16*>(a.w);
@@ -800,31 +847,32 @@ void launch_adapted(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t st) 
 
 void launch_adapted_grad(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t st) {
   Packer pack;
-  if (p.pack_x) pack.add(a.x, 0, a.xp, nullptr, 1, a.rows, a.d_in, a.rows, p.kp, false);
-  if (p.pack_dy) pack.add(a.dy, 0, a.dyp, nullptr, 1, a.rows, a.d_out, a.rows, p.np, false);
-  if (a.out) pack.add(a.w, a.w_f32, a.wp, nullptr, 1, a.d_out, a.d_in, a.d_in, p.np, true);
-  if (p.pack_down) pack.add(a.down, a.a_f32, a.down_hi, a.a_f32 ? a.down_lo : nullptr, a.adapters, a.rank, a.d_in, a.rank,
-                            p.kp, false);
-  pack.add(a.up, a.a_f32, a.up_hi, a.a_f32 ? a.up_lo : nullptr, a.adapters, a.d_out, a.rank, a.rank, p.np, true);
-  if (a.out) pack.add(a.down, a.a_f32, a.down_t, nullptr, a.adapters, a.rank, a.d_in, a.d_in, p.rp, true);
+  if (p.pack_x) pack.add(a.x, 0, a.xp, nullptr, nullptr, 1, a.rows, a.d_in, a.rows, p.kp, false);
+  if (p.pack_dy) pack.add(a.dy, 0, a.dyp, nullptr, nullptr, 1, a.rows, a.d_out, a.rows, p.np, false);
+  if (a.out) pack.add(a.w, a.w_f32, a.wp, nullptr, nullptr, 1, a.d_out, a.d_in, a.d_in, p.np, true);
+  if (p.pack_down)
+    pack.add(a.down, a.a_f32, a.down_hi, a.down_mid, a.down_lo, a.adapters, a.rank, a.d_in, a.rank, p.kp, false);
+  pack.add(a.up, a.a_f32, a.up_hi, a.up_mid, a.up_lo, a.adapters, a.d_out, a.rank, a.rank, p.np, true);
+  if (a.out) pack.add(a.down, a.a_f32, a.down_t, nullptr, nullptr, a.adapters, a.rank, a.d_in, a.d_in, p.rp, true);
   pack.launch(st);
   ThinArgs t{};
   t.job[0].x = p.pack_x ? a.xp : a.x;
-  t.job[0].hi = p.pack_down ? a.down_hi : static_cast<const bf16*>(a.down);
-  t.job[0].lo = a.a_f32 ? a.down_lo : nullptr;
+  const bf16* down[3] = {p.pack_down ? a.down_hi : static_cast<const bf16*>(a.down), a.down_mid, a.down_lo};
+  const bf16* up[3] = {a.up_hi, a.up_mid, a.up_lo};
+  for (int i = 0; i < 3; ++i) {
+    t.job[0].mat[i] = down[i];
+    t.job[1].mat[i] = up[i];
+  }
   t.job[0].u = a.u;
   t.job[0].K = p.kp;
   t.job[1].x = p.pack_dy ? a.dyp : a.dy;
-  t.job[1].hi = a.up_hi;
-  t.job[1].lo = a.a_f32 ? a.up_lo : nullptr;
   t.job[1].u = a.v;
   t.job[1].K = p.np;
   t.job[0].mat_rows = t.job[1].mat_rows = a.rank;
   t.q = requests_of(a);
   t.ids = a.ids;
   t.rank = a.rank;
-  t.ld = 2 * p.rp;
-  a.a_f32 ? launch_thin<true, true>(t, p.rp, 2, st) : launch_thin<false, true>(t, p.rp, 2, st);
+  a.a_f32 ? launch_thin<3, true>(t, p.rp, 2, st) : launch_thin<1, true>(t, p.rp, 2, st);
   if (a.out) {
     ProductArgs g{};
     g.x = t.job[1].x;
@@ -837,7 +885,7 @@ void launch_adapted_grad(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t
     g.K = p.np;
     g.N = a.d_in;
     g.RP = p.rp;
-    g.ld = 2 * p.rp;
+    g.ld = parts_ld(p.rp);
     launch_product(g, st);
   }
   const bool join = p.chunks > 1;

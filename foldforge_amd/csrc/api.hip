@@ -623,7 +623,7 @@ size_t adapted_ws(void* ws, const AdaptedPlan& p, AdaptedArgs& a, int backward) 
   if (!backward) {
     if (p.pack_w) a.wp = cv.take<bf16>((size_t)a.d_out * p.kp);
     if (p.pack_up) a.upp = cv.take<bf16>((size_t)a.adapters * a.d_out * p.rp);
-    a.u = cv.take<bf16>((size_t)a.rows * p.rp);
+    a.u = cv.take<bf16>((size_t)a.rows * p.ld);
     return cv.used;
   }
   if (p.pack_dy) a.dyp = cv.take<bf16>((size_t)a.rows * p.np);
@@ -631,11 +631,13 @@ size_t adapted_ws(void* ws, const AdaptedPlan& p, AdaptedArgs& a, int backward) 
   a.down_t = cv.take<bf16>((size_t)a.adapters * a.d_in * p.rp);
   a.up_hi = cv.take<bf16>(mats * p.np);
   if (a.a_f32) {
+    a.down_mid = cv.take<bf16>(mats * p.kp);
     a.down_lo = cv.take<bf16>(mats * p.kp);
+    a.up_mid = cv.take<bf16>(mats * p.np);
     a.up_lo = cv.take<bf16>(mats * p.np);
   }
-  a.u = cv.take<bf16>((size_t)a.rows * 2 * p.rp);
-  a.v = cv.take<bf16>((size_t)a.rows * 2 * p.rp);
+  a.u = cv.take<bf16>((size_t)a.rows * p.ld);
+  a.v = cv.take<bf16>((size_t)a.rows * p.ld);
   if (p.chunks > 1) {
     a.part[0] = cv.take<float>(p.chunks * mats * a.d_in);
     a.part[1] = cv.take<float>(p.chunks * mats * a.d_out);

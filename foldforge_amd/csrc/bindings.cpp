@@ -110,6 +110,67 @@ PyObject* activation_ok(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+bool plain(const at::Tensor& t, at::Device device) {
+  return t.layout() == at::kStrided && t.device() == device && t.is_contiguous();
+}
+bool aligned(const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0; }
+// FFK_DTYPE_* of a bf16 / fp32 tensor, -1 for another.
+int dtype_code(const at::Tensor& t) {
+  return t.scalar_type() == at::kBFloat16 ? FFK_DTYPE_BF16 : t.scalar_type() == at::kFloat ? FFK_DTYPE_F32 : -1;
+}
+
+// adapted_sizes(x, weight, bias, down, up, scale, offsets, adapter): (rows, d_in, d_out, adapters, rank, requests, weight's
+// dtype, adapters' dtype) where every tensor (bias and scale may be None) is as a projection with adapters takes it, None
+// where not (the caller looks closer; sizes out of the kernels' range are left to it).
+PyObject* adapted_sizes(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8) return PyErr_Format(PyExc_TypeError, "adapted_sizes: 8 tensors");
+  for (int i = 0; i < 8; ++i)
+    if (!THPVariable_Check(args[i]) && !((i == 2 || i == 5) && args[i] == Py_None)) Py_RETURN_NONE;
+  const at::Tensor &x = THPVariable_Unpack(args[0]), &w = THPVariable_Unpack(args[1]), &down = THPVariable_Unpack(args[3]),
+                   &up = THPVariable_Unpack(args[4]), &offsets = THPVariable_Unpack(args[6]),
+                   &adapter = THPVariable_Unpack(args[7]);
+  const at::Device device = x.device();
+  const int wc = dtype_code(w), ac = dtype_code(down);
+  if (!x.is_cuda() || !plain(x, device) || x.scalar_type() != at::kBFloat16 || x.dim() == 0 || wc < 0 || ac < 0 ||
+      dtype_code(up) != ac || w.dim() != 2 || down.dim() != 3 || up.dim() != 3 || !plain(w, device) ||
+      !plain(down, device) || !plain(up, device) || !plain(offsets, device) || !plain(adapter, device) ||
+      offsets.dim() != 1 || adapter.dim() != 1 || offsets.scalar_type() != at::kInt ||
+      adapter.scalar_type() != at::kInt || offsets.numel() != adapter.numel() + 1)
+    Py_RETURN_NONE;
+  const int64_t d_out = w.size(0), d_in = w.size(1), adapters = down.size(0), rank = down.size(1);
+  if (d_in <= 0 || d_out <= 0 || x.size(x.dim() - 1) != d_in || down.size(2) != d_in || up.size(0) != adapters ||
+      up.size(1) != d_out || up.size(2) != rank || !aligned(x) || !aligned(w) || !aligned(down) || !aligned(up))
+    Py_RETURN_NONE;
+  const int64_t sizes[2] = {d_out, adapters};
+  for (int i = 0; i < 2; ++i) {
+    PyObject* o = args[i ? 5 : 2];
+    if (o == Py_None) continue;
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (t.scalar_type() != at::kFloat || t.dim() != 1 || t.size(0) != sizes[i] || !plain(t, device)) Py_RETURN_NONE;
+  }
+  return Py_BuildValue("(LLLLLLii)", (long long)(x.numel() / d_in), (long long)d_in, (long long)d_out, (long long)adapters,
+                       (long long)rank, (long long)adapter.numel(), wc, ac);
+  END_HANDLE_TH_ERRORS
+}
+
+// like(x, other): whether both are contiguous bf16 / fp32 tensors of one shape, type and GPU, with a last axis (other may be
+// None).
+PyObject* like(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 2) return PyErr_Format(PyExc_TypeError, "like(tensor, tensor or None)");
+  if (!THPVariable_Check(args[0]) || !(args[1] == Py_None || THPVariable_Check(args[1]))) Py_RETURN_FALSE;
+  const at::Tensor& x = THPVariable_Unpack(args[0]);
+  if (!x.is_cuda() || !plain(x, x.device()) || dtype_code(x) < 0 || x.dim() == 0 || x.size(x.dim() - 1) == 0)
+    Py_RETURN_FALSE;
+  if (args[1] != Py_None) {
+    const at::Tensor& o = THPVariable_Unpack(args[1]);
+    if (!plain(o, x.device()) || o.scalar_type() != x.scalar_type() || o.sizes() != x.sizes()) Py_RETURN_FALSE;
+  }
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 // empties(tensor, ((shape, kind), ...)): new tensors on the tensor's device, kind 0 bf16, 1 fp32, 2 uint8, 3 e4m3 (a
 // call's outputs and workspace in one step: four torch.empty cost 5 us of the caller's time).
 PyObject* empties(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -152,6 +213,8 @@ PyObject* empties(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyMethodDef methods[] = {
     {"params_ok", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&params_ok)), METH_FASTCALL, nullptr},
     {"activation_ok", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&activation_ok)), METH_FASTCALL, nullptr},
+    {"adapted_sizes", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&adapted_sizes)), METH_FASTCALL, nullptr},
+    {"like", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&like)), METH_FASTCALL, nullptr},
     {"empties", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&empties)), METH_FASTCALL, nullptr},
     FFK_CALL(ffk_layer_norm),
     FFK_CALL(ffk_layer_norm_linear),

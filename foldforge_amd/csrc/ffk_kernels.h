@@ -427,7 +427,7 @@ void launch_dropout(const DropoutArgs& a, hipStream_t stream);
 
 // A projection with low-rank adapters of many requests (adapted.hip; rows > 0).
 struct AdaptedPlan {
-  int rp;            // rank rounded up to 16, 32, 64 or 128
+  int rp, ld;        // rank rounded up to 16, 32, 64 or 128; channels of a row of u and v
   int64_t kp, np;    // d_in and d_out rounded up to 64
   int few;           // few rows: operands straight from the call's tensors
   int pack_x, pack_dy, pack_w, pack_down, pack_up;  // which the products read from copies (backward: w and up always)
@@ -447,9 +447,10 @@ struct AdaptedArgs {
   // workspace (adapted_ws)
   int32_t* ids;                       // [rows]
   bf16 *xp, *dyp, *wp;                // padded copies of x, dy; w bf16 (backward: turned)
-  bf16 *down_hi, *down_lo, *down_t;   // [adapters][rank][kp] twice, [adapters][d_in][rp]
-  bf16 *upp, *up_hi, *up_lo;          // [adapters][d_out][rp], [adapters][rank][np] twice
-  bf16 *u, *v;                        // [rows][rp], backward [rows][2 rp]
+  bf16 *down_hi, *down_mid, *down_lo; // [adapters][rank][kp] each
+  bf16 *up_hi, *up_mid, *up_lo;       // [adapters][rank][np] each
+  bf16 *down_t, *upp;                 // [adapters][d_in][rp], [adapters][d_out][rp]
+  bf16 *u, *v;                        // [rows][ld]
   float* few_u;                       // [rows][rank]
   float* part[2];                     // [chunks][adapters][rank][d_in], .. [d_out]
 };

@@ -440,15 +440,20 @@ def dropout_add(update: Tensor, residual: Tensor | None = None, *, p: float, see
     :func:`dropout_backward` with the same ones draws it again. Calls of one seed are told apart by their offsets.
     ``seed`` on the device, int64 ``(seed, offset)`` read when the kernel runs, is for captured calls: a graph that counts
     its offset up draws anew at each replay. A dropped value does not reach the result, whatever it is."""
-    _rows_tensor(update, "update")
-    if residual is not None and not (isinstance(residual, Tensor) and residual.shape == update.shape
-                                     and residual.dtype == update.dtype and residual.device == update.device
-                                     and residual.is_contiguous()):
-        _refuse(f"residual must be a contiguous {update.dtype} tensor {tuple(update.shape)} on {update.device}")
+    on_gpu = isinstance(update, Tensor) and update.is_cuda
+    if not (on_gpu and _native.calls().like(update, residual)):
+        _rows_tensor(update, "update")
+        if residual is not None and not (isinstance(residual, Tensor) and residual.shape == update.shape
+                                         and residual.dtype == update.dtype and residual.device == update.device
+                                         and residual.is_contiguous()):
+            _refuse(f"residual must be a contiguous {update.dtype} tensor {tuple(update.shape)} on {update.device}")
     dropped = dropped_of_levels(p)
     state, seed, offset = _drawn(seed, offset, update.device)
     axes = mask_axes(update.shape, shared)
-    out = _output(out, tuple(update.shape), update.dtype, update.device)
+    if out is None:
+        out = torch.empty_like(update)
+    else:
+        out = _output(out, tuple(update.shape), update.dtype, update.device)
     if update.numel():
         _call(update.device, "dropout_add", update, residual, out, state, seed, offset, *axes, dropped,
               _dtype_code(update.dtype))
@@ -496,9 +501,13 @@ class _Adapted(NamedTuple):
     adapter_dtype: int
 
 
-def _adapted(x: Tensor, weight: Tensor, down: Tensor, up: Tensor, scale: Tensor | None, offsets: Tensor,
-             adapter: Tensor) -> _Adapted:
+def _adapted(x: Tensor, weight: Tensor, bias: Tensor | None, down: Tensor, up: Tensor, scale: Tensor | None,
+             offsets: Tensor, adapter: Tensor) -> _Adapted:
     """The sizes of a projection with adapters, its tensors checked (the C-ABI receives pointers)."""
+    if isinstance(x, Tensor) and x.is_cuda:
+        sizes = _native.calls().adapted_sizes(x, weight, bias, down, up, scale, offsets, adapter)
+        if sizes is not None and sizes[0] < 2**31 and adapted_linear_supported(sizes[1], sizes[2], sizes[4], sizes[3]):
+            return _Adapted._make(sizes)
     rows, dev = _rows_tensor(x, "x"), x.device
     if x.dtype != torch.bfloat16:
         _refuse(f"x must be bf16 (got {x.dtype})")
@@ -525,6 +534,10 @@ def _adapted(x: Tensor, weight: Tensor, down: Tensor, up: Tensor, scale: Tensor 
         _refuse(f"offsets has {offsets.numel()} entries for {adapter.numel()} requests (one more than they)")
     if rows >= 2**31:
         _refuse(f"x has {rows} rows (fewer than 2^31)")
+    if bias is not None and not _param(bias, dev, "bias", (d_out,)).data_ptr() == bias.data_ptr():
+        _refuse("bias must be contiguous")
+    if x.data_ptr() % 16:
+        _refuse("x must be 16-byte aligned")
     return _Adapted(rows, d_in, d_out, n, rank, adapter.numel(), codes[0], codes[1])
 
 
@@ -537,16 +550,19 @@ def adapted_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, dow
     adapter ``adapter[r]`` (int32, on the device): one row each in a batch of single tokens, ``[0, N^2, 2 N^2, ...]`` for
     pair tensors of several targets. Rows of no request, and requests whose adapter is none of them (-1), have the
     projection alone. Output bf16 ``[..., d_out]``. Any widths; rank up to 128."""
-    q = _adapted(x, weight, down, up, scale, offsets, adapter)
-    if x.data_ptr() % 16:
-        _refuse("x must be 16-byte aligned")
-    bias = _affine(bias, x, "bias", q.d_out)
-    out = _output(out, (*x.shape[:-1], q.d_out), torch.bfloat16, x.device)
-    if out.data_ptr() % 16:
-        _refuse("out must be 16-byte aligned")
+    q = _adapted(x, weight, bias, down, up, scale, offsets, adapter)
+    shape = (*x.shape[:-1], q.d_out)
+    if out is not None:
+        _output(out, shape, torch.bfloat16, x.device)
+        if out.data_ptr() % 16:
+            _refuse("out must be 16-byte aligned")
+        if x.data_ptr() < out.data_ptr() + 2 * out.numel() and out.data_ptr() < x.data_ptr() + 2 * x.numel():
+            _refuse("out must not overlap x")
+    lib = _native.calls()
+    size = lib.ffk_adapted_linear_workspace(q.rows, q.d_in, q.d_out, q.adapters, q.rank, q.weight_dtype, q.adapter_dtype)
+    ws, *new = lib.empties(x, (((size,), _U8), *(((shape, _BF16),) if out is None else ())))
+    out = new[0] if out is None else out
     if q.rows:
-        ws = _workspace(_native.calls().ffk_adapted_linear_workspace(
-            q.rows, q.d_in, q.d_out, q.adapters, q.rank, q.weight_dtype, q.adapter_dtype), x.device)
         _call(x.device, "adapted_linear", x, weight, bias, down, up, scale, offsets, adapter, out, ws, ws.numel(), *q)
     return out
 
@@ -566,13 +582,12 @@ def adapted_linear_backward(dy: Tensor, x: Tensor, weight: Tensor, *, down: Tens
     (``with_x=False``: not computed), ``down`` and ``up`` in ``grad_dtype``, sums over all rows of an adapter in fp32 and a
     fixed order (zeros for an adapter without rows). The projection itself is frozen: ``weight`` and the bias have no
     gradient here."""
-    q = _adapted(x, weight, down, up, scale, offsets, adapter)
+    q = _adapted(x, weight, None, down, up, scale, offsets, adapter)
     if not (isinstance(dy, Tensor) and dy.dtype == torch.bfloat16 and dy.device == x.device and dy.is_contiguous()
             and tuple(dy.shape) == (*x.shape[:-1], q.d_out)):
         _refuse(f"dy must be a contiguous bf16 tensor {(*x.shape[:-1], q.d_out)} on {x.device}")
-    for t, name in ((dy, "dy"), (x, "x")):
-        if t.data_ptr() % 16:
-            _refuse(f"{name} must be 16-byte aligned")
+    if dy.data_ptr() % 16:
+        _refuse("dy must be 16-byte aligned")
     code = _grad_dtype(grad_dtype)
     if not q.rows:
         return AdaptedGradients(torch.empty_like(x) if with_x else None, torch.zeros_like(down, dtype=grad_dtype),

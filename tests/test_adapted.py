@@ -68,6 +68,7 @@ BAD = [
 
 
 @pytest.mark.parametrize("change,message", BAD + [({"bias": torch.zeros(23)}, "bias"),
+                                                  ({"bias": torch.zeros(48)[::2]}, "bias"),
                                                   ({"out": torch.zeros(6, 24)}, "out"),
                                                   ({"out": torch.zeros(24, 6, dtype=torch.bfloat16).T}, "out")])
 def test_forward_refusals(on_cpu, change, message):
@@ -87,6 +88,13 @@ def test_backward_refusals(on_cpu, change, message):
         args["dy"] = torch.zeros(*args["x"].shape[:-1], 24, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match=message):
         kernels.adapted_linear_backward(args.pop("dy"), args.pop("x"), args.pop("weight"), **args)
+
+
+def test_an_output_over_the_input_is_refused(on_cpu, monkeypatch):
+    memory = torch.zeros(400, dtype=torch.bfloat16)
+    args = {**_call(d_in=24), "x": memory[:144].view(6, 24)}
+    with pytest.raises(ValueError, match="overlap"):
+        kernels.adapted_linear(args.pop("x"), args.pop("weight"), out=memory[8:152].view(6, 24), **{**args, "bias": None})
 
 
 def test_sizes_that_are_served():

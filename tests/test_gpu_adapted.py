@@ -3,11 +3,11 @@
 Tolerances. A value is a sum of products whose magnitudes ``mag`` the oracle gives at the absolute values of everything.
 Each fp32 operation is off by at most 2^-24 of its result, and no sum is longer than its terms' count: ``n 2^-24 mag``.
 An operand rounded to bf16 is off by at most 2^-8 of itself, and with it every product that it enters: fp32 weights and the
-rows ``A x`` (above 256 rows) in the outputs. For the adapters' gradients the rows and the fp32 adapters are kept as two bf16:
-what the first leaves (2^-8) is rounded once more (2^-8 of it): 2^-16 each. A bf16 result adds 2^-8 of itself. These bound
-every value. In norm, roundings of many terms add in quadrature: r = 2^-8 / sqrt(3) of the result for each operand rounded,
-so sqrt(4) r = 4.5e-3 for the outputs (weight, rows, adapters and result), held to 1e-2 as every op of the stack, and
-sqrt(3) 2^-16 / sqrt(3) = 1.5e-5 for fp32 gradients at most (2^-17 / sqrt(3) for an ordinary rounding: 8e-6).
+rows ``A x`` (above 256 rows) in the outputs. For the adapters' gradients the rows and the fp32 adapters are kept as three
+bf16: each leaves 2^-8 of what it rounds, 2^-24 after the third, as fp32 itself. A bf16 result adds 2^-8 of itself. These
+bound every value. In norm, roundings of many terms add in quadrature: r = 2^-8 / sqrt(3) of the result for each operand
+rounded, so sqrt(4) r = 4.5e-3 for the outputs (weight, rows, adapters and result), held to 1e-2 as every op of the stack,
+and sqrt(n) 2^-24 for fp32 gradients, 1.2e-5 for the longest sum here (n = 40000 rows and a width), held to 1.5e-5.
 """
 
 from __future__ import annotations
@@ -100,7 +100,7 @@ def check_backward(t, got, grad_dtype=F32):
         near(got.x, want[0], tol, 1e-2, "dx")
     for g, w, m, width, name in ((got.down, want[1], mag[1], d_out, "down"), (got.up, want[2], mag[2], d_in, "up")):
         assert g.dtype == grad_dtype
-        tol = ((1 if t["down"].dtype == BF16 else 2) * 2.0**-16 + (width + rows + 8) * 2.0**-24) * m
+        tol = (width + rows + 10) * 2.0**-24 * m
         if grad_dtype == BF16:
             tol += HALF * w.abs()
         near(g, w, tol, 1e-2 if grad_dtype == BF16 else 1.5e-5, name)
