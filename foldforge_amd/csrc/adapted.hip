@@ -15,6 +15,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "ffk_adapted.h"
 #include "ffk_device.h"
 #include "ffk_kernels.h"
 
@@ -22,19 +23,8 @@ namespace ffk {
 
 namespace {
 
-__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-}
-
 // ---------------------------------------------------------------------------------------------------------
 // which adapter a row has
-
-struct Requests {
-  const int32_t *offsets, *adapter;  // [count + 1], [count]
-  const float* scale;                // [adapters], or null (1)
-  int count, adapters;
-  int64_t rows;
-};
 
 // id[i], i < 64: the adapter of row row0 + i, -1 for none (and behind the last row). All threads of the workgroup (of NT);
 // start and before are its scratch. One pass over the offsets: how many begin at or before the first row, and which begin at
@@ -67,8 +57,6 @@ __device__ __forceinline__ void tile_ids(const Requests& q, int64_t row0, int* i
   }
   __syncthreads();
 }
-
-__device__ __forceinline__ float scale_of(const Requests& q, int a) { return q.scale ? q.scale[a] : 1.f; }
 
 // ---------------------------------------------------------------------------------------------------------
 // operands in the products' orders
@@ -792,6 +780,7 @@ AdaptedPlan adapted_plan(int64_t rows, int d_in, int d_out, int adapters, int ra
 }
 
 void launch_adapted(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t st) {
+  if (adapted_rows_served(a.rows, a.d_in, a.d_out, a.rank, a.requests)) return launch_adapted_rows(a, st);
   const Requests q = requests_of(a);
   if (p.few) {
     FewArgs f{};

@@ -454,6 +454,9 @@ struct AdaptedArgs {
   float* few_u;                       // [rows][rank]
   float* part[2];                     // [chunks][adapters][rank][d_in], .. [d_out]
 };
+// many rows of the stacks' widths: one pass (adapted_rows.hip)
+bool adapted_rows_served(int64_t rows, int d_in, int d_out, int rank, int requests);
+void launch_adapted_rows(const AdaptedArgs& a, hipStream_t stream);
 void launch_adapted(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t stream);
 void launch_adapted_grad(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t stream);
 

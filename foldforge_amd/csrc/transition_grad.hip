@@ -660,49 +660,10 @@ __global__ __launch_bounds__(256, 2) void gemm128(const Gemm64Args p) {
 // ---------------------------------------------------------------------------------------------------------
 // The fused form (d = 64 or 128): two kernels, the hidden rows stay in registers.
 
-// A row of D values of 2 bytes in LDS, D / 8 pieces of 16 bytes: piece p of row r lies at piece p ^ swz(r), as above.
-template <int D>
-__device__ __forceinline__ int swz(int r) {
-  if constexpr (D == 64) return swz64(r);
-  return (r & 1) << 3 | (r & 2) << 1 | (((r >> 2) ^ (r >> 3)) & 1) << 1 | ((r >> 2) & 1);
-}
-template <int D>
-__device__ __forceinline__ int off_row(int r, int p) { return r * D + 8 * (p ^ swz<D>(r)); }
-
-// 1 KB (512 / D rows) of a row-major array of D-value rows goes to LDS in one transfer, swizzled: lane L copies piece
-// (L % P) ^ swz of row r0 + L / P (P = D / 8; r0 a multiple of 512 / D). The lane's offset from row r0, in bytes:
-template <int D>
-__device__ __forceinline__ uint32_t kb_offset(int r0, int lane) {
-  constexpr int P = D / 8;
-  return 2 * D * (lane / P) + 16 * ((lane % P) ^ swz<D>(r0 + lane / P));
-}
 // Nothing is scheduled across: left alone the compiler fetches each operand right before its product and waits out the
 // LDS latency every time, so the products' loops fetch a step or two ahead in the order they are written.
 __device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
-// LDS reads by byte address. A piece's number enters an address by XOR (of bits below the row's), so that a lane needs one
-// address for a tile: piece p + 2^i, with bit i of p clear, is at the address of p with that bit turned over.
-template <typename V>
-__device__ __forceinline__ V lds_at(uint32_t a) {
-  return *(const __attribute__((address_space(3))) V*)(a);
-}
-// Operand of a 16 x 16 product over 32 k from a tile of D-channel rows that are k: lanes of quarter q hold rows 4 q + 0..3
-// and 16 + 4 q + 0..3 of one channel. a: turned_at(...) of the tile, its channels 16 c .. by ^ (c << 5).
-template <int D>
-__device__ __forceinline__ uint32_t turned_at(int lane) {
-  const int j = lane & 15, r = 4 * (lane >> 4) + (j >> 2);
-  return 2 * off_row<D>(r, (j & 3) >> 1) + 8 * (j & 1);
-}
-template <int D>
-__device__ __forceinline__ bf16x8 ld_turned16(uint32_t a) {
-  union {
-    s16x4 s[2];
-    bf16x8 v;
-  } o;
-  o.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a));
-  o.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + 32 * D));
-  return o.v;
-}
 // One wave's 16 x 16 tile over 32 k: a lane holds row / column lane % 16 of its operands at 8 k, and rows 4 (lane / 16)
 // + 0..3 of column lane % 16 of the result.
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
