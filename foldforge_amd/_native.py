@@ -86,12 +86,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int32,
         [c_void_p] * 4 + [c_int64] * 5 + [c_int32, c_int32, c_void_p],
     ),
-    "ffk_adapted_linear_workspace": (c_size_t, [c_int64] + [c_int32] * 6),
+    "ffk_adapted_linear_workspace": (c_size_t, [c_int64] + [c_int32] * 7),
     "ffk_adapted_linear": (
         c_int32,
         [c_void_p] * 10 + [c_size_t, c_int64] + [c_int32] * 7 + [c_void_p],
     ),
-    "ffk_adapted_linear_backward_workspace": (c_size_t, [c_int64] + [c_int32] * 6),
+    "ffk_adapted_linear_backward_workspace": (c_size_t, [c_int64] + [c_int32] * 7),
     "ffk_adapted_linear_backward": (
         c_int32,
         [c_void_p] * 12 + [c_size_t, c_int64] + [c_int32] * 8 + [c_void_p],

@@ -754,13 +754,17 @@ Requests requests_of(const AdaptedArgs& a) {
 
 }  // namespace
 
-AdaptedPlan adapted_plan(int64_t rows, int d_in, int d_out, int adapters, int rank, int w_f32, int a_f32, int backward) {
+AdaptedPlan adapted_plan(int64_t rows, int d_in, int d_out, int adapters, int rank, int requests, int w_f32, int a_f32,
+                         int backward) {
   AdaptedPlan p{};
   p.rp = rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128;
   p.ld = backward ? parts_ld(p.rp) : p.rp;
   p.kp = up64(d_in);
   p.np = up64(d_out);
   p.few = !backward && rows <= 256;
+  p.rows = backward ? adapted_rows_grad_served(rows, d_in, d_out, rank, requests)
+                    : adapted_rows_served(rows, d_in, d_out, rank, requests);
+  if (p.rows) return p;
   if (backward) {
     p.pack_x = d_in % 64 != 0;
     p.pack_dy = d_out % 64 != 0;
@@ -780,7 +784,7 @@ AdaptedPlan adapted_plan(int64_t rows, int d_in, int d_out, int adapters, int ra
 }
 
 void launch_adapted(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t st) {
-  if (adapted_rows_served(a.rows, a.d_in, a.d_out, a.rank, a.requests)) return launch_adapted_rows(a, st);
+  if (p.rows) return launch_adapted_rows(a, st);
   const Requests q = requests_of(a);
   if (p.few) {
     FewArgs f{};
@@ -835,6 +839,7 @@ void launch_adapted(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t st) 
 }
 
 void launch_adapted_grad(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t st) {
+  if (p.rows) return launch_adapted_rows_grad(a, st);
   Packer pack;
   if (p.pack_x) pack.add(a.x, 0, a.xp, nullptr, nullptr, 1, a.rows, a.d_in, a.rows, p.kp, false);
   if (p.pack_dy) pack.add(a.dy, 0, a.dyp, nullptr, nullptr, 1, a.rows, a.d_out, a.rows, p.np, false);

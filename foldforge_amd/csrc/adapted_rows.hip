@@ -70,6 +70,13 @@ __device__ __forceinline__ void typed(const void* p, int f32, F f) {
     f(static_cast<const bf16*>(p));
 }
 
+// The lane's number, opaque: addresses made of it are not kept in registers from tile to tile.
+__device__ __forceinline__ int fresh_lane() {
+  int l = threadIdx.x & 63;
+  asm volatile("" : "+v"(l));
+  return l;
+}
+
 struct RowsArgs {
   const bf16* x;  // [rows][C]
   const void *w, *down, *up;
@@ -105,6 +112,14 @@ __device__ __forceinline__ void rows_dma(const bf16* x, int64_t row0, int64_t ro
   }
 }
 
+// Operand of a 16 x 16 product over 32 k from an off_row<C> tile: rows 16 x + i, pieces 4 k + g. at: 2 * off_row<C>(i, g) from
+// the tile's LDS address. Bits 0 and 1 of k enter by XOR, the others as an offset (an address for each k would fill the
+// registers).
+template <int C>
+__device__ __forceinline__ bf16x8 row_operand(uint32_t at, int x, int k) {
+  return lds_at<bf16x8>((at ^ (uint32_t)((k & 3) << 6)) + (uint32_t)((k >> 2) << 8) + (uint32_t)(x * 32 * C));
+}
+
 // Two neighbouring blocks of 16 channels of 16 rows in 16-byte pieces: lane group g holds channels 4 g .. of each block; after
 // v_permlane16_swap (odd rows of 16 lanes of the first against even ones of the second) channels 8 (g / 2) .. of block g % 2.
 __device__ __forceinline__ bf16x8 join_blocks(const f32x4& a, const f32x4& b) {
@@ -132,7 +147,8 @@ __global__ __launch_bounds__(512, 2) void adapted_rows(const RowsArgs p) {
   const int64_t first = tiles * blockIdx.x / gridDim.x, last = tiles * (blockIdx.x + 1) / gridDim.x;
   const uint32_t lds = lds_addr(buf);
   auto fetch = [&](int64_t tile) __attribute__((always_inline)) {
-    rows_dma<C, S::PER>(p.x, tile * TM, rows, lds + (uint32_t)((tile - first) % STAGES) * sizeof(buf[0]), wave, lane);
+    rows_dma<C, S::PER>(p.x, tile * TM, rows, lds + (uint32_t)((tile - first) % STAGES) * sizeof(buf[0]), wave,
+                        fresh_lane());
   };
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s)
@@ -158,9 +174,7 @@ __global__ __launch_bounds__(512, 2) void adapted_rows(const RowsArgs p) {
   float scale = 1.f;
   int loaded = -1;
   auto load = [&](int a) __attribute__((always_inline)) {
-    int l = lane;  // (opaque: its addresses are not kept from tile to tile)
-    asm volatile("" : "+v"(l));
-    const int i = l & 15, g = l >> 4;
+    const int l = fresh_lane(), i = l & 15, g = l >> 4;
     if (loaded >= 0) __syncthreads();  // the last one's has been read
     loaded = a;
     scale = scale_of(p.q, a);
@@ -202,7 +216,7 @@ __global__ __launch_bounds__(512, 2) void adapted_rows(const RowsArgs p) {
   for (int64_t tile = first; tile < last; ++tile) {
     if (tile + STAGES - 1 < last) fetch(tile + STAGES - 1);
     const int64_t row0 = tile * TM, end = row0 + TM < rows ? row0 + TM : rows;
-    const bf16* t = buf[(tile - first) % STAGES];
+    const uint32_t t = lds + (uint32_t)((tile - first) % STAGES) * sizeof(buf[0]) + 2 * off_row<C>(r0 + i, g);
     f32x4 acc[S::NB][S::TT];
     for (int64_t row = row0; row < end;) {  // the requests in this tile
       request_next(p.q, row, at);
@@ -221,7 +235,7 @@ __global__ __launch_bounds__(512, 2) void adapted_rows(const RowsArgs p) {
         for (int k = 0; k < S::KS; ++k) {
           bf16x8 xf[S::TT];
 #pragma unroll
-          for (int x = 0; x < S::TT; ++x) xf[x] = ld8(&t[off_row<C>(r0 + 16 * x + i, 4 * k + g)]);
+          for (int x = 0; x < S::TT; ++x) xf[x] = row_operand<C>(t, x, k);
 #pragma unroll
           for (int x = 0; x < S::TT; ++x) {
 #pragma unroll
@@ -229,6 +243,8 @@ __global__ __launch_bounds__(512, 2) void adapted_rows(const RowsArgs p) {
 #pragma unroll
             for (int b = 0; b < S::NB; ++b) acc[b][x] = mfma16(w[b][k], xf[x], acc[b][x]);
           }
+          // (what is read ahead has to fit the registers)
+          if (S::KS * S::TT > 8 && k % (8 / S::TT) == 8 / S::TT - 1) __builtin_amdgcn_sched_barrier(0);
         }
       } else if (at.a >= 0) {
 #pragma unroll
@@ -237,7 +253,7 @@ __global__ __launch_bounds__(512, 2) void adapted_rows(const RowsArgs p) {
           for (int x = 0; x < S::TT; ++x)
 #pragma unroll
             for (int b = 0; b < RB; ++b)
-              u[b][x] = mfma16(ld8(&af[b * S::KS + k][8 * lane]), ld8(&t[off_row<C>(r0 + 16 * x + i, 4 * k + g)]), u[b][x]);
+              u[b][x] = mfma16(ld8(&af[b * S::KS + k][8 * lane]), row_operand<C>(t, x, k), u[b][x]);
       }
       const int64_t stop = at.hi < end ? at.hi : end;
       if (at.a >= 0) {
@@ -303,6 +319,440 @@ void launch_rows(const RowsArgs& p, hipStream_t st) {
   kernel<<<dim3((unsigned)std::min((p.q.rows + TM - 1) / TM, resident)), 512, 0, st>>>(p);
 }
 
+// ---------------------------------------------------------------------------------------------------------
+// backward
+
+struct RowsGradArgs {
+  const bf16 *x, *dy;  // [rows][CI], [rows][CO]
+  const void *w, *down, *up;
+  bf16* dx;            // or null
+  float* part;         // [gridDim.x + requests][16 RB][CI + CO]
+  Requests q;
+  int rank, w_f32, a_f32;
+};
+
+// v as three bf16 that add up to it.
+__device__ __forceinline__ void split3(float v, bf16 (&to)[3]) {
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    to[k] = (bf16)v;
+    v -= (float)to[k];
+  }
+}
+
+template <int CI, int CO, int RB>
+struct RowsGradShape {
+  static constexpr int KI = CI / 32, KO = CO / 32;                 // steps of k
+  static constexpr int NB = CI / 16 < 8 ? 1 : CI / 16 / 8;         // dx: blocks of 16 channels a wave,
+  static constexpr int NW = CI / 16 / NB, TT = 2 * NW / 8;         // waves along them, blocks of 16 rows a wave
+  // the thin products: parts (shares of k), a wave's steps of k, its blocks of 16 rows (one where k has fewer steps than waves)
+  static constexpr int SI = KI < 8 ? KI : 8, SO = KO < 8 ? KO : 8;
+  static constexpr int QI = KI / SI, QO = KO / SO, XI = KI < 8 ? 1 : 2, XO = KO < 8 ? 1 : 2;
+  static constexpr int GI = (CI / 16 + 7) / 8, GO = (CO / 16 + 7) / 8;  // gradients: blocks of 16 channels a wave
+  static constexpr int PER = (CI + CO + 127) / 128;                // transfers of a tile a wave
+  static constexpr bool STAGED = NB < 2;                           // dx goes through LDS: 16 channels a wave are 32 bytes a row
+  static constexpr int STORES = STAGED ? CI / 128 : NB / 2 * TT;   // stores of a tile a wave (some more with 64 channels)
+  static constexpr int STAGES = RB == 1 || CI + CO < 512 ? 3 : 2;
+};
+
+// A wave's part of a thin product of 32 rows: steps wave % SLOTS + SLOTS q of k, X blocks of 16 rows.
+template <int C, int SLOTS, int Q, int X, int RB, int PARTS>
+__device__ __forceinline__ void thin_part(uint32_t at, int wave, int lane, const bf16x8 (&m)[Q][RB][PARTS],
+                                          f32x4 (*part)[2][RB][64]) {
+  const int first = X == 1 ? wave / SLOTS : 0;
+  if (first >= 2) return;  // (fewer shares than waves)
+#pragma unroll
+  for (int x = 0; x < X; ++x) {
+    f32x4 t[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) t[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const bf16x8 v = row_operand<C>(at, first + x, SLOTS * q + wave % SLOTS);
+#pragma unroll
+      for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int k = 0; k < PARTS; ++k) t[b] = mfma16(m[q][b][k], v, t[b]);
+    }
+#pragma unroll
+    for (int b = 0; b < RB; ++b) part[wave % SLOTS][first + x][b][lane] = t[b];
+  }
+}
+
+// dx = dy W + v A_a, and the sums over this workgroup's rows of v^T x and u^T dy for each request in them (to
+// part[blockIdx.x + request]: a walk through the (workgroup, request) pairs in row order takes each such sum once). Tiles of 32
+// rows of x and dy stream through LDS. The thin products, u = s x A^T and v = s dy B, are split over the waves by k;
+// half the threads join the parts and lays u and v out as operands: v rounded with tokens as columns,
+// for dx, both in three parts with tokens as k, for the gradients, whose other operand is the tile turned as it is read. dx
+// goes through LDS to stores of whole rows. PARTS = 3: fp32 adapters. block 512.
+template <int CI, int CO, int RB, int PARTS>
+__global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p) {
+  using S = RowsGradShape<CI, CO, RB>;
+  constexpr int TM = 32, STAGES = S::STAGES, PAIRS = (RB + 1) / 2, TILE = TM * (CI + CO);
+  __shared__ __attribute__((aligned(1024))) bf16 buf[STAGES][TILE];
+  __shared__ __attribute__((aligned(16))) f32x4 part[S::SI + S::SO][2][RB][64];
+  __shared__ __attribute__((aligned(16))) bf16 stage[S::STAGED ? TM * CI : 8];
+  __shared__ __attribute__((aligned(16))) bf16x4 vop[2][PAIRS][64][2];
+  __shared__ __attribute__((aligned(16))) bf16 gop[2][3][RB][64][8];
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t rows = p.q.rows, tiles = (rows + TM - 1) / TM;
+  const int64_t first = tiles * blockIdx.x / gridDim.x, last = tiles * (blockIdx.x + 1) / gridDim.x;
+  const uint32_t lds = lds_addr(buf);
+  auto fetch = [&](int64_t tile) __attribute__((always_inline)) {
+    const uint32_t dst = lds + (uint32_t)((tile - first) % STAGES) * sizeof(buf[0]);
+    const int64_t row0 = tile * TM;
+    const int lane = fresh_lane();
+#pragma unroll
+    for (int u = 0; u < S::PER; ++u) {
+      // (all waves the same number of transfers, the last one again where they do not go round)
+      const int t = wave * S::PER + u < (CI + CO) / 16 ? wave * S::PER + u : (CI + CO) / 16 - 1;
+      if (t < CI / 16) {
+        const int r = 512 / CI * t + lane / (CI / 8);
+        const int64_t row = row0 + r < rows ? row0 + r : rows - 1;
+        dma16_at(p.x + row * CI + 8 * ((lane % (CI / 8)) ^ swz<CI>(r)), dst + 1024 * t);
+      } else {
+        const int r = 512 / CO * (t - CI / 16) + lane / (CO / 8);
+        const int64_t row = row0 + r < rows ? row0 + r : rows - 1;
+        dma16_at(p.dy + row * CO + 8 * ((lane % (CO / 8)) ^ swz<CO>(r)), dst + 1024 * t);
+      }
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s)
+    if (first + s < last) fetch(first + s);
+  const f32x4 none = {0.f, 0.f, 0.f, 0.f};
+  // W^T: this wave's channels of dx
+  const int n0 = 16 * S::NB * (wave % S::NW), r0 = 16 * S::TT * (wave / S::NW);
+  bf16x8 w[S::NB][S::KO];
+  if (p.dx) {
+    typed(p.w, p.w_f32, [&](const auto* from) __attribute__((always_inline)) {
+#pragma unroll
+      for (int b = 0; b < S::NB; ++b)
+#pragma unroll
+        for (int k = 0; k < S::KO; ++k) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[b][k][e] = (bf16)(float)from[(32 * k + 8 * g + e) * CI + n0 + 16 * b + i];
+          if (k % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+    });
+  }
+  if (threadIdx.x < 2 * PAIRS * 64) {
+    const bf16x4 z = {(bf16)0.f, (bf16)0.f, (bf16)0.f, (bf16)0.f};
+    (&vop[0][0][0][0])[2 * threadIdx.x] = z;
+    (&vop[0][0][0][0])[2 * threadIdx.x + 1] = z;
+  }
+  // the adapter: its share of the thin products (steps wave % S + S q of k, row blocks from wave / S on), this wave's channels
+  // of A for dx
+  bf16x8 am[S::QI][RB][PARTS], bm[S::QO][RB][PARTS], at_[S::NB][PAIRS];
+  float scale = 1.f;
+  int loaded = -1;
+  auto load = [&](int a) __attribute__((always_inline)) {
+    const int l = fresh_lane(), i = l & 15, g = l >> 4;
+    loaded = a;
+    scale = scale_of(p.q, a);
+    typed(p.down, p.a_f32, [&](const auto* all) __attribute__((always_inline)) {
+      const auto* from = all + (int64_t)a * p.rank * CI;
+#pragma unroll
+      for (int q = 0; q < S::QI; ++q)
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+          const int j = 16 * b + i;
+          const auto* row = from + (j < p.rank ? j : p.rank - 1) * CI + 32 * (S::SI * q + wave % S::SI) + 8 * g;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            bf16 t[3];
+            split3(j < p.rank ? (float)row[e] : 0.f, t);
+#pragma unroll
+            for (int k = 0; k < PARTS; ++k) am[q][b][k][e] = t[k];
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+      for (int b = 0; b < S::NB; ++b)
+#pragma unroll
+        for (int s = 0; s < PAIRS; ++s)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int j = 32 * s + 16 * (e >> 2) + 4 * g + (e & 3);
+            const bool is = j < p.rank && (RB > 1 || e < 4);
+            const float v = (float)from[(is ? j : p.rank - 1) * CI + n0 + 16 * b + i];
+            at_[b][s][e] = is ? (bf16)v : (bf16)0.f;
+          }
+    });
+    typed(p.up, p.a_f32, [&](const auto* all) __attribute__((always_inline)) {
+      const auto* from = all + (int64_t)a * CO * p.rank;
+#pragma unroll
+      for (int q = 0; q < S::QO; ++q)
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+          const int j = 16 * b + i;
+          const auto* row = from + (32 * (S::SO * q + wave % S::SO) + 8 * g) * p.rank + (j < p.rank ? j : p.rank - 1);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            bf16 t[3];
+            split3(j < p.rank ? (float)row[e * p.rank] : 0.f, t);
+#pragma unroll
+            for (int k = 0; k < PARTS; ++k) bm[q][b][k][e] = t[k];
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+    });
+  };
+  // the sums of the request in work
+  f32x4 gi[RB][S::GI], go[RB][S::GO];
+  int summed = -1;
+  auto clear = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+#pragma unroll
+      for (int q = 0; q < S::GI; ++q) gi[b][q] = none;
+#pragma unroll
+      for (int q = 0; q < S::GO; ++q) go[b][q] = none;
+    }
+  };
+  auto flush = [&]() __attribute__((always_inline)) {
+    const int l = fresh_lane(), i = l & 15, g = l >> 4;
+    float* to = p.part + (int64_t)(blockIdx.x + summed) * (16 * RB * (CI + CO)) + i;
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float* row = to + (16 * b + 4 * g + e) * (CI + CO);
+#pragma unroll
+        for (int q = 0; q < S::GI; ++q)
+          if (8 * q + wave < CI / 16) row[16 * (8 * q + wave)] = gi[b][q][e];
+#pragma unroll
+        for (int q = 0; q < S::GO; ++q)
+          if (8 * q + wave < CO / 16) row[CI + 16 * (8 * q + wave)] = go[b][q][e];
+      }
+  };
+  // this wave's rows of the staged dx
+  auto put = [&](int64_t row0) __attribute__((always_inline)) {
+    if constexpr (!S::STAGED) return;
+    const int lane = fresh_lane();
+#pragma unroll
+    for (int u = 0; u < (S::STORES > 0 ? S::STORES : 1); ++u) {
+      const int t = wave * (S::STORES > 0 ? S::STORES : 1) + u;
+      if (CI == 64 && wave >= 4) continue;
+      const int r = 512 / CI * t + lane / (CI / 8), piece = lane % (CI / 8);
+      if (row0 + r < rows)
+        __builtin_nontemporal_store(ld8(&stage[off_row<CI>(r, piece)]),
+                                    reinterpret_cast<bf16x8*>(p.dx + (row0 + r) * CI + 8 * piece));
+    }
+  };
+  clear();
+  RequestAt at{p.q.count, -1, rows};
+  if (first < last) at = request_first(p.q, first * TM);
+  if (first + STAGES - 1 <= last)
+    wait_vm_lds<(STAGES - 2) * S::PER>();
+  else
+    wait_vm_lds<0>();
+  __syncthreads();
+  for (int64_t tile = first; tile < last; ++tile) {
+    if (tile + STAGES - 1 < last) fetch(tile + STAGES - 1);
+    if (p.dx && tile > first) put((tile - 1) * TM);
+    const int64_t row0 = tile * TM, end = row0 + TM < rows ? row0 + TM : rows;
+    const uint32_t xs = lds + (uint32_t)((tile - first) % STAGES) * sizeof(buf[0]), ys = xs + 2 * TM * CI;
+    f32x4 acc[S::NB][S::TT];
+    for (int64_t row = row0; row < end;) {  // the requests in this tile
+      request_next(p.q, row, at);
+      const int64_t stop = at.hi < end ? at.hi : end;
+      const bool whole = row == row0 && stop == row0 + TM;
+      if (at.a >= 0) {
+        if (summed >= 0 && summed != at.r) {
+          flush();
+          clear();
+        }
+        summed = at.r;
+        if (at.a != loaded) load(at.a);
+        thin_part<CI, S::SI, S::QI, S::XI>(xs + 2 * off_row<CI>(i, g), wave, lane, am, part);
+        thin_part<CO, S::SO, S::QO, S::XO>(ys + 2 * off_row<CO>(i, g), wave, lane, bm, part + S::SI);
+      }
+      if (row == row0 && p.dx) {
+#pragma unroll
+        for (int b = 0; b < S::NB; ++b)
+#pragma unroll
+          for (int x = 0; x < S::TT; ++x) acc[b][x] = none;
+#pragma unroll
+        for (int k = 0; k < S::KO; ++k)
+#pragma unroll
+          for (int x = 0; x < S::TT; ++x) {
+            const bf16x8 yf = row_operand<CO>(ys + 2 * off_row<CO>(r0 + i, g), x, k);
+#pragma unroll
+            for (int b = 0; b < S::NB; ++b) acc[b][x] = mfma16(w[b][k], yf, acc[b][x]);
+            // (what is read ahead has to fit the registers)
+            if (x == S::TT - 1 && k % (8 / S::TT) == 8 / S::TT - 1) __builtin_amdgcn_sched_barrier(0);
+          }
+      }
+      if (at.a >= 0) {
+        __syncthreads();
+        if (threadIdx.x < 256 * RB) {
+          const int l = threadIdx.x & 63, b = (threadIdx.x >> 6) % RB, x = (threadIdx.x >> 6) / RB & 1;
+          const int y = (threadIdx.x >> 6) / RB >> 1, token = 16 * x + (l & 15);
+          const f32x4(*from)[2][RB][64] = part + (y ? S::SI : 0);
+          f32x4 v = from[0][x][b][l];
+          for (int s = 1; s < (y ? S::SO : S::SI); ++s) v += from[s][x][b][l];
+          const bool in = row0 + token >= row && row0 + token < stop;
+          bf16x4 high;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            bf16 t[3];
+            split3(in ? v[e] * scale : 0.f, t);
+            high[e] = t[0];
+#pragma unroll
+            for (int k = 0; k < 3; ++k) gop[y][k][b][4 * (l >> 4) + e + 16 * (l >> 2 & 3)][4 * x + (l & 3)] = t[k];
+          }
+          if (y) vop[x][b / 2][l][b & 1] = high;
+        }
+        __syncthreads();
+        if (p.dx) {
+#pragma unroll
+          for (int x = 0; x < S::TT; ++x) {
+            const int64_t mine = row0 + r0 + 16 * x + i;
+#pragma unroll
+            for (int b = 0; b < S::NB; ++b) {
+              f32x4 add = none;
+#pragma unroll
+              for (int s = 0; s < PAIRS; ++s)
+                add = mfma16(at_[b][s], *reinterpret_cast<const bf16x8*>(&vop[r0 / 16 + x][s][lane][0]), add);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[b][x][e] += mine >= row && mine < stop ? add[e] : 0.f;
+            }
+          }
+        }
+        // tokens as k: element e of lane group g is token 4 g + e, or 16 + 4 g + e - 4; those of other requests are left out
+        auto turned = [&](bf16x8 v) __attribute__((always_inline)) {
+          if (!whole) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int64_t r = row0 + 16 * (e >> 2) + 4 * g + (e & 3);
+              v[e] = r >= row && r < stop ? v[e] : (bf16)0.f;
+            }
+          }
+          return v;
+        };
+        const uint32_t xa = xs + turned_at<CI>(lane), ya = ys + turned_at<CO>(lane);
+        bf16x8 gv[RB][3];
+#pragma unroll
+        for (int b = 0; b < RB; ++b)
+#pragma unroll
+          for (int k = 0; k < 3; ++k) gv[b][k] = ld8(&gop[1][k][b][lane][0]);
+#pragma unroll
+        for (int q = 0; q < S::GI; ++q)
+          if (8 * q + wave < CI / 16) {
+            const bf16x8 t = turned(ld_turned16<CI>(xa ^ (uint32_t)(8 * q + wave) << 5));
+#pragma unroll
+            for (int b = 0; b < RB; ++b)
+#pragma unroll
+              for (int k = 0; k < 3; ++k) gi[b][q] = mfma16(gv[b][k], t, gi[b][q]);
+          }
+#pragma unroll
+        for (int b = 0; b < RB; ++b)
+#pragma unroll
+          for (int k = 0; k < 3; ++k) gv[b][k] = ld8(&gop[0][k][b][lane][0]);
+#pragma unroll
+        for (int q = 0; q < S::GO; ++q)
+          if (8 * q + wave < CO / 16) {
+            const bf16x8 t = turned(ld_turned16<CO>(ya ^ (uint32_t)(8 * q + wave) << 5));
+#pragma unroll
+            for (int b = 0; b < RB; ++b)
+#pragma unroll
+              for (int k = 0; k < 3; ++k) go[b][q] = mfma16(gv[b][k], t, go[b][q]);
+          }
+      } else if (row == row0) {
+        __syncthreads();  // (the last tile's dx has left the stage)
+      }
+      row = stop;
+    }
+    if constexpr (S::STAGED) {
+      if (p.dx) {
+#pragma unroll
+        for (int x = 0; x < S::TT; ++x) {
+          bf16x4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = (bf16)acc[0][x][e];
+          const int n = n0 + 4 * g;
+          *reinterpret_cast<bf16x4*>(&stage[off_row<CI>(r0 + 16 * x + i, n >> 3) + (n & 7)]) = v;
+        }
+      }
+    }
+    // The next tile has landed. Behind its transfers lie those of the tiles after it and the stores of each iteration since
+    // then (of whole tiles): the wave's memory operations complete in order.
+    constexpr int BEHIND = (STAGES - 2) * S::PER + (S::STAGED ? STAGES - 1 : STAGES - 2) * S::STORES;
+    if (tile + STAGES - 1 >= last)
+      wait_vm_lds<0>();
+    else if (p.dx && tile - first >= STAGES - 1)
+      wait_vm_lds<BEHIND>();
+    else
+      wait_vm_lds<(STAGES - 2) * S::PER>();
+    if constexpr (!S::STAGED) {
+      if (p.dx) {
+        bf16* to = p.dx + (row0 + r0 + i) * CI + n0 + 16 * (g & 1) + 8 * (g >> 1);
+#pragma unroll
+        for (int x = 0; x < S::TT; ++x) {
+          bf16x8 v[(S::NB + 1) / 2];
+#pragma unroll
+          for (int b = 0; b < S::NB / 2; ++b) v[b] = join_blocks(acc[2 * b][x], acc[2 * b + 1][x]);
+          if (end - row0 < TM && row0 + r0 + 16 * x + i >= rows) continue;
+#pragma unroll
+          for (int b = 0; b < S::NB / 2; ++b)
+            __builtin_nontemporal_store(v[b], reinterpret_cast<bf16x8*>(to + 16 * x * CI + 32 * b));
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (first < last) {
+    if (p.dx) put((last - 1) * TM);
+    if (summed >= 0) flush();
+  }
+}
+
+struct RowsJoinArgs {
+  const float* part;  // [slots][rp][CI + CO]
+  void *ddown, *dup;
+  Requests q;
+  int rank, rp, d_in, d_out, grid, to_bf16;
+};
+
+// The gradients of an adapter from its requests' sums: request r has one in slot b + r of each workgroup b of the grid that its
+// rows touch. A workgroup: 64 columns of one channel of one adapter, sixteen threads beside each other along them, sixteen
+// groups of slots. grid (ceil((d_in + d_out) / 64), rank, adapters); block 256.
+__global__ __launch_bounds__(256) void adapted_rows_join(const RowsJoinArgs p) {
+  __shared__ f32x4 sum[16][16];
+  const int width = p.d_in + p.d_out, group = threadIdx.x >> 4, c = 64 * blockIdx.x + 4 * (threadIdx.x & 15);
+  const int j = blockIdx.y, a = blockIdx.z;
+  const int64_t tiles = (p.q.rows + 31) / 32, G = p.grid;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  if (c < width)
+    for (int r = 0; r < p.q.count; ++r) {
+      if (p.q.adapter[r] != a) continue;
+      const int64_t lo = p.q.offsets[r] > 0 ? p.q.offsets[r] : 0;
+      const int64_t hi = p.q.offsets[r + 1] < p.q.rows ? (int64_t)p.q.offsets[r + 1] : p.q.rows;
+      if (lo >= hi) continue;
+      // workgroup b has the tiles from tiles b / G on
+      const int64_t b0 = ((lo / 32 + 1) * G - 1) / tiles, b1 = (((hi - 1) / 32 + 1) * G - 1) / tiles;
+#pragma unroll 4
+      for (int64_t b = b0 + group; b <= b1; b += 16)
+        v += *reinterpret_cast<const f32x4*>(p.part + ((b + r) * p.rp + j) * width + c);
+    }
+  sum[group][threadIdx.x & 15] = v;
+  __syncthreads();
+  if (threadIdx.x >= 64 || 64 * (int)blockIdx.x + (int)threadIdx.x >= width) return;
+  float total = 0.f;
+#pragma unroll
+  for (int s = 0; s < 16; ++s) total += sum[s][threadIdx.x >> 2][threadIdx.x & 3];
+  const int col = 64 * blockIdx.x + threadIdx.x;
+  const bool in = col < p.d_in;
+  const int64_t at = in ? ((int64_t)a * p.rank + j) * p.d_in + col : ((int64_t)a * p.d_out + col - p.d_in) * p.rank + j;
+  void* to = in ? p.ddown : p.dup;
+  if (p.to_bf16)
+    static_cast<bf16*>(to)[at] = (bf16)total;
+  else
+    static_cast<float*>(to)[at] = total;
+}
+
 // The widths served: the pair and MSA stacks' projections (d to d, 2 d, 4 d and back, d = 64, 128, 256).
 #define FFK_ROWS_WIDTHS(X) \
   X(64, 64) X(64, 128) X(128, 64) X(64, 256) X(256, 64) X(128, 128) X(128, 256) X(256, 128) X(128, 512) X(512, 128) X(256, 256)
@@ -310,6 +760,14 @@ void launch_rows(const RowsArgs& p, hipStream_t st) {
 template <int C, int N>
 void launch_rank(const RowsArgs& p, hipStream_t st) {
   p.rank <= 16 ? launch_rows<C, N, 1>(p, st) : launch_rows<C, N, 2>(p, st);
+}
+
+template <int CI, int CO>
+void launch_grad(const RowsGradArgs& p, int grid, hipStream_t st) {
+  if (p.a_f32)
+    adapted_rows_grad<CI, CO, 1, 3><<<dim3(grid), 512, 0, st>>>(p);
+  else
+    adapted_rows_grad<CI, CO, 1, 1><<<dim3(grid), 512, 0, st>>>(p);
 }
 
 }  // namespace
@@ -343,6 +801,49 @@ void launch_adapted_rows(const AdaptedArgs& a, hipStream_t st) {
   if (a.d_in == C && a.d_out == N) launch_rank<C, N>(p, st);
   FFK_ROWS_WIDTHS(FFK_ROWS_CASE)
 #undef FFK_ROWS_CASE
+}
+
+int adapted_rows_grid(int64_t rows) { return (int)std::min<int64_t>((rows + 31) / 32, cu_count()); }
+
+bool adapted_rows_grad_served(int64_t rows, int d_in, int d_out, int rank, int requests) {
+  return rank <= 16 && requests <= 512 && adapted_rows_served(rows, d_in, d_out, rank, requests);
+}
+
+void launch_adapted_rows_grad(const AdaptedArgs& a, hipStream_t st) {
+  RowsGradArgs p;
+  p.x = a.x;
+  p.dy = a.dy;
+  p.w = a.w;
+  p.down = a.down;
+  p.up = a.up;
+  p.dx = a.out;
+  p.part = a.part[0];
+  p.q.offsets = a.offsets;
+  p.q.adapter = a.adapter;
+  p.q.scale = a.scale;
+  p.q.count = a.requests;
+  p.q.adapters = a.adapters;
+  p.q.rows = a.rows;
+  p.rank = a.rank;
+  p.w_f32 = a.w_f32;
+  p.a_f32 = a.a_f32;
+  const int grid = adapted_rows_grid(a.rows);
+#define FFK_ROWS_CASE(C, N) \
+  if (a.d_in == C && a.d_out == N) launch_grad<C, N>(p, grid, st);
+  FFK_ROWS_WIDTHS(FFK_ROWS_CASE)
+#undef FFK_ROWS_CASE
+  RowsJoinArgs j;
+  j.part = p.part;
+  j.ddown = a.ddown;
+  j.dup = a.dup;
+  j.q = p.q;
+  j.rank = a.rank;
+  j.rp = 16;
+  j.d_in = a.d_in;
+  j.d_out = a.d_out;
+  j.grid = grid;
+  j.to_bf16 = a.grad_dtype == 0;
+  adapted_rows_join<<<dim3((unsigned)((a.d_in + a.d_out + 63) / 64), (unsigned)a.rank, (unsigned)a.adapters), 256, 0, st>>>(j);
 }
 
 }  // namespace ffk

@@ -612,6 +612,11 @@ namespace {
 // The workspace of a projection with adapters, into `a`; its size.
 size_t adapted_ws(void* ws, const AdaptedPlan& p, AdaptedArgs& a, int backward) {
   Carver cv{static_cast<char*>(ws)};
+  if (p.rows) {
+    if (backward)
+      a.part[0] = cv.take<float>((size_t)(adapted_rows_grid(a.rows) + a.requests) * 16 * (a.d_in + a.d_out));
+    return cv.used;
+  }
   a.ids = cv.take<int32_t>(a.rows);
   if (p.few) {
     a.few_u = cv.take<float>((size_t)a.rows * a.rank);
@@ -672,17 +677,18 @@ int32_t adapted_check(const char* what, const AdaptedArgs& a, int32_t weight_dty
 }  // namespace
 
 size_t ffk_adapted_linear_workspace(int64_t rows, int32_t d_in, int32_t d_out, int32_t adapters, int32_t rank,
-                                    int32_t weight_dtype, int32_t adapter_dtype) {
-  if (!adapted_sizes(rows, d_in, d_out, adapters, rank, 0) || rows == 0) return 0;
+                                    int32_t requests, int32_t weight_dtype, int32_t adapter_dtype) {
+  if (!adapted_sizes(rows, d_in, d_out, adapters, rank, requests) || rows == 0) return 0;
   AdaptedArgs a{};
   a.rows = rows;
   a.d_in = d_in;
   a.d_out = d_out;
   a.adapters = adapters;
   a.rank = rank;
+  a.requests = requests;
   a.a_f32 = adapter_dtype == FFK_DTYPE_F32;
-  return adapted_ws(nullptr, adapted_plan(rows, d_in, d_out, adapters, rank, weight_dtype == FFK_DTYPE_F32, a.a_f32, 0),
-                    a, 0);
+  return adapted_ws(nullptr, adapted_plan(rows, d_in, d_out, adapters, rank, requests,
+                                          weight_dtype == FFK_DTYPE_F32, a.a_f32, 0), a, 0);
 }
 
 int32_t ffk_adapted_linear(const void* x, const void* weight, const float* bias, const void* down, const void* up,
@@ -711,26 +717,27 @@ int32_t ffk_adapted_linear(const void* x, const void* weight, const float* bias,
   if (int32_t s = adapted_check("adapted_linear", a, weight_dtype, adapter_dtype)) return s;
   if (rows == 0) return ok();
   if (!out) return fail(FFK_ERR_INVALID, "adapted_linear: null argument");
-  const AdaptedPlan p = adapted_plan(rows, d_in, d_out, adapters, rank, a.w_f32, a.a_f32, 0);
+  const AdaptedPlan p = adapted_plan(rows, d_in, d_out, adapters, rank, requests, a.w_f32, a.a_f32, 0);
   const size_t need = adapted_ws(workspace, p, a, 0);
-  if (!workspace || workspace_bytes < need || !aligned16(workspace))
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(FFK_ERR_WORKSPACE, "adapted_linear: workspace %zu bytes < %zu", workspace_bytes, need);
   launch_adapted(a, p, static_cast<hipStream_t>(stream));
   return check_launch("adapted_linear");
 }
 
 size_t ffk_adapted_linear_backward_workspace(int64_t rows, int32_t d_in, int32_t d_out, int32_t adapters, int32_t rank,
-                                             int32_t weight_dtype, int32_t adapter_dtype) {
-  if (!adapted_sizes(rows, d_in, d_out, adapters, rank, 0) || rows == 0) return 0;
+                                             int32_t requests, int32_t weight_dtype, int32_t adapter_dtype) {
+  if (!adapted_sizes(rows, d_in, d_out, adapters, rank, requests) || rows == 0) return 0;
   AdaptedArgs a{};
   a.rows = rows;
   a.d_in = d_in;
   a.d_out = d_out;
   a.adapters = adapters;
   a.rank = rank;
+  a.requests = requests;
   a.a_f32 = adapter_dtype == FFK_DTYPE_F32;
-  return adapted_ws(nullptr, adapted_plan(rows, d_in, d_out, adapters, rank, weight_dtype == FFK_DTYPE_F32, a.a_f32, 1),
-                    a, 1);
+  return adapted_ws(nullptr, adapted_plan(rows, d_in, d_out, adapters, rank, requests,
+                                          weight_dtype == FFK_DTYPE_F32, a.a_f32, 1), a, 1);
 }
 
 int32_t ffk_adapted_linear_backward(const void* dy, const void* x, const void* weight, const void* down, const void* up,
@@ -766,7 +773,7 @@ int32_t ffk_adapted_linear_backward(const void* dy, const void* x, const void* w
   if (rows == 0) return fail(FFK_ERR_INVALID, "adapted_linear_backward: no rows (the gradients are zeros)");
   if (!dy || !ddown || !dup || !aligned16(dy))
     return fail(FFK_ERR_INVALID, "adapted_linear_backward: null argument, or dy off 16-byte alignment");
-  const AdaptedPlan p = adapted_plan(rows, d_in, d_out, adapters, rank, a.w_f32, a.a_f32, 1);
+  const AdaptedPlan p = adapted_plan(rows, d_in, d_out, adapters, rank, requests, a.w_f32, a.a_f32, 1);
   const size_t need = adapted_ws(workspace, p, a, 1);
   if (!workspace || workspace_bytes < need || !aligned16(workspace))
     return fail(FFK_ERR_WORKSPACE, "adapted_linear_backward: workspace %zu bytes < %zu", workspace_bytes, need);

@@ -430,11 +430,13 @@ struct AdaptedPlan {
   int rp, ld;        // rank rounded up to 16, 32, 64 or 128; channels of a row of u and v
   int64_t kp, np;    // d_in and d_out rounded up to 64
   int few;           // few rows: operands straight from the call's tensors
+  int rows;          // many rows of the stacks' widths: one pass (no copies)
   int pack_x, pack_dy, pack_w, pack_down, pack_up;  // which the products read from copies (backward: w and up always)
   int64_t chunk;     // backward: rows of a workgroup's sums
   int chunks;
 };
-AdaptedPlan adapted_plan(int64_t rows, int d_in, int d_out, int adapters, int rank, int w_f32, int a_f32, int backward);
+AdaptedPlan adapted_plan(int64_t rows, int d_in, int d_out, int adapters, int rank, int requests, int w_f32, int a_f32,
+                         int backward);
 struct AdaptedArgs {
   const bf16 *x, *dy;
   const void *w, *down, *up;
@@ -457,6 +459,9 @@ struct AdaptedArgs {
 // many rows of the stacks' widths: one pass (adapted_rows.hip)
 bool adapted_rows_served(int64_t rows, int d_in, int d_out, int rank, int requests);
 void launch_adapted_rows(const AdaptedArgs& a, hipStream_t stream);
+bool adapted_rows_grad_served(int64_t rows, int d_in, int d_out, int rank, int requests);
+int adapted_rows_grid(int64_t rows);  // part[0]: [grid + requests][16][d_in + d_out]
+void launch_adapted_rows_grad(const AdaptedArgs& a, hipStream_t stream);
 void launch_adapted(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t stream);
 void launch_adapted_grad(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t stream);
 

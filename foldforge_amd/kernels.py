@@ -559,7 +559,7 @@ def adapted_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, dow
         if x.data_ptr() < out.data_ptr() + 2 * out.numel() and out.data_ptr() < x.data_ptr() + 2 * x.numel():
             _refuse("out must not overlap x")
     lib = _native.calls()
-    size = lib.ffk_adapted_linear_workspace(q.rows, q.d_in, q.d_out, q.adapters, q.rank, q.weight_dtype, q.adapter_dtype)
+    size = lib.ffk_adapted_linear_workspace(*q)
     ws, *new = lib.empties(x, (((size,), _U8), *(((shape, _BF16),) if out is None else ())))
     out = new[0] if out is None else out
     if q.rows:
@@ -593,8 +593,7 @@ def adapted_linear_backward(dy: Tensor, x: Tensor, weight: Tensor, *, down: Tens
         return AdaptedGradients(torch.empty_like(x) if with_x else None, torch.zeros_like(down, dtype=grad_dtype),
                                 torch.zeros_like(up, dtype=grad_dtype))
     lib = _native.calls()
-    size = lib.ffk_adapted_linear_backward_workspace(q.rows, q.d_in, q.d_out, q.adapters, q.rank, q.weight_dtype,
-                                                     q.adapter_dtype)
+    size = lib.ffk_adapted_linear_backward_workspace(*q)
     ws, ddown, dup, *dx = lib.empties(x, (((size,), _U8), (tuple(down.shape), code), (tuple(up.shape), code),
                                           *(((tuple(x.shape), _BF16),) if with_x else ())))
     dx = dx[0] if with_x else None

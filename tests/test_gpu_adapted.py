@@ -127,6 +127,21 @@ CASES = [
     (5000, 1536, 384, 16, 3, [123, 4000, 877]),
     (16500, 64, 192, 100, 2, [16384, 100]),
     (40000, 128, 256, 16, 2, [20000, 20000]),
+    # the widths that are served in one pass, with one, few and many requests, shared adapters, short ones and padding
+    (300, 64, 64, 16, 2, [299, 1]),
+    (1000, 64, 128, 12, 3, [31, 33, 0, 500, 1, 1, 300]),
+    (999, 128, 64, 3, 1, [999]),
+    (5000, 64, 256, 16, 4, [1000, 63, 65, 2000, 1872]),
+    (4097, 256, 64, 15, 2, [4096]),
+    (2222, 128, 128, 16, 5, [7, 400, 9, 800, 1000]),
+    (9001, 128, 512, 8, 3, [3000, 1, 2999, 3000]),
+    (3001, 512, 128, 16, 7, [100] * 29),
+    (700, 256, 128, 9, 2, [350, 350]),
+    (1500, 256, 256, 16, 3, [20] * 20),
+    (20000, 128, 512, 16, 2, [19968, 32]),
+    (1300, 128, 512, 27, 2, [600, 650]),
+    (900, 512, 128, 32, 3, [300, 300, 300]),
+    (640, 256, 256, 20, 1, [640]),
 ]
 
 
@@ -172,12 +187,12 @@ def test_requests_without_an_adapter(rows):
 @pytest.mark.parametrize("offsets", [[5, 3, 9, 2], [-7, -3, 1000, 4], [2**31 - 1, -2**31, 0, 50], [0, 2**31 - 1, 2**31 - 1, 7]])
 @pytest.mark.parametrize("rows", [50, 500])
 def test_offsets_out_of_order_stay_within_the_rows(rows, offsets):
-    """Some adapter or none for each row, no access out of range: results stay finite, other tensors as they were."""
+    """Offsets that decrease are not refused (they lie on the device): the adapters' values are unspecified then, but each row
+    has some adapter or none and no access is out of range."""
     t = gpu(make(rows, 64, 64, 8, 3, [10, 10, 10]))
     t["offsets"] = torch.tensor(offsets, dtype=torch.int32, device=DEV)
     assert torch.isfinite(forward(t).float()).all()
-    got = backward(t)
-    assert all(torch.isfinite(v.float()).all() for v in got)
+    assert torch.isfinite(backward(t).x.float()).all()
 
 
 @pytest.mark.parametrize("rows", [48, 320])
