@@ -30,16 +30,15 @@ __device__ __forceinline__ int adapter_at(const Requests& q, int r) {
 __device__ __forceinline__ int64_t request_end(const Requests& q, int r) {
   return r < q.count ? (int64_t)q.offsets[r + 1] : q.rows;  // (r = -1: the rows before the first request)
 }
-__device__ __forceinline__ RequestAt request_first(const Requests& q, int64_t row) {
-  int lo = -1, hi = q.count;  // the latest r with offsets[r] <= row
-  while (lo < hi) {
-    const int mid = lo + (hi - lo + 1) / 2;
-    if (q.offsets[mid] <= row)
-      lo = mid;
-    else
-      hi = mid - 1;
+__device__ __forceinline__ RequestAt request_first(const Requests& q, int64_t row, int lane) {
+  int before = 0;  // the offsets up to `row` (in order: of the first requests), counted by a wave
+#pragma unroll 4
+  for (int i = 0; i <= q.count; i += 64) {
+    const int at = i + lane < q.count ? i + lane : q.count;
+    before += __popcll(__ballot(q.offsets[at] <= row && i + lane <= q.count));
   }
-  return {lo, adapter_at(q, lo), request_end(q, lo)};
+  const int r = before - 1;
+  return {r, adapter_at(q, r), request_end(q, r)};
 }
 __device__ __forceinline__ void request_next(const Requests& q, int64_t row, RequestAt& at) {
   while (at.r < q.count && at.hi <= row) {
@@ -59,6 +58,33 @@ __device__ __forceinline__ bf16x8 operand8(const T* p) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) r[e] = (bf16)(float)v[e];
   return r;
+}
+
+// A row of `rank` numbers as an operand that goes with the thin product's accumulators as they lie: element e < 4 is number
+// 4 g + e, the others 16 on.
+template <int RB, typename T>
+__device__ __forceinline__ void rank_operand(const T* row, int rank, int g, bf16x8 (&to)[(RB + 1) / 2]) {
+  typedef T four __attribute__((__vector_size__(4 * sizeof(T)), aligned(sizeof(T))));
+#pragma unroll
+  for (int h = 0; h < RB + (RB & 1); ++h) {
+    const int j = 16 * h + 4 * g;
+    bf16x8& t = to[h >> 1];
+    const int e = 4 * (h & 1);
+    if (h >= RB) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) t[e + c] = (bf16)0.f;
+    } else if (rank % 4 == 0) {  // four numbers are all there or none
+      const four v = *reinterpret_cast<const four*>(row + (j < rank ? j : 0));
+#pragma unroll
+      for (int c = 0; c < 4; ++c) t[e + c] = j < rank ? (bf16)(float)v[c] : (bf16)0.f;
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const bf16 v = (bf16)(float)row[j + c < rank ? j + c : rank - 1];
+        t[e + c] = j + c < rank ? v : (bf16)0.f;
+      }
+    }
+  }
 }
 
 // f(a pointer of the type that p has).
@@ -83,10 +109,10 @@ struct RowsArgs {
   const float* bias;
   bf16* out;      // [rows][N]
   Requests q;
-  int rank, w_f32, a_f32;
+  int N, rank, w_f32, a_f32;
 };
 
-// How a tile of rows of C channels and N outputs are shared among 8 waves.
+// How a tile of rows of C channels and N of a workgroup's outputs are shared among 8 waves.
 template <int C, int N>
 struct RowsShape {
   static constexpr int TM = C <= 256 && N <= 256 ? 64 : 32;       // rows of a tile
@@ -103,12 +129,12 @@ struct RowsShape {
 // A tile of rows to LDS (off_row<C>), 1 KB a transfer: a wave's share. Rows behind the last are the last again.
 template <int C, int PER>
 __device__ __forceinline__ void rows_dma(const bf16* x, int64_t row0, int64_t rows, uint32_t dst, int wave, int lane) {
-  constexpr int P = C / 8, R = 512 / C;  // pieces of a row, rows of a transfer
+  constexpr int P = C / 8;  // pieces of a row
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
-    const int t = wave * PER + u, r = R * t + lane / P;
+    const int t = wave * PER + u, piece = 64 * t + lane, r = piece / P;
     const int64_t row = row0 + r < rows ? row0 + r : rows - 1;
-    dma16_at(x + row * C + 8 * ((lane % P) ^ swz<C>(r)), dst + 1024 * t);
+    dma16_at(x + row * C + 8 * ((piece % P) ^ swz<C>(r)), dst + 1024 * t);
   }
 }
 
@@ -134,18 +160,21 @@ __device__ __forceinline__ bf16x8 join_blocks(const f32x4& a, const f32x4& b) {
 }
 
 // out = x W^T + b + u B_a^T, u = s_a x A_a^T rounded to bf16. W and the adapters are read once a workgroup (the adapter's
-// again where it changes). The tiles in LDS: one in work, the others on their way. rank <= 16 RB. grid: consecutive tiles each;
-// block 512.
-template <int C, int N, int RB>
-__global__ __launch_bounds__(512, 2) void adapted_rows(const RowsArgs p) {
-  using S = RowsShape<C, N>;
+// again where it changes). The tiles in LDS: one in work, the others on their way. rank <= 16 RB. grid: ranges of consecutive
+// tiles, for each the slices of NS outputs (neighbours, so that a range's rows are fetched into one XCD's L2 once); block 512.
+template <int C, int NS, int RB>
+__global__ __launch_bounds__(512, 2) void adapted_rows(const RowsArgs p, int slices) {
+  using S = RowsShape<C, NS>;
   constexpr int PAIRS = (RB + 1) / 2, TM = S::TM, STAGES = C == 512 && RB == 2 ? 3 : S::STAGES;
   __shared__ __attribute__((aligned(16))) bf16 buf[STAGES][TM * C], af[RB * S::KS][64 * 8];
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t rows = p.q.rows, tiles = (rows + TM - 1) / TM;
-  const int64_t first = tiles * blockIdx.x / gridDim.x, last = tiles * (blockIdx.x + 1) / gridDim.x;
+  const int N = p.N, id = (int)xcd_remap(blockIdx.x, gridDim.x), range = id / slices, ranges = gridDim.x / slices;
+  const int64_t first = tiles * range / ranges, last = tiles * (range + 1) / ranges;
   const uint32_t lds = lds_addr(buf);
+  RequestAt at{p.q.count, -1, rows};
+  if (first < last) at = request_first(p.q, first * TM, lane);  // (ahead of the transfers, which it would wait for)
   auto fetch = [&](int64_t tile) __attribute__((always_inline)) {
     rows_dma<C, S::PER>(p.x, tile * TM, rows, lds + (uint32_t)((tile - first) % STAGES) * sizeof(buf[0]), wave,
                         fresh_lane());
@@ -154,14 +183,14 @@ __global__ __launch_bounds__(512, 2) void adapted_rows(const RowsArgs p) {
   for (int s = 0; s < STAGES - 1; ++s)
     if (first + s < last) fetch(first + s);
   // this wave's channels of W, and its rows of a tile
-  const int n0 = 16 * S::NB * (wave % S::NW), r0 = 16 * S::TT * (wave / S::NW);
+  const int n0 = NS * (id % slices) + 16 * S::NB * (wave % S::NW), r0 = 16 * S::TT * (wave / S::NW);
   bf16x8 w[S::NB][S::KS];
   typed(p.w, p.w_f32, [&](const auto* from) __attribute__((always_inline)) {
 #pragma unroll
     for (int b = 0; b < S::NB; ++b)
 #pragma unroll
       for (int k = 0; k < S::KS; ++k) {
-        w[b][k] = operand8(from + (n0 + 16 * b + i) * C + 32 * k + 8 * g);
+        w[b][k] = operand8(from + (int64_t)(n0 + 16 * b + i) * C + 32 * k + 8 * g);
         if (k % 8 == 7) __builtin_amdgcn_sched_barrier(0);  // (fp32: what is in flight has to fit the registers)
       }
   });
@@ -191,23 +220,12 @@ __global__ __launch_bounds__(512, 2) void adapted_rows(const RowsArgs p) {
     typed(p.up, p.a_f32, [&](const auto* from) __attribute__((always_inline)) {
 #pragma unroll
       for (int b = 0; b < S::NB; ++b) {
-        const auto* row = from + ((int64_t)a * N + n0 + 16 * b + i) * p.rank;
-#pragma unroll
-        for (int s = 0; s < PAIRS; ++s)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int j = 32 * s + 16 * (e >> 2) + 4 * g + (e & 3);
-            const bool is = j < p.rank && (RB > 1 || e < 4);
-            const bf16 v = (bf16)(float)row[is ? j : p.rank - 1];
-            bf[b][s][e] = is ? v : (bf16)0.f;
-          }
-        __builtin_amdgcn_sched_barrier(0);
+        rank_operand<RB>(from + ((int64_t)a * N + n0 + 16 * b + i) * p.rank, p.rank, g, bf[b]);
+        if (b % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       }
     });
     __syncthreads();
   };
-  RequestAt at{p.q.count, -1, rows};
-  if (first < last) at = request_first(p.q, first * TM);
   if (first + STAGES - 1 <= last)
     wait_vm_lds<(STAGES - 2) * S::PER>();
   else
@@ -305,18 +323,36 @@ __global__ __launch_bounds__(512, 2) void adapted_rows(const RowsArgs p) {
       if (end - row0 < TM && row0 + r0 + 16 * x + i >= rows) continue;
 #pragma unroll
       for (int b = 0; b < S::NB / 2; ++b)
-        __builtin_nontemporal_store(v[b], reinterpret_cast<bf16x8*>(to + 16 * x * N + 32 * b));
+        __builtin_nontemporal_store(v[b], reinterpret_cast<bf16x8*>(to + (int64_t)16 * x * N + 32 * b));
     }
     __syncthreads();
   }
 }
 
-template <int C, int N, int RB>
+template <int C, int NS, int RB>
 void launch_rows(const RowsArgs& p, hipStream_t st) {
-  const auto kernel = adapted_rows<C, N, RB>;
-  constexpr int TM = RowsShape<C, N>::TM;
+  const auto kernel = adapted_rows<C, NS, RB>;
+  constexpr int TM = RowsShape<C, NS>::TM;
   const int64_t resident = (int64_t)cu_count() * resident_blocks(reinterpret_cast<const void*>(kernel), 512, 0);
-  kernel<<<dim3((unsigned)std::min((p.q.rows + TM - 1) / TM, resident)), 512, 0, st>>>(p);
+  const int64_t slices = p.N / NS, ranges = std::min((p.q.rows + TM - 1) / TM, std::max<int64_t>(1, resident / slices));
+  kernel<<<dim3((unsigned)(ranges * slices)), 512, 0, st>>>(p, (int)slices);
+}
+
+template <int C, int NS>
+void launch_rank(const RowsArgs& p, hipStream_t st) {
+  p.rank <= 16 ? launch_rows<C, NS, 1>(p, st) : launch_rows<C, NS, 2>(p, st);
+}
+
+// The widest slice of the outputs that divides them and whose weights the registers hold.
+template <int C>
+void launch_width(const RowsArgs& p, hipStream_t st) {
+  if constexpr (C == 128)
+    if (p.N % 512 == 0) return launch_rank<C, 512>(p, st);
+  if constexpr (C <= 384)
+    if (p.N % 256 == 0) return launch_rank<C, 256>(p, st);
+  if constexpr (C <= 256)
+    if (p.N % 128 != 0) return launch_rank<C, 64>(p, st);
+  launch_rank<C, 128>(p, st);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -399,6 +435,8 @@ __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p
   const int64_t rows = p.q.rows, tiles = (rows + TM - 1) / TM;
   const int64_t first = tiles * blockIdx.x / gridDim.x, last = tiles * (blockIdx.x + 1) / gridDim.x;
   const uint32_t lds = lds_addr(buf);
+  RequestAt at{p.q.count, -1, rows};
+  if (first < last) at = request_first(p.q, first * TM, lane);  // (ahead of the transfers, which it would wait for)
   auto fetch = [&](int64_t tile) __attribute__((always_inline)) {
     const uint32_t dst = lds + (uint32_t)((tile - first) % STAGES) * sizeof(buf[0]);
     const int64_t row0 = tile * TM;
@@ -542,8 +580,6 @@ __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p
     }
   };
   clear();
-  RequestAt at{p.q.count, -1, rows};
-  if (first < last) at = request_first(p.q, first * TM);
   if (first + STAGES - 1 <= last)
     wait_vm_lds<(STAGES - 2) * S::PER>();
   else
@@ -753,14 +789,9 @@ __global__ __launch_bounds__(256) void adapted_rows_join(const RowsJoinArgs p) {
     static_cast<float*>(to)[at] = total;
 }
 
-// The widths served: the pair and MSA stacks' projections (d to d, 2 d, 4 d and back, d = 64, 128, 256).
+// The widths of the backward pass: the pair and MSA stacks' projections (d to d, 2 d, 4 d and back, d = 64, 128, 256).
 #define FFK_ROWS_WIDTHS(X) \
   X(64, 64) X(64, 128) X(128, 64) X(64, 256) X(256, 64) X(128, 128) X(128, 256) X(256, 128) X(128, 512) X(512, 128) X(256, 256)
-
-template <int C, int N>
-void launch_rank(const RowsArgs& p, hipStream_t st) {
-  p.rank <= 16 ? launch_rows<C, N, 1>(p, st) : launch_rows<C, N, 2>(p, st);
-}
 
 template <int CI, int CO>
 void launch_grad(const RowsGradArgs& p, int grid, hipStream_t st) {
@@ -773,10 +804,7 @@ void launch_grad(const RowsGradArgs& p, int grid, hipStream_t st) {
 }  // namespace
 
 bool adapted_rows_served(int64_t rows, int d_in, int d_out, int rank, int requests) {
-  bool width = false;
-#define FFK_ROWS_IS(C, N) width = width || (d_in == C && d_out == N);
-  FFK_ROWS_WIDTHS(FFK_ROWS_IS)
-#undef FFK_ROWS_IS
+  const bool width = d_in == 64 || d_in == 128 || d_in == 256 ? d_out % 64 == 0 : (d_in == 384 || d_in == 512) && d_out % 128 == 0;
   return width && rank <= 32 && rows > 256 && rows >= 64 * (int64_t)requests;
 }
 
@@ -794,19 +822,27 @@ void launch_adapted_rows(const AdaptedArgs& a, hipStream_t st) {
   p.q.count = a.requests;
   p.q.adapters = a.adapters;
   p.q.rows = a.rows;
+  p.N = a.d_out;
   p.rank = a.rank;
   p.w_f32 = a.w_f32;
   p.a_f32 = a.a_f32;
-#define FFK_ROWS_CASE(C, N) \
-  if (a.d_in == C && a.d_out == N) launch_rank<C, N>(p, st);
-  FFK_ROWS_WIDTHS(FFK_ROWS_CASE)
-#undef FFK_ROWS_CASE
+  switch (a.d_in) {
+    case 64: return launch_width<64>(p, st);
+    case 128: return launch_width<128>(p, st);
+    case 256: return launch_width<256>(p, st);
+    case 384: return launch_width<384>(p, st);
+    default: return launch_width<512>(p, st);
+  }
 }
 
 int adapted_rows_grid(int64_t rows) { return (int)std::min<int64_t>((rows + 31) / 32, cu_count()); }
 
 bool adapted_rows_grad_served(int64_t rows, int d_in, int d_out, int rank, int requests) {
-  return rank <= 16 && requests <= 512 && adapted_rows_served(rows, d_in, d_out, rank, requests);
+  bool width = false;
+#define FFK_ROWS_IS(C, N) width = width || (d_in == C && d_out == N);
+  FFK_ROWS_WIDTHS(FFK_ROWS_IS)
+#undef FFK_ROWS_IS
+  return width && rank <= 16 && rows > 256 && requests <= 512 && rows >= 64 * (int64_t)requests;
 }
 
 void launch_adapted_rows_grad(const AdaptedArgs& a, hipStream_t st) {
