@@ -140,7 +140,7 @@ struct ThinArgs {
 // grid (ceil(rows / (64 / KS)), share, jobs); block 256. KEEP: u in three parts (rows of parts_ld), else rounded (of RP).
 template <int RP, int PARTS, bool KEEP, int KS>
 __global__ __launch_bounds__(256) void adapted_thin(const ThinArgs p) {
-  constexpr int N = RP / 16, TM = 64 / KS, U = N * PARTS <= 3 ? 4 : N * PARTS <= 6 ? 2 : 1;  // steps of k in flight
+  constexpr int N = RP / 16, TM = 64 / KS, U = N * PARTS <= 2 ? 6 : N * PARTS <= 4 ? 4 : 2;  // steps of k in flight
   constexpr int ld = KEEP ? parts_ld(RP) : RP;
   __shared__ int id[64], start[64], before;
   __shared__ f32x4 red[KS == 1 ? 1 : 4][N][64];
@@ -198,6 +198,8 @@ __global__ __launch_bounds__(256) void adapted_thin(const ThinArgs p) {
 #pragma unroll
       for (int k = 0; k < PARTS; ++k) m[k][n] = j.mat[k] + ((int64_t)a * j.mat_rows + r) * j.K + 8 * g;
     }
+    const float s = scale_of(p.q, a);
+    // so many steps of k, all their operands asked for before the first product
     const auto steps = [&](int k, auto count) __attribute__((always_inline)) {
       constexpr int C = decltype(count)::value;
       bf16x8 xf[C], mf[C][PARTS][N];
@@ -209,6 +211,7 @@ __global__ __launch_bounds__(256) void adapted_thin(const ThinArgs p) {
 #pragma unroll
           for (int n = 0; n < N; ++n) mf[c][q][n] = ld8(m[q][n] + k + 32 * KS * c);
       }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -218,9 +221,14 @@ __global__ __launch_bounds__(256) void adapted_thin(const ThinArgs p) {
     };
     int k = KS == 1 ? 0 : 32 * wave;
     for (; k + 32 * KS * (U - 1) < j.K; k += 32 * KS * U) steps(k, std::integral_constant<int, U>());
-    if constexpr (U > 1)
-      for (; k < j.K; k += 32 * KS) steps(k, std::integral_constant<int, 1>());
-    const float s = scale_of(p.q, a);
+    switch ((j.K - k + 32 * KS - 1) / (32 * KS)) {
+      case 5: if constexpr (U > 5) steps(k, std::integral_constant<int, 5>()); break;
+      case 4: if constexpr (U > 4) steps(k, std::integral_constant<int, 4>()); break;
+      case 3: if constexpr (U > 3) steps(k, std::integral_constant<int, 3>()); break;
+      case 2: if constexpr (U > 2) steps(k, std::integral_constant<int, 2>()); break;
+      case 1: if constexpr (U > 1) steps(k, std::integral_constant<int, 1>()); break;
+      default: break;
+    }
     if constexpr (KS == 1) {
       if (is) {
 #pragma unroll
@@ -279,6 +287,12 @@ __global__ __launch_bounds__(256, 2) void adapted_product(const ProductArgs p) {
   for (int c = 0; c < WT; ++c)
 #pragma unroll
     for (int t = 0; t < XT; ++t) acc[c][t] = zero16();
+  int ids[XT];  // (asked for ahead of the transfers)
+#pragma unroll
+  for (int x = 0; x < XT; ++x) {
+    const int64_t row = m0 + wm * (TM / 2) + 32 * x + li;
+    ids[x] = p.ids[row < p.rows ? row : p.rows - 1];
+  }
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s)
     if (s < steps) fetch(s);
@@ -314,7 +328,7 @@ __global__ __launch_bounds__(256, 2) void adapted_product(const ProductArgs p) {
   for (int x = 0; x < XT; ++x) {
     const int64_t row = m0 + wm * (TM / 2) + 32 * x + li;
     const bool real = row < p.rows;
-    const int mine = real ? p.ids[row] : -1;
+    const int mine = real ? ids[x] : -1;
     const bf16* u = p.u + (real ? row : p.rows - 1) * p.ld + 8 * g;
     uint64_t todo = __ballot(mine >= 0) & 0xffffffffu;
     while (todo != 0) {
@@ -402,10 +416,19 @@ __global__ __launch_bounds__(256) void adapted_grad(const GradArgs p) {
   const int c0 = 64 * ((int)blockIdx.x - (which ? p.job[0].tiles : 0)), a = blockIdx.y;
   const int64_t begin = blockIdx.z * p.chunk, end = begin + p.chunk < p.rows ? begin + p.chunk : p.rows;
   const int tiles = (int)((end - begin + 63) / 64);
-  for (int t = wave; t < tiles; t += 4) {
-    const int64_t row = begin + 64 * t + lane;
-    const uint64_t m = __ballot(row < end && p.ids[row] == a);
-    if (lane == 0) has[t] = m;
+  for (int t0 = wave; t0 < tiles; t0 += 4 * 8) {  // eight tiles' ids in flight
+    int id[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int64_t row = begin + 64 * (t0 + 4 * u) + lane;
+      id[u] = p.ids[row < end ? row : end - 1];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int t = t0 + 4 * u;
+      const uint64_t m = __ballot(begin + 64 * t + lane < end && id[u] == a);
+      if (lane == 0 && t < tiles) has[t] = m;
+    }
   }
   __syncthreads();
   if (wave == 0) {
@@ -502,16 +525,24 @@ struct JoinArgs {
   int chunks, rank, to_bf16;
 };
 
-// The chunks' sums in order. grid: ceil of both jobs' counts / 256; block 256.
+// The chunks' sums: 64 values a workgroup, four groups of chunks beside each other, joined in order. grid: ceil of both jobs'
+// counts / 64; block 256.
 __global__ __launch_bounds__(256) void adapted_join(const JoinArgs p) {
-  int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t head = (p.job[0].count + 255) / 256 * 256;
-  const int which = i >= head ? 1 : 0;
+  __shared__ float sum[4][64];
+  int64_t i = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  const int64_t head = (p.job[0].count + 63) / 64 * 64;
+  const int which = (int64_t)blockIdx.x * 64 >= head ? 1 : 0;
   const JoinJob& j = p.job[which];
   if (which) i -= head;
-  if (i >= j.count) return;
   float v = 0.f;
-  for (int k = 0; k < p.chunks; ++k) v += j.part[k * j.count + i];
+  if (i < j.count) {
+#pragma unroll 8
+    for (int k = threadIdx.x >> 6; k < p.chunks; k += 4) v += j.part[k * j.count + i];
+  }
+  sum[threadIdx.x >> 6][threadIdx.x & 63] = v;
+  __syncthreads();
+  if (threadIdx.x >= 64 || i >= j.count) return;
+  v = (sum[0][threadIdx.x] + sum[1][threadIdx.x]) + (sum[2][threadIdx.x] + sum[3][threadIdx.x]);
   const int64_t c = i % j.cols, row = i / j.cols % p.rank, a = i / j.cols / p.rank;
   const int64_t at = a * p.rank * j.cols + row * j.sj + c * j.sc;
   if (p.to_bf16)
@@ -634,6 +665,7 @@ __global__ __launch_bounds__(512) void adapted_few(const FewArgs p) {
 #pragma unroll
       for (int t = 0; t < RT; ++t) xf[u][t].load(x[t], k + 256 * u + 8 * g, p.K);
     }
+    __builtin_amdgcn_sched_barrier(0);  // (all of them asked for before the first product)
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -770,8 +802,9 @@ AdaptedPlan adapted_plan(int64_t rows, int d_in, int d_out, int adapters, int ra
     p.pack_dy = d_out % 64 != 0;
     p.pack_down = a_f32 || d_in % 64 != 0;
     const int64_t tiles = (p.kp + p.np) / 64 * adapters;
-    // some four workgroups a CU, of chunks of 256 rows at least
-    int64_t chunks = std::max<int64_t>(1, std::min<int64_t>((1024 + tiles - 1) / tiles, (rows + 255) / 256));
+    // some four workgroups a CU, of 512 of their adapter's rows at least
+    const int64_t used = std::max(1, std::min(adapters, requests));
+    const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>((1024 + tiles - 1) / tiles, rows / (512 * used)));
     p.chunk = std::min<int64_t>(up64((rows + chunks - 1) / chunks), 64 * kMostGradTiles);
     p.chunks = (int)((rows + p.chunk - 1) / p.chunk);
   } else {
@@ -910,7 +943,7 @@ void launch_adapted_grad(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t
     e.job[i].sc = sc[i];
     e.job[i].count = count;
     e.job[i].cols = j.cols;
-    counts += (count + 255) / 256;
+    counts += (count + 63) / 64;
   }
   d.ids = a.ids;
   d.rows = a.rows;

@@ -226,6 +226,7 @@ __global__ __launch_bounds__(512, 2) void adapted_rows(const RowsArgs p, int sli
     });
     __syncthreads();
   };
+  if (at.a >= 0) load(at.a);
   if (first + STAGES - 1 <= last)
     wait_vm_lds<(STAGES - 2) * S::PER>();
   else

@@ -17,6 +17,10 @@ struct Requests {
   int64_t rows;
 };
 
-__device__ __forceinline__ float scale_of(const Requests& q, int a) { return q.scale ? q.scale[a] : 1.f; }
+// (read from some address in any case: a branch would wait for the value)
+__device__ __forceinline__ float scale_of(const Requests& q, int a) {
+  const float v = *(q.scale ? q.scale + a : reinterpret_cast<const float*>(q.offsets));
+  return q.scale ? v : 1.f;
+}
 
 }  // namespace ffk
