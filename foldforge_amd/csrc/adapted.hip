@@ -26,26 +26,30 @@ namespace {
 // ---------------------------------------------------------------------------------------------------------
 // which adapter a row has
 
-// id[i], i < 64: the adapter of row row0 + i, -1 for none (and behind the last row). All threads of the workgroup (of NT);
-// start and before are its scratch. One pass over the offsets: how many begin at or before the first row, and which begin at
-// each of the others; then the latest request that begins at or before each row. Offsets out of order give some adapter or
-// none, never an access out of range.
-template <int NT>
-__device__ __forceinline__ void tile_ids(const Requests& q, int64_t row0, int* id, int* start, int* before) {
+// id[i], i < 64: the adapter of row row0 + i, -1 for none (and behind the last row). All threads of the workgroup; start is
+// scratch. The first wave passes over the offsets once: how many begin at or before the first row, and which begin at each of
+// the others; then the latest request that begins at or before each row. Offsets out of order give some adapter or none, never
+// an access out of range.
+__device__ __forceinline__ void tile_ids(const Requests& q, int64_t row0, int* id, int* start) {
   const int tid = threadIdx.x;
-  if (tid < 64) start[tid] = -1;
-  if (tid == 0) *before = 0;
-  __syncthreads();
-  for (int i = tid; i <= q.count; i += NT) {
-    const int64_t at = (int64_t)q.offsets[i] - row0;
-    if (at <= 0)
-      atomicMax(before, i + 1);  // (in order: the number of such offsets)
-    else if (at < 64)
-      atomicMax(&start[at], i);
-  }
-  __syncthreads();
   if (tid < 64) {
-    int r = tid == 0 ? *before - 1 : start[tid];
+    start[tid] = -1;
+    __builtin_amdgcn_wave_barrier();  // (the wave's own: LDS operations complete in order)
+    int before = 0;
+    for (int i0 = tid; i0 - tid <= q.count; i0 += 256) {
+      int offset[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) offset[u] = q.offsets[i0 + 64 * u < q.count ? i0 + 64 * u : q.count];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + 64 * u;
+        const int64_t at = offset[u] - row0;
+        before += __popcll(__ballot(i <= q.count && at <= 0));
+        if (i <= q.count && at > 0 && at < 64) atomicMax(&start[at], i);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+    int r = tid == 0 ? before - 1 : start[tid];
 #pragma unroll
     for (int m = 1; m < 64; m *= 2) {
       const int o = __shfl_up(r, m, 64);
@@ -58,28 +62,80 @@ __device__ __forceinline__ void tile_ids(const Requests& q, int64_t row0, int* i
   __syncthreads();
 }
 
+// Eight values at p[k ..], those from n on read as zeros. EVEN: n a multiple of 8 (the values lie in one 16- or 32-byte
+// piece or none do): no branch, so that loads can run ahead of each other.
+template <typename T, bool EVEN>
+struct Raw8 {
+  typedef T vec __attribute__((__vector_size__(8 * sizeof(T)), aligned(sizeof(T))));
+  vec v;
+  bool in;
+  __device__ __forceinline__ void load(const T* p, int k, int n) {
+    in = k < n;
+    if constexpr (EVEN) {
+      v = *reinterpret_cast<const vec*>(p + (in ? k : 0));
+    } else if (k + 8 <= n) {
+      v = *reinterpret_cast<const vec*>(p + k);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = k + e < n ? p[k + e] : (T)0.f;
+    }
+  }
+  // the same from a column: p[(k ..) * stride]
+  __device__ __forceinline__ void load_column(const T* p, int k, int n, int stride) {
+    in = true;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const T t = p[(int64_t)(k + e < n ? k + e : n - 1) * stride];
+      v[e] = k + e < n ? t : (T)0.f;
+    }
+  }
+  __device__ __forceinline__ float operator[](int e) const { return in ? (float)v[e] : 0.f; }
+  __device__ __forceinline__ bf16x8 operand() const {
+    bf16x8 o;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = in ? (bf16)(float)v[e] : (bf16)0.f;
+    return o;
+  }
+  // in so many bf16 that add up to it
+  template <int PARTS>
+  __device__ __forceinline__ void parts(bf16x8 (&o)[PARTS]) const {
+    if constexpr (PARTS == 1) {
+      o[0] = operand();
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float t = in ? (float)v[e] : 0.f;
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q) {
+          o[q][e] = (bf16)t;
+          t -= (float)o[q][e];
+        }
+      }
+    }
+  }
+};
+
 // ---------------------------------------------------------------------------------------------------------
 // operands in the products' orders
 
-// dst [batch][out_rows][out_cols] bf16 from src [batch][rows][cols] (turn: transposed), zeros outside; with mid and lo in
-// three parts that add up to the fp32 value.
+// dst [batch][out_rows][out_cols] bf16 from src [batch][rows][cols] (turn: transposed), zeros outside.
 struct PackJob {
   const void* src;
-  bf16 *hi, *mid, *lo;  // mid and lo may be null
+  bf16* dst;
   int64_t rows, cols, out_rows, out_cols, tiles;  // tiles: of 32 x 32, all batches
   int f32, turn;
 };
-constexpr int kPackJobs = 6;
+constexpr int kPackJobs = 5;
 struct PackArgs {
   PackJob job[kPackJobs];
   int jobs;
+  int64_t tiles;
 };
 
-// The 32 x 32 tiles of the destinations, the jobs' one after the other. block 256.
-__global__ __launch_bounds__(256) void adapted_pack(const PackArgs p, int64_t tiles) {
-  __shared__ float t[32][33];
+// The 32 x 32 tiles of the destinations, the jobs' one after the other, from tile `first` on in steps.
+__device__ __forceinline__ void pack_tiles(const PackArgs& p, int64_t first, int64_t step, float (&t)[32][33]) {
   const int col = threadIdx.x & 31, row = threadIdx.x >> 5;
-  for (int64_t at = blockIdx.x; at < tiles; at += gridDim.x) {
+  for (int64_t at = first; at < p.tiles; at += step) {
     int64_t tile = at;
     int which = 0;
     while (which + 1 < p.jobs && tile >= p.job[which].tiles) tile -= p.job[which++].tiles;
@@ -104,14 +160,7 @@ __global__ __launch_bounds__(256) void adapted_pack(const PackArgs p, int64_t ti
       if (r >= j.out_rows || c >= j.out_cols) continue;
       const float v = j.turn ? t[col][row + 8 * i] : t[row + 8 * i][col];
       const int64_t to = (batch * j.out_rows + r) * j.out_cols + c;
-      const bf16 h = (bf16)v;
-      j.hi[to] = h;
-      if (j.mid) {
-        const float left = v - (float)h;
-        const bf16 m = (bf16)left;
-        j.mid[to] = m;
-        j.lo[to] = (bf16)(left - (float)m);
-      }
+      j.dst[to] = (bf16)v;
     }
     __syncthreads();
   }
@@ -124,37 +173,45 @@ __global__ __launch_bounds__(256) void adapted_pack(const PackArgs p, int64_t ti
 constexpr int parts_ld(int rp) { return rp == 16 ? 64 : rp == 32 ? 128 : 3 * rp; }
 
 struct ThinJob {
-  const bf16 *x, *mat[3];  // x [rows][K], the adapters' matrices [adapters][mat_rows][K] (PARTS = 3: in three parts)
-  bf16* u;                 // [rows][ld]: s_a (matrix x) in RP channels, zeros from `rank` on
-  int K, mat_rows;         // K a multiple of 64
+  const bf16* x;    // [rows][K]
+  const void* mat;  // the adapters' [adapters][rank][K], or (turned) [adapters][K][rank]
+  bf16* u;          // [rows][ld]: s_a (matrix x) in RP channels, zeros from `rank` on
+  int K, turned;
 };
 struct ThinArgs {
   ThinJob job[2];
   Requests q;
-  int32_t* ids;  // [rows], written by the first job's first workgroups
+  int32_t* ids;  // [rows], written with the first job
   int rank;
+  int64_t row_blocks;
+  int share, jobs;  // workgroups: row_blocks x share x jobs
+};
+
+struct ThinLds {
+  int id[64], start[64];
 };
 
 // 64 / KS rows a workgroup, of 4 waves: KS = 1, 16 rows a wave; KS = 4, all 16 rows, a quarter of K a wave (few rows: more
-// workgroups). Each adapter of the rows in turn, gridDim.y workgroups share them; a lane holds a token and 4 channels.
-// grid (ceil(rows / (64 / KS)), share, jobs); block 256. KEEP: u in three parts (rows of parts_ld), else rounded (of RP).
-template <int RP, int PARTS, bool KEEP, int KS>
-__global__ __launch_bounds__(256) void adapted_thin(const ThinArgs p) {
-  constexpr int N = RP / 16, TM = 64 / KS, U = N * PARTS <= 2 ? 6 : N * PARTS <= 4 ? 4 : 2;  // steps of k in flight
+// workgroups). Each adapter of the rows in turn, `share` workgroups share them; a lane holds a token and 4 channels. Operands
+// straight from the call's tensors. EVEN: K a multiple of 8. KEEP: u in three parts (rows of parts_ld; fp32 adapters in three
+// parts as well), else rounded (rows of RP).
+template <typename TA, int RP, bool KEEP, int KS, bool EVEN>
+__device__ __forceinline__ void thin_rows(const ThinArgs& p, int64_t block, ThinLds& lds, f32x4 (*red)[RP / 16][64]) {
+  constexpr int PARTS = KEEP && sizeof(TA) == 4 ? 3 : 1;
+  constexpr int N = RP / 16, TM = 64 / KS, U = N * PARTS <= 3 ? 6 : N * PARTS <= 6 ? 2 : 1;  // steps of k in flight
   constexpr int ld = KEEP ? parts_ld(RP) : RP;
-  __shared__ int id[64], start[64], before;
-  __shared__ f32x4 red[KS == 1 ? 1 : 4][N][64];
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row0 = (int64_t)blockIdx.x * TM;
-  const ThinJob& j = p.job[blockIdx.z];
-  tile_ids<256>(p.q, row0, id, start, &before);
-  if (blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x < TM && row0 + threadIdx.x < p.q.rows)
-    p.ids[row0 + threadIdx.x] = id[threadIdx.x];
+  const int64_t row0 = block % p.row_blocks * TM;
+  const int shared = (int)(block / p.row_blocks % p.share), which = (int)(block / p.row_blocks / p.share);
+  const ThinJob& j = p.job[which];
+  tile_ids(p.q, row0, lds.id, lds.start);
+  if (shared == 0 && which == 0 && threadIdx.x < TM && row0 + threadIdx.x < p.q.rows)
+    p.ids[row0 + threadIdx.x] = lds.id[threadIdx.x];
   const int first = KS == 1 ? 16 * wave : 0;  // of the wave's rows
   const int64_t row = row0 + first + i;
-  const int mine = id[first + i];
-  const bf16* x = j.x + (row < p.q.rows ? row : p.q.rows - 1) * j.K + 8 * g;
+  const int mine = lds.id[first + i];
+  const bf16* x = j.x + (row < p.q.rows ? row : p.q.rows - 1) * j.K;
   auto store = [&](int n, const f32x4& v) __attribute__((always_inline)) {
     bf16x4 part[3];
 #pragma unroll
@@ -178,7 +235,7 @@ __global__ __launch_bounds__(256) void adapted_thin(const ThinArgs p) {
     }
   };
   const f32x4 none = {0.f, 0.f, 0.f, 0.f};
-  if (blockIdx.y == 0 && mine < 0 && row < p.q.rows && (KS == 1 || wave == 0)) {
+  if (shared == 0 && mine < 0 && row < p.q.rows && (KS == 1 || wave == 0)) {
 #pragma unroll
     for (int n = 0; n < N; ++n) store(n, none);
   }
@@ -187,48 +244,57 @@ __global__ __launch_bounds__(256) void adapted_thin(const ThinArgs p) {
     const int a = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
     const bool is = mine == a;
     todo &= ~__ballot(is);
-    if (turn % gridDim.y != blockIdx.y) continue;
+    if (turn % p.share != shared) continue;
     f32x4 acc[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) acc[n] = none;
-    const bf16* m[PARTS][N];
+    const TA* m[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int r = 16 * n + i < j.mat_rows ? 16 * n + i : j.mat_rows - 1;
-#pragma unroll
-      for (int k = 0; k < PARTS; ++k) m[k][n] = j.mat[k] + ((int64_t)a * j.mat_rows + r) * j.K + 8 * g;
+      const int r = 16 * n + i < p.rank ? 16 * n + i : p.rank - 1;
+      m[n] = static_cast<const TA*>(j.mat) + (int64_t)a * p.rank * j.K + (j.turned ? r : (int64_t)r * j.K);
     }
     const float s = scale_of(p.q, a);
     // so many steps of k, all their operands asked for before the first product
     const auto steps = [&](int k, auto count) __attribute__((always_inline)) {
       constexpr int C = decltype(count)::value;
-      bf16x8 xf[C], mf[C][PARTS][N];
+      Raw8<bf16, EVEN> xf[C];
+      Raw8<TA, EVEN> mf[C][N];
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        xf[c] = ld8(x + k + 32 * KS * c);
+      for (int c = 0; c < C; ++c) xf[c].load(x, k + 32 * KS * c + 8 * g, j.K);
+      if (j.turned) {
 #pragma unroll
-        for (int q = 0; q < PARTS; ++q)
+        for (int c = 0; c < C; ++c)
 #pragma unroll
-          for (int n = 0; n < N; ++n) mf[c][q][n] = ld8(m[q][n] + k + 32 * KS * c);
+          for (int n = 0; n < N; ++n) mf[c][n].load_column(m[n], k + 32 * KS * c + 8 * g, j.K, p.rank);
+      } else {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int n = 0; n < N; ++n) mf[c][n].load(m[n], k + 32 * KS * c + 8 * g, j.K);
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int c = 0; c < C; ++c)
+      for (int c = 0; c < C; ++c) {
+        const bf16x8 xv = xf[c].operand();
 #pragma unroll
-        for (int q = 0; q < PARTS; ++q)
+        for (int n = 0; n < N; ++n) {
+          bf16x8 mv[PARTS];
+          mf[c][n].template parts<PARTS>(mv);
 #pragma unroll
-          for (int n = 0; n < N; ++n) acc[n] = mfma16(mf[c][q][n], xf[c], acc[n]);
+          for (int q = 0; q < PARTS; ++q) acc[n] = mfma16(mv[q], xv, acc[n]);
+        }
+      }
     };
     int k = KS == 1 ? 0 : 32 * wave;
     for (; k + 32 * KS * (U - 1) < j.K; k += 32 * KS * U) steps(k, std::integral_constant<int, U>());
-    switch ((j.K - k + 32 * KS - 1) / (32 * KS)) {
-      case 5: if constexpr (U > 5) steps(k, std::integral_constant<int, 5>()); break;
-      case 4: if constexpr (U > 4) steps(k, std::integral_constant<int, 4>()); break;
-      case 3: if constexpr (U > 3) steps(k, std::integral_constant<int, 3>()); break;
-      case 2: if constexpr (U > 2) steps(k, std::integral_constant<int, 2>()); break;
-      case 1: if constexpr (U > 1) steps(k, std::integral_constant<int, 1>()); break;
-      default: break;
-    }
+    if constexpr (U > 3)
+      if (k + 32 * KS * 2 < j.K) {
+        steps(k, std::integral_constant<int, 3>());
+        k += 32 * KS * 3;
+      }
+    if constexpr (U > 1)
+      for (; k < j.K; k += 32 * KS) steps(k, std::integral_constant<int, 1>());
     if constexpr (KS == 1) {
       if (is) {
 #pragma unroll
@@ -244,6 +310,24 @@ __global__ __launch_bounds__(256) void adapted_thin(const ThinArgs p) {
         if (n % 4 == wave && is) store(n, (red[0][n][lane] + red[1][n][lane] + (red[2][n][lane] + red[3][n][lane])) * s);
     }
   }
+}
+
+// What a call makes first, in one launch: the thin products, and (the workgroups behind theirs) the operands that the wide
+// product reads from copies. block 256.
+template <typename TA, int RP, bool KEEP, int KS, bool EVEN>
+__global__ __launch_bounds__(256) void adapted_prepare(const ThinArgs t, const PackArgs p) {
+  __shared__ union {
+    struct {
+      ThinLds lds;
+      f32x4 red[KS == 1 ? 1 : 4][RP / 16][64];
+    } thin;
+    float tile[32][33];
+  } s;
+  const int64_t blocks = t.row_blocks * t.share * t.jobs;
+  if (blockIdx.x < blocks)
+    thin_rows<TA, RP, KEEP, KS, EVEN>(t, blockIdx.x, s.thin.lds, s.thin.red);
+  else
+    pack_tiles(p, blockIdx.x - blocks, gridDim.x - blocks, s.tile);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -262,14 +346,14 @@ struct ProductArgs {
 // out = x W^T + u B_a^T + bias in TM rows x TN channels a workgroup, a quarter of them a wave: weight rows x token rows, so a
 // lane holds a token. K in steps of 64 through STAGES buffers by LDS DMA. The adapters of a wave's 32 tokens one after the
 // other at the end, each added to the lanes that have it. grid: m tiles x n tiles, the n tiles of an m tile neighbours (they
-// share its rows in an XCD's L2); block 256.
+// share its rows in an XCD's L2).
 template <int TM, int TN, int STAGES>
-__global__ __launch_bounds__(256, 2) void adapted_product(const ProductArgs p) {
+__device__ __forceinline__ void product_tile(const ProductArgs& p, uint32_t block, uint32_t blocks,
+                                             bf16 (&buf)[STAGES][TM / 64 + TN / 64][64 * 64]) {
   constexpr int XT = TM / 64, WT = TN / 64, PER = 2 * (XT + WT);  // 64 x 64 tiles a step, transfers of a wave
-  __shared__ __attribute__((aligned(16))) bf16 buf[STAGES][XT + WT][64 * 64];
   const int lane = threadIdx.x & 63, g = lane >> 5, li = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
-  const uint32_t id = xcd_remap(blockIdx.x, gridDim.x);
+  const uint32_t id = xcd_remap(block, blocks);
   const int64_t m0 = (int64_t)(id / p.n_tiles) * TM;
   const int n0 = (int)(id % p.n_tiles) * TN;
   const int steps = p.K / 64;
@@ -380,6 +464,12 @@ __global__ __launch_bounds__(256, 2) void adapted_product(const ProductArgs p) {
   }
 }
 
+template <int TM, int TN, int STAGES>
+__global__ __launch_bounds__(256, 2) void adapted_product(const ProductArgs p) {
+  __shared__ __attribute__((aligned(16))) bf16 buf[STAGES][TM / 64 + TN / 64][64 * 64];
+  product_tile<TM, TN, STAGES>(p, blockIdx.x, gridDim.x, buf);
+}
+
 // ---------------------------------------------------------------------------------------------------------
 // the adapters' gradients
 
@@ -393,7 +483,7 @@ struct GradArgs {
   GradJob job[2];
   const int32_t* ids;
   int64_t rows, chunk, chunk_stride[2];  // rows of a chunk: a multiple of 64, at most 64 * kMostGradTiles
-  int rank, to_bf16;
+  int rank, to_bf16, adapters;
 };
 constexpr int kMostGradTiles = 256;
 
@@ -401,20 +491,31 @@ constexpr int kMostGradTiles = 256;
 // row of the adapter's, in order, through three buffers by LDS DMA; the rows of others in them are zeroed there. A wave takes
 // 16 of a tile's rows (k of the product; both operands turned as they are read), the waves' sums meet at the end in a fixed
 // order. The parts are products of their own into one sum (RP = 16: high and middle ones the 32 rows of one, low ones and
-// zeros of another). grid (both jobs' tiles, adapters, chunks); block 256.
+// zeros of another). Workgroups: both jobs' tiles x adapters x chunks.
 template <int RP>
-__global__ __launch_bounds__(256) void adapted_grad(const GradArgs p) {
+struct GradLds {
+  static constexpr int VT = parts_ld(RP) / 64, STAGES = RP == 128 ? 2 : 3;
+  __attribute__((aligned(16))) bf16 buf[STAGES][1 + VT][64 * 64];
+  uint64_t has[kMostGradTiles];  // which rows of a tile are the adapter's
+  int list[kMostGradTiles], listed;
+};
+template <int RP>
+__device__ __forceinline__ void grad_tile(const GradArgs& p, int64_t block, GradLds<RP>& s_) {
   constexpr int ld = parts_ld(RP), VT = ld / 64, JB = RP <= 32 ? 1 : RP / 32, BLOCKS = RP == 16 ? 2 : 3 * RP / 32;
-  constexpr int STAGES = RP == 128 ? 2 : 3, PER = 2 * (1 + VT);
-  __shared__ __attribute__((aligned(16))) bf16 buf[STAGES][1 + VT][64 * 64];
-  __shared__ uint64_t has[kMostGradTiles];  // which rows of a tile are the adapter's
-  __shared__ int list[kMostGradTiles], listed;
+  constexpr int STAGES = GradLds<RP>::STAGES, PER = 2 * (1 + VT);
+  auto& buf = s_.buf;
+  auto& has = s_.has;
+  auto& list = s_.list;
+  int& listed = s_.listed;
+  const int across = p.job[0].tiles + p.job[1].tiles, tile = (int)(block % across);
+  const int a = (int)(block / across % p.adapters);
+  const int64_t chunk = block / across / p.adapters;
   const int lane = threadIdx.x & 63, g = lane >> 5, li = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int which = (int)blockIdx.x >= p.job[0].tiles ? 1 : 0;
+  const int which = tile >= p.job[0].tiles ? 1 : 0;
   const GradJob& j = p.job[which];
-  const int c0 = 64 * ((int)blockIdx.x - (which ? p.job[0].tiles : 0)), a = blockIdx.y;
-  const int64_t begin = blockIdx.z * p.chunk, end = begin + p.chunk < p.rows ? begin + p.chunk : p.rows;
+  const int c0 = 64 * (tile - (which ? p.job[0].tiles : 0));
+  const int64_t begin = chunk * p.chunk, end = begin + p.chunk < p.rows ? begin + p.chunk : p.rows;
   const int tiles = (int)((end - begin + 63) / 64);
   for (int t0 = wave; t0 < tiles; t0 += 4 * 8) {  // eight tiles' ids in flight
     int id[8];
@@ -504,13 +605,26 @@ __global__ __launch_bounds__(256) void adapted_grad(const GradArgs p) {
       const int row = 32 * b + (i >> 6), c = c0 + (i & 63);
       if (row >= p.rank || c >= j.cols) continue;
       const int64_t at =
-          blockIdx.z * p.chunk_stride[which] + (int64_t)a * p.rank * j.cols + row * j.sj + c * j.sc;
+          chunk * p.chunk_stride[which] + (int64_t)a * p.rank * j.cols + row * j.sj + c * j.sc;
       if (p.to_bf16)
         static_cast<bf16*>(j.to)[at] = (bf16)v;
       else
         static_cast<float*>(j.to)[at] = v;
     }
   }
+}
+
+// The gradients, and (the first workgroups) dx where it is wanted: both go by the thin products alone. block 256.
+template <int RP, int TM, int TN, int STAGES>
+__global__ __launch_bounds__(256) void adapted_finish(const ProductArgs t, const GradArgs g, uint32_t product_blocks) {
+  __shared__ union U {
+    __attribute__((aligned(16))) bf16 buf[STAGES][TM / 64 + TN / 64][64 * 64];
+    GradLds<RP> grad;
+  } s;
+  if (blockIdx.x < product_blocks)
+    product_tile<TM, TN, STAGES>(t, blockIdx.x, product_blocks, s.buf);
+  else
+    grad_tile<RP>(g, blockIdx.x - product_blocks, s.grad);
 }
 
 struct JoinJob {
@@ -554,33 +668,6 @@ __global__ __launch_bounds__(256) void adapted_join(const JoinArgs p) {
 // ---------------------------------------------------------------------------------------------------------
 // few rows
 
-// Eight values at p[k ..], those from n on read as zeros. EVEN: n a multiple of 8 (the values lie in one 16- or 32-byte
-// piece or none do): no branch, so that loads can run ahead of each other.
-template <typename T, bool EVEN>
-struct Raw8 {
-  typedef T vec __attribute__((__vector_size__(8 * sizeof(T)), aligned(sizeof(T))));
-  vec v;
-  bool in;
-  __device__ __forceinline__ void load(const T* p, int k, int n) {
-    in = k < n;
-    if constexpr (EVEN) {
-      v = *reinterpret_cast<const vec*>(p + (in ? k : 0));
-    } else if (k + 8 <= n) {
-      v = *reinterpret_cast<const vec*>(p + k);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = k + e < n ? p[k + e] : (T)0.f;
-    }
-  }
-  __device__ __forceinline__ float operator[](int e) const { return in ? (float)v[e] : 0.f; }
-  __device__ __forceinline__ bf16x8 operand() const {
-    bf16x8 o;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = in ? (bf16)(float)v[e] : (bf16)0.f;
-    return o;
-  }
-};
-
 struct FewArgs {
   const bf16* x;
   const void *w, *down, *up;
@@ -595,10 +682,10 @@ struct FewArgs {
 // u of one row a workgroup in fp32, two channels a wave at a time, k across the lanes. grid rows; block 512.
 template <typename TA, bool EVEN>
 __global__ __launch_bounds__(512) void adapted_few_thin(const FewArgs p) {
-  __shared__ int id[64], start[64], before;
+  __shared__ int id[64], start[64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t row = blockIdx.x;
-  tile_ids<512>(p.q, row, id, start, &before);
+  tile_ids(p.q, row, id, start);
   const int a = id[0];
   if (threadIdx.x == 0) p.ids[row] = a;
   if (a < 0) return;
@@ -716,14 +803,11 @@ int64_t tiles32(int64_t batch, int64_t rows, int64_t cols) { return batch * ((ro
 
 struct Packer {
   PackArgs args{};
-  int64_t tiles = 0;
-  void add(const void* src, int f32, bf16* hi, bf16* mid, bf16* lo, int64_t batch, int64_t rows, int64_t cols, int64_t out_rows,
+  void add(const void* src, int f32, bf16* dst, int64_t batch, int64_t rows, int64_t cols, int64_t out_rows,
            int64_t out_cols, bool turn) {
     PackJob j;
     j.src = src;
-    j.hi = hi;
-    j.mid = mid;
-    j.lo = lo;
+    j.dst = dst;
     j.rows = rows;
     j.cols = cols;
     j.out_rows = out_rows;
@@ -732,43 +816,60 @@ struct Packer {
     j.f32 = f32;
     j.turn = turn;
     args.job[args.jobs++] = j;
-    tiles += j.tiles;
-  }
-  void launch(hipStream_t st) const {
-    if (tiles > 0) adapted_pack<<<dim3((unsigned)std::min<int64_t>(tiles, 1 << 20)), 256, 0, st>>>(args, tiles);
+    args.tiles += j.tiles;
   }
 };
 
-template <int PARTS, bool KEEP>
-void launch_thin(const ThinArgs& a, int rp, int jobs, hipStream_t st) {
-  const int64_t rows = a.q.rows;
+template <typename TA, int RP, bool KEEP>
+void launch_prepare_as(const ThinArgs& t, const PackArgs& p, bool split, bool even, hipStream_t st) {
+  const dim3 grid((unsigned)(t.row_blocks * t.share * t.jobs + std::min<int64_t>(p.tiles, 1 << 20)));
+  if (split)
+    even ? adapted_prepare<TA, RP, KEEP, 4, true><<<grid, 256, 0, st>>>(t, p)
+         : adapted_prepare<TA, RP, KEEP, 4, false><<<grid, 256, 0, st>>>(t, p);
+  else
+    even ? adapted_prepare<TA, RP, KEEP, 1, true><<<grid, 256, 0, st>>>(t, p)
+         : adapted_prepare<TA, RP, KEEP, 1, false><<<grid, 256, 0, st>>>(t, p);
+}
+template <bool KEEP>
+void launch_prepare(ThinArgs t, const PackArgs& p, int rp, int a_f32, hipStream_t st) {
+  const int64_t rows = t.q.rows;
   // few rows: a quarter of k a wave, so that the chip is filled, and the adapters of 16 rows shared out where they may be many
   const bool split = rows < 64 * 256;
-  const int share = split && a.q.count > (int)(rows / 16) ? 4 : 1;
-  const dim3 grid((unsigned)((rows + (split ? 15 : 63)) / (split ? 16 : 64)), share, jobs);
-#define FFK_THIN(RP)                                      \
-  if (rp == RP) {                                         \
-    if (split)                                            \
-      adapted_thin<RP, PARTS, KEEP, 4><<<grid, 256, 0, st>>>(a); \
-    else                                                  \
-      adapted_thin<RP, PARTS, KEEP, 1><<<grid, 256, 0, st>>>(a); \
+  const bool even = t.job[0].K % 8 == 0 && (t.jobs == 1 || t.job[1].K % 8 == 0);
+  t.share = split && t.q.count > (int)(rows / 16) ? 4 : 1;
+  t.row_blocks = (rows + (split ? 15 : 63)) / (split ? 16 : 64);
+#define FFK_PREPARE(RP)                                                           \
+  if (rp == RP) {                                                                 \
+    a_f32 ? launch_prepare_as<float, RP, KEEP>(t, p, split, even, st)             \
+          : launch_prepare_as<bf16, RP, KEEP>(t, p, split, even, st);             \
   }
-  FFK_THIN(16)
-  FFK_THIN(32)
-  FFK_THIN(64)
-  FFK_THIN(128)
-#undef FFK_THIN
+  FFK_PREPARE(16)
+  FFK_PREPARE(32)
+  FFK_PREPARE(64)
+  FFK_PREPARE(128)
+#undef FFK_PREPARE
 }
 
+// Tiles of 128 x 128 where they fill the chip, of 64 x 64 where not.
+bool big_tiles(int64_t rows, int N) { return N > 64 && ((rows + 127) / 128) * ((N + 127) / 128) >= 256; }
+
 void launch_product(ProductArgs a, hipStream_t st) {
-  const int64_t big = ((a.rows + 127) / 128) * ((a.N + 127) / 128);
-  if (big >= 256 && a.N > 64) {
-    a.n_tiles = (a.N + 127) / 128;
-    adapted_product<128, 128, 2><<<dim3((unsigned)big), 256, 0, st>>>(a);
-  } else {
-    a.n_tiles = (a.N + 63) / 64;
-    adapted_product<64, 64, 4><<<dim3((unsigned)((a.rows + 63) / 64 * a.n_tiles)), 256, 0, st>>>(a);
-  }
+  const bool big = big_tiles(a.rows, a.N);
+  const int t = big ? 128 : 64;
+  a.n_tiles = (a.N + t - 1) / t;
+  const dim3 grid((unsigned)((a.rows + t - 1) / t * a.n_tiles));
+  big ? adapted_product<128, 128, 2><<<grid, 256, 0, st>>>(a) : adapted_product<64, 64, 4><<<grid, 256, 0, st>>>(a);
+}
+
+template <int RP>
+void launch_finish(ProductArgs a, const GradArgs& g, int chunks, hipStream_t st) {
+  const bool big = a.out && big_tiles(a.rows, a.N);
+  const int t = big ? 128 : 64;
+  a.n_tiles = (a.N + t - 1) / t;
+  const uint32_t product = a.out ? (uint32_t)((a.rows + t - 1) / t * a.n_tiles) : 0;
+  const dim3 grid(product + (unsigned)((int64_t)(g.job[0].tiles + g.job[1].tiles) * g.adapters * chunks));
+  big ? adapted_finish<RP, 128, 128, 2><<<grid, 256, 0, st>>>(a, g, product)
+      : adapted_finish<RP, 64, 64, 3><<<grid, 256, 0, st>>>(a, g, product);
 }
 
 int64_t up64(int64_t n) { return (n + 63) / 64 * 64; }
@@ -797,10 +898,9 @@ AdaptedPlan adapted_plan(int64_t rows, int d_in, int d_out, int adapters, int ra
   p.rows = backward ? adapted_rows_grad_served(rows, d_in, d_out, rank, requests)
                     : adapted_rows_served(rows, d_in, d_out, rank, requests);
   if (p.rows) return p;
+  p.pack_x = d_in % 64 != 0;
   if (backward) {
-    p.pack_x = d_in % 64 != 0;
     p.pack_dy = d_out % 64 != 0;
-    p.pack_down = a_f32 || d_in % 64 != 0;
     const int64_t tiles = (p.kp + p.np) / 64 * adapters;
     // some four workgroups a CU, of 512 of their adapter's rows at least
     const int64_t used = std::max(1, std::min(adapters, requests));
@@ -808,9 +908,7 @@ AdaptedPlan adapted_plan(int64_t rows, int d_in, int d_out, int adapters, int ra
     p.chunk = std::min<int64_t>(up64((rows + chunks - 1) / chunks), 64 * kMostGradTiles);
     p.chunks = (int)((rows + p.chunk - 1) / p.chunk);
   } else {
-    p.pack_x = d_in % 64 != 0;
     p.pack_w = w_f32 || d_in % 64 != 0;
-    p.pack_down = a_f32 || d_in % 64 != 0;
     p.pack_up = a_f32 || rank != p.rp;
   }
   return p;
@@ -840,23 +938,21 @@ void launch_adapted(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t st) 
     return;
   }
   Packer pack;
-  if (p.pack_x) pack.add(a.x, 0, a.xp, nullptr, nullptr, 1, a.rows, a.d_in, a.rows, p.kp, false);
-  if (p.pack_w) pack.add(a.w, a.w_f32, a.wp, nullptr, nullptr, 1, a.d_out, a.d_in, a.d_out, p.kp, false);
-  if (p.pack_down) pack.add(a.down, a.a_f32, a.down_hi, nullptr, nullptr, a.adapters, a.rank, a.d_in, a.rank, p.kp, false);
-  if (p.pack_up) pack.add(a.up, a.a_f32, a.upp, nullptr, nullptr, a.adapters, a.d_out, a.rank, a.d_out, p.rp, false);
-  pack.launch(st);
+  if (p.pack_x) pack.add(a.x, 0, a.xp, 1, a.rows, a.d_in, a.rows, p.kp, false);
+  if (p.pack_w) pack.add(a.w, a.w_f32, a.wp, 1, a.d_out, a.d_in, a.d_out, p.kp, false);
+  if (p.pack_up) pack.add(a.up, a.a_f32, a.upp, a.adapters, a.d_out, a.rank, a.d_out, p.rp, false);
   ThinArgs t{};
-  t.job[0].x = p.pack_x ? a.xp : a.x;
-  t.job[0].mat[0] = p.pack_down ? a.down_hi : static_cast<const bf16*>(a.down);
+  t.job[0].x = a.x;
+  t.job[0].mat = a.down;
   t.job[0].u = a.u;
-  t.job[0].K = p.kp;
-  t.job[0].mat_rows = a.rank;
+  t.job[0].K = a.d_in;
   t.q = q;
   t.ids = a.ids;
   t.rank = a.rank;
-  launch_thin<1, false>(t, p.rp, 1, st);
+  t.jobs = 1;
+  launch_prepare<false>(t, pack.args, p.rp, a.a_f32, st);
   ProductArgs g{};
-  g.x = t.job[0].x;
+  g.x = p.pack_x ? a.xp : a.x;
   g.w = p.pack_w ? a.wp : static_cast<const bf16*>(a.w);
   g.u = a.u;
   g.b = p.pack_up ? a.upp : static_cast<const bf16*>(a.up);
@@ -867,61 +963,52 @@ void launch_adapted(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t st) 
   g.K = p.kp;
   g.N = a.d_out;
   g.RP = p.rp;
-  g.ld = p.rp;
+  g.ld = p.ld;
   launch_product(g, st);
 }
 
 void launch_adapted_grad(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t st) {
   if (p.rows) return launch_adapted_rows_grad(a, st);
   Packer pack;
-  if (p.pack_x) pack.add(a.x, 0, a.xp, nullptr, nullptr, 1, a.rows, a.d_in, a.rows, p.kp, false);
-  if (p.pack_dy) pack.add(a.dy, 0, a.dyp, nullptr, nullptr, 1, a.rows, a.d_out, a.rows, p.np, false);
-  if (a.out) pack.add(a.w, a.w_f32, a.wp, nullptr, nullptr, 1, a.d_out, a.d_in, a.d_in, p.np, true);
-  if (p.pack_down)
-    pack.add(a.down, a.a_f32, a.down_hi, a.down_mid, a.down_lo, a.adapters, a.rank, a.d_in, a.rank, p.kp, false);
-  pack.add(a.up, a.a_f32, a.up_hi, a.up_mid, a.up_lo, a.adapters, a.d_out, a.rank, a.rank, p.np, true);
-  if (a.out) pack.add(a.down, a.a_f32, a.down_t, nullptr, nullptr, a.adapters, a.rank, a.d_in, a.d_in, p.rp, true);
-  pack.launch(st);
+  if (p.pack_x) pack.add(a.x, 0, a.xp, 1, a.rows, a.d_in, a.rows, p.kp, false);
+  if (p.pack_dy) pack.add(a.dy, 0, a.dyp, 1, a.rows, a.d_out, a.rows, p.np, false);
+  if (a.out) pack.add(a.w, a.w_f32, a.wp, 1, a.d_out, a.d_in, a.d_in, p.np, true);
+  if (a.out) pack.add(a.down, a.a_f32, a.down_t, a.adapters, a.rank, a.d_in, a.d_in, p.rp, true);
   ThinArgs t{};
-  t.job[0].x = p.pack_x ? a.xp : a.x;
-  const bf16* down[3] = {p.pack_down ? a.down_hi : static_cast<const bf16*>(a.down), a.down_mid, a.down_lo};
-  const bf16* up[3] = {a.up_hi, a.up_mid, a.up_lo};
-  for (int i = 0; i < 3; ++i) {
-    t.job[0].mat[i] = down[i];
-    t.job[1].mat[i] = up[i];
-  }
+  t.job[0].x = a.x;
+  t.job[0].mat = a.down;
   t.job[0].u = a.u;
-  t.job[0].K = p.kp;
-  t.job[1].x = p.pack_dy ? a.dyp : a.dy;
+  t.job[0].K = a.d_in;
+  t.job[1].x = a.dy;
+  t.job[1].mat = a.up;
   t.job[1].u = a.v;
-  t.job[1].K = p.np;
-  t.job[0].mat_rows = t.job[1].mat_rows = a.rank;
+  t.job[1].K = a.d_out;
+  t.job[1].turned = 1;
   t.q = requests_of(a);
   t.ids = a.ids;
   t.rank = a.rank;
-  a.a_f32 ? launch_thin<3, true>(t, p.rp, 2, st) : launch_thin<1, true>(t, p.rp, 2, st);
-  if (a.out) {
-    ProductArgs g{};
-    g.x = t.job[1].x;
-    g.w = a.wp;
-    g.u = a.v;
-    g.b = a.down_t;
-    g.ids = a.ids;
-    g.out = a.out;
-    g.rows = a.rows;
-    g.K = p.np;
-    g.N = a.d_in;
-    g.RP = p.rp;
-    g.ld = parts_ld(p.rp);
-    launch_product(g, st);
-  }
+  t.jobs = 2;
+  launch_prepare<true>(t, pack.args, p.rp, a.a_f32, st);
+  const bf16 *x = p.pack_x ? a.xp : a.x, *dy = p.pack_dy ? a.dyp : a.dy;
+  ProductArgs g{};
+  g.x = dy;
+  g.w = a.wp;
+  g.u = a.v;
+  g.b = a.down_t;
+  g.ids = a.ids;
+  g.out = a.out;
+  g.rows = a.rows;
+  g.K = p.np;
+  g.N = a.d_in;
+  g.RP = p.rp;
+  g.ld = p.ld;
   const bool join = p.chunks > 1;
   GradArgs d{};
-  d.job[0].x = t.job[0].x;
+  d.job[0].x = x;
   d.job[0].v = a.v;
   d.job[0].cols = a.d_in;
   d.job[0].ld_x = p.kp;
-  d.job[1].x = t.job[1].x;
+  d.job[1].x = dy;
   d.job[1].v = a.u;
   d.job[1].cols = a.d_out;
   d.job[1].ld_x = p.np;
@@ -933,7 +1020,7 @@ void launch_adapted_grad(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t
     GradJob& j = d.job[i];
     const int64_t count = (int64_t)a.adapters * a.rank * j.cols;
     j.tiles = j.ld_x / 64;
-    j.to = join ? (i ? a.part[1] : a.part[0]) : to[i];
+    j.to = join ? a.part[i] : to[i];
     j.sj = join ? j.cols : sj[i];
     j.sc = join ? 1 : sc[i];
     d.chunk_stride[i] = join ? count : 0;
@@ -949,13 +1036,13 @@ void launch_adapted_grad(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t
   d.rows = a.rows;
   d.chunk = p.chunk;
   d.rank = a.rank;
+  d.adapters = a.adapters;
   d.to_bf16 = !join && a.grad_dtype == 0;
-  const dim3 grid((unsigned)(d.job[0].tiles + d.job[1].tiles), (unsigned)a.adapters, (unsigned)p.chunks);
   switch (p.rp) {
-    case 16: adapted_grad<16><<<grid, 256, 0, st>>>(d); break;
-    case 32: adapted_grad<32><<<grid, 256, 0, st>>>(d); break;
-    case 64: adapted_grad<64><<<grid, 256, 0, st>>>(d); break;
-    default: adapted_grad<128><<<grid, 256, 0, st>>>(d);
+    case 16: launch_finish<16>(g, d, p.chunks, st); break;
+    case 32: launch_finish<32>(g, d, p.chunks, st); break;
+    case 64: launch_finish<64>(g, d, p.chunks, st); break;
+    default: launch_finish<128>(g, d, p.chunks, st);
   }
   if (join) {
     e.chunks = p.chunks;

@@ -32,10 +32,12 @@ __device__ __forceinline__ int64_t request_end(const Requests& q, int r) {
 }
 __device__ __forceinline__ RequestAt request_first(const Requests& q, int64_t row, int lane) {
   int before = 0;  // the offsets up to `row` (in order: of the first requests), counted by a wave
-#pragma unroll 4
-  for (int i = 0; i <= q.count; i += 64) {
-    const int at = i + lane < q.count ? i + lane : q.count;
-    before += __popcll(__ballot(q.offsets[at] <= row && i + lane <= q.count));
+  for (int i0 = lane; i0 - lane <= q.count; i0 += 256) {
+    int offset[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) offset[u] = q.offsets[i0 + 64 * u < q.count ? i0 + 64 * u : q.count];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) before += __popcll(__ballot(offset[u] <= row && i0 + 64 * u <= q.count));
   }
   const int r = before - 1;
   return {r, adapter_at(q, r), request_end(q, r)};

@@ -624,7 +624,6 @@ size_t adapted_ws(void* ws, const AdaptedPlan& p, AdaptedArgs& a, int backward) 
   }
   const size_t mats = (size_t)a.adapters * a.rank;
   if (p.pack_x) a.xp = cv.take<bf16>((size_t)a.rows * p.kp);
-  if (p.pack_down) a.down_hi = cv.take<bf16>(mats * p.kp);
   if (!backward) {
     if (p.pack_w) a.wp = cv.take<bf16>((size_t)a.d_out * p.kp);
     if (p.pack_up) a.upp = cv.take<bf16>((size_t)a.adapters * a.d_out * p.rp);
@@ -634,13 +633,6 @@ size_t adapted_ws(void* ws, const AdaptedPlan& p, AdaptedArgs& a, int backward) 
   if (p.pack_dy) a.dyp = cv.take<bf16>((size_t)a.rows * p.np);
   a.wp = cv.take<bf16>((size_t)a.d_in * p.np);
   a.down_t = cv.take<bf16>((size_t)a.adapters * a.d_in * p.rp);
-  a.up_hi = cv.take<bf16>(mats * p.np);
-  if (a.a_f32) {
-    a.down_mid = cv.take<bf16>(mats * p.kp);
-    a.down_lo = cv.take<bf16>(mats * p.kp);
-    a.up_mid = cv.take<bf16>(mats * p.np);
-    a.up_lo = cv.take<bf16>(mats * p.np);
-  }
   a.u = cv.take<bf16>((size_t)a.rows * p.ld);
   a.v = cv.take<bf16>((size_t)a.rows * p.ld);
   if (p.chunks > 1) {

@@ -431,7 +431,7 @@ struct AdaptedPlan {
   int64_t kp, np;    // d_in and d_out rounded up to 64
   int few;           // few rows: operands straight from the call's tensors
   int rows;          // many rows of the stacks' widths: one pass (no copies)
-  int pack_x, pack_dy, pack_w, pack_down, pack_up;  // which the products read from copies (backward: w and up always)
+  int pack_x, pack_dy, pack_w, pack_up;  // which the wide product reads from copies (backward: w and down always)
   int64_t chunk;     // backward: rows of a workgroup's sums
   int chunks;
 };
@@ -449,8 +449,6 @@ struct AdaptedArgs {
   // workspace (adapted_ws)
   int32_t* ids;                       // [rows]
   bf16 *xp, *dyp, *wp;                // padded copies of x, dy; w bf16 (backward: turned)
-  bf16 *down_hi, *down_mid, *down_lo; // [adapters][rank][kp] each
-  bf16 *up_hi, *up_mid, *up_lo;       // [adapters][rank][np] each
   bf16 *down_t, *upp;                 // [adapters][d_in][rp], [adapters][d_out][rp]
   bf16 *u, *v;                        // [rows][ld]
   float* few_u;                       // [rows][rank]
