@@ -141,12 +141,59 @@ class EngineOp:
         dispatch.note_call(self, backend)  # type: ignore[arg-type]
         return backend
 
+    #: the axis along which the op's dropout has one mask (None: the op has none)
+    dropout_axis: int | None = None
+
+    def active_dropout(self) -> "Dropout | None":
+        """The op's dropout (:func:`foldforge_amd.training.set_dropout`) where it applies: in training mode."""
+        return self._modules.get("dropout") if self.training else None  # type: ignore[attr-defined]
+
     def forward(self, *args: Any, **kwargs: Any) -> Any:
+        dropout = self.active_dropout()
+        if dropout is not None:
+            return dropout(self._update(args, kwargs), args[0])
         return getattr(self, f"_forward_{self._route(args, kwargs)}")(*args, **kwargs)
 
     def delta(self, *args: Any, **kwargs: Any) -> Tensor:
         """The bare update ``f(x)`` (the forward returns ``x + f(x)``)."""
+        update, dropout = self._update(args, kwargs), self.active_dropout()
+        return update if dropout is None else dropout(update)
+
+    def _update(self, args: tuple, kwargs: dict) -> Tensor:
         return getattr(self, f"_forward_{self._route(args, kwargs)}")(*args, residual=False, **kwargs)
+
+
+class Dropout(EngineOp, nn.Module):
+    """The dropout of an op's update and its sum with the residual (:func:`foldforge_amd.kernels.dropout_add`): rate ``p``,
+    one mask along ``axis``, each call's draw from ``stream`` (a :class:`foldforge_amd.training.DropoutStream`). Both
+    backends draw the same mask."""
+
+    def __init__(self, p: float, axis: int | None, stream: "training.DropoutStream", backend: str = "pytorch") -> None:
+        nn.Module.__init__(self)
+        kernels.dropped_of_levels(p)  # (the rate's range)
+        self.p, self.axis, self.stream = p, axis, stream
+        self._init_backend(backend)
+
+    def _unsupported_hip(self, update: Tensor, residual: Tensor | None = None) -> str | None:
+        reason = hip_reason(update, residual)
+        if reason is not None:
+            return reason
+        if update.dtype not in (torch.bfloat16, torch.float32):
+            return f"dtype {update.dtype} (the kernel takes bf16 or fp32)"
+        return None
+
+    def forward(self, update: Tensor, residual: Tensor | None = None) -> Tensor:
+        return getattr(self, f"_forward_{self._route((update, residual), {})}")(update, residual)
+
+    def _forward_pytorch(self, update: Tensor, residual: Tensor | None = None) -> Tensor:
+        return torch_ops.dropout_add(update, residual, shared=self.axis, dropped=kernels.dropped_of_levels(self.p),
+                                     seed=self.stream.seed, offset=self.stream.take())
+
+    def _forward_hip(self, update: Tensor, residual: Tensor | None = None) -> Tensor:
+        how = dict(p=self.p, seed=self.stream.seed, offset=self.stream.take(), shared=self.axis)
+        if torch.is_grad_enabled() and (update.requires_grad or (residual is not None and residual.requires_grad)):
+            return training.dropout_add(update, residual, **how)
+        return kernels.dropout_add(update.contiguous(), None if residual is None else residual.contiguous(), **how)
 
 
 def _spec(**paths: str) -> tuple[tuple[str, str, str], ...]:
@@ -260,6 +307,7 @@ class TriangleMultiplication(EngineOp, MasterWeights, nn.Module):
     (equations ``legacy/reference/triangle.py:19-49``; parameters ``legacy/released.py:166-173``)."""
 
     divide_by_length = False
+    dropout_axis = 1  # AF3's row-wise dropout: one mask for all rows
 
     def __init__(self, d_pair: int, d_hidden: int | None = None, outgoing: bool = True,
                  p_drop: float = 0.0, model: str | None = None, backend: str = "pytorch") -> None:
@@ -363,6 +411,7 @@ class TriangleAttention(EngineOp, MasterWeights, nn.Module):
         hidden = d_pair if d_hidden is None else d_hidden
         self.d_pair, self.n_head, self.d_hidden = d_pair, n_head, hidden
         self.starting, self.p_drop, self.model = starting, p_drop, model
+        self.dropout_axis = 1 if starting else 2  # row-wise, and column-wise around the ending node
         self.ln_pair = LayerNorm(d_pair)
         self.to_bias = _linear(d_pair, n_head)
         self.to_query = _linear(d_pair, hidden)
@@ -437,9 +486,48 @@ class TriangleAttentionChai1Confidence(TriangleAttentionAF3):
     dual_output = True
 
 
+class TransitionAdapters(MasterWeights, nn.Module):
+    """Low-rank adapters beside a Transition's three projections, ``adapters`` of them of one rank, and which of them each
+    element of a batch has (:func:`foldforge_amd.training.adapt`, :func:`foldforge_amd.training.select_adapters`)."""
+
+    NAMES = ("expand_a", "expand_b", "squeeze")
+
+    def __init__(self, d: int, n: int, rank: int, adapters: int, scale: float, generator: torch.Generator) -> None:
+        nn.Module.__init__(self)
+        self.master_weights = True
+        for name in self.NAMES:
+            d_in, d_out = (n * d, d) if name == "squeeze" else (d, n * d)
+            if not kernels.adapted_linear_supported(d_in, d_out, rank, adapters):
+                raise ValueError(f"{adapters} adapters of rank {rank} at {d_in} -> {d_out} (rank 1 to {kernels.MOST_RANK})")
+            down = torch.randn(adapters, rank, d_in, generator=generator) * d_in**-0.5
+            self.register_parameter(f"{name}_down", nn.Parameter(down))
+            self.register_parameter(f"{name}_up", nn.Parameter(torch.zeros(adapters, d_out, rank)))
+        self.register_buffer("scale", torch.full((adapters,), float(scale)))
+        self.adapter: Tensor | None = None
+
+    def matrices(self, name: str) -> tuple[Tensor, Tensor]:
+        """``(down, up)`` of a projection."""
+        return getattr(self, f"{name}_down"), getattr(self, f"{name}_up")
+
+    def of(self, x: Tensor) -> Tensor:
+        """The adapter of each element of the batch ``x [B, ..., d]``."""
+        if self.adapter is None:
+            return torch.zeros(x.shape[0], dtype=torch.int32, device=x.device)
+        if tuple(self.adapter.shape) != (x.shape[0],):
+            raise ValueError(f"{tuple(self.adapter.shape)} adapters are selected for a batch of {x.shape[0]}")
+        return self.adapter
+
+    def requests(self, x: Tensor) -> tuple[Tensor, Tensor]:
+        """``(offsets, adapter)`` of the rows of ``x``: every element of the batch is a request."""
+        batch, rows = x.shape[0], x.shape[1:-1].numel()
+        return torch.arange(batch + 1, dtype=torch.int32, device=x.device) * rows, self.of(x)
+
+
 class Transition(EngineOp, MasterWeights, nn.Module):
     """SwiGLU transition, residual included (``legacy/reference/transition.py:28-59``;
-    parameters ``legacy/released.py:211-224``)."""
+    parameters ``legacy/released.py:211-224``). With ``adapters`` (:func:`foldforge_amd.training.adapt`) each projection has
+    the low-rank adapter of the batch element beside it; on ``hip`` it then runs as a norm, the three projections
+    (:func:`foldforge_amd.kernels.adapted_linear`) and the gate between them."""
 
     #: what a differentiated ``hip`` call keeps of its input (as :class:`LayerNorm`)
     keep: str | None = None
@@ -447,6 +535,7 @@ class Transition(EngineOp, MasterWeights, nn.Module):
     def __init__(self, d_hidden: int, n: int = 4, backend: str = "pytorch") -> None:
         nn.Module.__init__(self)
         self.d, self.n = d_hidden, n
+        self.adapters: TransitionAdapters | None = None
         self.ln_in = LayerNorm(d_hidden)
         self.expand_a = _linear(d_hidden, n * d_hidden)
         self.expand_b = _linear(d_hidden, n * d_hidden)
@@ -459,6 +548,8 @@ class Transition(EngineOp, MasterWeights, nn.Module):
             return reason
         if x.dtype != torch.bfloat16:
             return f"{x.dtype} activations (the kernel takes bf16)"
+        if self.adapters is not None:
+            return None if x.dim() > 1 and x.shape[-1] == self.d else f"shape {tuple(x.shape)} (a batch of rows of {self.d})"
         if not kernels.transition_supported(self.d, self.n):
             return (f"width {self.d} x {self.n} (the kernels take 128 x 4, or d and "
                     "n * d multiples of 64)")
@@ -474,11 +565,30 @@ class Transition(EngineOp, MasterWeights, nn.Module):
     def _forward_hip(self, x: Tensor, *, residual: bool = True) -> Tensor:
         if self.dead:
             return x if residual else torch.zeros_like(x)
+        if self.adapters is not None:
+            return self._adapted(x, residual)
         if training.wanted(self, x):
             return training.transition(x, residual=residual, eps=self.ln_in.eps, keep=self.keep,
                                        **_read(self, _TRANSITION))
         return kernels.transition(
             x.contiguous(), residual=residual, eps=self.ln_in.eps, **_read(self, _TRANSITION))
+
+    def _adapted(self, x: Tensor, residual: bool) -> Tensor:
+        offsets, adapter = self.adapters.requests(x)  # type: ignore[union-attr]
+        graph = torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters()))
+        linear = training.adapted_linear if graph else kernels.adapted_linear
+
+        def project(t: Tensor, name: str) -> Tensor:
+            down, up = self.adapters.matrices(name)  # type: ignore[union-attr]
+            return linear(t, getattr(self, name).weight, down=down, up=up, scale=self.adapters.scale,  # type: ignore
+                          offsets=offsets, adapter=adapter)
+
+        w, b, eps = self.ln_in.weight, self.ln_in.bias, self.ln_in.eps
+        h = training.layer_norm(x, w, b, eps, keep=self.keep or "input") if graph else kernels.layer_norm(
+            x.contiguous(), w, b, eps)
+        gate = nn.functional.silu(project(h, "expand_a").float()) * project(h, "expand_b").float()
+        y = project(gate.to(x.dtype), "squeeze")
+        return x + y if residual else y
 
 
 class AttentionPairBias(EngineOp, MasterWeights, nn.Module):
@@ -555,6 +665,7 @@ class MSAPairWeightedAveraging(EngineOp, MasterWeights, nn.Module):
         nn.Module.__init__(self)
         dh = d_msa // n_head if d_hidden is None else d_hidden
         self.d_msa, self.d_pair, self.n_head, self.d_hidden, self.p_drop = d_msa, d_pair, n_head, dh, p_drop
+        self.dropout_axis = 1  # one mask for all MSA rows
         self.ln_msa = LayerNorm(d_msa)
         self.ln_pair = LayerNorm(d_pair, bias=False)
         self.to_bias = _linear(d_pair, n_head)
@@ -685,7 +796,8 @@ def _fused_attention_transition(att: "TriangleAttention", tr: "Transition") -> b
     no projection biases, neither op dead)."""
     return (not att.dead and not tr.dead and not att.untransposed_output and not att.dual_output
             and att.to_gate.bias is None and att.to_out.bias is None
-            and (att.d_pair, att.n_head, att.d_hidden) == (128, 4, 128) and (tr.d, tr.n) == (128, 4))
+            and (att.d_pair, att.n_head, att.d_hidden) == (128, 4, 128) and (tr.d, tr.n) == (128, 4)
+            and tr.adapters is None)
 
 
 def attention_then_transition(att: "TriangleAttention", tr: "Transition", z: Tensor, mask: Tensor,
@@ -695,6 +807,8 @@ def attention_then_transition(att: "TriangleAttention", tr: "Transition", z: Ten
     one call runs them with the attention's output projection inside the transition kernel
     (``kernels.triangle_attention_transition``: the same results, the attention output never
     written). Each op is routed (refusal policy, ledger) exactly as its own call would be."""
+    if att.active_dropout() is not None:
+        return tr(att(z, mask))
     b_att = att._route((z, mask), {})
     # (a transition that is to be differentiated runs by itself: it keeps its input)
     if b_att == "hip" and fuse and _fused_attention_transition(att, tr) and not training.wanted(tr, z):
@@ -753,14 +867,16 @@ class PairformerBlock(MasterWeights, nn.Module):
         super().__init__()
         self.config = config
         c = config
-        self.tri_multi_outgoing = TriangleMultiplication(c.d_pair, c.d_hidden_tri_multi, outgoing=True)
-        self.tri_multi_incoming = TriangleMultiplication(c.d_pair, c.d_hidden_tri_multi, outgoing=False)
+        self.tri_multi_outgoing = TriangleMultiplication(
+            c.d_pair, c.d_hidden_tri_multi, outgoing=True, p_drop=c.p_drop)
+        self.tri_multi_incoming = TriangleMultiplication(
+            c.d_pair, c.d_hidden_tri_multi, outgoing=False, p_drop=c.p_drop)
         if c.use_triangle_attention:
             hidden = c.n_head_tri_attention * c.d_hidden_tri_attention
             self.tri_atten_starting = TriangleAttention(
-                c.d_pair, c.n_head_tri_attention, d_hidden=hidden, starting=True, model=c.model)
+                c.d_pair, c.n_head_tri_attention, d_hidden=hidden, starting=True, p_drop=c.p_drop, model=c.model)
             self.tri_atten_ending = TriangleAttention(
-                c.d_pair, c.n_head_tri_attention, d_hidden=hidden, starting=False, model=c.model)
+                c.d_pair, c.n_head_tri_attention, d_hidden=hidden, starting=False, p_drop=c.p_drop, model=c.model)
         self.transition_pair = Transition(c.d_pair, c.pair_transition_n)
         if c.d_single > 0:
             self.single_attention = AttentionPairBias(

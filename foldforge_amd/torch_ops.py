@@ -12,6 +12,8 @@ parameters and returns the input dtype. Equations: the reference's legacy statem
 
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.nn.functional as F
 
@@ -28,6 +30,50 @@ def _ln(x: Tensor, w: Tensor | None, b: Tensor | None, eps: float) -> Tensor:
 
 def _lin(x: Tensor, w: Tensor, b: Tensor | None = None) -> Tensor:
     return F.linear(x, w.float(), None if b is None else b.float())
+
+
+def _philox_round(words, k0: int, k1: int):
+    """One round of Philox4x32 on 32-bit words held in int64 (of a product the upper half of the 64 bits that wrap)."""
+    a, b, c, d = words
+    low = 0xFFFFFFFF
+    left, right = a * 0xD2511F53, c * 0xCD9E8D57
+    return (((right >> 32) & low) ^ b ^ k0, right & low, ((left >> 32) & low) ^ d ^ k1, left & low)
+
+
+def dropout_mask(shape: tuple[int, ...], shared: int | None, dropped: int, seed: int, offset: int,
+                 device: torch.device) -> Tensor:
+    """Which values :func:`foldforge_amd.kernels.dropout_add` keeps, of size 1 along ``shared``."""
+    shape = list(shape)
+    if shared is not None:
+        shape[shared] = 1
+    n = math.prod(shape)
+    block = torch.arange(-(-n // 8), dtype=torch.int64, device=device)
+    words = (block & 0xFFFFFFFF, block >> 32, torch.full_like(block, offset & 0xFFFFFFFF),
+             torch.full_like(block, offset >> 32))
+    k0, k1 = seed & 0xFFFFFFFF, seed >> 32
+    for _ in range(10):
+        words = _philox_round(words, k0, k1)
+        k0, k1 = (k0 + 0x9E3779B9) & 0xFFFFFFFF, (k1 + 0xBB67AE85) & 0xFFFFFFFF
+    numbers = torch.stack([half for w in words for half in (w & 0xFFFF, w >> 16)], -1).flatten()
+    return (numbers[:n] >= dropped).view(shape)
+
+
+def dropout_add(update: Tensor, residual: Tensor | None, *, shared: int | None, dropped: int, seed: int,
+                offset: int) -> Tensor:
+    keep = dropout_mask(tuple(update.shape), shared, dropped, seed, offset, update.device)
+    y = torch.where(keep, update.float() * (65536 / max(65536 - dropped, 1)), 0.0)
+    return (y if residual is None else residual.float() + y).to(update.dtype)
+
+
+def adapted_linear(x: Tensor, w: Tensor, down: Tensor, up: Tensor, scale: Tensor, adapter: Tensor) -> Tensor:
+    """``x [B, ..., d_in]`` fp32 through ``w`` and, for each batch element, its adapter (outside 0 .. n - 1: none)."""
+    y = F.linear(x, w.float())
+    has = (adapter >= 0) & (adapter < down.shape[0])
+    a = torch.where(has, adapter, 0).long()
+    flat = x.reshape(x.shape[0], -1, x.shape[-1])
+    u = flat @ down.float()[a].transpose(1, 2).contiguous()
+    add = (u * scale[a][:, None, None]) @ up.float()[a].transpose(1, 2).contiguous()
+    return y + torch.where(has[:, None, None], add, 0.0).view(y.shape)
 
 
 def triangle_multiplication(m, x: Tensor, mask: Tensor, *, residual: bool = True) -> Tensor:
@@ -104,7 +150,15 @@ def transition(m, x: Tensor, *, residual: bool = True) -> Tensor:
     dtype = x.dtype
     z = x.float()
     h = _ln(z, m.ln_in.weight, m.ln_in.bias, m.ln_in.eps)
-    y = _lin(F.silu(_lin(h, m.expand_a.weight)) * _lin(h, m.expand_b.weight), m.squeeze.weight)
+    if m.adapters is not None:
+        of = m.adapters.of(x)
+
+        def lin(t: Tensor, name: str) -> Tensor:
+            return adapted_linear(t, getattr(m, name).weight, *m.adapters.matrices(name), m.adapters.scale, of)
+    else:
+        def lin(t: Tensor, name: str) -> Tensor:
+            return _lin(t, getattr(m, name).weight)
+    y = lin(F.silu(lin(h, "expand_a")) * lin(h, "expand_b"), "squeeze")
     return (z + y if residual else y).to(dtype)
 
 

@@ -13,6 +13,10 @@ again); with ``keep="8bit"`` the gradient is taken at the values that the 8 bits
 parameters are fp32; the transition's come from products on bf16 and fp16 operands, as its forward pass, and are off by some
 3e-3 of their norm (``pytorch``: fp32 throughout). They differentiate once.
 
+:func:`dropout_add` and :func:`adapted_linear` are the differentiable forms of the kernels of those names.
+:func:`set_dropout` gives the ops that carry a rate (``p_drop``) their dropout, :func:`adapt` gives a model's Transitions
+low-rank adapters, one for each of several requests, beside their frozen projections.
+
 Autograd does not reach into graph capture here: a backward pass whose leaves were used by an eager graph on
 another stream ends the process when it is captured, so these functions refuse a capturing stream. A captured step
 calls the kernels' functions themselves (``transition_checkpoint``, ``transition_backward``, ...).
@@ -124,6 +128,132 @@ def transition(x: Tensor, *, ln_weight: Tensor, ln_bias: Tensor, expand_a: Tenso
         raise ValueError(f"width {d} x {expand_a.shape[0] // d} (the backward kernels take a multiple of 64 up to "
                          "768, factor up to 64)")
     return _Transition.apply(x.contiguous(), ln_weight, ln_bias, expand_a, expand_b, squeeze, residual, float(eps), keep)
+
+
+class _DropoutAdd(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, update, residual, p, seed, offset, shared):
+        if isinstance(seed, Tensor):
+            seed = seed.clone()  # (the backward pass draws this mask, whatever the caller's tensor holds by then)
+        ctx.save_for_backward(seed if isinstance(seed, Tensor) else None)
+        ctx.draw = dict(p=p, seed=seed if not isinstance(seed, Tensor) else 0, offset=offset, shared=shared)
+        return kernels.dropout_add(update, residual, **{**ctx.draw, "seed": seed})
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        _eager()
+        need_update, need_residual = ctx.needs_input_grad[:2]
+        (seed,) = ctx.saved_tensors
+        draw = ctx.draw if seed is None else {**ctx.draw, "seed": seed}
+        update = kernels.dropout_backward(dy.contiguous(), **draw) if need_update else None
+        return update, dy if need_residual else None, None, None, None, None
+
+
+def dropout_add(update: Tensor, residual: Tensor | None = None, *, p: float, seed: int | Tensor, offset: int = 0,
+                shared: int | None = None) -> Tensor:
+    """:func:`foldforge_amd.kernels.dropout_add`, differentiable: nothing is kept for the backward pass, which draws the
+    mask again."""
+    _eager()
+    return _DropoutAdd.apply(update.contiguous(), None if residual is None else residual.contiguous(), float(p), seed,
+                             offset, shared)
+
+
+class _AdaptedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, down, up, scale, offsets, adapter):
+        y = kernels.adapted_linear(x, weight, bias, down=down, up=up, scale=scale, offsets=offsets, adapter=adapter)
+        ctx.save_for_backward(x, weight, down, up, scale, offsets, adapter)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        _eager()
+        x, weight, down, up, scale, offsets, adapter = ctx.saved_tensors
+        dy = dy.contiguous()
+        if dy.data_ptr() % 16:
+            dy = dy.clone()
+        grads = kernels.adapted_linear_backward(dy, x, weight, down=down, up=up, scale=scale, offsets=offsets,
+                                                adapter=adapter, with_x=ctx.needs_input_grad[0], grad_dtype=down.dtype)
+        need_down, need_up = ctx.needs_input_grad[3:5]
+        return grads.x, None, None, grads.down if need_down else None, grads.up if need_up else None, None, None, None
+
+
+def adapted_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, down: Tensor, up: Tensor,
+                   scale: Tensor | None = None, offsets: Tensor, adapter: Tensor) -> Tensor:
+    """:func:`foldforge_amd.kernels.adapted_linear`, differentiable in ``x``, ``down`` and ``up``. The projection and the
+    scales are frozen: ones that ask for a gradient are refused."""
+    _eager()
+    for t, name in ((weight, "weight"), (bias, "bias"), (scale, "scale")):
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} asks for a gradient: a projection with adapters is frozen (requires_grad_(False))")
+    x = x.contiguous()
+    return _AdaptedLinear.apply(x.clone() if x.data_ptr() % 16 else x, weight, bias, down, up, scale, offsets, adapter)
+
+
+class DropoutStream:
+    """The draws of a run's dropouts: one seed, and an offset of its own for each call. ``offset`` is where the next call
+    begins; with ``seed`` it is all that a checkpoint has to hold to go on with the same draws."""
+
+    def __init__(self, seed: int, offset: int = 0) -> None:
+        self.seed, self.offset = seed, offset
+
+    def take(self) -> int:
+        """The offset of one call."""
+        self.offset += 1
+        return self.offset - 1
+
+
+def set_dropout(model: nn.Module, stream: DropoutStream | None, p: float | None = None) -> list[str]:
+    """Give every op of ``model`` that has a dropout (the triangle ops and the MSA pair-weighted averaging) its own, drawn
+    from ``stream``, at the op's rate ``p_drop`` or at ``p``; ops at rate 0 get none. The masks are AF3's: one for all rows
+    of a pair or MSA tensor, for the ending node's attention one for all columns. They apply where the module is in training
+    mode (``model.train()``), to the update before it is added, with or without gradients. ``stream=None`` takes them
+    away. Returns the names of the ops that have one now."""
+    from foldforge_amd.modules import Dropout, device_arch
+
+    named = []
+    for name, module in list(_ops(model)):
+        if getattr(module, "dropout_axis", None) is None:
+            continue
+        module._modules.pop("dropout", None)
+        rate = module.p_drop if p is None else p
+        if stream is None or rate == 0.0:
+            continue
+        device = next(module.parameters()).device
+        hip = device.type == "cuda" and device_arch(device) == "gfx950"
+        module.dropout = Dropout(rate, module.dropout_axis, stream, backend="hip" if hip else "pytorch")
+        module.dropout.train(module.training)
+        named.append(name)
+    return named
+
+
+def adapt(model: nn.Module, rank: int, *, adapters: int = 1, scale: float = 1.0, seed: int = 0) -> list[str]:
+    """Give every Transition of ``model`` ``adapters`` low-rank adapters of ``rank`` beside each of its three projections
+    (``down`` normal of deviation ``d_in^-1/2``, ``up`` zeros: the model's results are as before at first), fp32, and
+    freeze the model's own parameters: the adapters alone ask for gradients (with :func:`install`, pass
+    ``requires_grad=False`` there). A checkpoint of the model itself is loaded before. Returns the names of the
+    Transitions."""
+    from foldforge_amd.modules import Transition, TransitionAdapters
+
+    generator = torch.Generator().manual_seed(seed)
+    made = {name: (module, TransitionAdapters(module.d, module.n, rank, adapters, scale, generator))
+            for name, module in _ops(model) if isinstance(module, Transition)}
+    model.requires_grad_(False)
+    for module, new in made.values():
+        module.adapters = new.to(module.squeeze.weight.device)
+    return list(made)
+
+
+def select_adapters(model: nn.Module, adapter: Tensor | None) -> None:
+    """Which adapter each element of a batch has: ``adapter [B]`` int32 on the device (-1: none), for all adapted ops of
+    ``model``; None: the first for all."""
+    from foldforge_amd.modules import TransitionAdapters
+
+    for module in model.modules():
+        if isinstance(module, TransitionAdapters):
+            module.adapter = adapter
 
 
 def wanted(module: nn.Module, *inputs: Tensor) -> bool:

@@ -1,0 +1,162 @@
+"""Dropout and adapters in the op classes, on the CPU: the ``pytorch`` backend's masks are the oracle's, rates and axes per op,
+batches with an adapter each against merged weights."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from foldforge_amd import dispatch, factories, modules, torch_ops, training
+from foldforge_amd.trunk import randomise
+from oracle import training as oracle
+
+
+def _block(p_drop=0.25, **how):
+    block = modules.PairformerBlock(modules.PairformerConfig(d_pair=64, d_hidden_tri_multi=64, d_hidden_tri_attention=16,
+                                                             p_drop=p_drop, **how))
+    return randomise(block, 3)
+
+
+def _inputs(n=9, batch=1, d=64):
+    g = torch.Generator().manual_seed(1)
+    mask = torch.ones(batch, n, dtype=torch.bool)
+    mask[:, -1] = False
+    return torch.randn(batch, n, n, d, generator=g), mask
+
+
+@pytest.mark.parametrize("shape,shared", [((5, 451), None), ((2, 5, 7, 12), 1), ((2, 5, 7, 12), 2), ((3, 1, 8), 0)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_plain_dropout_is_the_oracles(shape, shared, dtype):
+    g = torch.Generator().manual_seed(0)
+    x, res = torch.randn(*shape, generator=g).to(dtype), torch.randn(*shape, generator=g).to(dtype)
+    seed, offset = 2**62 + 12345, 2**40 + 7
+    got = torch_ops.dropout_add(x, res, shared=shared, dropped=round(65536 * 0.3), seed=seed, offset=offset)
+    want = oracle.dropout_add(x, res, shared, 0.3, seed, offset)
+    size = x.double().abs() * 65536 / (65536 - round(65536 * 0.3)) + res.double().abs()
+    assert ((got.double() - want).abs() <= 3 * 2.0**-24 * size + torch.finfo(dtype).eps / 2 * want.abs()).all()
+    alone = torch_ops.dropout_add(x, None, shared=shared, dropped=round(65536 * 0.3), seed=seed, offset=offset)
+    assert torch.equal(alone != 0, oracle.dropout_mask(shape, shared, 0.3, seed, offset).expand(shape) & (x != 0))
+
+
+def test_ops_get_their_rate_and_axis():
+    block = _block()
+    names = training.set_dropout(block, training.DropoutStream(5))
+    assert names == ["tri_multi_outgoing", "tri_multi_incoming", "tri_atten_starting", "tri_atten_ending"]
+    assert [getattr(block, n).dropout.axis for n in names] == [1, 1, 1, 2]
+    assert all(getattr(block, n).dropout.p == 0.25 for n in names)
+    assert not any("dropout" in k for k in block.state_dict())
+    assert training.set_dropout(block, training.DropoutStream(5), p=0.0) == []
+    assert block.tri_atten_ending.active_dropout() is None
+    assert training.set_dropout(_block(p_drop=0.0), training.DropoutStream(5)) == []
+    msa = factories.msa_pair_weighted_averaging(64, 128)
+    assert training.set_dropout(msa, training.DropoutStream(5), p=0.15) == [""] and msa.dropout.axis == 1
+    with pytest.raises(ValueError, match="p must"):
+        training.set_dropout(block, training.DropoutStream(5), p=1.5)
+
+
+@pytest.mark.parametrize("parallel", [False, True])
+def test_block_drops_each_update(parallel):
+    """Every op's own update through the mask of its draw, in order; none in evaluation mode."""
+    block, (z, mask) = _block(parallel=parallel), _inputs()
+    plain = block(z, mask)
+    training.set_dropout(block, training.DropoutStream(11))
+    block.eval()
+    assert torch.equal(block(z, mask), plain)
+    block.train()
+    got = block(z, mask)
+    ops = [(block.tri_multi_outgoing, 1), (block.tri_multi_incoming, 1), (block.tri_atten_starting, 1),
+           (block.tri_atten_ending, 2)]
+    want, updates = z, []
+    for i, (op, axis) in enumerate(ops):
+        update = op._forward_pytorch(z if parallel else want, mask, residual=False)
+        dropped = oracle.dropout_add(update, None, axis, 0.25, 11, i).float()
+        updates.append(dropped)
+        want = want + dropped
+    want = z + sum(updates) + block.transition_pair.delta(z) if parallel else block.transition_pair(want)
+    assert torch.allclose(got, want, rtol=1e-5, atol=1e-5)
+    assert not torch.equal(block(z, mask), got)  # the next draws
+    training.set_dropout(block, None)
+    assert torch.equal(block(z, mask), plain)
+
+
+def test_stream_goes_on_from_a_checkpoint():
+    block, (z, mask) = _block(), _inputs()
+    stream = training.DropoutStream(11)
+    training.set_dropout(block, stream)
+    block(z, mask)
+    seed, offset = stream.seed, stream.offset
+    want = block(z, mask)
+    training.set_dropout(block, training.DropoutStream(seed, offset))
+    assert torch.equal(block(z, mask), want)
+
+
+def test_calls_are_counted_where_they_run():
+    block, (z, mask) = _block(), _inputs()
+    training.set_dropout(block, training.DropoutStream(1))
+    dispatch.clear_ledgers(block)
+    block(z, mask)
+    assert dispatch.served_count(block, "pytorch") == 5
+    assert dispatch.ledger_of(block.tri_multi_outgoing.dropout).served["pytorch"] == 1
+
+
+def _adapted(batch=3, adapters=2, rank=4):
+    block = _block(p_drop=0.0)
+    names = training.adapt(block, rank, adapters=adapters, scale=0.5, seed=2)
+    assert names == ["transition_pair"]
+    g = torch.Generator().manual_seed(4)
+    ad = block.transition_pair.adapters
+    with torch.no_grad():
+        for n in ad.NAMES:
+            ad.matrices(n)[1].copy_(0.1 * torch.randn(ad.matrices(n)[1].shape, generator=g))
+    return block.transition_pair, _inputs(batch=batch)[0]
+
+
+def test_new_adapters_change_nothing():
+    block, (z, mask) = _block(p_drop=0.0), _inputs()
+    want = block(z, mask)
+    training.adapt(block, 8)
+    assert torch.equal(block(z, mask), want)
+    asks = {n for n, p in block.named_parameters() if p.requires_grad}
+    assert asks == {f"transition_pair.adapters.{m}_{k}" for m in ("expand_a", "expand_b", "squeeze") for k in ("down", "up")}
+    assert all(p.dtype == torch.float32 for p in block.transition_pair.adapters.parameters())
+
+
+def test_each_batch_element_runs_its_own_adapter():
+    """Against the transition with W + s B A for its weights."""
+    tr, z = _adapted()
+    training.select_adapters(tr, torch.tensor([1, -1, 0], dtype=torch.int32))
+    got = tr(z)
+    for b, a in enumerate((1, -1, 0)):
+        merged = modules.Transition(tr.d, tr.n)
+        merged.load_state_dict({k: v for k, v in tr.state_dict().items() if not k.startswith("adapters")})
+        if a >= 0:
+            with torch.no_grad():
+                for n in tr.adapters.NAMES:
+                    down, up = tr.adapters.matrices(n)
+                    getattr(merged, n).weight += 0.5 * up[a] @ down[a]
+        assert torch.allclose(got[b:b + 1], merged(z[b:b + 1]), rtol=1e-4, atol=1e-5)
+    with pytest.raises(ValueError, match="batch"):
+        tr(z[:2])
+    training.select_adapters(tr, None)
+    assert not torch.equal(tr(z)[1], got[1])
+
+
+def test_gradients_reach_the_adapters_alone():
+    tr, z = _adapted()
+    training.select_adapters(tr, torch.tensor([1, 1, -1], dtype=torch.int32))
+    tr(z).square().sum().backward()
+    for n, p in tr.named_parameters():
+        assert (p.grad is not None) == n.startswith("adapters"), n
+    assert not tr.adapters.squeeze_up.grad[0].any() and tr.adapters.squeeze_up.grad[1].any()
+
+
+def test_refusals():
+    block = _block()
+    with pytest.raises(ValueError, match="rank"):
+        training.adapt(block, 129)
+    assert block.transition_pair.adapters is None and block.transition_pair.squeeze.weight.requires_grad
+    x = torch.zeros(2, 8, dtype=torch.bfloat16)
+    w = torch.zeros(8, 8, requires_grad=True)
+    with pytest.raises(ValueError, match="frozen"):
+        training.adapted_linear(x, w, down=torch.zeros(1, 2, 8), up=torch.zeros(1, 8, 2),
+                                offsets=torch.zeros(2, dtype=torch.int32), adapter=torch.zeros(1, dtype=torch.int32))
