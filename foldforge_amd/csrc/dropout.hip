@@ -121,7 +121,8 @@ __global__ __launch_bounds__(256) void dropout_shared(const DropoutArgs a, int l
   const T* x = static_cast<const T*>(a.x);
   const T* res = static_cast<const T*>(a.residual);
   for (int64_t w = blockIdx.x; w < a.outer * tiles * chunks; w += gridDim.x) {
-    const int64_t chunk = w % chunks, tile = w / chunks % tiles, o = w / chunks / tiles;
+    // (neighbours beside each other in memory)
+    const int64_t tile = w % tiles, chunk = w / tiles % chunks, o = w / tiles / chunks;
     const int64_t i = 8 * (tile * lanes + (threadIdx.x & (lanes - 1)));
     if (i >= a.inner) continue;
     const int count = a.inner - i < 8 ? (int)(a.inner - i) : 8;
