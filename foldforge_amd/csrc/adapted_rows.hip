@@ -429,6 +429,7 @@ __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p
   using S = RowsGradShape<CI, CO, RB>;
   constexpr int TM = 32, STAGES = S::STAGES, PAIRS = (RB + 1) / 2, TILE = TM * (CI + CO);
   __shared__ __attribute__((aligned(1024))) bf16 buf[STAGES][TILE];
+  static_assert(STAGES == 3, "");
   __shared__ __attribute__((aligned(16))) f32x4 part[S::SI + S::SO][2][RB][64];
   __shared__ __attribute__((aligned(16))) bf16 stage[S::STAGED ? TM * CI : 8];
   __shared__ __attribute__((aligned(16))) bf16x4 vop[2][PAIRS][64][2];
@@ -583,32 +584,125 @@ __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p
     }
   };
   clear();
-  if (first + STAGES - 1 <= last)
-    wait_vm_lds<(STAGES - 2) * S::PER>();
+  f32x4 acc[S::NB][S::TT];
+  // What is left of rows lo to hi of the tile at xs (request r): their part of dx beyond dy W, and the gradients' sums
+  auto finish = [&](uint32_t xs, int lo, int hi, int r) __attribute__((always_inline)) {
+    const uint32_t ys = xs + 2 * TM * CI;
+    const bool whole = lo == 0 && hi == TM;
+    if (summed != r) {
+      if (summed >= 0) {
+        flush();
+        clear();
+      }
+      summed = r;
+    }
+    if (p.dx) {
+#pragma unroll
+      for (int x = 0; x < S::TT; ++x) {
+        const int mine = r0 + 16 * x + i;
+#pragma unroll
+        for (int b = 0; b < S::NB; ++b) {
+          f32x4 add = none;
+#pragma unroll
+          for (int s = 0; s < PAIRS; ++s)
+            add = mfma16(at_[b][s], *reinterpret_cast<const bf16x8*>(&vop[r0 / 16 + x][s][lane][0]), add);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[b][x][e] += mine >= lo && mine < hi ? add[e] : 0.f;
+        }
+      }
+    }
+    // tokens as k: element e of lane group g is token 4 g + e, or 16 + 4 g + e - 4; those of other requests are left out
+    auto turned = [&](bf16x8 v) __attribute__((always_inline)) {
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int t = 16 * (e >> 2) + 4 * g + (e & 3);
+          v[e] = t >= lo && t < hi ? v[e] : (bf16)0.f;
+        }
+      }
+      return v;
+    };
+    const uint32_t xa = xs + turned_at<CI>(lane), ya = ys + turned_at<CO>(lane);
+    bf16x8 gv[RB][3];
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+      for (int k = 0; k < 3; ++k) gv[b][k] = ld8(&gop[1][k][b][lane][0]);
+#pragma unroll
+    for (int q = 0; q < S::GI; ++q)
+      if (8 * q + wave < CI / 16) {
+        const bf16x8 t = turned(ld_turned16<CI>(xa ^ (uint32_t)(8 * q + wave) << 5));
+#pragma unroll
+        for (int b = 0; b < RB; ++b)
+#pragma unroll
+          for (int k = 0; k < 3; ++k) gi[b][q] = mfma16(gv[b][k], t, gi[b][q]);
+      }
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+      for (int k = 0; k < 3; ++k) gv[b][k] = ld8(&gop[0][k][b][lane][0]);
+#pragma unroll
+    for (int q = 0; q < S::GO; ++q)
+      if (8 * q + wave < CO / 16) {
+        const bf16x8 t = turned(ld_turned16<CO>(ya ^ (uint32_t)(8 * q + wave) << 5));
+#pragma unroll
+        for (int b = 0; b < RB; ++b)
+#pragma unroll
+          for (int k = 0; k < 3; ++k) go[b][q] = mfma16(gv[b][k], t, go[b][q]);
+      }
+  };
+  // dx of the tile at row0: to the stage, or to its rows
+  auto emit = [&](int64_t row0) __attribute__((always_inline)) {
+    if constexpr (S::STAGED) {
+#pragma unroll
+      for (int x = 0; x < S::TT; ++x) {
+        bf16x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (bf16)acc[0][x][e];
+        const int n = n0 + 4 * g;
+        *reinterpret_cast<bf16x4*>(&stage[off_row<CI>(r0 + 16 * x + i, n >> 3) + (n & 7)]) = v;
+      }
+    } else {
+      bf16* to = p.dx + (row0 + r0 + i) * CI + n0 + 16 * (g & 1) + 8 * (g >> 1);
+#pragma unroll
+      for (int x = 0; x < S::TT; ++x) {
+        bf16x8 v[(S::NB + 1) / 2];
+#pragma unroll
+        for (int b = 0; b < S::NB / 2; ++b) v[b] = join_blocks(acc[2 * b][x], acc[2 * b + 1][x]);
+        if (rows - row0 < TM && row0 + r0 + 16 * x + i >= rows) continue;
+#pragma unroll
+        for (int b = 0; b < S::NB / 2; ++b)
+          __builtin_nontemporal_store(v[b], reinterpret_cast<bf16x8*>(to + 16 * x * CI + 32 * b));
+      }
+    }
+  };
+  if (first + 1 < last)
+    wait_vm_lds<S::PER>();
   else
     wait_vm_lds<0>();
   __syncthreads();
-  for (int64_t tile = first; tile < last; ++tile) {
-    if (tile + STAGES - 1 < last) fetch(tile + STAGES - 1);
-    if (p.dx && tile > first) put((tile - 1) * TM);
-    const int64_t row0 = tile * TM, end = row0 + TM < rows ? row0 + TM : rows;
-    const uint32_t xs = lds + (uint32_t)((tile - first) % STAGES) * sizeof(buf[0]), ys = xs + 2 * TM * CI;
-    f32x4 acc[S::NB][S::TT];
-    for (int64_t row = row0; row < end;) {  // the requests in this tile
-      request_next(p.q, row, at);
-      const int64_t stop = at.hi < end ? at.hi : end;
-      const bool whole = row == row0 && stop == row0 + TM;
+  // A step is the rows of one request in one tile: what is left of the step before, beside this one's products, and behind a
+  // barrier the join of the thin ones. So two barriers a step, and in the longer half the matrix instructions of one step hide
+  // the latencies of another's. A tile's buffer is free for the tile two on in the second half of the next tile's first step.
+  uint32_t xs0 = 0;  // the step before: its tile, rows and request (-1: none, or no adapter)
+  int lo0 = 0, hi0 = 0, r0_ = -1;
+  for (int64_t tile = first;;) {
+    int lo = 0, hi;
+    const int64_t row0 = tile * TM;
+    const int end = rows - row0 < TM ? (int)(rows - row0) : TM;
+    const uint32_t xs = lds + (uint32_t)((tile - first) % 3) * sizeof(buf[0]), ys = xs + 2 * TM * CI;
+    do {
+      if (r0_ >= 0) finish(xs0, lo0, hi0, r0_);
+      if (lo == 0 && p.dx && tile > first) emit(row0 - TM);
+      if (tile >= last) goto done;
+      request_next(p.q, row0 + lo, at);
+      hi = __builtin_amdgcn_readfirstlane(at.hi - row0 < end ? (int)(at.hi - row0) : end);
       if (at.a >= 0) {
-        if (summed >= 0 && summed != at.r) {
-          flush();
-          clear();
-        }
-        summed = at.r;
         if (at.a != loaded) load(at.a);
         thin_part<CI, S::SI, S::QI, S::XI>(xs + 2 * off_row<CI>(i, g), wave, lane, am, part);
         thin_part<CO, S::SO, S::QO, S::XO>(ys + 2 * off_row<CO>(i, g), wave, lane, bm, part + S::SI);
       }
-      if (row == row0 && p.dx) {
+      if (lo == 0 && p.dx) {
 #pragma unroll
         for (int b = 0; b < S::NB; ++b)
 #pragma unroll
@@ -624,124 +718,49 @@ __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p
             if (x == S::TT - 1 && k % (8 / S::TT) == 8 / S::TT - 1) __builtin_amdgcn_sched_barrier(0);
           }
       }
-      if (at.a >= 0) {
-        __syncthreads();
-        if (threadIdx.x < 256 * RB) {
-          const int l = threadIdx.x & 63, b = (threadIdx.x >> 6) % RB, x = (threadIdx.x >> 6) / RB & 1;
-          const int y = (threadIdx.x >> 6) / RB >> 1, token = 16 * x + (l & 15);
-          const f32x4(*from)[2][RB][64] = part + (y ? S::SI : 0);
-          f32x4 v = from[0][x][b][l];
-          for (int s = 1; s < (y ? S::SO : S::SI); ++s) v += from[s][x][b][l];
-          const bool in = row0 + token >= row && row0 + token < stop;
-          bf16x4 high;
+      __syncthreads();
+      if (lo == 0 && tile + 2 < last) fetch(tile + 2);
+      if (at.a >= 0 && threadIdx.x < 256 * RB) {
+        const int l = threadIdx.x & 63, b = (threadIdx.x >> 6) % RB, x = (threadIdx.x >> 6) / RB & 1;
+        const int y = (threadIdx.x >> 6) / RB >> 1, token = 16 * x + (l & 15);
+        const f32x4(*from)[2][RB][64] = part + (y ? S::SI : 0);
+        f32x4 v = from[0][x][b][l];
+        for (int s = 1; s < (y ? S::SO : S::SI); ++s) v += from[s][x][b][l];
+        const bool in = token >= lo && token < hi;
+        bf16x4 high;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            bf16 t[3];
-            split3(in ? v[e] * scale : 0.f, t);
-            high[e] = t[0];
+        for (int e = 0; e < 4; ++e) {
+          bf16 t[3];
+          split3(in ? v[e] * scale : 0.f, t);
+          high[e] = t[0];
 #pragma unroll
-            for (int k = 0; k < 3; ++k) gop[y][k][b][4 * (l >> 4) + e + 16 * (l >> 2 & 3)][4 * x + (l & 3)] = t[k];
-          }
-          if (y) vop[x][b / 2][l][b & 1] = high;
+          for (int k = 0; k < 3; ++k) gop[y][k][b][4 * (l >> 4) + e + 16 * (l >> 2 & 3)][4 * x + (l & 3)] = t[k];
         }
-        __syncthreads();
-        if (p.dx) {
-#pragma unroll
-          for (int x = 0; x < S::TT; ++x) {
-            const int64_t mine = row0 + r0 + 16 * x + i;
-#pragma unroll
-            for (int b = 0; b < S::NB; ++b) {
-              f32x4 add = none;
-#pragma unroll
-              for (int s = 0; s < PAIRS; ++s)
-                add = mfma16(at_[b][s], *reinterpret_cast<const bf16x8*>(&vop[r0 / 16 + x][s][lane][0]), add);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) acc[b][x][e] += mine >= row && mine < stop ? add[e] : 0.f;
-            }
-          }
-        }
-        // tokens as k: element e of lane group g is token 4 g + e, or 16 + 4 g + e - 4; those of other requests are left out
-        auto turned = [&](bf16x8 v) __attribute__((always_inline)) {
-          if (!whole) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int64_t r = row0 + 16 * (e >> 2) + 4 * g + (e & 3);
-              v[e] = r >= row && r < stop ? v[e] : (bf16)0.f;
-            }
-          }
-          return v;
-        };
-        const uint32_t xa = xs + turned_at<CI>(lane), ya = ys + turned_at<CO>(lane);
-        bf16x8 gv[RB][3];
-#pragma unroll
-        for (int b = 0; b < RB; ++b)
-#pragma unroll
-          for (int k = 0; k < 3; ++k) gv[b][k] = ld8(&gop[1][k][b][lane][0]);
-#pragma unroll
-        for (int q = 0; q < S::GI; ++q)
-          if (8 * q + wave < CI / 16) {
-            const bf16x8 t = turned(ld_turned16<CI>(xa ^ (uint32_t)(8 * q + wave) << 5));
-#pragma unroll
-            for (int b = 0; b < RB; ++b)
-#pragma unroll
-              for (int k = 0; k < 3; ++k) gi[b][q] = mfma16(gv[b][k], t, gi[b][q]);
-          }
-#pragma unroll
-        for (int b = 0; b < RB; ++b)
-#pragma unroll
-          for (int k = 0; k < 3; ++k) gv[b][k] = ld8(&gop[0][k][b][lane][0]);
-#pragma unroll
-        for (int q = 0; q < S::GO; ++q)
-          if (8 * q + wave < CO / 16) {
-            const bf16x8 t = turned(ld_turned16<CO>(ya ^ (uint32_t)(8 * q + wave) << 5));
-#pragma unroll
-            for (int b = 0; b < RB; ++b)
-#pragma unroll
-              for (int k = 0; k < 3; ++k) go[b][q] = mfma16(gv[b][k], t, go[b][q]);
-          }
-      } else if (row == row0) {
-        __syncthreads();  // (the last tile's dx has left the stage)
+        if (y) vop[x][b / 2][l][b & 1] = high;
       }
-      row = stop;
-    }
-    if constexpr (S::STAGED) {
-      if (p.dx) {
-#pragma unroll
-        for (int x = 0; x < S::TT; ++x) {
-          bf16x4 v;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = (bf16)acc[0][x][e];
-          const int n = n0 + 4 * g;
-          *reinterpret_cast<bf16x4*>(&stage[off_row<CI>(r0 + 16 * x + i, n >> 3) + (n & 7)]) = v;
-        }
+      if (lo == 0) {
+        if (p.dx && tile > first) put(row0 - TM);
+        // The next tile has landed: behind its transfers lie those of the tile after it and the stores since then (of whole
+        // tiles): the wave's memory operations complete in order.
+        constexpr int BEHIND = S::PER + (S::STAGED ? 2 : 1) * S::STORES;
+        if (tile + 2 >= last)
+          wait_vm_lds<0>();
+        else if (p.dx && tile - first >= 2)
+          wait_vm_lds<BEHIND>();
+        else
+          wait_vm_lds<S::PER>();
       }
-    }
-    // The next tile has landed. Behind its transfers lie those of the tiles after it and the stores of each iteration since
-    // then (of whole tiles): the wave's memory operations complete in order.
-    constexpr int BEHIND = (STAGES - 2) * S::PER + (S::STAGED ? STAGES - 1 : STAGES - 2) * S::STORES;
-    if (tile + STAGES - 1 >= last)
-      wait_vm_lds<0>();
-    else if (p.dx && tile - first >= STAGES - 1)
-      wait_vm_lds<BEHIND>();
-    else
-      wait_vm_lds<(STAGES - 2) * S::PER>();
-    if constexpr (!S::STAGED) {
-      if (p.dx) {
-        bf16* to = p.dx + (row0 + r0 + i) * CI + n0 + 16 * (g & 1) + 8 * (g >> 1);
-#pragma unroll
-        for (int x = 0; x < S::TT; ++x) {
-          bf16x8 v[(S::NB + 1) / 2];
-#pragma unroll
-          for (int b = 0; b < S::NB / 2; ++b) v[b] = join_blocks(acc[2 * b][x], acc[2 * b + 1][x]);
-          if (end - row0 < TM && row0 + r0 + 16 * x + i >= rows) continue;
-#pragma unroll
-          for (int b = 0; b < S::NB / 2; ++b)
-            __builtin_nontemporal_store(v[b], reinterpret_cast<bf16x8*>(to + 16 * x * CI + 32 * b));
-        }
-      }
-    }
-    __syncthreads();
+      __syncthreads();
+      xs0 = xs;
+      lo0 = lo;
+      hi0 = hi;
+      r0_ = at.a >= 0 ? at.r : -1;
+      lo = hi;
+    } while (lo < end);
+    ++tile;
   }
+done:
+  __syncthreads();
   if (first < last) {
     if (p.dx) put((last - 1) * TM);
     if (summed >= 0) flush();
