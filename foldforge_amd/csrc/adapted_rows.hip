@@ -391,8 +391,12 @@ struct RowsGradShape {
   static constexpr int PER = (CI + CO + 127) / 128;                // transfers of a tile a wave
   static constexpr bool STAGED = NB < 2;                           // dx goes through LDS: 16 channels a wave are 32 bytes a row
   static constexpr int STORES = STAGED ? CI / 128 : NB / 2 * TT;   // stores of a tile a wave (some more with 64 channels)
-  static constexpr int STAGES = RB == 1 || CI + CO < 512 ? 3 : 2;
 };
+
+// 16 x 16 x 16: lane group g holds k from 4 g on.
+__device__ __forceinline__ f32x4 mfma16_16(bf16x4 a, bf16x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+}
 
 // A wave's part of a thin product of 32 rows: steps wave % SLOTS + SLOTS q of k, X blocks of 16 rows.
 template <int C, int SLOTS, int Q, int X, int RB, int PARTS>
@@ -420,30 +424,32 @@ __device__ __forceinline__ void thin_part(uint32_t at, int wave, int lane, const
 
 // dx = dy W + v A_a, and the sums over this workgroup's rows of v^T x and u^T dy for each request in them (to
 // part[blockIdx.x + request]: a walk through the (workgroup, request) pairs in row order takes each such sum once). Tiles of 32
-// rows of x and dy stream through LDS. The thin products, u = s x A^T and v = s dy B, are split over the waves by k;
-// half the threads join the parts and lays u and v out as operands: v rounded with tokens as columns,
-// for dx, both in three parts with tokens as k, for the gradients, whose other operand is the tile turned as it is read. dx
-// goes through LDS to stores of whole rows. PARTS = 3: fp32 adapters. block 512.
+// rows of x and dy stream through LDS. The thin products, u = s x A^T and v = s dy B, are split over the waves by k; half the
+// waves join the parts and lay u and v out as operands: v with tokens as columns for dx (rounded to bf16 as dy is), both in
+// three bf16 parts with tokens as k for the gradients (their sum is as exact as fp32's), whose other operand is the tile turned
+// as it is read. dx of 16 channels a wave goes through LDS to stores of whole rows. PARTS = 3: fp32 adapters, in three parts
+// as well. block 512.
+// 262144 rows, 128 -> 512, rank 16: 140 us, of which the rows' traffic (403 MB at the rate of a copy) is 79; a step's own work
+// is about as long, and one workgroup of a compute unit has only its own eight waves to hide it with. Measured and not
+// kept: dy W by halves of k with half the reads of dy (143 us, and 3 us more for few rows), three barriers a step (144).
 template <int CI, int CO, int RB, int PARTS>
 __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p) {
   using S = RowsGradShape<CI, CO, RB>;
-  constexpr int TM = 32, STAGES = S::STAGES, PAIRS = (RB + 1) / 2, TILE = TM * (CI + CO);
-  __shared__ __attribute__((aligned(1024))) bf16 buf[STAGES][TILE];
-  static_assert(STAGES == 3, "");
+  constexpr int TM = 32, TILE = TM * (CI + CO);
+  __shared__ __attribute__((aligned(1024))) bf16 buf[3][TILE];
   __shared__ __attribute__((aligned(16))) f32x4 part[S::SI + S::SO][2][RB][64];
   __shared__ __attribute__((aligned(16))) bf16 stage[S::STAGED ? TM * CI : 8];
-  __shared__ __attribute__((aligned(16))) bf16x4 vop[2][PAIRS][64][2];
+  __shared__ __attribute__((aligned(16))) bf16x4 vop[2][RB][64];
   __shared__ __attribute__((aligned(16))) bf16 gop[2][3][RB][64][8];
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t rows = p.q.rows, tiles = (rows + TM - 1) / TM;
-  const int64_t first = tiles * blockIdx.x / gridDim.x, last = tiles * (blockIdx.x + 1) / gridDim.x;
+  const int first = (int)(tiles * blockIdx.x / gridDim.x), last = (int)(tiles * (blockIdx.x + 1) / gridDim.x);
   const uint32_t lds = lds_addr(buf);
   RequestAt at{p.q.count, -1, rows};
-  if (first < last) at = request_first(p.q, first * TM, lane);  // (ahead of the transfers, which it would wait for)
-  auto fetch = [&](int64_t tile) __attribute__((always_inline)) {
-    const uint32_t dst = lds + (uint32_t)((tile - first) % STAGES) * sizeof(buf[0]);
-    const int64_t row0 = tile * TM;
+  if (first < last) at = request_first(p.q, (int64_t)first * TM, lane);  // (ahead of the transfers, which it would wait for)
+  auto fetch = [&](int tile, uint32_t dst) __attribute__((always_inline)) {
+    const int64_t row0 = (int64_t)tile * TM;
     const int lane = fresh_lane();
 #pragma unroll
     for (int u = 0; u < S::PER; ++u) {
@@ -460,9 +466,8 @@ __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p
       }
     }
   };
-#pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s)
-    if (first + s < last) fetch(first + s);
+  if (first < last) fetch(first, lds);
+  if (first + 1 < last) fetch(first + 1, lds + sizeof(buf[0]));
   const f32x4 none = {0.f, 0.f, 0.f, 0.f};
   // W^T: this wave's channels of dx
   const int n0 = 16 * S::NB * (wave % S::NW), r0 = 16 * S::TT * (wave / S::NW);
@@ -479,14 +484,10 @@ __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p
         }
     });
   }
-  if (threadIdx.x < 2 * PAIRS * 64) {
-    const bf16x4 z = {(bf16)0.f, (bf16)0.f, (bf16)0.f, (bf16)0.f};
-    (&vop[0][0][0][0])[2 * threadIdx.x] = z;
-    (&vop[0][0][0][0])[2 * threadIdx.x + 1] = z;
-  }
   // the adapter: its share of the thin products (steps wave % S + S q of k, row blocks from wave / S on), this wave's channels
   // of A for dx
-  bf16x8 am[S::QI][RB][PARTS], bm[S::QO][RB][PARTS], at_[S::NB][PAIRS];
+  bf16x8 am[S::QI][RB][PARTS], bm[S::QO][RB][PARTS];
+  bf16x4 at_[S::NB][RB];
   float scale = 1.f;
   int loaded = -1;
   auto load = [&](int a) __attribute__((always_inline)) {
@@ -513,13 +514,12 @@ __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p
 #pragma unroll
       for (int b = 0; b < S::NB; ++b)
 #pragma unroll
-        for (int s = 0; s < PAIRS; ++s)
+        for (int s = 0; s < RB; ++s)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int j = 32 * s + 16 * (e >> 2) + 4 * g + (e & 3);
-            const bool is = j < p.rank && (RB > 1 || e < 4);
-            const float v = (float)from[(is ? j : p.rank - 1) * CI + n0 + 16 * b + i];
-            at_[b][s][e] = is ? (bf16)v : (bf16)0.f;
+          for (int e = 0; e < 4; ++e) {
+            const int j = 16 * s + 4 * g + e;
+            const float v = (float)from[(j < p.rank ? j : p.rank - 1) * CI + n0 + 16 * b + i];
+            at_[b][s][e] = j < p.rank ? (bf16)v : (bf16)0.f;
           }
     });
     typed(p.up, p.a_f32, [&](const auto* all) __attribute__((always_inline)) {
@@ -604,8 +604,7 @@ __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p
         for (int b = 0; b < S::NB; ++b) {
           f32x4 add = none;
 #pragma unroll
-          for (int s = 0; s < PAIRS; ++s)
-            add = mfma16(at_[b][s], *reinterpret_cast<const bf16x8*>(&vop[r0 / 16 + x][s][lane][0]), add);
+          for (int s = 0; s < RB; ++s) add = mfma16_16(at_[b][s], vop[r0 / 16 + x][s][lane], add);
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[b][x][e] += mine >= lo && mine < hi ? add[e] : 0.f;
         }
@@ -686,11 +685,12 @@ __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p
   // the latencies of another's. A tile's buffer is free for the tile two on in the second half of the next tile's first step.
   uint32_t xs0 = 0;  // the step before: its tile, rows and request (-1: none, or no adapter)
   int lo0 = 0, hi0 = 0, r0_ = -1;
-  for (int64_t tile = first;;) {
+  uint32_t xs = lds;  // this tile's buffer, of three in turn
+  for (int tile = first;; ++tile) {
     int lo = 0, hi;
-    const int64_t row0 = tile * TM;
+    const int64_t row0 = (int64_t)tile * TM;
     const int end = rows - row0 < TM ? (int)(rows - row0) : TM;
-    const uint32_t xs = lds + (uint32_t)((tile - first) % 3) * sizeof(buf[0]), ys = xs + 2 * TM * CI;
+    const uint32_t ys = xs + 2 * TM * CI;
     do {
       if (r0_ >= 0) finish(xs0, lo0, hi0, r0_);
       if (lo == 0 && p.dx && tile > first) emit(row0 - TM);
@@ -719,10 +719,10 @@ __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p
           }
       }
       __syncthreads();
-      if (lo == 0 && tile + 2 < last) fetch(tile + 2);
-      if (at.a >= 0 && threadIdx.x < 256 * RB) {
-        const int l = threadIdx.x & 63, b = (threadIdx.x >> 6) % RB, x = (threadIdx.x >> 6) / RB & 1;
-        const int y = (threadIdx.x >> 6) / RB >> 1, token = 16 * x + (l & 15);
+      if (lo == 0 && tile + 2 < last) fetch(tile + 2, xs == lds ? lds + 2 * sizeof(buf[0]) : xs - sizeof(buf[0]));
+      if (at.a >= 0 && wave < 4 * RB) {
+        const int l = lane, b = wave % RB, x = wave / RB & 1;
+        const int y = wave / RB >> 1, token = 16 * x + (l & 15);
         const f32x4(*from)[2][RB][64] = part + (y ? S::SI : 0);
         f32x4 v = from[0][x][b][l];
         for (int s = 1; s < (y ? S::SO : S::SI); ++s) v += from[s][x][b][l];
@@ -736,7 +736,7 @@ __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p
 #pragma unroll
           for (int k = 0; k < 3; ++k) gop[y][k][b][4 * (l >> 4) + e + 16 * (l >> 2 & 3)][4 * x + (l & 3)] = t[k];
         }
-        if (y) vop[x][b / 2][l][b & 1] = high;
+        if (y) vop[x][b][l] = high;
       }
       if (lo == 0) {
         if (p.dx && tile > first) put(row0 - TM);
@@ -757,12 +757,12 @@ __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p
       r0_ = at.a >= 0 ? at.r : -1;
       lo = hi;
     } while (lo < end);
-    ++tile;
+    xs = xs == lds + 2 * sizeof(buf[0]) ? lds : xs + sizeof(buf[0]);
   }
 done:
   __syncthreads();
   if (first < last) {
-    if (p.dx) put((last - 1) * TM);
+    if (p.dx) put((int64_t)(last - 1) * TM);
     if (summed >= 0) flush();
   }
 }
