@@ -450,19 +450,17 @@ __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p
   if (first < last) at = request_first(p.q, (int64_t)first * TM, lane);  // (ahead of the transfers, which it would wait for)
   auto fetch = [&](int tile, uint32_t dst) __attribute__((always_inline)) {
     const int64_t row0 = (int64_t)tile * TM;
-    const int lane = fresh_lane();
+    const int lane = fresh_lane(), left = rows - row0 < TM ? (int)(rows - row0) : TM;
 #pragma unroll
     for (int u = 0; u < S::PER; ++u) {
       // (all waves the same number of transfers, the last one again where they do not go round)
       const int t = wave * S::PER + u < (CI + CO) / 16 ? wave * S::PER + u : (CI + CO) / 16 - 1;
       if (t < CI / 16) {
-        const int r = 512 / CI * t + lane / (CI / 8);
-        const int64_t row = row0 + r < rows ? row0 + r : rows - 1;
-        dma16_at(p.x + row * CI + 8 * ((lane % (CI / 8)) ^ swz<CI>(r)), dst + 1024 * t);
+        const int r = 512 / CI * t + lane / (CI / 8), row = r < left ? r : left - 1;
+        dma16(p.x + row0 * CI, (uint32_t)(2 * CI * row + 16 * ((lane % (CI / 8)) ^ swz<CI>(r))), dst + 1024 * t);
       } else {
-        const int r = 512 / CO * (t - CI / 16) + lane / (CO / 8);
-        const int64_t row = row0 + r < rows ? row0 + r : rows - 1;
-        dma16_at(p.dy + row * CO + 8 * ((lane % (CO / 8)) ^ swz<CO>(r)), dst + 1024 * t);
+        const int r = 512 / CO * (t - CI / 16) + lane / (CO / 8), row = r < left ? r : left - 1;
+        dma16(p.dy + row0 * CO, (uint32_t)(2 * CO * row + 16 * ((lane % (CO / 8)) ^ swz<CO>(r))), dst + 1024 * t);
       }
     }
   };
@@ -572,15 +570,15 @@ __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p
   // this wave's rows of the staged dx
   auto put = [&](int64_t row0) __attribute__((always_inline)) {
     if constexpr (!S::STAGED) return;
-    const int lane = fresh_lane();
+    const int lane = fresh_lane(), left = rows - row0 < TM ? (int)(rows - row0) : TM;
 #pragma unroll
     for (int u = 0; u < (S::STORES > 0 ? S::STORES : 1); ++u) {
       const int t = wave * (S::STORES > 0 ? S::STORES : 1) + u;
       if (CI == 64 && wave >= 4) continue;
       const int r = 512 / CI * t + lane / (CI / 8), piece = lane % (CI / 8);
-      if (row0 + r < rows)
+      if (r < left)
         __builtin_nontemporal_store(ld8(&stage[off_row<CI>(r, piece)]),
-                                    reinterpret_cast<bf16x8*>(p.dx + (row0 + r) * CI + 8 * piece));
+                                    reinterpret_cast<bf16x8*>(p.dx + row0 * CI + (r * CI + 8 * piece)));
     }
   };
   clear();
@@ -662,13 +660,14 @@ __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p
         *reinterpret_cast<bf16x4*>(&stage[off_row<CI>(r0 + 16 * x + i, n >> 3) + (n & 7)]) = v;
       }
     } else {
-      bf16* to = p.dx + (row0 + r0 + i) * CI + n0 + 16 * (g & 1) + 8 * (g >> 1);
+      const int left = rows - row0 < TM ? (int)(rows - row0) : TM;
+      bf16* to = p.dx + row0 * CI + ((r0 + i) * CI + n0 + 16 * (g & 1) + 8 * (g >> 1));
 #pragma unroll
       for (int x = 0; x < S::TT; ++x) {
         bf16x8 v[(S::NB + 1) / 2];
 #pragma unroll
         for (int b = 0; b < S::NB / 2; ++b) v[b] = join_blocks(acc[2 * b][x], acc[2 * b + 1][x]);
-        if (rows - row0 < TM && row0 + r0 + 16 * x + i >= rows) continue;
+        if (left < TM && r0 + 16 * x + i >= left) continue;
 #pragma unroll
         for (int b = 0; b < S::NB / 2; ++b)
           __builtin_nontemporal_store(v[b], reinterpret_cast<bf16x8*>(to + 16 * x * CI + 32 * b));
