@@ -105,6 +105,13 @@ __device__ __forceinline__ int fresh_lane() {
   return l;
 }
 
+// A loaded value is there from here on. Before a loop with transfers in flight: the compiler's own wait for a load that it has
+// seen no use of before the loop would stand in the loop, at the first use, and be one for all transfers, each time round.
+template <typename T>
+__device__ __forceinline__ void landed(T& v) {
+  asm volatile("" : "+v"(v));
+}
+
 struct RowsArgs {
   const bf16* x;  // [rows][C]
   const void *w, *down, *up;
@@ -132,11 +139,11 @@ struct RowsShape {
 template <int C, int PER>
 __device__ __forceinline__ void rows_dma(const bf16* x, int64_t row0, int64_t rows, uint32_t dst, int wave, int lane) {
   constexpr int P = C / 8;  // pieces of a row
+  const int left = rows - row0 < PER * 4096 / C ? (int)(rows - row0) : PER * 4096 / C;
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
-    const int t = wave * PER + u, piece = 64 * t + lane, r = piece / P;
-    const int64_t row = row0 + r < rows ? row0 + r : rows - 1;
-    dma16_at(x + row * C + 8 * ((piece % P) ^ swz<C>(r)), dst + 1024 * t);
+    const int t = wave * PER + u, piece = 64 * t + lane, r = piece / P, row = r < left ? r : left - 1;
+    dma16(x + row0 * C, (uint32_t)(2 * C * row + 16 * ((piece % P) ^ swz<C>(r))), dst + 1024 * t);
   }
 }
 
@@ -173,17 +180,16 @@ __global__ __launch_bounds__(512, 2) void adapted_rows(const RowsArgs p, int sli
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t rows = p.q.rows, tiles = (rows + TM - 1) / TM;
   const int N = p.N, id = (int)xcd_remap(blockIdx.x, gridDim.x), range = id / slices, ranges = gridDim.x / slices;
-  const int64_t first = tiles * range / ranges, last = tiles * (range + 1) / ranges;
+  const int first = (int)(tiles * range / ranges), last = (int)(tiles * (range + 1) / ranges);
   const uint32_t lds = lds_addr(buf);
   RequestAt at{p.q.count, -1, rows};
-  if (first < last) at = request_first(p.q, first * TM, lane);  // (ahead of the transfers, which it would wait for)
-  auto fetch = [&](int64_t tile) __attribute__((always_inline)) {
-    rows_dma<C, S::PER>(p.x, tile * TM, rows, lds + (uint32_t)((tile - first) % STAGES) * sizeof(buf[0]), wave,
-                        fresh_lane());
+  if (first < last) at = request_first(p.q, (int64_t)first * TM, lane);  // (ahead of the transfers, which it would wait for)
+  auto fetch = [&](int tile, uint32_t dst) __attribute__((always_inline)) {
+    rows_dma<C, S::PER>(p.x, (int64_t)tile * TM, rows, dst, wave, fresh_lane());
   };
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s)
-    if (first + s < last) fetch(first + s);
+    if (first + s < last) fetch(first + s, lds + s * sizeof(buf[0]));
   // this wave's channels of W, and its rows of a tile
   const int n0 = NS * (id % slices) + 16 * S::NB * (wave % S::NW), r0 = 16 * S::TT * (wave / S::NW);
   bf16x8 w[S::NB][S::KS];
@@ -226,28 +232,42 @@ __global__ __launch_bounds__(512, 2) void adapted_rows(const RowsArgs p, int sli
         if (b % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       }
     });
+    landed(scale);
+#pragma unroll
+    for (int b = 0; b < S::NB; ++b)
+#pragma unroll
+      for (int s = 0; s < PAIRS; ++s) landed(bf[b][s]);
     __syncthreads();
   };
   if (at.a >= 0) load(at.a);
+#pragma unroll
+  for (int b = 0; b < S::NB; ++b) {
+    landed(bias[b]);
+#pragma unroll
+    for (int k = 0; k < S::KS; ++k) landed(w[b][k]);
+  }
   if (first + STAGES - 1 <= last)
     wait_vm_lds<(STAGES - 2) * S::PER>();
   else
     wait_vm_lds<0>();
   __syncthreads();
-  for (int64_t tile = first; tile < last; ++tile) {
-    if (tile + STAGES - 1 < last) fetch(tile + STAGES - 1);
-    const int64_t row0 = tile * TM, end = row0 + TM < rows ? row0 + TM : rows;
-    const uint32_t t = lds + (uint32_t)((tile - first) % STAGES) * sizeof(buf[0]) + 2 * off_row<C>(r0 + i, g);
+  uint32_t xs = lds;  // this tile's buffer
+  constexpr uint32_t TOP = (STAGES - 1) * sizeof(buf[0]);
+  for (int tile = first; tile < last; ++tile) {
+    if (tile + STAGES - 1 < last) fetch(tile + STAGES - 1, xs == lds ? lds + TOP : xs - sizeof(buf[0]));
+    const int64_t row0 = (int64_t)tile * TM;
+    const int end = rows - row0 < TM ? (int)(rows - row0) : TM;
+    const uint32_t t = xs + 2 * off_row<C>(r0 + i, g);
     f32x4 acc[S::NB][S::TT];
-    for (int64_t row = row0; row < end;) {  // the requests in this tile
-      request_next(p.q, row, at);
+    for (int lo = 0; lo < end;) {  // the requests in this tile
+      request_next(p.q, row0 + lo, at);
       if (at.a >= 0 && at.a != loaded) load(at.a);
       f32x4 u[RB][S::TT];
 #pragma unroll
       for (int x = 0; x < S::TT; ++x)
 #pragma unroll
         for (int b = 0; b < RB; ++b) u[b][x] = none;
-      if (row == row0) {
+      if (lo == 0) {
 #pragma unroll
         for (int x = 0; x < S::TT; ++x)
 #pragma unroll
@@ -276,12 +296,12 @@ __global__ __launch_bounds__(512, 2) void adapted_rows(const RowsArgs p, int sli
             for (int b = 0; b < RB; ++b)
               u[b][x] = mfma16(ld8(&af[b * S::KS + k][8 * lane]), row_operand<C>(t, x, k), u[b][x]);
       }
-      const int64_t stop = at.hi < end ? at.hi : end;
+      const int hi = __builtin_amdgcn_readfirstlane(at.hi - row0 < end ? (int)(at.hi - row0) : end);
       if (at.a >= 0) {
-        const bool whole = row == row0 && stop == end;
+        const bool whole = lo == 0 && hi == end;
 #pragma unroll
         for (int x = 0; x < S::TT; ++x) {
-          const int64_t mine = row0 + r0 + 16 * x + i;
+          const int mine = r0 + 16 * x + i;
           bf16x8 uf[PAIRS];
 #pragma unroll
           for (int s = 0; s < PAIRS; ++s)
@@ -302,12 +322,12 @@ __global__ __launch_bounds__(512, 2) void adapted_rows(const RowsArgs p, int sli
 #pragma unroll
               for (int s = 0; s < PAIRS; ++s) add = mfma16(bf[b][s], uf[s], add);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) acc[b][x][e] += mine >= row && mine < stop ? add[e] : 0.f;
+              for (int e = 0; e < 4; ++e) acc[b][x][e] += mine >= lo && mine < hi ? add[e] : 0.f;
             }
           }
         }
       }
-      row = stop;
+      lo = hi;
     }
     // The next tile has landed. Behind its transfers lie those of the tiles after it and the stores of as many tiles before
     // this one (all full: none is short but the last of all): the wave's memory operations complete in order.
@@ -317,18 +337,19 @@ __global__ __launch_bounds__(512, 2) void adapted_rows(const RowsArgs p, int sli
       wait_vm_lds<(STAGES - 2) * (S::PER + S::STORES)>();
     else
       wait_vm_lds<(STAGES - 2) * S::PER>();
-    bf16* to = p.out + (row0 + r0 + i) * N + n0 + 16 * (g & 1) + 8 * (g >> 1);
+    bf16* to = p.out + row0 * N + ((r0 + i) * N + n0 + 16 * (g & 1) + 8 * (g >> 1));
 #pragma unroll
     for (int x = 0; x < S::TT; ++x) {
       bf16x8 v[S::NB / 2];
 #pragma unroll
       for (int b = 0; b < S::NB / 2; ++b) v[b] = join_blocks(acc[2 * b][x], acc[2 * b + 1][x]);
-      if (end - row0 < TM && row0 + r0 + 16 * x + i >= rows) continue;
+      if (end < TM && r0 + 16 * x + i >= end) continue;
 #pragma unroll
       for (int b = 0; b < S::NB / 2; ++b)
-        __builtin_nontemporal_store(v[b], reinterpret_cast<bf16x8*>(to + (int64_t)16 * x * N + 32 * b));
+        __builtin_nontemporal_store(v[b], reinterpret_cast<bf16x8*>(to + 16 * x * N + 32 * b));
     }
     __syncthreads();
+    xs = xs == lds + TOP ? lds : xs + sizeof(buf[0]);
   }
 }
 
@@ -336,8 +357,9 @@ template <int C, int NS, int RB>
 void launch_rows(const RowsArgs& p, hipStream_t st) {
   const auto kernel = adapted_rows<C, NS, RB>;
   constexpr int TM = RowsShape<C, NS>::TM;
-  const int64_t resident = (int64_t)cu_count() * resident_blocks(reinterpret_cast<const void*>(kernel), 512, 0);
-  const int64_t slices = p.N / NS, ranges = std::min((p.q.rows + TM - 1) / TM, std::max<int64_t>(1, resident / slices));
+  // One workgroup a compute unit, also where registers and LDS hold two: its tiles in flight suffice, and two read W twice
+  // (262144 rows, 64 -> 256: 36 us, with two 48; 64 -> 128: 23, with two 27).
+  const int64_t slices = p.N / NS, ranges = std::min((p.q.rows + TM - 1) / TM, std::max<int64_t>(1, cu_count() / slices));
   kernel<<<dim3((unsigned)(ranges * slices)), 512, 0, st>>>(p, (int)slices);
 }
 
