@@ -307,8 +307,10 @@ __global__ __launch_bounds__(512, 2) void adapted_rows(const RowsArgs p, int sli
           for (int s = 0; s < PAIRS; ++s)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
+              // (behind the rank zeros, not the sums of zeros, which an infinite input makes NaN)
               const int b = 2 * s + (e >> 2);
-              uf[s][e] = b < RB ? (bf16)(u[b < RB ? b : 0][x][e & 3] * scale) : (bf16)0.f;
+              const bool in = b < RB && 16 * b + 4 * g + (e & 3) < p.rank;
+              uf[s][e] = in ? (bf16)(u[b < RB ? b : 0][x][e & 3] * scale) : (bf16)0.f;
             }
           if (whole) {
 #pragma unroll
@@ -752,7 +754,7 @@ __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           bf16 t[3];
-          split3(in ? v[e] * scale : 0.f, t);
+          split3(in && 16 * b + 4 * (l >> 4) + e < p.rank ? v[e] * scale : 0.f, t);  // (an infinite input: v times zeros is NaN)
           high[e] = t[0];
 #pragma unroll
           for (int k = 0; k < 3; ++k) gop[y][k][b][4 * (l >> 4) + e + 16 * (l >> 2 & 3)][4 * x + (l & 3)] = t[k];

@@ -215,6 +215,26 @@ def test_a_request_keeps_its_infinities_to_itself(rows, value):
     assert not torch.isfinite(a.up[1]).all() and not torch.isfinite(a.down[1]).all()
 
 
+@pytest.mark.parametrize("rows, d_in, d_out", [(20, 64, 64), (400, 64, 64), (400, 128, 192), (400, 72, 64)])
+def test_an_infinite_input_stays_infinite(rows, d_in, d_out):
+    """Weights above zero at the infinite channel: the row's every output is the infinity that the sums give, at a rank that
+    fills no block of the products."""
+    t = make(rows, d_in, d_out, 5, 2, [rows // 2, rows - rows // 2])
+    for name, at in (("weight", (slice(None), 3)), ("down", (..., 3)), ("up", ...)):
+        t[name][at] = t[name][at].abs() + 0.125
+    t["x"][rows // 2 + 1, 3] = float("inf")
+    y = forward(gpu(t)).cpu()
+    assert (y[rows // 2 + 1] == float("inf")).all()
+    assert y.isfinite().sum() == (rows - 1) * d_out
+    t = make(rows, d_in, d_out, 5, 2, [rows // 2, rows - rows // 2])
+    for name, at in (("weight", 3), ("down", ...), ("up", (slice(None), 3))):
+        t[name][at] = t[name][at].abs() + 0.125
+    t["dy"][rows // 2 + 1, 3] = float("inf")
+    dx = backward(gpu(t)).x.cpu()
+    assert (dx[rows // 2 + 1] == float("inf")).all()
+    assert dx.isfinite().sum() == (rows - 1) * d_in
+
+
 def test_requests_that_share_an_adapter():
     t = make(900, 128, 128, 16, 2, [100, 200, 300, 250], ids=[1, 0, 1, 1])
     check_forward(t, forward(gpu(t)))
