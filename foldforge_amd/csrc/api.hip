@@ -708,7 +708,7 @@ int32_t ffk_adapted_linear(const void* x, const void* weight, const float* bias,
   a.a_f32 = adapter_dtype == FFK_DTYPE_F32;
   if (int32_t s = adapted_check("adapted_linear", a, weight_dtype, adapter_dtype)) return s;
   if (rows == 0) return ok();
-  if (!out) return fail(FFK_ERR_INVALID, "adapted_linear: null argument");
+  if (!out || out == x) return fail(FFK_ERR_INVALID, "adapted_linear: the output is null or x");
   const AdaptedPlan p = adapted_plan(rows, d_in, d_out, adapters, rank, requests, a.w_f32, a.a_f32, 0);
   const size_t need = adapted_ws(workspace, p, a, 0);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
@@ -765,6 +765,7 @@ int32_t ffk_adapted_linear_backward(const void* dy, const void* x, const void* w
   if (rows == 0) return fail(FFK_ERR_INVALID, "adapted_linear_backward: no rows (the gradients are zeros)");
   if (!dy || !ddown || !dup || !aligned16(dy))
     return fail(FFK_ERR_INVALID, "adapted_linear_backward: null argument, or dy off 16-byte alignment");
+  if (dx && (dx == x || dx == dy)) return fail(FFK_ERR_INVALID, "adapted_linear_backward: dx may not be x or dy");
   const AdaptedPlan p = adapted_plan(rows, d_in, d_out, adapters, rank, requests, a.w_f32, a.a_f32, 1);
   const size_t need = adapted_ws(workspace, p, a, 1);
   if (!workspace || workspace_bytes < need || !aligned16(workspace))

@@ -128,8 +128,9 @@ int32_t ffk_dropout_add(const void* x, const void* residual, void* out, const in
  * [adapters, rank, d_in] and up B [adapters, d_out, rank] in adapter_dtype (bf16 or fp32 each); scale s [adapters] fp32 or
  * NULL (1). Request r has the rows offsets[r] .. offsets[r + 1] - 1 (offsets [requests + 1], not decreasing; none where they
  * are the same); rows of no request, and requests whose adapter is not in [0, adapters), get W x + bias. Two requests may
- * share an adapter (offsets that decrease give unspecified values). x, out, the weights: 16-byte aligned; rank up to 128, widths up to 65536. Products of bf16
- * operands (fp32 ones are rounded), fp32 sums; the rows A x in fp32 up to 256 rows, in bf16 above.
+ * share an adapter (offsets that decrease give unspecified values). x, out, the weights: 16-byte aligned, out not x; rank up
+ * to 128, widths up to 65536. Products of bf16 operands (fp32 ones are rounded), fp32 sums; the rows A x in fp32 up to 256
+ * rows, in bf16 above.
  */
 size_t ffk_adapted_linear_workspace(int64_t rows, int32_t d_in, int32_t d_out, int32_t adapters, int32_t rank,
                                     int32_t requests, int32_t weight_dtype, int32_t adapter_dtype);

@@ -274,6 +274,20 @@ def test_leading_axes_and_an_output():
     assert backward(g).x.shape == (2, 12, 12, 64)
 
 
+def test_entries_refuse_an_output_over_an_input():
+    t = gpu(make(40, 64, 64, 8, 1, [40]))
+    q = kernels._adapted(*(t[k] for k in ("x", "weight", "bias", "down", "up", "scale", "offsets", "adapter")))
+    ws = torch.empty(1 << 20, dtype=torch.uint8, device=DEV)
+    args = [t[k] for k in ("weight", "bias", "down", "up", "scale", "offsets", "adapter")]
+    with pytest.raises(RuntimeError, match="null or x"):
+        kernels._call(t["x"].device, "adapted_linear", t["x"], *args, t["x"], ws, ws.numel(), *q)
+    grads = [torch.empty_like(t[k], dtype=F32) for k in ("down", "up")]
+    args.pop(1)
+    for dx in (t["x"], t["dy"]):
+        with pytest.raises(RuntimeError, match="dx may not be"):
+            kernels._call(dx.device, "adapted_linear_backward", t["dy"], t["x"], *args, dx, *grads, ws, ws.numel(), *q, 1)
+
+
 def test_no_rows():
     t = gpu(make(0, 64, 64, 8, 2, [0, 0]))
     assert forward(t).shape == (0, 64)
