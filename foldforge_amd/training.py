@@ -194,9 +194,14 @@ def adapted_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, dow
 
 class DropoutStream:
     """The draws of a run's dropouts: one seed, and an offset of its own for each call. ``offset`` is where the next call
-    begins; with ``seed`` it is all that a checkpoint has to hold to go on with the same draws."""
+    begins; with ``seed`` it is all that a checkpoint has to hold to go on with the same draws. A forward pass that is run
+    again for its backward pass has to start from the offset that it had (set ``offset`` back for it); ranks that see other
+    data take other seeds."""
 
     def __init__(self, seed: int, offset: int = 0) -> None:
+        for value, name in ((seed, "seed"), (offset, "offset")):
+            if not isinstance(value, int) or not 0 <= value < 2**63:
+                raise ValueError(f"{name} must be a whole number in [0, 2^63) (got {value!r})")
         self.seed, self.offset = seed, offset
 
     def take(self) -> int:

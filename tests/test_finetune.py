@@ -90,6 +90,12 @@ def test_stream_goes_on_from_a_checkpoint():
     assert torch.equal(block(z, mask), want)
 
 
+@pytest.mark.parametrize("seed, offset", [(-1, 0), (2**63, 0), (1, -1), (torch.tensor([1, 0]), 0), (0.5, 0)])
+def test_a_stream_is_of_whole_numbers(seed, offset):
+    with pytest.raises(ValueError, match="whole number"):
+        training.DropoutStream(seed, offset)
+
+
 def test_calls_are_counted_where_they_run():
     block, (z, mask) = _block(), _inputs()
     training.set_dropout(block, training.DropoutStream(1))
