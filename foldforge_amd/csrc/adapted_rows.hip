@@ -624,6 +624,8 @@ __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p
         const int mine = r0 + 16 * x + i;
 #pragma unroll
         for (int b = 0; b < S::NB; ++b) {
+          // (selected, also where the whole tile is one request's: behind a branch around the selection the compiler has left
+          // out the wait for the product's result)
           f32x4 add = none;
 #pragma unroll
           for (int s = 0; s < RB; ++s) add = mfma16_16(at_[b][s], vop[r0 / 16 + x][s][lane], add);

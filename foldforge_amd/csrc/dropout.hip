@@ -112,7 +112,8 @@ __global__ __launch_bounds__(256) void dropout_each(const DropoutArgs a) {
 constexpr int kDropRows = 4;  // rows a thread has in flight
 
 // shared > 1: a thread draws its eight numbers once and takes them down `rows` rows. A workgroup: `lanes` threads along the
-// inner axis, 256 / lanes beside each other along the shared one. It walks over the outer x ceil(pieces / lanes) x ceil(shared / rows) pieces of work.
+// inner axis, 256 / lanes beside each other along the shared one. It walks over the outer x ceil(pieces / lanes) x
+// ceil(shared / rows) pieces of work.
 template <typename T, bool RES, bool WIDE>
 __global__ __launch_bounds__(256) void dropout_shared(const DropoutArgs a, int lanes, int64_t tiles, int64_t chunks,
                                                       int64_t rows) {
@@ -153,7 +154,7 @@ __global__ __launch_bounds__(256) void dropout_shared(const DropoutArgs a, int l
 template <typename T, bool RES, bool WIDE>
 void launch(const DropoutArgs& a, hipStream_t stream) {
   const int64_t pieces = (a.inner + 7) / 8;
-  if (a.shared == 1) {  // (outer is 1: dropout_layout)
+  if (a.shared == 1) {  // (one run: outer is 1)
     dropout_each<T, RES, WIDE><<<dim3((unsigned)std::min<int64_t>((pieces + 255) / 256, 256 * 16)), 256, 0, stream>>>(a);
     return;
   }
