@@ -23,7 +23,8 @@ Modules
                it pins the released-to-engine conversion.
 
 ``training``   fp64 8-bit activations and backward passes of LayerNorm and the
-               transition, written out from the formulas.
+               transition, written out from the formulas; dropout masks, and
+               projections with low-rank adapters with their gradients.
 
 Pinning status (what each function is checked against, in ``tests/test_oracle.py``
 and ``tests/test_released.py``):
@@ -54,7 +55,10 @@ and ``tests/test_released.py``):
                             backend match it (2e-5 per op, 1e-4 per block).
 * ``training``              autograd in fp64, differences, torch's own e4m3, and
                             half a step's bound of the codes
-                            (``tests/test_training_oracle.py``).
+                            (``tests/test_training_oracle.py``); the generator's
+                            published answers (``tests/test_dropout.py``), the
+                            adapters' gradients against autograd
+                            (``tests/test_adapted.py``).
 
 Conventions the reference leaves open (engine ``pytorch`` backend outputs at
 padded positions are not pinned by any reference test, which compare valid
