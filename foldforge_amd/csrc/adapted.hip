@@ -191,14 +191,15 @@ struct ThinLds {
   int id[64], start[64];
 };
 
-// 64 / KS rows a workgroup, of 4 waves: KS = 1, 16 rows a wave; KS = 4, all 16 rows, a quarter of K a wave (few rows: more
-// workgroups). Each adapter of the rows in turn, `share` workgroups share them; a lane holds a token and 4 channels. Operands
-// straight from the call's tensors. EVEN: K a multiple of 8. KEEP: u in three parts (rows of parts_ld; fp32 adapters in three
-// parts as well), else rounded (rows of RP).
-template <typename TA, int RP, bool KEEP, int KS, bool EVEN>
+// 16 rows a workgroup of 4 waves, a quarter of K a wave (16 rows a wave over all of K leave the chip half empty with few rows
+// and are no faster with many: 768 -> 768 of rank 48 in tiles 43 us against 30 at 4000 rows, 142 against 132 at 40000; the
+// backward pass 407 against 311). Each adapter of the rows in turn, `share` workgroups share them; a lane holds a token and 4
+// channels. Operands straight from the call's tensors. EVEN: K a multiple of 8. KEEP: u in three parts (rows of parts_ld; fp32
+// adapters in three parts as well), else rounded (rows of RP).
+template <typename TA, int RP, bool KEEP, bool EVEN>
 __device__ __forceinline__ void thin_rows(const ThinArgs& p, int64_t block, ThinLds& lds, f32x4 (*red)[RP / 16][64]) {
   constexpr int PARTS = KEEP && sizeof(TA) == 4 ? 3 : 1;
-  constexpr int N = RP / 16, TM = 64 / KS, U = N * PARTS <= 3 ? 6 : N * PARTS <= 6 ? 2 : 1;  // steps of k in flight
+  constexpr int N = RP / 16, TM = 16, U = N * PARTS <= 3 ? 6 : N * PARTS <= 6 ? 2 : 1;  // steps of k in flight
   constexpr int ld = KEEP ? parts_ld(RP) : RP;
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -208,9 +209,8 @@ __device__ __forceinline__ void thin_rows(const ThinArgs& p, int64_t block, Thin
   tile_ids(p.q, row0, lds.id, lds.start);
   if (shared == 0 && which == 0 && threadIdx.x < TM && row0 + threadIdx.x < p.q.rows)
     p.ids[row0 + threadIdx.x] = lds.id[threadIdx.x];
-  const int first = KS == 1 ? 16 * wave : 0;  // of the wave's rows
-  const int64_t row = row0 + first + i;
-  const int mine = lds.id[first + i];
+  const int64_t row = row0 + i;
+  const int mine = lds.id[i];
   const bf16* x = j.x + (row < p.q.rows ? row : p.q.rows - 1) * j.K;
   auto store = [&](int n, const f32x4& v) __attribute__((always_inline)) {
     bf16x4 part[3];
@@ -235,7 +235,7 @@ __device__ __forceinline__ void thin_rows(const ThinArgs& p, int64_t block, Thin
     }
   };
   const f32x4 none = {0.f, 0.f, 0.f, 0.f};
-  if (shared == 0 && mine < 0 && row < p.q.rows && (KS == 1 || wave == 0)) {
+  if (shared == 0 && mine < 0 && row < p.q.rows && wave == 0) {
 #pragma unroll
     for (int n = 0; n < N; ++n) store(n, none);
   }
@@ -288,8 +288,8 @@ __device__ __forceinline__ void thin_rows(const ThinArgs& p, int64_t block, Thin
     };
     // (a wave's share of k in one piece: its steps share cache lines)
     const int all = (j.K + 31) / 32;
-    int k = KS == 1 ? 0 : all * wave / 4;
-    const int stop = KS == 1 ? all : all * (wave + 1) / 4;
+    int k = all * wave / 4;
+    const int stop = all * (wave + 1) / 4;
     for (; k + U <= stop; k += U) steps(32 * k, std::integral_constant<int, U>());
     if constexpr (U > 3)
       if (k + 3 <= stop) {
@@ -298,37 +298,30 @@ __device__ __forceinline__ void thin_rows(const ThinArgs& p, int64_t block, Thin
       }
     if constexpr (U > 1)
       for (; k < stop; ++k) steps(32 * k, std::integral_constant<int, 1>());
-    if constexpr (KS == 1) {
-      if (is) {
+    __syncthreads();
 #pragma unroll
-        for (int n = 0; n < N; ++n) store(n, acc[n] * s);
-      }
-    } else {
-      __syncthreads();
+    for (int n = 0; n < N; ++n) red[wave][n][lane] = acc[n];
+    __syncthreads();
 #pragma unroll
-      for (int n = 0; n < N; ++n) red[wave][n][lane] = acc[n];
-      __syncthreads();
-#pragma unroll
-      for (int n = 0; n < N; ++n)
-        if (n % 4 == wave && is) store(n, (red[0][n][lane] + red[1][n][lane] + (red[2][n][lane] + red[3][n][lane])) * s);
-    }
+    for (int n = 0; n < N; ++n)
+      if (n % 4 == wave && is) store(n, (red[0][n][lane] + red[1][n][lane] + (red[2][n][lane] + red[3][n][lane])) * s);
   }
 }
 
 // What a call makes first, in one launch: the thin products, and (the workgroups behind theirs) the operands that the wide
 // product reads from copies. block 256.
-template <typename TA, int RP, bool KEEP, int KS, bool EVEN>
+template <typename TA, int RP, bool KEEP, bool EVEN>
 __global__ __launch_bounds__(256) void adapted_prepare(const ThinArgs t, const PackArgs p) {
   __shared__ union {
     struct {
       ThinLds lds;
-      f32x4 red[KS == 1 ? 1 : 4][RP / 16][64];
+      f32x4 red[4][RP / 16][64];
     } thin;
     float tile[32][33];
   } s;
   const int64_t blocks = t.row_blocks * t.share * t.jobs;
   if (blockIdx.x < blocks)
-    thin_rows<TA, RP, KEEP, KS, EVEN>(t, blockIdx.x, s.thin.lds, s.thin.red);
+    thin_rows<TA, RP, KEEP, EVEN>(t, blockIdx.x, s.thin.lds, s.thin.red);
   else
     pack_tiles(p, blockIdx.x - blocks, gridDim.x - blocks, s.tile);
 }
@@ -824,27 +817,21 @@ struct Packer {
 };
 
 template <typename TA, int RP, bool KEEP>
-void launch_prepare_as(const ThinArgs& t, const PackArgs& p, bool split, bool even, hipStream_t st) {
+void launch_prepare_as(const ThinArgs& t, const PackArgs& p, bool even, hipStream_t st) {
   const dim3 grid((unsigned)(t.row_blocks * t.share * t.jobs + std::min<int64_t>(p.tiles, 1 << 20)));
-  if (split)
-    even ? adapted_prepare<TA, RP, KEEP, 4, true><<<grid, 256, 0, st>>>(t, p)
-         : adapted_prepare<TA, RP, KEEP, 4, false><<<grid, 256, 0, st>>>(t, p);
-  else
-    even ? adapted_prepare<TA, RP, KEEP, 1, true><<<grid, 256, 0, st>>>(t, p)
-         : adapted_prepare<TA, RP, KEEP, 1, false><<<grid, 256, 0, st>>>(t, p);
+  even ? adapted_prepare<TA, RP, KEEP, true><<<grid, 256, 0, st>>>(t, p)
+       : adapted_prepare<TA, RP, KEEP, false><<<grid, 256, 0, st>>>(t, p);
 }
 template <bool KEEP>
 void launch_prepare(ThinArgs t, const PackArgs& p, int rp, int a_f32, hipStream_t st) {
   const int64_t rows = t.q.rows;
-  // few rows: a quarter of k a wave, so that the chip is filled, and the adapters of 16 rows shared out where they may be many
-  const bool split = rows < 64 * 256;
   const bool even = t.job[0].K % 8 == 0 && (t.jobs == 1 || t.job[1].K % 8 == 0);
-  t.share = split && t.q.count > (int)(rows / 16) ? 4 : 1;
-  t.row_blocks = (rows + (split ? 15 : 63)) / (split ? 16 : 64);
+  t.share = t.q.count > rows / 16 ? 4 : 1;  // (16 rows may have many adapters)
+  t.row_blocks = (rows + 15) / 16;
 #define FFK_PREPARE(RP)                                                           \
   if (rp == RP) {                                                                 \
-    a_f32 ? launch_prepare_as<float, RP, KEEP>(t, p, split, even, st)             \
-          : launch_prepare_as<bf16, RP, KEEP>(t, p, split, even, st);             \
+    a_f32 ? launch_prepare_as<float, RP, KEEP>(t, p, even, st)             \
+          : launch_prepare_as<bf16, RP, KEEP>(t, p, even, st);             \
   }
   FFK_PREPARE(16)
   FFK_PREPARE(32)
@@ -853,8 +840,10 @@ void launch_prepare(ThinArgs t, const PackArgs& p, int rp, int a_f32, hipStream_
 #undef FFK_PREPARE
 }
 
-// Tiles of 128 x 128 where they fill the chip, of 64 x 64 where not.
-bool big_tiles(int64_t rows, int N) { return N > 64 && ((rows + 127) / 128) * ((N + 127) / 128) >= 256; }
+// Tiles of 128 x 128 from half a chip's worth on, else of 64 x 64 (us in 128s against 64s): 96 tiles 768 -> 768 26.3 : 21.6,
+// 1536 -> 384 34.4 : 30.6; 141 to 144 tiles 26.7 : 28.2 and 40.6 : 42.9. Backward: 48 tiles 30.4 : 29.2, 96 tiles 33.3 : 37.3 and
+// (449 channels) 26.3 : 23.7, 192 tiles 28.3 : 31.4.
+bool big_tiles(int64_t rows, int N) { return N > 64 && ((rows + 127) / 128) * ((N + 127) / 128) >= 128; }
 
 void launch_product(ProductArgs a, hipStream_t st) {
   const bool big = big_tiles(a.rows, a.N);

@@ -159,6 +159,76 @@ def test_backward_is_the_definition(case, weight, adapter):
     check_backward(t, backward(gpu(t)))
 
 
+#: rows from which on the backward pass (and the forward of wide rows) is one pass: a tile more or less, short requests, long
+#: ones, rows before, between and behind them
+MANY = [
+    (4096, 64, 64, 16, 2, [4000, 96]),
+    (4129, 64, 128, 12, 3, [31, 33, 0, 500, 1, 1, 3500]),
+    (5000, 128, 64, 3, 1, [5000]),
+    (4100, 64, 256, 16, 4, [1000, 63, 65, 2000, 872]),
+    (4097, 256, 64, 15, 2, [4096]),
+    (6000, 128, 128, 16, 5, [7, 400, 9, 800, 1000] + [64] * 40),
+    (8200, 128, 256, 16, 2, [4100, 4100]),
+    (8193, 256, 128, 9, 2, [350, 350]),
+    (8192, 256, 256, 5, 3, [17] * 100),
+    (8999, 512, 128, 16, 7, [100] * 89),
+    (8400, 128, 512, 11, 8, [64] * 131),
+    (32768, 64, 64, 16, 9, [64] * 512),
+    (12300, 256, 256, 20, 2, [6000, 6300]),
+    (12289, 512, 256, 32, 3, [300, 300, 11000]),
+    (6145, 384, 384, 16, 9, [96] * 64),
+    (6200, 384, 256, 31, 1, [6177]),
+]
+
+
+@pytest.mark.parametrize("weight,adapter", [(BF16, BF16), (F32, F32)])
+@pytest.mark.parametrize("case", MANY, ids=lambda c: "x".join(map(str, c[:5])))
+def test_many_rows(case, weight, adapter):
+    t = make(*case, weight=weight, adapter=adapter, seed=case[0], bias=case[0] % 2 == 1)
+    check_forward(t, forward(gpu(t)))
+    check_backward(t, backward(gpu(t)))
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_many_rows_keep_infinities_to_their_request(value):
+    n = 1399
+    t = make(3 * n, 128, 128, 13, 3, [n, n, n], adapter=F32)
+    sick = {k: None if v is None else v.clone() for k, v in t.items()}
+    for row in (n, 2 * n - 1):  # the request's ends, in tiles that it shares
+        sick["x"][row] = value
+        sick["dy"][row] = value
+    sick["up"][1, 3] = value
+    sick["down"][1, :, 5] = value
+    other = torch.ones(3 * n, dtype=torch.bool)
+    other[n:2 * n] = False
+    assert torch.equal(forward(gpu(sick)).cpu()[other], forward(gpu(t)).cpu()[other])
+    a, b = backward(gpu(sick)), backward(gpu(t))
+    assert torch.equal(a.x.cpu()[other], b.x.cpu()[other])
+    for i in (0, 2):
+        assert torch.equal(a.down[i], b.down[i]) and torch.equal(a.up[i], b.up[i])
+
+
+def test_many_rows_and_an_infinite_gradient():
+    rows, d = 4500, 64
+    t = make(rows, d, d, 5, 2, [rows // 2, rows - rows // 2])
+    for name, at in (("weight", 3), ("down", ...), ("up", (slice(None), 3))):
+        t[name][at] = t[name][at].abs() + 0.125
+    t["dy"][rows // 2 + 1, 3] = float("inf")
+    dx = backward(gpu(t)).x.cpu()
+    assert (dx[rows // 2 + 1] == float("inf")).all()
+    assert dx.isfinite().sum() == (rows - 1) * d
+
+
+def test_backward_forms_of_many_rows():
+    t = make(4200, 128, 128, 8, 3, [2000, 2], adapter=F32, scale=False)
+    g = gpu(t)
+    whole = backward(g)
+    short = backward(g, with_x=False)
+    assert short.x is None and torch.equal(short.down, whole.down) and torch.equal(short.up, whole.up)
+    check_backward(t, backward(g, grad_dtype=BF16), BF16)
+    assert not whole.down[2].any() and not whole.up[2].any()  # an adapter without rows
+
+
 @pytest.mark.parametrize("rows", [5, 300])
 def test_backward_forms(rows):
     t = make(rows, 128, 192, 8, 3, [rows // 2, 2], adapter=F32, scale=False)
@@ -171,7 +241,7 @@ def test_backward_forms(rows):
     assert not whole.down[2].any() and not whole.up[2].any()  # an adapter without rows
 
 
-@pytest.mark.parametrize("rows", [40, 400])
+@pytest.mark.parametrize("rows", [40, 400, 4500])
 def test_requests_without_an_adapter(rows):
     """Ids that are none of the adapters, rows before the first and behind the last request: the projection alone."""
     n = rows // 5
@@ -185,7 +255,7 @@ def test_requests_without_an_adapter(rows):
 
 
 @pytest.mark.parametrize("offsets", [[5, 3, 9, 2], [-7, -3, 1000, 4], [2**31 - 1, -2**31, 0, 50], [0, 2**31 - 1, 2**31 - 1, 7]])
-@pytest.mark.parametrize("rows", [50, 500])
+@pytest.mark.parametrize("rows", [50, 500, 5000])
 def test_offsets_out_of_order_stay_within_the_rows(rows, offsets):
     """Offsets that decrease are not refused (they lie on the device): the adapters' values are unspecified then, but each row
     has some adapter or none and no access is out of range."""
@@ -295,7 +365,7 @@ def test_no_rows():
     assert got.x.shape == (0, 64) and not got.down.any() and not got.up.any()
 
 
-@pytest.mark.parametrize("rows", [3, 700])
+@pytest.mark.parametrize("rows", [3, 700, 8200])
 def test_captured_calls(rows):
     """A forward and a backward pass in a graph, replayed on new values between other work."""
     a, b = (make(rows, 128, 256, 8, 2, [rows // 3, rows // 2], adapter=F32, seed=s) for s in (1, 2))
