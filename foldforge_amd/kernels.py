@@ -454,6 +454,9 @@ def dropout_add(update: Tensor, residual: Tensor | None = None, *, p: float, see
         out = torch.empty_like(update)
     else:
         out = _output(out, tuple(update.shape), update.dtype, update.device)
+        for t, name in ((update, "update"), (residual, "residual")):
+            if t is not None and 0 < abs(out.data_ptr() - t.data_ptr()) < t.numel() * t.element_size():
+                _refuse(f"out overlaps {name} in part (it may be the whole of it)")
     if update.numel():
         _call(update.device, "dropout_add", update, residual, out, state, seed, offset, *axes, dropped,
               _dtype_code(update.dtype))

@@ -72,6 +72,15 @@ def test_refusals(on_cpu, args, how, message):
         kernels.dropout_add(*args, **{"p": 0.1, "seed": 1, **how})
 
 
+@pytest.mark.parametrize("which", ["update", "residual"])
+def test_an_output_over_a_part_of_an_input_is_refused(on_cpu, which):
+    memory = torch.zeros(100)
+    args = {"update": torch.zeros(4, 8), "residual": torch.zeros(4, 8), which: memory[:32].view(4, 8)}
+    for at in (1, 31):
+        with pytest.raises(ValueError, match="overlaps " + which):
+            kernels.dropout_add(**args, p=0.1, seed=1, out=memory[at:at + 32].view(4, 8))
+
+
 def test_axes_of_the_mask():
     assert kernels.mask_axes((2, 3, 4, 5), None) == (1, 1, 120)
     assert kernels.mask_axes((2, 3, 4, 5), 1) == (2, 3, 20)
