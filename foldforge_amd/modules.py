@@ -24,6 +24,7 @@ no fallback of its own: if the native library is missing the call raises.
 
 from __future__ import annotations
 
+import inspect
 from dataclasses import dataclass, fields
 from typing import Any
 
@@ -151,13 +152,18 @@ class EngineOp:
     def forward(self, *args: Any, **kwargs: Any) -> Any:
         dropout = self.active_dropout()
         if dropout is not None:
-            return dropout(self._update(args, kwargs), args[0])
+            residual = kwargs.pop("residual", True)
+            return dropout(self._update(args, kwargs), self._input(args, kwargs) if residual else None)
         return getattr(self, f"_forward_{self._route(args, kwargs)}")(*args, **kwargs)
 
     def delta(self, *args: Any, **kwargs: Any) -> Tensor:
         """The bare update ``f(x)`` (the forward returns ``x + f(x)``)."""
         update, dropout = self._update(args, kwargs), self.active_dropout()
         return update if dropout is None else dropout(update)
+
+    def _input(self, args: tuple, kwargs: dict) -> Tensor:
+        """What the op updates: its first argument, in place or by name."""
+        return args[0] if args else kwargs[next(iter(inspect.signature(self._forward_pytorch).parameters))]  # type: ignore
 
     def _update(self, args: tuple, kwargs: dict) -> Tensor:
         return getattr(self, f"_forward_{self._route(args, kwargs)}")(*args, residual=False, **kwargs)

@@ -166,3 +166,27 @@ def test_refusals():
     with pytest.raises(ValueError, match="frozen"):
         training.adapted_linear(x, w, down=torch.zeros(1, 2, 8), up=torch.zeros(1, 8, 2),
                                 offsets=torch.zeros(2, dtype=torch.int32), adapter=torch.zeros(1, dtype=torch.int32))
+
+
+def test_calls_by_name_and_without_the_residual_under_dropout():
+    """Every form of a call that an op takes without a dropout, it takes with one."""
+    block, (z, mask) = _block(), _inputs()
+    g = torch.Generator().manual_seed(6)
+    msa, msa_op = torch.randn(1, 3, 9, 64, generator=g), randomise(modules.MSAPairWeightedAveraging(64, 64), 3)
+    for op, axis, first, args in ((block.tri_multi_outgoing, 1, "x", (z, mask)), (block.tri_atten_ending, 2, "x", (z, mask)),
+                                  (msa_op, 1, "m", (msa, z, mask))):
+        names = (first, "mask") if len(args) == 2 else (first, "z", "mask")
+        by_name = dict(zip(reversed(names), reversed(args)))  # (the input is not the first of them)
+        for dropped in (False, True):
+            update = op._forward_pytorch(*args, residual=False)
+            whole = op._forward_pytorch(*args)
+            training.set_dropout(op, training.DropoutStream(9) if dropped else None, p=0.25)
+            if dropped:
+                keep = [oracle.dropout_mask(update.shape, axis, 0.25, 9, i) for i in range(4)]
+            for i, (got, added) in enumerate(((op(*args), True), (op(**by_name), True), (op(*args, residual=False), False),
+                                              (op(**by_name, residual=False), False))):
+                want = whole if added else update
+                if dropped:
+                    want = torch.where(keep[i], update * (4 / 3), 0.0) + (args[0] if added else 0.0)
+                # (a scale, its product and a sum in fp32: 3 roundings of 2^-24 of values below 2^6)
+                assert ((got - want).abs() <= 3 * 2.0**-18).all(), (type(op).__name__, dropped, i)
