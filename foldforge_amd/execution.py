@@ -20,6 +20,8 @@ from typing import Any
 
 import torch
 
+from foldforge_amd import training
+
 Tensor = torch.Tensor
 
 
@@ -31,7 +33,8 @@ class CapturedCall:
     the next replay overwrites (clone them to keep a result). ``kwargs`` are fixed at capture
     time (e.g. the number of passes). Two warm-up calls run on a side stream first, as the
     reference does, so that one-time work (library loading, allocator growth) stays out of
-    the graph.
+    the graph. A model in training mode whose ops have a dropout
+    (:func:`foldforge_amd.training.set_dropout`) is refused: its masks would be the same at each replay.
     """
 
     def __init__(self, fn: Callable[..., Any], tensors: Sequence[Tensor], *, warmup: int = 2,
@@ -42,13 +45,13 @@ class CapturedCall:
         self.inputs = tuple(t.detach().clone() for t in tensors)
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
-        with torch.no_grad(), torch.cuda.stream(side):
+        with torch.no_grad(), torch.cuda.stream(side), training.replayed():
             for _ in range(warmup):
                 fn(*self.inputs, **kwargs)
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
         self.graph = torch.cuda.CUDAGraph()
-        with torch.no_grad(), torch.cuda.graph(self.graph):
+        with torch.no_grad(), torch.cuda.graph(self.graph), training.replayed():
             self.output = fn(*self.inputs, **kwargs)
         torch.cuda.synchronize()
 

@@ -25,6 +25,8 @@ calls the kernels' functions themselves (``transition_checkpoint``, ``transition
 from __future__ import annotations
 
 from collections.abc import Iterator
+from contextlib import contextmanager
+from contextvars import ContextVar
 
 import torch
 from torch import nn
@@ -192,11 +194,26 @@ def adapted_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, dow
     return _AdaptedLinear.apply(x.clone() if x.data_ptr() % 16 else x, weight, bias, down, up, scale, offsets, adapter)
 
 
+#: whether what runs now is to be captured and replayed
+_REPLAYED: ContextVar[bool] = ContextVar("replayed", default=False)
+
+
+@contextmanager
+def replayed() -> Iterator[None]:
+    """What runs inside is captured, or is the warm-up of a capture: a :class:`DropoutStream` refuses it."""
+    token = _REPLAYED.set(True)
+    try:
+        yield
+    finally:
+        _REPLAYED.reset(token)
+
+
 class DropoutStream:
     """The draws of a run's dropouts: one seed, and an offset of its own for each call. ``offset`` is where the next call
     begins; with ``seed`` it is all that a checkpoint has to hold to go on with the same draws. A forward pass that is run
     again for its backward pass has to start from the offset that it had (set ``offset`` back for it); ranks that see other
-    data take other seeds."""
+    data take other seeds. A captured graph would replay the offsets of its capture, one mask for ever: calls under capture
+    are refused (:func:`foldforge_amd.kernels.dropout_add` takes a seed on the device there)."""
 
     def __init__(self, seed: int, offset: int = 0) -> None:
         for value, name in ((seed, "seed"), (offset, "offset")):
@@ -206,6 +223,9 @@ class DropoutStream:
 
     def take(self) -> int:
         """The offset of one call."""
+        if _REPLAYED.get() or (torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()):
+            raise RuntimeError("a captured graph would replay one dropout mask: capture the model in evaluation mode, or "
+                               "call foldforge_amd.kernels.dropout_add with a seed on the device")
         self.offset += 1
         return self.offset - 1
 

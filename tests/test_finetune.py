@@ -190,3 +190,24 @@ def test_calls_by_name_and_without_the_residual_under_dropout():
                     want = torch.where(keep[i], update * (4 / 3), 0.0) + (args[0] if added else 0.0)
                 # (a scale, its product and a sum in fp32: 3 roundings of 2^-24 of values below 2^6)
                 assert ((got - want).abs() <= 3 * 2.0**-18).all(), (type(op).__name__, dropped, i)
+
+
+def test_a_stream_refuses_a_capture(monkeypatch):
+    """A graph would replay the offsets that its capture saw."""
+    block, (z, mask) = _block(), _inputs()
+    stream = training.DropoutStream(11, 40)
+    training.set_dropout(block, stream)
+    with training.replayed(), pytest.raises(RuntimeError, match="capture"):
+        block(z, mask)
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="capture"):
+        block(z, mask)
+    assert stream.offset == 40
+    block.eval()
+    with training.replayed():
+        block(z, mask)
+    monkeypatch.undo()
+    block.train()
+    block(z, mask)
+    assert stream.offset == 44

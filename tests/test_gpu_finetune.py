@@ -11,7 +11,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from foldforge_amd import dispatch, kernels, modules, training
+from foldforge_amd import dispatch, execution, kernels, modules, training
 from foldforge_amd.trunk import PairformerTrunk, randomise
 from oracle import training as oracle
 
@@ -211,3 +211,34 @@ def test_overlapped_trunk_with_dropout_and_adapters():
         torch.cuda.synchronize()
     for got in results[1:]:
         assert torch.equal(got[0], results[0][0]) and torch.equal(got[1], results[0][1])
+
+
+def test_a_captured_model_with_dropout_is_refused():
+    """Before the capture begins: the streams are as they were. In evaluation mode it is captured, with adapters of each
+    element, and every replay gives the eager values."""
+    model = randomise(PairformerTrunk(2, d_single=384), 3, out_scale=0.25)
+    for block in model.blocks:
+        block.set_master_weights()
+        block.set_backend("hip")
+    model.to(DEV)
+    _with_adapters(model, 2)
+    training.select_adapters(model, torch.tensor([1], dtype=torch.int32, device=DEV))
+    z, mask = _inputs(n=32)
+    s = torch.randn(1, 32, 384, generator=torch.Generator().manual_seed(3)).to(DEV, BF16)
+    stream = training.DropoutStream(4, 10)
+    training.set_dropout(model, stream, p=0.25)
+    with pytest.raises(RuntimeError, match="dropout"):
+        execution.capture_trunk(model, z, mask, s)
+    assert stream.offset == 10
+    with torch.no_grad():
+        model(z, mask, s)
+    assert stream.offset == 18
+    model.eval()
+    captured = execution.capture_trunk(model, z, mask, s)
+    for step in range(3):
+        zs = z + step
+        got = [t.clone() for t in captured(zs, mask, s)]
+        with torch.no_grad():
+            want = model(zs, mask, s)
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
