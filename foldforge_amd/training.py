@@ -25,7 +25,7 @@ calls the kernels' functions themselves (``transition_checkpoint``, ``transition
 from __future__ import annotations
 
 from collections.abc import Iterator
-from contextlib import contextmanager
+from contextlib import AbstractContextManager, contextmanager, nullcontext
 from contextvars import ContextVar
 
 import torch
@@ -211,8 +211,10 @@ def replayed() -> Iterator[None]:
 class DropoutStream:
     """The draws of a run's dropouts: one seed, and an offset of its own for each call. ``offset`` is where the next call
     begins; with ``seed`` it is all that a checkpoint has to hold to go on with the same draws. A forward pass that is run
-    again for its backward pass has to start from the offset that it had (set ``offset`` back for it); ranks that see other
-    data take other seeds. A captured graph would replay the offsets of its capture, one mask for ever: calls under capture
+    again for its backward pass has to start from the offset that it had (set ``offset`` back for it, or run it under
+    :meth:`at`; :meth:`recomputed` gives ``torch.utils.checkpoint`` both), else its gradients would be another mask's: a
+    forward pass inside a backward pass that did not set the offset is refused. Ranks that see other data take other seeds.
+    A captured graph would replay the offsets of its capture, one mask for ever: calls under capture
     are refused (:func:`foldforge_amd.kernels.dropout_add` takes a seed on the device there)."""
 
     def __init__(self, seed: int, offset: int = 0) -> None:
@@ -221,13 +223,41 @@ class DropoutStream:
                 raise ValueError(f"{name} must be a whole number in [0, 2^63) (got {value!r})")
         self.seed, self.offset = seed, offset
 
+    @property
+    def offset(self) -> int:
+        return self._offset
+
+    @offset.setter
+    def offset(self, value: int) -> None:
+        self._offset = value
+        self._placed = torch._C._current_graph_task_id()  # (the backward pass that set it, -1 for none)
+
+    @contextmanager
+    def at(self, offset: int) -> Iterator[None]:
+        """The draws from ``offset`` on inside; afterwards the stream goes on where it was."""
+        before = self._offset, self._placed
+        self.offset = offset
+        try:
+            yield
+        finally:
+            self._offset, self._placed = before
+
+    def recomputed(self) -> tuple[AbstractContextManager, AbstractContextManager]:
+        """``torch.utils.checkpoint.checkpoint(..., use_reentrant=False, context_fn=stream.recomputed)``: the forward pass
+        draws on, its second run draws what it drew."""
+        return nullcontext(), self.at(self.offset)
+
     def take(self) -> int:
         """The offset of one call."""
         if _REPLAYED.get() or (torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()):
             raise RuntimeError("a captured graph would replay one dropout mask: capture the model in evaluation mode, or "
                                "call foldforge_amd.kernels.dropout_add with a seed on the device")
-        self.offset += 1
-        return self.offset - 1
+        task = torch._C._current_graph_task_id()
+        if task != -1 and task != self._placed:
+            raise RuntimeError("a forward pass run again inside a backward pass would draw other masks than it did: set the "
+                               "DropoutStream's offset to where it began (checkpoint: context_fn=stream.recomputed)")
+        self._offset += 1
+        return self._offset - 1
 
 
 def set_dropout(model: nn.Module, stream: DropoutStream | None, p: float | None = None) -> list[str]:

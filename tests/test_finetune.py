@@ -3,8 +3,11 @@ batches with an adapter each against merged weights."""
 
 from __future__ import annotations
 
+from contextlib import nullcontext
+
 import pytest
 import torch
+from torch.utils.checkpoint import checkpoint
 
 from foldforge_amd import dispatch, factories, modules, torch_ops, training
 from foldforge_amd.trunk import randomise
@@ -211,3 +214,65 @@ def test_a_stream_refuses_a_capture(monkeypatch):
     block.train()
     block(z, mask)
     assert stream.offset == 44
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_a_recomputed_forward_draws_its_masks_again(reentrant):
+    """Under torch.utils.checkpoint without the stream's context the gradients would be another mask's: an error."""
+    block, (z, mask) = _block(), _inputs()
+    stream = training.DropoutStream(11)
+    training.set_dropout(block, stream)
+    z.requires_grad_(True)
+    dy = torch.randn(z.shape, generator=torch.Generator().manual_seed(7))
+
+    def gradients(run):
+        z.grad, stream.offset = None, 5
+        block.zero_grad()
+        y = run()
+        y.backward(dy)
+        return [z.grad.clone()] + [p.grad.clone() for p in block.parameters()] + [y.detach()]
+
+    want = gradients(lambda: block(z, mask))
+    assert stream.offset == 9
+    with pytest.raises(RuntimeError, match="offset"):
+        gradients(lambda: checkpoint(block, z, mask, use_reentrant=reentrant))
+    if reentrant:  # by hand: the offset set back where the second run begins
+        calls = []
+
+        def run(*args):
+            with stream.at(5) if calls else nullcontext():
+                calls.append(1)
+                return block(*args)
+
+        got = gradients(lambda: checkpoint(run, z, mask, use_reentrant=True))
+    else:
+        got = gradients(lambda: checkpoint(block, z, mask, use_reentrant=False, context_fn=stream.recomputed))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert stream.offset == 9  # the next forward pass goes on behind the first
+    # one call with the context (the one that is run again first), one without
+    with pytest.raises(RuntimeError, match="offset"):
+        gradients(lambda: checkpoint(block, checkpoint(block, z, mask, use_reentrant=reentrant), mask, use_reentrant=False,
+                                     context_fn=stream.recomputed))
+
+
+def test_a_stream_set_back_inside_a_backward_pass():
+    """The offset set by hand, as a recomputing autograd function does."""
+    stream = training.DropoutStream(3)
+    taken = []
+
+    class Again(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            ctx.offset = stream.offset
+            taken.append(stream.take())
+            return x.clone()
+
+        @staticmethod
+        def backward(ctx, dy):
+            stream.offset = ctx.offset
+            taken.append(stream.take())
+            return dy
+
+    x = torch.ones(1, requires_grad=True)
+    Again.apply(x).backward()
+    assert taken == [0, 0] and stream.take() == 1
