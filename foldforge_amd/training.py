@@ -24,6 +24,7 @@ calls the kernels' functions themselves (``transition_checkpoint``, ``transition
 
 from __future__ import annotations
 
+import threading
 from collections.abc import Iterator
 from contextlib import AbstractContextManager, contextmanager, nullcontext
 from contextvars import ContextVar
@@ -208,6 +209,10 @@ def replayed() -> Iterator[None]:
         _REPLAYED.reset(token)
 
 
+#: held while an offset is taken (threads of one process may share a stream; one lock for all keeps streams copyable)
+_TAKING = threading.Lock()
+
+
 class DropoutStream:
     """The draws of a run's dropouts: one seed, and an offset of its own for each call. ``offset`` is where the next call
     begins; with ``seed`` it is all that a checkpoint has to hold to go on with the same draws. A forward pass that is run
@@ -256,8 +261,9 @@ class DropoutStream:
         if task != -1 and task != self._placed:
             raise RuntimeError("a forward pass run again inside a backward pass would draw other masks than it did: set the "
                                "DropoutStream's offset to where it began (checkpoint: context_fn=stream.recomputed)")
-        self._offset += 1
-        return self._offset - 1
+        with _TAKING:
+            self._offset += 1
+            return self._offset - 1
 
 
 def set_dropout(model: nn.Module, stream: DropoutStream | None, p: float | None = None) -> list[str]:

@@ -3,6 +3,9 @@ batches with an adapter each against merged weights."""
 
 from __future__ import annotations
 
+import copy
+import time
+from concurrent.futures import ThreadPoolExecutor
 from contextlib import nullcontext
 
 import pytest
@@ -276,3 +279,17 @@ def test_a_stream_set_back_inside_a_backward_pass():
     x = torch.ones(1, requires_grad=True)
     Again.apply(x).backward()
     assert taken == [0, 0] and stream.take() == 1
+
+
+def test_draws_of_two_threads_are_their_own():
+    """A thread that is held between reading the offset and counting it up does not share it."""
+    class Slow(int):
+        def __add__(self, other):
+            time.sleep(0.005)
+            return Slow(int(self) + other)
+
+    stream = training.DropoutStream(1, Slow(0))
+    with ThreadPoolExecutor(4) as pool:
+        taken = [int(t) for t in pool.map(lambda _: stream.take(), range(24))]
+    assert sorted(taken) == list(range(24))
+    assert copy.deepcopy(stream).take() == 24
