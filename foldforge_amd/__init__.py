@@ -15,14 +15,15 @@ __version__ = "0.1.0"
 def load(name: str = "pairformer-trunk", checkpoint=None, *, backend: str = "miniworld",
          dtype=None, device="cuda", blocks: int = 48, seed: int = 0, d_single: int = 384,
          engine_ops=None, unsupported: str = "fallback", out_scale: float | None = 0.25,
-         family: str = "alphafold3"):
+         family: str = "alphafold3", p_drop: float = 0.0):
     """A configured trunk on ``device`` with ``backend`` applied to every op module.
 
     ``checkpoint``: a miniworld-format file (``*.miniworld.pt`` of ``family``; a whole-model
     file contributes its ``evoformer.trunk_pairformer.<i>`` blocks), a ``.safetensors`` file or
     a weights-only torch state dict in the trunk's keys
     (``blocks.<i>.tri_multi_outgoing.to_left.weight`` ...); without one the parameters are
-    seeded random init (:func:`foldforge_amd.trunk.randomise`).
+    seeded random init (:func:`foldforge_amd.trunk.randomise`). ``p_drop``: the rate of the
+    triangle ops' dropout, for :func:`foldforge_amd.training.set_dropout`.
     """
     import torch
 
@@ -34,7 +35,7 @@ def load(name: str = "pairformer-trunk", checkpoint=None, *, backend: str = "min
         raise ValueError(f"unknown model {name!r}; this build serves 'pairformer-trunk'")
     dtype = torch.bfloat16 if dtype is None else dtype
     plan = dispatch.Plan.of(backend, engine_ops, unsupported)
-    model = PairformerTrunk(blocks, d_single=d_single)
+    model = PairformerTrunk(blocks, d_single=d_single, p_drop=p_drop)
     if checkpoint is None:
         randomise(model, seed, out_scale=out_scale)
     else:

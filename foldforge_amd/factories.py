@@ -95,26 +95,26 @@ def transition(d_hidden: int, n: int = 4, *, precision: Precision = "master",
 
 def triangle_multiplication(d_pair: int, *, outgoing: bool, d_hidden: int | None = None,
                             divide_by_length: bool = False, precision: Precision = "master",
-                            norm_eps: float | None = None) -> TriangleMultiplication:
-    module = TriangleMultiplication(d_pair, d_hidden=d_hidden, outgoing=outgoing, p_drop=0.0,
+                            norm_eps: float | None = None, p_drop: float = 0.0) -> TriangleMultiplication:
+    module = TriangleMultiplication(d_pair, d_hidden=d_hidden, outgoing=outgoing, p_drop=p_drop,
                                     model="rf3" if divide_by_length else None)
     return finish(module, precision, norm_eps=norm_eps)
 
 
 def triangle_attention(d_pair: int, n_head: int, *, starting: bool, model: str,
                        d_hidden: int | None = None, precision: Precision = "master",
-                       norm_eps: float | None = None) -> TriangleAttention:
-    module = TriangleAttention(d_pair, n_head, d_hidden=d_hidden, starting=starting, p_drop=0.0,
+                       norm_eps: float | None = None, p_drop: float = 0.0) -> TriangleAttention:
+    module = TriangleAttention(d_pair, n_head, d_hidden=d_hidden, starting=starting, p_drop=p_drop,
                                model=model)
     return finish(module, precision, norm_eps=norm_eps)
 
 
 def msa_pair_weighted_averaging(d_msa: int, d_pair: int, n_head: int = 8,
                                 d_hidden: int | None = None, *, precision: Precision = "master",
-                                norm_eps: float | None = None) -> MSAPairWeightedAveraging:
+                                norm_eps: float | None = None, p_drop: float = 0.0) -> MSAPairWeightedAveraging:
     """``MSAPairWeightedAveraging`` (residual included), as
     ``src/foldforge/modules/engine/modules.py:214-226`` builds it."""
-    return finish(MSAPairWeightedAveraging(d_msa, d_pair, n_head, d_hidden, p_drop=0.0),
+    return finish(MSAPairWeightedAveraging(d_msa, d_pair, n_head, d_hidden, p_drop=p_drop),
                   precision, norm_eps=norm_eps)
 
 
@@ -149,14 +149,16 @@ def pairformer_block(*, d_pair: int, triangle_model: str, d_single: int = 0,
                      single_gate_bias: float = 0.0, pair_transition_n: int = 4,
                      single_transition_n: int = 4, use_triangle_attention: bool = True,
                      parallel: bool = False, divide_by_length: bool = False,
-                     precision: Precision = "master", norm_eps: float | None = None) -> PairformerBlock:
-    """One block, residuals included (``src/foldforge/modules/engine/pairformer.py:16-62``)."""
+                     precision: Precision = "master", norm_eps: float | None = None,
+                     p_drop: float = 0.0) -> PairformerBlock:
+    """One block, residuals included (``src/foldforge/modules/engine/pairformer.py:16-62``). ``p_drop``: the rate that
+    :func:`foldforge_amd.training.set_dropout` gives its triangle ops."""
     config = PairformerConfig(
         d_pair=d_pair,
         d_hidden_tri_multi=d_pair if d_hidden_tri_multi is None else d_hidden_tri_multi,
         d_hidden_tri_attention=d_hidden_tri_attention,
         n_head_tri_attention=n_head_tri_attention,
-        p_drop=0.0,
+        p_drop=p_drop,
         use_triangle_attention=use_triangle_attention,
         model=triangle_model,
         d_single=d_single,
@@ -169,8 +171,8 @@ def pairformer_block(*, d_pair: int, triangle_model: str, d_single: int = 0,
     block = PairformerBlock(config)
     if divide_by_length:
         hidden = config.d_hidden_tri_multi
-        block.tri_multi_outgoing = TriangleMultiplication(d_pair, hidden, outgoing=True, model="rf3")
-        block.tri_multi_incoming = TriangleMultiplication(d_pair, hidden, outgoing=False, model="rf3")
+        block.tri_multi_outgoing = TriangleMultiplication(d_pair, hidden, outgoing=True, p_drop=p_drop, model="rf3")
+        block.tri_multi_incoming = TriangleMultiplication(d_pair, hidden, outgoing=False, p_drop=p_drop, model="rf3")
     return finish(block, precision, norm_eps=norm_eps)
 
 
@@ -179,7 +181,7 @@ def msa_block(c_msa: int = 64, c_pair: int = 128, n_heads_pair: int = 4, *,
               **options) -> MSABlock:
     """An AF3 MSA-stack block (``src/foldforge/modules/engine/graph.py:240-276``); ``options``
     are :class:`foldforge_amd.modules.MSABlock`'s (Boltz order, Chai-1 parallel stages, the
-    outer-product-mean form)."""
+    outer-product-mean form, the dropouts' rates)."""
     return finish(MSABlock(c_msa, c_pair, n_heads_pair, **options), precision, norm_eps=norm_eps)
 
 

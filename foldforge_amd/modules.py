@@ -945,6 +945,8 @@ class MSABlock(MasterWeights, nn.Module):
     triangle attentions when ``with_pair_attention``, the transition). Every part owns its
     residual except the outer product mean, whose raw update is added here. ``parallel`` is
     Chai-1's block (every update of a stage reads the stage's input, ``graph.py:316-340``).
+    ``p_drop`` and ``p_drop_msa`` are the rates that :func:`foldforge_amd.training.set_dropout` gives the triangle ops
+    and the averaging (AF3: 0.25 and 0.15).
 
     ``block(msa [M, L, c_m], pair [L, L, c_z], msa_mask [M, L], pair_mask [L, L])`` ->
     ``(msa, pair)``: unbatched, like the reference's block; MSA rows are real where
@@ -959,7 +961,7 @@ class MSABlock(MasterWeights, nn.Module):
                  triangle_model: str = "af3", msa_first: bool = False, parallel: bool = False,
                  opm_channel: int = 32, opm_groups: int = 1, opm_projection_bias: bool = False,
                  opm_normalize_before_proj: bool = False,
-                 opm_count_offset: float | None = 1e-3) -> None:
+                 opm_count_offset: float | None = 1e-3, p_drop: float = 0.0, p_drop_msa: float = 0.0) -> None:
         super().__init__()
         if parallel and msa_first:
             raise ValueError("a parallel MSA block runs the outer product mean first")
@@ -968,13 +970,15 @@ class MSABlock(MasterWeights, nn.Module):
             c_msa, c_pair, opm_channel * opm_groups, groups=opm_groups,
             projection_bias=opm_projection_bias, normalize_before_proj=opm_normalize_before_proj,
             count_offset=None if opm_groups > 1 else opm_count_offset)
-        self.msa_attention1 = MSAPairWeightedAveraging(c_msa, c_pair, 8, msa_value_dim)
+        self.msa_attention1 = MSAPairWeightedAveraging(c_msa, c_pair, 8, msa_value_dim, p_drop=p_drop_msa)
         self.msa_transition = Transition(c_msa, 4)
-        self.triangle_multiplication_outgoing = TriangleMultiplication(c_pair, outgoing=True)
-        self.triangle_multiplication_incoming = TriangleMultiplication(c_pair, outgoing=False)
+        self.triangle_multiplication_outgoing = TriangleMultiplication(c_pair, outgoing=True, p_drop=p_drop)
+        self.triangle_multiplication_incoming = TriangleMultiplication(c_pair, outgoing=False, p_drop=p_drop)
         if with_pair_attention:
-            self.pair_attention1 = TriangleAttention(c_pair, n_heads_pair, starting=True, model=triangle_model)
-            self.pair_attention2 = TriangleAttention(c_pair, n_heads_pair, starting=False, model=triangle_model)
+            self.pair_attention1 = TriangleAttention(
+                c_pair, n_heads_pair, starting=True, p_drop=p_drop, model=triangle_model)
+            self.pair_attention2 = TriangleAttention(
+                c_pair, n_heads_pair, starting=False, p_drop=p_drop, model=triangle_model)
         self.pair_transition = Transition(c_pair, 4)
         self.backend = "pytorch"
 

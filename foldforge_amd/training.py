@@ -268,7 +268,8 @@ class DropoutStream:
 
 def set_dropout(model: nn.Module, stream: DropoutStream | None, p: float | None = None) -> list[str]:
     """Give every op of ``model`` that has a dropout (the triangle ops and the MSA pair-weighted averaging) its own, drawn
-    from ``stream``, at the op's rate ``p_drop`` or at ``p``; ops at rate 0 get none. The masks are AF3's: one for all rows
+    from ``stream``, at the op's rate ``p_drop`` (the factories', the trunk's and the blocks' keyword; 0 by default) or, all
+    of them, at ``p``; ops at rate 0 get none. The masks are AF3's: one for all rows
     of a pair or MSA tensor, for the ending node's attention one for all columns. They apply where the module is in training
     mode (``model.train()``), to the update before it is added, with or without gradients. ``stream=None`` takes them
     away. Returns the names of the ops that have one now."""

@@ -56,11 +56,11 @@ class PairformerTrunk(nn.Module):
 
     def __init__(self, n_blocks: int = 48, *, d_pair: int = 128, d_single: int = 384,
                  n_head_single: int = 16, triangle_model: str = "af3",
-                 precision: str = "master") -> None:
+                 precision: str = "master", p_drop: float = 0.0) -> None:
         super().__init__()
         self.blocks = nn.ModuleList(
             pairformer_block(d_pair=d_pair, triangle_model=triangle_model, d_single=d_single,
-                             n_head_single=n_head_single, precision=precision)  # type: ignore[arg-type]
+                             n_head_single=n_head_single, precision=precision, p_drop=p_drop)  # type: ignore[arg-type]
             for _ in range(n_blocks)
         )
 

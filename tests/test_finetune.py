@@ -12,8 +12,9 @@ import pytest
 import torch
 from torch.utils.checkpoint import checkpoint
 
+import foldforge_amd
 from foldforge_amd import dispatch, factories, modules, torch_ops, training
-from foldforge_amd.trunk import randomise
+from foldforge_amd.trunk import PairformerTrunk, randomise
 from oracle import training as oracle
 
 
@@ -293,3 +294,23 @@ def test_draws_of_two_threads_are_their_own():
         taken = [int(t) for t in pool.map(lambda _: stream.take(), range(24))]
     assert sorted(taken) == list(range(24))
     assert copy.deepcopy(stream).take() == 24
+
+
+def test_models_are_built_with_their_rates():
+    """AF3's two rates through every way to build a model; without them no op has a dropout."""
+    stream, tri = training.DropoutStream(1), dict(d_pair=64, n_head=4, starting=True, model="af3")
+    made = [(factories.triangle_multiplication(64, outgoing=True, p_drop=0.25), 1, {0.25}),
+            (factories.triangle_attention(**tri, p_drop=0.25), 1, {0.25}),
+            (factories.msa_pair_weighted_averaging(64, 64, p_drop=0.15), 1, {0.15}),
+            (factories.pairformer_block(d_pair=64, triangle_model="af3", p_drop=0.25), 4, {0.25}),
+            (factories.pairformer_block(d_pair=64, triangle_model="af3", divide_by_length=True, p_drop=0.25), 4, {0.25}),
+            (factories.msa_block(64, 64, p_drop=0.25, p_drop_msa=0.15), 5, {0.25, 0.15}),
+            (PairformerTrunk(2, d_pair=64, d_single=0, p_drop=0.25), 8, {0.25}),
+            (foldforge_amd.load(backend="pytorch", device="cpu", blocks=1, d_single=0, p_drop=0.25), 4, {0.25})]
+    for model, ops, rates in made:
+        names = training.set_dropout(model, stream)
+        assert len(names) == ops
+        assert {m.p for m in model.modules() if isinstance(m, modules.Dropout)} == rates
+        assert all("msa_attention" not in n or model.get_submodule(n).dropout.p == 0.15 for n in names)
+    assert training.set_dropout(factories.msa_block(64, 64), stream) == []
+    assert training.set_dropout(PairformerTrunk(1, d_pair=64, d_single=0), stream) == []
