@@ -245,9 +245,9 @@ __device__ __forceinline__ void thin_rows(const ThinArgs& p, int64_t block, Thin
     const bool is = mine == a;
     todo &= ~__ballot(is);
     if (turn % p.share != shared) continue;
-    f32x4 acc[N];
+    f32x4 acc[N], rest[N];
 #pragma unroll
-    for (int n = 0; n < N; ++n) acc[n] = none;
+    for (int n = 0; n < N; ++n) acc[n] = rest[n] = none;
     const TA* m[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
@@ -282,7 +282,10 @@ __device__ __forceinline__ void thin_rows(const ThinArgs& p, int64_t block, Thin
           bf16x8 mv[PARTS];
           mf[c][n].template parts<PARTS>(mv);
 #pragma unroll
-          for (int q = 0; q < PARTS; ++q) acc[n] = mfma16(mv[q], xv, acc[n]);
+          for (int q = 0; q < PARTS; ++q) {
+            f32x4& to = q ? rest[n] : acc[n];
+            to = mfma16(mv[q], xv, to);
+          }
         }
       }
     };
@@ -300,7 +303,7 @@ __device__ __forceinline__ void thin_rows(const ThinArgs& p, int64_t block, Thin
       for (; k < stop; ++k) steps(32 * k, std::integral_constant<int, 1>());
     __syncthreads();
 #pragma unroll
-    for (int n = 0; n < N; ++n) red[wave][n][lane] = acc[n];
+    for (int n = 0; n < N; ++n) red[wave][n][lane] = PARTS > 1 ? parts_sum(acc[n], rest[n]) : acc[n];
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < N; ++n)
@@ -487,8 +490,8 @@ constexpr int kMostGradTiles = 256;
 // sum over a chunk's rows of adapter blockIdx.y of v x^T: RP channels x 64 columns a workgroup. Tiles of 64 rows that have a
 // row of the adapter's, in order, through three buffers by LDS DMA; the rows of others in them are zeroed there. A wave takes
 // 16 of a tile's rows (k of the product; both operands turned as they are read), the waves' sums meet at the end in a fixed
-// order. The parts are products of their own into one sum (RP = 16: high and middle ones the 32 rows of one, low ones and
-// zeros of another). Workgroups: both jobs' tiles x adapters x chunks.
+// order. The parts are products of their own, the high ones' sum apart from that of the others (RP = 16: high and middle ones
+// the 32 rows of one product, low ones and zeros of another). Workgroups: both jobs' tiles x adapters x chunks.
 template <int RP>
 struct GradLds {
   static constexpr int VT = parts_ld(RP) / 64, STAGES = RP == 128 ? 2 : 3;
@@ -549,9 +552,9 @@ __device__ __forceinline__ void grad_tile(const GradArgs& p, int64_t block, Grad
 #pragma unroll
     for (int t = 0; t < VT; ++t) tile_dma(j.v, ld, row0, p.rows - 1, 64 * t, at + 8192 * (1 + t), wave, lane);
   };
-  f32x16 acc[JB][2];
+  f32x16 acc[2][JB][2];
 #pragma unroll
-  for (int b = 0; b < JB; ++b) acc[b][0] = acc[b][1] = zero16();
+  for (int b = 0; b < JB; ++b) acc[0][b][0] = acc[0][b][1] = acc[1][b][0] = acc[1][b][1] = zero16();
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s)
     if (s < steps) fetch(s);
@@ -579,26 +582,27 @@ __device__ __forceinline__ void grad_tile(const GradArgs& p, int64_t block, Grad
     for (int b = 0; b < BLOCKS; ++b) {  // 32 channels each: the high parts, the middle, the low ones
       const bf16x8 v = ld_turned(t[1 + b / 2], 32 * (b & 1), 16 * wave, lane);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) acc[b % JB][h] = mfma32(v, x[h], acc[b % JB][h]);
+      for (int h = 0; h < 2; ++h) acc[b >= JB][b % JB][h] = mfma32(v, x[h], acc[b >= JB][b % JB][h]);
     }
   }
-  float* sum = reinterpret_cast<float*>(buf);  // [wave][32][64]
+  constexpr int ROWS = RP == 16 ? 16 : 32;
+  float* sum = reinterpret_cast<float*>(buf);  // [wave][ROWS][64]
 #pragma unroll
   for (int b = 0; b < JB; ++b) {
     __syncthreads();
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sum[(wave * 32 + acc_row(r, g)) * 64 + 32 * h + li] = acc[b][h][r];
+      for (int r = 0; r < ROWS / 2; ++r) {
+        // (RP = 16: the middle parts' rows are 16 behind the high ones', eight registers on)
+        const float rest = RP == 16 ? acc[0][b][h][(r + 8) & 15] + acc[1][b][h][r] : acc[1][b][h][r];
+        sum[(wave * ROWS + acc_row(r, g)) * 64 + 32 * h + li] = parts_sum(acc[0][b][h][r], rest);
+      }
     __syncthreads();
-    for (int i = threadIdx.x; i < (RP == 16 ? 16 : 32) * 64; i += 256) {
+    for (int i = threadIdx.x; i < ROWS * 64; i += 256) {
       float v = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) v += sum[w * 2048 + i];
-      if constexpr (RP == 16) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) v += sum[w * 2048 + 1024 + i];
-      }
+      for (int w = 0; w < 4; ++w) v += sum[w * ROWS * 64 + i];
       const int row = 32 * b + (i >> 6), c = c0 + (i & 63);
       if (row >= p.rank || c >= j.cols) continue;
       const int64_t at =

@@ -432,19 +432,22 @@ __device__ __forceinline__ void thin_part(uint32_t at, int wave, int lane, const
   if (first >= 2) return;  // (fewer shares than waves)
 #pragma unroll
   for (int x = 0; x < X; ++x) {
-    f32x4 t[RB];
+    f32x4 t[RB], rest[RB];
 #pragma unroll
-    for (int b = 0; b < RB; ++b) t[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int b = 0; b < RB; ++b) t[b] = rest[b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       const bf16x8 v = row_operand<C>(at, first + x, SLOTS * q + wave % SLOTS);
 #pragma unroll
       for (int b = 0; b < RB; ++b)
 #pragma unroll
-        for (int k = 0; k < PARTS; ++k) t[b] = mfma16(m[q][b][k], v, t[b]);
+        for (int k = 0; k < PARTS; ++k) {
+          f32x4& to = k ? rest[b] : t[b];
+          to = mfma16(m[q][b][k], v, to);
+        }
     }
 #pragma unroll
-    for (int b = 0; b < RB; ++b) part[wave % SLOTS][first + x][b][lane] = t[b];
+    for (int b = 0; b < RB; ++b) part[wave % SLOTS][first + x][b][lane] = PARTS > 1 ? parts_sum(t[b], rest[b]) : t[b];
   }
 }
 
@@ -565,17 +568,19 @@ __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p
         }
     });
   };
-  // the sums of the request in work
-  f32x4 gi[RB][S::GI], go[RB][S::GO];
+  // the sums of the request in work: of the first parts of v and u, and of the others
+  f32x4 gi[2][RB][S::GI], go[2][RB][S::GO];
   int summed = -1;
   auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
-      for (int q = 0; q < S::GI; ++q) gi[b][q] = none;
+      for (int b = 0; b < RB; ++b) {
 #pragma unroll
-      for (int q = 0; q < S::GO; ++q) go[b][q] = none;
-    }
+        for (int q = 0; q < S::GI; ++q) gi[k][b][q] = none;
+#pragma unroll
+        for (int q = 0; q < S::GO; ++q) go[k][b][q] = none;
+      }
   };
   auto flush = [&]() __attribute__((always_inline)) {
     const int l = fresh_lane(), i = l & 15, g = l >> 4;
@@ -587,10 +592,10 @@ __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p
         float* row = to + (16 * b + 4 * g + e) * (CI + CO);
 #pragma unroll
         for (int q = 0; q < S::GI; ++q)
-          if (8 * q + wave < CI / 16) row[16 * (8 * q + wave)] = gi[b][q][e];
+          if (8 * q + wave < CI / 16) row[16 * (8 * q + wave)] = parts_sum(gi[0][b][q][e], gi[1][b][q][e]);
 #pragma unroll
         for (int q = 0; q < S::GO; ++q)
-          if (8 * q + wave < CO / 16) row[CI + 16 * (8 * q + wave)] = go[b][q][e];
+          if (8 * q + wave < CO / 16) row[CI + 16 * (8 * q + wave)] = parts_sum(go[0][b][q][e], go[1][b][q][e]);
       }
   };
   // this wave's rows of the staged dx
@@ -660,7 +665,7 @@ __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p
 #pragma unroll
         for (int b = 0; b < RB; ++b)
 #pragma unroll
-          for (int k = 0; k < 3; ++k) gi[b][q] = mfma16(gv[b][k], t, gi[b][q]);
+          for (int k = 0; k < 3; ++k) gi[k > 0][b][q] = mfma16(gv[b][k], t, gi[k > 0][b][q]);
       }
 #pragma unroll
     for (int b = 0; b < RB; ++b)
@@ -673,7 +678,7 @@ __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p
 #pragma unroll
         for (int b = 0; b < RB; ++b)
 #pragma unroll
-          for (int k = 0; k < 3; ++k) go[b][q] = mfma16(gv[b][k], t, go[b][q]);
+          for (int k = 0; k < 3; ++k) go[k > 0][b][q] = mfma16(gv[b][k], t, go[k > 0][b][q]);
       }
   };
   // dx of the tile at row0: to the stage, or to its rows

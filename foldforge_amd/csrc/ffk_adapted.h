@@ -23,4 +23,17 @@ __device__ __forceinline__ float scale_of(const Requests& q, int a) {
   return q.scale ? v : 1.f;
 }
 
+// A sum of products one of whose operands is kept as bf16 parts: `first` is that of the first parts, `rest` that of the
+// others. What an infinity leaves for its other parts is NaN, and so is an infinite other operand's product with parts of both
+// signs or of zero: where the first parts' sum is not finite it is the value by itself.
+__device__ __forceinline__ float parts_sum(float first, float rest) {
+  return __builtin_isfinite(first) ? first + rest : first;
+}
+__device__ __forceinline__ f32x4 parts_sum(const f32x4& first, const f32x4& rest) {
+  f32x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = parts_sum(first[e], rest[e]);
+  return v;
+}
+
 }  // namespace ffk

@@ -403,3 +403,36 @@ def test_two_streams_at_once():
         torch.cuda.synchronize()
         for p, q in zip(got, want):
             assert all(torch.equal(u, v) for u, v in zip(p, q))
+
+
+#: rows, d_in, d_out, rank: one pass at narrow and wide widths; tiles of each block of ranks
+INFINITE = [(4500, 128, 512, 7), (4500, 64, 64, 16), (8300, 256, 256, 5), (130, 72, 100, 5), (130, 64, 128, 32), (700, 384, 192, 40),
+            (300, 128, 64, 100)]
+
+
+@pytest.mark.parametrize("where", ["x", "dy", "down", "up"])
+@pytest.mark.parametrize("adapter", [BF16, F32])
+@pytest.mark.parametrize("rows, d_in, d_out, rank", INFINITE)
+def test_infinite_gradients_are_the_definitions(rows, d_in, d_out, rank, adapter, where):
+    """An infinity in the rows or in an adapter: each gradient is infinite, of its sign, or NaN, where the sums at 64 bits
+    are, and near them everywhere else. (u, v and fp32 adapters are kept in parts, whose own sums would be NaN.)"""
+    t = make(rows, d_in, d_out, rank, 3, [rows // 3] * 3, adapter=adapter)
+    row = rows // 3 + 1  # the second request's
+    at = {"x": (row, 3), "dy": (row, 3), "down": (1, rank - 1, 3), "up": (1, 3, rank - 1)}[where]
+    t[where][at] = float("-inf")
+    got = backward(gpu(t))
+    args, of = [t[k] for k in ("dy", "x", "weight", "down", "up", "scale")], rows_of(t)
+    want = oracle.adapted_linear_backward(*args, of)
+    mag = oracle.adapted_linear_backward(*(a.abs() for a in args), of)
+    unlike = 0
+    for g, w, m, width in zip(got, want, mag, (d_out, d_out, d_in)):
+        g = g.double().cpu()
+        assert torch.equal(g.isnan(), w.isnan()) and torch.equal(g.isposinf(), w.isposinf())
+        assert torch.equal(g.isneginf(), w.isneginf())
+        unlike += int((~w.isfinite()).sum())
+        tol = (width + rows + 10) * 2.0**-24 * m
+        if w.shape == t["x"].shape:  # dx: bf16, from bf16 adapters and rounded v
+            tol = tol + HALF * w.abs() + (1 if adapter == BF16 else 2) * HALF * (1 + 2 * HALF) * m
+        fine = w.isfinite()
+        assert ((g - w).abs()[fine] <= tol[fine]).all()
+    assert unlike > rank
