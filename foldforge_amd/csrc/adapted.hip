@@ -791,6 +791,7 @@ template <typename TW, typename TA, bool EVEN>
 void launch_few(const FewArgs& f, hipStream_t st) {
   const int64_t rows = f.q.rows;
   adapted_few_thin<TA, EVEN><<<dim3((unsigned)rows), 512, 0, st>>>(f);
+  if (hipPeekAtLastError() != hipSuccess) return;  // (the next launch would index by ids that are not there)
   const unsigned across = (unsigned)((f.N + 15) / 16);
   if (rows <= 16)
     adapted_few<TW, TA, 1, EVEN><<<dim3(across), 512, 0, st>>>(f);
@@ -801,6 +802,8 @@ template <typename TW, typename TA>
 void launch_few(const FewArgs& f, hipStream_t st) {
   f.K % 8 == 0 ? launch_few<TW, TA, true>(f, st) : launch_few<TW, TA, false>(f, st);
 }
+
+constexpr int64_t kMostPackBlocks = 1 << 20;
 
 int64_t tiles32(int64_t batch, int64_t rows, int64_t cols) { return batch * ((rows + 31) / 32) * ((cols + 31) / 32); }
 
@@ -825,15 +828,17 @@ struct Packer {
 
 template <typename TA, int RP, bool KEEP>
 void launch_prepare_as(const ThinArgs& t, const PackArgs& p, bool even, hipStream_t st) {
-  const dim3 grid((unsigned)(t.row_blocks * t.share * t.jobs + std::min<int64_t>(p.tiles, 1 << 20)));
+  const dim3 grid((unsigned)(t.row_blocks * t.share * t.jobs + std::min(p.tiles, kMostPackBlocks)));
   even ? adapted_prepare<TA, RP, KEEP, true><<<grid, 256, 0, st>>>(t, p)
        : adapted_prepare<TA, RP, KEEP, false><<<grid, 256, 0, st>>>(t, p);
 }
+int thin_share(int64_t rows, int requests) { return requests > rows / 16 ? 4 : 1; }  // (16 rows may have many adapters)
+
 template <bool KEEP>
 void launch_prepare(ThinArgs t, const PackArgs& p, int rp, int a_f32, hipStream_t st) {
   const int64_t rows = t.q.rows;
   const bool even = t.job[0].K % 8 == 0 && (t.jobs == 1 || t.job[1].K % 8 == 0);
-  t.share = t.q.count > rows / 16 ? 4 : 1;  // (16 rows may have many adapters)
+  t.share = thin_share(rows, t.q.count);
   t.row_blocks = (rows + 15) / 16;
 #define FFK_PREPARE(RP)                                                           \
   if (rp == RP) {                                                                 \
@@ -889,6 +894,7 @@ Requests requests_of(const AdaptedArgs& a) {
 AdaptedPlan adapted_plan(int64_t rows, int d_in, int d_out, int adapters, int rank, int requests, int w_f32, int a_f32,
                          int backward) {
   AdaptedPlan p{};
+  p.fits = 1;
   p.rp = rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128;
   p.ld = backward ? parts_ld(p.rp) : p.rp;
   p.kp = up64(d_in);
@@ -912,6 +918,15 @@ AdaptedPlan adapted_plan(int64_t rows, int d_in, int d_out, int adapters, int ra
     p.pack_w = w_f32 || d_in % 64 != 0;
     p.pack_up = a_f32 || rank != p.rp;
   }
+  if (p.few) return p;
+  const int64_t product = (rows + 63) / 64 * (((backward ? d_in : d_out) + 63) / 64);
+  int64_t blocks = (rows + 15) / 16 * thin_share(rows, requests) * (backward ? 2 : 1) + kMostPackBlocks;
+  blocks = std::max(blocks, product);
+  if (backward) {
+    const int64_t sums = (p.kp + p.np) / 64 * adapters * p.chunks, values = (int64_t)adapters * rank * (d_in + d_out);
+    blocks = std::max(blocks, std::max(product + sums, p.chunks > 1 ? values / 64 + 2 : 0));
+  }
+  p.fits = blocks < (int64_t(1) << 24);  // (of 256 threads)
   return p;
 }
 
@@ -952,6 +967,7 @@ void launch_adapted(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t st) 
   t.rank = a.rank;
   t.jobs = 1;
   launch_prepare<false>(t, pack.args, p.rp, a.a_f32, st);
+  if (hipPeekAtLastError() != hipSuccess) return;  // (the next launch would index by ids that are not there)
   ProductArgs g{};
   g.x = p.pack_x ? a.xp : a.x;
   g.w = p.pack_w ? a.wp : static_cast<const bf16*>(a.w);
@@ -990,6 +1006,7 @@ void launch_adapted_grad(const AdaptedArgs& a, const AdaptedPlan& p, hipStream_t
   t.rank = a.rank;
   t.jobs = 2;
   launch_prepare<true>(t, pack.args, p.rp, a.a_f32, st);
+  if (hipPeekAtLastError() != hipSuccess) return;
   const bf16 *x = p.pack_x ? a.xp : a.x, *dy = p.pack_dy ? a.dyp : a.dy;
   ProductArgs g{};
   g.x = dy;

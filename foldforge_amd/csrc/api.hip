@@ -653,6 +653,11 @@ bool adapted_sizes(int64_t rows, int32_t d_in, int32_t d_out, int32_t adapters, 
          ((rows + 63) / 64) * ((std::max(d_in, d_out) + 63) / 64) < (1 << 24);
 }
 
+int32_t adapted_fits(const char* what, const AdaptedArgs& a, const AdaptedPlan& p) {
+  if (p.fits) return FFK_OK;
+  return fail(FFK_ERR_INVALID, "%s: rows=%lld d_in=%d d_out=%d adapters=%d rank=%d requests=%d take more workgroups than a launch has", what, (long long)a.rows, a.d_in, a.d_out, a.adapters, a.rank, a.requests);
+}
+
 int32_t adapted_check(const char* what, const AdaptedArgs& a, int32_t weight_dtype, int32_t adapter_dtype) {
   if (!adapted_sizes(a.rows, a.d_in, a.d_out, a.adapters, a.rank, a.requests))
     return fail(FFK_ERR_INVALID, "%s: rows=%lld d_in=%d d_out=%d adapters=%d rank=%d requests=%d (widths up to 65536, rank up to 128, fewer than 65536 adapters)", what, (long long)a.rows, a.d_in, a.d_out, a.adapters, a.rank, a.requests);
@@ -679,8 +684,8 @@ size_t ffk_adapted_linear_workspace(int64_t rows, int32_t d_in, int32_t d_out, i
   a.rank = rank;
   a.requests = requests;
   a.a_f32 = adapter_dtype == FFK_DTYPE_F32;
-  return adapted_ws(nullptr, adapted_plan(rows, d_in, d_out, adapters, rank, requests,
-                                          weight_dtype == FFK_DTYPE_F32, a.a_f32, 0), a, 0);
+  const AdaptedPlan p = adapted_plan(rows, d_in, d_out, adapters, rank, requests, weight_dtype == FFK_DTYPE_F32, a.a_f32, 0);
+  return p.fits ? adapted_ws(nullptr, p, a, 0) : 0;
 }
 
 int32_t ffk_adapted_linear(const void* x, const void* weight, const float* bias, const void* down, const void* up,
@@ -710,6 +715,7 @@ int32_t ffk_adapted_linear(const void* x, const void* weight, const float* bias,
   if (rows == 0) return ok();
   if (!out || out == x) return fail(FFK_ERR_INVALID, "adapted_linear: the output is null or x");
   const AdaptedPlan p = adapted_plan(rows, d_in, d_out, adapters, rank, requests, a.w_f32, a.a_f32, 0);
+  if (int32_t s = adapted_fits("adapted_linear", a, p)) return s;
   const size_t need = adapted_ws(workspace, p, a, 0);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(FFK_ERR_WORKSPACE, "adapted_linear: workspace %zu bytes < %zu", workspace_bytes, need);
@@ -728,8 +734,8 @@ size_t ffk_adapted_linear_backward_workspace(int64_t rows, int32_t d_in, int32_t
   a.rank = rank;
   a.requests = requests;
   a.a_f32 = adapter_dtype == FFK_DTYPE_F32;
-  return adapted_ws(nullptr, adapted_plan(rows, d_in, d_out, adapters, rank, requests,
-                                          weight_dtype == FFK_DTYPE_F32, a.a_f32, 1), a, 1);
+  const AdaptedPlan p = adapted_plan(rows, d_in, d_out, adapters, rank, requests, weight_dtype == FFK_DTYPE_F32, a.a_f32, 1);
+  return p.fits ? adapted_ws(nullptr, p, a, 1) : 0;
 }
 
 int32_t ffk_adapted_linear_backward(const void* dy, const void* x, const void* weight, const void* down, const void* up,
@@ -767,6 +773,7 @@ int32_t ffk_adapted_linear_backward(const void* dy, const void* x, const void* w
     return fail(FFK_ERR_INVALID, "adapted_linear_backward: null argument, or dy off 16-byte alignment");
   if (dx && (dx == x || dx == dy)) return fail(FFK_ERR_INVALID, "adapted_linear_backward: dx may not be x or dy");
   const AdaptedPlan p = adapted_plan(rows, d_in, d_out, adapters, rank, requests, a.w_f32, a.a_f32, 1);
+  if (int32_t s = adapted_fits("adapted_linear_backward", a, p)) return s;
   const size_t need = adapted_ws(workspace, p, a, 1);
   if (!workspace || workspace_bytes < need || !aligned16(workspace))
     return fail(FFK_ERR_WORKSPACE, "adapted_linear_backward: workspace %zu bytes < %zu", workspace_bytes, need);

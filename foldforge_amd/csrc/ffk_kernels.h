@@ -434,6 +434,7 @@ struct AdaptedPlan {
   int pack_x, pack_dy, pack_w, pack_up;  // which the wide product reads from copies (backward: w and down always)
   int64_t chunk;     // backward: rows of a workgroup's sums
   int chunks;
+  int fits;          // every launch has fewer than 2^32 threads
 };
 AdaptedPlan adapted_plan(int64_t rows, int d_in, int d_out, int adapters, int rank, int requests, int w_f32, int a_f32,
                          int backward);

@@ -129,8 +129,8 @@ int32_t ffk_dropout_add(const void* x, const void* residual, void* out, const in
  * NULL (1). Request r has the rows offsets[r] .. offsets[r + 1] - 1 (offsets [requests + 1], not decreasing; none where they
  * are the same); rows of no request, and requests whose adapter is not in [0, adapters), get W x + bias. Two requests may
  * share an adapter (offsets that decrease give unspecified values). x, out, the weights: 16-byte aligned, out not x; rank up
- * to 128, widths up to 65536. Products of bf16 operands (fp32 ones are rounded), fp32 sums; the rows A x in fp32 up to 256
- * rows, in bf16 above.
+ * to 128, widths up to 65536; sizes whose launches would have 2^24 workgroups or more are refused. Products of bf16 operands
+ * (fp32 ones are rounded), fp32 sums; the rows A x in fp32 up to 256 rows, in bf16 above.
  */
 size_t ffk_adapted_linear_workspace(int64_t rows, int32_t d_in, int32_t d_out, int32_t adapters, int32_t rank,
                                     int32_t requests, int32_t weight_dtype, int32_t adapter_dtype);

@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from foldforge_amd import kernels
+from foldforge_amd import _native, kernels
 from oracle import training as oracle
 
 
@@ -102,3 +102,19 @@ def test_sizes_that_are_served():
     for d_in, d_out, rank, n in ((0, 8, 4, 1), (8, 65537, 4, 1), (8, 8, 0, 1), (8, 8, 129, 1), (8, 8, 4, 65536),
                                  (65536, 8, 128, 4096)):
         assert not kernels.adapted_linear_supported(d_in, d_out, rank, n)
+
+
+def test_calls_of_more_workgroups_than_a_launch_has():
+    """2^24 workgroups of 256 threads are more than a launch takes: such a call is refused (its workspace is 0) before
+    anything runs, the largest below it is not."""
+    lib = _native.lib()
+    forward, backward = lib.ffk_adapted_linear_workspace, lib.ffk_adapted_linear_backward_workspace
+    bf16 = (0, 0)
+    # 16 rows a workgroup for the thin products (four of them where requests are short), forward and of both matrices backward
+    assert forward(2**27, 64, 64, 1, 48, 1, *bf16) > 0 and forward(2**28, 64, 64, 1, 48, 1, *bf16) == 0
+    assert forward(2**25, 64, 64, 1, 48, 2**25, *bf16) > 0 and forward(2**26, 64, 64, 1, 48, 2**26, *bf16) == 0
+    assert backward(2**26, 64, 64, 1, 48, 1, *bf16) > 0 and backward(2**27, 64, 64, 1, 48, 1, *bf16) == 0
+    # a sum of every adapter in each 16384 rows
+    assert backward(2**19, 72, 72, 65535, 1, 16, *bf16) > 0 and backward(2**20, 72, 72, 65535, 1, 16, *bf16) == 0
+    # and the join of those sums
+    assert backward(2**15, 8192, 8192, 1000, 64, 16, *bf16) > 0 and backward(2**15, 8192, 8192, 1000, 128, 16, *bf16) == 0
