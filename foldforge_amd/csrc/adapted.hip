@@ -27,16 +27,16 @@ namespace {
 // which adapter a row has
 
 // id[i], i < 64: the adapter of row row0 + i, -1 for none (and behind the last row). All threads of the workgroup; start is
-// scratch. The first wave passes over the offsets once: how many begin at or before the first row, and which begin at each of
-// the others; then the latest request that begins at or before each row. Offsets out of order give some adapter or none, never
-// an access out of range.
+// scratch. The first wave passes over the offsets near the tile's rows: how many begin at or before the first row, and which
+// begin at each of the others; then the latest request that begins at or before each row. Offsets out of order give some
+// adapter or none, never an access out of range.
 __device__ __forceinline__ void tile_ids(const Requests& q, int64_t row0, int* id, int* start) {
   const int tid = threadIdx.x;
   if (tid < 64) {
     start[tid] = -1;
     __builtin_amdgcn_wave_barrier();  // (the wave's own: LDS operations complete in order)
-    int before = 0;
-    for (int i0 = tid; i0 - tid <= q.count; i0 += 256) {
+    int before = (int)offsets_near(q, row0, tid).from;
+    for (int i0 = before + tid; i0 - tid <= q.count; i0 += 256) {
       int offset[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) offset[u] = q.offsets[i0 + 64 * u < q.count ? i0 + 64 * u : q.count];
@@ -47,6 +47,7 @@ __device__ __forceinline__ void tile_ids(const Requests& q, int64_t row0, int* i
         before += __popcll(__ballot(i <= q.count && at <= 0));
         if (i <= q.count && at > 0 && at < 64) atomicMax(&start[at], i);
       }
+      if (__ballot(offset[3] - row0 >= 64)) break;  // (the others begin behind the tile)
     }
     __builtin_amdgcn_wave_barrier();
     int r = tid == 0 ? before - 1 : start[tid];

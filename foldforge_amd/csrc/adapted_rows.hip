@@ -31,14 +31,17 @@ __device__ __forceinline__ int64_t request_end(const Requests& q, int r) {
   return r < q.count ? (int64_t)q.offsets[r + 1] : q.rows;  // (r = -1: the rows before the first request)
 }
 __device__ __forceinline__ RequestAt request_first(const Requests& q, int64_t row, int lane) {
-  int before = 0;  // the offsets up to `row` (in order: of the first requests), counted by a wave
-  for (int i0 = lane; i0 - lane <= q.count; i0 += 256) {
-    int offset[4];
+  const OffsetRange near = offsets_near(q, row, lane);
+  int before = (int)near.from;  // the offsets up to `row` (in order: of the first requests), counted by a wave
+  int offset[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) offset[u] = q.offsets[i0 + 64 * u < q.count ? i0 + 64 * u : q.count];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) before += __popcll(__ballot(offset[u] <= row && i0 + 64 * u <= q.count));
+  for (int u = 0; u < 4; ++u) {
+    const int64_t i = near.from + lane + 64 * u;
+    offset[u] = q.offsets[i < q.count ? i : q.count];
   }
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    before += __popcll(__ballot(near.from + lane + 64 * u < near.to && offset[u] <= row));
   const int r = before - 1;
   return {r, adapter_at(q, r), request_end(q, r)};
 }

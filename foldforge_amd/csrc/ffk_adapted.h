@@ -23,6 +23,22 @@ __device__ __forceinline__ float scale_of(const Requests& q, int a) {
   return q.scale ? v : 1.f;
 }
 
+// The offsets from `from` on, 256 at most, among which the first behind `row` is (`to` where none of them is): those before
+// are at or before the row. By 64 probes of a wave a round; offsets out of order give some place among them.
+// 100000 one-row requests, 64 -> 64: 0.11 ms forward and 0.25 backward (3.2 and 6.5 with each workgroup passing over them all).
+struct OffsetRange {
+  int64_t from, to;
+};
+__device__ __forceinline__ OffsetRange offsets_near(const Requests& q, int64_t row, int lane) {
+  OffsetRange r{0, (int64_t)q.count + 1};
+  while (r.to - r.from > 256) {
+    const int64_t step = (r.to - r.from + 63) / 64, at = r.from + (lane + 1) * step - 1;
+    r.from += __popcll(__ballot(at < r.to && q.offsets[at < r.to ? at : r.to - 1] <= row)) * step;
+    if (r.from + step - 1 < r.to) r.to = r.from + step - 1;
+  }
+  return r;
+}
+
 // A sum of products one of whose operands is kept as bf16 parts: `first` is that of the first parts, `rest` that of the
 // others. What an infinity leaves for its other parts is NaN, and so is an infinite other operand's product with parts of both
 // signs or of zero: where the first parts' sum is not finite it is the value by itself.

@@ -436,3 +436,42 @@ def test_infinite_gradients_are_the_definitions(rows, d_in, d_out, rank, adapter
         fine = w.isfinite()
         assert ((g - w).abs()[fine] <= tol[fine]).all()
     assert unlike > rank
+
+
+@pytest.mark.parametrize("rows, lengths", [(30011, [1] * 30000), (2000, [0] * 700 + [1000] + [0] * 9000 + [3, 0, 0, 900]),
+                                           (300, [0] * 300 + [150, 0, 149] + [0] * 5000), (700, [2] * 300 + [0] * 257 + [99])])
+def test_requests_by_the_thousand(rows, lengths):
+    """One-row requests, and runs of empty ones, that no workgroup can walk from the first."""
+    t = make(rows, 64, 72, 8, 5, lengths, adapter=F32)
+    check_forward(t, forward(gpu(t)))
+    check_backward(t, backward(gpu(t)))
+
+
+def test_offsets_of_many_requests_out_of_order():
+    """Any values: some adapter or none, no access out of range."""
+    g = torch.Generator().manual_seed(3)
+    for rows in (300, 3000):
+        t = gpu(make(rows, 64, 64, 8, 3, [1] * 5000))
+        for low, high in ((0, rows), (-2**31, 2**31 - 1), (rows - 1, rows + 1)):
+            t["offsets"] = torch.randint(low, high, (5001,), generator=g, dtype=torch.int64).to(DEV, torch.int32)
+            assert torch.isfinite(forward(t).float()).all()
+            assert torch.isfinite(backward(t).x.float()).all()
+
+
+def test_time_grows_with_the_rows_of_short_requests():
+    """Ten times the one-row requests take some ten times as long, not a hundred times: no workgroup passes over all of
+    them. (Both calls in the form for short requests; 30 leaves three times the rows' share to noise.)"""
+    def time(n):
+        t = gpu(make(n, 64, 64, 8, 4, [1] * n))
+        times = []
+        for _ in range(4):
+            start, end = torch.cuda.Event(True), torch.cuda.Event(True)
+            start.record()
+            for _ in range(3):
+                backward(t)
+            end.record()
+            torch.cuda.synchronize()
+            times.append(start.elapsed_time(end))
+        return min(times)
+
+    assert time(200_000) <= 30 * time(20_000)
