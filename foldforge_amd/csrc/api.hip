@@ -649,6 +649,7 @@ constexpr int kMostRank = 128;
 bool adapted_sizes(int64_t rows, int32_t d_in, int32_t d_out, int32_t adapters, int32_t rank, int32_t requests) {
   return rows >= 0 && rows <= 0x7fffffffLL && d_in > 0 && d_in <= kMostAdapted && d_out > 0 && d_out <= kMostAdapted &&
          adapters > 0 && adapters < kMostAdapted && rank > 0 && rank <= kMostRank && requests >= 0 &&
+         requests < 0x7fffffff - 1024 &&  // (the kernels count offsets in steps of 256 in 32 bits)
          (int64_t)adapters * rank * std::max(d_in, d_out) <= 0x7fffffffLL &&
          ((rows + 63) / 64) * ((std::max(d_in, d_out) + 63) / 64) < (1 << 24);
 }

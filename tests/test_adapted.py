@@ -118,3 +118,11 @@ def test_calls_of_more_workgroups_than_a_launch_has():
     assert backward(2**19, 72, 72, 65535, 1, 16, *bf16) > 0 and backward(2**20, 72, 72, 65535, 1, 16, *bf16) == 0
     # and the join of those sums
     assert backward(2**15, 8192, 8192, 1000, 64, 16, *bf16) > 0 and backward(2**15, 8192, 8192, 1000, 128, 16, *bf16) == 0
+
+
+def test_as_many_requests_as_are_counted_in_32_bits():
+    """The passes over the offsets go on in steps of 256: a count next to 2^31 would run over and never end."""
+    lib = _native.lib()
+    for size in (lib.ffk_adapted_linear_workspace, lib.ffk_adapted_linear_backward_workspace):
+        assert size(1000, 72, 72, 1, 4, 2**31 - 2000, 0, 0) > 0
+        assert size(1000, 72, 72, 1, 4, 2**31 - 1, 0, 0) == 0
