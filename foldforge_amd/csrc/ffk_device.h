@@ -38,6 +38,14 @@ __device__ __forceinline__ f32x16 zero16() {
   return z;
 }
 
+// The wait states that another use of a 32 x 32 product's result has to stand off, for products in front of a branch: behind
+// the join of two paths the compiler counts them along one, and where that is the longer path the other's come too short.
+__device__ __forceinline__ void products_written() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 11");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // Row (within a 32x32 MFMA tile) held by accumulator register r of lane group g.
 __device__ __forceinline__ int acc_row(int r, int g) { return 8 * (r >> 2) + 4 * g + (r & 3); }
 

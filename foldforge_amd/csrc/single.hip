@@ -949,6 +949,7 @@ __global__ __launch_bounds__(64 * stream_waves(K), stream_simd_waves(EPI, K)) vo
       const f32x16 acc = product(ot - ot0, false);
       int seg = 0, cbase = 0;
       if (EPI == kEpiApb) (void)tile_weight_row<EPI>(a, ot, li, seg, cbase);
+      if constexpr (EPI == kEpiResid && K == 256) products_written();
       if (m < a.M) row_epilogue<EPI>(a, acc, m, ot, seg, cbase, g, lb, 0.f, rpre, ypre);
     };
     if constexpr (EPI == kEpiTrimul) {
@@ -959,6 +960,7 @@ __global__ __launch_bounds__(64 * stream_waves(K), stream_simd_waves(EPI, K)) vo
       for (int u = 0; u < nt; u += 2) {
         f32x16 y = product(u, true);
         const f32x16 gate = product(u + 1, true);
+        products_written();
         if (bits != ~0u) {
 #pragma unroll
           for (int v = 0; v < 4; ++v)
