@@ -6,6 +6,7 @@ results, whose magnitudes |residual| + |scaled update| bounds, and the output's 
 
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
@@ -154,3 +155,24 @@ def test_two_streams_at_once():
                 got[i] = kernels.dropout_add(xg, rg, p=0.25, seed=4, offset=i, shared=1)
         torch.cuda.synchronize()
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("shape, shared", [((2**31 + 4099,), None), ((1, 2, 2**31 + 1001), 1), ((2, 3, 2**30 + 8), 1)])
+def test_more_values_than_32_bits_count(shape, shared):
+    """Places and mask numbers behind 2^31, in place, at both ends and around the powers of two."""
+    x = torch.ones(shape, dtype=BF16, device=DEV)
+    assert kernels.dropout_backward(x, p=0.5, seed=2**40 + 3, offset=9, shared=shared, out=x) is x
+    flat, n = x.view(-1), x.numel()
+    inner = shape[-1] if shared is not None else n
+    for begin in (0, 2**30 - 50, 2**31 - 50, 2**32 - 50, inner - 60, inner * shape[0] - 60, n - 100):
+        if not 0 <= begin < n - 1:
+            continue
+        place = torch.arange(begin, min(begin + 100, n))
+        row, col = place // inner, place % inner
+        number = col if shared is None else row // shape[1] * inner + col  # of the mask
+        block = (number >> 3).numpy().astype("uint64")
+        counter = np.stack([block % 2**32, block // 2**32, np.full_like(block, 9), np.zeros_like(block)], 1)
+        words = oracle.philox(counter, 2**40 + 3)
+        halves = np.stack([words % 2**16, words // 2**16], 2).reshape(-1, 8)
+        keep = torch.from_numpy(halves[np.arange(len(place)), (number & 7).numpy()] >= 32768)
+        assert torch.equal(flat[begin:begin + len(place)].cpu(), 2.0 * keep.to(BF16)), begin

@@ -242,3 +242,47 @@ def test_a_captured_model_with_dropout_is_refused():
             want = model(zs, mask, s)
         torch.cuda.synchronize()
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_adapters_of_a_model_that_keeps_8_bits():
+    """``keep="8bit"`` after ``adapt``: the values and the adapters' gradients are those of ``"input"`` bit for bit (the
+    projections keep their own inputs). The input's gradient passes the norm at the values that the 8 bits stand for, each off
+    by at most 2^-4 of itself: of dx = rstd (g - mean g - n mean(g n)), rstd and both n by as much at most."""
+    tr = randomise(modules.Transition(128, 4), 3)
+    tr.set_master_weights()
+    tr.to(DEV)
+    _with_adapters(tr, 2)
+    training.select_adapters(tr, torch.tensor([1, 0], dtype=torch.int32, device=DEV))
+    g = torch.Generator().manual_seed(2)
+    x, dy = (torch.randn(2, 24, 24, 128, generator=g).to(DEV, BF16) for _ in range(2))
+    results = []
+    for keep in ("input", "8bit"):
+        assert training.install(tr, keep, requires_grad=False)["hip"] == [""]
+        leaf = x.clone().requires_grad_(True)
+        tr.zero_grad()
+        update = tr.delta(leaf)
+        update.backward(dy)
+        results.append((update.detach(), leaf.grad, *(p.grad.clone() for p in tr.parameters() if p.requires_grad)))
+    assert len(results[0]) == 8
+    for i, (a, b) in enumerate(zip(*results)):
+        if i == 1:
+            assert 0 < _norm(b, a) <= 3 * 2.0**-4
+        else:
+            assert torch.equal(a, b), i
+
+
+def test_new_adapters_on_the_kernels():
+    """``up`` of zeros: the op runs as its three projections, whose results it rounds, and stays as near to the equations as the
+    op without adapters does."""
+    tr = randomise(modules.Transition(128, 4), 3)
+    tr.set_master_weights()
+    tr.to(DEV)
+    x = torch.randn(2, 24, 24, 128, generator=torch.Generator().manual_seed(2)).to(DEV, BF16)
+    with torch.no_grad():
+        want = tr.delta(x.float())
+        training.adapt(tr, 8, adapters=2)
+        tr.set_backend("hip")
+        for selected in (None, torch.tensor([1, -1], dtype=torch.int32, device=DEV)):
+            training.select_adapters(tr, selected)
+            assert _norm(tr.delta(x), want) <= 1e-2
+            assert torch.equal(tr(x), x + tr.delta(x))
