@@ -146,8 +146,12 @@ class EngineOp:
     dropout_axis: int | None = None
 
     def active_dropout(self) -> "Dropout | None":
-        """The op's dropout (:func:`foldforge_amd.training.set_dropout`) where it applies: in training mode."""
-        return self._modules.get("dropout") if self.training else None  # type: ignore[attr-defined]
+        """The op's dropout (:func:`foldforge_amd.training.set_dropout`) where it applies: in training mode. It refuses as
+        the op does."""
+        dropout = self._modules.get("dropout") if self.training else None  # type: ignore[attr-defined]
+        if dropout is not None:
+            dropout.refusal_policy = self.refusal_policy
+        return dropout
 
     def forward(self, *args: Any, **kwargs: Any) -> Any:
         dropout = self.active_dropout()

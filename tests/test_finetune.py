@@ -314,3 +314,24 @@ def test_models_are_built_with_their_rates():
         assert all("msa_attention" not in n or model.get_submodule(n).dropout.p == 0.15 for n in names)
     assert training.set_dropout(factories.msa_block(64, 64), stream) == []
     assert training.set_dropout(PairformerTrunk(1, d_pair=64, d_single=0), stream) == []
+
+
+def test_a_dropout_refuses_as_its_op_does():
+    """What the kernel does not take falls back, or raises, by the policy of the op, also one that is set later."""
+    block, (z, mask) = _block(), _inputs()
+    op = block.tri_multi_outgoing
+    training.set_dropout(block, training.DropoutStream(3, 20))
+    op.dropout.set_backend("hip")  # (the tensors are on the CPU)
+    with pytest.raises(modules.BackendUnsupported):
+        op(z, mask)
+    dispatch.set_refusal(block, "fallback")
+    op.dropout.stream.offset = 20
+    got = op(z, mask)
+    assert dispatch.ledger_of(op.dropout).served["pytorch"] == 1
+    op.dropout.set_backend("pytorch")
+    op.dropout.stream.offset = 20
+    assert torch.equal(op(z, mask), got)
+    op.dropout.set_backend("hip")
+    dispatch.set_refusal(block, "error")
+    with pytest.raises(dispatch.BackendUnsupportedError):
+        op.delta(z, mask)
