@@ -899,14 +899,16 @@ void launch_grad(const RowsGradArgs& p, int grid, hipStream_t st) {
 }  // namespace
 
 // Against tiles (adapted.hip; us, one pass : tiles, rank 16). Up to 128 channels in it is the faster at every size (128 -> 512:
-// 300 rows 9.1 : 10.4, 64000 29 : 43; in requests of 500 12.1 : 10.7 at 4000 and 12.0 : 13.3 at 8000). Wider ones read W into
-// registers first: 256 -> 256 in requests of 500 13.2 : 11.5 at 8000, 13.5 : 16.3 at 16000; 512 -> 128 13.1 : 11.8 and 14.9 :
-// 16.4; 384 -> 384 13.6 : 12.1 at 4000, 15.2 : 17.8 at 8000. Requests of 100 rows cost it a little more (384 -> 1536 64000 rows
-// 163 : 155, 256 -> 256 31 : 47), below 64 rows the adapters' turns outweigh the rest (32000 rows of 512 23 : 29, 4000 of 250 15 : 11).
+// 300 rows 9.1 : 10.4, 64000 26 : 44). Wider ones read W into registers first: 256 -> 256 in requests of 500 12.5 : 9.3 at 4000
+// rows, 13.0 : 15.2 at 16000; 512 -> 128 14.3 : 11.1 and 16.7 : 17.7; 384 -> 384 13.3 : 11.3 and 21.2 : 21.8. An adapter's turn
+// costs it more than tiles, so short requests need many rows: 32 rows each 8.9 : 11.3 (64 -> 256), 8.7 : 9.3 (128 -> 128) and
+// 13.7 : 14.3 (256 -> 256) at 16000, 24 : 29, 21 : 25 and 36 : 39 at 64000, but 8.1 : 6.9, 7.9 : 7.2 and 12.7 : 8.3 at 4000; 16 rows
+// each 39 : 32 (64 -> 256, 64000 rows). 384 channels, whose waves all take the thin product: 27 : 21 at 32 rows each, 27 : 25 at
+// 62, 23 : 23 at 100 (16000 rows).
 bool adapted_rows_served(int64_t rows, int d_in, int d_out, int rank, int requests) {
   const bool width = d_in == 64 || d_in == 128 || d_in == 256 ? d_out % 64 == 0 : (d_in == 384 || d_in == 512) && d_out % 128 == 0;
-  const int64_t least = d_in <= 128 ? 257 : d_in == 384 ? 6144 : 12288;
-  return width && rank <= 32 && rows >= least && rows >= 64 * (int64_t)requests;
+  const int64_t least = d_in <= 128 ? 257 : d_in == 384 ? 6144 : 12288, each = d_in != 384 && rows >= 16000 ? 32 : 64;
+  return width && rank <= 32 && rows >= least && rows >= each * requests;
 }
 
 void launch_adapted_rows(const AdaptedArgs& a, hipStream_t st) {
@@ -938,16 +940,17 @@ void launch_adapted_rows(const AdaptedArgs& a, hipStream_t st) {
 
 int adapted_rows_grid(int64_t rows) { return (int)std::min<int64_t>((rows + 31) / 32, cu_count()); }
 
-// Against tiles (us, one pass : tiles, fp32 adapters of rank 16): 64 -> 64 14.2 : 17.1 at 4000 rows, 128 -> 128 17.3 : 18.9 in
-// requests of 1000, both no faster at 1000; 128 -> 512 24.3 : 20.7 at 4000, 27.6 : 25.4 at 8000, 31.0 : 34.2 at 16000 and
-// 56 : 101 at 64000. Requests of 100 rows: 16000 rows 30 : 34 (128 -> 128), 41 : 40 (128 -> 512).
+// Against tiles (us, one pass : tiles, fp32 adapters of rank 16; requests of 500): 64 -> 64 15.3 : 14.9 at 4000 rows, 16.6 : 23.7
+// at 8000, 128 -> 128 16.9 : 15.6 and 18.9 : 25.2; 128 -> 512 24.6 : 17.8 at 4000, 28.4 : 29.3 at 8000, 43 : 69 at 32000. Requests
+// of 48 rows: 20 : 26 (64 -> 64, 4000 rows), 28 : 47 (128 -> 128, 8000), 40 : 52 and 60 : 56 (128 -> 512, 8000 and 16000); of 32:
+// 25 : 37 (64 -> 64, 8000), but 44 : 39 at 16000 and 59 : 47 (128 -> 512).
 bool adapted_rows_grad_served(int64_t rows, int d_in, int d_out, int rank, int requests) {
   bool width = false;
 #define FFK_ROWS_IS(C, N) width = width || (d_in == C && d_out == N);
   FFK_ROWS_WIDTHS(FFK_ROWS_IS)
 #undef FFK_ROWS_IS
   const int64_t least = d_in + d_out <= 320 ? 4096 : 8192;
-  return width && rank <= 16 && rows >= least && requests <= kMostRowsRequests && rows >= 64 * (int64_t)requests;
+  return width && rank <= 16 && rows >= least && requests <= kMostRowsRequests && rows >= 48 * (int64_t)requests;
 }
 
 void launch_adapted_rows_grad(const AdaptedArgs& a, hipStream_t st) {

@@ -155,3 +155,25 @@ def test_more_values_than_32_bits_count(rank, served):
     got = backward(g)
     check_backward(t, kernels.AdaptedGradients(got.x[at.to(DEV)], got.down, got.up))
     assert int((got.x != 0).any(1).sum()) <= len(at)
+
+
+@pytest.mark.parametrize("rows, d_in, d_out, each, served", [(16000, 64, 256, 32, "rows"), (16000, 128, 128, 32, "rows"),
+                                                             (16031, 256, 192, 32, "rows"), (16016, 512, 128, 33, "rows"),
+                                                             (15990, 128, 128, 63, "tiles"), (16000, 128, 512, 31, "tiles"),
+                                                             (16000, 384, 384, 63, "tiles"), (6400, 384, 128, 64, "rows")])
+def test_short_requests(rows, d_in, d_out, each, served):
+    """Several requests to a tile, forward."""
+    t = make(rows, d_in, d_out, 9, 5, [each] * (rows // each), adapter=F32)
+    g = gpu(t)
+    assert form(g, "forward") == served
+    check_forward(t, forward(g))
+
+
+@pytest.mark.parametrize("rows, d_in, d_out, each, served", [(4100, 64, 64, 48, "rows"), (8200, 128, 512, 48, "rows"),
+                                                             (4100, 128, 128, 47, "tiles"), (8200, 512, 128, 50, "rows"),
+                                                             (24600, 256, 256, 48, "rows")])
+def test_short_requests_backward(rows, d_in, d_out, each, served):
+    t = make(rows, d_in, d_out, 9, 5, [each] * (rows // each), adapter=F32)
+    g = gpu(t)
+    assert form(g, "backward") == served
+    check_backward(t, backward(g))
