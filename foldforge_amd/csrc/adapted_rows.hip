@@ -16,8 +16,10 @@ namespace ffk {
 
 namespace {
 
-// The request that a row lies in, walked upwards: rows [.., hi) from the row asked for on have adapter a (-1: none). All
-// scalar. Offsets out of order give some request, never an access out of range.
+// The request that a row lies in, walked upwards: rows [.., hi) from the row asked for on have adapter a (-1: none). The same in
+// all lanes. The walk reads the offset and the adapter by vector loads (the kernel also stores, so the compiler makes no scalar
+// ones) and waits for each with everything else in flight: a boundary between requests drains the tiles on their way, twice, and
+// so does each empty request. Offsets out of order give some request, never an access out of range.
 struct RequestAt {
   int r, a;
   int64_t hi;
@@ -175,7 +177,9 @@ __device__ __forceinline__ bf16x8 join_blocks(const f32x4& a, const f32x4& b) {
 // again where it changes). The tiles in LDS: one in work, the others on their way. rank <= 16 RB. grid: ranges of consecutive
 // tiles, for each the slices of NS outputs (neighbours, so that a range's rows are fetched into one XCD's L2 once); block 512.
 // 262144 rows of rank 16: 64 -> 128 23 us (4.5 TB/s), 128 -> 128 30 (4.5), 256 -> 64 33 (5.1), 128 -> 512 79 (4.2), 512 -> 128 74
-// to 78 (4.4): bytes, the more so the narrower. 16000 rows, 384 -> 1536: 38 us, chains of tiles behind W's slices.
+// to 78 (4.4): bytes, the more so the narrower. 16000 rows, 384 -> 1536: 38 us, chains of tiles behind W's slices. 512 -> 128
+// needs 10 registers more than there are: W alone takes half of them, and what is spilled is read again behind a wait for all
+// transfers.
 template <int C, int NS, int RB>
 __global__ __launch_bounds__(512, 2) void adapted_rows(const RowsArgs p, int slices) {
   using S = RowsShape<C, NS>;
@@ -461,8 +465,8 @@ __device__ __forceinline__ void thin_part(uint32_t at, int wave, int lane, const
 // three bf16 parts with tokens as k for the gradients (their sum is as exact as fp32's), whose other operand is the tile turned
 // as it is read. dx of 16 channels a wave goes through LDS to stores of whole rows. PARTS = 3: fp32 adapters, in three parts
 // as well. block 512.
-// 262144 rows, 128 -> 512, rank 16: 138 us, of which the rows' traffic (403 MB at the rate of a copy) is 79; a step's own work
-// is about as long, and one workgroup of a compute unit has only its own eight waves to hide it with. Measured and not
+// 262144 rows, 128 -> 512, rank 16: 138 us (fp32 adapters 143 to 150), of which the rows' traffic (403 MB at the rate of a copy)
+// is 79; a step's own work is about as long, and one workgroup of a compute unit has only its own eight waves to hide it with. Measured and not
 // kept: dy W by halves of k with half the reads of dy (143 us, and 3 us more for few rows), three barriers a step (144).
 template <int CI, int CO, int RB, int PARTS>
 __global__ __launch_bounds__(512, 2) void adapted_rows_grad(const RowsGradArgs p) {

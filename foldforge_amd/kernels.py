@@ -552,7 +552,8 @@ def adapted_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, dow
     (None: 1). Request ``r`` has the rows ``offsets[r]`` to ``offsets[r + 1]`` of ``x`` (its leading axes flattened) and the
     adapter ``adapter[r]`` (int32, on the device): one row each in a batch of single tokens, ``[0, N^2, 2 N^2, ...]`` for
     pair tensors of several targets. Rows of no request, and requests whose adapter is none of them (-1), have the
-    projection alone. Output bf16 ``[..., d_out]``. Any widths; rank up to 128."""
+    projection alone. Output bf16 ``[..., d_out]``. Any widths; rank up to 128. The products' operands are bf16: fp32 weights are
+    rounded, and so are, from some hundred rows on, the adapters and the rows ``x A_a^T`` (``include/foldforge_amd.h``)."""
     q = _adapted(x, weight, bias, down, up, scale, offsets, adapter)
     shape = (*x.shape[:-1], q.d_out)
     if out is not None:

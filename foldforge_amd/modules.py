@@ -537,7 +537,9 @@ class Transition(EngineOp, MasterWeights, nn.Module):
     """SwiGLU transition, residual included (``legacy/reference/transition.py:28-59``;
     parameters ``legacy/released.py:211-224``). With ``adapters`` (:func:`foldforge_amd.training.adapt`) each projection has
     the low-rank adapter of the batch element beside it; on ``hip`` it then runs as a norm, the three projections
-    (:func:`foldforge_amd.kernels.adapted_linear`) and the gate between them."""
+    (:func:`foldforge_amd.kernels.adapted_linear`) and, in torch, the gate between them and the sum with the input. Both
+    expansions and the update are bf16 between those, where the fused kernel keeps them in fp32, and under autograd the gate
+    keeps its fp32 operands: 2 GB for 512 x 512 rows of 128 channels, whatever ``keep`` says of the op's input."""
 
     #: what a differentiated ``hip`` call keeps of its input (as :class:`LayerNorm`)
     keep: str | None = None

@@ -293,7 +293,8 @@ def set_dropout(model: nn.Module, stream: DropoutStream | None, p: float | None 
 
 def adapt(model: nn.Module, rank: int, *, adapters: int = 1, scale: float = 1.0, seed: int = 0) -> list[str]:
     """Give every Transition of ``model`` ``adapters`` low-rank adapters of ``rank`` beside each of its three projections
-    (``down`` normal of deviation ``d_in^-1/2``, ``up`` zeros: the model's results are as before at first), fp32, and
+    (``down`` normal of deviation ``d_in^-1/2``, ``up`` zeros: the model's results are as before at first, on ``hip`` but for
+    the roundings of the projections' results, which the op without adapters does not make), fp32, and
     freeze the model's own parameters: the adapters alone ask for gradients (with :func:`install`, pass
     ``requires_grad=False`` there). A checkpoint of the model itself is loaded before. Returns the names of the
     Transitions."""

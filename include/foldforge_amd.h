@@ -130,7 +130,8 @@ int32_t ffk_dropout_add(const void* x, const void* residual, void* out, const in
  * are the same); rows of no request, and requests whose adapter is not in [0, adapters), get W x + bias. Two requests may
  * share an adapter (offsets that decrease give unspecified values). x, out, the weights: 16-byte aligned, out not x; rank up
  * to 128, widths up to 65536; sizes whose launches would have 2^24 workgroups or more are refused. Products of bf16 operands
- * (fp32 ones are rounded), fp32 sums; the rows A x in fp32 up to 256 rows, in bf16 above.
+ * (fp32 ones are rounded), fp32 sums. Up to 256 rows the adapter's part is fp32 throughout, from 385 on (rank above 32: from 257
+ * on) the rows A x and fp32 adapters are rounded to bf16; between them either holds, by width and requests.
  */
 size_t ffk_adapted_linear_workspace(int64_t rows, int32_t d_in, int32_t d_out, int32_t adapters, int32_t rank,
                                     int32_t requests, int32_t weight_dtype, int32_t adapter_dtype);
@@ -142,7 +143,8 @@ int32_t ffk_adapted_linear(const void* x, const void* weight, const float* bias,
 /*
  * The gradients of ffk_adapted_linear at the output's gradient dy [rows, d_out] bf16, rows > 0: dx [rows, d_in] bf16 (NULL:
  * not wanted; may not be dy or x), ddown and dup like down and up in grad_dtype, each the sum over all rows of its adapter in
- * fp32 and a fixed order (zeros for an adapter without rows). W and bias are frozen: no gradient.
+ * fp32 and a fixed order (zeros for an adapter without rows); an infinity in them is infinite or NaN as the sums are. W and
+ * bias are frozen: no gradient. dx from W, the adapters and v = s B^T dy rounded to bf16.
  */
 size_t ffk_adapted_linear_backward_workspace(int64_t rows, int32_t d_in, int32_t d_out, int32_t adapters, int32_t rank,
                                              int32_t requests, int32_t weight_dtype, int32_t adapter_dtype);
